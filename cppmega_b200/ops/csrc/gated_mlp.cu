@@ -1,0 +1,432 @@
+// Gated feed-forward block on CTA pairs: y = (act(x Wg^T) * (x Wu^T)) W2^T with w1 = [Wg; Wu].
+//   gate_up_kernel    one product with both projections: a tile of 256 tokens holds the same columns of gate and up side by side in
+//                     TMEM, the epilogue forms h = act(g) u from the fp32 accumulators and stores h and, for training, g and u.
+//   gate_grad_kernel  dh = dy W2 stays in TMEM; the epilogue reads g and u and stores dg = dh u act'(g), du = dh act(g).
+// The other products (h W2^T, [dg du] w1, [dg du]^T x, dy^T h) are the dense ones of gemm_pair.cu.  Against linear, activation, linear
+// this saves writing and reading dh, reading [g u] in the forward, and two launches.
+//
+// Both kernels are the 256 x 256 x 64 tcgen05.mma.cta_group::2 pipeline of gemm_pair.cu (6 stages of 32 KB, two accumulators in TMEM,
+// every wait bounded, no multicast).  The first CTA of a pair loads the gate rows of w1 and the second the up rows, so that the tile is
+// one ordinary 256-column product.  The epilogue has eight warps, two to a TMEM quadrant: its exponentials, and in the backward its
+// loads of g and u, have to fit under the main loop of the next tile.
+#include "gemm_pair.cuh"
+
+extern "C" int cm_gemm_bf16(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc,
+                            int a_mn, int b_mn, int out_fp32, int accumulate, int* err, cudaStream_t stream);
+
+namespace cm {
+namespace mlp {
+
+using namespace pair2;
+
+constexpr int BM = 128;                 // rows of one CTA; a tile has 2 * BM
+constexpr int BK = 64;
+constexpr int UMMA_K = 16;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int STAGES = 6;
+constexpr int A_BYTES = BM * BK * 2;
+constexpr int STAGE_BYTES = 2 * A_BYTES;
+constexpr int STORE_BYTES = 32 * 64;    // one warp's 32 rows x 32 columns of bf16
+constexpr int STORE_BUFS = 2;
+constexpr int STORE_OFF = STAGES * STAGE_BYTES;
+constexpr int BAR_OFF = STORE_OFF + EPI_WARPS * STORE_BUFS * STORE_BYTES;
+constexpr int SMEM_TOTAL = BAR_OFF + 256 + 1024;
+
+enum Act : int { SILU = 0, GELU_TANH = 1, RELU = 2 };
+
+struct Args {
+  int M, F, K;            // tokens, ffn columns, reduction (hidden)
+  int bn;                 // accumulator columns of a tile: 256 or 128
+  const __nv_bfloat16* gu;   // backward: saved [g | u], rows of 2F
+  int save;               // forward: store g and u
+  int* err;
+};
+
+__device__ __forceinline__ void mma_2cta(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+
+// act(g), and its slope.  exp and the division are the fast ones: their errors (a few 2^-22) vanish in the bf16 results.
+template <int ACT>
+__device__ __forceinline__ float act_of(float g) {
+  if constexpr (ACT == RELU) return fmaxf(g, 0.f);
+  if constexpr (ACT == SILU) return g * __fdividef(1.f, 1.f + __expf(-g));
+  const float t = 0.7978845608f * (g + 0.044715f * g * g * g);
+  return g * __fdividef(1.f, 1.f + __expf(-2.f * t));           // (1 + tanh t) / 2 = sigmoid(2 t)
+}
+template <int ACT>
+__device__ __forceinline__ void act_slope(float g, float& a, float& slope) {
+  if constexpr (ACT == RELU) {
+    a = fmaxf(g, 0.f);
+    slope = g > 0.f ? 1.f : 0.f;
+  } else if constexpr (ACT == SILU) {
+    const float q = __fdividef(1.f, 1.f + __expf(-g));
+    a = g * q;
+    slope = q * (1.f + g * (1.f - q));
+  } else {
+    const float t = 0.7978845608f * (g + 0.044715f * g * g * g);
+    const float q = __fdividef(1.f, 1.f + __expf(-2.f * t));
+    a = g * q;
+    slope = q * (1.f + 2.f * g * (1.f - q) * 0.7978845608f * (1.f + 3.f * 0.044715f * g * g));
+  }
+}
+
+// A warp's 32 rows x 32 columns on their way out: a ring of staging buffers (64-byte swizzle), each left by one bulk tensor store.
+struct Outbox {
+  uint8_t* base;
+  int lane;
+  uint32_t at = 0;
+  __device__ __forceinline__ void put(const CUtensorMap* map, const uint32_t (&v)[16], int col, int row) {
+    uint8_t* buf = base + at * STORE_BYTES;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(STORE_BUFS - 1) : "memory");   // this buffer has been read
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      bulk_store_2d(map, buf, col, row);
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    at = at + 1 == STORE_BUFS ? 0 : at + 1;
+  }
+};
+
+// BACK = false: A = x, B = w1 (rows of g and u), outputs h (tmO0), g (tmO1), u (tmO2).
+// BACK = true:  A = dy, B = w2 (reduction rows), outputs dg (tmO1), du (tmO2).
+template <bool BACK, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmO0,
+             const __grid_constant__ CUtensorMap tmO1, const __grid_constant__ CUtensorMap tmO2, const Args args) {
+  extern __shared__ uint8_t smem_raw[];
+  // the dynamic segment starts at the same offset in both CTAs, so the aligned offsets agree as the descriptors need
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + BAR_OFF);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* tmem_full = empty_bar + STAGES;
+  uint64_t* tmem_empty = tmem_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int half = args.bn >> 1;
+  const int cols = BACK ? args.bn : half;                       // ffn columns of a tile
+  const int tiles_n = (args.F + cols - 1) / cols, tiles_m = (args.M + 2 * BM - 1) / (2 * BM), total = tiles_m * tiles_n;
+  const int nkb = (args.K + BK - 1) / BK;
+  const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
+  // bands of 8 row tiles, as in gemm_pair.cu: the tiles in flight share their operands in L2
+  auto place = [&](int tile, int& m0, int& n0) {
+    const int band_tiles = 8 * tiles_n, b = tile / band_tiles, in = tile - b * band_tiles, rows = min(8, tiles_m - b * 8);
+    m0 = (b * 8 + in % rows) * 2 * BM;
+    n0 = (in / rows) * cols;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tmem_full[b], 1);
+      mbar_init(&tmem_empty[b], 2 * EPI_WARPS);
+    }
+    *abort_flag = (args.err && *reinterpret_cast<volatile int*>(args.err) != 0) ? 1 : 0;   // an earlier kernel gave up: drain
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------ TMA producer (both CTAs) ------------------------------
+    if (elect_one()) {
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmB);
+      const uint32_t pair_bytes = 2 * (A_BYTES + half * 128);
+      uint32_t stage = 0, phase = 0, used = 0;
+      bool ok = *abort_flag == 0;
+      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+        int m0, n0;
+        place(tile, m0, n0);
+        const int ma = m0 + rank * BM, nb = BACK ? n0 + rank * half : n0 + rank * args.F;
+        for (int kb = 0; kb < nkb; ++kb) {
+          ok = mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, args.err, ERR_WAIT_EMPTY);
+          if (!ok) break;
+          uint8_t* sa = smem + stage * STAGE_BYTES;
+          uint8_t* sb = sa + A_BYTES;
+          if (rank == 0) mbar_expect_tx(&full_bar[stage], pair_bytes);
+          const uint32_t bar = map_to_rank(smem_u32(&full_bar[stage]), 0);
+          const int k0 = kb * BK;
+          load_2d(sa, &tmA, bar, k0, ma);                                                // box [128 rows, 64 k]
+          if (!BACK) {
+            load_2d(sb, &tmB, bar, k0, nb);                                              // box [half rows, 64 k]
+          } else {
+            for (int c = 0; c < half / 64; ++c) load_2d(sb + c * (BK * 128), &tmB, bar, nb + c * 64, k0);   // boxes [64 k, 64 n]
+          }
+          if (used < STAGES) ++used;
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      // the last releases of this CTA's stages come from the partner: see them arrive before the barriers go away
+      for (uint32_t i = 0; i < used && ok; ++i) {
+        const uint32_t s = (stage + STAGES - 1 - i) % STAGES;
+        const uint32_t ph = (stage >= i + 1) ? phase : phase ^ 1;
+        ok = mbar_wait(&empty_bar[s], ph, abort_flag, args.err, ERR_WAIT_EMPTY);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------ MMA issuer (first CTA) ------------------------------
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = umma_idesc_bf16(2 * BM, args.bn, false, BACK);
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = *abort_flag == 0;
+      for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+        ok = mbar_wait(&tmem_empty[acc], acc_phase ^ 1, abort_flag, args.err, ERR_WAIT_TMEM_EMPTY);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * 256;
+        for (int kb = 0; kb < nkb; ++kb) {
+          ok = mbar_wait(&full_bar[stage], phase, abort_flag, args.err, ERR_WAIT_FULL);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * STAGE_BYTES);
+          const uint32_t sb = sa + A_BYTES;
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k) {
+            const uint64_t ad = umma_desc_sw128(sa + k * (UMMA_K * 2), 16, 1024);
+            const uint64_t bd = BACK ? umma_desc_sw128(sb + k * (UMMA_K * 128), BK * 128, 1024) : umma_desc_sw128(sb + k * (UMMA_K * 2), 16, 1024);
+            mma_2cta(d_tmem, ad, bd, idesc, (kb | k) != 0);
+          }
+          commit_pair(&empty_bar[stage]);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        commit_pair(&tmem_full[acc]);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+    }
+  } else {
+    // ------------------------------ epilogue (both CTAs) ------------------------------
+    const int q = warp & 3;                                     // TMEM lane quadrant this warp may read
+    const int part = (warp - 2) >> 2;                           // which half of the tile's columns
+    Outbox out{smem + STORE_OFF + (warp - 2) * STORE_BUFS * STORE_BYTES, lane};
+    const int c_begin = part * (cols >> 1), c_end = c_begin + (cols >> 1);
+    uint32_t acc = 0, acc_phase = 0;
+    bool ok = *abort_flag == 0;
+    for (int tile = first_tile; tile < total && ok; tile += tile_step) {
+      int m0, n0;
+      place(tile, m0, n0);
+      const int row0 = m0 + rank * BM + q * 32, row = row0 + lane;
+      uint4 gv[4], uv[4];
+      auto fetch = [&](int c) {                                 // g and u of 32 columns: requested ahead of their use
+        const __nv_bfloat16* p = args.gu + (long long)row * 2 * args.F + n0 + c;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const bool on = row < args.M && n0 + c + 8 * v < args.F;
+          gv[v] = on ? reinterpret_cast<const uint4*>(p)[v] : make_uint4(0, 0, 0, 0);
+          uv[v] = on ? reinterpret_cast<const uint4*>(p + args.F)[v] : make_uint4(0, 0, 0, 0);
+        }
+      };
+      if (BACK) fetch(c_begin);
+      ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], acc_phase, abort_flag, args.err, ERR_WAIT_TMEM_FULL));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t t_base = tmem_base + acc * 256 + (uint32_t(q * 32) << 16);
+      if (row0 < args.M) {
+        for (int c = c_begin; c < c_end && n0 + c < args.F; c += 32) {
+          if constexpr (!BACK) {
+            uint32_t g[32], u[32];
+            tmem_ld_32x32(t_base + c, g);
+            tmem_ld_32x32(t_base + half + c, u);
+            tmem_ld_wait();
+            uint32_t o[16];
+            if (args.save) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = pack_bf16(__uint_as_float(g[2 * j]), __uint_as_float(g[2 * j + 1]));
+              out.put(&tmO1, o, n0 + c, row0);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = pack_bf16(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
+              out.put(&tmO2, o, n0 + c, row0);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              o[j] = pack_bf16(act_of<ACT>(__uint_as_float(g[2 * j])) * __uint_as_float(u[2 * j]),
+                               act_of<ACT>(__uint_as_float(g[2 * j + 1])) * __uint_as_float(u[2 * j + 1]));
+            out.put(&tmO0, o, n0 + c, row0);
+          } else {
+            uint32_t d[32];
+            tmem_ld_32x32(t_base + c, d);
+            uint4 gc[4], uc[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) { gc[v] = gv[v]; uc[v] = uv[v]; }
+            if (c + 32 < c_end) fetch(c + 32);
+            tmem_ld_wait();
+            uint32_t og[16], ou[16];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const __nv_bfloat162* gb = reinterpret_cast<const __nv_bfloat162*>(&gc[v]);
+              const __nv_bfloat162* ub = reinterpret_cast<const __nv_bfloat162*>(&uc[v]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 g = __bfloat1622float2(gb[j]), u = __bfloat1622float2(ub[j]);
+                float a0, s0, a1, s1;
+                act_slope<ACT>(g.x, a0, s0);
+                act_slope<ACT>(g.y, a1, s1);
+                const float d0 = __uint_as_float(d[8 * v + 2 * j]), d1 = __uint_as_float(d[8 * v + 2 * j + 1]);
+                og[4 * v + j] = pack_bf16(d0 * u.x * s0, d1 * u.y * s1);
+                ou[4 * v + j] = pack_bf16(d0 * a0, d1 * a1);
+              }
+            }
+            out.put(&tmO1, og, n0 + c, row0);
+            out.put(&tmO2, ou, n0 + c, row0);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&tmem_empty[acc]), 0));
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+
+  // ------------------------------ teardown ------------------------------
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // let TMA copies and MMAs still in flight land before the pair's shared memory is released
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+    __syncthreads();
+  }
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// A [rows, cols] result with row pitch ld as the target of bulk stores: boxes of 32 rows x 32 columns.
+static int make_out_map(CUtensorMap* out, void* base, long long rows, long long cols, long long ld) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) return -1;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+  cuuint32_t box[2] = {32, 32}, one[2] = {1, 1};
+  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : int(r);
+}
+
+template <bool BACK, int ACT>
+static int launch(const CUtensorMap* maps, const Args& args, cudaStream_t stream) {
+  auto kern = gated_kernel<BACK, ACT>;
+  static PerDevice configured;
+  if (configured.first()) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL) != cudaSuccess) return -2;
+    configured.done();
+  }
+  const int cols = BACK ? args.bn : args.bn / 2;
+  const long long tiles = (long long)((args.M + 2 * BM - 1) / (2 * BM)) * ((args.F + cols - 1) / cols);
+  if (tiles > 0x7fffffff) return -10;
+  const int pairs = sm_count() / 2;
+  const int grid = 2 * int(tiles < pairs ? tiles : pairs);
+  kern<<<grid, THREADS, SMEM_TOTAL, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], args);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+template <bool BACK>
+static int launch_act(int act, const CUtensorMap* maps, const Args& args, cudaStream_t stream) {
+  switch (act) {
+    case SILU: return launch<BACK, SILU>(maps, args, stream);
+    case GELU_TANH: return launch<BACK, GELU_TANH>(maps, args, stream);
+    case RELU: return launch<BACK, RELU>(maps, args, stream);
+  }
+  return -10;
+}
+
+// Accumulator columns of a tile: waves of pairs, weighted as in plan_dense (a 128-column tile takes 0.74 of a 256-column one's time).
+static int plan_bn(int M, int F, bool back) {
+  const long long pairs = sm_count() / 2, tm = (M + 2 * BM - 1) / (2 * BM);
+  auto waves = [&](int bn) {
+    const int cols = back ? bn : bn / 2;
+    return (tm * ((F + cols - 1) / cols) + pairs - 1) / pairs;
+  };
+  return waves(128) * 17.8 < waves(256) * 24.2 ? 128 : 256;
+}
+
+static bool tma_ok(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
+
+}  // namespace mlp
+}  // namespace cm
+
+using namespace cm;
+
+// y[M, Ho] = (act(x w1[:F]^T) * (x w1[F:]^T)) w2^T; x [M, H] with row pitch ldx, w1 [2F, H], w2 [Ho, F], h [M, F]; gu [M, 2F] or null
+// (not kept).  act: 0 silu, 1 gelu (tanh form), 2 relu.
+extern "C" int cm_gated_mlp_fwd(const void* x, long long ldx, const void* w1, const void* w2, void* gu, void* h, void* y, int M, int H,
+                                int F, int Ho, int act, int* err, cudaStream_t stream) {
+  if (M <= 0 || H <= 0 || F <= 0 || Ho <= 0) return 0;
+  if (H % 8 || F % 8 || Ho % 8 || !mlp::tma_ok(x, ldx) || !mlp::tma_ok(w1, H) || !mlp::tma_ok(w2, F) || !mlp::tma_ok(gu, 0) ||
+      !mlp::tma_ok(h, F) || !mlp::tma_ok(y, Ho))
+    return -10;
+  mlp::Args args{M, F, H, mlp::plan_bn(M, F, false), nullptr, gu != nullptr, err};
+  CUtensorMap maps[5];
+  int rc = make_tmap_2d_bf16(&maps[0], x, M, H, ldx, mlp::BM);
+  if (!rc) rc = make_tmap_2d_bf16(&maps[1], w1, 2ll * F, H, H, args.bn / 2);
+  if (!rc) rc = mlp::make_out_map(&maps[2], h, M, F, F);
+  maps[3] = maps[4] = maps[2];
+  if (!rc && gu) rc = mlp::make_out_map(&maps[3], gu, M, F, 2ll * F);
+  if (!rc && gu) rc = mlp::make_out_map(&maps[4], static_cast<__nv_bfloat16*>(gu) + F, M, F, 2ll * F);
+  if (rc) return rc;
+  rc = mlp::launch_act<false>(act, maps, args, stream);
+  if (rc) return rc;
+  return cm_gemm_bf16(h, w2, y, M, Ho, F, F, F, Ho, 0, 0, 0, 0, err, stream);
+}
+
+// Gradients from dy [M, Ho] (row pitch lddy): dgu [M, 2F] is work space; dx [M, H], dw1, dw2 may be null.  dw1 / dw2: fp32 or bf16
+// (dw*_fp32), added to what is there with acc*.
+extern "C" int cm_gated_mlp_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w1, const void* w2, const void* gu,
+                                const void* h, void* dgu, void* dx, void* dw1, int dw1_fp32, int acc1, void* dw2, int dw2_fp32, int acc2,
+                                int M, int H, int F, int Ho, int act, int* err, cudaStream_t stream) {
+  if (M <= 0 || H <= 0 || F <= 0 || Ho <= 0) return 0;
+  if (H % 8 || F % 8 || Ho % 8 || !mlp::tma_ok(dy, lddy) || !mlp::tma_ok(x, ldx) || !mlp::tma_ok(w1, H) || !mlp::tma_ok(w2, F) ||
+      !mlp::tma_ok(gu, 0) || !mlp::tma_ok(h, F) || !mlp::tma_ok(dgu, 0))
+    return -10;
+  int rc = 0;
+  if (dx || dw1) {
+    mlp::Args args{M, F, Ho, mlp::plan_bn(M, F, true), static_cast<const __nv_bfloat16*>(gu), 0, err};
+    CUtensorMap maps[5];
+    rc = make_tmap_2d_bf16(&maps[0], dy, M, Ho, lddy, mlp::BM);
+    if (!rc) rc = make_tmap_2d_bf16(&maps[1], w2, Ho, F, F, 64);
+    if (!rc) rc = mlp::make_out_map(&maps[3], dgu, M, F, 2ll * F);
+    if (!rc) rc = mlp::make_out_map(&maps[4], static_cast<__nv_bfloat16*>(dgu) + F, M, F, 2ll * F);
+    maps[2] = maps[3];
+    if (!rc) rc = mlp::launch_act<true>(act, maps, args, stream);
+    if (!rc && dx) rc = cm_gemm_bf16(dgu, w1, dx, M, H, 2 * F, 2ll * F, H, H, 0, 1, 0, 0, err, stream);
+    if (!rc && dw1) rc = cm_gemm_bf16(dgu, x, dw1, 2 * F, H, M, 2ll * F, ldx, H, 1, 1, dw1_fp32, acc1, err, stream);
+  }
+  if (!rc && dw2) rc = cm_gemm_bf16(dy, h, dw2, Ho, F, M, lddy, F, F, 1, 1, dw2_fp32, acc2, err, stream);
+  return rc;
+}

@@ -1,0 +1,212 @@
+// Gated RMS norm of a mixer's output, forward and backward, in bf16, fp16 or fp32.  Groups of `group` channels normalise apart
+// (rms(v) = v * rsqrt(mean(v^2) + eps)), a(z) = z sigmoid(z):
+//   norm first:  y = rms(x) w a(z)          gate first:  y = rms(x a(z)) w          without z: y = rms(x) w
+// Backward, with xh the normalised values, r the reciprocal norm and dn = dy a(z) (norm first) or dy:
+//   du = r (dn w - xh mean(dn w xh));  dw = sum dn xh
+//   norm first:  dx = du,  dz = dy xh w a'(z)         gate first:  dx = du a(z),  dz = du x a'(z)
+// A team of threads holds one group of one row; blockIdx.y is the group, so that a thread keeps its channels over the rows of the
+// backward and adds their weight gradient in registers.  Bound by memory: three rows moved forward, five backward; the gate is read
+// where it lies (a column slice of the projection has its own pitch).  The weight gradient is summed in a fixed order.
+#include "row_vec.cuh"
+
+namespace cm {
+
+struct GatedArgs {
+  const void *x, *z, *w, *dy;      // z may be null
+  long long sx, sz, sdy;           // elements between rows
+  void *y, *dx, *dz;               // packed rows
+  float *rstd;                     // [rows][groups]; may be null in the forward
+  float *part;                     // [blocks][width]; null: not wanted
+  long long rows;
+  int width, group;
+  float eps;
+  int gate_first;
+};
+
+__device__ __forceinline__ float sigmoid_of(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+
+template <typename T, int TPR, int VPT, bool VEC>
+__global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArgs a) {
+  constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
+  __shared__ float red[2 * (TPR > 32 ? TPR / 32 : 1)];
+  const int t = threadIdx.x % TPR, g0 = blockIdx.y * a.group;
+  const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int G = row < a.rows ? a.group : 0;
+  uint4 xv[VPT], zv[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    xv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.sx + g0, t + i * TPR, G);
+    zv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.z) + row * a.sz + g0, t + i * TPR, a.z ? G : 0);
+  }
+  float ss[1] = {0.f};
+  float u[VPT][N];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    rv_unpack<T>(xv[i], u[i]);
+    if (a.gate_first && a.z) {
+      float z[N];
+      rv_unpack<T>(zv[i], z);
+#pragma unroll
+      for (int j = 0; j < N; ++j) u[i][j] *= z[j] * sigmoid_of(z[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) ss[0] += u[i][j] * u[i][j];
+  }
+  rv_team_sum<TPR, 1>(ss, red, 0);
+  const float r = rsqrtf(ss[0] / a.group + a.eps);
+  if (row >= a.rows) return;
+  if (t == 0 && a.rstd) a.rstd[row * gridDim.y + blockIdx.y] = r;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    float w[N];
+    rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, t + i * TPR, G), w);
+#pragma unroll
+    for (int j = 0; j < N; ++j) u[i][j] *= r * w[j];
+    if (!a.gate_first && a.z) {
+      float z[N];
+      rv_unpack<T>(zv[i], z);
+#pragma unroll
+      for (int j = 0; j < N; ++j) u[i][j] *= z[j] * sigmoid_of(z[j]);
+    }
+    rv_store<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + g0, t + i * TPR, G, rv_pack<T>(u[i]));
+  }
+}
+
+template <typename T, int TPR, int VPT, bool VEC>
+__global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArgs a) {
+  constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
+  __shared__ float red[2 * (TPR > 32 ? TPR / 32 : 1)];
+  __shared__ float scratch[RPB > 1 ? RPB * TPR * VPT * N : 1];
+  const int t = threadIdx.x % TPR, g0 = blockIdx.y * a.group;
+  float acc[VPT][N] = {};
+  int turn = 0;
+  for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += (long long)gridDim.x * RPB, turn ^= 1) {
+    const long long row = row0 + threadIdx.x / TPR;
+    const int G = row < a.rows ? a.group : 0;
+    uint4 xv[VPT], zv[VPT], dv[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t + i * TPR;
+      xv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.sx + g0, c, G);
+      zv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.z) + row * a.sz + g0, c, a.z ? G : 0);
+      dv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.sdy + g0, c, G);
+    }
+    const float r = G ? a.rstd[row * gridDim.y + blockIdx.y] : 0.f;
+    float s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float x[N], z[N], d[N], w[N];
+      rv_unpack<T>(xv[i], x);
+      rv_unpack<T>(zv[i], z);
+      rv_unpack<T>(dv[i], d);
+      rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, t + i * TPR, G), w);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float gate = a.z ? z[j] * sigmoid_of(z[j]) : 1.f;
+        const float hat = (a.gate_first ? x[j] * gate : x[j]) * r, dn = a.gate_first ? d[j] : d[j] * gate;
+        acc[i][j] += dn * hat;
+        s[0] += dn * w[j] * hat;
+      }
+    }
+    rv_team_sum<TPR, 1>(s, red, turn);
+    if (!G) continue;
+    const float m = s[0] / a.group;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t + i * TPR;
+      float x[N], z[N], d[N], w[N];
+      rv_unpack<T>(xv[i], x);
+      rv_unpack<T>(zv[i], z);
+      rv_unpack<T>(dv[i], d);
+      rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, c, G), w);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float q = sigmoid_of(z[j]), gate = a.z ? z[j] * q : 1.f, slope = q * (1.f + z[j] * (1.f - q));
+        if (a.gate_first) {
+          const float du = r * (d[j] * w[j] - x[j] * gate * r * m);
+          z[j] = du * x[j] * slope;
+          x[j] = du * gate;
+        } else {
+          const float hat = x[j] * r;
+          z[j] = d[j] * hat * w[j] * slope;
+          x[j] = r * (d[j] * gate * w[j] - hat * m);
+        }
+      }
+      rv_store<T, VEC>(reinterpret_cast<T*>(a.dx) + row * a.width + g0, c, G, rv_pack<T>(x));
+      if (a.dz) rv_store<T, VEC>(reinterpret_cast<T*>(a.dz) + row * a.width + g0, c, G, rv_pack<T>(z));
+    }
+  }
+  if (a.part) rv_partial<T, TPR, VPT>(acc, a.part + (long long)blockIdx.x * a.width + g0, a.group, scratch);
+}
+
+template <typename T>
+static int gated_launch(const GatedArgs& a, bool back, int blocks, cudaStream_t s) {
+  const int size = sizeof(T), nvec = (a.group + RowVec<T>::N - 1) / RowVec<T>::N, groups = a.width / a.group;
+  auto fits = [&](const void* p, long long pitch) { return !p || ((reinterpret_cast<uintptr_t>(p) | (pitch * size)) & 15) == 0; };
+  const bool vec = a.group * size % 16 == 0 && fits(a.x, a.sx) && fits(a.z, a.sz) && fits(a.w, 0) && fits(a.dy, a.sdy) &&
+                   fits(a.y, a.width) && fits(a.dx, a.width) && fits(a.dz, a.width);
+  const int team = rv_team(nvec, vec);
+#define CM_GATED(TPR, VPT, VEC)                                                                                                  \
+  [&] {                                                                                                                          \
+    constexpr int TB = rv_block<TPR>(), RPB = TB / TPR;                                                                          \
+    if (back) gated_norm_bwd<T, TPR, VPT, VEC><<<dim3(blocks, groups), TB, 0, s>>>(a);                                           \
+    else gated_norm_fwd<T, TPR, VPT, VEC><<<dim3(unsigned((a.rows + RPB - 1) / RPB), groups), TB, 0, s>>>(a);                    \
+    return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                                           \
+  }()
+  CM_ROW_TEAM(team, vec, CM_GATED);
+#undef CM_GATED
+}
+
+static int gated_any(const GatedArgs& a, int dtype, bool back, int blocks, cudaStream_t s) {
+  if (a.group <= 0 || a.width % a.group || a.width / a.group > 65535) return -10;
+  switch (dtype) {
+    case ROW_BF16: return gated_launch<__nv_bfloat16>(a, back, blocks, s);
+    case ROW_FP16: return gated_launch<__half>(a, back, blocks, s);
+    case ROW_FP32: return gated_launch<float>(a, back, blocks, s);
+  }
+  return -10;
+}
+
+}  // namespace cm
+
+using namespace cm;
+
+// dtype: 0 bf16, 1 fp16, 2 fp32.  z, rstd may be null; sx, sz: elements between rows; y packed; rstd [rows][width / group].
+extern "C" int cm_rmsnorm_gated_fwd(const void* x, long long sx, const void* z, long long sz, const void* w, void* y, float* rstd,
+                                    long long rows, int width, int group, int gate_first, float eps, int dtype, cudaStream_t s) {
+  if (rows <= 0 || width <= 0) return 0;
+  GatedArgs a{};
+  a.x = x; a.sx = sx; a.z = z; a.sz = sz; a.w = w; a.y = y; a.rstd = rstd; a.rows = rows; a.width = width; a.group = group;
+  a.gate_first = gate_first; a.eps = eps;
+  return gated_any(a, dtype, false, 0, s);
+}
+
+// Blocks along the rows, and with that the partial rows of the weight gradient.
+extern "C" int cm_rmsnorm_gated_parts(long long rows, int width, int group, int dtype) {
+  const int n = dtype == ROW_FP32 ? 4 : 8, nvec = (group + n - 1) / n, groups = width / group;
+  const long long threads = nvec <= 256 ? 128 : nvec <= 512 ? 256 : nvec <= 1024 ? 512 : 1024;
+  const long long most = ((long long)sm_count() * (1024 / threads) + groups - 1) / groups;
+  return int(rows < most ? (rows < 1 ? 1 : rows) : most);
+}
+
+// part: [cm_rmsnorm_gated_parts][width] floats of work space, with dw; dz, dw may be null.  dx, dz packed.
+extern "C" int cm_rmsnorm_gated_bwd(const void* x, long long sx, const void* z, long long sz, const void* w, const void* dy, long long sdy,
+                                    const float* rstd, void* dx, void* dz, void* dw, float* part, long long rows, int width, int group,
+                                    int gate_first, int dtype, cudaStream_t s) {
+  if (rows <= 0 || width <= 0) return 0;
+  if (group <= 0) return -10;
+  const int blocks = cm_rmsnorm_gated_parts(rows, width, group, dtype);
+  GatedArgs a{};
+  a.x = x; a.sx = sx; a.z = z; a.sz = sz; a.w = w; a.dy = dy; a.sdy = sdy; a.rstd = const_cast<float*>(rstd); a.dx = dx; a.dz = dz;
+  a.part = dw ? part : nullptr; a.rows = rows; a.width = width; a.group = group; a.gate_first = gate_first;
+  const int rc = gated_any(a, dtype, true, blocks, s);
+  if (rc || !dw) return rc;
+  ColumnSums c{};
+  c.partial[0] = part;
+  c.out[0] = dw;
+  const dim3 grid((width + 31) / 32, 1);
+  if (dtype == ROW_BF16) rv_column_sum<__nv_bfloat16><<<grid, 256, 0, s>>>(c, blocks, width);
+  else if (dtype == ROW_FP16) rv_column_sum<__half><<<grid, 256, 0, s>>>(c, blocks, width);
+  else rv_column_sum<float><<<grid, 256, 0, s>>>(c, blocks, width);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}

@@ -1,0 +1,334 @@
+// The residual step of a layer with the norms on both sides of the block, forward and backward, in bf16, fp16 or fp32:
+//   p = rms(y) post   (or y)            rms(v) = v * rsqrt(mean(v^2) + eps)
+//   h = residual + scale * gate * p     gate: none, one per channel, or one per element; rounded to the stream's type
+//   n = rms(h) weight                   of the rounded h: what the stream holds is what is normalised
+// Backward, with a = scale * gate * post, r and rho the two reciprocal norms, yh = y r, hh = h rho, and dh0 the gradient that reaches h
+// from its other readers:
+//   g = dn weight;  dh = rho (g - hh mean(g hh)) + dh0;  dresidual = dh;  dweight = sum dn hh
+//   dp = scale gate dh;  dgate = scale dh p;  dpost = sum dp yh;  dy = r (a dh - yh mean(a dh yh))
+// The second mean is linear in the first: with S1 = sum g hh, S2 = sum a yh (rho g + dh0), S3 = sum a yh hh it is
+// (S2 - rho S1 S3 / W) / W, so that a row is read once and reduced once.
+// Bound by memory: forward 4 rows moved, backward 6 (4 read).  Sums over rows go through one partial row per block and a second
+// kernel in a fixed order: the same call gives the same bits.
+#include "row_vec.cuh"
+
+namespace cm {
+
+struct ResidualArgs {
+  const void *y, *res, *w, *post, *gate;      // post, gate may be null
+  long long sy, sres;                         // elements between rows
+  int gate_rows;                              // gate: 0 one per channel, 1 one per element (packed rows)
+  void *n, *h;
+  float *rstd_y, *rstd_h;                     // may be null
+  long long rows;
+  int width;
+  float scale, eps;
+  // backward
+  const void *dn, *dh;                        // either may be null: zero
+  long long sdn, sdh;
+  void *dres, *dy, *dgate_rows;               // dy null: the same as dres
+  float *part_w, *part_post, *part_gate;      // [blocks][width]; null: not wanted
+};
+
+template <typename T, int TPR, int VPT, bool VEC, bool FULL>
+__global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_fwd(const ResidualArgs a) {
+  constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
+  __shared__ float red[2 * (TPR > 32 ? TPR / 32 : 1)];
+  const int t = threadIdx.x % TPR, W = a.width;
+  const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+  const bool on = row < a.rows;
+  const int w_on = on ? W : 0;                // a team past the last row reads and writes nothing but takes part in the sums
+  const T* yr = reinterpret_cast<const T*>(a.y) + row * a.sy;
+  const T* xr = reinterpret_cast<const T*>(a.res) + row * a.sres;
+  uint4 yv[VPT], hv[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    yv[i] = rv_load<T, VEC>(yr, t + i * TPR, w_on);
+    hv[i] = rv_load<T, VEC>(xr, t + i * TPR, w_on);
+  }
+  float r = 1.f;
+  const bool post = FULL && a.post;
+  if (post) {
+    float ss[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float f[N];
+      rv_unpack<T>(yv[i], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) ss[0] += f[j] * f[j];
+    }
+    rv_team_sum<TPR, 1>(ss, red, 0);
+    r = rsqrtf(ss[0] / W + a.eps);
+    if (on && t == 0 && a.rstd_y) a.rstd_y[row] = r;
+  }
+  float ss[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    float y[N], x[N];
+    rv_unpack<T>(yv[i], y);
+    rv_unpack<T>(hv[i], x);
+    if constexpr (FULL) {
+      if (post) {
+        float p[N];
+        rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), t + i * TPR, W), p);
+#pragma unroll
+        for (int j = 0; j < N; ++j) y[j] *= r * p[j];
+      }
+      if (a.gate) {
+        float g[N];
+        rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.gate) + (a.gate_rows ? row * W : 0ll), t + i * TPR, w_on), g);
+#pragma unroll
+        for (int j = 0; j < N; ++j) y[j] *= g[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] += a.scale * y[j];
+    hv[i] = rv_pack<T>(x);
+    rv_unpack<T>(hv[i], x);                   // the stream's value
+#pragma unroll
+    for (int j = 0; j < N; ++j) ss[0] += x[j] * x[j];
+  }
+  rv_team_sum<TPR, 1>(ss, red, 1);
+  const float rho = rsqrtf(ss[0] / W + a.eps);
+  if (!on) return;
+  if (t == 0 && a.rstd_h) a.rstd_h[row] = rho;
+  T* hr = reinterpret_cast<T*>(a.h) + row * W;
+  T* nr = reinterpret_cast<T*>(a.n) + row * W;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    float x[N], w[N];
+    rv_unpack<T>(hv[i], x);
+    rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w), t + i * TPR, W), w);
+    rv_store<T, VEC>(hr, t + i * TPR, W, hv[i]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = x[j] * rho * w[j];
+    rv_store<T, VEC>(nr, t + i * TPR, W, rv_pack<T>(x));
+  }
+}
+
+template <typename T, int TPR, int VPT, bool VEC, bool FULL>
+__global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_bwd(const ResidualArgs a) {
+  constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
+  __shared__ float red[2 * 3 * (TPR > 32 ? TPR / 32 : 1)];
+  __shared__ float scratch[RPB > 1 ? RPB * TPR * VPT * N : 1];
+  const int t = threadIdx.x % TPR, W = a.width;
+  float acc_w[VPT][N] = {}, acc_p[FULL ? VPT : 1][N] = {}, acc_g[FULL ? VPT : 1][N] = {};
+  const bool post = FULL && a.post, gate = FULL && a.gate;
+  int turn = 0;
+  for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += (long long)gridDim.x * RPB, turn ^= 1) {
+    const long long row = row0 + threadIdx.x / TPR;
+    const bool on = row < a.rows;
+    const int w_on = on ? W : 0;
+    uint4 gv[VPT], dv[VPT], hv[VPT], yv[FULL ? VPT : 1], tv[FULL ? VPT : 1];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t + i * TPR;
+      gv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.dn) + row * a.sdn, c, a.dn ? w_on : 0);
+      dv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.dh) + row * a.sdh, c, a.dh ? w_on : 0);
+      hv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.h) + row * W, c, w_on);
+      if constexpr (FULL) {
+        yv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.y) + row * a.sy, c, w_on);
+        if (gate && a.gate_rows) tv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.gate) + row * W, c, w_on);
+      }
+    }
+    const float rho = on ? a.rstd_h[row] : 0.f, r = on && post ? a.rstd_y[row] : 1.f;
+    // scale * gate * post of vector i
+    auto factor = [&](int i, float (&f)[N], bool with_post) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] = a.scale;
+      if constexpr (FULL) {
+        float q[N];
+        if (gate) {
+          rv_unpack<T>(a.gate_rows ? tv[i] : rv_load<T, VEC>(reinterpret_cast<const T*>(a.gate), t + i * TPR, W), q);
+#pragma unroll
+          for (int j = 0; j < N; ++j) f[j] *= q[j];
+        }
+        if (with_post) {
+          rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), t + i * TPR, W), q);
+#pragma unroll
+          for (int j = 0; j < N; ++j) f[j] *= q[j];
+        }
+      }
+    };
+    float s[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float g[N], h[N], w[N];
+      rv_unpack<T>(gv[i], g);
+      rv_unpack<T>(hv[i], h);
+      rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w), t + i * TPR, W), w);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        h[j] *= rho;
+        acc_w[i][j] += g[j] * h[j];
+        g[j] *= w[j];
+        s[0] += g[j] * h[j];
+      }
+      if constexpr (FULL) {
+        if (post) {
+          float d[N], y[N], f[N];
+          rv_unpack<T>(dv[i], d);
+          rv_unpack<T>(yv[i], y);
+          factor(i, f, true);
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const float ay = f[j] * y[j] * r;
+            s[1] += ay * (rho * g[j] + d[j]);
+            s[2] += ay * h[j];
+          }
+        }
+      }
+    }
+    if (post) rv_team_sum<TPR, 3>(s, red, turn);
+    else rv_team_sum<TPR, 1>(reinterpret_cast<float(&)[1]>(s), red, turn);
+    const float m1 = s[0] / W, m2 = (s[1] - rho * m1 * s[2]) / W;
+    if (!on) continue;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t + i * TPR;
+      float g[N], h[N], w[N], d[N];
+      rv_unpack<T>(gv[i], g);
+      rv_unpack<T>(hv[i], h);
+      rv_unpack<T>(dv[i], d);
+      rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w), c, W), w);
+#pragma unroll
+      for (int j = 0; j < N; ++j) d[j] += rho * (g[j] * w[j] - h[j] * rho * m1);
+      rv_store<T, VEC>(reinterpret_cast<T*>(a.dres) + row * W, c, W, rv_pack<T>(d));
+      if constexpr (FULL) {
+        float y[N], f[N];
+        rv_unpack<T>(yv[i], y);
+        float p[N];                           // y with the post norm: what the gate multiplies
+#pragma unroll
+        for (int j = 0; j < N; ++j) p[j] = y[j] *= r;
+        float q[N];
+        if (post) {
+          rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), c, W), q);
+#pragma unroll
+          for (int j = 0; j < N; ++j) p[j] *= q[j];
+        }
+        factor(i, f, false);
+        float dg[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) dg[j] = a.scale * d[j] * p[j];
+        if (gate && a.gate_rows) {
+          if (a.dgate_rows) rv_store<T, VEC>(reinterpret_cast<T*>(a.dgate_rows) + row * W, c, W, rv_pack<T>(dg));
+        } else {
+#pragma unroll
+          for (int j = 0; j < N; ++j) acc_g[i][j] += dg[j];
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) d[j] *= f[j];              // dp
+        if (post) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            acc_p[i][j] += d[j] * y[j];
+            d[j] = r * (d[j] * q[j] - y[j] * m2);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) d[j] *= a.scale;
+      }
+      if (a.dy) rv_store<T, VEC>(reinterpret_cast<T*>(a.dy) + row * W, c, W, rv_pack<T>(d));
+    }
+  }
+  const long long at = (long long)blockIdx.x * W;
+  if (a.part_w) rv_partial<T, TPR, VPT>(acc_w, a.part_w + at, W, scratch);
+  if constexpr (FULL) {
+    if (a.part_post) rv_partial<T, TPR, VPT>(acc_p, a.part_post + at, W, scratch);
+    if (a.part_gate) rv_partial<T, TPR, VPT>(acc_g, a.part_gate + at, W, scratch);
+  }
+}
+
+static bool aligned16(const void* p, long long pitch, int size) { return !p || ((reinterpret_cast<uintptr_t>(p) | (pitch * size)) & 15) == 0; }
+
+static bool residual_vec(const ResidualArgs& a, int size) {
+  const long long W = a.width;
+  return (W * size) % 16 == 0 && aligned16(a.y, a.sy, size) && aligned16(a.res, a.sres, size) && aligned16(a.w, 0, size) &&
+         aligned16(a.post, 0, size) && aligned16(a.gate, 0, size) && aligned16(a.n, 0, size) && aligned16(a.h, 0, size) &&
+         aligned16(a.dn, a.sdn, size) && aligned16(a.dh, a.sdh, size) && aligned16(a.dres, 0, size) && aligned16(a.dy, 0, size) &&
+         aligned16(a.dgate_rows, 0, size);
+}
+
+template <typename T, bool FULL>
+static int residual_launch(const ResidualArgs& a, bool back, int blocks, cudaStream_t s) {
+  const int size = sizeof(T), nvec = (a.width + RowVec<T>::N - 1) / RowVec<T>::N;
+  const bool vec = residual_vec(a, size);
+  const int team = rv_team(nvec, vec);
+#define CM_RES(TPR, VPT, VEC)                                                                                                     \
+  [&] {                                                                                                                           \
+    constexpr int TB = rv_block<TPR>(), RPB = TB / TPR;                                                                           \
+    if (back) residual_norm_bwd<T, TPR, VPT, VEC, FULL><<<blocks, TB, 0, s>>>(a);                                                 \
+    else residual_norm_fwd<T, TPR, VPT, VEC, FULL><<<unsigned((a.rows + RPB - 1) / RPB), TB, 0, s>>>(a);                          \
+    return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                                            \
+  }()
+  CM_ROW_TEAM(team, vec, CM_RES);
+#undef CM_RES
+}
+
+static int residual_any(const ResidualArgs& a, int dtype, bool back, int blocks, cudaStream_t s) {
+  const bool full = a.post || a.gate;
+  switch (dtype) {
+    case ROW_BF16: return full ? residual_launch<__nv_bfloat16, true>(a, back, blocks, s) : residual_launch<__nv_bfloat16, false>(a, back, blocks, s);
+    case ROW_FP16: return full ? residual_launch<__half, true>(a, back, blocks, s) : residual_launch<__half, false>(a, back, blocks, s);
+    case ROW_FP32: return full ? residual_launch<float, true>(a, back, blocks, s) : residual_launch<float, false>(a, back, blocks, s);
+  }
+  return -10;
+}
+
+}  // namespace cm
+
+using namespace cm;
+
+// dtype: 0 bf16, 1 fp16, 2 fp32 (all tensors; the statistics are fp32).  post / gate / rstd_* may be null.  sy, sres: elements between
+// rows; gate_rows: the gate has a row per row of y.
+extern "C" int cm_residual_rmsnorm_fwd(const void* y, long long sy, const void* res, long long sres, const void* w, const void* post,
+                                       const void* gate, int gate_rows, void* n, void* h, float* rstd_y, float* rstd_h, long long rows,
+                                       int width, float scale, float eps, int dtype, cudaStream_t s) {
+  if (rows <= 0 || width <= 0) return 0;
+  ResidualArgs a{};
+  a.y = y; a.sy = sy; a.res = res; a.sres = sres; a.w = w; a.post = post; a.gate = gate; a.gate_rows = gate_rows;
+  a.n = n; a.h = h; a.rstd_y = rstd_y; a.rstd_h = rstd_h; a.rows = rows; a.width = width; a.scale = scale; a.eps = eps;
+  return residual_any(a, dtype, false, 0, s);
+}
+
+// Blocks of the backward kernel, and with that the partial rows of a column sum, for this many rows.
+extern "C" int cm_row_norm_parts(long long rows, int width, int dtype) {
+  const int n = dtype == ROW_FP32 ? 4 : 8, nvec = (width + n - 1) / n;
+  const long long threads = nvec <= 64 ? 128 : nvec <= 256 ? 128 : nvec <= 512 ? 256 : nvec <= 1024 ? 512 : 1024;
+  const long long most = (long long)sm_count() * (1024 / threads);
+  return int(rows < most ? (rows < 1 ? 1 : rows) : most);
+}
+
+// part: [3][cm_row_norm_parts][width] floats of work space.  dn, dh (gradients of n and h) may be null; dy null: it is dres (no post
+// norm, no gate, scale 1); dw, dpost, dgate (one per channel), dgate_rows may be null.
+extern "C" int cm_residual_rmsnorm_bwd(const void* dn, long long sdn, const void* dh, long long sdh, const void* h, const void* y,
+                                       long long sy, const void* w, const void* post, const void* gate, int gate_rows,
+                                       const float* rstd_y, const float* rstd_h, void* dres, void* dy, void* dgate_rows, void* dw,
+                                       void* dpost, void* dgate, float* part, long long rows, int width, float scale, int dtype,
+                                       cudaStream_t s) {
+  if (rows <= 0 || width <= 0) return 0;
+  const int blocks = cm_row_norm_parts(rows, width, dtype);
+  ResidualArgs a{};
+  a.dn = dn; a.sdn = sdn; a.dh = dh; a.sdh = sdh; a.h = const_cast<void*>(h); a.y = y; a.sy = sy; a.w = w; a.post = post; a.gate = gate;
+  a.gate_rows = gate_rows; a.rstd_y = const_cast<float*>(rstd_y); a.rstd_h = const_cast<float*>(rstd_h); a.dres = dres; a.dy = dy;
+  a.dgate_rows = dgate_rows; a.rows = rows; a.width = width; a.scale = scale;
+  ColumnSums c{};
+  int sums = 0;
+  auto want = [&](void* out, float*& slot) {
+    if (!out) return;
+    slot = part + (long long)sums * blocks * width;
+    c.partial[sums] = slot;
+    c.out[sums++] = out;
+  };
+  want(dw, a.part_w);
+  want(dpost, a.part_post);
+  want(dgate, a.part_gate);
+  const int rc = residual_any(a, dtype, true, blocks, s);
+  if (rc || !sums) return rc;
+  const dim3 grid((width + 31) / 32, sums);
+  if (dtype == ROW_BF16) rv_column_sum<__nv_bfloat16><<<grid, 256, 0, s>>>(c, blocks, width);
+  else if (dtype == ROW_FP16) rv_column_sum<__half><<<grid, 256, 0, s>>>(c, blocks, width);
+  else rv_column_sum<float><<<grid, 256, 0, s>>>(c, blocks, width);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}

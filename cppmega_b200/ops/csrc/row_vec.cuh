@@ -1,0 +1,200 @@
+// Rows of bf16, fp16 or fp32 held in registers as 16-byte vectors by a team of TPR threads (vector i of thread t: t + i TPR).
+// VEC: every row starts on a 16-byte boundary and ends on one; otherwise the same vectors are moved element by element, the elements
+// past the row read as zero and are not written.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace cm {
+
+template <typename T>
+struct RowVec {
+  static constexpr int N = 16 / int(sizeof(T));
+};
+
+template <typename T>
+__device__ __forceinline__ void rv_unpack(const uint4& v, float (&f)[RowVec<T>::N]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  } else {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float2 p;
+      if constexpr (sizeof(T) == 2 && __is_same(T, __half)) p = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+      else p = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[j]));
+      f[2 * j] = p.x;
+      f[2 * j + 1] = p.y;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 rv_pack(const float (&f)[RowVec<T>::N]) {
+  if constexpr (sizeof(T) == 4) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  } else {
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (__is_same(T, __half)) {
+        const __half2 p = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+        u[j] = *reinterpret_cast<const uint32_t*>(&p);
+      } else {
+        u[j] = pack_bf16(f[2 * j], f[2 * j + 1]);
+      }
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+// vector `i` of the row (zero past its end)
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 rv_load(const T* __restrict__ row, int i, int width) {
+  constexpr int N = RowVec<T>::N;
+  if constexpr (VEC) {
+    return i * N < width ? reinterpret_cast<const uint4*>(row)[i] : make_uint4(0, 0, 0, 0);
+  } else {
+    float f[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = i * N + j < width ? float(row[i * N + j]) : 0.f;
+    return rv_pack<T>(f);
+  }
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void rv_store(T* __restrict__ row, int i, int width, const uint4& v) {
+  constexpr int N = RowVec<T>::N;
+  if constexpr (VEC) {
+    if (i * N < width) reinterpret_cast<uint4*>(row)[i] = v;
+  } else {
+    float f[N];
+    rv_unpack<T>(v, f);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i * N + j < width) row[i * N + j] = T(f[j]);
+  }
+}
+
+// Sums of K values over the TPR threads that hold a row, in every one of them.  A team of up to 32 lies within a warp and all lanes
+// of the warp take part; a larger one is the whole block.  `red`: [2][K][TPR / 32] floats of shared memory; `turn` alternates
+// between calls, so that one barrier a call is enough.
+template <int TPR, int K>
+__device__ __forceinline__ void rv_team_sum(float (&v)[K], float* red, int turn) {
+#pragma unroll
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if constexpr (TPR > 32) {
+    constexpr int NW = TPR / 32;
+    float* r = red + turn * K * NW;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) r[k * NW + (threadIdx.x >> 5)] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) s += r[k * NW + w];
+      v[k] = s;
+    }
+  }
+}
+
+template <int TPR>
+constexpr int rv_block() { return TPR < 128 ? 128 : TPR; }
+
+// Column sums that the rows' threads hold, one partial row per block: partial[blockIdx][column].  Teams of the same block are added in
+// shared memory (`scratch`, (rows per block) x VPT x TPR x N floats), in a fixed order.
+template <typename T, int TPR, int VPT>
+__device__ __forceinline__ void rv_partial(const float (&acc)[VPT][RowVec<T>::N], float* __restrict__ out, int width, float* scratch) {
+  constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
+  const int t = threadIdx.x % TPR;
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int c = (t + i * TPR) * N + j;
+        if (c < width) out[c] = acc[i][j];
+      }
+  } else {
+    constexpr int W = VPT * TPR * N;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) scratch[(threadIdx.x / TPR) * W + (t + i * TPR) * N + j] = acc[i][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < width; c += rv_block<TPR>()) {
+      float s = 0.f;
+#pragma unroll
+      for (int r = 0; r < RPB; ++r) s += scratch[r * W + c];
+      out[c] = s;
+    }
+  }
+}
+
+// out[c] = sum over p of partial[p][c], c < width, in a fixed order; blockIdx.y chooses one of up to three sums.
+struct ColumnSums {
+  const float* partial[3];
+  void* out[3];
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) rv_column_sum(const ColumnSums s, int parts, int width) {
+  __shared__ float red[8][33];
+  const float* __restrict__ in = s.partial[blockIdx.y];
+  T* out = reinterpret_cast<T*>(s.out[blockIdx.y]);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float a = 0.f;
+  if (c < width)
+    for (int p = w; p < parts; p += 8) a += in[(long long)p * width + c];
+  red[w][lane] = a;
+  __syncthreads();
+  if (w == 0 && c < width) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += red[k][lane];
+    out[c] = T(t);
+  }
+}
+
+enum RowType : int { ROW_BF16 = 0, ROW_FP16 = 1, ROW_FP32 = 2 };
+
+// The team of a row of `nvec` vectors, as 16 * threads + vectors a thread; 0: too wide.
+static inline int rv_team(int nvec, bool vec) {
+  if (!vec) return nvec <= 64 ? 16 * 32 + 2 : nvec <= 256 ? 16 * 128 + 2 : nvec <= 1024 ? 16 * 512 + 2 : nvec <= 4096 ? 16 * 1024 + 4 : 0;
+  return nvec <= 8 ? 16 * 8 + 1 : nvec <= 32 ? 16 * 32 + 1 : nvec <= 64 ? 16 * 32 + 2 : nvec <= 128 ? 16 * 128 + 1
+         : nvec <= 256 ? 16 * 128 + 2 : nvec <= 512 ? 16 * 256 + 2 : nvec <= 1024 ? 16 * 512 + 2 : nvec <= 2048 ? 16 * 1024 + 2
+         : nvec <= 4096 ? 16 * 1024 + 4 : 0;
+}
+
+// CM_ROW_TEAM(team, vec, F): calls F(threads, vectors, vec) with compile-time values; -10 for a team that does not exist.
+#define CM_ROW_TEAM(team, vec, F)                                                                                   \
+  if (vec) {                                                                                                        \
+    switch (team) {                                                                                                 \
+      case 16 * 8 + 1: return F(8, 1, true);                                                                        \
+      case 16 * 32 + 1: return F(32, 1, true);                                                                      \
+      case 16 * 32 + 2: return F(32, 2, true);                                                                      \
+      case 16 * 128 + 1: return F(128, 1, true);                                                                    \
+      case 16 * 128 + 2: return F(128, 2, true);                                                                    \
+      case 16 * 256 + 2: return F(256, 2, true);                                                                    \
+      case 16 * 512 + 2: return F(512, 2, true);                                                                    \
+      case 16 * 1024 + 2: return F(1024, 2, true);                                                                  \
+      case 16 * 1024 + 4: return F(1024, 4, true);                                                                  \
+    }                                                                                                               \
+  } else {                                                                                                          \
+    switch (team) {                                                                                                 \
+      case 16 * 32 + 2: return F(32, 2, false);                                                                     \
+      case 16 * 128 + 2: return F(128, 2, false);                                                                   \
+      case 16 * 512 + 2: return F(512, 2, false);                                                                   \
+      case 16 * 1024 + 4: return F(1024, 4, false);                                                                 \
+    }                                                                                                               \
+  }                                                                                                                 \
+  return -10
+
+}  // namespace cm

@@ -62,10 +62,11 @@ def _declare(L: ctypes.CDLL) -> None:
         if fn is not None:
             fn.argtypes = args
             fn.restype = i32
-    from . import attention, extra, kernels4
+    from . import attention, block, extra, kernels4
     extra.declare(L)
     kernels4.declare(L)
     attention.declare(L)
+    block.declare(L)
 
 
 def stream_ptr() -> int:
@@ -389,10 +390,11 @@ def _register() -> None:
     F_.register_cuda("rmsnorm", rmsnorm)
     F_.register_cuda("swiglu", swiglu)
     F_.register_cuda("adamw_shard", adamw_shard)
-    from . import attention, extra, kernels4
+    from . import attention, block, extra, kernels4
     extra.register()
     kernels4.register()
     attention.register()
+    block.register()
 
 
 if torch.cuda.is_available():

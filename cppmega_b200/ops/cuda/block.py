@@ -1,0 +1,318 @@
+"""The operators around a dense block: gated feed-forward (``csrc/gated_mlp.cu``), residual step with its norms
+(``csrc/residual_norm.cu``) and gated norm of a mixer's output (``csrc/gated_norm.cu``), with their autograd wrappers.
+
+The wrappers take their tensors as they come: leading dimensions of any number, rows of any pitch (column slices of a wider
+projection are read in place), widths that no vector divides.  Work space is allocated per call on the current stream.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import functional as F_
+
+ACTIVATIONS = {"silu": 0, "gelu_tanh": 1, "relu": 2}
+ROW_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_WIDTH = 16384          # widest normalised row
+
+
+def declare(L: ctypes.CDLL) -> None:
+    vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+    sig = {
+        "cm_gated_mlp_fwd": [vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp],
+        "cm_gated_mlp_bwd": [vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp],
+        "cm_residual_rmsnorm_fwd": [vp, i64, vp, i64, vp, vp, vp, i32, vp, vp, vp, vp, i64, i32, f32, f32, i32, vp],
+        "cm_row_norm_parts": [i64, i32, i32],
+        "cm_residual_rmsnorm_bwd": [vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, f32,
+                                    i32, vp],
+        "cm_rmsnorm_gated_fwd": [vp, i64, vp, i64, vp, vp, vp, i64, i32, i32, i32, f32, i32, vp],
+        "cm_rmsnorm_gated_parts": [i64, i32, i32, i32],
+        "cm_rmsnorm_gated_bwd": [vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, vp],
+    }
+    for name, args in sig.items():
+        fn = getattr(L, name, None)
+        if fn is not None:
+            fn.argtypes = args
+            fn.restype = i32
+
+
+def _lib():
+    from . import lib
+    return lib()
+
+
+def _stream() -> int:
+    from . import stream_ptr
+    return stream_ptr()
+
+
+def _call(name: str, *args) -> None:
+    rc = getattr(_lib(), name)(*args)
+    if rc:
+        from . import KernelError
+        raise KernelError(f"{name} failed with code {rc}")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _device_of(t: torch.Tensor):
+    """Launches go to the device of the tensors, whichever is current."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _rows(t: torch.Tensor):
+    """``(tensor, elements between rows)`` of the [rows, width] view of a tensor whose rows are contiguous and evenly spaced; any
+    other tensor is copied."""
+    from . import fast_contiguous
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    if t.stride(-1) == 1 or t.shape[-1] == 1:
+        pitch = expect = None
+        for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if n == 1:
+                continue
+            if pitch is None:
+                pitch = expect = s
+            if s != expect:
+                pitch = 0
+                break
+            expect = s * n
+        if pitch is None:
+            return t, t.shape[-1]
+        if pitch >= t.shape[-1]:
+            return t, pitch
+    return fast_contiguous(t), t.shape[-1]
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ---------------------------------------------------------------------------
+# gated feed-forward block
+# ---------------------------------------------------------------------------
+
+def _tma_rows(t: torch.Tensor):
+    """As :func:`_rows`, for a bf16 operand that is read through a tensor map: 16-byte rows and base."""
+    t, pitch = _rows(t)
+    if pitch % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        pitch = t.shape[-1]
+    return t, pitch
+
+
+def _mlp_forward(x, w1, w2, act, keep):
+    from . import err_word
+    x, ldx = _tma_rows(x)
+    H, F, Ho = w1.shape[1], w2.shape[1], w2.shape[0]
+    M = x.numel() // H
+    y = torch.empty(*x.shape[:-1], Ho, dtype=x.dtype, device=x.device)
+    h = torch.empty(M, F, dtype=x.dtype, device=x.device)
+    gu = torch.empty(M, 2 * F, dtype=x.dtype, device=x.device) if keep else None
+    _call("cm_gated_mlp_fwd", x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), _ptr(gu), h.data_ptr(), y.data_ptr(), M, H, F, Ho, act,
+          err_word(x.device).data_ptr(), _stream())
+    F_.count_launch("gated_mlp")
+    return y, x, gu, h
+
+
+class GatedMLPFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w1, w2, act):
+        y, x, gu, h = _mlp_forward(x, w1, w2, act, keep=True)
+        ctx.save_for_backward(x, w1, w2, gu, h)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        from . import err_word, wgrad_into_main_grad
+        x, w1, w2, gu, h = ctx.saved_tensors
+        need_x, need_w1, need_w2, _ = ctx.needs_input_grad
+        H, F, Ho = w1.shape[1], w2.shape[1], w2.shape[0]
+        M = h.shape[0]
+        dy, lddy = _tma_rows(dy)
+        x, ldx = _tma_rows(x)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        into = {1: (None, 0, 0), 2: (None, 0, 0)}                  # (result, its type, added to what is there) per weight
+
+        def target(i, w):
+            def run(out, acc):
+                t = torch.empty_like(w) if out is None else out
+                into[i] = (t, int(t.dtype == torch.float32), int(acc))
+                return t
+            return run
+
+        dw1 = wgrad_into_main_grad(w1, target(1, w1)) if need_w1 else None
+        dw2 = wgrad_into_main_grad(w2, target(2, w2)) if need_w2 else None
+        dgu = torch.empty_like(gu) if need_x or need_w1 else None
+        (t1, f1, a1), (t2, f2, a2) = into[1], into[2]
+        _call("cm_gated_mlp_bwd", dy.data_ptr(), lddy, x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), gu.data_ptr(), h.data_ptr(),
+              _ptr(dgu), _ptr(dx), _ptr(t1), f1, a1, _ptr(t2), f2, a2, M, H, F, Ho, ctx.act, err_word(x.device).data_ptr(), _stream())
+        F_.count_launch("gated_mlp_bwd")
+        return dx, dw1, dw2, None
+
+
+def gated_mlp(x, w1, w2, activation):
+    """None where the kernels do not apply: they take bf16 throughout and widths that are multiples of 8."""
+    if not (x.dtype == w1.dtype == w2.dtype == torch.bfloat16 and w1.is_contiguous() and w2.is_contiguous() and x.numel() > 0
+            and x.shape[-1] % 8 == 0 and w2.shape[0] % 8 == 0 and w2.shape[1] % 8 == 0 and w1.data_ptr() % 16 == 0
+            and w2.data_ptr() % 16 == 0 and x.numel() // x.shape[-1] < 2 ** 31):
+        return None
+    with _device_of(x):
+        if _wants_grad(x, w1, w2):
+            return GatedMLPFn.apply(x, w1, w2, ACTIVATIONS[activation])
+        return _mlp_forward(x, w1, w2, ACTIVATIONS[activation], keep=False)[0]
+
+
+# ---------------------------------------------------------------------------
+# residual step with its norms
+# ---------------------------------------------------------------------------
+
+def _residual_forward(y, residual, weight, post, gate, scale, eps, keep):
+    y, sy = _rows(y)
+    residual, sres = _rows(residual)
+    W = y.shape[-1]
+    R = y.numel() // W
+    n = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    h = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    stats = torch.empty(2, R, dtype=torch.float32, device=y.device) if keep else None
+    _call("cm_residual_rmsnorm_fwd", y.data_ptr(), sy, residual.data_ptr(), sres, weight.data_ptr(), _ptr(post), _ptr(gate),
+          int(gate is not None and gate.dim() > 1), n.data_ptr(), h.data_ptr(), _ptr(stats), None if stats is None else stats[1].data_ptr(),
+          R, W, scale, eps, ROW_TYPES[y.dtype], _stream())
+    F_.count_launch("residual_rmsnorm")
+    return n, h, y, stats
+
+
+class ResidualRMSNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, residual, weight, post, gate, scale, eps):
+        n, h, y, stats = _residual_forward(y, residual, weight, post, gate, scale, eps, keep=True)
+        # the block's output is read again only where a norm or a gate stands between it and the stream
+        ctx.save_for_backward(h, y if post is not None or gate is not None else None, weight, post, gate, stats)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return n, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dn, dh):
+        if dn is None and dh is None:
+            return (None,) * 7
+        h, y, weight, post, gate, stats = ctx.saved_tensors
+        need_y, _, need_w, need_post, need_gate = ctx.needs_input_grad[:5]
+        W = h.shape[-1]
+        R = h.numel() // W
+        dt, dev = h.dtype, h.device
+        sy = sdn = sdh = 0
+        if y is not None:
+            y, sy = _rows(y)
+        if dn is not None:
+            dn, sdn = _rows(dn)
+        if dh is not None:
+            dh, sdh = _rows(dh)
+        per_row = gate is not None and gate.dim() > 1
+        dres = torch.empty(h.shape, dtype=dt, device=dev)
+        same = y is None and ctx.scale == 1.0
+        dy = torch.empty(h.shape, dtype=dt, device=dev) if need_y and not same else None
+        dgate_rows = torch.empty(h.shape, dtype=dt, device=dev) if need_gate and per_row else None
+        sums = [torch.empty(W, dtype=dt, device=dev) if need else None for need in (need_w, need_post, need_gate and not per_row)]
+        wanted = sum(t is not None for t in sums)
+        dtype = ROW_TYPES[dt]
+        part = torch.empty(wanted * _lib().cm_row_norm_parts(R, W, dtype) * W, dtype=torch.float32, device=dev) if wanted else None
+        _call("cm_residual_rmsnorm_bwd", _ptr(dn), sdn, _ptr(dh), sdh, h.data_ptr(), _ptr(y), sy, weight.data_ptr(), _ptr(post), _ptr(gate),
+              int(per_row), stats.data_ptr(), stats[1].data_ptr(), dres.data_ptr(), _ptr(dy), _ptr(dgate_rows), *map(_ptr, sums), _ptr(part),
+              R, W, ctx.scale, dtype, _stream())
+        F_.count_launch("residual_rmsnorm_bwd")
+        dw, dpost, dgate = sums
+        return (dres if same else dy), dres, dw, dpost, (dgate_rows if per_row else dgate), None, None
+
+
+def residual_rmsnorm(y, residual, weight, post_weight, gate, scale, eps):
+    """None where the kernels do not apply: one type for all tensors (bf16, fp16 or fp32), rows of at most 16384."""
+    every = [t for t in (y, residual, weight, post_weight, gate) if t is not None]
+    if y.dtype not in ROW_TYPES or any(t.dtype != y.dtype for t in every) or y.shape[-1] > MAX_WIDTH or y.numel() == 0:
+        return None
+    weight = weight.contiguous()
+    post_weight = None if post_weight is None else post_weight.contiguous()
+    gate = None if gate is None else gate.contiguous()
+    with _device_of(y):
+        if _wants_grad(*every):
+            return ResidualRMSNormFn.apply(y, residual, weight, post_weight, gate, float(scale), float(eps))
+        return _residual_forward(y, residual, weight, post_weight, gate, float(scale), float(eps), keep=False)[:2]
+
+
+# ---------------------------------------------------------------------------
+# gated norm
+# ---------------------------------------------------------------------------
+
+def _gated_forward(x, weight, z, eps, group, gate_first, keep):
+    x, sx = _rows(x)
+    sz = 0
+    if z is not None:
+        z, sz = _rows(z)
+    W = x.shape[-1]
+    R = x.numel() // W
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rstd = torch.empty(R * (W // group), dtype=torch.float32, device=x.device) if keep else None
+    _call("cm_rmsnorm_gated_fwd", x.data_ptr(), sx, _ptr(z), sz, weight.data_ptr(), y.data_ptr(), _ptr(rstd), R, W, group, int(gate_first),
+          eps, ROW_TYPES[x.dtype], _stream())
+    F_.count_launch("rmsnorm_gated")
+    return y, x, z, rstd
+
+
+class GatedRMSNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, z, eps, group, gate_first):
+        y, x, z, rstd = _gated_forward(x, weight, z, eps, group, gate_first, keep=True)
+        ctx.save_for_backward(x, weight, z, rstd)
+        ctx.group, ctx.gate_first = group, gate_first
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, z, rstd = ctx.saved_tensors
+        _, need_w, need_z = ctx.needs_input_grad[:3]
+        W, dt, dev = x.shape[-1], x.dtype, x.device
+        R = x.numel() // W
+        x, sx = _rows(x)
+        dy, sdy = _rows(dy)
+        sz = 0
+        if z is not None:
+            z, sz = _rows(z)
+        dx = torch.empty(x.shape, dtype=dt, device=dev)
+        dz = torch.empty(x.shape, dtype=dt, device=dev) if need_z else None
+        dw = part = None
+        dtype = ROW_TYPES[dt]
+        if need_w:
+            dw = torch.empty(W, dtype=dt, device=dev)
+            part = torch.empty(_lib().cm_rmsnorm_gated_parts(R, W, ctx.group, dtype) * W, dtype=torch.float32, device=dev)
+        _call("cm_rmsnorm_gated_bwd", x.data_ptr(), sx, _ptr(z), sz, weight.data_ptr(), dy.data_ptr(), sdy, rstd.data_ptr(), dx.data_ptr(),
+              _ptr(dz), _ptr(dw), _ptr(part), R, W, ctx.group, int(ctx.gate_first), dtype, _stream())
+        F_.count_launch("rmsnorm_gated_bwd")
+        return dx, dw, dz, None, None, None
+
+
+def rmsnorm_gated(x, weight, z, eps, group, norm_before_gate):
+    """None where the kernels do not apply: one type for all tensors (bf16, fp16 or fp32), groups of at most 16384 channels and at
+    most 65535 of them."""
+    every = [t for t in (x, weight, z) if t is not None]
+    if x.dtype not in ROW_TYPES or any(t.dtype != x.dtype for t in every) or group > MAX_WIDTH or x.numel() == 0 or x.shape[-1] // group > 65535:
+        return None
+    weight = weight.contiguous()
+    with _device_of(x):
+        if _wants_grad(*every):
+            return GatedRMSNormFn.apply(x, weight, z, float(eps), group, not norm_before_gate)
+        return _gated_forward(x, weight, z, float(eps), group, not norm_before_gate, keep=False)[0]
+
+
+def register() -> None:
+    F_.register_cuda("gated_mlp", gated_mlp)
+    F_.register_cuda("residual_rmsnorm", residual_rmsnorm)
+    F_.register_cuda("rmsnorm_gated", rmsnorm_gated)

@@ -108,6 +108,17 @@ def _cuda(name: str, *tensors) -> Optional[Callable]:
     return fn
 
 
+def _require(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def _same_device(name: str, first: torch.Tensor, *others) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+
+
 # ---- dense ---------------------------------------------------------------
 
 _PRECISION_RECIPE = "bf16"
@@ -248,8 +259,42 @@ def rmsnorm(x, weight, eps: float = 1e-5):
 
 
 def rmsnorm_gated(x, weight, z=None, eps: float = 1e-5, group_size=None, norm_before_gate=True):
-    _miss("rmsnorm_gated", x)          # PyTorch definition on every device
+    """RMS norm of a mixer's output with a SiLU gate: ``rms(x) * weight * silu(z)``, or ``rms(x * silu(z)) * weight`` with
+    ``norm_before_gate=False``; every ``group_size`` channels normalise apart (default: the whole row).  ``x``, ``z`` [..., D] of
+    one type, rows of any pitch (column slices of a projection are read in place), ``weight`` [D]."""
+    D = x.shape[-1]
+    group = int(group_size) if group_size else D
+    fn = _cuda("rmsnorm_gated", x)
+    if fn is not None:
+        y = None
+        if weight.shape == (D,) and (z is None or z.shape == x.shape) and D % group == 0:
+            _same_device("rmsnorm_gated", x, weight, z)
+            y = fn(x, weight, z, eps, group, norm_before_gate)
+        if y is not None:
+            return y
+        _miss("rmsnorm_gated(shape/dtype)", x)
     return ref.rmsnorm_gated(x, weight, z, eps, group_size, norm_before_gate)
+
+
+def residual_rmsnorm(y, residual, weight, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-5):
+    """The step between two blocks: ``h = residual + scale * gate * p`` with ``p = rms(y) * post_weight`` (``y`` itself without a
+    post norm), and the norm the next block reads, ``n = rms(h) * weight``.  Returns ``(n, h)``, both in the type of ``y``; ``n``
+    is the norm of ``h`` as rounded to that type.  ``y``, ``residual`` [..., D]; ``gate`` [D] (one per channel, shared by all
+    rows) or the shape of ``y``; ``weight``, ``post_weight`` [D]."""
+    D = y.shape[-1]
+    _require(residual.shape == y.shape, f"residual_rmsnorm: block output {tuple(y.shape)}, residual {tuple(residual.shape)}")
+    for name, t in (("weight", weight), ("post_weight", post_weight)):
+        _require(t is None or t.shape == (D,), f"residual_rmsnorm: {name} {None if t is None else tuple(t.shape)} for rows of {D}")
+    _require(gate is None or gate.shape == (D,) or gate.shape == y.shape,
+             f"residual_rmsnorm: gate {None if gate is None else tuple(gate.shape)} is neither ({D},) nor {tuple(y.shape)}")
+    _same_device("residual_rmsnorm", y, residual, weight, post_weight, gate)
+    fn = _cuda("residual_rmsnorm", y)
+    if fn is not None:
+        out = fn(y, residual, weight, post_weight, gate, scale, eps)
+        if out is not None:
+            return out
+        _miss("residual_rmsnorm(shape/dtype)", y)
+    return ref.residual_rmsnorm(y, residual, weight, post_weight, gate, scale, eps)
 
 
 def head_linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
@@ -263,6 +308,25 @@ def head_linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
             return y
     _miss("head_linear(library bmm)", x)
     return torch.einsum("...hi,hoi->...ho", x, w.to(x.dtype))
+
+
+def gated_mlp(x, w1, w2, activation: str = "silu"):
+    """Gated feed-forward block ``(act(x Wg^T) * (x Wu^T)) W2^T``: ``x`` [..., H], ``w1`` [2F, H] (the gate rows, then the up rows),
+    ``w2`` [Ho, F]; ``activation`` is ``silu``, ``gelu_tanh`` or ``relu``.  In bf16 with widths that are multiples of 8 the
+    projections, the activation and the product are one kernel, and so are their gradients; under an FP8 recipe, and for anything
+    else, it is :func:`linear`, activation, :func:`linear`."""
+    _require(activation in ref.GATED_ACTIVATIONS, f"gated_mlp: unknown activation {activation!r}, one of {sorted(ref.GATED_ACTIVATIONS)}")
+    _require(w1.dim() == 2 and w2.dim() == 2 and x.dim() >= 1 and w1.shape[1] == x.shape[-1] and w1.shape[0] == 2 * w2.shape[1],
+             f"gated_mlp: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}")
+    _same_device("gated_mlp", x, w1, w2)
+    fn = _cuda("gated_mlp", x) if _PRECISION_RECIPE == "bf16" else None
+    if fn is not None:
+        y = fn(x, w1, w2, activation)
+        if y is not None:
+            return y
+        _miss("gated_mlp(shape/dtype)", x)
+    gate_up = linear(x, w1)
+    return linear(swiglu(gate_up) if activation == "silu" else ref.gated_activation(gate_up, activation), w2)
 
 
 def swiglu(gate_up):

@@ -53,6 +53,37 @@ def swiglu(gate_up: torch.Tensor) -> torch.Tensor:
     return (F.silu(a.float()) * b.float()).to(gate_up.dtype)
 
 
+GATED_ACTIVATIONS = {
+    "silu": F.silu,
+    "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"),
+    "relu": F.relu,
+}
+
+
+def gated_activation(gate_up: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """``act(a) * b`` for ``gate_up = [a | b]`` along the last dim."""
+    a, b = gate_up.chunk(2, dim=-1)
+    return (GATED_ACTIVATIONS[activation](a.float()) * b.float()).to(gate_up.dtype)
+
+
+def gated_mlp(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """``(act(x Wg^T) * (x Wu^T)) W2^T`` with ``w1 = [Wg; Wu]``, in fp32 throughout."""
+    return (gated_activation(x.float() @ w1.float().t(), activation) @ w2.float().t()).to(x.dtype)
+
+
+def residual_rmsnorm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, post_weight: Optional[torch.Tensor] = None,
+                     gate: Optional[torch.Tensor] = None, scale: float = 1.0, eps: float = 1e-5):
+    """``h = residual + scale * gate * p``, ``p = rms(y) * post_weight`` or ``y``; ``n = rms(h) * weight`` of the rounded ``h``.
+    Returns ``(n, h)``."""
+    p = y.float()
+    if post_weight is not None:
+        p = p * torch.rsqrt(p.pow(2).mean(-1, keepdim=True) + eps) * post_weight.float()
+    if gate is not None:
+        p = p * gate.float()
+    h = (residual.float() + scale * p).to(y.dtype)
+    return rmsnorm(h, weight, eps), h
+
+
 # ---------------------------------------------------------------------------
 # rotary embedding (attention)
 # ---------------------------------------------------------------------------
