@@ -9,6 +9,10 @@
 // every wait bounded, no multicast).  The first CTA of a pair loads the gate rows of w1 and the second the up rows, so that the tile is
 // one ordinary 256-column product.  The epilogue has eight warps, two to a TMEM quadrant: its exponentials, and in the backward its
 // loads of g and u, have to fit under the main loop of the next tile.
+//
+// Few tokens (serving): both products read their weights once through few_rows.cu; the sums of the first one's partial tiles, the
+// activation and the product are one small kernel, the sums of the second another.
+#include "few_rows.cuh"
 #include "gemm_pair.cuh"
 
 extern "C" int cm_gemm_bf16(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc,
@@ -376,6 +380,76 @@ static int plan_bn(int M, int F, bool back) {
   return waves(128) * 17.8 < waves(256) * 24.2 ? 128 : 256;
 }
 
+// ------------------------------ few tokens ------------------------------
+// A tile's sum over its partial tiles, for TOKS tokens of one weight row: their loads are in flight together, and the place of a partial
+// tile is found once for all of them.
+constexpr int TOKS = 8;
+__device__ __forceinline__ void few_sum(const float* __restrict__ part, const few::Cut& cut, int row, int tok0, float (&s)[TOKS]) {
+  const int t = row / few::TILE, in = row % few::TILE, n = min(TOKS, cut.tokens - tok0);
+#pragma unroll
+  for (int j = 0; j < TOKS; ++j) s[j] = 0.f;
+  for (int c = cut.first(t); c <= cut.last(t); ++c) {
+    const float* p = part + cut.at(c, t) + tok0 * few::TILE + in;
+#pragma unroll
+    for (int j = 0; j < TOKS; ++j)
+      if (j < n) s[j] += p[j * few::TILE];
+  }
+}
+
+// h[token][f] = act(g) u from rows f and F + f of the first product; g, u kept for training.
+template <int ACT>
+__global__ void __launch_bounds__(128) few_gate_kernel(const float* __restrict__ part, const few::Cut cut, int F, __nv_bfloat16* __restrict__ h,
+                                                       __nv_bfloat16* __restrict__ gu) {
+  const int f = blockIdx.x * 128 + threadIdx.x, tok0 = blockIdx.y * TOKS;
+  few::wait_for_input();
+  few::let_next_start();
+  if (f >= F) return;
+  float g[TOKS], u[TOKS];
+  few_sum(part, cut, f, tok0, g);
+  few_sum(part, cut, F + f, tok0, u);
+#pragma unroll
+  for (int j = 0; j < TOKS; ++j) {
+    const long long tok = tok0 + j;
+    if (tok >= cut.tokens) break;
+    h[tok * F + f] = __float2bfloat16(act_of<ACT>(g[j]) * u[j]);
+    if (gu) {
+      gu[tok * 2 * F + f] = __float2bfloat16(g[j]);
+      gu[tok * 2 * F + F + f] = __float2bfloat16(u[j]);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(128) few_sum_kernel(const float* __restrict__ part, const few::Cut cut, int N, __nv_bfloat16* __restrict__ y) {
+  const int n = blockIdx.x * few::TILE + threadIdx.x, tok0 = blockIdx.y * TOKS;
+  few::wait_for_input();
+  if (n >= N) return;
+  float s[TOKS];
+  few_sum(part, cut, n, tok0, s);
+#pragma unroll
+  for (int j = 0; j < TOKS; ++j)
+    if (tok0 + j < cut.tokens) y[(long long)(tok0 + j) * N + n] = __float2bfloat16(s[j]);
+}
+
+// Tokens up to which the weights are streamed by few_rows.cu.
+constexpr int FEW_TOKENS = 256;
+
+static int few_forward(const void* x, long long ldx, const void* w1, const void* w2, __nv_bfloat16* gu, __nv_bfloat16* h, __nv_bfloat16* y,
+                       float* ws, int M, int H, int F, int Ho, int act, int* err, cudaStream_t stream) {
+  const few::Cut c1 = few::cut_for(M, 2 * F, H), c2 = few::cut_for(M, Ho, F);
+  int rc = few::launch_partials(x, ldx, w1, ws, c1, 2 * F, H, false, err, stream);
+  if (rc) return rc;
+  const dim3 grid((F + 127) / 128, (M + TOKS - 1) / TOKS);
+  switch (act) {
+    case SILU: rc = few::launch_early(few_gate_kernel<SILU>, grid, 128, 0, stream, ws, c1, F, h, gu); break;
+    case GELU_TANH: rc = few::launch_early(few_gate_kernel<GELU_TANH>, grid, 128, 0, stream, ws, c1, F, h, gu); break;
+    case RELU: rc = few::launch_early(few_gate_kernel<RELU>, grid, 128, 0, stream, ws, c1, F, h, gu); break;
+    default: rc = -10;
+  }
+  if (!rc) rc = few::launch_partials(h, F, w2, ws, c2, Ho, F, true, err, stream);
+  if (!rc) rc = few::launch_early(few_sum_kernel, dim3((Ho + few::TILE - 1) / few::TILE, (M + TOKS - 1) / TOKS), 128, 0, stream, ws, c2, Ho, y);
+  return rc;
+}
+
 static bool tma_ok(const void* p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 
 }  // namespace mlp
@@ -383,14 +457,26 @@ static bool tma_ok(const void* p, long long ld) { return (reinterpret_cast<uintp
 
 using namespace cm;
 
+// Floats of work space that the forward needs; 0: none.
+extern "C" long long cm_gated_mlp_fwd_ws(int M, int H, int F, int Ho) {
+  if (M > mlp::FEW_TOKENS || M <= 0) return 0;
+  const long long a = few::cut_for(M, 2 * F, H).floats(), b = few::cut_for(M, Ho, F).floats();
+  return a > b ? a : b;
+}
+
 // y[M, Ho] = (act(x w1[:F]^T) * (x w1[F:]^T)) w2^T; x [M, H] with row pitch ldx, w1 [2F, H], w2 [Ho, F], h [M, F]; gu [M, 2F] or null
-// (not kept).  act: 0 silu, 1 gelu (tanh form), 2 relu.
-extern "C" int cm_gated_mlp_fwd(const void* x, long long ldx, const void* w1, const void* w2, void* gu, void* h, void* y, int M, int H,
-                                int F, int Ho, int act, int* err, cudaStream_t stream) {
+// (not kept).  act: 0 silu, 1 gelu (tanh form), 2 relu.  ws: cm_gated_mlp_fwd_ws floats of work space.
+extern "C" int cm_gated_mlp_fwd(const void* x, long long ldx, const void* w1, const void* w2, void* gu, void* h, void* y, float* ws, int M,
+                                int H, int F, int Ho, int act, int* err, cudaStream_t stream) {
   if (M <= 0 || H <= 0 || F <= 0 || Ho <= 0) return 0;
   if (H % 8 || F % 8 || Ho % 8 || !mlp::tma_ok(x, ldx) || !mlp::tma_ok(w1, H) || !mlp::tma_ok(w2, F) || !mlp::tma_ok(gu, 0) ||
       !mlp::tma_ok(h, F) || !mlp::tma_ok(y, Ho))
     return -10;
+  if (M <= mlp::FEW_TOKENS) {
+    if (!ws) return -10;
+    return mlp::few_forward(x, ldx, w1, w2, static_cast<__nv_bfloat16*>(gu), static_cast<__nv_bfloat16*>(h), static_cast<__nv_bfloat16*>(y), ws,
+                            M, H, F, Ho, act, err, stream);
+  }
   mlp::Args args{M, F, H, mlp::plan_bn(M, F, false), nullptr, gu != nullptr, err};
   CUtensorMap maps[5];
   int rc = make_tmap_2d_bf16(&maps[0], x, M, H, ldx, mlp::BM);

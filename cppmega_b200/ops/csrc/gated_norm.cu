@@ -75,30 +75,38 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArg
 template <typename T, int TPR, int VPT, bool VEC>
 __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArgs a) {
   constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
+  extern __shared__ __align__(16) uint4 dyn[];
   __shared__ float red[2 * (TPR > 32 ? TPR / 32 : 1)];
   __shared__ float scratch[RPB > 1 ? RPB * TPR * VPT * N : 1];
+  enum { XX = 0, DY = 1, ZZ = 2 };
   const int t = threadIdx.x % TPR, g0 = blockIdx.y * a.group;
   float acc[VPT][N] = {};
+  RowRing<T, TPR, VPT, VEC, rv_stages(TPR, VPT), 3> in;
+  in.ring = dyn;
+  in.ops = 3;
+  in.width = a.group;
+  in.rows = a.rows;
+  in.base[XX] = reinterpret_cast<const T*>(a.x) + g0;
+  in.base[DY] = reinterpret_cast<const T*>(a.dy) + g0;
+  in.base[ZZ] = a.z ? reinterpret_cast<const T*>(a.z) + g0 : nullptr;
+  in.pitch[XX] = a.sx;
+  in.pitch[DY] = a.sdy;
+  in.pitch[ZZ] = a.sz;
+  const long long step = (long long)gridDim.x * RPB;
+  in.start((long long)blockIdx.x * RPB + threadIdx.x / TPR, step);
   int turn = 0;
-  for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += (long long)gridDim.x * RPB, turn ^= 1) {
+  for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += step, turn ^= 1) {
     const long long row = row0 + threadIdx.x / TPR;
     const int G = row < a.rows ? a.group : 0;
-    uint4 xv[VPT], zv[VPT], dv[VPT];
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = t + i * TPR;
-      xv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.sx + g0, c, G);
-      zv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.z) + row * a.sz + g0, c, a.z ? G : 0);
-      dv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.sdy + g0, c, G);
-    }
     const float r = G ? a.rstd[row * gridDim.y + blockIdx.y] : 0.f;
+    in.wait(row);
     float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       float x[N], z[N], d[N], w[N];
-      rv_unpack<T>(xv[i], x);
-      rv_unpack<T>(zv[i], z);
-      rv_unpack<T>(dv[i], d);
+      rv_unpack<T>(in.get(XX, i), x);
+      rv_unpack<T>(in.get(ZZ, i), z);
+      rv_unpack<T>(in.get(DY, i), d);
       rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, t + i * TPR, G), w);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -109,15 +117,14 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
       }
     }
     rv_team_sum<TPR, 1>(s, red, turn);
-    if (!G) continue;
     const float m = s[0] / a.group;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * TPR;
       float x[N], z[N], d[N], w[N];
-      rv_unpack<T>(xv[i], x);
-      rv_unpack<T>(zv[i], z);
-      rv_unpack<T>(dv[i], d);
+      rv_unpack<T>(in.get(XX, i), x);
+      rv_unpack<T>(in.get(ZZ, i), z);
+      rv_unpack<T>(in.get(DY, i), d);
       rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, c, G), w);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -135,29 +142,41 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
       rv_store<T, VEC>(reinterpret_cast<T*>(a.dx) + row * a.width + g0, c, G, rv_pack<T>(x));
       if (a.dz) rv_store<T, VEC>(reinterpret_cast<T*>(a.dz) + row * a.width + g0, c, G, rv_pack<T>(z));
     }
+    in.next(row + (long long)rv_stages(TPR, VPT) * step);
   }
   if (a.part) rv_partial<T, TPR, VPT>(acc, a.part + (long long)blockIdx.x * a.width + g0, a.group, scratch);
 }
 
 template <typename T>
-static int gated_launch(const GatedArgs& a, bool back, int blocks, cudaStream_t s) {
+static int gated_launch(const GatedArgs& a, bool back, int& blocks, cudaStream_t s) {
   const int size = sizeof(T), nvec = (a.group + RowVec<T>::N - 1) / RowVec<T>::N, groups = a.width / a.group;
   auto fits = [&](const void* p, long long pitch) { return !p || ((reinterpret_cast<uintptr_t>(p) | (pitch * size)) & 15) == 0; };
   const bool vec = a.group * size % 16 == 0 && fits(a.x, a.sx) && fits(a.z, a.sz) && fits(a.w, 0) && fits(a.dy, a.sdy) &&
                    fits(a.y, a.width) && fits(a.dx, a.width) && fits(a.dz, a.width);
-  const int team = rv_team(nvec, vec);
+  const int team = rv_team(nvec, vec, true);
 #define CM_GATED(TPR, VPT, VEC)                                                                                                  \
   [&] {                                                                                                                          \
     constexpr int TB = rv_block<TPR>(), RPB = TB / TPR;                                                                          \
-    if (back) gated_norm_bwd<T, TPR, VPT, VEC><<<dim3(blocks, groups), TB, 0, s>>>(a);                                           \
-    else gated_norm_fwd<T, TPR, VPT, VEC><<<dim3(unsigned((a.rows + RPB - 1) / RPB), groups), TB, 0, s>>>(a);                    \
+    if (back) {                                                                                                                  \
+      auto kern = gated_norm_bwd<T, TPR, VPT, VEC>;                                                                              \
+      constexpr int RING = VEC ? rv_stages(TPR, VPT) * VPT * TB * 16 * 3 : 0;                                                    \
+      static PerDevice configured;                                                                                               \
+      if (configured.first()) {                                                                                                  \
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING) != cudaSuccess) return -2;             \
+        configured.done();                                                                                                       \
+      }                                                                                                                          \
+      static int resident;                                                                                                       \
+      blocks = rv_blocks(kern, TB, RING, RPB, a.rows, groups, resident);                                                         \
+      kern<<<dim3(blocks, groups), TB, RING, s>>>(a);                                                                            \
+    } else gated_norm_fwd<T, TPR, VPT, VEC><<<dim3(unsigned((a.rows + RPB - 1) / RPB), groups), TB, 0, s>>>(a);                    \
     return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                                           \
   }()
   CM_ROW_TEAM(team, vec, CM_GATED);
 #undef CM_GATED
 }
 
-static int gated_any(const GatedArgs& a, int dtype, bool back, int blocks, cudaStream_t s) {
+// `blocks`: out, the partial rows of the backward's weight gradient
+static int gated_any(const GatedArgs& a, int dtype, bool back, int& blocks, cudaStream_t s) {
   if (a.group <= 0 || a.width % a.group || a.width / a.group > 65535) return -10;
   switch (dtype) {
     case ROW_BF16: return gated_launch<__nv_bfloat16>(a, back, blocks, s);
@@ -178,35 +197,27 @@ extern "C" int cm_rmsnorm_gated_fwd(const void* x, long long sx, const void* z, 
   GatedArgs a{};
   a.x = x; a.sx = sx; a.z = z; a.sz = sz; a.w = w; a.y = y; a.rstd = rstd; a.rows = rows; a.width = width; a.group = group;
   a.gate_first = gate_first; a.eps = eps;
-  return gated_any(a, dtype, false, 0, s);
+  int blocks = 0;
+  return gated_any(a, dtype, false, blocks, s);
 }
 
-// Blocks along the rows, and with that the partial rows of the weight gradient.
-extern "C" int cm_rmsnorm_gated_parts(long long rows, int width, int group, int dtype) {
-  const int n = dtype == ROW_FP32 ? 4 : 8, nvec = (group + n - 1) / n, groups = width / group;
-  const long long threads = nvec <= 256 ? 128 : nvec <= 512 ? 256 : nvec <= 1024 ? 512 : 1024;
-  const long long most = ((long long)sm_count() * (1024 / threads) + groups - 1) / groups;
-  return int(rows < most ? (rows < 1 ? 1 : rows) : most);
-}
-
-// part: [cm_rmsnorm_gated_parts][width] floats of work space, with dw; dz, dw may be null.  dx, dz packed.
+// part: [cm_row_norm_parts][width] floats of work space, with dw; dz, dw may be null.  dx, dz packed.
 extern "C" int cm_rmsnorm_gated_bwd(const void* x, long long sx, const void* z, long long sz, const void* w, const void* dy, long long sdy,
                                     const float* rstd, void* dx, void* dz, void* dw, float* part, long long rows, int width, int group,
                                     int gate_first, int dtype, cudaStream_t s) {
   if (rows <= 0 || width <= 0) return 0;
-  if (group <= 0) return -10;
-  const int blocks = cm_rmsnorm_gated_parts(rows, width, group, dtype);
   GatedArgs a{};
   a.x = x; a.sx = sx; a.z = z; a.sz = sz; a.w = w; a.dy = dy; a.sdy = sdy; a.rstd = const_cast<float*>(rstd); a.dx = dx; a.dz = dz;
   a.part = dw ? part : nullptr; a.rows = rows; a.width = width; a.group = group; a.gate_first = gate_first;
+  int blocks = 0;
   const int rc = gated_any(a, dtype, true, blocks, s);
   if (rc || !dw) return rc;
   ColumnSums c{};
   c.partial[0] = part;
   c.out[0] = dw;
   const dim3 grid((width + 31) / 32, 1);
-  if (dtype == ROW_BF16) rv_column_sum<__nv_bfloat16><<<grid, 256, 0, s>>>(c, blocks, width);
-  else if (dtype == ROW_FP16) rv_column_sum<__half><<<grid, 256, 0, s>>>(c, blocks, width);
-  else rv_column_sum<float><<<grid, 256, 0, s>>>(c, blocks, width);
+  if (dtype == ROW_BF16) rv_column_sum<__nv_bfloat16><<<grid, 1024, 0, s>>>(c, blocks, width);
+  else if (dtype == ROW_FP16) rv_column_sum<__half><<<grid, 1024, 0, s>>>(c, blocks, width);
+  else rv_column_sum<float><<<grid, 1024, 0, s>>>(c, blocks, width);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }

@@ -28,6 +28,7 @@ struct ResidualArgs {
   long long sdn, sdh;
   void *dres, *dy, *dgate_rows;               // dy null: the same as dres
   float *part_w, *part_post, *part_gate;      // [blocks][width]; null: not wanted
+  int ring_ops;                               // operands in the ring
 };
 
 template <typename T, int TPR, int VPT, bool VEC, bool FULL>
@@ -109,53 +110,56 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_fwd(const Resid
 template <typename T, int TPR, int VPT, bool VEC, bool FULL>
 __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_bwd(const ResidualArgs a) {
   constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
+  extern __shared__ __align__(16) uint4 dyn[];
   __shared__ float red[2 * 3 * (TPR > 32 ? TPR / 32 : 1)];
   __shared__ float scratch[RPB > 1 ? RPB * TPR * VPT * N : 1];
+  enum { DN = 0, DH = 1, HH = 2, YY = 3, GG = 4 };
   const int t = threadIdx.x % TPR, W = a.width;
   float acc_w[VPT][N] = {}, acc_p[FULL ? VPT : 1][N] = {}, acc_g[FULL ? VPT : 1][N] = {};
   const bool post = FULL && a.post, gate = FULL && a.gate;
-  int turn = 0;
-  for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += (long long)gridDim.x * RPB, turn ^= 1) {
-    const long long row = row0 + threadIdx.x / TPR;
-    const bool on = row < a.rows;
-    const int w_on = on ? W : 0;
-    uint4 gv[VPT], dv[VPT], hv[VPT], yv[FULL ? VPT : 1], tv[FULL ? VPT : 1];
+  RowRing<T, TPR, VPT, VEC, rv_stages(TPR, VPT), FULL ? 5 : 3> in;
+  in.ring = dyn;
+  in.ops = a.ring_ops;
+  in.width = W;
+  in.rows = a.rows;
+  auto operand = [&](int op, const void* p, long long pitch) {
+    in.base[op] = reinterpret_cast<const T*>(p);
+    in.pitch[op] = pitch;
+  };
+  operand(DN, a.dn, a.sdn);
+  operand(DH, a.dh, a.sdh);
+  operand(HH, a.h, W);
+  if constexpr (FULL) {
+    operand(YY, a.y, a.sy);
+    operand(GG, a.gate_rows ? a.gate : nullptr, W);
+  }
+  const long long step = (long long)gridDim.x * RPB, first = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+  in.start(first, step);
+  // scale * gate of vector i
+  auto gated = [&](int i, float (&f)[N]) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = t + i * TPR;
-      gv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.dn) + row * a.sdn, c, a.dn ? w_on : 0);
-      dv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.dh) + row * a.sdh, c, a.dh ? w_on : 0);
-      hv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.h) + row * W, c, w_on);
-      if constexpr (FULL) {
-        yv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.y) + row * a.sy, c, w_on);
-        if (gate && a.gate_rows) tv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.gate) + row * W, c, w_on);
+    for (int j = 0; j < N; ++j) f[j] = a.scale;
+    if constexpr (FULL) {
+      if (gate) {
+        float q[N];
+        rv_unpack<T>(a.gate_rows ? in.get(GG, i) : rv_load<T, VEC>(reinterpret_cast<const T*>(a.gate), t + i * TPR, W), q);
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] *= q[j];
       }
     }
+  };
+  int turn = 0;
+  for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += step, turn ^= 1) {
+    const long long row = row0 + threadIdx.x / TPR;
+    const bool on = row < a.rows;
     const float rho = on ? a.rstd_h[row] : 0.f, r = on && post ? a.rstd_y[row] : 1.f;
-    // scale * gate * post of vector i
-    auto factor = [&](int i, float (&f)[N], bool with_post) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) f[j] = a.scale;
-      if constexpr (FULL) {
-        float q[N];
-        if (gate) {
-          rv_unpack<T>(a.gate_rows ? tv[i] : rv_load<T, VEC>(reinterpret_cast<const T*>(a.gate), t + i * TPR, W), q);
-#pragma unroll
-          for (int j = 0; j < N; ++j) f[j] *= q[j];
-        }
-        if (with_post) {
-          rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), t + i * TPR, W), q);
-#pragma unroll
-          for (int j = 0; j < N; ++j) f[j] *= q[j];
-        }
-      }
-    };
+    in.wait(row);
     float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       float g[N], h[N], w[N];
-      rv_unpack<T>(gv[i], g);
-      rv_unpack<T>(hv[i], h);
+      rv_unpack<T>(in.get(DN, i), g);
+      rv_unpack<T>(in.get(HH, i), h);
       rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w), t + i * TPR, W), w);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -166,13 +170,14 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_bwd(const Resid
       }
       if constexpr (FULL) {
         if (post) {
-          float d[N], y[N], f[N];
-          rv_unpack<T>(dv[i], d);
-          rv_unpack<T>(yv[i], y);
-          factor(i, f, true);
+          float d[N], y[N], f[N], p[N];
+          rv_unpack<T>(in.get(DH, i), d);
+          rv_unpack<T>(in.get(YY, i), y);
+          rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), t + i * TPR, W), p);
+          gated(i, f);
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            const float ay = f[j] * y[j] * r;
+            const float ay = f[j] * p[j] * y[j] * r;
             s[1] += ay * (rho * g[j] + d[j]);
             s[2] += ay * h[j];
           }
@@ -182,46 +187,45 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_bwd(const Resid
     if (post) rv_team_sum<TPR, 3>(s, red, turn);
     else rv_team_sum<TPR, 1>(reinterpret_cast<float(&)[1]>(s), red, turn);
     const float m1 = s[0] / W, m2 = (s[1] - rho * m1 * s[2]) / W;
-    if (!on) continue;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * TPR;
       float g[N], h[N], w[N], d[N];
-      rv_unpack<T>(gv[i], g);
-      rv_unpack<T>(hv[i], h);
-      rv_unpack<T>(dv[i], d);
+      rv_unpack<T>(in.get(DN, i), g);
+      rv_unpack<T>(in.get(HH, i), h);
+      rv_unpack<T>(in.get(DH, i), d);
       rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w), c, W), w);
 #pragma unroll
       for (int j = 0; j < N; ++j) d[j] += rho * (g[j] * w[j] - h[j] * rho * m1);
-      rv_store<T, VEC>(reinterpret_cast<T*>(a.dres) + row * W, c, W, rv_pack<T>(d));
+      rv_store<T, VEC>(reinterpret_cast<T*>(a.dres) + row * W, c, on ? W : 0, rv_pack<T>(d));
       if constexpr (FULL) {
-        float y[N], f[N];
-        rv_unpack<T>(yv[i], y);
-        float p[N];                           // y with the post norm: what the gate multiplies
+        float y[N], f[N], q[N], p[N];         // p: y with the post norm, which the gate multiplies
+        rv_unpack<T>(in.get(YY, i), y);
 #pragma unroll
         for (int j = 0; j < N; ++j) p[j] = y[j] *= r;
-        float q[N];
         if (post) {
           rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), c, W), q);
 #pragma unroll
           for (int j = 0; j < N; ++j) p[j] *= q[j];
         }
-        factor(i, f, false);
-        float dg[N];
+        gated(i, f);
+        if (gate) {
+          float dg[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) dg[j] = a.scale * d[j] * p[j];
-        if (gate && a.gate_rows) {
-          if (a.dgate_rows) rv_store<T, VEC>(reinterpret_cast<T*>(a.dgate_rows) + row * W, c, W, rv_pack<T>(dg));
-        } else {
+          for (int j = 0; j < N; ++j) dg[j] = on ? a.scale * d[j] * p[j] : 0.f;
+          if (a.gate_rows) {
+            if (a.dgate_rows) rv_store<T, VEC>(reinterpret_cast<T*>(a.dgate_rows) + row * W, c, on ? W : 0, rv_pack<T>(dg));
+          } else {
 #pragma unroll
-          for (int j = 0; j < N; ++j) acc_g[i][j] += dg[j];
+            for (int j = 0; j < N; ++j) acc_g[i][j] += dg[j];
+          }
         }
 #pragma unroll
         for (int j = 0; j < N; ++j) d[j] *= f[j];              // dp
         if (post) {
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            acc_p[i][j] += d[j] * y[j];
+            if (on) acc_p[i][j] += d[j] * y[j];
             d[j] = r * (d[j] * q[j] - y[j] * m2);
           }
         }
@@ -229,8 +233,9 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_bwd(const Resid
 #pragma unroll
         for (int j = 0; j < N; ++j) d[j] *= a.scale;
       }
-      if (a.dy) rv_store<T, VEC>(reinterpret_cast<T*>(a.dy) + row * W, c, W, rv_pack<T>(d));
+      if (a.dy) rv_store<T, VEC>(reinterpret_cast<T*>(a.dy) + row * W, c, on ? W : 0, rv_pack<T>(d));
     }
+    in.next(row + (long long)rv_stages(TPR, VPT) * step);
   }
   const long long at = (long long)blockIdx.x * W;
   if (a.part_w) rv_partial<T, TPR, VPT>(acc_w, a.part_w + at, W, scratch);
@@ -251,22 +256,33 @@ static bool residual_vec(const ResidualArgs& a, int size) {
 }
 
 template <typename T, bool FULL>
-static int residual_launch(const ResidualArgs& a, bool back, int blocks, cudaStream_t s) {
+static int residual_launch(const ResidualArgs& a, bool back, int& blocks, cudaStream_t s) {
   const int size = sizeof(T), nvec = (a.width + RowVec<T>::N - 1) / RowVec<T>::N;
   const bool vec = residual_vec(a, size);
-  const int team = rv_team(nvec, vec);
+  const int team = rv_team(nvec, vec, false);
 #define CM_RES(TPR, VPT, VEC)                                                                                                     \
   [&] {                                                                                                                           \
     constexpr int TB = rv_block<TPR>(), RPB = TB / TPR;                                                                           \
-    if (back) residual_norm_bwd<T, TPR, VPT, VEC, FULL><<<blocks, TB, 0, s>>>(a);                                                 \
-    else residual_norm_fwd<T, TPR, VPT, VEC, FULL><<<unsigned((a.rows + RPB - 1) / RPB), TB, 0, s>>>(a);                          \
+    if (back) {                                                                                                                   \
+      auto kern = residual_norm_bwd<T, TPR, VPT, VEC, FULL>;                                                                      \
+      constexpr int SLOT = VEC ? rv_stages(TPR, VPT) * VPT * TB * 16 : 0;                                                         \
+      static PerDevice configured;                                                                                                \
+      if (configured.first()) {                                                                                                   \
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SLOT * (FULL ? 5 : 3)) != cudaSuccess) return -2; \
+        configured.done();                                                                                                        \
+      }                                                                                                                           \
+      static int resident[6];                                                                                                     \
+      blocks = rv_blocks(kern, TB, SLOT * a.ring_ops, RPB, a.rows, 1, resident[a.ring_ops]);                                      \
+      kern<<<blocks, TB, SLOT * a.ring_ops, s>>>(a);                                                                              \
+    } else residual_norm_fwd<T, TPR, VPT, VEC, FULL><<<unsigned((a.rows + RPB - 1) / RPB), TB, 0, s>>>(a);                          \
     return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                                            \
   }()
   CM_ROW_TEAM(team, vec, CM_RES);
 #undef CM_RES
 }
 
-static int residual_any(const ResidualArgs& a, int dtype, bool back, int blocks, cudaStream_t s) {
+// `blocks`: out, the partial rows of a backward's column sums
+static int residual_any(const ResidualArgs& a, int dtype, bool back, int& blocks, cudaStream_t s) {
   const bool full = a.post || a.gate;
   switch (dtype) {
     case ROW_BF16: return full ? residual_launch<__nv_bfloat16, true>(a, back, blocks, s) : residual_launch<__nv_bfloat16, false>(a, back, blocks, s);
@@ -289,16 +305,12 @@ extern "C" int cm_residual_rmsnorm_fwd(const void* y, long long sy, const void* 
   ResidualArgs a{};
   a.y = y; a.sy = sy; a.res = res; a.sres = sres; a.w = w; a.post = post; a.gate = gate; a.gate_rows = gate_rows;
   a.n = n; a.h = h; a.rstd_y = rstd_y; a.rstd_h = rstd_h; a.rows = rows; a.width = width; a.scale = scale; a.eps = eps;
-  return residual_any(a, dtype, false, 0, s);
+  int blocks = 0;
+  return residual_any(a, dtype, false, blocks, s);
 }
 
-// Blocks of the backward kernel, and with that the partial rows of a column sum, for this many rows.
-extern "C" int cm_row_norm_parts(long long rows, int width, int dtype) {
-  const int n = dtype == ROW_FP32 ? 4 : 8, nvec = (width + n - 1) / n;
-  const long long threads = nvec <= 64 ? 128 : nvec <= 256 ? 128 : nvec <= 512 ? 256 : nvec <= 1024 ? 512 : 1024;
-  const long long most = (long long)sm_count() * (1024 / threads);
-  return int(rows < most ? (rows < 1 ? 1 : rows) : most);
-}
+// Partial rows of a column sum that the backward needs room for.
+extern "C" int cm_row_norm_parts(long long rows) { return int(rv_most_blocks(rows)); }
 
 // part: [3][cm_row_norm_parts][width] floats of work space.  dn, dh (gradients of n and h) may be null; dy null: it is dres (no post
 // norm, no gate, scale 1); dw, dpost, dgate (one per channel), dgate_rows may be null.
@@ -308,27 +320,28 @@ extern "C" int cm_residual_rmsnorm_bwd(const void* dn, long long sdn, const void
                                        void* dpost, void* dgate, float* part, long long rows, int width, float scale, int dtype,
                                        cudaStream_t s) {
   if (rows <= 0 || width <= 0) return 0;
-  const int blocks = cm_row_norm_parts(rows, width, dtype);
   ResidualArgs a{};
   a.dn = dn; a.sdn = sdn; a.dh = dh; a.sdh = sdh; a.h = const_cast<void*>(h); a.y = y; a.sy = sy; a.w = w; a.post = post; a.gate = gate;
   a.gate_rows = gate_rows; a.rstd_y = const_cast<float*>(rstd_y); a.rstd_h = const_cast<float*>(rstd_h); a.dres = dres; a.dy = dy;
   a.dgate_rows = dgate_rows; a.rows = rows; a.width = width; a.scale = scale;
+  a.ring_ops = !post && !gate ? 3 : gate && gate_rows ? 5 : 4;
   ColumnSums c{};
   int sums = 0;
   auto want = [&](void* out, float*& slot) {
     if (!out) return;
-    slot = part + (long long)sums * blocks * width;
+    slot = part + sums * rv_most_blocks(rows) * width;
     c.partial[sums] = slot;
     c.out[sums++] = out;
   };
   want(dw, a.part_w);
   want(dpost, a.part_post);
   want(dgate, a.part_gate);
+  int blocks = 0;
   const int rc = residual_any(a, dtype, true, blocks, s);
   if (rc || !sums) return rc;
   const dim3 grid((width + 31) / 32, sums);
-  if (dtype == ROW_BF16) rv_column_sum<__nv_bfloat16><<<grid, 256, 0, s>>>(c, blocks, width);
-  else if (dtype == ROW_FP16) rv_column_sum<__half><<<grid, 256, 0, s>>>(c, blocks, width);
-  else rv_column_sum<float><<<grid, 256, 0, s>>>(c, blocks, width);
+  if (dtype == ROW_BF16) rv_column_sum<__nv_bfloat16><<<grid, 1024, 0, s>>>(c, blocks, width);
+  else if (dtype == ROW_FP16) rv_column_sum<__half><<<grid, 1024, 0, s>>>(c, blocks, width);
+  else rv_column_sum<float><<<grid, 1024, 0, s>>>(c, blocks, width);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }

@@ -138,35 +138,118 @@ __device__ __forceinline__ void rv_partial(const float (&acc)[VPT][RowVec<T>::N]
   }
 }
 
-// out[c] = sum over p of partial[p][c], c < width, in a fixed order; blockIdx.y chooses one of up to three sums.
+// The operand rows of a backward kernel on their way in.  Every thread copies its own vectors of the next NS rows into shared memory
+// with asynchronous copies and reads back only what it copied, so the copies need no barrier and keep running over the barriers of the
+// rows' sums; read back twice (before and after a row's sum) they take no registers in between.  NS = 0, and rows that are not on 16
+// bytes: plain loads, twice.
+template <typename T, int TPR, int VPT, bool VEC, int NS, int OPS>
+struct RowRing {
+  static constexpr bool ON = VEC && NS > 0;
+  static constexpr int TB = rv_block<TPR>(), N = RowVec<T>::N;
+  uint4* ring;               // [NS][ops][VPT][TB]
+  const T* base[OPS];        // null: zero
+  long long pitch[OPS];
+  int ops, width;
+  long long rows;
+  int slot = 0;
+  long long row = 0;
+
+  __device__ __forceinline__ uint4* at(int op, int i) const { return ring + ((slot * ops + op) * VPT + i) * TB + threadIdx.x; }
+  // start the copies of row `r` into the current slot (an empty group past the last row)
+  __device__ __forceinline__ void request(long long r) {
+    if constexpr (ON) {
+#pragma unroll
+      for (int op = 0; op < OPS; ++op) {
+        if (op < ops && base[op] && r < rows) {
+          const T* src = base[op] + r * pitch[op];
+#pragma unroll
+          for (int i = 0; i < VPT; ++i) {
+            const int c = int(threadIdx.x) % TPR + i * TPR;
+            if (c * N < width)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(at(op, i))), "l"(src + c * N) : "memory");
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  }
+  __device__ __forceinline__ void start(long long first, long long step) {
+    if constexpr (ON) {
+      for (int s = 0; s < NS; ++s) {
+        request(first + s * step);
+        slot = slot + 1 == NS ? 0 : slot + 1;
+      }
+    }
+  }
+  __device__ __forceinline__ void wait(long long r) {
+    row = r;
+    if constexpr (ON) asm volatile("cp.async.wait_group %0;" ::"n"(NS > 0 ? NS - 1 : 0) : "memory");
+  }
+  __device__ __forceinline__ uint4 get(int op, int i) const {
+    const int c = int(threadIdx.x) % TPR + i * TPR;
+    if constexpr (ON) return base[op] && row < rows && c * N < width ? *at(op, i) : make_uint4(0, 0, 0, 0);
+    else return rv_load<T, VEC>(base[op] + row * pitch[op], c, base[op] && row < rows ? width : 0);
+  }
+  __device__ __forceinline__ void next(long long ahead) {
+    if constexpr (ON) {
+      request(ahead);
+      slot = slot + 1 == NS ? 0 : slot + 1;
+    }
+  }
+};
+
+// Rows ahead of a backward kernel, by the vectors that a block holds of one operand.
+constexpr int rv_stages(int tpr, int vpt) {
+  const int held = (tpr < 128 ? 128 : tpr) * vpt;
+  return held <= 256 ? 4 : held <= 512 ? 3 : held <= 1024 ? 2 : 0;
+}
+// Blocks of a backward kernel: those that an SM holds at once, at most RV_BLOCKS_PER_SM, each with a row at least.
+constexpr int RV_BLOCKS_PER_SM = 4;
+static inline long long rv_most_blocks(long long rows) {
+  const long long most = (long long)sm_count() * RV_BLOCKS_PER_SM;
+  return rows < most ? rows : most;
+}
+// `resident`: answers of the runtime, by operands in the ring, for one kernel (0: not asked yet)
+template <typename K>
+static int rv_blocks(K kern, int threads, int smem, int rows_per_block, long long rows, int share, int& resident) {
+  if (resident == 0) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess || n < 1) n = 1;
+    resident = n < RV_BLOCKS_PER_SM ? n : RV_BLOCKS_PER_SM;
+  }
+  const long long want = (rows + rows_per_block - 1) / rows_per_block, most = ((long long)sm_count() * resident + share - 1) / share;
+  return int(want < most ? want : most);
+}
+
+// out[c] = sum over p of partial[p][c], c < width, in a fixed order; blockIdx.y chooses one of up to three sums.  32 threads share a
+// column: with 8, and one load in flight each, 592 partial rows of 4096 took 16 us.
 struct ColumnSums {
   const float* partial[3];
   void* out[3];
 };
 
 template <typename T>
-__global__ void __launch_bounds__(256) rv_column_sum(const ColumnSums s, int parts, int width) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) rv_column_sum(const ColumnSums s, int parts, int width) {
+  __shared__ float red[32][33];
   const float* __restrict__ in = s.partial[blockIdx.y];
   T* out = reinterpret_cast<T*>(s.out[blockIdx.y]);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float a = 0.f;
-  if (c < width)
-    for (int p = w; p < parts; p += 8) a += in[(long long)p * width + c];
+  if (c < width) {
+#pragma unroll 8
+    for (int p = w; p < parts; p += 32) a += in[(long long)p * width + c];
+  }
   red[w][lane] = a;
   __syncthreads();
-  if (w == 0 && c < width) {
-    float t = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) t += red[k][lane];
-    out[c] = T(t);
-  }
+  const float t = warp_sum(red[lane][w]);
+  if (lane == 0 && blockIdx.x * 32 + w < width) out[blockIdx.x * 32 + w] = T(t);
 }
 
 enum RowType : int { ROW_BF16 = 0, ROW_FP16 = 1, ROW_FP32 = 2 };
 
-// The team of a row of `nvec` vectors, as 16 * threads + vectors a thread; 0: too wide.
-static inline int rv_team(int nvec, bool vec) {
+// The team of a row of `nvec` vectors, as 16 * threads + vectors a thread; 0: too wide.  `by_warp`: up to 128 vectors go to one warp.
+static inline int rv_team(int nvec, bool vec, bool by_warp) {
+  if (vec && by_warp && nvec > 64 && nvec <= 128) return 16 * 32 + 4;
   if (!vec) return nvec <= 64 ? 16 * 32 + 2 : nvec <= 256 ? 16 * 128 + 2 : nvec <= 1024 ? 16 * 512 + 2 : nvec <= 4096 ? 16 * 1024 + 4 : 0;
   return nvec <= 8 ? 16 * 8 + 1 : nvec <= 32 ? 16 * 32 + 1 : nvec <= 64 ? 16 * 32 + 2 : nvec <= 128 ? 16 * 128 + 1
          : nvec <= 256 ? 16 * 128 + 2 : nvec <= 512 ? 16 * 256 + 2 : nvec <= 1024 ? 16 * 512 + 2 : nvec <= 2048 ? 16 * 1024 + 2
@@ -180,6 +263,7 @@ static inline int rv_team(int nvec, bool vec) {
       case 16 * 8 + 1: return F(8, 1, true);                                                                        \
       case 16 * 32 + 1: return F(32, 1, true);                                                                      \
       case 16 * 32 + 2: return F(32, 2, true);                                                                      \
+      case 16 * 32 + 4: return F(32, 4, true);                                                                      \
       case 16 * 128 + 1: return F(128, 1, true);                                                                    \
       case 16 * 128 + 2: return F(128, 2, true);                                                                    \
       case 16 * 256 + 2: return F(256, 2, true);                                                                    \

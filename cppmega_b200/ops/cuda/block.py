@@ -22,14 +22,13 @@ MAX_WIDTH = 16384          # widest normalised row
 def declare(L: ctypes.CDLL) -> None:
     vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
     sig = {
-        "cm_gated_mlp_fwd": [vp, i64, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp],
+        "cm_gated_mlp_fwd": [vp, i64, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp],
         "cm_gated_mlp_bwd": [vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp],
         "cm_residual_rmsnorm_fwd": [vp, i64, vp, i64, vp, vp, vp, i32, vp, vp, vp, vp, i64, i32, f32, f32, i32, vp],
-        "cm_row_norm_parts": [i64, i32, i32],
+        "cm_row_norm_parts": [i64],
         "cm_residual_rmsnorm_bwd": [vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, f32,
                                     i32, vp],
         "cm_rmsnorm_gated_fwd": [vp, i64, vp, i64, vp, vp, vp, i64, i32, i32, i32, f32, i32, vp],
-        "cm_rmsnorm_gated_parts": [i64, i32, i32, i32],
         "cm_rmsnorm_gated_bwd": [vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, vp],
     }
     for name, args in sig.items():
@@ -37,6 +36,8 @@ def declare(L: ctypes.CDLL) -> None:
         if fn is not None:
             fn.argtypes = args
             fn.restype = i32
+    if hasattr(L, "cm_gated_mlp_fwd_ws"):
+        L.cm_gated_mlp_fwd_ws.argtypes, L.cm_gated_mlp_fwd_ws.restype = [i32, i32, i32, i32], i64
 
 
 def _lib():
@@ -114,8 +115,10 @@ def _mlp_forward(x, w1, w2, act, keep):
     y = torch.empty(*x.shape[:-1], Ho, dtype=x.dtype, device=x.device)
     h = torch.empty(M, F, dtype=x.dtype, device=x.device)
     gu = torch.empty(M, 2 * F, dtype=x.dtype, device=x.device) if keep else None
-    _call("cm_gated_mlp_fwd", x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), _ptr(gu), h.data_ptr(), y.data_ptr(), M, H, F, Ho, act,
-          err_word(x.device).data_ptr(), _stream())
+    floats = _lib().cm_gated_mlp_fwd_ws(M, H, F, Ho)
+    ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
+    _call("cm_gated_mlp_fwd", x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), _ptr(gu), h.data_ptr(), y.data_ptr(), _ptr(ws), M, H, F, Ho,
+          act, err_word(x.device).data_ptr(), _stream())
     F_.count_launch("gated_mlp")
     return y, x, gu, h
 
@@ -224,7 +227,7 @@ class ResidualRMSNormFn(torch.autograd.Function):
         sums = [torch.empty(W, dtype=dt, device=dev) if need else None for need in (need_w, need_post, need_gate and not per_row)]
         wanted = sum(t is not None for t in sums)
         dtype = ROW_TYPES[dt]
-        part = torch.empty(wanted * _lib().cm_row_norm_parts(R, W, dtype) * W, dtype=torch.float32, device=dev) if wanted else None
+        part = torch.empty(wanted * _lib().cm_row_norm_parts(R) * W, dtype=torch.float32, device=dev) if wanted else None
         _call("cm_residual_rmsnorm_bwd", _ptr(dn), sdn, _ptr(dh), sdh, h.data_ptr(), _ptr(y), sy, weight.data_ptr(), _ptr(post), _ptr(gate),
               int(per_row), stats.data_ptr(), stats[1].data_ptr(), dres.data_ptr(), _ptr(dy), _ptr(dgate_rows), *map(_ptr, sums), _ptr(part),
               R, W, ctx.scale, dtype, _stream())
@@ -292,7 +295,7 @@ class GatedRMSNormFn(torch.autograd.Function):
         dtype = ROW_TYPES[dt]
         if need_w:
             dw = torch.empty(W, dtype=dt, device=dev)
-            part = torch.empty(_lib().cm_rmsnorm_gated_parts(R, W, ctx.group, dtype) * W, dtype=torch.float32, device=dev)
+            part = torch.empty(_lib().cm_row_norm_parts(R) * W, dtype=torch.float32, device=dev)
         _call("cm_rmsnorm_gated_bwd", x.data_ptr(), sx, _ptr(z), sz, weight.data_ptr(), dy.data_ptr(), sdy, rstd.data_ptr(), dx.data_ptr(),
               _ptr(dz), _ptr(dw), _ptr(part), R, W, ctx.group, int(ctx.gate_first), dtype, _stream())
         F_.count_launch("rmsnorm_gated_bwd")

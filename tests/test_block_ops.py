@@ -93,10 +93,10 @@ def test_kernel_entry_points_refuse():
     """Argument checks of the C entries; nothing is launched."""
     from cppmega_b200.ops.cuda import lib
     L = lib()
-    assert L.cm_gated_mlp_fwd(16, 12, 16, 16, None, 16, 16, 4, 12, 8, 8, 0, None, None) == -10        # width of 12
-    assert L.cm_gated_mlp_fwd(8, 16, 16, 16, None, 16, 16, 4, 16, 8, 8, 0, None, None) == -10         # base not on 16 bytes
-    assert L.cm_gated_mlp_fwd(16, 12, 16, 16, None, 16, 16, 4, 8, 8, 8, 0, None, None) == -10         # row pitch of 12
-    assert L.cm_gated_mlp_fwd(16, 16, 16, 16, None, 16, 16, 0, 16, 8, 8, 0, None, None) == 0          # no tokens
+    assert L.cm_gated_mlp_fwd(16, 12, 16, 16, None, 16, 16, 16, 4, 12, 8, 8, 0, None, None) == -10        # width of 12
+    assert L.cm_gated_mlp_fwd(8, 16, 16, 16, None, 16, 16, 16, 4, 16, 8, 8, 0, None, None) == -10         # base not on 16 bytes
+    assert L.cm_gated_mlp_fwd(16, 12, 16, 16, None, 16, 16, 16, 4, 8, 8, 8, 0, None, None) == -10         # row pitch of 12
+    assert L.cm_gated_mlp_fwd(16, 16, 16, 16, None, 16, 16, 16, 0, 16, 8, 8, 0, None, None) == 0          # no tokens
     assert L.cm_residual_rmsnorm_fwd(16, 8, 16, 8, 16, None, None, 0, 16, 16, None, None, 2, 8, 1.0, 1e-5, 3, None) == -10     # no such type
     assert L.cm_residual_rmsnorm_fwd(16, 8, 16, 8, 16, None, None, 0, 16, 16, None, None, 2, 40000, 1.0, 1e-5, 0, None) == -10  # too wide
     assert L.cm_rmsnorm_gated_fwd(16, 8, None, 0, 16, 16, None, 2, 8, 3, 0, 1e-5, 0, None) == -10     # groups that do not divide
