@@ -23,7 +23,12 @@ struct GatedArgs {
   int gate_first;
 };
 
-__device__ __forceinline__ float sigmoid_of(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+// 1 / (1 + inf) is 0, as it should be
+__device__ __forceinline__ float sigmoid_of(float z) {
+  float q;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + __expf(-z)));
+  return q;
+}
 
 template <typename T, int TPR, int VPT, bool VEC>
 __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArgs a) {
@@ -72,7 +77,10 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArg
   }
 }
 
-template <typename T, int TPR, int VPT, bool VEC>
+// What depends on the row's mean waits in registers for it (the normalised value, dn w, and with the gate first the gate and x a'(z)):
+// computed twice, the two transcendentals of every element made this kernel instruction bound (433 us at 16384 x 8192 in groups of
+// 1024).  The gradient of a gate behind the norm does not depend on the mean and leaves before it.
+template <typename T, int TPR, int VPT, bool VEC, bool GATE_FIRST>
 __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArgs a) {
   constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
   extern __shared__ __align__(16) uint4 dyn[];
@@ -80,6 +88,8 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
   __shared__ float scratch[RPB > 1 ? RPB * TPR * VPT * N : 1];
   enum { XX = 0, DY = 1, ZZ = 2 };
   const int t = threadIdx.x % TPR, g0 = blockIdx.y * a.group;
+  const bool has_z = a.z != nullptr;
+  const float inv_group = 1.f / a.group;
   float acc[VPT][N] = {};
   RowRing<T, TPR, VPT, VEC, rv_stages(TPR, VPT), 3> in;
   in.ring = dyn;
@@ -88,12 +98,15 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
   in.rows = a.rows;
   in.base[XX] = reinterpret_cast<const T*>(a.x) + g0;
   in.base[DY] = reinterpret_cast<const T*>(a.dy) + g0;
-  in.base[ZZ] = a.z ? reinterpret_cast<const T*>(a.z) + g0 : nullptr;
+  in.base[ZZ] = has_z ? reinterpret_cast<const T*>(a.z) + g0 : nullptr;
   in.pitch[XX] = a.sx;
   in.pitch[DY] = a.sdy;
   in.pitch[ZZ] = a.sz;
   const long long step = (long long)gridDim.x * RPB;
   in.start((long long)blockIdx.x * RPB + threadIdx.x / TPR, step);
+  uint4 wv[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) wv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, t + i * TPR, a.group);
   int turn = 0;
   for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += step, turn ^= 1) {
     const long long row = row0 + threadIdx.x / TPR;
@@ -101,48 +114,57 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
     const float r = G ? a.rstd[row * gridDim.y + blockIdx.y] : 0.f;
     in.wait(row);
     float s[1] = {0.f};
+    float hat[VPT][N], dnw[VPT][N], gate[GATE_FIRST ? VPT : 1][N], xs[GATE_FIRST ? VPT : 1][N];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       float x[N], z[N], d[N], w[N];
       rv_unpack<T>(in.get(XX, i), x);
       rv_unpack<T>(in.get(ZZ, i), z);
       rv_unpack<T>(in.get(DY, i), d);
-      rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, t + i * TPR, G), w);
+      rv_unpack<T>(wv[i], w);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float gate = a.z ? z[j] * sigmoid_of(z[j]) : 1.f;
-        const float hat = (a.gate_first ? x[j] * gate : x[j]) * r, dn = a.gate_first ? d[j] : d[j] * gate;
-        acc[i][j] += dn * hat;
-        s[0] += dn * w[j] * hat;
+        const float q = sigmoid_of(z[j]), g = has_z ? z[j] * q : 1.f, slope = q + z[j] * q * (1.f - q);
+        if constexpr (GATE_FIRST) {
+          gate[i][j] = g;
+          xs[i][j] = x[j] * slope;
+          hat[i][j] = x[j] * g * r;
+          dnw[i][j] = d[j] * w[j];
+          acc[i][j] += d[j] * hat[i][j];
+        } else {
+          hat[i][j] = x[j] * r;
+          const float dh = d[j] * hat[i][j];
+          acc[i][j] += dh * g;
+          dnw[i][j] = d[j] * g * w[j];
+          z[j] = dh * w[j] * slope;
+        }
+        s[0] += dnw[i][j] * hat[i][j];
       }
+      if constexpr (!GATE_FIRST)
+        if (a.dz) rv_store<T, VEC>(reinterpret_cast<T*>(a.dz) + row * a.width + g0, t + i * TPR, G, rv_pack<T>(z));
     }
+    in.next(row + (long long)rv_stages(TPR, VPT) * step);
     rv_team_sum<TPR, 1>(s, red, turn);
-    const float m = s[0] / a.group;
+    const float m = s[0] * inv_group;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * TPR;
-      float x[N], z[N], d[N], w[N];
-      rv_unpack<T>(in.get(XX, i), x);
-      rv_unpack<T>(in.get(ZZ, i), z);
-      rv_unpack<T>(in.get(DY, i), d);
-      rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, c, G), w);
+      float x[N];
+      if constexpr (GATE_FIRST) {
+        float z[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float q = sigmoid_of(z[j]), gate = a.z ? z[j] * q : 1.f, slope = q * (1.f + z[j] * (1.f - q));
-        if (a.gate_first) {
-          const float du = r * (d[j] * w[j] - x[j] * gate * r * m);
-          z[j] = du * x[j] * slope;
-          x[j] = du * gate;
-        } else {
-          const float hat = x[j] * r;
-          z[j] = d[j] * hat * w[j] * slope;
-          x[j] = r * (d[j] * gate * w[j] - hat * m);
+        for (int j = 0; j < N; ++j) {
+          const float du = r * (dnw[i][j] - hat[i][j] * m);
+          x[j] = du * gate[i][j];
+          z[j] = du * xs[i][j];
         }
+        if (a.dz) rv_store<T, VEC>(reinterpret_cast<T*>(a.dz) + row * a.width + g0, c, G, rv_pack<T>(z));
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = r * (dnw[i][j] - hat[i][j] * m);
       }
       rv_store<T, VEC>(reinterpret_cast<T*>(a.dx) + row * a.width + g0, c, G, rv_pack<T>(x));
-      if (a.dz) rv_store<T, VEC>(reinterpret_cast<T*>(a.dz) + row * a.width + g0, c, G, rv_pack<T>(z));
     }
-    in.next(row + (long long)rv_stages(TPR, VPT) * step);
   }
   if (a.part) rv_partial<T, TPR, VPT>(acc, a.part + (long long)blockIdx.x * a.width + g0, a.group, scratch);
 }
@@ -153,20 +175,20 @@ static int gated_launch(const GatedArgs& a, bool back, int& blocks, cudaStream_t
   auto fits = [&](const void* p, long long pitch) { return !p || ((reinterpret_cast<uintptr_t>(p) | (pitch * size)) & 15) == 0; };
   const bool vec = a.group * size % 16 == 0 && fits(a.x, a.sx) && fits(a.z, a.sz) && fits(a.w, 0) && fits(a.dy, a.sdy) &&
                    fits(a.y, a.width) && fits(a.dx, a.width) && fits(a.dz, a.width);
-  const int team = rv_team(nvec, vec, true);
+  const int team = rv_team(nvec, vec, !back);
 #define CM_GATED(TPR, VPT, VEC)                                                                                                  \
   [&] {                                                                                                                          \
     constexpr int TB = rv_block<TPR>(), RPB = TB / TPR;                                                                          \
     if (back) {                                                                                                                  \
-      auto kern = gated_norm_bwd<T, TPR, VPT, VEC>;                                                                              \
+      auto kern = a.gate_first ? gated_norm_bwd<T, TPR, VPT, VEC, true> : gated_norm_bwd<T, TPR, VPT, VEC, false>;               \
       constexpr int RING = VEC ? rv_stages(TPR, VPT) * VPT * TB * 16 * 3 : 0;                                                    \
-      static PerDevice configured;                                                                                               \
-      if (configured.first()) {                                                                                                  \
+      static PerDevice configured[2];                                                                                            \
+      if (configured[a.gate_first].first()) {                                                                                    \
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING) != cudaSuccess) return -2;             \
-        configured.done();                                                                                                       \
+        configured[a.gate_first].done();                                                                                         \
       }                                                                                                                          \
-      static int resident;                                                                                                       \
-      blocks = rv_blocks(kern, TB, RING, RPB, a.rows, groups, resident);                                                         \
+      static int resident[2];                                                                                                    \
+      blocks = rv_blocks(kern, TB, RING, RPB, a.rows, groups, resident[a.gate_first]);                                                         \
       kern<<<dim3(blocks, groups), TB, RING, s>>>(a);                                                                            \
     } else gated_norm_fwd<T, TPR, VPT, VEC><<<dim3(unsigned((a.rows + RPB - 1) / RPB), groups), TB, 0, s>>>(a);                    \
     return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                                           \
@@ -196,7 +218,7 @@ extern "C" int cm_rmsnorm_gated_fwd(const void* x, long long sx, const void* z, 
   if (rows <= 0 || width <= 0) return 0;
   GatedArgs a{};
   a.x = x; a.sx = sx; a.z = z; a.sz = sz; a.w = w; a.y = y; a.rstd = rstd; a.rows = rows; a.width = width; a.group = group;
-  a.gate_first = gate_first; a.eps = eps;
+  a.gate_first = gate_first != 0; a.eps = eps;
   int blocks = 0;
   return gated_any(a, dtype, false, blocks, s);
 }
@@ -208,7 +230,7 @@ extern "C" int cm_rmsnorm_gated_bwd(const void* x, long long sx, const void* z, 
   if (rows <= 0 || width <= 0) return 0;
   GatedArgs a{};
   a.x = x; a.sx = sx; a.z = z; a.sz = sz; a.w = w; a.dy = dy; a.sdy = sdy; a.rstd = const_cast<float*>(rstd); a.dx = dx; a.dz = dz;
-  a.part = dw ? part : nullptr; a.rows = rows; a.width = width; a.group = group; a.gate_first = gate_first;
+  a.part = dw ? part : nullptr; a.rows = rows; a.width = width; a.group = group; a.gate_first = gate_first != 0;
   int blocks = 0;
   const int rc = gated_any(a, dtype, true, blocks, s);
   if (rc || !dw) return rc;

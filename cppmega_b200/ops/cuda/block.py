@@ -12,6 +12,7 @@ import ctypes
 import torch
 from torch.autograd.function import once_differentiable
 
+from .. import cuda as _cu
 from .. import functional as F_
 
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1, "relu": 2}
@@ -40,21 +41,8 @@ def declare(L: ctypes.CDLL) -> None:
         L.cm_gated_mlp_fwd_ws.argtypes, L.cm_gated_mlp_fwd_ws.restype = [i32, i32, i32, i32], i64
 
 
-def _lib():
-    from . import lib
-    return lib()
-
-
-def _stream() -> int:
-    from . import stream_ptr
-    return stream_ptr()
-
-
-def _call(name: str, *args) -> None:
-    rc = getattr(_lib(), name)(*args)
-    if rc:
-        from . import KernelError
-        raise KernelError(f"{name} failed with code {rc}")
+def _failed(name: str, rc: int) -> None:
+    raise _cu.KernelError(f"{name} failed with code {rc}")
 
 
 def _ptr(t):
@@ -69,7 +57,6 @@ def _device_of(t: torch.Tensor):
 def _rows(t: torch.Tensor):
     """``(tensor, elements between rows)`` of the [rows, width] view of a tensor whose rows are contiguous and evenly spaced; any
     other tensor is copied."""
-    from . import fast_contiguous
     if t.is_contiguous():
         return t, t.shape[-1]
     if t.stride(-1) == 1 or t.shape[-1] == 1:
@@ -87,11 +74,12 @@ def _rows(t: torch.Tensor):
             return t, t.shape[-1]
         if pitch >= t.shape[-1]:
             return t, pitch
-    return fast_contiguous(t), t.shape[-1]
+    return _cu.fast_contiguous(t), t.shape[-1]
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A packed tensor of the same shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 # ---------------------------------------------------------------------------
@@ -108,17 +96,19 @@ def _tma_rows(t: torch.Tensor):
 
 
 def _mlp_forward(x, w1, w2, act, keep):
-    from . import err_word
+    L = _cu.lib()
     x, ldx = _tma_rows(x)
     H, F, Ho = w1.shape[1], w2.shape[1], w2.shape[0]
     M = x.numel() // H
-    y = torch.empty(*x.shape[:-1], Ho, dtype=x.dtype, device=x.device)
-    h = torch.empty(M, F, dtype=x.dtype, device=x.device)
-    gu = torch.empty(M, 2 * F, dtype=x.dtype, device=x.device) if keep else None
-    floats = _lib().cm_gated_mlp_fwd_ws(M, H, F, Ho)
+    y = _like(x) if Ho == H else x.new_empty(*x.shape[:-1], Ho)
+    h = x.new_empty(M, F)
+    gu = x.new_empty(M, 2 * F) if keep else None
+    floats = L.cm_gated_mlp_fwd_ws(M, H, F, Ho)
     ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
-    _call("cm_gated_mlp_fwd", x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), _ptr(gu), h.data_ptr(), y.data_ptr(), _ptr(ws), M, H, F, Ho,
-          act, err_word(x.device).data_ptr(), _stream())
+    rc = L.cm_gated_mlp_fwd(x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), _ptr(gu), h.data_ptr(), y.data_ptr(), _ptr(ws), M, H, F, Ho,
+                            act, _cu.err_word(x.device).data_ptr(), _cu.stream_ptr())
+    if rc:
+        _failed("cm_gated_mlp_fwd", rc)
     F_.count_launch("gated_mlp")
     return y, x, gu, h
 
@@ -134,29 +124,29 @@ class GatedMLPFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        from . import err_word, wgrad_into_main_grad
         x, w1, w2, gu, h = ctx.saved_tensors
         need_x, need_w1, need_w2, _ = ctx.needs_input_grad
         H, F, Ho = w1.shape[1], w2.shape[1], w2.shape[0]
-        M = h.shape[0]
         dy, lddy = _tma_rows(dy)
         x, ldx = _tma_rows(x)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        into = {1: (None, 0, 0), 2: (None, 0, 0)}                  # (result, its type, added to what is there) per weight
+        dx = _like(x) if need_x else None
+        into = [(None, 0, 0), (None, 0, 0)]                        # (result, fp32, added to what is there) of each weight
 
         def target(i, w):
             def run(out, acc):
                 t = torch.empty_like(w) if out is None else out
-                into[i] = (t, int(t.dtype == torch.float32), int(acc))
+                into[i] = (t.data_ptr(), int(t.dtype == torch.float32), int(acc))
                 return t
             return run
 
-        dw1 = wgrad_into_main_grad(w1, target(1, w1)) if need_w1 else None
-        dw2 = wgrad_into_main_grad(w2, target(2, w2)) if need_w2 else None
+        dw1 = _cu.wgrad_into_main_grad(w1, target(0, w1)) if need_w1 else None
+        dw2 = _cu.wgrad_into_main_grad(w2, target(1, w2)) if need_w2 else None
         dgu = torch.empty_like(gu) if need_x or need_w1 else None
-        (t1, f1, a1), (t2, f2, a2) = into[1], into[2]
-        _call("cm_gated_mlp_bwd", dy.data_ptr(), lddy, x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), gu.data_ptr(), h.data_ptr(),
-              _ptr(dgu), _ptr(dx), _ptr(t1), f1, a1, _ptr(t2), f2, a2, M, H, F, Ho, ctx.act, err_word(x.device).data_ptr(), _stream())
+        rc = _cu.lib().cm_gated_mlp_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), gu.data_ptr(), h.data_ptr(),
+                                        _ptr(dgu), _ptr(dx), *into[0], *into[1], h.shape[0], H, F, Ho, ctx.act,
+                                        _cu.err_word(x.device).data_ptr(), _cu.stream_ptr())
+        if rc:
+            _failed("cm_gated_mlp_bwd", rc)
         F_.count_launch("gated_mlp_bwd")
         return dx, dw1, dw2, None
 
@@ -168,7 +158,7 @@ def gated_mlp(x, w1, w2, activation):
             and w2.data_ptr() % 16 == 0 and x.numel() // x.shape[-1] < 2 ** 31):
         return None
     with _device_of(x):
-        if _wants_grad(x, w1, w2):
+        if torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad):
             return GatedMLPFn.apply(x, w1, w2, ACTIVATIONS[activation])
         return _mlp_forward(x, w1, w2, ACTIVATIONS[activation], keep=False)[0]
 
@@ -182,12 +172,14 @@ def _residual_forward(y, residual, weight, post, gate, scale, eps, keep):
     residual, sres = _rows(residual)
     W = y.shape[-1]
     R = y.numel() // W
-    n = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    h = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    stats = torch.empty(2, R, dtype=torch.float32, device=y.device) if keep else None
-    _call("cm_residual_rmsnorm_fwd", y.data_ptr(), sy, residual.data_ptr(), sres, weight.data_ptr(), _ptr(post), _ptr(gate),
-          int(gate is not None and gate.dim() > 1), n.data_ptr(), h.data_ptr(), _ptr(stats), None if stats is None else stats[1].data_ptr(),
-          R, W, scale, eps, ROW_TYPES[y.dtype], _stream())
+    n, h = _like(y), _like(y)
+    stats = torch.empty(2 * R, dtype=torch.float32, device=y.device) if keep else None         # 1 / rms of y, then of h
+    at = stats.data_ptr() if keep else None
+    rc = _cu.lib().cm_residual_rmsnorm_fwd(y.data_ptr(), sy, residual.data_ptr(), sres, weight.data_ptr(), _ptr(post), _ptr(gate),
+                                           int(gate is not None and gate.dim() > 1), n.data_ptr(), h.data_ptr(), at,
+                                           at + 4 * R if keep else None, R, W, scale, eps, ROW_TYPES[y.dtype], _cu.stream_ptr())
+    if rc:
+        _failed("cm_residual_rmsnorm_fwd", rc)
     F_.count_launch("residual_rmsnorm")
     return n, h, y, stats
 
@@ -211,7 +203,6 @@ class ResidualRMSNormFn(torch.autograd.Function):
         need_y, _, need_w, need_post, need_gate = ctx.needs_input_grad[:5]
         W = h.shape[-1]
         R = h.numel() // W
-        dt, dev = h.dtype, h.device
         sy = sdn = sdh = 0
         if y is not None:
             y, sy = _rows(y)
@@ -220,32 +211,40 @@ class ResidualRMSNormFn(torch.autograd.Function):
         if dh is not None:
             dh, sdh = _rows(dh)
         per_row = gate is not None and gate.dim() > 1
-        dres = torch.empty(h.shape, dtype=dt, device=dev)
         same = y is None and ctx.scale == 1.0
-        dy = torch.empty(h.shape, dtype=dt, device=dev) if need_y and not same else None
-        dgate_rows = torch.empty(h.shape, dtype=dt, device=dev) if need_gate and per_row else None
-        sums = [torch.empty(W, dtype=dt, device=dev) if need else None for need in (need_w, need_post, need_gate and not per_row)]
-        wanted = sum(t is not None for t in sums)
-        dtype = ROW_TYPES[dt]
-        part = torch.empty(wanted * _lib().cm_row_norm_parts(R) * W, dtype=torch.float32, device=dev) if wanted else None
-        _call("cm_residual_rmsnorm_bwd", _ptr(dn), sdn, _ptr(dh), sdh, h.data_ptr(), _ptr(y), sy, weight.data_ptr(), _ptr(post), _ptr(gate),
-              int(per_row), stats.data_ptr(), stats[1].data_ptr(), dres.data_ptr(), _ptr(dy), _ptr(dgate_rows), *map(_ptr, sums), _ptr(part),
-              R, W, ctx.scale, dtype, _stream())
+        dres = torch.empty_like(h)
+        dy = torch.empty_like(h) if need_y and not same else None
+        dgate = torch.empty_like(gate) if need_gate else None
+        dw = torch.empty_like(weight) if need_w else None
+        dpost = torch.empty_like(post) if need_post else None
+        sums = need_w + need_post + (need_gate and not per_row)
+        L = _cu.lib()
+        part = torch.empty(sums * L.cm_row_norm_parts(R) * W, dtype=torch.float32, device=h.device) if sums else None
+        at = stats.data_ptr()
+        rc = L.cm_residual_rmsnorm_bwd(_ptr(dn), sdn, _ptr(dh), sdh, h.data_ptr(), _ptr(y), sy, weight.data_ptr(), _ptr(post), _ptr(gate),
+                                       int(per_row), at, at + 4 * R, dres.data_ptr(), _ptr(dy), _ptr(dgate) if per_row else None, _ptr(dw),
+                                       _ptr(dpost), None if per_row else _ptr(dgate), _ptr(part), R, W, ctx.scale, ROW_TYPES[h.dtype],
+                                       _cu.stream_ptr())
+        if rc:
+            _failed("cm_residual_rmsnorm_bwd", rc)
         F_.count_launch("residual_rmsnorm_bwd")
-        dw, dpost, dgate = sums
-        return (dres if same else dy), dres, dw, dpost, (dgate_rows if per_row else dgate), None, None
+        return (dres if same else dy), dres, dw, dpost, dgate, None, None
 
 
 def residual_rmsnorm(y, residual, weight, post_weight, gate, scale, eps):
     """None where the kernels do not apply: one type for all tensors (bf16, fp16 or fp32), rows of at most 16384."""
-    every = [t for t in (y, residual, weight, post_weight, gate) if t is not None]
-    if y.dtype not in ROW_TYPES or any(t.dtype != y.dtype for t in every) or y.shape[-1] > MAX_WIDTH or y.numel() == 0:
+    dt = y.dtype
+    if (dt not in ROW_TYPES or residual.dtype != dt or weight.dtype != dt or (post_weight is not None and post_weight.dtype != dt)
+            or (gate is not None and gate.dtype != dt) or y.shape[-1] > MAX_WIDTH or y.numel() == 0):
         return None
     weight = weight.contiguous()
-    post_weight = None if post_weight is None else post_weight.contiguous()
-    gate = None if gate is None else gate.contiguous()
+    if post_weight is not None:
+        post_weight = post_weight.contiguous()
+    if gate is not None:
+        gate = gate.contiguous()
     with _device_of(y):
-        if _wants_grad(*every):
+        if torch.is_grad_enabled() and (y.requires_grad or residual.requires_grad or weight.requires_grad
+                                        or (post_weight is not None and post_weight.requires_grad) or (gate is not None and gate.requires_grad)):
             return ResidualRMSNormFn.apply(y, residual, weight, post_weight, gate, float(scale), float(eps))
         return _residual_forward(y, residual, weight, post_weight, gate, float(scale), float(eps), keep=False)[:2]
 
@@ -261,10 +260,12 @@ def _gated_forward(x, weight, z, eps, group, gate_first, keep):
         z, sz = _rows(z)
     W = x.shape[-1]
     R = x.numel() // W
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _like(x)
     rstd = torch.empty(R * (W // group), dtype=torch.float32, device=x.device) if keep else None
-    _call("cm_rmsnorm_gated_fwd", x.data_ptr(), sx, _ptr(z), sz, weight.data_ptr(), y.data_ptr(), _ptr(rstd), R, W, group, int(gate_first),
-          eps, ROW_TYPES[x.dtype], _stream())
+    rc = _cu.lib().cm_rmsnorm_gated_fwd(x.data_ptr(), sx, _ptr(z), sz, weight.data_ptr(), y.data_ptr(), _ptr(rstd), R, W, group,
+                                        int(gate_first), eps, ROW_TYPES[x.dtype], _cu.stream_ptr())
+    if rc:
+        _failed("cm_rmsnorm_gated_fwd", rc)
     F_.count_launch("rmsnorm_gated")
     return y, x, z, rstd
 
@@ -282,22 +283,25 @@ class GatedRMSNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, z, rstd = ctx.saved_tensors
         _, need_w, need_z = ctx.needs_input_grad[:3]
-        W, dt, dev = x.shape[-1], x.dtype, x.device
+        W = x.shape[-1]
         R = x.numel() // W
         x, sx = _rows(x)
         dy, sdy = _rows(dy)
         sz = 0
         if z is not None:
             z, sz = _rows(z)
-        dx = torch.empty(x.shape, dtype=dt, device=dev)
-        dz = torch.empty(x.shape, dtype=dt, device=dev) if need_z else None
+        dx = _like(x)
+        dz = torch.empty_like(dx) if need_z else None
         dw = part = None
-        dtype = ROW_TYPES[dt]
+        L = _cu.lib()
         if need_w:
-            dw = torch.empty(W, dtype=dt, device=dev)
-            part = torch.empty(_lib().cm_row_norm_parts(R) * W, dtype=torch.float32, device=dev)
-        _call("cm_rmsnorm_gated_bwd", x.data_ptr(), sx, _ptr(z), sz, weight.data_ptr(), dy.data_ptr(), sdy, rstd.data_ptr(), dx.data_ptr(),
-              _ptr(dz), _ptr(dw), _ptr(part), R, W, ctx.group, int(ctx.gate_first), dtype, _stream())
+            dw = torch.empty_like(weight)
+            part = torch.empty(L.cm_row_norm_parts(R) * W, dtype=torch.float32, device=x.device)
+        rc = L.cm_rmsnorm_gated_bwd(x.data_ptr(), sx, _ptr(z), sz, weight.data_ptr(), dy.data_ptr(), sdy, rstd.data_ptr(), dx.data_ptr(),
+                                    _ptr(dz), _ptr(dw), _ptr(part), R, W, ctx.group, int(ctx.gate_first), ROW_TYPES[x.dtype],
+                                    _cu.stream_ptr())
+        if rc:
+            _failed("cm_rmsnorm_gated_bwd", rc)
         F_.count_launch("rmsnorm_gated_bwd")
         return dx, dw, dz, None, None, None
 
@@ -305,12 +309,13 @@ class GatedRMSNormFn(torch.autograd.Function):
 def rmsnorm_gated(x, weight, z, eps, group, norm_before_gate):
     """None where the kernels do not apply: one type for all tensors (bf16, fp16 or fp32), groups of at most 16384 channels and at
     most 65535 of them."""
-    every = [t for t in (x, weight, z) if t is not None]
-    if x.dtype not in ROW_TYPES or any(t.dtype != x.dtype for t in every) or group > MAX_WIDTH or x.numel() == 0 or x.shape[-1] // group > 65535:
+    dt = x.dtype
+    if (dt not in ROW_TYPES or weight.dtype != dt or (z is not None and z.dtype != dt) or group > MAX_WIDTH or x.numel() == 0
+            or x.shape[-1] // group > 65535):
         return None
     weight = weight.contiguous()
     with _device_of(x):
-        if _wants_grad(*every):
+        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (z is not None and z.requires_grad)):
             return GatedRMSNormFn.apply(x, weight, z, float(eps), group, not norm_before_gate)
         return _gated_forward(x, weight, z, float(eps), group, not norm_before_gate, keep=False)[0]
 

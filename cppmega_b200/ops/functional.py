@@ -108,15 +108,11 @@ def _cuda(name: str, *tensors) -> Optional[Callable]:
     return fn
 
 
-def _require(ok: bool, message: str) -> None:
-    if not ok:
-        raise ValueError(message)
-
-
 def _same_device(name: str, first: torch.Tensor, *others) -> None:
+    dev = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
 
 
 # ---- dense ---------------------------------------------------------------
@@ -281,12 +277,14 @@ def residual_rmsnorm(y, residual, weight, post_weight=None, gate=None, scale: fl
     post norm), and the norm the next block reads, ``n = rms(h) * weight``.  Returns ``(n, h)``, both in the type of ``y``; ``n``
     is the norm of ``h`` as rounded to that type.  ``y``, ``residual`` [..., D]; ``gate`` [D] (one per channel, shared by all
     rows) or the shape of ``y``; ``weight``, ``post_weight`` [D]."""
-    D = y.shape[-1]
-    _require(residual.shape == y.shape, f"residual_rmsnorm: block output {tuple(y.shape)}, residual {tuple(residual.shape)}")
-    for name, t in (("weight", weight), ("post_weight", post_weight)):
-        _require(t is None or t.shape == (D,), f"residual_rmsnorm: {name} {None if t is None else tuple(t.shape)} for rows of {D}")
-    _require(gate is None or gate.shape == (D,) or gate.shape == y.shape,
-             f"residual_rmsnorm: gate {None if gate is None else tuple(gate.shape)} is neither ({D},) nor {tuple(y.shape)}")
+    row = y.shape[-1:]
+    if residual.shape != y.shape:
+        raise ValueError(f"residual_rmsnorm: block output {tuple(y.shape)}, residual {tuple(residual.shape)}")
+    if weight.shape != row or (post_weight is not None and post_weight.shape != row):
+        raise ValueError(f"residual_rmsnorm: weight {tuple(weight.shape)}, post_weight "
+                         f"{None if post_weight is None else tuple(post_weight.shape)} for rows of {tuple(row)}")
+    if gate is not None and gate.shape != row and gate.shape != y.shape:
+        raise ValueError(f"residual_rmsnorm: gate {tuple(gate.shape)} is neither {tuple(row)} nor {tuple(y.shape)}")
     _same_device("residual_rmsnorm", y, residual, weight, post_weight, gate)
     fn = _cuda("residual_rmsnorm", y)
     if fn is not None:
@@ -315,9 +313,10 @@ def gated_mlp(x, w1, w2, activation: str = "silu"):
     ``w2`` [Ho, F]; ``activation`` is ``silu``, ``gelu_tanh`` or ``relu``.  In bf16 with widths that are multiples of 8 the
     projections, the activation and the product are one kernel, and so are their gradients; under an FP8 recipe, and for anything
     else, it is :func:`linear`, activation, :func:`linear`."""
-    _require(activation in ref.GATED_ACTIVATIONS, f"gated_mlp: unknown activation {activation!r}, one of {sorted(ref.GATED_ACTIVATIONS)}")
-    _require(w1.dim() == 2 and w2.dim() == 2 and x.dim() >= 1 and w1.shape[1] == x.shape[-1] and w1.shape[0] == 2 * w2.shape[1],
-             f"gated_mlp: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}")
+    if activation not in ref.GATED_ACTIVATIONS:
+        raise ValueError(f"gated_mlp: unknown activation {activation!r}, one of {sorted(ref.GATED_ACTIVATIONS)}")
+    if w1.dim() != 2 or w2.dim() != 2 or x.dim() < 1 or w1.shape[1] != x.shape[-1] or w1.shape[0] != 2 * w2.shape[1]:
+        raise ValueError(f"gated_mlp: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}")
     _same_device("gated_mlp", x, w1, w2)
     fn = _cuda("gated_mlp", x) if _PRECISION_RECIPE == "bf16" else None
     if fn is not None:
