@@ -8,6 +8,7 @@
 // backward and adds their weight gradient in registers.  Bound by memory: three rows moved forward, five backward; the gate is read
 // where it lies (a column slice of the projection has its own pitch).  The weight gradient is summed in a fixed order.
 #include "row_vec.cuh"
+#define CM_ROW_TEAM_BY_WARP(F) case 16 * 32 + 4: return F(32, 4, true);
 
 namespace cm {
 
@@ -22,13 +23,6 @@ struct GatedArgs {
   float eps;
   int gate_first;
 };
-
-// 1 / (1 + inf) is 0, as it should be
-__device__ __forceinline__ float sigmoid_of(float z) {
-  float q;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + __expf(-z)));
-  return q;
-}
 
 template <typename T, int TPR, int VPT, bool VEC>
 __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArgs a) {
@@ -52,7 +46,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArg
       float z[N];
       rv_unpack<T>(zv[i], z);
 #pragma unroll
-      for (int j = 0; j < N; ++j) u[i][j] *= z[j] * sigmoid_of(z[j]);
+      for (int j = 0; j < N; ++j) u[i][j] *= z[j] * rv_sigmoid(z[j]);
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) ss[0] += u[i][j] * u[i][j];
@@ -71,7 +65,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArg
       float z[N];
       rv_unpack<T>(zv[i], z);
 #pragma unroll
-      for (int j = 0; j < N; ++j) u[i][j] *= z[j] * sigmoid_of(z[j]);
+      for (int j = 0; j < N; ++j) u[i][j] *= z[j] * rv_sigmoid(z[j]);
     }
     rv_store<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + g0, t + i * TPR, G, rv_pack<T>(u[i]));
   }
@@ -113,6 +107,8 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
     const int G = row < a.rows ? a.group : 0;
     const float r = G ? a.rstd[row * gridDim.y + blockIdx.y] : 0.f;
     in.wait(row);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) rv_keep_packed(wv[i]);
     float s[1] = {0.f};
     float hat[VPT][N], dnw[VPT][N], gate[GATE_FIRST ? VPT : 1][N], xs[GATE_FIRST ? VPT : 1][N];
 #pragma unroll
@@ -124,7 +120,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
       rv_unpack<T>(wv[i], w);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float q = sigmoid_of(z[j]), g = has_z ? z[j] * q : 1.f, slope = q + z[j] * q * (1.f - q);
+        const float q = rv_sigmoid(z[j]), g = has_z ? z[j] * q : 1.f, slope = q + g * (1.f - q);    // without z no slope is used
         if constexpr (GATE_FIRST) {
           gate[i][j] = g;
           xs[i][j] = x[j] * slope;

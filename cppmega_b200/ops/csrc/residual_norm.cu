@@ -11,6 +11,7 @@
 // Bound by memory: forward 4 rows moved, backward 6 (4 read).  Sums over rows go through one partial row per block and a second
 // kernel in a fixed order: the same call gives the same bits.
 #include "row_vec.cuh"
+#define CM_ROW_TEAM_BY_WARP(F)
 
 namespace cm {
 
@@ -108,10 +109,10 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_fwd(const Resid
 }
 
 template <typename T, int TPR, int VPT, bool VEC, bool FULL>
-__global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_bwd(const ResidualArgs a) {
+__global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : (FULL ? 512 : 768) / rv_block<TPR>()) residual_norm_bwd(const ResidualArgs a) {
   constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
   extern __shared__ __align__(16) uint4 dyn[];
-  __shared__ float red[2 * 3 * (TPR > 32 ? TPR / 32 : 1)];
+  __shared__ float red[2 * (FULL ? 3 : 1) * (TPR > 32 ? TPR / 32 : 1)];
   __shared__ float scratch[RPB > 1 ? RPB * TPR * VPT * N : 1];
   enum { DN = 0, DH = 1, HH = 2, YY = 3, GG = 4 };
   const int t = threadIdx.x % TPR, W = a.width;
@@ -135,99 +136,97 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_bwd(const Resid
   }
   const long long step = (long long)gridDim.x * RPB, first = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
   in.start(first, step);
-  // scale * gate of vector i
-  auto gated = [&](int i, float (&f)[N]) {
+  // the parameters of this thread's columns, as they come; a missing post norm or gate is a factor of one
+  uint4 wv[VPT], pv[FULL ? VPT : 1], tv[FULL ? VPT : 1];
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = a.scale;
+  for (int i = 0; i < VPT; ++i) {
+    wv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.w), t + i * TPR, W);
     if constexpr (FULL) {
-      if (gate) {
-        float q[N];
-        rv_unpack<T>(a.gate_rows ? in.get(GG, i) : rv_load<T, VEC>(reinterpret_cast<const T*>(a.gate), t + i * TPR, W), q);
-#pragma unroll
-        for (int j = 0; j < N; ++j) f[j] *= q[j];
-      }
+      pv[i] = post ? rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), t + i * TPR, W) : rv_ones<T>();
+      tv[i] = gate && !a.gate_rows ? rv_load<T, VEC>(reinterpret_cast<const T*>(a.gate), t + i * TPR, W) : rv_ones<T>();
     }
-  };
+  }
+  const float inv_w = 1.f / W;
   int turn = 0;
   for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += step, turn ^= 1) {
     const long long row = row0 + threadIdx.x / TPR;
     const bool on = row < a.rows;
-    const float rho = on ? a.rstd_h[row] : 0.f, r = on && post ? a.rstd_y[row] : 1.f;
+    const float rho = on ? a.rstd_h[row] : 0.f, r = post ? (on ? a.rstd_y[row] : 0.f) : 1.f;
     in.wait(row);
-    float s[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      rv_keep_packed(wv[i]);
+      if constexpr (FULL) {
+        rv_keep_packed(pv[i]);
+        rv_keep_packed(tv[i]);
+      }
+    }
+    // s[0] = sum g h, s[1] = sum gate post y (rho g + dh0), s[2] = sum gate post y h: the constant factors follow behind the sums
+    float s[FULL ? 3 : 1] = {};
+    float dt[VPT][N], hv[FULL ? 1 : VPT][N];                // rho g + dh0, h
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       float g[N], h[N], w[N];
       rv_unpack<T>(in.get(DN, i), g);
       rv_unpack<T>(in.get(HH, i), h);
-      rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w), t + i * TPR, W), w);
+      rv_unpack<T>(in.get(DH, i), dt[i]);
+      rv_unpack<T>(wv[i], w);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        h[j] *= rho;
-        acc_w[i][j] += g[j] * h[j];
+        acc_w[i][j] += g[j] * (h[j] * rho);
         g[j] *= w[j];
         s[0] += g[j] * h[j];
+        dt[i][j] += rho * g[j];
+        if constexpr (!FULL) hv[i][j] = h[j];
       }
       if constexpr (FULL) {
-        if (post) {
-          float d[N], y[N], f[N], p[N];
-          rv_unpack<T>(in.get(DH, i), d);
-          rv_unpack<T>(in.get(YY, i), y);
-          rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), t + i * TPR, W), p);
-          gated(i, f);
+        float y[N], p[N], q[N];
+        rv_unpack<T>(in.get(YY, i), y);
+        rv_unpack<T>(pv[i], p);
+        rv_unpack<T>(a.gate_rows ? in.get(GG, i) : tv[i], q);
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            const float ay = f[j] * p[j] * y[j] * r;
-            s[1] += ay * (rho * g[j] + d[j]);
-            s[2] += ay * h[j];
-          }
+        for (int j = 0; j < N; ++j) {
+          const float ay = p[j] * q[j] * y[j];
+          s[1] += ay * dt[i][j];
+          s[2] += ay * h[j];
         }
       }
     }
-    if (post) rv_team_sum<TPR, 3>(s, red, turn);
-    else rv_team_sum<TPR, 1>(reinterpret_cast<float(&)[1]>(s), red, turn);
-    const float m1 = s[0] / W, m2 = (s[1] - rho * m1 * s[2]) / W;
+    rv_team_sum<TPR, FULL ? 3 : 1>(s, red, turn);
+    const float k = rho * rho * rho * s[0] * inv_w;         // dh = rho g + dh0 - k h
+    float m2 = 0.f;                                         // mean(gate post dh yh)
+    if constexpr (FULL) m2 = post ? r * (s[1] - k * s[2]) * inv_w : 0.f;
+    const float sr = a.scale * r;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = t + i * TPR;
-      float g[N], h[N], w[N], d[N];
-      rv_unpack<T>(in.get(DN, i), g);
-      rv_unpack<T>(in.get(HH, i), h);
-      rv_unpack<T>(in.get(DH, i), d);
-      rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w), c, W), w);
+      float d[N];
+      if constexpr (FULL) {
+        rv_unpack<T>(in.get(HH, i), d);
 #pragma unroll
-      for (int j = 0; j < N; ++j) d[j] += rho * (g[j] * w[j] - h[j] * rho * m1);
+        for (int j = 0; j < N; ++j) d[j] = dt[i][j] - k * d[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) d[j] = dt[i][j] - k * hv[i][j];
+      }
       rv_store<T, VEC>(reinterpret_cast<T*>(a.dres) + row * W, c, on ? W : 0, rv_pack<T>(d));
       if constexpr (FULL) {
-        float y[N], f[N], q[N], p[N];         // p: y with the post norm, which the gate multiplies
+        float y[N], p[N], q[N];
         rv_unpack<T>(in.get(YY, i), y);
-#pragma unroll
-        for (int j = 0; j < N; ++j) p[j] = y[j] *= r;
-        if (post) {
-          rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), c, W), q);
-#pragma unroll
-          for (int j = 0; j < N; ++j) p[j] *= q[j];
-        }
-        gated(i, f);
-        if (gate) {
+        rv_unpack<T>(pv[i], p);
+        rv_unpack<T>(a.gate_rows ? in.get(GG, i) : tv[i], q);
+        if (a.dgate_rows) {
           float dg[N];
 #pragma unroll
-          for (int j = 0; j < N; ++j) dg[j] = on ? a.scale * d[j] * p[j] : 0.f;
-          if (a.gate_rows) {
-            if (a.dgate_rows) rv_store<T, VEC>(reinterpret_cast<T*>(a.dgate_rows) + row * W, c, on ? W : 0, rv_pack<T>(dg));
-          } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) acc_g[i][j] += dg[j];
-          }
+          for (int j = 0; j < N; ++j) dg[j] = sr * d[j] * (y[j] * p[j]);
+          rv_store<T, VEC>(reinterpret_cast<T*>(a.dgate_rows) + row * W, c, on ? W : 0, rv_pack<T>(dg));
         }
 #pragma unroll
-        for (int j = 0; j < N; ++j) d[j] *= f[j];              // dp
-        if (post) {
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            if (on) acc_p[i][j] += d[j] * y[j];
-            d[j] = r * (d[j] * q[j] - y[j] * m2);
-          }
+        for (int j = 0; j < N; ++j) {
+          const float yh = y[j] * r, e = d[j] * q[j];
+          acc_g[i][j] += d[j] * (yh * p[j]);
+          acc_p[i][j] += e * yh;
+          d[j] = sr * (e * p[j] - yh * m2);
         }
       } else {
 #pragma unroll
@@ -236,6 +235,15 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_bwd(const Resid
       if (a.dy) rv_store<T, VEC>(reinterpret_cast<T*>(a.dy) + row * W, c, on ? W : 0, rv_pack<T>(d));
     }
     in.next(row + (long long)rv_stages(TPR, VPT) * step);
+  }
+  if constexpr (FULL) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        acc_g[i][j] *= a.scale;
+        acc_p[i][j] *= a.scale;
+      }
   }
   const long long at = (long long)blockIdx.x * W;
   if (a.part_w) rv_partial<T, TPR, VPT>(acc_w, a.part_w + at, W, scratch);

@@ -49,6 +49,26 @@ __device__ __forceinline__ uint4 rv_pack(const float (&f)[RowVec<T>::N]) {
   }
 }
 
+// 1 / (1 + exp(-z)): the exponential's error is a few 2^-24 (1 + |z|); 1 / (1 + inf) is 0, as it should be
+__device__ __forceinline__ float rv_sigmoid(float z) {
+  float e, q;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));
+  return q;
+}
+
+// Keeps a vector packed: its unpacked values are formed again after this point instead of being held in registers.
+__device__ __forceinline__ void rv_keep_packed(uint4& v) { asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)); }
+
+// a vector of ones
+template <typename T>
+__device__ __forceinline__ uint4 rv_ones() {
+  float f[RowVec<T>::N];
+#pragma unroll
+  for (int j = 0; j < RowVec<T>::N; ++j) f[j] = 1.f;
+  return rv_pack<T>(f);
+}
+
 // vector `i` of the row (zero past its end)
 template <typename T, bool VEC>
 __device__ __forceinline__ uint4 rv_load(const T* __restrict__ row, int i, int width) {
@@ -260,10 +280,10 @@ static inline int rv_team(int nvec, bool vec, bool by_warp) {
 #define CM_ROW_TEAM(team, vec, F)                                                                                   \
   if (vec) {                                                                                                        \
     switch (team) {                                                                                                 \
+      CM_ROW_TEAM_BY_WARP(F)                                                                                        \
       case 16 * 8 + 1: return F(8, 1, true);                                                                        \
       case 16 * 32 + 1: return F(32, 1, true);                                                                      \
       case 16 * 32 + 2: return F(32, 2, true);                                                                      \
-      case 16 * 32 + 4: return F(32, 4, true);                                                                      \
       case 16 * 128 + 1: return F(128, 1, true);                                                                    \
       case 16 * 128 + 2: return F(128, 2, true);                                                                    \
       case 16 * 256 + 2: return F(256, 2, true);                                                                    \

@@ -1,6 +1,6 @@
 """Small, self-terminating workloads for Nsight Compute captures of single kernels.
 
-    python -m cppmega_b200.tools.ncu_cases {gemm,gemm_wgrad,attention,head_linear,scan_fwd,scan_bwd,m2rnn,m2rnn_bwd,sparse_mla,indexer,ce,rmsnorm,rmsnorm_bwd,adamw,quantize,strided_copy,moe_local,mxfp8_gemm}
+    python -m cppmega_b200.tools.ncu_cases {gemm,gemm_wgrad,attention,head_linear,scan_fwd,scan_bwd,m2rnn,m2rnn_bwd,sparse_mla,indexer,ce,rmsnorm,rmsnorm_bwd,adamw,quantize,strided_copy,moe_local,mxfp8_gemm,residual_norm,gated_norm,gated_mlp,gated_mlp_few}
 
 Each case launches its kernel three times on inputs that exceed the 126 MB L2 but hold at most a few GB, so a
 ``--set full`` capture of one launch finishes in a minute or two:
@@ -266,10 +266,51 @@ def case_head_linear():
     assert not F_.fallback_counts(), F_.fallback_counts()
 
 
+def case_residual_norm():
+    """The residual step, 16384 x 4096: plain, then with post norm and a gate per channel (forward and backward)."""
+    from cppmega_b200.ops import functional as F_
+    y, x = (torch.randn(16384, 4096, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    w, post, gate = (torch.ones(4096, device="cuda").bfloat16().requires_grad_() for _ in range(3))
+    g = torch.randn(16384, 4096, device="cuda").bfloat16()
+    for extra in ({}, dict(post_weight=post, gate=gate, scale=0.5)):
+        for _ in range(3):
+            torch.autograd.backward(F_.residual_rmsnorm(y, x, w, **extra), [g, g])
+    torch.cuda.synchronize()
+
+
+def case_gated_norm():
+    """The gated norm of the Mamba mixer, 16384 x 8192 in groups of 1024 (forward and backward)."""
+    from cppmega_b200.ops import functional as F_
+    x, z = (torch.randn(16384, 8192, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    w = torch.ones(8192, device="cuda").bfloat16().requires_grad_()
+    g = torch.randn(16384, 8192, device="cuda").bfloat16()
+    for _ in range(3):
+        F_.rmsnorm_gated(x, w, z, 1e-5, 1024).backward(g)
+    torch.cuda.synchronize()
+
+
+def case_gated_mlp(tokens: int = 4096):
+    """The gated feed-forward block at the quarter model's widths (forward and backward), or a few tokens through it."""
+    from cppmega_b200.ops import cuda as cu
+    from cppmega_b200.ops import functional as F_
+    train = tokens > 256
+    x = torch.randn(tokens, 3584, device="cuda").bfloat16().requires_grad_(train)
+    w1 = (torch.randn(2 * 18944, 3584, device="cuda") * 0.02).bfloat16().requires_grad_(train)
+    w2 = (torch.randn(3584, 18944, device="cuda") * 0.01).bfloat16().requires_grad_(train)
+    for _ in range(3):
+        y = F_.gated_mlp(x, w1, w2)
+        if train:
+            y.backward(x.detach())
+    torch.cuda.synchronize()
+    cu.check_errors()
+
+
 CASES = {"gemm": case_gemm, "attention": case_attention, "head_linear": case_head_linear, "gemm_wgrad": lambda: case_gemm(True, True), "scan_fwd": case_scan_fwd,
          "scan_bwd": case_scan_bwd, "m2rnn": case_m2rnn, "ce": case_ce, "rmsnorm": case_rmsnorm, "mxfp8_gemm": case_mxfp8_gemm,
          "m2rnn_bwd": case_m2rnn_bwd, "sparse_mla": case_sparse_mla, "indexer": case_indexer,
-         "rmsnorm_bwd": case_rmsnorm_bwd, "adamw": case_adamw, "quantize": case_quantize, "strided_copy": case_strided_copy, "moe_local": case_moe_local}
+         "rmsnorm_bwd": case_rmsnorm_bwd, "adamw": case_adamw, "quantize": case_quantize, "strided_copy": case_strided_copy, "moe_local": case_moe_local,
+         "residual_norm": case_residual_norm, "gated_norm": case_gated_norm, "gated_mlp": case_gated_mlp,
+         "gated_mlp_few": lambda: case_gated_mlp(24)}
 
 if __name__ == "__main__":
     name = sys.argv[1] if len(sys.argv) > 1 else ""
