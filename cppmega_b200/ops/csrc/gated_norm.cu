@@ -24,32 +24,34 @@ struct GatedArgs {
   int gate_first;
 };
 
-template <typename T, int TPR, int VPT, bool VEC>
+template <typename T, int TPR, int VPT, bool VEC, bool GATE_FIRST>
 __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArgs a) {
   constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
   __shared__ float red[2 * (TPR > 32 ? TPR / 32 : 1)];
   const int t = threadIdx.x % TPR, g0 = blockIdx.y * a.group;
   const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
   const int G = row < a.rows ? a.group : 0;
+  const bool has_z = a.z != nullptr;
   uint4 xv[VPT], zv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     xv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.sx + g0, t + i * TPR, G);
-    zv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.z) + row * a.sz + g0, t + i * TPR, a.z ? G : 0);
+    zv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.z) + row * a.sz + g0, t + i * TPR, has_z ? G : 0);
   }
   float ss[1] = {0.f};
-  float u[VPT][N];
+  float gated[GATE_FIRST ? VPT : 1][N];                    // x a(z): the sigmoids are not formed twice
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    rv_unpack<T>(xv[i], u[i]);
-    if (a.gate_first && a.z) {
+    float x[N];
+    rv_unpack<T>(xv[i], x);
+    if constexpr (GATE_FIRST) {
       float z[N];
       rv_unpack<T>(zv[i], z);
 #pragma unroll
-      for (int j = 0; j < N; ++j) u[i][j] *= z[j] * rv_sigmoid(z[j]);
+      for (int j = 0; j < N; ++j) gated[i][j] = x[j] *= has_z ? z[j] * rv_sigmoid(z[j]) : 1.f;
     }
 #pragma unroll
-    for (int j = 0; j < N; ++j) ss[0] += u[i][j] * u[i][j];
+    for (int j = 0; j < N; ++j) ss[0] += x[j] * x[j];
   }
   rv_team_sum<TPR, 1>(ss, red, 0);
   const float r = rsqrtf(ss[0] / a.group + a.eps);
@@ -57,17 +59,20 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArg
   if (t == 0 && a.rstd) a.rstd[row * gridDim.y + blockIdx.y] = r;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    float w[N];
+    float x[N], w[N];
     rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, t + i * TPR, G), w);
+    if constexpr (GATE_FIRST) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) u[i][j] *= r * w[j];
-    if (!a.gate_first && a.z) {
+      for (int j = 0; j < N; ++j) x[j] = gated[i][j] * r * w[j];
+    } else {
       float z[N];
+      rv_keep_packed(xv[i]);
+      rv_unpack<T>(xv[i], x);
       rv_unpack<T>(zv[i], z);
 #pragma unroll
-      for (int j = 0; j < N; ++j) u[i][j] *= z[j] * rv_sigmoid(z[j]);
+      for (int j = 0; j < N; ++j) x[j] *= r * w[j] * (has_z ? z[j] * rv_sigmoid(z[j]) : 1.f);
     }
-    rv_store<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + g0, t + i * TPR, G, rv_pack<T>(u[i]));
+    rv_store<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + g0, t + i * TPR, G, rv_pack<T>(x));
   }
 }
 
@@ -101,11 +106,14 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
   uint4 wv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) wv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, t + i * TPR, a.group);
+  auto stat = [&](long long row) { return row < a.rows ? a.rstd[row * gridDim.y + blockIdx.y] : 0.f; };
+  float next_r = stat((long long)blockIdx.x * RPB + threadIdx.x / TPR);      // requested a row ahead
   int turn = 0;
   for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += step, turn ^= 1) {
     const long long row = row0 + threadIdx.x / TPR;
     const int G = row < a.rows ? a.group : 0;
-    const float r = G ? a.rstd[row * gridDim.y + blockIdx.y] : 0.f;
+    const float r = next_r;
+    next_r = stat(row + step);
     in.wait(row);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) rv_keep_packed(wv[i]);
@@ -184,9 +192,12 @@ static int gated_launch(const GatedArgs& a, bool back, int& blocks, cudaStream_t
         configured[a.gate_first].done();                                                                                         \
       }                                                                                                                          \
       static int resident[2];                                                                                                    \
-      blocks = rv_blocks(kern, TB, RING, RPB, a.rows, groups, resident[a.gate_first]);                                                         \
+      blocks = rv_blocks(kern, TB, RING, RPB, a.rows, a.width, groups, resident[a.gate_first]);                                                         \
       kern<<<dim3(blocks, groups), TB, RING, s>>>(a);                                                                            \
-    } else gated_norm_fwd<T, TPR, VPT, VEC><<<dim3(unsigned((a.rows + RPB - 1) / RPB), groups), TB, 0, s>>>(a);                    \
+    } else {                                                                                                                     \
+      auto kern = a.gate_first ? gated_norm_fwd<T, TPR, VPT, VEC, true> : gated_norm_fwd<T, TPR, VPT, VEC, false>;               \
+      kern<<<dim3(unsigned((a.rows + RPB - 1) / RPB), groups), TB, 0, s>>>(a);                                                   \
+    }                                                                                                                            \
     return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                                           \
   }()
   CM_ROW_TEAM(team, vec, CM_GATED);
@@ -219,7 +230,12 @@ extern "C" int cm_rmsnorm_gated_fwd(const void* x, long long sx, const void* z, 
   return gated_any(a, dtype, false, blocks, s);
 }
 
-// part: [cm_row_norm_parts][width] floats of work space, with dw; dz, dw may be null.  dx, dz packed.
+// Partial rows of the weight gradient that the backward needs room for.
+extern "C" int cm_rmsnorm_gated_parts(long long rows, int width, int group) {
+  return group > 0 ? int(rv_most_blocks(rows, width, width / group)) : 0;
+}
+
+// part: [cm_rmsnorm_gated_parts][width] floats of work space, with dw; dz, dw may be null.  dx, dz packed.
 extern "C" int cm_rmsnorm_gated_bwd(const void* x, long long sx, const void* z, long long sz, const void* w, const void* dy, long long sdy,
                                     const float* rstd, void* dx, void* dz, void* dw, float* part, long long rows, int width, int group,
                                     int gate_first, int dtype, cudaStream_t s) {

@@ -147,11 +147,18 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
     }
   }
   const float inv_w = 1.f / W;
+  float next_rho, next_r;                                   // of the next row, requested a row ahead
+  auto stats = [&](long long row) {
+    next_rho = row < a.rows ? a.rstd_h[row] : 0.f;
+    next_r = !post ? 1.f : row < a.rows ? a.rstd_y[row] : 0.f;
+  };
+  stats(first);
   int turn = 0;
   for (long long row0 = (long long)blockIdx.x * RPB; row0 < a.rows; row0 += step, turn ^= 1) {
     const long long row = row0 + threadIdx.x / TPR;
     const bool on = row < a.rows;
-    const float rho = on ? a.rstd_h[row] : 0.f, r = post ? (on ? a.rstd_y[row] : 0.f) : 1.f;
+    const float rho = next_rho, r = next_r;
+    stats(row + step);
     in.wait(row);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -280,7 +287,7 @@ static int residual_launch(const ResidualArgs& a, bool back, int& blocks, cudaSt
         configured.done();                                                                                                        \
       }                                                                                                                           \
       static int resident[6];                                                                                                     \
-      blocks = rv_blocks(kern, TB, SLOT * a.ring_ops, RPB, a.rows, 1, resident[a.ring_ops]);                                      \
+      blocks = rv_blocks(kern, TB, SLOT * a.ring_ops, RPB, a.rows, a.width, 1, resident[a.ring_ops]);                                    \
       kern<<<blocks, TB, SLOT * a.ring_ops, s>>>(a);                                                                              \
     } else residual_norm_fwd<T, TPR, VPT, VEC, FULL><<<unsigned((a.rows + RPB - 1) / RPB), TB, 0, s>>>(a);                          \
     return cudaGetLastError() == cudaSuccess ? 0 : -3;                                                                            \
@@ -318,9 +325,9 @@ extern "C" int cm_residual_rmsnorm_fwd(const void* y, long long sy, const void* 
 }
 
 // Partial rows of a column sum that the backward needs room for.
-extern "C" int cm_row_norm_parts(long long rows) { return int(rv_most_blocks(rows)); }
+extern "C" int cm_residual_rmsnorm_parts(long long rows, int width) { return int(rv_most_blocks(rows, width, 1)); }
 
-// part: [3][cm_row_norm_parts][width] floats of work space.  dn, dh (gradients of n and h) may be null; dy null: it is dres (no post
+// part: [3][cm_residual_rmsnorm_parts][width] floats of work space.  dn, dh (gradients of n and h) may be null; dy null: it is dres (no post
 // norm, no gate, scale 1); dw, dpost, dgate (one per channel), dgate_rows may be null.
 extern "C" int cm_residual_rmsnorm_bwd(const void* dn, long long sdn, const void* dh, long long sdh, const void* h, const void* y,
                                        long long sy, const void* w, const void* post, const void* gate, int gate_rows,
@@ -337,7 +344,7 @@ extern "C" int cm_residual_rmsnorm_bwd(const void* dn, long long sdn, const void
   int sums = 0;
   auto want = [&](void* out, float*& slot) {
     if (!out) return;
-    slot = part + sums * rv_most_blocks(rows) * width;
+    slot = part + sums * rv_most_blocks(rows, width, 1) * width;
     c.partial[sums] = slot;
     c.out[sums++] = out;
   };

@@ -223,22 +223,24 @@ constexpr int rv_stages(int tpr, int vpt) {
   const int held = (tpr < 128 ? 128 : tpr) * vpt;
   return held <= 256 ? 4 : held <= 512 ? 3 : held <= 1024 ? 2 : 0;
 }
-// Blocks of a backward kernel: those that an SM holds at once, at most RV_BLOCKS_PER_SM, each with a row at least.
-constexpr int RV_BLOCKS_PER_SM = 4;
-static inline long long rv_most_blocks(long long rows) {
-  const long long most = (long long)sm_count() * RV_BLOCKS_PER_SM;
+// Blocks of a backward kernel: those that the SMs hold at once, up to this many for each, shared by `share` sections of the rows; and no
+// more than there are rows.  (Four blocks of 128 threads an SM left the gated norm's backward waiting for memory: 281 us, 16 warps.)
+static inline long long rv_most_blocks(long long rows, int width, int share) {
+  const int per_sm = width / share <= 2048 ? 8 : 4;
+  const long long most = ((long long)sm_count() * per_sm + share - 1) / share;
   return rows < most ? rows : most;
 }
-// `resident`: answers of the runtime, by operands in the ring, for one kernel (0: not asked yet)
+// `resident`: the runtime's answer for one kernel and amount of shared memory (0: not asked yet)
 template <typename K>
-static int rv_blocks(K kern, int threads, int smem, int rows_per_block, long long rows, int share, int& resident) {
+static int rv_blocks(K kern, int threads, int smem, int rows_per_block, long long rows, int width, int share, int& resident) {
   if (resident == 0) {
     int n = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess || n < 1) n = 1;
-    resident = n < RV_BLOCKS_PER_SM ? n : RV_BLOCKS_PER_SM;
+    resident = n;
   }
-  const long long want = (rows + rows_per_block - 1) / rows_per_block, most = ((long long)sm_count() * resident + share - 1) / share;
-  return int(want < most ? want : most);
+  const long long want = (rows + rows_per_block - 1) / rows_per_block, fit = ((long long)sm_count() * resident + share - 1) / share;
+  const long long most = rv_most_blocks(rows, width, share), n = fit < most ? fit : most;
+  return int(want < n ? want : n);
 }
 
 // out[c] = sum over p of partial[p][c], c < width, in a fixed order; blockIdx.y chooses one of up to three sums.  32 threads share a

@@ -26,7 +26,8 @@ def declare(L: ctypes.CDLL) -> None:
         "cm_gated_mlp_fwd": [vp, i64, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp],
         "cm_gated_mlp_bwd": [vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp],
         "cm_residual_rmsnorm_fwd": [vp, i64, vp, i64, vp, vp, vp, i32, vp, vp, vp, vp, i64, i32, f32, f32, i32, vp],
-        "cm_row_norm_parts": [i64],
+        "cm_residual_rmsnorm_parts": [i64, i32],
+        "cm_rmsnorm_gated_parts": [i64, i32, i32],
         "cm_residual_rmsnorm_bwd": [vp, i64, vp, i64, vp, vp, i64, vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, f32,
                                     i32, vp],
         "cm_rmsnorm_gated_fwd": [vp, i64, vp, i64, vp, vp, vp, i64, i32, i32, i32, f32, i32, vp],
@@ -219,7 +220,7 @@ class ResidualRMSNormFn(torch.autograd.Function):
         dpost = torch.empty_like(post) if need_post else None
         sums = need_w + need_post + (need_gate and not per_row)
         L = _cu.lib()
-        part = torch.empty(sums * L.cm_row_norm_parts(R) * W, dtype=torch.float32, device=h.device) if sums else None
+        part = torch.empty(sums * L.cm_residual_rmsnorm_parts(R, W) * W, dtype=torch.float32, device=h.device) if sums else None
         at = stats.data_ptr()
         rc = L.cm_residual_rmsnorm_bwd(_ptr(dn), sdn, _ptr(dh), sdh, h.data_ptr(), _ptr(y), sy, weight.data_ptr(), _ptr(post), _ptr(gate),
                                        int(per_row), at, at + 4 * R, dres.data_ptr(), _ptr(dy), _ptr(dgate) if per_row else None, _ptr(dw),
@@ -296,7 +297,7 @@ class GatedRMSNormFn(torch.autograd.Function):
         L = _cu.lib()
         if need_w:
             dw = torch.empty_like(weight)
-            part = torch.empty(L.cm_row_norm_parts(R) * W, dtype=torch.float32, device=x.device)
+            part = torch.empty(L.cm_rmsnorm_gated_parts(R, W, ctx.group) * W, dtype=torch.float32, device=x.device)
         rc = L.cm_rmsnorm_gated_bwd(x.data_ptr(), sx, _ptr(z), sz, weight.data_ptr(), dy.data_ptr(), sdy, rstd.data_ptr(), dx.data_ptr(),
                                     _ptr(dz), _ptr(dw), _ptr(part), R, W, ctx.group, int(ctx.gate_first), ROW_TYPES[x.dtype],
                                     _cu.stream_ptr())
