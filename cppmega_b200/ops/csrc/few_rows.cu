@@ -203,7 +203,7 @@ int launch_partials(const void* X, long long ldx, const void* W, float* part, co
     configured.done();
   }
   const int smem = a.stages * stage_bytes + SMEM_EXTRA;
-  if (early) return launch_early(few_rows_kernel, dim3(cut.grid), THREADS, smem, stream, tmW, tmX, a);
+  if (early) return launch_early(few_rows_kernel, dim3(cut.grid), dim3(THREADS), smem, stream, tmW, tmX, a);
   few_rows_kernel<<<cut.grid, THREADS, smem, stream>>>(tmW, tmX, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }

@@ -32,13 +32,13 @@ __device__ __forceinline__ void wait_for_input() { asm volatile("griddepcontrol.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename... P, typename... A>
-inline int launch_early(void (*kern)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, A... args) {
+inline int launch_early(void (*kern)(P...), dim3 grid, dim3 block, int smem, cudaStream_t stream, A... args) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;

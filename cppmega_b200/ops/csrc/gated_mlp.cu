@@ -382,31 +382,61 @@ static int plan_bn(int M, int F, bool back) {
 
 // ------------------------------ few tokens ------------------------------
 // A tile's sum over its partial tiles, for TOKS tokens of one weight row: their loads are in flight together, and the place of a partial
-// tile is found once for all of them.
-constexpr int TOKS = 8;
-__device__ __forceinline__ void few_sum(const float* __restrict__ part, const few::Cut& cut, int row, int tok0, float (&s)[TOKS]) {
-  const int t = row / few::TILE, in = row % few::TILE, n = min(TOKS, cut.tokens - tok0);
+// tile is found once for all of them.  A long reduction over few tiles leaves dozens of partial tiles; blockDim.y threads then share them
+// (first + y, first + y + blockDim.y, ...) and their sums are added in that order.
+constexpr int TOKS = 8, MAX_SHARE = 8;
+struct FewSums {
+  float s[MAX_SHARE - 1][TOKS][few::TILE];
+};
+__device__ __forceinline__ void few_sum(const float* __restrict__ part, const few::Cut& cut, int row, int tok0, FewSums* share, float (&s)[TOKS]) {
+  const int t = row / few::TILE, in = row % few::TILE, n = cut.tokens - tok0, c1 = cut.last(t);
+  const float* p0 = part + tok0 * few::TILE + in;
 #pragma unroll
   for (int j = 0; j < TOKS; ++j) s[j] = 0.f;
-  for (int c = cut.first(t); c <= cut.last(t); ++c) {
-    const float* p = part + cut.at(c, t) + tok0 * few::TILE + in;
+  for (int c = cut.first(t) + threadIdx.y; c <= c1; c += blockDim.y) {
+    const float* p = p0 + cut.at(c, t);
+    float v[TOKS];
+    if (n >= TOKS) {
 #pragma unroll
-    for (int j = 0; j < TOKS; ++j)
-      if (j < n) s[j] += p[j * few::TILE];
+      for (int j = 0; j < TOKS; ++j) v[j] = p[j * few::TILE];
+    } else {
+#pragma unroll
+      for (int j = 0; j < TOKS; ++j) v[j] = j < n ? p[j * few::TILE] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < TOKS; ++j) s[j] += v[j];
   }
+  if (blockDim.y == 1) return;
+  if (threadIdx.y > 0) {
+#pragma unroll
+    for (int j = 0; j < TOKS; ++j) share->s[threadIdx.y - 1][j][threadIdx.x] = s[j];
+  }
+  __syncthreads();
+  if (threadIdx.y == 0) {
+    for (int y = 1; y < blockDim.y; ++y)
+#pragma unroll
+      for (int j = 0; j < TOKS; ++j) s[j] += share->s[y - 1][j][threadIdx.x];
+  }
+}
+// threads that share a tile's partial tiles
+static int few_share(const few::Cut& c) {
+  const int most = c.nkb / c.q + 2;
+  return most <= 4 ? 1 : most <= 16 ? 4 : MAX_SHARE;
 }
 
 // h[token][f] = act(g) u from rows f and F + f of the first product; g, u kept for training.
 template <int ACT>
-__global__ void __launch_bounds__(128) few_gate_kernel(const float* __restrict__ part, const few::Cut cut, int F, __nv_bfloat16* __restrict__ h,
-                                                       __nv_bfloat16* __restrict__ gu) {
-  const int f = blockIdx.x * 128 + threadIdx.x, tok0 = blockIdx.y * TOKS;
+__global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_gate_kernel(const float* __restrict__ part, const few::Cut cut, int F,
+                                                                         __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ gu) {
+  __shared__ FewSums share;
+  const int f = min(int(blockIdx.x * few::TILE + threadIdx.x), F - 1), tok0 = blockIdx.y * TOKS;       // the last block repeats its last row
   few::wait_for_input();
   few::let_next_start();
-  if (f >= F) return;
   float g[TOKS], u[TOKS];
-  few_sum(part, cut, f, tok0, g);
-  few_sum(part, cut, F + f, tok0, u);
+  few_sum(part, cut, f, tok0, &share, g);
+  __syncthreads();
+  few_sum(part, cut, F + f, tok0, &share, u);
+  if (threadIdx.y > 0) return;
 #pragma unroll
   for (int j = 0; j < TOKS; ++j) {
     const long long tok = tok0 + j;
@@ -419,34 +449,43 @@ __global__ void __launch_bounds__(128) few_gate_kernel(const float* __restrict__
   }
 }
 
-__global__ void __launch_bounds__(128) few_sum_kernel(const float* __restrict__ part, const few::Cut cut, int N, __nv_bfloat16* __restrict__ y) {
-  const int n = blockIdx.x * few::TILE + threadIdx.x, tok0 = blockIdx.y * TOKS;
+__global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_sum_kernel(const float* __restrict__ part, const few::Cut cut, int N,
+                                                                        __nv_bfloat16* __restrict__ y) {
+  __shared__ FewSums share;
+  const int n = min(int(blockIdx.x * few::TILE + threadIdx.x), N - 1), tok0 = blockIdx.y * TOKS;
   few::wait_for_input();
-  if (n >= N) return;
   float s[TOKS];
-  few_sum(part, cut, n, tok0, s);
+  few_sum(part, cut, n, tok0, &share, s);
+  if (threadIdx.y > 0) return;
 #pragma unroll
   for (int j = 0; j < TOKS; ++j)
     if (tok0 + j < cut.tokens) y[(long long)(tok0 + j) * N + n] = __float2bfloat16(s[j]);
 }
 
-// Tokens up to which the weights are streamed by few_rows.cu.
-constexpr int FEW_TOKENS = 256;
+// Tokens up to which the weights are streamed by few_rows.cu.  Device time, streamed and in tiles, in us:
+//   hidden x ffn    1 token       64           128
+//   4096 x 21504    92 / 220    100 / 147    113 / 149
+//   1024 x  8192    22 /  45     23 /  41     27 /  42
+//   1024 x  2048    13 /  21     15 /  18
+//    256 x   512     9 /   9     11 /  10
+// A long ffn leaves the second product of the tiles few of them, each with a long reduction.
+static bool few_tokens(int M, int F) { return M <= (F >= 8192 ? 192 : 64); }
 
 static int few_forward(const void* x, long long ldx, const void* w1, const void* w2, __nv_bfloat16* gu, __nv_bfloat16* h, __nv_bfloat16* y,
                        float* ws, int M, int H, int F, int Ho, int act, int* err, cudaStream_t stream) {
   const few::Cut c1 = few::cut_for(M, 2 * F, H), c2 = few::cut_for(M, Ho, F);
   int rc = few::launch_partials(x, ldx, w1, ws, c1, 2 * F, H, false, err, stream);
   if (rc) return rc;
-  const dim3 grid((F + 127) / 128, (M + TOKS - 1) / TOKS);
+  const dim3 grid((F + few::TILE - 1) / few::TILE, (M + TOKS - 1) / TOKS), block(few::TILE, few_share(c1));
   switch (act) {
-    case SILU: rc = few::launch_early(few_gate_kernel<SILU>, grid, 128, 0, stream, ws, c1, F, h, gu); break;
-    case GELU_TANH: rc = few::launch_early(few_gate_kernel<GELU_TANH>, grid, 128, 0, stream, ws, c1, F, h, gu); break;
-    case RELU: rc = few::launch_early(few_gate_kernel<RELU>, grid, 128, 0, stream, ws, c1, F, h, gu); break;
+    case SILU: rc = few::launch_early(few_gate_kernel<SILU>, grid, block, 0, stream, ws, c1, F, h, gu); break;
+    case GELU_TANH: rc = few::launch_early(few_gate_kernel<GELU_TANH>, grid, block, 0, stream, ws, c1, F, h, gu); break;
+    case RELU: rc = few::launch_early(few_gate_kernel<RELU>, grid, block, 0, stream, ws, c1, F, h, gu); break;
     default: rc = -10;
   }
   if (!rc) rc = few::launch_partials(h, F, w2, ws, c2, Ho, F, true, err, stream);
-  if (!rc) rc = few::launch_early(few_sum_kernel, dim3((Ho + few::TILE - 1) / few::TILE, (M + TOKS - 1) / TOKS), 128, 0, stream, ws, c2, Ho, y);
+  if (!rc) rc = few::launch_early(few_sum_kernel, dim3((Ho + few::TILE - 1) / few::TILE, (M + TOKS - 1) / TOKS), dim3(few::TILE, few_share(c2)), 0,
+                                  stream, ws, c2, Ho, y);
   return rc;
 }
 
@@ -459,7 +498,7 @@ using namespace cm;
 
 // Floats of work space that the forward needs; 0: none.
 extern "C" long long cm_gated_mlp_fwd_ws(int M, int H, int F, int Ho) {
-  if (M > mlp::FEW_TOKENS || M <= 0) return 0;
+  if (M <= 0 || !mlp::few_tokens(M, F)) return 0;
   const long long a = few::cut_for(M, 2 * F, H).floats(), b = few::cut_for(M, Ho, F).floats();
   return a > b ? a : b;
 }
@@ -472,7 +511,7 @@ extern "C" int cm_gated_mlp_fwd(const void* x, long long ldx, const void* w1, co
   if (H % 8 || F % 8 || Ho % 8 || !mlp::tma_ok(x, ldx) || !mlp::tma_ok(w1, H) || !mlp::tma_ok(w2, F) || !mlp::tma_ok(gu, 0) ||
       !mlp::tma_ok(h, F) || !mlp::tma_ok(y, Ho))
     return -10;
-  if (M <= mlp::FEW_TOKENS) {
+  if (mlp::few_tokens(M, F)) {
     if (!ws) return -10;
     return mlp::few_forward(x, ldx, w1, w2, static_cast<__nv_bfloat16*>(gu), static_cast<__nv_bfloat16*>(h), static_cast<__nv_bfloat16*>(y), ws,
                             M, H, F, Ho, act, err, stream);

@@ -91,18 +91,14 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
   const float inv_group = 1.f / a.group;
   float acc[VPT][N] = {};
   RowRing<T, TPR, VPT, VEC, rv_stages(TPR, VPT), 3> in;
-  in.ring = dyn;
   in.ops = 3;
   in.width = a.group;
   in.rows = a.rows;
-  in.base[XX] = reinterpret_cast<const T*>(a.x) + g0;
-  in.base[DY] = reinterpret_cast<const T*>(a.dy) + g0;
-  in.base[ZZ] = has_z ? reinterpret_cast<const T*>(a.z) + g0 : nullptr;
-  in.pitch[XX] = a.sx;
-  in.pitch[DY] = a.sdy;
-  in.pitch[ZZ] = a.sz;
+  in.set(XX, reinterpret_cast<const T*>(a.x) + g0, a.sx);
+  in.set(DY, reinterpret_cast<const T*>(a.dy) + g0, a.sdy);
+  in.set(ZZ, has_z ? reinterpret_cast<const T*>(a.z) + g0 : nullptr, a.sz);
   const long long step = (long long)gridDim.x * RPB;
-  in.start((long long)blockIdx.x * RPB + threadIdx.x / TPR, step);
+  in.start(dyn, (long long)blockIdx.x * RPB + threadIdx.x / TPR, step);
   uint4 wv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) wv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, t + i * TPR, a.group);
@@ -114,7 +110,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
     const int G = row < a.rows ? a.group : 0;
     const float r = next_r;
     next_r = stat(row + step);
-    in.wait(row);
+    in.wait();
 #pragma unroll
     for (int i = 0; i < VPT; ++i) rv_keep_packed(wv[i]);
     float s[1] = {0.f};
@@ -147,7 +143,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
       if constexpr (!GATE_FIRST)
         if (a.dz) rv_store<T, VEC>(reinterpret_cast<T*>(a.dz) + row * a.width + g0, t + i * TPR, G, rv_pack<T>(z));
     }
-    in.next(row + (long long)rv_stages(TPR, VPT) * step);
+    in.next();
     rv_team_sum<TPR, 1>(s, red, turn);
     const float m = s[0] * inv_group;
 #pragma unroll
@@ -170,6 +166,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
       rv_store<T, VEC>(reinterpret_cast<T*>(a.dx) + row * a.width + g0, c, G, rv_pack<T>(x));
     }
   }
+  in.drain();
   if (a.part) rv_partial<T, TPR, VPT>(acc, a.part + (long long)blockIdx.x * a.width + g0, a.group, scratch);
 }
 

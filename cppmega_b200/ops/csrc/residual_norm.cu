@@ -114,28 +114,23 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
   extern __shared__ __align__(16) uint4 dyn[];
   __shared__ float red[2 * (FULL ? 3 : 1) * (TPR > 32 ? TPR / 32 : 1)];
   __shared__ float scratch[RPB > 1 ? RPB * TPR * VPT * N : 1];
-  enum { DN = 0, DH = 1, HH = 2, YY = 3, GG = 4 };
+  enum { HH = 0, DN = 1, DH = 2, YY = 3, GG = 4 };
   const int t = threadIdx.x % TPR, W = a.width;
-  float acc_w[VPT][N] = {}, acc_p[FULL ? VPT : 1][N] = {}, acc_g[FULL ? VPT : 1][N] = {};
+  float acc_w[VPT][N] = {}, acc_y[FULL ? VPT : 1][N] = {};
   const bool post = FULL && a.post, gate = FULL && a.gate;
   RowRing<T, TPR, VPT, VEC, rv_stages(TPR, VPT), FULL ? 5 : 3> in;
-  in.ring = dyn;
   in.ops = a.ring_ops;
   in.width = W;
   in.rows = a.rows;
-  auto operand = [&](int op, const void* p, long long pitch) {
-    in.base[op] = reinterpret_cast<const T*>(p);
-    in.pitch[op] = pitch;
-  };
-  operand(DN, a.dn, a.sdn);
-  operand(DH, a.dh, a.sdh);
-  operand(HH, a.h, W);
+  in.set(DN, a.dn, a.sdn);
+  in.set(DH, a.dh, a.sdh);
+  in.set(HH, a.h, W);
   if constexpr (FULL) {
-    operand(YY, a.y, a.sy);
-    operand(GG, a.gate_rows ? a.gate : nullptr, W);
+    in.set(YY, a.y, a.sy);
+    in.set(GG, a.gate_rows ? a.gate : nullptr, W);
   }
   const long long step = (long long)gridDim.x * RPB, first = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
-  in.start(first, step);
+  in.start(dyn, first, step);
   // the parameters of this thread's columns, as they come; a missing post norm or gate is a factor of one
   uint4 wv[VPT], pv[FULL ? VPT : 1], tv[FULL ? VPT : 1];
 #pragma unroll
@@ -159,7 +154,7 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
     const bool on = row < a.rows;
     const float rho = next_rho, r = next_r;
     stats(row + step);
-    in.wait(row);
+    in.wait();
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       rv_keep_packed(wv[i]);
@@ -231,8 +226,7 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           const float yh = y[j] * r, e = d[j] * q[j];
-          acc_g[i][j] += d[j] * (yh * p[j]);
-          acc_p[i][j] += e * yh;
+          acc_y[i][j] += (a.gate_rows ? e : d[j]) * yh;
           d[j] = sr * (e * p[j] - yh * m2);
         }
       } else {
@@ -241,22 +235,27 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
       }
       if (a.dy) rv_store<T, VEC>(reinterpret_cast<T*>(a.dy) + row * W, c, on ? W : 0, rv_pack<T>(d));
     }
-    in.next(row + (long long)rv_stages(TPR, VPT) * step);
+    in.next();
   }
-  if constexpr (FULL) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        acc_g[i][j] *= a.scale;
-        acc_p[i][j] *= a.scale;
-      }
-  }
+  in.drain();
   const long long at = (long long)blockIdx.x * W;
   if (a.part_w) rv_partial<T, TPR, VPT>(acc_w, a.part_w + at, W, scratch);
   if constexpr (FULL) {
-    if (a.part_post) rv_partial<T, TPR, VPT>(acc_p, a.part_post + at, W, scratch);
-    if (a.part_gate) rv_partial<T, TPR, VPT>(acc_g, a.part_gate + at, W, scratch);
+    // with a gate per channel both its gradient and the post norm's are the sum of dh yh, times the other one's factor; with a gate per
+    // element the sum already holds the gate
+    auto out = [&](float* part, const uint4 (&factor)[VPT]) {
+      float sum[VPT][N];
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float f[N];
+        rv_unpack<T>(factor[i], f);
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum[i][j] = a.scale * f[j] * acc_y[i][j];
+      }
+      rv_partial<T, TPR, VPT>(sum, part + at, W, scratch);
+    };
+    if (a.part_post) out(a.part_post, tv);
+    if (a.part_gate) out(a.part_gate, pv);
   }
 }
 

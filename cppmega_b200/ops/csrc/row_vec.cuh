@@ -162,59 +162,68 @@ __device__ __forceinline__ void rv_partial(const float (&acc)[VPT][RowVec<T>::N]
 // with asynchronous copies and reads back only what it copied, so the copies need no barrier and keep running over the barriers of the
 // rows' sums; read back twice (before and after a row's sum) they take no registers in between.  NS = 0, and rows that are not on 16
 // bytes: plain loads, twice.
+// What lies past a row's end, past the last row, or belongs to an absent operand is filled with zeros by the copy itself.
 template <typename T, int TPR, int VPT, bool VEC, int NS, int OPS>
 struct RowRing {
   static constexpr bool ON = VEC && NS > 0;
-  static constexpr int TB = rv_block<TPR>(), N = RowVec<T>::N;
-  uint4* ring;               // [NS][ops][VPT][TB]
-  const T* base[OPS];        // null: zero
+  static constexpr int TB = rv_block<TPR>(), N = RowVec<T>::N, SLOTS = NS > 0 ? NS : 1;
+  uint4* mine;               // [ops][NS][VPT][TB], at this thread
+  const T* base[OPS];        // first row; null: zero
   long long pitch[OPS];
-  int ops, width;
-  long long rows;
-  int slot = 0;
-  long long row = 0;
+  int ops, width, first;     // first: this thread's first vector
+  long long rows, row, ahead, step;
+  int slot;
 
-  __device__ __forceinline__ uint4* at(int op, int i) const { return ring + ((slot * ops + op) * VPT + i) * TB + threadIdx.x; }
-  // start the copies of row `r` into the current slot (an empty group past the last row)
-  __device__ __forceinline__ void request(long long r) {
+  __device__ __forceinline__ void set(int op, const void* p, long long elements) {
+    base[op] = reinterpret_cast<const T*>(p);
+    pitch[op] = elements;
+  }
+  // the copies of the row NS rows ahead, into the slot that has just been used
+  __device__ __forceinline__ void request() {
     if constexpr (ON) {
+      const bool there = ahead < rows;
 #pragma unroll
       for (int op = 0; op < OPS; ++op) {
-        if (op < ops && base[op] && r < rows) {
-          const T* src = base[op] + r * pitch[op];
+        if (op < ops) {
+          const T* src = base[op] ? base[op] + ahead * pitch[op] + first * N : nullptr;
 #pragma unroll
           for (int i = 0; i < VPT; ++i) {
-            const int c = int(threadIdx.x) % TPR + i * TPR;
-            if (c * N < width)
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(at(op, i))), "l"(src + c * N) : "memory");
+            const bool on = src && there && (first + i * TPR) * N < width;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(mine + (op * SLOTS * VPT + i) * TB + slot * (VPT * TB))),
+                         "l"(on ? src + i * (TPR * N) : base[0]), "r"(on ? 16 : 0)
+                         : "memory");
           }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
+      slot = slot + 1 == SLOTS ? 0 : slot + 1;
     }
+    ahead += step;
   }
-  __device__ __forceinline__ void start(long long first, long long step) {
-    if constexpr (ON) {
-      for (int s = 0; s < NS; ++s) {
-        request(first + s * step);
-        slot = slot + 1 == NS ? 0 : slot + 1;
-      }
-    }
+  __device__ __forceinline__ void start(uint4* shared, long long first_row, long long rows_apart) {
+    mine = shared + threadIdx.x;
+    first = int(threadIdx.x) % TPR;
+    row = ahead = first_row;
+    step = rows_apart;
+    slot = 0;
+    if constexpr (ON)
+      for (int s = 0; s < NS; ++s) request();
   }
-  __device__ __forceinline__ void wait(long long r) {
-    row = r;
+  __device__ __forceinline__ void wait() {
     if constexpr (ON) asm volatile("cp.async.wait_group %0;" ::"n"(NS > 0 ? NS - 1 : 0) : "memory");
   }
   __device__ __forceinline__ uint4 get(int op, int i) const {
-    const int c = int(threadIdx.x) % TPR + i * TPR;
-    if constexpr (ON) return base[op] && row < rows && c * N < width ? *at(op, i) : make_uint4(0, 0, 0, 0);
-    else return rv_load<T, VEC>(base[op] + row * pitch[op], c, base[op] && row < rows ? width : 0);
+    if constexpr (ON) return mine[(op * SLOTS * VPT + i) * TB + slot * (VPT * TB)];
+    else return rv_load<T, VEC>(base[op] + row * pitch[op], first + i * TPR, base[op] && row < rows ? width : 0);
   }
-  __device__ __forceinline__ void next(long long ahead) {
-    if constexpr (ON) {
-      request(ahead);
-      slot = slot + 1 == NS ? 0 : slot + 1;
-    }
+  // no copy may be on its way when the block ends
+  __device__ __forceinline__ void drain() {
+    if constexpr (ON) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
+  // this row has been read
+  __device__ __forceinline__ void next() {
+    request();
+    row += step;
   }
 };
 
