@@ -25,8 +25,15 @@ class RMSNorm(nn.Module):
         self.weight.sequence_parallel_grad = sequence_parallel
         self.weight.no_weight_decay = True
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, gate: Optional[torch.Tensor] = None, norm_before_gate: bool = True) -> torch.Tensor:
+        """``gate``: the SiLU-gated form of a mixer's output norm (:func:`cppmega_b200.ops.functional.rmsnorm_gated`)."""
+        if gate is not None:
+            return F_.rmsnorm_gated(x, self.weight, gate, self.eps, None, norm_before_gate)
         return F_.rmsnorm(x, self.weight, self.eps)
+
+
+def _hooked(m: nn.Module) -> bool:
+    return bool(m._forward_pre_hooks or m._forward_hooks or m._backward_hooks or m._backward_pre_hooks)
 
 
 class DenseMLP(nn.Module):
@@ -35,6 +42,7 @@ class DenseMLP(nn.Module):
     def __init__(self, hidden: int, ffn: int, pc: ParallelContext, *, std: float, out_std: float,
                  dtype=torch.float32, name: str = "mlp", seed: int = 1234):
         super().__init__()
+        self.pc = pc
         self.linear_fc1 = ColumnParallelLinear(hidden, 2 * ffn, pc, std=std, dtype=dtype,
                                                seed=seed_for(name + ".linear_fc1", seed),
                                                partition_sizes=[ffn, ffn], name=name + ".linear_fc1")
@@ -42,6 +50,10 @@ class DenseMLP(nn.Module):
                                             seed=seed_for(name + ".linear_fc2", seed), name=name + ".linear_fc2")
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        # as one operator where the two linears are plain products: no tensor parallelism, and nothing hooked to them (a precision
+        # rule or a probe on one of them wants its calls)
+        if self.pc.tp == 1 and not (_hooked(self.linear_fc1) or _hooked(self.linear_fc2)):
+            return F_.gated_mlp(x, self.linear_fc1.weight, self.linear_fc2.weight)
         return self.linear_fc2(F_.swiglu(self.linear_fc1(x)))
 
 

@@ -40,9 +40,8 @@ class SharedMTPBlock(nn.Module):
         h = F_.rmsnorm(x, self.ln1, self.eps)
         qkv = F_.linear(h, self.qkv.weight).reshape(B, S, 3, self.heads, self.head_dim)
         o = F_.causal_attention(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], self.head_dim ** -0.5)
-        x = x + F_.linear(o.reshape(B, S, H), self.out_proj.weight)
-        h = F_.rmsnorm(x, self.ln2, self.eps)
-        return x + F_.linear(F_.swiglu(F_.linear(h, self.gate_up.weight)), self.down.weight)
+        h, x = F_.residual_rmsnorm(F_.linear(o.reshape(B, S, H), self.out_proj.weight), x, self.ln2, eps=self.eps)
+        return x + F_.gated_mlp(h, self.gate_up.weight, self.down.weight)
 
 
 class FastMTPHead(nn.Module):

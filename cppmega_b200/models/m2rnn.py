@@ -80,6 +80,5 @@ class M2RNNMixer(nn.Module):
         y = F_.m2rnn_scan(q, k, v, self.state_weight, f)                                       # [B,S,H,V]
         if self.D is not None:
             y = y + v * self.D
-        y = y.flatten(-2, -1) * F.silu(g)
-        y = self.g_norm(y)
+        y = self.g_norm(y.flatten(-2, -1), gate=g, norm_before_gate=False)                     # g is read in place from proj
         return F_.linear(y, self.output_projection.weight)

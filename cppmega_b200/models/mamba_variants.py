@@ -125,7 +125,7 @@ class SSDMixer(nn.Module):
             Cm, Bm, xs.reshape(B_, S, H, P), ADT, DTt, trap_t, self.C_bias if v.bc_bias else zeros,
             self.B_bias if v.bc_bias else zeros, ones, None, ones, angles, self.D, None,
             self.cfg.mamba3.rotary_dim_divisor, max(self.cfg.mamba3.chunk_size, 32))
-        y = self.norm(y.reshape(B_, S, self.d_inner).to(x.dtype)) * F.silu(z)
+        y = self.norm(y.reshape(B_, S, self.d_inner).to(x.dtype), gate=z)
         return self.out_proj(y)
 
 

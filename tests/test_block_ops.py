@@ -102,3 +102,42 @@ def test_kernel_entry_points_refuse():
     assert L.cm_rmsnorm_gated_fwd(16, 8, None, 0, 16, 16, None, 2, 8, 3, 0, 1e-5, 0, None) == -10     # groups that do not divide
     assert L.cm_rmsnorm_gated_fwd(16, 8, None, 0, 16, 16, None, 2, 8, 0, 0, 1e-5, 0, None) == -10
     assert L.cm_rmsnorm_gated_fwd(16, 8, None, 0, 16, 16, None, 0, 8, 8, 0, 1e-5, 0, None) == 0
+
+
+def _mlp(tp_hook=None):
+    from cppmega_b200.models.common import DenseMLP
+    from cppmega_b200.parallel.state import single_process_context
+    m = DenseMLP(32, 48, single_process_context(), std=0.1, out_std=0.1, dtype=torch.float32, seed=3)
+    return m
+
+
+def test_dense_mlp_is_the_operator_and_heeds_hooks():
+    m, x = _mlp(), _r(2, 5, 32).float()
+    want = m.linear_fc2(F_.swiglu(m.linear_fc1(x)))
+    assert torch.equal(m(x), want)
+    seen = []
+    for child in (m.linear_fc1, m.linear_fc2):
+        hook = child.register_forward_hook(lambda mod, args, out: seen.append(mod))
+        assert torch.equal(m(x), want) and seen[-1] is child
+        hook.remove()
+    n = len(seen)
+    m(x)
+    assert len(seen) == n
+
+
+def test_dense_mlp_under_a_recipe_stays_two_linears(monkeypatch):
+    m, x = _mlp(), _r(2, 5, 32).float()
+    calls = []
+    plain = F_.linear
+    monkeypatch.setattr(F_, "linear", lambda a, w: (calls.append(F_.precision_recipe()), plain(a, w))[1])
+    with F_.precision_scope("mxfp8"):
+        m(x)
+    assert calls == ["mxfp8", "mxfp8"]
+
+
+def test_norm_module_with_a_gate():
+    from cppmega_b200.models.common import RMSNorm
+    m, x, z = RMSNorm(24), _r(3, 24).float(), _r(3, 24, seed=1).float()
+    silu = z * torch.sigmoid(z)
+    assert torch.allclose(m(x, gate=z), m(x) * silu, rtol=1e-5, atol=1e-6)
+    assert torch.allclose(m(x, gate=z, norm_before_gate=False), m(x * silu), rtol=1e-5, atol=1e-6)
