@@ -2,7 +2,7 @@
 //   gate_up_kernel    one product with both projections: a tile of 256 tokens holds the same columns of gate and up side by side in
 //                     TMEM, the epilogue forms h = act(g) u from the fp32 accumulators and stores h and, for training, g and u.
 //   gate_grad_kernel  dh = dy W2 stays in TMEM; the epilogue reads g and u and stores dg = dh u act'(g), du = dh act(g).
-// The other products (h W2^T, [dg du] w1, [dg du]^T x, dy^T h) are the dense ones of gemm_pair.cu.  Against linear, activation, linear
+// The other products (h W2^T, [dg du] w1, [dg du]^T x, dy^T h) are dense ones, with the last wave shared (gemm_split.cu).  Against linear, activation, linear
 // this saves writing and reading dh, reading [g u] in the forward, and two launches.
 //
 // Both kernels are the 256 x 256 x 64 tcgen05.mma.cta_group::2 pipeline of gemm_pair.cu (6 stages of 32 KB, two accumulators in TMEM,
@@ -13,10 +13,8 @@
 // Few tokens (serving): both products read their weights once through few_rows.cu; the sums of the first one's partial tiles, the
 // activation and the product are one small kernel, the sums of the second another.
 #include "few_rows.cuh"
-#include "gemm_pair.cuh"
-
-extern "C" int cm_gemm_bf16(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc,
-                            int a_mn, int b_mn, int out_fp32, int accumulate, int* err, cudaStream_t stream);
+#include "gemm_split.cuh"
+#include "pair_issue.cuh"
 
 namespace cm {
 namespace mlp {
@@ -46,21 +44,6 @@ struct Args {
   int save;               // forward: store g and u
   int* err;
 };
-
-__device__ __forceinline__ void mma_2cta(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
-      "}\n" ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void bulk_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
-               "r"(smem_u32(src)), "r"(c0), "r"(c1)
-               : "memory");
-}
 
 // act(g), and its slope.  exp and the division are the fast ones: their errors (a few 2^-22) vanish in the bf16 results.
 template <int ACT>
@@ -498,7 +481,8 @@ using namespace cm;
 
 // Floats of work space that the forward needs; 0: none.
 extern "C" long long cm_gated_mlp_fwd_ws(int M, int H, int F, int Ho) {
-  if (M <= 0 || !mlp::few_tokens(M, F)) return 0;
+  if (M <= 0) return 0;
+  if (!mlp::few_tokens(M, F)) return split::plan(sm_count(), M, Ho, F, false).floats;
   const long long a = few::cut_for(M, 2 * F, H).floats(), b = few::cut_for(M, Ho, F).floats();
   return a > b ? a : b;
 }
@@ -527,14 +511,23 @@ extern "C" int cm_gated_mlp_fwd(const void* x, long long ldx, const void* w1, co
   if (rc) return rc;
   rc = mlp::launch_act<false>(act, maps, args, stream);
   if (rc) return rc;
-  return cm_gemm_bf16(h, w2, y, M, Ho, F, F, F, Ho, 0, 0, 0, 0, err, stream);
+  return split::gemm(h, w2, y, M, Ho, F, F, F, Ho, false, false, false, false, ws, err, stream);
+}
+
+// Floats of work space that the backward needs; 0: none.
+extern "C" long long cm_gated_mlp_bwd_ws(int M, int H, int F, int Ho) {
+  if (M <= 0) return 0;
+  const int sms = sm_count();
+  const long long n[3] = {split::plan(sms, M, H, 2 * F, true).floats, split::plan(sms, 2 * F, H, M, true).floats,
+                          split::plan(sms, Ho, F, M, true).floats};
+  return n[0] > n[1] ? (n[0] > n[2] ? n[0] : n[2]) : (n[1] > n[2] ? n[1] : n[2]);
 }
 
 // Gradients from dy [M, Ho] (row pitch lddy): dgu [M, 2F] is work space; dx [M, H], dw1, dw2 may be null.  dw1 / dw2: fp32 or bf16
-// (dw*_fp32), added to what is there with acc*.
+// (dw*_fp32), added to what is there with acc*.  ws: cm_gated_mlp_bwd_ws floats of work space.
 extern "C" int cm_gated_mlp_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w1, const void* w2, const void* gu,
                                 const void* h, void* dgu, void* dx, void* dw1, int dw1_fp32, int acc1, void* dw2, int dw2_fp32, int acc2,
-                                int M, int H, int F, int Ho, int act, int* err, cudaStream_t stream) {
+                                float* ws, int M, int H, int F, int Ho, int act, int* err, cudaStream_t stream) {
   if (M <= 0 || H <= 0 || F <= 0 || Ho <= 0) return 0;
   if (H % 8 || F % 8 || Ho % 8 || !mlp::tma_ok(dy, lddy) || !mlp::tma_ok(x, ldx) || !mlp::tma_ok(w1, H) || !mlp::tma_ok(w2, F) ||
       !mlp::tma_ok(gu, 0) || !mlp::tma_ok(h, F) || !mlp::tma_ok(dgu, 0))
@@ -549,9 +542,9 @@ extern "C" int cm_gated_mlp_bwd(const void* dy, long long lddy, const void* x, l
     if (!rc) rc = mlp::make_out_map(&maps[4], static_cast<__nv_bfloat16*>(dgu) + F, M, F, 2ll * F);
     maps[2] = maps[3];
     if (!rc) rc = mlp::launch_act<true>(act, maps, args, stream);
-    if (!rc && dx) rc = cm_gemm_bf16(dgu, w1, dx, M, H, 2 * F, 2ll * F, H, H, 0, 1, 0, 0, err, stream);
-    if (!rc && dw1) rc = cm_gemm_bf16(dgu, x, dw1, 2 * F, H, M, 2ll * F, ldx, H, 1, 1, dw1_fp32, acc1, err, stream);
+    if (!rc && dx) rc = split::gemm(dgu, w1, dx, M, H, 2 * F, 2ll * F, H, H, false, true, false, false, ws, err, stream);
+    if (!rc && dw1) rc = split::gemm(dgu, x, dw1, 2 * F, H, M, 2ll * F, ldx, H, true, true, dw1_fp32, acc1, ws, err, stream);
   }
-  if (!rc && dw2) rc = cm_gemm_bf16(dy, h, dw2, Ho, F, M, lddy, F, F, 1, 1, dw2_fp32, acc2, err, stream);
+  if (!rc && dw2) rc = split::gemm(dy, h, dw2, Ho, F, M, lddy, F, F, true, true, dw2_fp32, acc2, ws, err, stream);
   return rc;
 }

@@ -24,7 +24,8 @@ def declare(L: ctypes.CDLL) -> None:
     vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
     sig = {
         "cm_gated_mlp_fwd": [vp, i64, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp],
-        "cm_gated_mlp_bwd": [vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp],
+        "cm_gated_mlp_bwd": [vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp, i32, i32, vp, i32, i32, i32, i32, i32, vp, vp],
+        "cm_gemm_split": [vp, vp, vp, i32, i32, i32, i64, i64, i64, i32, i32, i32, i32, vp, vp, vp],
         "cm_residual_rmsnorm_fwd": [vp, i64, vp, i64, vp, vp, vp, i32, vp, vp, vp, vp, i64, i32, f32, f32, i32, vp],
         "cm_residual_rmsnorm_parts": [i64, i32],
         "cm_rmsnorm_gated_parts": [i64, i32, i32],
@@ -38,8 +39,9 @@ def declare(L: ctypes.CDLL) -> None:
         if fn is not None:
             fn.argtypes = args
             fn.restype = i32
-    if hasattr(L, "cm_gated_mlp_fwd_ws"):
-        L.cm_gated_mlp_fwd_ws.argtypes, L.cm_gated_mlp_fwd_ws.restype = [i32, i32, i32, i32], i64
+    for name, args in (("cm_gated_mlp_fwd_ws", [i32] * 4), ("cm_gated_mlp_bwd_ws", [i32] * 4), ("cm_gemm_split_plan", [i32] * 5 + [vp])):
+        if hasattr(L, name):
+            getattr(L, name).argtypes, getattr(L, name).restype = args, i64
 
 
 def _failed(name: str, rc: int) -> None:
@@ -143,9 +145,12 @@ class GatedMLPFn(torch.autograd.Function):
         dw1 = _cu.wgrad_into_main_grad(w1, target(0, w1)) if need_w1 else None
         dw2 = _cu.wgrad_into_main_grad(w2, target(1, w2)) if need_w2 else None
         dgu = torch.empty_like(gu) if need_x or need_w1 else None
-        rc = _cu.lib().cm_gated_mlp_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), gu.data_ptr(), h.data_ptr(),
-                                        _ptr(dgu), _ptr(dx), *into[0], *into[1], h.shape[0], H, F, Ho, ctx.act,
-                                        _cu.err_word(x.device).data_ptr(), _cu.stream_ptr())
+        L, M = _cu.lib(), h.shape[0]
+        floats = L.cm_gated_mlp_bwd_ws(M, H, F, Ho)
+        ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
+        rc = L.cm_gated_mlp_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), gu.data_ptr(), h.data_ptr(),
+                                _ptr(dgu), _ptr(dx), *into[0], *into[1], _ptr(ws), M, H, F, Ho, ctx.act,
+                                _cu.err_word(x.device).data_ptr(), _cu.stream_ptr())
         if rc:
             _failed("cm_gated_mlp_bwd", rc)
         F_.count_launch("gated_mlp_bwd")

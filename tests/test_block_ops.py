@@ -104,7 +104,39 @@ def test_kernel_entry_points_refuse():
     assert L.cm_rmsnorm_gated_fwd(16, 8, None, 0, 16, 16, None, 0, 8, 8, 0, 1e-5, 0, None) == 0
 
 
-def _mlp(tp_hook=None):
+@pytest.mark.parametrize("M,N,K,b_mn", [(4095, 3584, 18944, 0), (4095, 3584, 37888, 1), (512, 1024, 2048, 0), (512, 1024, 4096, 1), (300, 136, 1032, 0),
+                                        (16384, 4096, 21504, 0), (1, 8, 8, 0), (2064, 72, 300, 1), (257, 4096, 4096, 1), (20000, 264, 512, 0),
+                                        (4096, 1024, 512, 1), (43008, 4096, 16384, 1), (700, 1000, 20000, 1)])
+def test_split_plan(M, N, K, b_mn):
+    """Every row and every k block is worked on once, by runs that are not empty, and no wave of runs is left over."""
+    import ctypes
+    from cppmega_b200.ops.cuda import lib
+    L = lib()
+    out = (ctypes.c_int * 4)()
+    floats = L.cm_gemm_split_plan(148, M, N, K, b_mn, out)
+    whole, bn, slices, per = out
+    if slices == 0:
+        assert (whole, floats) == (M, 0)
+        return
+    nkb = -(-K // 64)
+    assert 0 <= whole < M and whole % 256 == 0 and bn in (128, 256) and slices >= 2
+    assert slices * per >= nkb > (slices - 1) * per
+    assert -(-(M - whole) // 256) * -(-N // bn) * slices <= 74
+    assert floats == slices * (M - whole) * N
+
+
+def test_split_plan_takes_the_products_it_is_for():
+    import ctypes
+    from cppmega_b200.ops.cuda import lib
+    out = (ctypes.c_int * 4)()
+    took = []
+    for args in ((4095, 3584, 18944, 0), (512, 1024, 4096, 1), (16384, 4096, 21504, 0)):
+        lib().cm_gemm_split_plan(148, *args, out)
+        took.append(out[2] > 0)
+    assert took == [True, True, False]
+
+
+def _mlp():
     from cppmega_b200.models.common import DenseMLP
     from cppmega_b200.parallel.state import single_process_context
     m = DenseMLP(32, 48, single_process_context(), std=0.1, out_std=0.1, dtype=torch.float32, seed=3)

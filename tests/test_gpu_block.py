@@ -289,6 +289,33 @@ def test_rmsnorm_gated_large_gates():
     assert (y[:, [0, 1, 2]] == 0).all() and (dz[:, [0, 1, 2]] == 0).all()
 
 
+# ---- dense products with shared last tiles --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("a_mn,b_mn", [(False, False), (False, True), (True, True), (True, False)])
+@pytest.mark.parametrize("M,N,K", [(512, 1024, 4096), (300, 136, 1032), (2064, 520, 8200), (5000, 1032, 4104), (256, 256, 16384), (40, 8, 2000)])
+@pytest.mark.parametrize("fp32,accumulate", [(False, False), (True, True), (False, True)])
+def test_gemm_split(a_mn, b_mn, M, N, K, fp32, accumulate):
+    import ctypes
+    from cppmega_b200.ops import cuda as cu
+    L = cu.lib()
+    a, b = _randn(*((K, M) if a_mn else (M, K))), _randn(*((K, N) if b_mn else (N, K)), seed=1)
+    if a_mn and M % 8:
+        pytest.skip("rows of 16 bytes")
+    c0 = _randn(M, N, dtype=torch.float32 if fp32 else torch.bfloat16, seed=2)
+    plan = (ctypes.c_int * 4)()
+    floats = L.cm_gemm_split_plan(torch.cuda.get_device_properties(0).multi_processor_count, M, N, K, int(b_mn), plan)
+    ws = torch.full((max(floats, 1),), float("nan"), dtype=torch.float32, device="cuda")
+    c = c0.clone()
+    rc = L.cm_gemm_split(a.data_ptr(), b.data_ptr(), c.data_ptr(), M, N, K, a.stride(0), b.stride(0), N, int(a_mn), int(b_mn), int(fp32),
+                         int(accumulate), ws.data_ptr(), cu.err_word().data_ptr(), cu.stream_ptr())
+    assert rc == 0
+    _check_errors()
+    x, y = (a.t() if a_mn else a).double(), (b if b_mn else b.t()).double()
+    want = x @ y + (c0.double() if accumulate else 0)
+    size = x.abs() @ y.abs() + c0.double().abs()
+    _within(c, want, (0 if fp32 else 2 ** -8) * want.abs() + (64 + K) * E32 * size, "C")
+
+
 # ---- gated feed-forward -----------------------------------------------------------------------------------------------
 
 @torch.enable_grad()
