@@ -12,6 +12,8 @@
 //
 // Few tokens (serving): both products read their weights once through few_rows.cu; the sums of the first one's partial tiles, the
 // activation and the product are one small kernel, the sums of the second another.
+#include <cuda_fp16.h>
+
 #include "few_rows.cuh"
 #include "gemm_split.cuh"
 #include "pair_issue.cuh"
@@ -37,11 +39,29 @@ constexpr int SMEM_TOTAL = BAR_OFF + 256 + 1024;
 
 enum Act : int { SILU = 0, GELU_TANH = 1, RELU = 2 };
 
+// g and u are kept for the backward as 16-bit floats of 11 bits under one power of two per row and 32 columns: as bf16 they would bring a
+// third rounding of 2^-9 into dx and dw1, next to those of the products' operands and of the results (3.0e-3 against 2.4e-3 of the
+// gradients' norm).  The largest value of a group lies in [2^14, 2^15); what is 2^29 times smaller loses bits, and nothing overflows.
+//   kept = [M][2F] fp16 (g, then u), then [2][groups][M] bytes: the exponent field of the power that the values were multiplied with
+struct Kept {
+  __half* v;
+  uint8_t* power;
+  long long plane;        // bytes between the powers of g and of u
+  __host__ __device__ static long long groups(int F) { return (F + 31) / 32; }
+  __host__ __device__ static long long bytes(long long M, int F) { return 4 * M * F + 2 * groups(F) * M; }
+  __host__ static Kept at(void* p, long long M, int F) {
+    return Kept{static_cast<__half*>(p), static_cast<uint8_t*>(p) + 4 * M * F, groups(F) * M};
+  }
+};
+// exponent field of the power for a group whose largest magnitude is m; 253 at most, so that its inverse is a normal number
+__device__ __forceinline__ uint32_t power_for(float m) { return min(268u - (__float_as_uint(m) >> 23), 253u); }
+__device__ __forceinline__ float power_of(uint32_t field) { return __uint_as_float(field << 23); }
+__device__ __forceinline__ float inverse_power(uint32_t field) { return __uint_as_float((254u - field) << 23); }
+
 struct Args {
   int M, F, K;            // tokens, ffn columns, reduction (hidden)
   int bn;                 // accumulator columns of a tile: 256 or 128
-  const __nv_bfloat16* gu;   // backward: saved [g | u], rows of 2F
-  int save;               // forward: store g and u
+  Kept kept;              // v null: not kept
   int* err;
 };
 
@@ -226,8 +246,14 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
       place(tile, m0, n0);
       const int row0 = m0 + rank * BM + q * 32, row = row0 + lane;
       uint4 gv[4], uv[4];
+      uint32_t gp = 127, up = 127;
       auto fetch = [&](int c) {                                 // g and u of 32 columns: requested ahead of their use
-        const __nv_bfloat16* p = args.gu + (long long)row * 2 * args.F + n0 + c;
+        const __half* p = args.kept.v + (long long)row * 2 * args.F + n0 + c;
+        if (row < args.M && n0 + c < args.F) {
+          const uint8_t* e = args.kept.power + (long long)((n0 + c) >> 5) * args.M + row;
+          gp = e[0];
+          up = e[args.kept.plane];
+        }
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           const bool on = row < args.M && n0 + c + 8 * v < args.F;
@@ -248,13 +274,29 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             tmem_ld_32x32(t_base + half + c, u);
             tmem_ld_wait();
             uint32_t o[16];
-            if (args.save) {
+            if (args.kept.v) {
+              auto keep = [&](const uint32_t (&v)[32], const CUtensorMap* map, uint8_t* power) {
+                float m = 0.f;
+                if (n0 + c + 32 <= args.F) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = pack_bf16(__uint_as_float(g[2 * j]), __uint_as_float(g[2 * j + 1]));
-              out.put(&tmO1, o, n0 + c, row0);
+                  for (int j = 0; j < 32; ++j) m = fmaxf(m, fabsf(__uint_as_float(v[j])));
+                } else {                                        // the gate's columns past the last are up's first rows: not of this group
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = pack_bf16(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
-              out.put(&tmO2, o, n0 + c, row0);
+                  for (int j = 0; j < 32; ++j)
+                    if (n0 + c + j < args.F) m = fmaxf(m, fabsf(__uint_as_float(v[j])));
+                }
+                const uint32_t field = power_for(m);
+                const float k = power_of(field);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  const __half2 p = __floats2half2_rn(__uint_as_float(v[2 * j]) * k, __uint_as_float(v[2 * j + 1]) * k);
+                  o[j] = *reinterpret_cast<const uint32_t*>(&p);
+                }
+                out.put(map, o, n0 + c, row0);
+                if (row < args.M) power[(long long)((n0 + c) >> 5) * args.M + row] = uint8_t(field);
+              };
+              keep(g, &tmO1, args.kept.power);
+              keep(u, &tmO2, args.kept.power + args.kept.plane);
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j)
@@ -267,21 +309,22 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             uint4 gc[4], uc[4];
 #pragma unroll
             for (int v = 0; v < 4; ++v) { gc[v] = gv[v]; uc[v] = uv[v]; }
+            const float gi = inverse_power(gp), ui = inverse_power(up);
             if (c + 32 < c_end) fetch(c + 32);
             tmem_ld_wait();
             uint32_t og[16], ou[16];
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-              const __nv_bfloat162* gb = reinterpret_cast<const __nv_bfloat162*>(&gc[v]);
-              const __nv_bfloat162* ub = reinterpret_cast<const __nv_bfloat162*>(&uc[v]);
+              const __half2* gb = reinterpret_cast<const __half2*>(&gc[v]);
+              const __half2* ub = reinterpret_cast<const __half2*>(&uc[v]);
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const float2 g = __bfloat1622float2(gb[j]), u = __bfloat1622float2(ub[j]);
+                const float2 g = __half22float2(gb[j]), u = __half22float2(ub[j]);
                 float a0, s0, a1, s1;
-                act_slope<ACT>(g.x, a0, s0);
-                act_slope<ACT>(g.y, a1, s1);
+                act_slope<ACT>(g.x * gi, a0, s0);
+                act_slope<ACT>(g.y * gi, a1, s1);
                 const float d0 = __uint_as_float(d[8 * v + 2 * j]), d1 = __uint_as_float(d[8 * v + 2 * j + 1]);
-                og[4 * v + j] = pack_bf16(d0 * u.x * s0, d1 * u.y * s1);
+                og[4 * v + j] = pack_bf16(d0 * (u.x * ui) * s0, d1 * (u.y * ui) * s1);
                 ou[4 * v + j] = pack_bf16(d0 * a0, d1 * a1);
               }
             }
@@ -410,9 +453,9 @@ static int few_share(const few::Cut& c) {
 // h[token][f] = act(g) u from rows f and F + f of the first product; g, u kept for training.
 template <int ACT>
 __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_gate_kernel(const float* __restrict__ part, const few::Cut cut, int F,
-                                                                         __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ gu) {
+                                                                         __nv_bfloat16* __restrict__ h, const Kept kept) {
   __shared__ FewSums share;
-  const int f = min(int(blockIdx.x * few::TILE + threadIdx.x), F - 1), tok0 = blockIdx.y * TOKS;       // the last block repeats its last row
+  const int col = blockIdx.x * few::TILE + threadIdx.x, f = min(col, F - 1), tok0 = blockIdx.y * TOKS;   // past the last column: repeats it
   few::wait_for_input();
   few::let_next_start();
   float g[TOKS], u[TOKS];
@@ -424,10 +467,18 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_gate_kernel(const f
   for (int j = 0; j < TOKS; ++j) {
     const long long tok = tok0 + j;
     if (tok >= cut.tokens) break;
-    h[tok * F + f] = __float2bfloat16(act_of<ACT>(g[j]) * u[j]);
-    if (gu) {
-      gu[tok * 2 * F + f] = __float2bfloat16(g[j]);
-      gu[tok * 2 * F + F + f] = __float2bfloat16(u[j]);
+    if (col < F) h[tok * F + f] = __float2bfloat16(act_of<ACT>(g[j]) * u[j]);
+    if (kept.v) {                             // a warp holds a group of 32 columns
+      const uint32_t gp = power_for(warp_max(fabsf(g[j]))), up = power_for(warp_max(fabsf(u[j])));
+      if (col < F) {
+        kept.v[tok * 2 * F + f] = __float2half_rn(g[j] * power_of(gp));
+        kept.v[tok * 2 * F + F + f] = __float2half_rn(u[j] * power_of(up));
+      }
+      if ((threadIdx.x & 31) == 0 && col < F) {
+        uint8_t* e = kept.power + (long long)(f >> 5) * cut.tokens + tok;
+        e[0] = uint8_t(gp);
+        e[kept.plane] = uint8_t(up);
+      }
     }
   }
 }
@@ -435,11 +486,11 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_gate_kernel(const f
 __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_sum_kernel(const float* __restrict__ part, const few::Cut cut, int N,
                                                                         __nv_bfloat16* __restrict__ y) {
   __shared__ FewSums share;
-  const int n = min(int(blockIdx.x * few::TILE + threadIdx.x), N - 1), tok0 = blockIdx.y * TOKS;
+  const int col = blockIdx.x * few::TILE + threadIdx.x, n = min(col, N - 1), tok0 = blockIdx.y * TOKS;
   few::wait_for_input();
   float s[TOKS];
   few_sum(part, cut, n, tok0, &share, s);
-  if (threadIdx.y > 0) return;
+  if (threadIdx.y > 0 || col >= N) return;
 #pragma unroll
   for (int j = 0; j < TOKS; ++j)
     if (tok0 + j < cut.tokens) y[(long long)(tok0 + j) * N + n] = __float2bfloat16(s[j]);
@@ -454,16 +505,16 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_sum_kernel(const fl
 // A long ffn leaves the second product of the tiles few of them, each with a long reduction.
 static bool few_tokens(int M, int F) { return M <= (F >= 8192 ? 192 : 64); }
 
-static int few_forward(const void* x, long long ldx, const void* w1, const void* w2, __nv_bfloat16* gu, __nv_bfloat16* h, __nv_bfloat16* y,
+static int few_forward(const void* x, long long ldx, const void* w1, const void* w2, const Kept& kept, __nv_bfloat16* h, __nv_bfloat16* y,
                        float* ws, int M, int H, int F, int Ho, int act, int* err, cudaStream_t stream) {
   const few::Cut c1 = few::cut_for(M, 2 * F, H), c2 = few::cut_for(M, Ho, F);
   int rc = few::launch_partials(x, ldx, w1, ws, c1, 2 * F, H, false, err, stream);
   if (rc) return rc;
   const dim3 grid((F + few::TILE - 1) / few::TILE, (M + TOKS - 1) / TOKS), block(few::TILE, few_share(c1));
   switch (act) {
-    case SILU: rc = few::launch_early(few_gate_kernel<SILU>, grid, block, 0, stream, ws, c1, F, h, gu); break;
-    case GELU_TANH: rc = few::launch_early(few_gate_kernel<GELU_TANH>, grid, block, 0, stream, ws, c1, F, h, gu); break;
-    case RELU: rc = few::launch_early(few_gate_kernel<RELU>, grid, block, 0, stream, ws, c1, F, h, gu); break;
+    case SILU: rc = few::launch_early(few_gate_kernel<SILU>, grid, block, 0, stream, ws, c1, F, h, kept); break;
+    case GELU_TANH: rc = few::launch_early(few_gate_kernel<GELU_TANH>, grid, block, 0, stream, ws, c1, F, h, kept); break;
+    case RELU: rc = few::launch_early(few_gate_kernel<RELU>, grid, block, 0, stream, ws, c1, F, h, kept); break;
     default: rc = -10;
   }
   if (!rc) rc = few::launch_partials(h, F, w2, ws, c2, Ho, F, true, err, stream);
@@ -479,6 +530,9 @@ static bool tma_ok(const void* p, long long ld) { return (reinterpret_cast<uintp
 
 using namespace cm;
 
+// Bytes that the forward keeps for the backward beside x and h.
+extern "C" long long cm_gated_mlp_kept(int M, int F) { return mlp::Kept::bytes(M, F); }
+
 // Floats of work space that the forward needs; 0: none.
 extern "C" long long cm_gated_mlp_fwd_ws(int M, int H, int F, int Ho) {
   if (M <= 0) return 0;
@@ -487,27 +541,27 @@ extern "C" long long cm_gated_mlp_fwd_ws(int M, int H, int F, int Ho) {
   return a > b ? a : b;
 }
 
-// y[M, Ho] = (act(x w1[:F]^T) * (x w1[F:]^T)) w2^T; x [M, H] with row pitch ldx, w1 [2F, H], w2 [Ho, F], h [M, F]; gu [M, 2F] or null
-// (not kept).  act: 0 silu, 1 gelu (tanh form), 2 relu.  ws: cm_gated_mlp_fwd_ws floats of work space.
-extern "C" int cm_gated_mlp_fwd(const void* x, long long ldx, const void* w1, const void* w2, void* gu, void* h, void* y, float* ws, int M,
+// y[M, Ho] = (act(x w1[:F]^T) * (x w1[F:]^T)) w2^T; x [M, H] with row pitch ldx, w1 [2F, H], w2 [Ho, F], h [M, F]; kept: cm_gated_mlp_kept
+// bytes, or null.  act: 0 silu, 1 gelu (tanh form), 2 relu.  ws: cm_gated_mlp_fwd_ws floats of work space.
+extern "C" int cm_gated_mlp_fwd(const void* x, long long ldx, const void* w1, const void* w2, void* kept, void* h, void* y, float* ws, int M,
                                 int H, int F, int Ho, int act, int* err, cudaStream_t stream) {
   if (M <= 0 || H <= 0 || F <= 0 || Ho <= 0) return 0;
-  if (H % 8 || F % 8 || Ho % 8 || !mlp::tma_ok(x, ldx) || !mlp::tma_ok(w1, H) || !mlp::tma_ok(w2, F) || !mlp::tma_ok(gu, 0) ||
+  if (H % 8 || F % 8 || Ho % 8 || !mlp::tma_ok(x, ldx) || !mlp::tma_ok(w1, H) || !mlp::tma_ok(w2, F) || !mlp::tma_ok(kept, 0) ||
       !mlp::tma_ok(h, F) || !mlp::tma_ok(y, Ho))
     return -10;
+  const mlp::Kept k = kept ? mlp::Kept::at(kept, M, F) : mlp::Kept{};
   if (mlp::few_tokens(M, F)) {
     if (!ws) return -10;
-    return mlp::few_forward(x, ldx, w1, w2, static_cast<__nv_bfloat16*>(gu), static_cast<__nv_bfloat16*>(h), static_cast<__nv_bfloat16*>(y), ws,
-                            M, H, F, Ho, act, err, stream);
+    return mlp::few_forward(x, ldx, w1, w2, k, static_cast<__nv_bfloat16*>(h), static_cast<__nv_bfloat16*>(y), ws, M, H, F, Ho, act, err, stream);
   }
-  mlp::Args args{M, F, H, mlp::plan_bn(M, F, false), nullptr, gu != nullptr, err};
+  mlp::Args args{M, F, H, mlp::plan_bn(M, F, false), k, err};
   CUtensorMap maps[5];
   int rc = make_tmap_2d_bf16(&maps[0], x, M, H, ldx, mlp::BM);
   if (!rc) rc = make_tmap_2d_bf16(&maps[1], w1, 2ll * F, H, H, args.bn / 2);
   if (!rc) rc = mlp::make_out_map(&maps[2], h, M, F, F);
   maps[3] = maps[4] = maps[2];
-  if (!rc && gu) rc = mlp::make_out_map(&maps[3], gu, M, F, 2ll * F);
-  if (!rc && gu) rc = mlp::make_out_map(&maps[4], static_cast<__nv_bfloat16*>(gu) + F, M, F, 2ll * F);
+  if (!rc && kept) rc = mlp::make_out_map(&maps[3], k.v, M, F, 2ll * F);
+  if (!rc && kept) rc = mlp::make_out_map(&maps[4], k.v + F, M, F, 2ll * F);
   if (rc) return rc;
   rc = mlp::launch_act<false>(act, maps, args, stream);
   if (rc) return rc;
@@ -525,16 +579,16 @@ extern "C" long long cm_gated_mlp_bwd_ws(int M, int H, int F, int Ho) {
 
 // Gradients from dy [M, Ho] (row pitch lddy): dgu [M, 2F] is work space; dx [M, H], dw1, dw2 may be null.  dw1 / dw2: fp32 or bf16
 // (dw*_fp32), added to what is there with acc*.  ws: cm_gated_mlp_bwd_ws floats of work space.
-extern "C" int cm_gated_mlp_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w1, const void* w2, const void* gu,
+extern "C" int cm_gated_mlp_bwd(const void* dy, long long lddy, const void* x, long long ldx, const void* w1, const void* w2, const void* kept,
                                 const void* h, void* dgu, void* dx, void* dw1, int dw1_fp32, int acc1, void* dw2, int dw2_fp32, int acc2,
                                 float* ws, int M, int H, int F, int Ho, int act, int* err, cudaStream_t stream) {
   if (M <= 0 || H <= 0 || F <= 0 || Ho <= 0) return 0;
   if (H % 8 || F % 8 || Ho % 8 || !mlp::tma_ok(dy, lddy) || !mlp::tma_ok(x, ldx) || !mlp::tma_ok(w1, H) || !mlp::tma_ok(w2, F) ||
-      !mlp::tma_ok(gu, 0) || !mlp::tma_ok(h, F) || !mlp::tma_ok(dgu, 0))
+      !mlp::tma_ok(kept, 0) || !mlp::tma_ok(h, F) || !mlp::tma_ok(dgu, 0))
     return -10;
   int rc = 0;
   if (dx || dw1) {
-    mlp::Args args{M, F, Ho, mlp::plan_bn(M, F, true), static_cast<const __nv_bfloat16*>(gu), 0, err};
+    mlp::Args args{M, F, Ho, mlp::plan_bn(M, F, true), mlp::Kept::at(const_cast<void*>(kept), M, F), err};
     CUtensorMap maps[5];
     rc = make_tmap_2d_bf16(&maps[0], dy, M, Ho, lddy, mlp::BM);
     if (!rc) rc = make_tmap_2d_bf16(&maps[1], w2, Ho, F, F, 64);

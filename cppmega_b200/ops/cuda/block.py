@@ -39,7 +39,8 @@ def declare(L: ctypes.CDLL) -> None:
         if fn is not None:
             fn.argtypes = args
             fn.restype = i32
-    for name, args in (("cm_gated_mlp_fwd_ws", [i32] * 4), ("cm_gated_mlp_bwd_ws", [i32] * 4), ("cm_gemm_split_plan", [i32] * 5 + [vp])):
+    for name, args in (("cm_gated_mlp_fwd_ws", [i32] * 4), ("cm_gated_mlp_bwd_ws", [i32] * 4), ("cm_gemm_split_plan", [i32] * 5 + [vp]),
+                       ("cm_gated_mlp_kept", [i32] * 2)):
         if hasattr(L, name):
             getattr(L, name).argtypes, getattr(L, name).restype = args, i64
 
@@ -105,29 +106,29 @@ def _mlp_forward(x, w1, w2, act, keep):
     M = x.numel() // H
     y = _like(x) if Ho == H else x.new_empty(*x.shape[:-1], Ho)
     h = x.new_empty(M, F)
-    gu = x.new_empty(M, 2 * F) if keep else None
+    kept = torch.empty(L.cm_gated_mlp_kept(M, F), dtype=torch.uint8, device=x.device) if keep else None
     floats = L.cm_gated_mlp_fwd_ws(M, H, F, Ho)
     ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
-    rc = L.cm_gated_mlp_fwd(x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), _ptr(gu), h.data_ptr(), y.data_ptr(), _ptr(ws), M, H, F, Ho,
+    rc = L.cm_gated_mlp_fwd(x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), _ptr(kept), h.data_ptr(), y.data_ptr(), _ptr(ws), M, H, F, Ho,
                             act, _cu.err_word(x.device).data_ptr(), _cu.stream_ptr())
     if rc:
         _failed("cm_gated_mlp_fwd", rc)
     F_.count_launch("gated_mlp")
-    return y, x, gu, h
+    return y, x, kept, h
 
 
 class GatedMLPFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w1, w2, act):
-        y, x, gu, h = _mlp_forward(x, w1, w2, act, keep=True)
-        ctx.save_for_backward(x, w1, w2, gu, h)
+        y, x, kept, h = _mlp_forward(x, w1, w2, act, keep=True)
+        ctx.save_for_backward(x, w1, w2, kept, h)
         ctx.act = act
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, w1, w2, gu, h = ctx.saved_tensors
+        x, w1, w2, kept, h = ctx.saved_tensors
         need_x, need_w1, need_w2, _ = ctx.needs_input_grad
         H, F, Ho = w1.shape[1], w2.shape[1], w2.shape[0]
         dy, lddy = _tma_rows(dy)
@@ -144,11 +145,11 @@ class GatedMLPFn(torch.autograd.Function):
 
         dw1 = _cu.wgrad_into_main_grad(w1, target(0, w1)) if need_w1 else None
         dw2 = _cu.wgrad_into_main_grad(w2, target(1, w2)) if need_w2 else None
-        dgu = torch.empty_like(gu) if need_x or need_w1 else None
+        dgu = x.new_empty(h.shape[0], 2 * F) if need_x or need_w1 else None
         L, M = _cu.lib(), h.shape[0]
         floats = L.cm_gated_mlp_bwd_ws(M, H, F, Ho)
         ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
-        rc = L.cm_gated_mlp_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), gu.data_ptr(), h.data_ptr(),
+        rc = L.cm_gated_mlp_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), kept.data_ptr(), h.data_ptr(),
                                 _ptr(dgu), _ptr(dx), *into[0], *into[1], _ptr(ws), M, H, F, Ho, ctx.act,
                                 _cu.err_word(x.device).data_ptr(), _cu.stream_ptr())
         if rc:

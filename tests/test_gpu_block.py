@@ -355,13 +355,17 @@ def _check_mlp(x, w1, w2, name, y, grads=None, dy=None):
     dy = dy.detach().double().reshape(T, Ho)
     dh = dy @ w2
     e_dh = acc(Ho) * (dy.abs() @ w2.abs())
-    # g and u are kept in bf16: |slope(g') - slope(g)| <= curve u, |a(g') - a(g)| <= 1.2 |g| u
-    e_s = (curve * u + 64 * E32) * torch.ones_like(g) + e_g * 1.2
+    # g and u are kept with 11 bits under a power of two per row and 32 columns: half a step is 2^-11 of the value, or 2^-25 under the
+    # power, which is 2^-39 of the group's largest (bounded here by the row's); |slope(g') - slope(g)| <= curve |g' - g| / |g|
+    k = 2.0 ** -11
+    tiny = lambda t: 2.0 ** -39 * t.abs().amax(1, keepdim=True)  # noqa: E731
+    e_s = (curve * k + 64 * E32) * torch.ones_like(g) + 1.2 * (e_g + tiny(g))
     if name == "relu":
-        e_s = (g.abs() <= e_g).double()                         # a gate whose sign the fp32 sum does not settle
+        e_s = (g.abs() <= e_g + tiny(g)).double()               # a gate whose sign the fp32 sum does not settle
     dg, du = dh * up * slope, dh * a
-    e_dg = e_dh * (up * slope).abs() + dh.abs() * ((u * up.abs() + e_u) * slope.abs() + up.abs() * e_s) + u * dg.abs()
-    e_du = e_dh * a.abs() + dh.abs() * (1.2 * (u * g.abs() + e_g) + 64 * E32 * (a.abs() + g.abs())) + u * du.abs()
+    e_up = k * up.abs() + e_u + tiny(up)
+    e_dg = e_dh * (up * slope).abs() + dh.abs() * (e_up * slope.abs() + (up.abs() + e_up) * e_s) + u * dg.abs()
+    e_du = e_dh * a.abs() + dh.abs() * (1.2 * (k * g.abs() + e_g + tiny(g)) + 64 * E32 * (a.abs() + g.abs())) + u * du.abs()
     dgu, e = torch.cat([dg, du], 1), torch.cat([e_dg, e_du], 1)
     out = {"x": (dgu @ w1, acc(2 * F) * (dgu.abs() @ w1.abs()) + 1.02 * (e @ w1.abs())),
            "w1": (dgu.t() @ x, acc(T) * (dgu.abs().t() @ x.abs()) + 1.02 * (e.t() @ x.abs())),
@@ -440,6 +444,23 @@ def test_gated_mlp_adds_into_main_grad(kind):
     y.backward(dy)
     for p, o in zip(leaves, once):                  # the same products added: exactly twice in fp32, one more rounding in bf16
         _within(p.main_grad, 2 * o.double(), (2 ** -8 if kind == torch.bfloat16 else 2 * E32) * (2 * o.double().abs()) + 1e-6, "main_grad")
+
+
+@pytest.mark.parametrize("T", [40, 300])
+def test_gated_mlp_gradients_of_far_apart_magnitudes(T):
+    """Columns of w1 scaled by up to 2^+-30 and rows of x by 2^+-20: the kept values have one power of two per row and 32 columns."""
+    x, w1, w2 = _mlp_inputs((T,), 64, 136, 64)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = x * torch.exp2(torch.randint(-20, 21, (T, 1), device="cuda", generator=g).float()).bfloat16()
+    rows = torch.exp2(torch.randint(-30, 31, (272, 1), device="cuda", generator=g).float())
+    rows[:136].clamp_(max=2.0 ** -22)               # gates in the range where the activation bends
+    w1 = (w1.float() * rows).bfloat16()
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    dy = _randn(T, 64, std=0.1, seed=9)
+    for name in ("silu", "gelu_tanh"):
+        y = F_.gated_mlp(*leaves, name)
+        grads = torch.autograd.grad(y, leaves, dy)
+        _check_mlp(*leaves, name, y, dict(zip(("x", "w1", "w2"), grads)), dy)
 
 
 def test_gated_mlp_nan_stays_in_its_row():
