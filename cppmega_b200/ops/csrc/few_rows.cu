@@ -22,15 +22,16 @@ struct Args {
   Cut cut;
   int tiles, n_pad, stages, acc_cols, tmem_cols;
   float* part;
-  int early;
+  int early, two;            // two: a second operand of the tokens' side, multiplied into the same sums
   int* err;
 };
 
 __global__ void __launch_bounds__(THREADS, 1)
-few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Args args) {
+few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmX2,
+                const Args args) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t b_bytes = uint32_t(args.n_pad) * BK * 2, stage_bytes = A_BYTES + b_bytes;
+  const uint32_t b_bytes = uint32_t(args.n_pad) * BK * 2, stage_bytes = A_BYTES + (args.two ? 2 : 1) * b_bytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + args.stages * stage_bytes);
   uint64_t* empty_bar = full_bar + MAX_STAGES;
   uint64_t* tmem_full = empty_bar + MAX_STAGES;
@@ -78,7 +79,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         tma_load_2d(smem + stage * stage_bytes, &tmW, &full_bar[stage], k0, tile * TILE);
       };
       auto tokens = [&](long long kb, uint32_t stage) {                 // box [n_pad rows, 64 k]
-        tma_load_2d(smem + stage * stage_bytes + A_BYTES, &tmX, &full_bar[stage], int(kb % cut.nkb) * BK, 0);
+        uint8_t* sb = smem + stage * stage_bytes + A_BYTES;
+        const int k0 = int(kb % cut.nkb) * BK;
+        tma_load_2d(sb, &tmX, &full_bar[stage], k0, 0);
+        if (args.two) tma_load_2d(sb + b_bytes, &tmX2, &full_bar[stage], k0, 0);
       };
       // the ring's first round of weights does not wait for the tokens
       const long long head = begin + args.stages < end ? begin + args.stages : end;
@@ -110,8 +114,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * stage_bytes), sb = sa + A_BYTES;
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k)
-            umma_f16(d, umma_desc_sw128(sa + k * 32, 16, 1024), umma_desc_sw128(sb + k * 32, 16, 1024), idesc, !first || k != 0);
+          for (int k = 0; k < BK / 16; ++k) {
+            const uint64_t ad = umma_desc_sw128(sa + k * 32, 16, 1024);
+            umma_f16(d, ad, umma_desc_sw128(sb + k * 32, 16, 1024), idesc, !first || k != 0);
+            if (args.two) umma_f16(d, ad, umma_desc_sw128(sb + b_bytes + k * 32, 16, 1024), idesc, 1);
+          }
           umma_commit(&empty_bar[stage]);
           if (++stage == uint32_t(args.stages)) { stage = 0; phase ^= 1; }
         }
@@ -177,9 +184,9 @@ Cut cut_for(int tokens, int N, int K) {
   return c;
 }
 
-int launch_partials(const void* X, long long ldx, const void* W, float* part, const Cut& cut, int N, int K, bool early, int* err,
+int launch_partials(const void* X, const void* X2, long long ldx, const void* W, float* part, const Cut& cut, int N, int K, bool early, int* err,
                     cudaStream_t stream) {
-  if (cut.tokens < 1 || cut.tokens > MAX_ROWS || cut.grid < 1) return -10;
+  if (cut.tokens < 1 || cut.tokens > (X2 ? MAX_ROWS / 4 : MAX_ROWS) || cut.grid < 1) return -10;
   Args a;
   a.cut = cut;
   a.tiles = (N + TILE - 1) / TILE;
@@ -187,15 +194,18 @@ int launch_partials(const void* X, long long ldx, const void* W, float* part, co
   a.acc_cols = (a.n_pad + 31) / 32 * 32;        // whole 32-column reads stay inside an accumulator's columns
   a.tmem_cols = 64;
   while (a.tmem_cols < 2 * a.acc_cols) a.tmem_cols *= 2;
-  const int stage_bytes = A_BYTES + a.n_pad * BK * 2;
+  a.two = X2 != nullptr;
+  const int stage_bytes = A_BYTES + (a.two ? 2 : 1) * a.n_pad * BK * 2;
   a.stages = (SMEM_LIMIT - SMEM_EXTRA) / stage_bytes;
   if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
   a.part = part;
   a.early = early;
   a.err = err;
-  CUtensorMap tmW, tmX;
+  CUtensorMap tmW, tmX, tmX2;
   int rc = make_tmap_2d_bf16(&tmW, W, N, K, K, TILE);
   if (!rc) rc = make_tmap_2d_bf16(&tmX, X, cut.tokens, K, ldx, a.n_pad);
+  tmX2 = tmX;
+  if (!rc && X2) rc = make_tmap_2d_bf16(&tmX2, X2, cut.tokens, K, ldx, a.n_pad);
   if (rc) return rc;
   static PerDevice configured;
   if (configured.first()) {
@@ -203,8 +213,8 @@ int launch_partials(const void* X, long long ldx, const void* W, float* part, co
     configured.done();
   }
   const int smem = a.stages * stage_bytes + SMEM_EXTRA;
-  if (early) return launch_early(few_rows_kernel, dim3(cut.grid), dim3(THREADS), smem, stream, tmW, tmX, a);
-  few_rows_kernel<<<cut.grid, THREADS, smem, stream>>>(tmW, tmX, a);
+  if (early) return launch_early(few_rows_kernel, dim3(cut.grid), dim3(THREADS), smem, stream, tmW, tmX, tmX2, a);
+  few_rows_kernel<<<cut.grid, THREADS, smem, stream>>>(tmW, tmX, tmX2, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 

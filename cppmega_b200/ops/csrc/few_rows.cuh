@@ -46,9 +46,9 @@ inline int launch_early(void (*kern)(P...), dim3 grid, dim3 block, int smem, cud
   return cudaLaunchKernelEx(&cfg, kern, P(args)...) == cudaSuccess ? 0 : -3;
 }
 
-// X: row pitch ldx; W: dense rows of K.  Bases and pitches on 16 bytes, K % 8 == 0, tokens <= MAX_ROWS.  early: X, and the work space's
+// X: row pitch ldx; X2: null, or what X lacks (X + X2 is multiplied; same pitch, tokens <= MAX_ROWS / 4); W: dense rows of K.  Bases and pitches on 16 bytes, K % 8 == 0, tokens <= MAX_ROWS.  early: X, and the work space's
 // last reader, are those of the kernel before it in the stream, and the weights are older: their loads start before that one has ended.
-int launch_partials(const void* X, long long ldx, const void* W, float* part, const Cut& cut, int N, int K, bool early, int* err,
+int launch_partials(const void* X, const void* X2, long long ldx, const void* W, float* part, const Cut& cut, int N, int K, bool early, int* err,
                     cudaStream_t stream);
 
 }  // namespace few

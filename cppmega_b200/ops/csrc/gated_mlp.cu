@@ -450,10 +450,12 @@ static int few_share(const few::Cut& c) {
   return most <= 4 ? 1 : most <= 16 ? 4 : MAX_SHARE;
 }
 
-// h[token][f] = act(g) u from rows f and F + f of the first product; g, u kept for training.
+// h[token][f] = act(g) u from rows f and F + f of the first product, and what its rounding to bf16 dropped (lo): the second
+// product takes both, which costs it 1 % and leaves y with the one rounding of the result.  g, u kept for training.
 template <int ACT>
 __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_gate_kernel(const float* __restrict__ part, const few::Cut cut, int F,
-                                                                         __nv_bfloat16* __restrict__ h, const Kept kept) {
+                                                                         __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ lo,
+                                                                         const Kept kept) {
   __shared__ FewSums share;
   const int col = blockIdx.x * few::TILE + threadIdx.x, f = min(col, F - 1), tok0 = blockIdx.y * TOKS;   // past the last column: repeats it
   few::wait_for_input();
@@ -467,7 +469,12 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_gate_kernel(const f
   for (int j = 0; j < TOKS; ++j) {
     const long long tok = tok0 + j;
     if (tok >= cut.tokens) break;
-    if (col < F) h[tok * F + f] = __float2bfloat16(act_of<ACT>(g[j]) * u[j]);
+    if (col < F) {
+      const float v = act_of<ACT>(g[j]) * u[j];
+      const __nv_bfloat16 hi = __float2bfloat16(v);
+      h[tok * F + f] = hi;
+      lo[tok * F + f] = __float2bfloat16(isfinite(v) ? v - __bfloat162float(hi) : 0.f);
+    }
     if (kept.v) {                             // a warp holds a group of 32 columns
       const uint32_t gp = power_for(warp_max(fabsf(g[j]))), up = power_for(warp_max(fabsf(u[j])));
       if (col < F) {
@@ -497,27 +504,30 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_sum_kernel(const fl
 }
 
 // Tokens up to which the weights are streamed by few_rows.cu.  Device time, streamed and in tiles, in us:
-//   hidden x ffn    1 token       64           128
-//   4096 x 21504    92 / 220    100 / 147    113 / 149
-//   1024 x  8192    22 /  45     23 /  41     27 /  42
-//   1024 x  2048    13 /  21     15 /  18
-//    256 x   512     9 /   9     11 /  10
-// A long ffn leaves the second product of the tiles few of them, each with a long reduction.
-static bool few_tokens(int M, int F) { return M <= (F >= 8192 ? 192 : 64); }
+//   hidden x ffn    1 token       24           64          128
+//   4096 x 21504    96 / 144     98 / 115    105 / 117    116 / 123
+//   3584 x 18944    77 / 101     78 /  83     84 /  85     93 /  90
+//   1024 x  2048    13 /  20     15 /  18     16 /  18     19 /  20
+//    256 x   512    11 /  10     12 /  10     12 /  10     11 /  11
+constexpr int FEW_TOKENS = few::MAX_ROWS / 4;
+
+// floats of the partial tiles, the larger of the two products', in whole 16 bytes; lo lies behind them
+static long long few_floats(const few::Cut& a, const few::Cut& b) { return a.floats() > b.floats() ? a.floats() : b.floats(); }
 
 static int few_forward(const void* x, long long ldx, const void* w1, const void* w2, const Kept& kept, __nv_bfloat16* h, __nv_bfloat16* y,
                        float* ws, int M, int H, int F, int Ho, int act, int* err, cudaStream_t stream) {
   const few::Cut c1 = few::cut_for(M, 2 * F, H), c2 = few::cut_for(M, Ho, F);
-  int rc = few::launch_partials(x, ldx, w1, ws, c1, 2 * F, H, false, err, stream);
+  __nv_bfloat16* lo = reinterpret_cast<__nv_bfloat16*>(ws + few_floats(c1, c2));
+  int rc = few::launch_partials(x, nullptr, ldx, w1, ws, c1, 2 * F, H, false, err, stream);
   if (rc) return rc;
   const dim3 grid((F + few::TILE - 1) / few::TILE, (M + TOKS - 1) / TOKS), block(few::TILE, few_share(c1));
   switch (act) {
-    case SILU: rc = few::launch_early(few_gate_kernel<SILU>, grid, block, 0, stream, ws, c1, F, h, kept); break;
-    case GELU_TANH: rc = few::launch_early(few_gate_kernel<GELU_TANH>, grid, block, 0, stream, ws, c1, F, h, kept); break;
-    case RELU: rc = few::launch_early(few_gate_kernel<RELU>, grid, block, 0, stream, ws, c1, F, h, kept); break;
+    case SILU: rc = few::launch_early(few_gate_kernel<SILU>, grid, block, 0, stream, ws, c1, F, h, lo, kept); break;
+    case GELU_TANH: rc = few::launch_early(few_gate_kernel<GELU_TANH>, grid, block, 0, stream, ws, c1, F, h, lo, kept); break;
+    case RELU: rc = few::launch_early(few_gate_kernel<RELU>, grid, block, 0, stream, ws, c1, F, h, lo, kept); break;
     default: rc = -10;
   }
-  if (!rc) rc = few::launch_partials(h, F, w2, ws, c2, Ho, F, true, err, stream);
+  if (!rc) rc = few::launch_partials(h, lo, F, w2, ws, c2, Ho, F, true, err, stream);
   if (!rc) rc = few::launch_early(few_sum_kernel, dim3((Ho + few::TILE - 1) / few::TILE, (M + TOKS - 1) / TOKS), dim3(few::TILE, few_share(c2)), 0,
                                   stream, ws, c2, Ho, y);
   return rc;
@@ -536,9 +546,8 @@ extern "C" long long cm_gated_mlp_kept(int M, int F) { return mlp::Kept::bytes(M
 // Floats of work space that the forward needs; 0: none.
 extern "C" long long cm_gated_mlp_fwd_ws(int M, int H, int F, int Ho) {
   if (M <= 0) return 0;
-  if (!mlp::few_tokens(M, F)) return split::plan(sm_count(), M, Ho, F, false).floats;
-  const long long a = few::cut_for(M, 2 * F, H).floats(), b = few::cut_for(M, Ho, F).floats();
-  return a > b ? a : b;
+  if (M > mlp::FEW_TOKENS) return split::plan(sm_count(), M, Ho, F, false).floats;
+  return mlp::few_floats(few::cut_for(M, 2 * F, H), few::cut_for(M, Ho, F)) + (long long)M * F / 2;
 }
 
 // y[M, Ho] = (act(x w1[:F]^T) * (x w1[F:]^T)) w2^T; x [M, H] with row pitch ldx, w1 [2F, H], w2 [Ho, F], h [M, F]; kept: cm_gated_mlp_kept
@@ -550,7 +559,7 @@ extern "C" int cm_gated_mlp_fwd(const void* x, long long ldx, const void* w1, co
       !mlp::tma_ok(h, F) || !mlp::tma_ok(y, Ho))
     return -10;
   const mlp::Kept k = kept ? mlp::Kept::at(kept, M, F) : mlp::Kept{};
-  if (mlp::few_tokens(M, F)) {
+  if (M <= mlp::FEW_TOKENS) {
     if (!ws) return -10;
     return mlp::few_forward(x, ldx, w1, w2, k, static_cast<__nv_bfloat16*>(h), static_cast<__nv_bfloat16*>(y), ws, M, H, F, Ho, act, err, stream);
   }
