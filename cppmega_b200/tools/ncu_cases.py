@@ -1,6 +1,6 @@
 """Small, self-terminating workloads for Nsight Compute captures of single kernels.
 
-    python -m cppmega_b200.tools.ncu_cases {gemm,gemm_wgrad,attention,head_linear,scan_fwd,scan_bwd,m2rnn,m2rnn_bwd,sparse_mla,indexer,ce,rmsnorm,rmsnorm_bwd,adamw,quantize,strided_copy,moe_local,mxfp8_gemm,residual_norm,gated_norm,gated_mlp,gated_mlp_few}
+    python -m cppmega_b200.tools.ncu_cases {gemm,gemm_wgrad,attention,head_linear,scan_fwd,scan_bwd,m2rnn,m2rnn_bwd,sparse_mla,indexer,ce,rmsnorm,rmsnorm_bwd,adamw,quantize,strided_copy,moe_local,mxfp8_gemm,residual_norm,gated_norm,gated_mlp,gated_mlp_few,gated_mlp_shared}
 
 Each case launches its kernel three times on inputs that exceed the 126 MB L2 but hold at most a few GB, so a
 ``--set full`` capture of one launch finishes in a minute or two:
@@ -289,14 +289,15 @@ def case_gated_norm():
     torch.cuda.synchronize()
 
 
-def case_gated_mlp(tokens: int = 4096):
-    """The gated feed-forward block at the quarter model's widths (forward and backward), or a few tokens through it."""
+def case_gated_mlp(tokens: int = 4096, hidden: int = 3584, ffn: int = 18944):
+    """The gated feed-forward block at the quarter model's widths (forward and backward), a few tokens through it, or the shared
+    expert of the full model."""
     from cppmega_b200.ops import cuda as cu
     from cppmega_b200.ops import functional as F_
     train = tokens > 256
-    x = torch.randn(tokens, 3584, device="cuda").bfloat16().requires_grad_(train)
-    w1 = (torch.randn(2 * 18944, 3584, device="cuda") * 0.02).bfloat16().requires_grad_(train)
-    w2 = (torch.randn(3584, 18944, device="cuda") * 0.01).bfloat16().requires_grad_(train)
+    x = torch.randn(tokens, hidden, device="cuda").bfloat16().requires_grad_(train)
+    w1 = (torch.randn(2 * ffn, hidden, device="cuda") * 0.02).bfloat16().requires_grad_(train)
+    w2 = (torch.randn(hidden, ffn, device="cuda") * 0.01).bfloat16().requires_grad_(train)
     for _ in range(3):
         y = F_.gated_mlp(x, w1, w2)
         if train:
@@ -310,7 +311,7 @@ CASES = {"gemm": case_gemm, "attention": case_attention, "head_linear": case_hea
          "m2rnn_bwd": case_m2rnn_bwd, "sparse_mla": case_sparse_mla, "indexer": case_indexer,
          "rmsnorm_bwd": case_rmsnorm_bwd, "adamw": case_adamw, "quantize": case_quantize, "strided_copy": case_strided_copy, "moe_local": case_moe_local,
          "residual_norm": case_residual_norm, "gated_norm": case_gated_norm, "gated_mlp": case_gated_mlp,
-         "gated_mlp_few": lambda: case_gated_mlp(24)}
+         "gated_mlp_few": lambda: case_gated_mlp(24), "gated_mlp_shared": lambda: case_gated_mlp(16384, 4096, 1024)}
 
 if __name__ == "__main__":
     name = sys.argv[1] if len(sys.argv) > 1 else ""

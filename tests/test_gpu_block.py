@@ -584,3 +584,135 @@ def test_block_backward_in_a_graph():
     graph.replay()
     _check_errors()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_residual_gradients_are_separate_tensors():
+    """Without gate and scale one gradient serves both inputs: what accumulates in one must not show in the other."""
+    y, x = (_randn(33, 64, dtype=torch.float32, seed=s).requires_grad_() for s in (1, 2))
+    w = _randn(64, dtype=torch.float32, mean=1.0, std=0.1, seed=3)
+    n, h = F_.residual_rmsnorm(y, x, w)
+    (n.sum() + h.sum()).backward()
+    assert torch.equal(y.grad, x.grad)
+    before = x.grad.clone()
+    y.grad.add_(1)
+    assert torch.equal(x.grad, before)
+    n, h = F_.residual_rmsnorm(y, x, w)
+    (n.sum() + h.sum()).backward()
+    assert torch.equal(x.grad, 2 * before) and torch.equal(y.grad, (before + 1) + before)
+
+
+def _dense_mlp(hidden=256, ffn=520):
+    from cppmega_b200.models.common import DenseMLP
+    from cppmega_b200.parallel.state import single_process_context
+    return DenseMLP(hidden, ffn, single_process_context(), std=hidden ** -0.5, out_std=ffn ** -0.5, dtype=torch.bfloat16, seed=3).cuda()
+
+
+def test_dense_mlp_module():
+    m = _dense_mlp()
+    x, dy = _randn(2, 60, 256), _randn(2, 60, 256, std=0.1, seed=1)
+    leaf = x.clone().requires_grad_()
+    F_.reset_counters()
+    y = m(leaf)
+    y.backward(dy)
+    assert F_.launch_counts() == {"gated_mlp": 1, "gated_mlp_bwd": 1} and not F_.fallback_counts()
+    _check_mlp(x, m.linear_fc1.weight, m.linear_fc2.weight, "silu", y, dict(x=leaf.grad, w1=m.linear_fc1.weight.grad, w2=m.linear_fc2.weight.grad), dy)
+
+
+def test_dense_mlp_module_captured():
+    """The module as a captured callable (the ``mlp`` scope of the graph option): replays give the eager bits."""
+    m = _dense_mlp()
+    x, dy = _randn(90, 256).requires_grad_(), _randn(90, 256, std=0.1, seed=1)
+    y = m(x)
+    want = [y.detach().clone(), *torch.autograd.grad(y, [x, *m.parameters()], dy)]
+    del y
+    graphed = torch.cuda.make_graphed_callables(_dense_mlp(), (torch.randn_like(x).requires_grad_(),))
+    for _ in range(2):
+        y = graphed(x)
+        got = [y.detach().clone(), *torch.autograd.grad(y, [x, *graphed.parameters()], dy)]
+        _check_errors()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_fastmtp_block():
+    """The shared block: attention, residual step, feed-forward - against the same block on its PyTorch definitions."""
+    from cppmega_b200.models.fastmtp import SharedMTPBlock
+    torch.manual_seed(0)
+    b = SharedMTPBlock(256, 2, 512, torch.bfloat16).cuda()
+    x, dy = _randn(2, 128, 256), _randn(2, 128, 256, std=0.1, seed=1)
+    res = []
+    for own in (True, False):
+        names = ("residual_rmsnorm", "gated_mlp")
+        (F_.enable_cuda if own else F_.disable_cuda)(*names)
+        try:
+            leaf = x.clone().requires_grad_()
+            y = b(leaf)
+            res.append([y.detach(), *torch.autograd.grad(y, [leaf, *b.parameters()], dy)])
+        finally:
+            F_.enable_cuda(*names)
+    _check_errors()
+    for p, q in zip(*res):                          # some ten roundings to bf16 on the longest path of either
+        assert (p.double() - q.double()).norm() <= 10 * 2 ** -8 * q.double().norm()
+
+
+def test_mixer_norm_reads_its_gate_in_place():
+    """The gate of the M2RNN mixer is a column slice of the projection whose rows are not a multiple of 16 bytes apart from it."""
+    from cppmega_b200.models.common import RMSNorm
+    norm = RMSNorm(136, dtype=torch.bfloat16).cuda()
+    proj = _randn(2, 30, 600).requires_grad_()
+    y, dy = _randn(2, 30, 136, seed=2).requires_grad_(), _randn(2, 30, 136, std=0.1, seed=3)
+    gate = proj[..., 451:587]
+    F_.reset_counters()
+    out = norm(y, gate=gate, norm_before_gate=False)
+    dx, dp, dw = torch.autograd.grad(out, [y, proj, norm.weight], dy)
+    assert set(F_.launch_counts()) == {"rmsnorm_gated", "rmsnorm_gated_bwd"} and not F_.fallback_counts()
+    assert (dp[..., :451] == 0).all() and (dp[..., 587:] == 0).all()
+    _check_gated(y, norm.weight, gate, 136, False, out, dict(x=dx, w=dw, z=dp[..., 451:587]), dy)
+
+
+def test_block_calls_from_two_threads():
+    """Two host threads, each on its own stream, get what one alone gets."""
+    import threading
+    p = {k: t.detach() for k, t in _step_params().items()}
+    ins = [[_randn(40 + 30 * i, 256, seed=5 + i), _randn(40 + 30 * i, 256, seed=9 + i)] for i in range(2)]
+    with torch.no_grad():
+        want = [_step(*i, p) for i in ins]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def work(k):
+        try:
+            with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[k] = _step(*ins[k], p)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                      # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    _check_errors()
+    for a, b in zip(got, want):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_rows_behind_the_last_one_are_left_alone():
+    """Results that end inside a larger buffer: the feed-forward's products write whole tiles, clipped at their last row and column."""
+    from cppmega_b200.ops import cuda as cu
+    L, T, H, F = cu.lib(), 70, 64, 72
+    x, w1, w2 = _mlp_inputs((T,), H, F, H)
+    for tokens in (T, 9):                           # tiles, and the path for few tokens
+        y = torch.full((tokens + 8, H), 7.0, dtype=torch.bfloat16, device="cuda")
+        h = torch.full((tokens + 8, F), 7.0, dtype=torch.bfloat16, device="cuda")
+        size = L.cm_gated_mlp_kept(tokens, F)
+        kept = torch.full((size + 64,), 99, dtype=torch.uint8, device="cuda")
+        floats = L.cm_gated_mlp_fwd_ws(tokens, H, F, H)
+        ws = torch.full((floats + 64,), 5.0, device="cuda")
+        assert L.cm_gated_mlp_fwd(x.data_ptr(), H, w1.data_ptr(), w2.data_ptr(), kept.data_ptr(), h.data_ptr(), y.data_ptr(), ws.data_ptr(), tokens,
+                                  H, F, H, 0, cu.err_word().data_ptr(), cu.stream_ptr()) == 0
+        _check_errors()
+        assert (y[tokens:] == 7).all() and (h[tokens:] == 7).all() and (kept[size:] == 99).all() and (ws[floats:] == 5).all()
+        _check_mlp(x[:tokens], w1, w2, "silu", y[:tokens])
