@@ -8,7 +8,7 @@
 // backward and adds their weight gradient in registers.  Bound by memory: three rows moved forward, five backward; the gate is read
 // where it lies (a column slice of the projection has its own pitch).  The weight gradient is summed in a fixed order.
 #include "row_vec.cuh"
-#define CM_ROW_TEAM_BY_WARP(F) case 16 * 32 + 4: return F(32, 4, true);
+#define CM_ROW_TEAM_BY_WARP(team, F) if (team == 16 * 32 + 4) return F(32, 4, true);
 
 namespace cm {
 
@@ -35,8 +35,8 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArg
   uint4 xv[VPT], zv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    xv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.sx + g0, t + i * TPR, G);
-    zv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.z) + row * a.sz + g0, t + i * TPR, has_z ? G : 0);
+    xv[i] = rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.x) + row * a.sx + g0, t, i, G);
+    zv[i] = rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.z) + row * a.sz + g0, t, i, has_z ? G : 0);
   }
   float ss[1] = {0.f};
   float gated[GATE_FIRST ? VPT : 1][N];                    // x a(z): the sigmoids are not formed twice
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArg
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     float x[N], w[N];
-    rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, t + i * TPR, G), w);
+    rv_unpack<T>(rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.w) + g0, t, i, G), w);
     if constexpr (GATE_FIRST) {
 #pragma unroll
       for (int j = 0; j < N; ++j) x[j] = gated[i][j] * r * w[j];
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArg
 #pragma unroll
       for (int j = 0; j < N; ++j) x[j] *= r * w[j] * (has_z ? z[j] * rv_sigmoid(z[j]) : 1.f);
     }
-    rv_store<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + g0, t + i * TPR, G, rv_pack<T>(x));
+    rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + g0, t, i, G, rv_pack<T>(x));
   }
 }
 
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
   in.start(dyn, (long long)blockIdx.x * RPB + threadIdx.x / TPR, step);
   uint4 wv[VPT];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) wv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.w) + g0, t + i * TPR, a.group);
+  for (int i = 0; i < VPT; ++i) wv[i] = rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.w) + g0, t, i, a.group);
   auto stat = [&](long long row) { return row < a.rows ? a.rstd[row * gridDim.y + blockIdx.y] : 0.f; };
   float next_r = stat((long long)blockIdx.x * RPB + threadIdx.x / TPR);      // requested a row ahead
   int turn = 0;
@@ -141,14 +141,13 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
         s[0] += dnw[i][j] * hat[i][j];
       }
       if constexpr (!GATE_FIRST)
-        if (a.dz) rv_store<T, VEC>(reinterpret_cast<T*>(a.dz) + row * a.width + g0, t + i * TPR, G, rv_pack<T>(z));
+        if (a.dz) rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.dz) + row * a.width + g0, t, i, G, rv_pack<T>(z));
     }
     in.next();
     rv_team_sum<TPR, 1>(s, red, turn);
     const float m = s[0] * inv_group;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = t + i * TPR;
       float x[N];
       if constexpr (GATE_FIRST) {
         float z[N];
@@ -158,16 +157,16 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
           x[j] = du * gate[i][j];
           z[j] = du * xs[i][j];
         }
-        if (a.dz) rv_store<T, VEC>(reinterpret_cast<T*>(a.dz) + row * a.width + g0, c, G, rv_pack<T>(z));
+        if (a.dz) rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.dz) + row * a.width + g0, t, i, G, rv_pack<T>(z));
       } else {
 #pragma unroll
         for (int j = 0; j < N; ++j) x[j] = r * (dnw[i][j] - hat[i][j] * m);
       }
-      rv_store<T, VEC>(reinterpret_cast<T*>(a.dx) + row * a.width + g0, c, G, rv_pack<T>(x));
+      rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.dx) + row * a.width + g0, t, i, G, rv_pack<T>(x));
     }
   }
   in.drain();
-  if (a.part) rv_partial<T, TPR, VPT>(acc, a.part + (long long)blockIdx.x * a.width + g0, a.group, scratch);
+  if (a.part) rv_partial<T, TPR, VPT, VEC>(acc, a.part + (long long)blockIdx.x * a.width + g0, a.group, scratch);
 }
 
 template <typename T>
@@ -182,7 +181,7 @@ static int gated_launch(const GatedArgs& a, bool back, int& blocks, cudaStream_t
     constexpr int TB = rv_block<TPR>(), RPB = TB / TPR;                                                                          \
     if (back) {                                                                                                                  \
       auto kern = a.gate_first ? gated_norm_bwd<T, TPR, VPT, VEC, true> : gated_norm_bwd<T, TPR, VPT, VEC, false>;               \
-      constexpr int RING = VEC ? rv_stages(TPR, VPT) * VPT * TB * 16 * 3 : 0;                                                    \
+      constexpr int RING = rv_slots(TPR, VPT, VEC) * VPT * TB * 16 * 3;                                                    \
       static PerDevice configured[2];                                                                                            \
       if (configured[a.gate_first].first()) {                                                                                    \
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING) != cudaSuccess) return -2;             \

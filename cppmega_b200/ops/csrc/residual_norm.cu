@@ -11,7 +11,7 @@
 // Bound by memory: forward 4 rows moved, backward 6 (4 read).  Sums over rows go through one partial row per block and a second
 // kernel in a fixed order: the same call gives the same bits.
 #include "row_vec.cuh"
-#define CM_ROW_TEAM_BY_WARP(F)
+#define CM_ROW_TEAM_BY_WARP(team, F)
 
 namespace cm {
 
@@ -45,8 +45,8 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_fwd(const Resid
   uint4 yv[VPT], hv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    yv[i] = rv_load<T, VEC>(yr, t + i * TPR, w_on);
-    hv[i] = rv_load<T, VEC>(xr, t + i * TPR, w_on);
+    yv[i] = rv_load<T, TPR, VEC>(yr, t, i, w_on);
+    hv[i] = rv_load<T, TPR, VEC>(xr, t, i, w_on);
   }
   float r = 1.f;
   const bool post = FULL && a.post;
@@ -72,13 +72,13 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_fwd(const Resid
     if constexpr (FULL) {
       if (post) {
         float p[N];
-        rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), t + i * TPR, W), p);
+        rv_unpack<T>(rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.post), t, i, W), p);
 #pragma unroll
         for (int j = 0; j < N; ++j) y[j] *= r * p[j];
       }
       if (a.gate) {
         float g[N];
-        rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.gate) + (a.gate_rows ? row * W : 0ll), t + i * TPR, w_on), g);
+        rv_unpack<T>(rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.gate) + (a.gate_rows ? row * W : 0ll), t, i, w_on), g);
 #pragma unroll
         for (int j = 0; j < N; ++j) y[j] *= g[j];
       }
@@ -100,11 +100,11 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_fwd(const Resid
   for (int i = 0; i < VPT; ++i) {
     float x[N], w[N];
     rv_unpack<T>(hv[i], x);
-    rv_unpack<T>(rv_load<T, VEC>(reinterpret_cast<const T*>(a.w), t + i * TPR, W), w);
-    rv_store<T, VEC>(hr, t + i * TPR, W, hv[i]);
+    rv_unpack<T>(rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.w), t, i, W), w);
+    rv_store<T, TPR, VEC>(hr, t, i, W, hv[i]);
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = x[j] * rho * w[j];
-    rv_store<T, VEC>(nr, t + i * TPR, W, rv_pack<T>(x));
+    rv_store<T, TPR, VEC>(nr, t, i, W, rv_pack<T>(x));
   }
 }
 
@@ -135,10 +135,10 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
   uint4 wv[VPT], pv[FULL ? VPT : 1], tv[FULL ? VPT : 1];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    wv[i] = rv_load<T, VEC>(reinterpret_cast<const T*>(a.w), t + i * TPR, W);
+    wv[i] = rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.w), t, i, W);
     if constexpr (FULL) {
-      pv[i] = post ? rv_load<T, VEC>(reinterpret_cast<const T*>(a.post), t + i * TPR, W) : rv_ones<T>();
-      tv[i] = gate && !a.gate_rows ? rv_load<T, VEC>(reinterpret_cast<const T*>(a.gate), t + i * TPR, W) : rv_ones<T>();
+      pv[i] = post ? rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.post), t, i, W) : rv_ones<T>();
+      tv[i] = gate && !a.gate_rows ? rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.gate), t, i, W) : rv_ones<T>();
     }
   }
   const float inv_w = 1.f / W;
@@ -201,7 +201,6 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
     const float sr = a.scale * r;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = t + i * TPR;
       float d[N];
       if constexpr (FULL) {
         rv_unpack<T>(in.get(HH, i), d);
@@ -211,7 +210,7 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
 #pragma unroll
         for (int j = 0; j < N; ++j) d[j] = dt[i][j] - k * hv[i][j];
       }
-      rv_store<T, VEC>(reinterpret_cast<T*>(a.dres) + row * W, c, on ? W : 0, rv_pack<T>(d));
+      rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.dres) + row * W, t, i, on ? W : 0, rv_pack<T>(d));
       if constexpr (FULL) {
         float y[N], p[N], q[N];
         rv_unpack<T>(in.get(YY, i), y);
@@ -221,7 +220,7 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
           float dg[N];
 #pragma unroll
           for (int j = 0; j < N; ++j) dg[j] = sr * d[j] * (y[j] * p[j]);
-          rv_store<T, VEC>(reinterpret_cast<T*>(a.dgate_rows) + row * W, c, on ? W : 0, rv_pack<T>(dg));
+          rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.dgate_rows) + row * W, t, i, on ? W : 0, rv_pack<T>(dg));
         }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
@@ -233,13 +232,13 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
 #pragma unroll
         for (int j = 0; j < N; ++j) d[j] *= a.scale;
       }
-      if (a.dy) rv_store<T, VEC>(reinterpret_cast<T*>(a.dy) + row * W, c, on ? W : 0, rv_pack<T>(d));
+      if (a.dy) rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.dy) + row * W, t, i, on ? W : 0, rv_pack<T>(d));
     }
     in.next();
   }
   in.drain();
   const long long at = (long long)blockIdx.x * W;
-  if (a.part_w) rv_partial<T, TPR, VPT>(acc_w, a.part_w + at, W, scratch);
+  if (a.part_w) rv_partial<T, TPR, VPT, VEC>(acc_w, a.part_w + at, W, scratch);
   if constexpr (FULL) {
     // with a gate per channel both its gradient and the post norm's are the sum of dh yh, times the other one's factor; with a gate per
     // element the sum already holds the gate
@@ -252,7 +251,7 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
 #pragma unroll
         for (int j = 0; j < N; ++j) sum[i][j] = a.scale * f[j] * acc_y[i][j];
       }
-      rv_partial<T, TPR, VPT>(sum, part + at, W, scratch);
+      rv_partial<T, TPR, VPT, VEC>(sum, part + at, W, scratch);
     };
     if (a.part_post) out(a.part_post, tv);
     if (a.part_gate) out(a.part_gate, pv);
@@ -279,7 +278,7 @@ static int residual_launch(const ResidualArgs& a, bool back, int& blocks, cudaSt
     constexpr int TB = rv_block<TPR>(), RPB = TB / TPR;                                                                           \
     if (back) {                                                                                                                   \
       auto kern = residual_norm_bwd<T, TPR, VPT, VEC, FULL>;                                                                      \
-      constexpr int SLOT = VEC ? rv_stages(TPR, VPT) * VPT * TB * 16 : 0;                                                         \
+      constexpr int SLOT = rv_slots(TPR, VPT, VEC) * VPT * TB * 16;                                                         \
       static PerDevice configured;                                                                                                \
       if (configured.first()) {                                                                                                   \
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SLOT * (FULL ? 5 : 3)) != cudaSuccess) return -2; \

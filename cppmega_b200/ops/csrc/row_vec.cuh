@@ -1,6 +1,8 @@
-// Rows of bf16, fp16 or fp32 held in registers as 16-byte vectors by a team of TPR threads (vector i of thread t: t + i TPR).
-// VEC: every row starts on a 16-byte boundary and ends on one; otherwise the same vectors are moved element by element, the elements
-// past the row read as zero and are not written.
+// Rows of bf16, fp16 or fp32 held in registers by a team of TPR threads, VPT packed vectors of N = 16 bytes each.
+// VEC: every row starts on a 16-byte boundary and ends on one, and vector i of thread t is the row's vector t + i TPR.  Otherwise rows
+// may start and end anywhere: element j of vector i of thread t is the row's element (i N + j) TPR + t, so that neighbouring threads
+// move neighbouring elements one at a time (with eight consecutive elements a thread, 16384 x 4095 took 5 times as long as 4096).
+// Elements past the row read as zero and are not written.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -11,6 +13,12 @@ namespace cm {
 template <typename T>
 struct RowVec {
   static constexpr int N = 16 / int(sizeof(T));
+  using Bits = uint16_t;
+};
+template <>
+struct RowVec<float> {
+  static constexpr int N = 4;
+  using Bits = uint32_t;
 };
 
 template <typename T>
@@ -69,31 +77,45 @@ __device__ __forceinline__ uint4 rv_ones() {
   return rv_pack<T>(f);
 }
 
-// vector `i` of the row (zero past its end)
-template <typename T, bool VEC>
-__device__ __forceinline__ uint4 rv_load(const T* __restrict__ row, int i, int width) {
+// column of element j of vector i of thread t
+template <typename T, int TPR, bool VEC>
+__device__ __forceinline__ int rv_column(int t, int i, int j) {
+  constexpr int N = RowVec<T>::N;
+  return VEC ? (t + i * TPR) * N + j : (i * N + j) * TPR + t;
+}
+
+// vector `i` of thread t (zero past the row's end)
+template <typename T, int TPR, bool VEC>
+__device__ __forceinline__ uint4 rv_load(const T* __restrict__ row, int t, int i, int width) {
   constexpr int N = RowVec<T>::N;
   if constexpr (VEC) {
-    return i * N < width ? reinterpret_cast<const uint4*>(row)[i] : make_uint4(0, 0, 0, 0);
+    return (t + i * TPR) * N < width ? reinterpret_cast<const uint4*>(row)[t + i * TPR] : make_uint4(0, 0, 0, 0);
   } else {
-    float f[N];
+    using Bits = typename RowVec<T>::Bits;
+    Bits e[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = i * N + j < width ? float(row[i * N + j]) : 0.f;
-    return rv_pack<T>(f);
+    for (int j = 0; j < N; ++j) {
+      const int c = rv_column<T, TPR, VEC>(t, i, j);
+      e[j] = c < width ? reinterpret_cast<const Bits*>(row)[c] : Bits(0);
+    }
+    if constexpr (sizeof(T) == 4) return make_uint4(e[0], e[1], e[2], e[3]);
+    else return make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16, e[6] | uint32_t(e[7]) << 16);
   }
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void rv_store(T* __restrict__ row, int i, int width, const uint4& v) {
+template <typename T, int TPR, bool VEC>
+__device__ __forceinline__ void rv_store(T* __restrict__ row, int t, int i, int width, const uint4& v) {
   constexpr int N = RowVec<T>::N;
   if constexpr (VEC) {
-    if (i * N < width) reinterpret_cast<uint4*>(row)[i] = v;
+    if ((t + i * TPR) * N < width) reinterpret_cast<uint4*>(row)[t + i * TPR] = v;
   } else {
-    float f[N];
-    rv_unpack<T>(v, f);
+    using Bits = typename RowVec<T>::Bits;
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (i * N + j < width) row[i * N + j] = T(f[j]);
+    for (int j = 0; j < N; ++j) {
+      const int c = rv_column<T, TPR, VEC>(t, i, j);
+      if (c < width) reinterpret_cast<Bits*>(row)[c] = sizeof(T) == 4 ? Bits(u[j & 3]) : Bits(u[j >> 1] >> ((j & 1) * 16));
+    }
   }
 }
 
@@ -129,7 +151,7 @@ constexpr int rv_block() { return TPR < 128 ? 128 : TPR; }
 
 // Column sums that the rows' threads hold, one partial row per block: partial[blockIdx][column].  Teams of the same block are added in
 // shared memory (`scratch`, (rows per block) x VPT x TPR x N floats), in a fixed order.
-template <typename T, int TPR, int VPT>
+template <typename T, int TPR, int VPT, bool VEC>
 __device__ __forceinline__ void rv_partial(const float (&acc)[VPT][RowVec<T>::N], float* __restrict__ out, int width, float* scratch) {
   constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
   const int t = threadIdx.x % TPR;
@@ -138,7 +160,7 @@ __device__ __forceinline__ void rv_partial(const float (&acc)[VPT][RowVec<T>::N]
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const int c = (t + i * TPR) * N + j;
+        const int c = rv_column<T, TPR, VEC>(t, i, j);
         if (c < width) out[c] = acc[i][j];
       }
   } else {
@@ -147,7 +169,7 @@ __device__ __forceinline__ void rv_partial(const float (&acc)[VPT][RowVec<T>::N]
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int j = 0; j < N; ++j) scratch[(threadIdx.x / TPR) * W + (t + i * TPR) * N + j] = acc[i][j];
+      for (int j = 0; j < N; ++j) scratch[(threadIdx.x / TPR) * W + rv_column<T, TPR, VEC>(t, i, j)] = acc[i][j];
     __syncthreads();
     for (int c = threadIdx.x; c < width; c += rv_block<TPR>()) {
       float s = 0.f;
@@ -160,13 +182,13 @@ __device__ __forceinline__ void rv_partial(const float (&acc)[VPT][RowVec<T>::N]
 
 // The operand rows of a backward kernel on their way in.  Every thread copies its own vectors of the next NS rows into shared memory
 // with asynchronous copies and reads back only what it copied, so the copies need no barrier and keep running over the barriers of the
-// rows' sums; read back twice (before and after a row's sum) they take no registers in between.  NS = 0, and rows that are not on 16
-// bytes: plain loads, twice.
+// rows' sums; read back twice (before and after a row's sum) they take no registers in between.  Rows that
+// are not on 16 bytes are loaded when their turn comes and wait in one slot; NS = 0: plain loads, twice.
 // What lies past a row's end, past the last row, or belongs to an absent operand is filled with zeros by the copy itself.
 template <typename T, int TPR, int VPT, bool VEC, int NS, int OPS>
 struct RowRing {
-  static constexpr bool ON = VEC && NS > 0;
-  static constexpr int TB = rv_block<TPR>(), N = RowVec<T>::N, SLOTS = NS > 0 ? NS : 1;
+  static constexpr bool ON = VEC && NS > 0, HELD = !VEC && NS > 0;
+  static constexpr int TB = rv_block<TPR>(), N = RowVec<T>::N, SLOTS = ON ? NS : 1;
   uint4* mine;               // [ops][NS][VPT][TB], at this thread
   const T* base[OPS];        // first row; null: zero
   long long pitch[OPS];
@@ -209,12 +231,24 @@ struct RowRing {
     if constexpr (ON)
       for (int s = 0; s < NS; ++s) request();
   }
+  __device__ __forceinline__ uint4 fetch(int op, int i) const {
+    return rv_load<T, TPR, VEC>(base[op] + row * pitch[op], first, i, base[op] && row < rows ? width : 0);
+  }
   __device__ __forceinline__ void wait() {
     if constexpr (ON) asm volatile("cp.async.wait_group %0;" ::"n"(NS > 0 ? NS - 1 : 0) : "memory");
+    if constexpr (HELD) {
+#pragma unroll
+      for (int op = 0; op < OPS; ++op) {
+        if (op < ops) {
+#pragma unroll
+          for (int i = 0; i < VPT; ++i) mine[(op * VPT + i) * TB] = fetch(op, i);
+        }
+      }
+    }
   }
   __device__ __forceinline__ uint4 get(int op, int i) const {
-    if constexpr (ON) return mine[(op * SLOTS * VPT + i) * TB + slot * (VPT * TB)];
-    else return rv_load<T, VEC>(base[op] + row * pitch[op], first + i * TPR, base[op] && row < rows ? width : 0);
+    if constexpr (ON || HELD) return mine[(op * SLOTS * VPT + i) * TB + slot * (VPT * TB)];
+    else return fetch(op, i);
   }
   // no copy may be on its way when the block ends
   __device__ __forceinline__ void drain() {
@@ -232,6 +266,9 @@ constexpr int rv_stages(int tpr, int vpt) {
   const int held = (tpr < 128 ? 128 : tpr) * vpt;
   return held <= 256 ? 4 : held <= 512 ? 3 : held <= 1024 ? 2 : 0;
 }
+// Slots of shared memory for one operand.
+constexpr int rv_slots(int tpr, int vpt, bool vec) { return vec ? rv_stages(tpr, vpt) : rv_stages(tpr, vpt) > 0 ? 1 : 0; }
+
 // Blocks of a backward kernel: those that the SMs hold at once, up to this many for each, shared by `share` sections of the rows; and no
 // more than there are rows.  (Four blocks of 128 threads an SM left the gated norm's backward waiting for memory: 281 us, 16 warps.)
 static inline long long rv_most_blocks(long long rows, int width, int share) {
@@ -281,35 +318,31 @@ enum RowType : int { ROW_BF16 = 0, ROW_FP16 = 1, ROW_FP32 = 2 };
 // The team of a row of `nvec` vectors, as 16 * threads + vectors a thread; 0: too wide.  `by_warp`: up to 128 vectors go to one warp.
 static inline int rv_team(int nvec, bool vec, bool by_warp) {
   if (vec && by_warp && nvec > 64 && nvec <= 128) return 16 * 32 + 4;
-  if (!vec) return nvec <= 64 ? 16 * 32 + 2 : nvec <= 256 ? 16 * 128 + 2 : nvec <= 1024 ? 16 * 512 + 2 : nvec <= 4096 ? 16 * 1024 + 4 : 0;
   return nvec <= 8 ? 16 * 8 + 1 : nvec <= 32 ? 16 * 32 + 1 : nvec <= 64 ? 16 * 32 + 2 : nvec <= 128 ? 16 * 128 + 1
          : nvec <= 256 ? 16 * 128 + 2 : nvec <= 512 ? 16 * 256 + 2 : nvec <= 1024 ? 16 * 512 + 2 : nvec <= 2048 ? 16 * 1024 + 2
          : nvec <= 4096 ? 16 * 1024 + 4 : 0;
 }
 
 // CM_ROW_TEAM(team, vec, F): calls F(threads, vectors, vec) with compile-time values; -10 for a team that does not exist.
-#define CM_ROW_TEAM(team, vec, F)                                                                                   \
-  if (vec) {                                                                                                        \
-    switch (team) {                                                                                                 \
-      CM_ROW_TEAM_BY_WARP(F)                                                                                        \
-      case 16 * 8 + 1: return F(8, 1, true);                                                                        \
-      case 16 * 32 + 1: return F(32, 1, true);                                                                      \
-      case 16 * 32 + 2: return F(32, 2, true);                                                                      \
-      case 16 * 128 + 1: return F(128, 1, true);                                                                    \
-      case 16 * 128 + 2: return F(128, 2, true);                                                                    \
-      case 16 * 256 + 2: return F(256, 2, true);                                                                    \
-      case 16 * 512 + 2: return F(512, 2, true);                                                                    \
-      case 16 * 1024 + 2: return F(1024, 2, true);                                                                  \
-      case 16 * 1024 + 4: return F(1024, 4, true);                                                                  \
-    }                                                                                                               \
-  } else {                                                                                                          \
-    switch (team) {                                                                                                 \
-      case 16 * 32 + 2: return F(32, 2, false);                                                                     \
-      case 16 * 128 + 2: return F(128, 2, false);                                                                   \
-      case 16 * 512 + 2: return F(512, 2, false);                                                                   \
-      case 16 * 1024 + 4: return F(1024, 4, false);                                                                 \
-    }                                                                                                               \
-  }                                                                                                                 \
+#define CM_ROW_TEAMS(team, VEC, F)                     \
+  switch (team) {                                      \
+    case 16 * 8 + 1: return F(8, 1, VEC);              \
+    case 16 * 32 + 1: return F(32, 1, VEC);            \
+    case 16 * 32 + 2: return F(32, 2, VEC);            \
+    case 16 * 128 + 1: return F(128, 1, VEC);          \
+    case 16 * 128 + 2: return F(128, 2, VEC);          \
+    case 16 * 256 + 2: return F(256, 2, VEC);          \
+    case 16 * 512 + 2: return F(512, 2, VEC);          \
+    case 16 * 1024 + 2: return F(1024, 2, VEC);        \
+    case 16 * 1024 + 4: return F(1024, 4, VEC);        \
+  }
+#define CM_ROW_TEAM(team, vec, F)                      \
+  if (vec) {                                           \
+    CM_ROW_TEAM_BY_WARP(team, F)                       \
+    CM_ROW_TEAMS(team, true, F)                        \
+  } else {                                             \
+    CM_ROW_TEAMS(team, false, F)                       \
+  }                                                    \
   return -10
 
 }  // namespace cm
