@@ -414,34 +414,55 @@ constexpr int TOKS = 8, MAX_SHARE = 8;
 struct FewSums {
   float s[MAX_SHARE - 1][TOKS][few::TILE];
 };
-__device__ __forceinline__ void few_sum(const float* __restrict__ part, const few::Cut& cut, int row, int tok0, FewSums* share, float (&s)[TOKS]) {
-  const int t = row / few::TILE, in = row % few::TILE, n = cut.tokens - tok0, c1 = cut.last(t);
-  const float* p0 = part + tok0 * few::TILE + in;
+// The sums of NR weight rows at once, so that their loads are in flight together as well.
+template <int NR>
+__device__ __forceinline__ void few_sum(const float* __restrict__ part, const few::Cut& cut, const int (&row)[NR], int tok0, FewSums* share,
+                                        float (&s)[NR][TOKS]) {
+  const int n = cut.tokens - tok0;
+  int tile[NR], c[NR], end[NR], left = 0;
 #pragma unroll
-  for (int j = 0; j < TOKS; ++j) s[j] = 0.f;
-  for (int c = cut.first(t) + threadIdx.y; c <= c1; c += blockDim.y) {
-    const float* p = p0 + cut.at(c, t);
-    float v[TOKS];
-    if (n >= TOKS) {
+  for (int r = 0; r < NR; ++r) {
+    tile[r] = row[r] / few::TILE;
+    c[r] = cut.first(tile[r]) + threadIdx.y;
+    end[r] = cut.last(tile[r]);
+    left = max(left, end[r] - c[r] + 1);
 #pragma unroll
-      for (int j = 0; j < TOKS; ++j) v[j] = p[j * few::TILE];
-    } else {
+    for (int j = 0; j < TOKS; ++j) s[r][j] = 0.f;
+  }
+  for (; left > 0; left -= blockDim.y) {
+    float v[NR][TOKS];
 #pragma unroll
-      for (int j = 0; j < TOKS; ++j) v[j] = j < n ? p[j * few::TILE] : 0.f;
+    for (int r = 0; r < NR; ++r) {
+      const float* p = part + cut.at(c[r], tile[r]) + tok0 * few::TILE + row[r] % few::TILE;
+      const bool on = c[r] <= end[r];
+      if (n >= TOKS) {
+#pragma unroll
+        for (int j = 0; j < TOKS; ++j) v[r][j] = on ? p[j * few::TILE] : 0.f;
+      } else {
+#pragma unroll
+        for (int j = 0; j < TOKS; ++j) v[r][j] = on && j < n ? p[j * few::TILE] : 0.f;
+      }
+      c[r] += blockDim.y;
     }
 #pragma unroll
-    for (int j = 0; j < TOKS; ++j) s[j] += v[j];
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int j = 0; j < TOKS; ++j) s[r][j] += v[r][j];
   }
   if (blockDim.y == 1) return;
-  if (threadIdx.y > 0) {
 #pragma unroll
-    for (int j = 0; j < TOKS; ++j) share->s[threadIdx.y - 1][j][threadIdx.x] = s[j];
-  }
-  __syncthreads();
-  if (threadIdx.y == 0) {
-    for (int y = 1; y < blockDim.y; ++y)
+  for (int r = 0; r < NR; ++r) {
+    if (threadIdx.y > 0) {
 #pragma unroll
-      for (int j = 0; j < TOKS; ++j) s[j] += share->s[y - 1][j][threadIdx.x];
+      for (int j = 0; j < TOKS; ++j) share->s[threadIdx.y - 1][j][threadIdx.x] = s[r][j];
+    }
+    __syncthreads();
+    if (threadIdx.y == 0) {
+      for (int y = 1; y < blockDim.y; ++y)
+#pragma unroll
+        for (int j = 0; j < TOKS; ++j) s[r][j] += share->s[y - 1][j][threadIdx.x];
+    }
+    __syncthreads();
   }
 }
 // threads that share a tile's partial tiles
@@ -460,11 +481,10 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_gate_kernel(const f
   const int col = blockIdx.x * few::TILE + threadIdx.x, f = min(col, F - 1), tok0 = blockIdx.y * TOKS;   // past the last column: repeats it
   few::wait_for_input();
   few::let_next_start();
-  float g[TOKS], u[TOKS];
-  few_sum(part, cut, f, tok0, &share, g);
-  __syncthreads();
-  few_sum(part, cut, F + f, tok0, &share, u);
+  float s[2][TOKS];
+  few_sum<2>(part, cut, {f, F + f}, tok0, &share, s);
   if (threadIdx.y > 0) return;
+  const float (&g)[TOKS] = s[0], (&u)[TOKS] = s[1];
 #pragma unroll
   for (int j = 0; j < TOKS; ++j) {
     const long long tok = tok0 + j;
@@ -495,12 +515,12 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_sum_kernel(const fl
   __shared__ FewSums share;
   const int col = blockIdx.x * few::TILE + threadIdx.x, n = min(col, N - 1), tok0 = blockIdx.y * TOKS;
   few::wait_for_input();
-  float s[TOKS];
-  few_sum(part, cut, n, tok0, &share, s);
+  float s[1][TOKS];
+  few_sum<1>(part, cut, {n}, tok0, &share, s);
   if (threadIdx.y > 0 || col >= N) return;
 #pragma unroll
   for (int j = 0; j < TOKS; ++j)
-    if (tok0 + j < cut.tokens) y[(long long)(tok0 + j) * N + n] = __float2bfloat16(s[j]);
+    if (tok0 + j < cut.tokens) y[(long long)(tok0 + j) * N + n] = __float2bfloat16(s[0][j]);
 }
 
 // Tokens up to which the weights are streamed by few_rows.cu.  Device time, streamed and in tiles, in us:

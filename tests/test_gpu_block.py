@@ -716,3 +716,39 @@ def test_rows_behind_the_last_one_are_left_alone():
         _check_errors()
         assert (y[tokens:] == 7).all() and (h[tokens:] == 7).all() and (kept[size:] == 99).all() and (ws[floats:] == 5).all()
         _check_mlp(x[:tokens], w1, w2, "silu", y[:tokens])
+
+
+def test_offsets_beyond_32_bits():
+    """Tensors of more than 2^31 elements: their last rows are those of a small call on the same rows."""
+    R, W, tail = 530000, 4096, 300
+    y = torch.empty(R, W, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    w = _randn(W, mean=1.0, std=0.1)
+    with torch.no_grad():
+        n, h = F_.residual_rmsnorm(y, y, w, post_weight=w, gate=w)
+        n1, h1 = F_.residual_rmsnorm(y[-tail:], y[-tail:], w, post_weight=w, gate=w)
+        assert torch.equal(n[-tail:], n1) and torch.equal(h[-tail:], h1)
+        del h
+        g = F_.rmsnorm_gated(y, w, n, EPS, 512, False)
+        assert torch.equal(g[-tail:], F_.rmsnorm_gated(y[-tail:], w, n[-tail:], EPS, 512, False))
+    del g, n
+    leaf = y.requires_grad_()
+    grads = []
+    for t in (leaf, leaf[-tail:]):
+        out, h = F_.residual_rmsnorm(t, t, w)
+        grads.append(torch.autograd.grad([out, h], leaf, [t.detach(), t.detach()])[0][-tail:].clone())
+        del out, h
+    assert torch.equal(*grads)
+    del leaf, y
+    T, H, F = 66000, 64, 16400                      # 2 T F kept values
+    x, w1, w2 = _mlp_inputs((T,), H, F, H)
+    dy = _randn(T, H, std=0.1, seed=9)
+    out = []
+    for k in (T, 512):
+        leaf = x[-k:].detach().requires_grad_()
+        res = F_.gated_mlp(leaf, w1, w2)
+        out.append([res.detach()[-tail:], torch.autograd.grad(res, leaf, dy[-k:])[0][-tail:]])
+        del res
+    _check_errors()
+    # the two calls may cut their reductions differently: one fp32 sum against another, rounded once (2 u for values at a border)
+    for a, b in zip(*out):
+        assert (a.double() - b.double()).abs().max() <= 2 * 2 ** -8 * b.double().abs().max()
