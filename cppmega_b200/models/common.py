@@ -10,6 +10,7 @@ import torch.nn as nn
 from ..ops import functional as F_
 from ..parallel.state import ParallelContext
 from ..parallel.tensor_parallel import ColumnParallelLinear, RowParallelLinear
+from ..utils import fp8_activations
 
 
 def seed_for(name: str, base: int = 1234) -> int:
@@ -50,9 +51,9 @@ class DenseMLP(nn.Module):
                                             seed=seed_for(name + ".linear_fc2", seed), name=name + ".linear_fc2")
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        # as one operator where the two linears are plain products: no tensor parallelism, and nothing hooked to them (a precision
-        # rule or a probe on one of them wants its calls)
-        if self.pc.tp == 1 and not (_hooked(self.linear_fc1) or _hooked(self.linear_fc2)):
+        # as one operator where the two linears are plain products: no tensor parallelism, nothing hooked to them (a precision
+        # rule or a probe on one of them wants its calls), and no FP8 storage of what is kept for backward
+        if self.pc.tp == 1 and not (_hooked(self.linear_fc1) or _hooked(self.linear_fc2) or fp8_activations.packing()):
             return F_.gated_mlp(x, self.linear_fc1.weight, self.linear_fc2.weight)
         return self.linear_fc2(F_.swiglu(self.linear_fc1(x)))
 

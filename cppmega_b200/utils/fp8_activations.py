@@ -190,6 +190,22 @@ class LayerAwareFp8Packer(Fp8ActivationPacker):
         return super().pack(t)
 
 
+class _PackingContext(torch.autograd.graph.saved_tensors_hooks):
+    def __enter__(self):
+        _state.packing = getattr(_state, "packing", 0) + 1
+        return super().__enter__()
+
+    def __exit__(self, *exc):
+        _state.packing -= 1
+        return super().__exit__(*exc)
+
+
+def packing() -> bool:
+    """Whether saved activations are being compressed: operators that keep them in a form of their own (bytes the hooks pass over)
+    step back for their plain composition then."""
+    return getattr(_state, "packing", 0) > 0 and not _disabled()
+
+
 def fp8_activation_context(*, recipe: str = "mxfp8", n_layers: int = 0, bf16_first: int = 0, bf16_last: int = 0,
                            clamp: bool = False, min_elements: int = MIN_ELEMENTS, enabled: bool = True):
     """Context manager under which saved activations are FP8-compressed (``enabled=False``: a no-op context)."""
@@ -200,4 +216,4 @@ def fp8_activation_context(*, recipe: str = "mxfp8", n_layers: int = 0, bf16_fir
                                                           min_elements=min_elements)
     else:
         packer = Fp8ActivationPacker(recipe=recipe, clamp=clamp, min_elements=min_elements)
-    return torch.autograd.graph.saved_tensors_hooks(packer.pack, packer.unpack)
+    return _PackingContext(packer.pack, packer.unpack)

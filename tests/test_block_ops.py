@@ -157,6 +157,23 @@ def test_dense_mlp_is_the_operator_and_heeds_hooks():
     assert len(seen) == n
 
 
+def test_dense_mlp_leaves_saved_activations_to_the_packer(monkeypatch):
+    from cppmega_b200.utils import fp8_activations as fa
+    m, x = _mlp(), _r(2, 5, 32).float()
+    calls = []
+    monkeypatch.setattr(F_, "gated_mlp", lambda *a: calls.append(1) or x)
+    with fa.fp8_activation_context():
+        assert fa.packing()
+        m(x)
+        with fa.fp8_quantize_disabled():
+            assert not fa.packing()
+            m(x)
+    assert not fa.packing() and len(calls) == 1
+    with fa.fp8_activation_context(enabled=False):
+        m(x)
+    assert len(calls) == 2
+
+
 def test_dense_mlp_under_a_recipe_stays_two_linears(monkeypatch):
     m, x = _mlp(), _r(2, 5, 32).float()
     calls = []
