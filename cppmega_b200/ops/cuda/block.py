@@ -162,7 +162,7 @@ def gated_mlp(x, w1, w2, activation):
     """None where the kernels do not apply: they take bf16 throughout and widths that are multiples of 8."""
     if not (x.dtype == w1.dtype == w2.dtype == torch.bfloat16 and w1.is_contiguous() and w2.is_contiguous() and x.numel() > 0
             and x.shape[-1] % 8 == 0 and w2.shape[0] % 8 == 0 and w2.shape[1] % 8 == 0 and w1.data_ptr() % 16 == 0
-            and w2.data_ptr() % 16 == 0 and x.numel() // x.shape[-1] < 2 ** 31):
+            and w2.data_ptr() % 16 == 0 and x.numel() // x.shape[-1] < 2 ** 30):
         return None
     with _device_of(x):
         if torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad):

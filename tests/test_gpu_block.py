@@ -292,15 +292,13 @@ def test_rmsnorm_gated_large_gates():
 # ---- dense products with shared last tiles --------------------------------------------------------------------------
 
 @pytest.mark.parametrize("a_mn,b_mn", [(False, False), (False, True), (True, True), (True, False)])
-@pytest.mark.parametrize("M,N,K", [(512, 1024, 4096), (300, 136, 1032), (2064, 520, 8200), (5000, 1032, 4104), (256, 256, 16384), (40, 8, 2000)])
+@pytest.mark.parametrize("M,N,K", [(512, 1024, 4096), (304, 136, 1032), (2064, 520, 8200), (5000, 1032, 4104), (256, 256, 16384), (40, 8, 2000)])
 @pytest.mark.parametrize("fp32,accumulate", [(False, False), (True, True), (False, True)])
 def test_gemm_split(a_mn, b_mn, M, N, K, fp32, accumulate):
     import ctypes
     from cppmega_b200.ops import cuda as cu
     L = cu.lib()
     a, b = _randn(*((K, M) if a_mn else (M, K))), _randn(*((K, N) if b_mn else (N, K)), seed=1)
-    if a_mn and M % 8:
-        pytest.skip("rows of 16 bytes")
     c0 = _randn(M, N, dtype=torch.float32 if fp32 else torch.bfloat16, seed=2)
     plan = (ctypes.c_int * 4)()
     floats = L.cm_gemm_split_plan(torch.cuda.get_device_properties(0).multi_processor_count, M, N, K, int(b_mn), plan)
@@ -463,15 +461,37 @@ def test_gated_mlp_gradients_of_far_apart_magnitudes(T):
         _check_mlp(*leaves, name, y, dict(zip(("x", "w1", "w2"), grads)), dy)
 
 
-def test_gated_mlp_nan_stays_in_its_row():
-    x, w1, w2 = _mlp_inputs((20,), 64, 72, 64)
+@pytest.mark.parametrize("name", ["silu", "gelu_tanh", "relu"])
+@pytest.mark.parametrize("T", [20, 90])
+def test_gated_mlp_nan_stays_in_its_row(T, name):
+    x, w1, w2 = _mlp_inputs((T,), 64, 72, 64)
     for grad in (False, True):
         xx = x.clone()
         xx[4, 7] = float("nan")
-        y = F_.gated_mlp(xx.requires_grad_(grad), w1, w2).detach()
+        y = F_.gated_mlp(xx.requires_grad_(grad), w1, w2, name).detach()
         assert torch.isnan(y[4].float()).all()
-        keep = [i for i in range(20) if i != 4]
+        keep = [i for i in range(T) if i != 4]
         assert torch.isfinite(y[keep].float()).all()
+
+
+@pytest.mark.parametrize("name", ["silu", "gelu_tanh", "relu"])
+@pytest.mark.parametrize("T", [20, 90])
+def test_gated_mlp_far_out(T, name):
+    """Gates of 1e3 to 1e18 on both sides: the activation is 0 or the gate, its slope 0 or 1, and nothing overflows on the way."""
+    x = torch.ones(T, 8, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    size = torch.tensor([1e3, 1e6, 1e10, 1e14, 1e18, 30.0, 200.0, 1e5], device="cuda")
+    w1 = torch.zeros(32, 8, device="cuda")
+    w1[:8, 0], w1[8:16, 0] = size, -size
+    w1[16:, 0] = 1.0
+    w1, w2 = w1.bfloat16(), torch.full((8, 16), 2.0 ** -70, device="cuda", dtype=torch.bfloat16)
+    y = F_.gated_mlp(x, w1, w2, name)
+    (dx,) = torch.autograd.grad(y, x, torch.full_like(y, 2.0 ** 70))
+    kept = w1[:8, 0].double()
+    # y is the sum of the positive gates; dx[0] is 8 times that sum twice over: once through the slopes, once through act(g)
+    total = kept.sum() * 2.0 ** -70
+    assert ((y.double() - total).abs() <= 3 * 2 ** -8 * total).all()
+    want = 8 * 2 * kept.sum()
+    assert ((dx[:, 0].double() - want).abs() <= 5 * 2 ** -8 * want).all() and torch.isfinite(dx.float()).all()
 
 
 def test_gated_mlp_against_differences():
