@@ -84,11 +84,17 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         tma_load_2d(sb, &tmX, &full_bar[stage], k0, 0);
         if (args.two) tma_load_2d(sb + b_bytes, &tmX2, &full_bar[stage], k0, 0);
       };
-      // the ring's first round of weights does not wait for the tokens
+      // behind another kernel the ring's first round of weights does not wait for the tokens; with the tokens at hand theirs go along
+      // (behind 200 KB of weights a block the first tile of them arrived 4.7 us after the start)
       const long long head = begin + args.stages < end ? begin + args.stages : end;
-      for (long long kb = begin; kb < head; ++kb) weights(kb, uint32_t(kb - begin));
-      if (args.early) wait_for_input();
-      for (long long kb = begin; kb < head; ++kb) tokens(kb, uint32_t(kb - begin));
+      for (long long kb = begin; kb < head; ++kb) {
+        weights(kb, uint32_t(kb - begin));
+        if (!args.early) tokens(kb, uint32_t(kb - begin));
+      }
+      if (args.early) {
+        wait_for_input();
+        for (long long kb = begin; kb < head; ++kb) tokens(kb, uint32_t(kb - begin));
+      }
       uint32_t stage = 0, phase = 0;                                    // the first round's release of a stage
       for (long long kb = head; kb < end; ++kb) {
         if (!mbar_wait(&empty_bar[stage], phase, abort_flag, args.err, ERR_WAIT_EMPTY)) break;

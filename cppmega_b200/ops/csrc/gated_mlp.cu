@@ -529,10 +529,10 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_sum_kernel(const fl
 
 // Tokens up to which the weights are streamed by few_rows.cu.  Device time, streamed and in tiles, in us:
 //   hidden x ffn    1 token       24           64          128
-//   4096 x 21504    96 / 144     98 / 115    105 / 117    116 / 123
-//   3584 x 18944    77 / 101     78 /  83     84 /  85     93 /  90
-//   1024 x  2048    13 /  20     15 /  18     16 /  18     19 /  20
-//    256 x   512    11 /  10     12 /  10     12 /  10     11 /  11
+//   4096 x 21504    93 / 144     98 / 115    104 / 118    116 / 123
+//   3584 x 18944    76 / 101     77 /  83     82 /  86     91 /  90
+//   1024 x  2048    13 /  20     14 /  18     15 /  18     19 /  20
+//    256 x   512    11 /  10     11 /  10     12 /  10     11 /  11
 constexpr int FEW_TOKENS = few::MAX_ROWS / 4;
 
 // floats of the partial tiles, the larger of the two products', in whole 16 bytes; lo lies behind them
