@@ -34,7 +34,7 @@ struct ResidualArgs {
 
 template <typename T, int TPR, int VPT, bool VEC, bool FULL>
 __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_fwd(const ResidualArgs a) {
-  constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
+  constexpr int H = RowVec<T>::N / 2, RPB = rv_block<TPR>() / TPR;
   __shared__ float red[2 * (TPR > 32 ? TPR / 32 : 1)];
   const int t = threadIdx.x % TPR, W = a.width;
   const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
@@ -51,72 +51,76 @@ __global__ void __launch_bounds__(rv_block<TPR>()) residual_norm_fwd(const Resid
   float r = 1.f;
   const bool post = FULL && a.post;
   if (post) {
-    float ss[1] = {0.f};
+    Pair sq = {};
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float f[N];
+      Pair f[H];
       rv_unpack<T>(yv[i], f);
 #pragma unroll
-      for (int j = 0; j < N; ++j) ss[0] += f[j] * f[j];
+      for (int j = 0; j < H; ++j) sq = pr_fma(f[j], f[j], sq);
     }
+    float ss[1] = {pr_sum(sq)};
     rv_team_sum<TPR, 1>(ss, red, 0);
     r = rsqrtf(ss[0] / W + a.eps);
     if (on && t == 0 && a.rstd_y) a.rstd_y[row] = r;
   }
-  float ss[1] = {0.f};
+  Pair sq = {};
+  const Pair sr = pr(a.scale * r);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    float y[N], x[N];
+    Pair y[H], x[H];
     rv_unpack<T>(yv[i], y);
     rv_unpack<T>(hv[i], x);
     if constexpr (FULL) {
       if (post) {
-        float p[N];
+        Pair p[H];
         rv_unpack<T>(rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.post), t, i, W), p);
 #pragma unroll
-        for (int j = 0; j < N; ++j) y[j] *= r * p[j];
+        for (int j = 0; j < H; ++j) y[j] = y[j] * p[j];
       }
       if (a.gate) {
-        float g[N];
+        Pair g[H];
         rv_unpack<T>(rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.gate) + (a.gate_rows ? row * W : 0ll), t, i, w_on), g);
 #pragma unroll
-        for (int j = 0; j < N; ++j) y[j] *= g[j];
+        for (int j = 0; j < H; ++j) y[j] = y[j] * g[j];
       }
     }
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] += a.scale * y[j];
+    for (int j = 0; j < H; ++j) x[j] = pr_fma(sr, y[j], x[j]);
     hv[i] = rv_pack<T>(x);
     rv_unpack<T>(hv[i], x);                   // the stream's value
 #pragma unroll
-    for (int j = 0; j < N; ++j) ss[0] += x[j] * x[j];
+    for (int j = 0; j < H; ++j) sq = pr_fma(x[j], x[j], sq);
   }
+  float ss[1] = {pr_sum(sq)};
   rv_team_sum<TPR, 1>(ss, red, 1);
   const float rho = rsqrtf(ss[0] / W + a.eps);
   if (!on) return;
   if (t == 0 && a.rstd_h) a.rstd_h[row] = rho;
   T* hr = reinterpret_cast<T*>(a.h) + row * W;
   T* nr = reinterpret_cast<T*>(a.n) + row * W;
+  const Pair rho2 = pr(rho);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    float x[N], w[N];
+    Pair x[H], w[H];
     rv_unpack<T>(hv[i], x);
     rv_unpack<T>(rv_load<T, TPR, VEC>(reinterpret_cast<const T*>(a.w), t, i, W), w);
     rv_store<T, TPR, VEC>(hr, t, i, W, hv[i]);
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = x[j] * rho * w[j];
+    for (int j = 0; j < H; ++j) x[j] = x[j] * rho2 * w[j];
     rv_store<T, TPR, VEC>(nr, t, i, W, rv_pack<T>(x));
   }
 }
 
 template <typename T, int TPR, int VPT, bool VEC, bool FULL>
 __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : (FULL ? 512 : 768) / rv_block<TPR>()) residual_norm_bwd(const ResidualArgs a) {
-  constexpr int N = RowVec<T>::N, RPB = rv_block<TPR>() / TPR;
+  constexpr int N = RowVec<T>::N, H = N / 2, RPB = rv_block<TPR>() / TPR;
   extern __shared__ __align__(16) uint4 dyn[];
   __shared__ float red[2 * (FULL ? 3 : 1) * (TPR > 32 ? TPR / 32 : 1)];
   __shared__ float scratch[RPB > 1 ? RPB * TPR * VPT * N : 1];
   enum { HH = 0, DN = 1, DH = 2, YY = 3, GG = 4 };
   const int t = threadIdx.x % TPR, W = a.width;
-  float acc_w[VPT][N] = {}, acc_y[FULL ? VPT : 1][N] = {};
+  Pair acc_w[VPT][H] = {}, acc_y[FULL ? VPT : 1][H] = {};
   const bool post = FULL && a.post, gate = FULL && a.gate;
   RowRing<T, TPR, VPT, VEC, rv_stages(TPR, VPT), FULL ? 5 : 3> in;
   in.ops = a.ring_ops;
@@ -164,73 +168,83 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
       }
     }
     // s[0] = sum g h, s[1] = sum gate post y (rho g + dh0), s[2] = sum gate post y h: the constant factors follow behind the sums
-    float s[FULL ? 3 : 1] = {};
-    float dt[VPT][N], hv[FULL ? 1 : VPT][N];                // rho g + dh0, h
+    Pair sp[FULL ? 3 : 1] = {};
+    Pair dt[VPT][H];                                        // rho g + dh0
+    const Pair rho2 = pr(rho);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float g[N], h[N], w[N];
+      Pair g[H], h[H], w[H];
       rv_unpack<T>(in.get(DN, i), g);
       rv_unpack<T>(in.get(HH, i), h);
       rv_unpack<T>(in.get(DH, i), dt[i]);
       rv_unpack<T>(wv[i], w);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        acc_w[i][j] += g[j] * (h[j] * rho);
-        g[j] *= w[j];
-        s[0] += g[j] * h[j];
-        dt[i][j] += rho * g[j];
-        if constexpr (!FULL) hv[i][j] = h[j];
+      for (int j = 0; j < H; ++j) {
+        acc_w[i][j] = pr_fma(g[j], h[j] * rho2, acc_w[i][j]);
+        g[j] = g[j] * w[j];
+        sp[0] = pr_fma(g[j], h[j], sp[0]);
+        dt[i][j] = pr_fma(rho2, g[j], dt[i][j]);
       }
       if constexpr (FULL) {
-        float y[N], p[N], q[N];
+        Pair y[H], p[H], q[H];
         rv_unpack<T>(in.get(YY, i), y);
         rv_unpack<T>(pv[i], p);
         rv_unpack<T>(a.gate_rows ? in.get(GG, i) : tv[i], q);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float ay = p[j] * q[j] * y[j];
-          s[1] += ay * dt[i][j];
-          s[2] += ay * h[j];
+        for (int j = 0; j < H; ++j) {
+          const Pair ay = p[j] * q[j] * y[j];
+          sp[1] = pr_fma(ay, dt[i][j], sp[1]);
+          sp[2] = pr_fma(ay, h[j], sp[2]);
         }
       }
     }
+    float s[FULL ? 3 : 1];
+#pragma unroll
+    for (int k = 0; k < (FULL ? 3 : 1); ++k) s[k] = pr_sum(sp[k]);
     rv_team_sum<TPR, FULL ? 3 : 1>(s, red, turn);
-    const float k = rho * rho * rho * s[0] * inv_w;         // dh = rho g + dh0 - k h
+    const float k = rho * s[0] * inv_w * rho * rho;         // dh = rho g + dh0 - k h; rho^3 alone may underflow
     float m2 = 0.f;                                         // mean(gate post dh yh)
     if constexpr (FULL) m2 = post ? r * (s[1] - k * s[2]) * inv_w : 0.f;
-    const float sr = a.scale * r;
+    const Pair k2 = pr(-k), r2 = pr(r), sr2 = pr(a.scale * r), m22 = pr(-m2), scale2 = pr(a.scale);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float d[N];
-      if constexpr (FULL) {
-        rv_unpack<T>(in.get(HH, i), d);
+      Pair d[H];
+      rv_unpack<T>(in.get(HH, i), d);
 #pragma unroll
-        for (int j = 0; j < N; ++j) d[j] = dt[i][j] - k * d[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) d[j] = dt[i][j] - k * hv[i][j];
-      }
+      for (int j = 0; j < H; ++j) d[j] = pr_fma(k2, d[j], dt[i][j]);
       rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.dres) + row * W, t, i, on ? W : 0, rv_pack<T>(d));
       if constexpr (FULL) {
-        float y[N], p[N], q[N];
+        Pair y[H], p[H], q[H];
         rv_unpack<T>(in.get(YY, i), y);
         rv_unpack<T>(pv[i], p);
-        rv_unpack<T>(a.gate_rows ? in.get(GG, i) : tv[i], q);
-        if (a.dgate_rows) {
-          float dg[N];
+        if (a.gate_rows) {
+          rv_unpack<T>(in.get(GG, i), q);
+          if (a.dgate_rows) {
+            Pair dg[H];
 #pragma unroll
-          for (int j = 0; j < N; ++j) dg[j] = sr * d[j] * (y[j] * p[j]);
-          rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.dgate_rows) + row * W, t, i, on ? W : 0, rv_pack<T>(dg));
+            for (int j = 0; j < H; ++j) dg[j] = sr2 * d[j] * (y[j] * p[j]);
+            rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.dgate_rows) + row * W, t, i, on ? W : 0, rv_pack<T>(dg));
+          }
+#pragma unroll
+          for (int j = 0; j < H; ++j) {
+            y[j] = y[j] * r2;
+            d[j] = d[j] * q[j];
+            acc_y[i][j] = pr_fma(d[j], y[j], acc_y[i][j]);
+          }
+        } else {
+          rv_unpack<T>(tv[i], q);
+#pragma unroll
+          for (int j = 0; j < H; ++j) {
+            y[j] = y[j] * r2;
+            acc_y[i][j] = pr_fma(d[j], y[j], acc_y[i][j]);
+            d[j] = d[j] * q[j];
+          }
         }
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float yh = y[j] * r, e = d[j] * q[j];
-          acc_y[i][j] += (a.gate_rows ? e : d[j]) * yh;
-          d[j] = sr * (e * p[j] - yh * m2);
-        }
+        for (int j = 0; j < H; ++j) d[j] = sr2 * pr_fma(m22, y[j], d[j] * p[j]);
       } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) d[j] *= a.scale;
+        for (int j = 0; j < H; ++j) d[j] = d[j] * scale2;
       }
       if (a.dy) rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.dy) + row * W, t, i, on ? W : 0, rv_pack<T>(d));
     }
@@ -243,13 +257,12 @@ __global__ void __launch_bounds__(rv_block<TPR>(), rv_block<TPR>() >= 512 ? 1 : 
     // with a gate per channel both its gradient and the post norm's are the sum of dh yh, times the other one's factor; with a gate per
     // element the sum already holds the gate
     auto out = [&](float* part, const uint4 (&factor)[VPT]) {
-      float sum[VPT][N];
+      Pair sum[VPT][H];
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        float f[N];
-        rv_unpack<T>(factor[i], f);
+        rv_unpack<T>(factor[i], sum[i]);
 #pragma unroll
-        for (int j = 0; j < N; ++j) sum[i][j] = a.scale * f[j] * acc_y[i][j];
+        for (int j = 0; j < H; ++j) sum[i][j] = pr(a.scale) * sum[i][j] * acc_y[i][j];
       }
       rv_partial<T, TPR, VPT, VEC>(sum, part + at, W, scratch);
     };

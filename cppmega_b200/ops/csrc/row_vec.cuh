@@ -65,6 +65,63 @@ __device__ __forceinline__ float rv_sigmoid(float z) {
   return q;
 }
 
+// Two fp32 values that one instruction works on (fma.rn.f32x2): the backward kernels are short of issue slots, not of arithmetic.
+struct Pair {
+  unsigned long long v;
+};
+__device__ __forceinline__ Pair pr(float lo, float hi) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ Pair pr(float both) { return pr(both, both); }
+__device__ __forceinline__ float2 pr_get(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+  return f;
+}
+__device__ __forceinline__ float pr_sum(Pair p) {
+  const float2 f = pr_get(p);
+  return f.x + f.y;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair pr_fma(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+
+template <typename T>
+__device__ __forceinline__ void rv_unpack(const uint4& v, Pair (&f)[RowVec<T>::N / 2]) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < RowVec<T>::N / 2; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      f[j] = pr(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
+    } else if constexpr (__is_same(T, __half)) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+      f[j] = pr(p.x, p.y);
+    } else {
+      f[j] = pr(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 rv_pack(const Pair (&f)[RowVec<T>::N / 2]) {
+  float g[RowVec<T>::N];
+#pragma unroll
+  for (int j = 0; j < RowVec<T>::N / 2; ++j) {
+    const float2 p = pr_get(f[j]);
+    g[2 * j] = p.x;
+    g[2 * j + 1] = p.y;
+  }
+  return rv_pack<T>(g);
+}
+
 // Keeps a vector packed: its unpacked values are formed again after this point instead of being held in registers.
 __device__ __forceinline__ void rv_keep_packed(uint4& v) { asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)); }
 
@@ -178,6 +235,20 @@ __device__ __forceinline__ void rv_partial(const float (&acc)[VPT][RowVec<T>::N]
       out[c] = s;
     }
   }
+}
+
+template <typename T, int TPR, int VPT, bool VEC>
+__device__ __forceinline__ void rv_partial(const Pair (&pairs)[VPT][RowVec<T>::N / 2], float* __restrict__ out, int width, float* scratch) {
+  float acc[VPT][RowVec<T>::N];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int j = 0; j < RowVec<T>::N / 2; ++j) {
+      const float2 p = pr_get(pairs[i][j]);
+      acc[i][2 * j] = p.x;
+      acc[i][2 * j + 1] = p.y;
+    }
+  rv_partial<T, TPR, VPT, VEC>(acc, out, width, scratch);
 }
 
 // The operand rows of a backward kernel on their way in.  Every thread copies its own vectors of the next NS rows into shared memory
