@@ -6,8 +6,8 @@ projection are read in place), widths that no vector divides.  Work space is all
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -53,9 +53,31 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _device_of(t: torch.Tensor):
-    """Launches go to the device of the tensors, whichever is current."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _on_device(fn):
+    """Launches go to the device of the tensors (the first argument's), whichever is current."""
+    @functools.wraps(fn)
+    def call(t, *args):
+        if not t.is_cuda or t.get_device() == torch._C._cuda_getDevice():
+            return fn(t, *args)
+        with torch.cuda.device(t.device):
+            return fn(t, *args)
+    return call
+
+
+def _first_order(fn):
+    """``backward`` without a graph of its own.  Only under ``create_graph`` does it go through the library's guard, which makes a second
+    derivative raise (the guard costs as much as a launch)."""
+    guarded = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+    return backward
+
+
+@functools.lru_cache(maxsize=1024)
+def _size(name: str, device: int, *args) -> int:
+    """The library's answer to a question about sizes on the current device."""
+    return getattr(_cu.lib(), name)(*args)
 
 
 def _rows(t: torch.Tensor):
@@ -106,8 +128,8 @@ def _mlp_forward(x, w1, w2, act, keep):
     M = x.numel() // H
     y = _like(x) if Ho == H else x.new_empty(*x.shape[:-1], Ho)
     h = x.new_empty(M, F)
-    kept = torch.empty(L.cm_gated_mlp_kept(M, F), dtype=torch.uint8, device=x.device) if keep else None
-    floats = L.cm_gated_mlp_fwd_ws(M, H, F, Ho)
+    kept = torch.empty(_size("cm_gated_mlp_kept", x.get_device(), M, F), dtype=torch.uint8, device=x.device) if keep else None
+    floats = _size("cm_gated_mlp_fwd_ws", x.get_device(), M, H, F, Ho)
     ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
     rc = L.cm_gated_mlp_fwd(x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), _ptr(kept), h.data_ptr(), y.data_ptr(), _ptr(ws), M, H, F, Ho,
                             act, _cu.err_word(x.device).data_ptr(), _cu.stream_ptr())
@@ -126,7 +148,7 @@ class GatedMLPFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, w1, w2, kept, h = ctx.saved_tensors
         need_x, need_w1, need_w2, _ = ctx.needs_input_grad
@@ -147,7 +169,7 @@ class GatedMLPFn(torch.autograd.Function):
         dw2 = _cu.wgrad_into_main_grad(w2, target(1, w2)) if need_w2 else None
         dgu = x.new_empty(h.shape[0], 2 * F) if need_x or need_w1 else None
         L, M = _cu.lib(), h.shape[0]
-        floats = L.cm_gated_mlp_bwd_ws(M, H, F, Ho)
+        floats = _size("cm_gated_mlp_bwd_ws", x.get_device(), M, H, F, Ho)
         ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
         rc = L.cm_gated_mlp_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, w1.data_ptr(), w2.data_ptr(), kept.data_ptr(), h.data_ptr(),
                                 _ptr(dgu), _ptr(dx), *into[0], *into[1], _ptr(ws), M, H, F, Ho, ctx.act,
@@ -158,16 +180,16 @@ class GatedMLPFn(torch.autograd.Function):
         return dx, dw1, dw2, None
 
 
+@_on_device
 def gated_mlp(x, w1, w2, activation):
     """None where the kernels do not apply: they take bf16 throughout and widths that are multiples of 8."""
     if not (x.dtype == w1.dtype == w2.dtype == torch.bfloat16 and w1.is_contiguous() and w2.is_contiguous() and x.numel() > 0
             and x.shape[-1] % 8 == 0 and w2.shape[0] % 8 == 0 and w2.shape[1] % 8 == 0 and w1.data_ptr() % 16 == 0
             and w2.data_ptr() % 16 == 0 and x.numel() // x.shape[-1] < 2 ** 30):
         return None
-    with _device_of(x):
-        if torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad):
-            return GatedMLPFn.apply(x, w1, w2, ACTIVATIONS[activation])
-        return _mlp_forward(x, w1, w2, ACTIVATIONS[activation], keep=False)[0]
+    if torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad):
+        return GatedMLPFn.apply(x, w1, w2, ACTIVATIONS[activation])
+    return _mlp_forward(x, w1, w2, ACTIVATIONS[activation], keep=False)[0]
 
 
 # ---------------------------------------------------------------------------
@@ -202,7 +224,7 @@ class ResidualRMSNormFn(torch.autograd.Function):
         return n, h
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dn, dh):
         if dn is None and dh is None:
             return (None,) * 7
@@ -226,7 +248,7 @@ class ResidualRMSNormFn(torch.autograd.Function):
         dpost = torch.empty_like(post) if need_post else None
         sums = need_w + need_post + (need_gate and not per_row)
         L = _cu.lib()
-        part = torch.empty(sums * L.cm_residual_rmsnorm_parts(R, W) * W, dtype=torch.float32, device=h.device) if sums else None
+        part = torch.empty(sums * _size("cm_residual_rmsnorm_parts", h.get_device(), R, W) * W, dtype=torch.float32, device=h.device) if sums else None
         at = stats.data_ptr()
         rc = L.cm_residual_rmsnorm_bwd(_ptr(dn), sdn, _ptr(dh), sdh, h.data_ptr(), _ptr(y), sy, weight.data_ptr(), _ptr(post), _ptr(gate),
                                        int(per_row), at, at + 4 * R, dres.data_ptr(), _ptr(dy), _ptr(dgate) if per_row else None, _ptr(dw),
@@ -238,6 +260,7 @@ class ResidualRMSNormFn(torch.autograd.Function):
         return (dres if same else dy), dres, dw, dpost, dgate, None, None
 
 
+@_on_device
 def residual_rmsnorm(y, residual, weight, post_weight, gate, scale, eps):
     """None where the kernels do not apply: one type for all tensors (bf16, fp16 or fp32), rows of at most 16384."""
     dt = y.dtype
@@ -249,11 +272,10 @@ def residual_rmsnorm(y, residual, weight, post_weight, gate, scale, eps):
         post_weight = post_weight.contiguous()
     if gate is not None:
         gate = gate.contiguous()
-    with _device_of(y):
-        if torch.is_grad_enabled() and (y.requires_grad or residual.requires_grad or weight.requires_grad
-                                        or (post_weight is not None and post_weight.requires_grad) or (gate is not None and gate.requires_grad)):
-            return ResidualRMSNormFn.apply(y, residual, weight, post_weight, gate, float(scale), float(eps))
-        return _residual_forward(y, residual, weight, post_weight, gate, float(scale), float(eps), keep=False)[:2]
+    if torch.is_grad_enabled() and (y.requires_grad or residual.requires_grad or weight.requires_grad
+                                    or (post_weight is not None and post_weight.requires_grad) or (gate is not None and gate.requires_grad)):
+        return ResidualRMSNormFn.apply(y, residual, weight, post_weight, gate, float(scale), float(eps))
+    return _residual_forward(y, residual, weight, post_weight, gate, float(scale), float(eps), keep=False)[:2]
 
 
 # ---------------------------------------------------------------------------
@@ -286,7 +308,7 @@ class GatedRMSNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, weight, z, rstd = ctx.saved_tensors
         _, need_w, need_z = ctx.needs_input_grad[:3]
@@ -303,7 +325,7 @@ class GatedRMSNormFn(torch.autograd.Function):
         L = _cu.lib()
         if need_w:
             dw = torch.empty_like(weight)
-            part = torch.empty(L.cm_rmsnorm_gated_parts(R, W, ctx.group) * W, dtype=torch.float32, device=x.device)
+            part = torch.empty(_size("cm_rmsnorm_gated_parts", x.get_device(), R, W, ctx.group) * W, dtype=torch.float32, device=x.device)
         rc = L.cm_rmsnorm_gated_bwd(x.data_ptr(), sx, _ptr(z), sz, weight.data_ptr(), dy.data_ptr(), sdy, rstd.data_ptr(), dx.data_ptr(),
                                     _ptr(dz), _ptr(dw), _ptr(part), R, W, ctx.group, int(ctx.gate_first), ROW_TYPES[x.dtype],
                                     _cu.stream_ptr())
@@ -313,6 +335,7 @@ class GatedRMSNormFn(torch.autograd.Function):
         return dx, dw, dz, None, None, None
 
 
+@_on_device
 def rmsnorm_gated(x, weight, z, eps, group, norm_before_gate):
     """None where the kernels do not apply: one type for all tensors (bf16, fp16 or fp32), groups of at most 16384 channels and at
     most 65535 of them."""
@@ -321,10 +344,9 @@ def rmsnorm_gated(x, weight, z, eps, group, norm_before_gate):
             or x.shape[-1] // group > 65535):
         return None
     weight = weight.contiguous()
-    with _device_of(x):
-        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (z is not None and z.requires_grad)):
-            return GatedRMSNormFn.apply(x, weight, z, float(eps), group, not norm_before_gate)
-        return _gated_forward(x, weight, z, float(eps), group, not norm_before_gate, keep=False)[0]
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (z is not None and z.requires_grad)):
+        return GatedRMSNormFn.apply(x, weight, z, float(eps), group, not norm_before_gate)
+    return _gated_forward(x, weight, z, float(eps), group, not norm_before_gate, keep=False)[0]
 
 
 def register() -> None:

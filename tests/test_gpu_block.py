@@ -772,3 +772,16 @@ def test_offsets_beyond_32_bits():
     # the two calls may cut their reductions differently: one fp32 sum against another, rounded once (2 u for values at a border)
     for a, b in zip(*out):
         assert (a.double() - b.double()).abs().max() <= 2 * 2 ** -8 * b.double().abs().max()
+
+
+def test_first_derivatives_only():
+    """Gradients under ``create_graph`` are right; differentiating them again raises."""
+    x = _randn(30, 64).requires_grad_()
+    w1, w2 = _randn(144, 64, std=0.1, seed=1).requires_grad_(), _randn(64, 72, std=0.1, seed=2)
+    w = _randn(64, mean=1.0, std=0.1, seed=3)
+    for call in (lambda: F_.gated_mlp(x, w1, w2), lambda: F_.residual_rmsnorm(x, x, w)[0], lambda: F_.rmsnorm_gated(x, w, x)):
+        (plain,) = torch.autograd.grad(call().sum(), x)
+        (g,) = torch.autograd.grad(call().sum(), x, create_graph=True)
+        assert torch.equal(plain, g)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
