@@ -190,3 +190,34 @@ def test_norm_module_with_a_gate():
     silu = z * torch.sigmoid(z)
     assert torch.allclose(m(x, gate=z), m(x) * silu, rtol=1e-5, atol=1e-6)
     assert torch.allclose(m(x, gate=z, norm_before_gate=False), m(x * silu), rtol=1e-5, atol=1e-6)
+
+
+def test_calls_go_to_the_device_of_their_tensors(monkeypatch):
+    """With another device current, the call runs with the tensors' device current and puts the other one back."""
+    from cppmega_b200.ops.cuda import block
+
+    class On:
+        is_cuda, device = True, "cuda:1"
+
+        def get_device(self):
+            return 1
+
+    class Guard:
+        def __init__(self, d):
+            seen.append(d)
+
+        def __enter__(self):
+            seen.append("in")
+
+        def __exit__(self, *exc):
+            seen.append("out")
+
+    seen = []
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    assert block._on_device(lambda t, a: seen.append("call") or a)(On(), 5) == 5
+    assert seen == ["cuda:1", "in", "call", "out"]
+    seen.clear()
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1, raising=False)
+    block._on_device(lambda t: seen.append("call"))(On())
+    assert seen == ["call"]
