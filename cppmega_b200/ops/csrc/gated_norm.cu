@@ -5,7 +5,8 @@
 //   du = r (dn w - xh mean(dn w xh));  dw = sum dn xh
 //   norm first:  dx = du,  dz = dy xh w a'(z)         gate first:  dx = du a(z),  dz = du x a'(z)
 // A team of threads holds one group of one row; blockIdx.y is the group, so that a thread keeps its channels over the rows of the
-// backward and adds their weight gradient in registers.  Bound by memory: three rows moved forward, five backward; the gate is read
+// backward and adds their weight gradient in registers.  Bound by memory: three rows moved forward, five backward (16384 x 8192 in groups of
+// 1024, bf16: 134 us and 219, at the copy rate 125 and 208; with the gate first 139 and 280); the gate is read
 // where it lies (a column slice of the projection has its own pitch).  The weight gradient is summed in a fixed order.
 #include "row_vec.cuh"
 #define CM_ROW_TEAM_BY_WARP(team, F) if (team == 16 * 32 + 4) return F(32, 4, true);
