@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 
 #include "few_rows.cuh"
+#include "fp32_pair.cuh"
 #include "gemm_split.cuh"
 #include "pair_issue.cuh"
 
@@ -66,31 +67,48 @@ struct Args {
   int* err;
 };
 
-// act(g), and its slope.  exp and the division are the fast ones: their errors (a few 2^-22) vanish in the bf16 results.
-__device__ __forceinline__ float relu_of(float g) { return g < 0.f ? 0.f : g; }      // NaN stays
-template <int ACT>
-__device__ __forceinline__ float act_of(float g) {
-  if constexpr (ACT == RELU) return relu_of(g);
-  if constexpr (ACT == SILU) return g * __fdividef(1.f, 1.f + __expf(-g));
-  const float t = 0.7978845608f * (g + 0.044715f * g * g * g);
-  return g * __fdividef(1.f, 1.f + __expf(-2.f * t));           // (1 + tanh t) / 2 = sigmoid(2 t)
+// act(g), and its slope, for two values at a time: the epilogues have two warps a scheduler, and their instructions are what a tile with a
+// short main loop waits for.  The logistic function's approximations err by a few 2^-24, which vanishes in the bf16 results.
+constexpr float GELU_C = 0.7978845608028654f, GELU_K = 0.044715f;      // sqrt(2 / pi); (1 + tanh t) / 2 = sigmoid(2 t)
+__device__ __forceinline__ Pair relu_of(Pair g) {
+  const float2 f = pr_get(g);
+  return pr(f.x < 0.f ? 0.f : f.x, f.y < 0.f ? 0.f : f.y);             // NaN stays
 }
 template <int ACT>
-__device__ __forceinline__ void act_slope(float g, float& a, float& slope) {
+__device__ __forceinline__ Pair act_of(Pair g) {
+  if constexpr (ACT == RELU) return relu_of(g);
+  if constexpr (ACT == SILU) return g * sigmoid_of(g);
+  return g * sigmoid_of(g * pr_fma(g * g, pr(2.f * GELU_C * GELU_K), pr(2.f * GELU_C)));
+}
+template <int ACT>
+__device__ __forceinline__ float act_of(float g) {
+  return pr_get(act_of<ACT>(pr(g))).x;
+}
+template <int ACT>
+__device__ __forceinline__ void act_slope(Pair g, Pair& a, Pair& slope) {
   if constexpr (ACT == RELU) {
+    const float2 f = pr_get(g);
     a = relu_of(g);
-    slope = g > 0.f ? 1.f : 0.f;
+    slope = pr(f.x > 0.f ? 1.f : 0.f, f.y > 0.f ? 1.f : 0.f);
   } else if constexpr (ACT == SILU) {
-    const float q = __fdividef(1.f, 1.f + __expf(-g));
+    const Pair q = sigmoid_of(g);
     a = g * q;
-    slope = q * (1.f + g * (1.f - q));
+    slope = pr_fma(a, pr_fma(pr(-1.f), q, pr(1.f)), q);                // q + g q (1 - q)
   } else {
-    const float t = 0.7978845608f * (g + 0.044715f * g * g * g);
-    const float q = __fdividef(1.f, 1.f + __expf(-2.f * t));
+    const Pair q = sigmoid_of(g * pr_fma(g * g, pr(2.f * GELU_C * GELU_K), pr(2.f * GELU_C)));
     a = g * q;
-    const float b = fminf(fmaxf(g, -1e6f), 1e6f);                // far out q or 1 - q is 0, and the factor must not be infinite
-    slope = q * (1.f + 2.f * b * (1.f - q) * 0.7978845608f * (1.f + 3.f * 0.044715f * b * b));
+    const float2 f = pr_get(g);                                        // far out q or 1 - q is 0, and the factor must not be infinite
+    const Pair b = pr(fminf(fmaxf(f.x, -1e6f), 1e6f), fminf(fmaxf(f.y, -1e6f), 1e6f));
+    const Pair inner = b * pr_fma(b * b, pr(6.f * GELU_C * GELU_K), pr(2.f * GELU_C));
+    slope = pr_fma(q * pr_fma(pr(-1.f), q, pr(1.f)), inner, q);        // q + q (1 - q) b 2 c (1 + 3 k b^2)
   }
+}
+
+// values 2 j and 2 j + 1 of an accumulator's row; two values as bf16
+__device__ __forceinline__ Pair two(const uint32_t (&v)[32], int j) { return pr(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])); }
+__device__ __forceinline__ uint32_t bf16_of(Pair p) {
+  const float2 f = pr_get(p);
+  return pack_bf16(f.x, f.y);
 }
 
 // A warp's 32 rows x 32 columns on their way out: a ring of staging buffers (64-byte swizzle), each left by one bulk tensor store.
@@ -292,7 +310,8 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 const float k = power_of(field);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                  const __half2 p = __floats2half2_rn(__uint_as_float(v[2 * j]) * k, __uint_as_float(v[2 * j + 1]) * k);
+                  const float2 f = pr_get(two(v, j) * pr(k));
+                  const __half2 p = __floats2half2_rn(f.x, f.y);
                   o[j] = *reinterpret_cast<const uint32_t*>(&p);
                 }
                 out.put(map, o, n0 + c, row0);
@@ -302,9 +321,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
               keep(u, &tmO2, args.kept.power + args.kept.plane);
             }
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              o[j] = pack_bf16(act_of<ACT>(__uint_as_float(g[2 * j])) * __uint_as_float(u[2 * j]),
-                               act_of<ACT>(__uint_as_float(g[2 * j + 1])) * __uint_as_float(u[2 * j + 1]));
+            for (int j = 0; j < 16; ++j) o[j] = bf16_of(act_of<ACT>(two(g, j)) * two(u, j));
             out.put(&tmO0, o, n0 + c, row0);
           } else {
             uint32_t d[32];
@@ -323,12 +340,11 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const float2 g = __half22float2(gb[j]), u = __half22float2(ub[j]);
-                float a0, s0, a1, s1;
-                act_slope<ACT>(g.x * gi, a0, s0);
-                act_slope<ACT>(g.y * gi, a1, s1);
-                const float d0 = __uint_as_float(d[8 * v + 2 * j]), d1 = __uint_as_float(d[8 * v + 2 * j + 1]);
-                og[4 * v + j] = pack_bf16(d0 * (u.x * ui) * s0, d1 * (u.y * ui) * s1);
-                ou[4 * v + j] = pack_bf16(d0 * a0, d1 * a1);
+                Pair a, slope;
+                act_slope<ACT>(pr(g.x, g.y) * pr(gi), a, slope);
+                const Pair dh = two(d, 4 * v + j);
+                og[4 * v + j] = bf16_of(dh * (pr(u.x, u.y) * pr(ui)) * slope);
+                ou[4 * v + j] = bf16_of(dh * a);
               }
             }
             out.put(&tmO1, og, n0 + c, row0);

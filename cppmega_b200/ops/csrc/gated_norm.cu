@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArg
       float z[N];
       rv_unpack<T>(zv[i], z);
 #pragma unroll
-      for (int j = 0; j < N; ++j) gated[i][j] = x[j] *= has_z ? z[j] * rv_sigmoid(z[j]) : 1.f;
+      for (int j = 0; j < N; ++j) gated[i][j] = x[j] *= has_z ? z[j] * sigmoid_of(z[j]) : 1.f;
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) ss[0] += x[j] * x[j];
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_fwd(const GatedArg
       rv_unpack<T>(xv[i], x);
       rv_unpack<T>(zv[i], z);
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] *= r * w[j] * (has_z ? z[j] * rv_sigmoid(z[j]) : 1.f);
+      for (int j = 0; j < N; ++j) x[j] *= r * w[j] * (has_z ? z[j] * sigmoid_of(z[j]) : 1.f);
     }
     rv_store<T, TPR, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + g0, t, i, G, rv_pack<T>(x));
   }
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(rv_block<TPR>()) gated_norm_bwd(const GatedArg
       rv_unpack<T>(wv[i], w);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float q = rv_sigmoid(z[j]), g = has_z ? z[j] * q : 1.f, slope = q + g * (1.f - q);    // without z no slope is used
+        const float q = sigmoid_of(z[j]), g = has_z ? z[j] * q : 1.f, slope = q + g * (1.f - q);    // without z no slope is used
         if constexpr (GATE_FIRST) {
           gate[i][j] = g;
           xs[i][j] = x[j] * slope;

@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "fp32_pair.cuh"
 
 namespace cm {
 
@@ -55,44 +56,6 @@ __device__ __forceinline__ uint4 rv_pack(const float (&f)[RowVec<T>::N]) {
     }
     return make_uint4(u[0], u[1], u[2], u[3]);
   }
-}
-
-// 1 / (1 + exp(-z)): the exponential's error is a few 2^-24 (1 + |z|); 1 / (1 + inf) is 0, as it should be
-__device__ __forceinline__ float rv_sigmoid(float z) {
-  float e, q;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));
-  return q;
-}
-
-// Two fp32 values that one instruction works on (fma.rn.f32x2): the backward kernels are short of issue slots, not of arithmetic.
-struct Pair {
-  unsigned long long v;
-};
-__device__ __forceinline__ Pair pr(float lo, float hi) {
-  Pair p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
-  return p;
-}
-__device__ __forceinline__ Pair pr(float both) { return pr(both, both); }
-__device__ __forceinline__ float2 pr_get(Pair p) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
-  return f;
-}
-__device__ __forceinline__ float pr_sum(Pair p) {
-  const float2 f = pr_get(p);
-  return f.x + f.y;
-}
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-  Pair d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ Pair pr_fma(Pair a, Pair b, Pair c) {
-  Pair d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
 }
 
 template <typename T>
