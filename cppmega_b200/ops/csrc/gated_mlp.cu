@@ -6,7 +6,7 @@
 // activation, linear this saves writing and reading dh, reading [g u] in the forward, and two launches.  Bound by the tensor cores:
 // 4096 x 3584 x 18944 forward 700 us at 94 % of the tensor pipe, backward 376 us at 89 %.
 //
-// Both kernels are the 256 x 256 x 64 tcgen05.mma.cta_group::2 pipeline of gemm_pair.cu (6 stages of 32 KB, two accumulators in TMEM,
+// Both kernels are the 256 x 256 x 64 tcgen05.mma.cta_group::2 pipeline of gemm_pair.cu (stages of 32 KB, two accumulators in TMEM,
 // every wait bounded, no multicast).  The first CTA of a pair loads the gate rows of w1 and the second the up rows, so that the tile is
 // one ordinary 256-column product.  The epilogue has eight warps, two to a TMEM quadrant: its exponentials, and in the backward its
 // loads of g and u, have to fit under the main loop of the next tile.
@@ -30,14 +30,21 @@ constexpr int BK = 64;
 constexpr int UMMA_K = 16;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
-constexpr int STAGES = 6;
 constexpr int A_BYTES = BM * BK * 2;
 constexpr int STAGE_BYTES = 2 * A_BYTES;
-constexpr int STORE_BYTES = 32 * 64;    // one warp's 32 rows x 32 columns of bf16
+constexpr int STORE_BYTES = 32 * 64;    // one warp's 32 rows x 32 columns of 16-bit values
 constexpr int STORE_BUFS = 2;
-constexpr int STORE_OFF = STAGES * STAGE_BYTES;
-constexpr int BAR_OFF = STORE_OFF + EPI_WARPS * STORE_BUFS * STORE_BYTES;
-constexpr int SMEM_TOTAL = BAR_OFF + 256 + 1024;
+// Shared memory: operand stages, store staging, and in the backward one chunk of g and u per epilogue warp on its way in.
+template <bool BACK>
+struct Smem {
+  static constexpr int STAGES = BACK ? 5 : 6;
+  static constexpr int FETCH_BYTES = BACK ? 2 * STORE_BYTES : 0;
+  static constexpr int STORE_OFF = STAGES * STAGE_BYTES;
+  static constexpr int FETCH_OFF = STORE_OFF + EPI_WARPS * STORE_BUFS * STORE_BYTES;
+  static constexpr int BAR_OFF = FETCH_OFF + EPI_WARPS * FETCH_BYTES;
+  static constexpr int TOTAL = BAR_OFF + 256 + 1024;
+};
+static_assert(Smem<true>::TOTAL <= 227 * 1024 && Smem<false>::TOTAL <= 227 * 1024, "shared memory of a block");
 
 enum Act : int { SILU = 0, GELU_TANH = 1, RELU = 2 };
 
@@ -139,10 +146,12 @@ template <bool BACK, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmO0,
              const __grid_constant__ CUtensorMap tmO1, const __grid_constant__ CUtensorMap tmO2, const Args args) {
+  using S = Smem<BACK>;
+  constexpr int STAGES = S::STAGES;
   extern __shared__ uint8_t smem_raw[];
   // the dynamic segment starts at the same offset in both CTAs, so the aligned offsets agree as the descriptors need
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + BAR_OFF);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tmem_full = empty_bar + STAGES;
   uint64_t* tmem_empty = tmem_full + 2;
@@ -258,38 +267,55 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     // ------------------------------ epilogue (both CTAs) ------------------------------
     const int q = warp & 3;                                     // TMEM lane quadrant this warp may read
     const int part = (warp - 2) >> 2;                           // which half of the tile's columns
-    Outbox out{smem + STORE_OFF + (warp - 2) * STORE_BUFS * STORE_BYTES, lane};
+    Outbox out{smem + S::STORE_OFF + (warp - 2) * STORE_BUFS * STORE_BYTES, lane};
     const int c_begin = part * (cols >> 1), c_end = c_begin + (cols >> 1);
+    // Backward: g and u of the chunks (32 rows x 32 columns) of this warp's tiles, in the order in which they are needed and one ahead,
+    // over the ends of tiles too.  Four lanes copy a row (64-byte swizzle, as in the Outbox), so that an instruction touches 8 lines
+    // where a lane to a row touched 32; past the last row or column come zeros.  The 32 KB cost a sixth operand stage.  Against a lane to a
+    // row, loaded into registers: this kernel 88 us from 95 at 16384 x 1024 x 2048 and 78 from 87 at 4096 x 512 x 8192, the same at
+    // hidden sizes of 2048 and more, and 1.5 us more of 87 (forward and backward) at 100 x 4096 x 4096, where one tile fills no pipeline.
+    uint8_t* inbox = smem + S::FETCH_OFF + (warp - 2) * S::FETCH_BYTES;
+    int ahead_tile = first_tile, ahead_c = c_begin;
+    uint32_t powers = 0;                                        // of the chunk on its way: g's, u's << 8
+    auto fetch = [&]() {
+      if (ahead_tile < total) {
+        int m0, n0;
+        place(ahead_tile, m0, n0);
+        const int base = m0 + rank * BM + q * 32, col = n0 + ahead_c, piece = lane & 3;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int r = v * 8 + (lane >> 2);
+          const bool on = base + r < args.M && col + 8 * piece < args.F;
+          const __half* p = on ? args.kept.v + (long long)(base + r) * 2 * args.F + col + 8 * piece : args.kept.v;
+          const uint32_t dst = smem_u32(inbox + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(on ? 16 : 0) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + STORE_BYTES), "l"(on ? p + args.F : p), "r"(on ? 16 : 0)
+                       : "memory");
+        }
+        powers = 127u | 127u << 8;
+        if (base + lane < args.M && col < args.F) {
+          const uint8_t* e = args.kept.power + (long long)(col >> 5) * args.M + base + lane;
+          powers = uint32_t(e[0]) | uint32_t(e[args.kept.plane]) << 8;
+        }
+        ahead_c += 32;
+        if (ahead_c == c_end) { ahead_c = c_begin; ahead_tile += tile_step; }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     uint32_t acc = 0, acc_phase = 0;
     bool ok = *abort_flag == 0;
+    if constexpr (BACK) fetch();
     for (int tile = first_tile; tile < total && ok; tile += tile_step) {
       int m0, n0;
       place(tile, m0, n0);
       const int row0 = m0 + rank * BM + q * 32, row = row0 + lane;
-      uint4 gv[4], uv[4];
-      uint32_t gp = 127, up = 127;
-      auto fetch = [&](int c) {                                 // g and u of 32 columns: requested ahead of their use
-        const __half* p = args.kept.v + (long long)row * 2 * args.F + n0 + c;
-        if (row < args.M && n0 + c < args.F) {
-          const uint8_t* e = args.kept.power + (long long)((n0 + c) >> 5) * args.M + row;
-          gp = e[0];
-          up = e[args.kept.plane];
-        }
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const bool on = row < args.M && n0 + c + 8 * v < args.F;
-          gv[v] = on ? reinterpret_cast<const uint4*>(p)[v] : make_uint4(0, 0, 0, 0);
-          uv[v] = on ? reinterpret_cast<const uint4*>(p + args.F)[v] : make_uint4(0, 0, 0, 0);
-        }
-      };
-      if (BACK) fetch(c_begin);
       ok = __all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], acc_phase, abort_flag, args.err, ERR_WAIT_TMEM_FULL));
       if (!ok) break;
       tc_fence_after();
       const uint32_t t_base = tmem_base + acc * 256 + (uint32_t(q * 32) << 16);
-      if (row0 < args.M) {
-        for (int c = c_begin; c < c_end && n0 + c < args.F; c += 32) {
-          if constexpr (!BACK) {
+      if constexpr (!BACK) {
+        if (row0 < args.M) {
+          for (int c = c_begin; c < c_end && n0 + c < args.F; c += 32) {
             uint32_t g[32], u[32];
             tmem_ld_32x32(t_base + c, g);
             tmem_ld_32x32(t_base + half + c, u);
@@ -323,33 +349,45 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
 #pragma unroll
             for (int j = 0; j < 16; ++j) o[j] = bf16_of(act_of<ACT>(two(g, j)) * two(u, j));
             out.put(&tmO0, o, n0 + c, row0);
-          } else {
-            uint32_t d[32];
-            tmem_ld_32x32(t_base + c, d);
-            uint4 gc[4], uc[4];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) { gc[v] = gv[v]; uc[v] = uv[v]; }
-            const float gi = inverse_power(gp), ui = inverse_power(up);
-            if (c + 32 < c_end) fetch(c + 32);
-            tmem_ld_wait();
-            uint32_t og[16], ou[16];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const __half2* gb = reinterpret_cast<const __half2*>(&gc[v]);
-              const __half2* ub = reinterpret_cast<const __half2*>(&uc[v]);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float2 g = __half22float2(gb[j]), u = __half22float2(ub[j]);
-                Pair a, slope;
-                act_slope<ACT>(pr(g.x, g.y) * pr(gi), a, slope);
-                const Pair dh = two(d, 4 * v + j);
-                og[4 * v + j] = bf16_of(dh * (pr(u.x, u.y) * pr(ui)) * slope);
-                ou[4 * v + j] = bf16_of(dh * a);
-              }
-            }
-            out.put(&tmO1, og, n0 + c, row0);
-            out.put(&tmO2, ou, n0 + c, row0);
           }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = c_begin; c < c_end; c += 32) {
+          const bool any = row0 < args.M && n0 + c < args.F;     // the same in all lanes
+          uint32_t d[32];
+          if (any) tmem_ld_32x32(t_base + c, d);
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          __syncwarp();
+          uint4 gc[4], uc[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int at = lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4);
+            gc[v] = *reinterpret_cast<const uint4*>(inbox + at);
+            uc[v] = *reinterpret_cast<const uint4*>(inbox + STORE_BYTES + at);
+          }
+          const float gi = inverse_power(powers & 255u), ui = inverse_power(powers >> 8);
+          __syncwarp();                                          // read by every lane: the next chunk may come
+          fetch();
+          if (!any) continue;
+          tmem_ld_wait();
+          uint32_t og[16], ou[16];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const __half2* gb = reinterpret_cast<const __half2*>(&gc[v]);
+            const __half2* ub = reinterpret_cast<const __half2*>(&uc[v]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 g = __half22float2(gb[j]), u = __half22float2(ub[j]);
+              Pair a, slope;
+              act_slope<ACT>(pr(g.x, g.y) * pr(gi), a, slope);
+              const Pair dh = two(d, 4 * v + j);
+              og[4 * v + j] = bf16_of(dh * (pr(u.x, u.y) * pr(ui)) * slope);
+              ou[4 * v + j] = bf16_of(dh * a);
+            }
+          }
+          out.put(&tmO1, og, n0 + c, row0);
+          out.put(&tmO2, ou, n0 + c, row0);
         }
       }
       tc_fence_before();
@@ -358,6 +396,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
+    if constexpr (BACK) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
   }
@@ -393,7 +432,7 @@ static int launch(const CUtensorMap* maps, const Args& args, cudaStream_t stream
   auto kern = gated_kernel<BACK, ACT>;
   static PerDevice configured;
   if (configured.first()) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_TOTAL) != cudaSuccess) return -2;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<BACK>::TOTAL) != cudaSuccess) return -2;
     configured.done();
   }
   const int cols = BACK ? args.bn : args.bn / 2;
@@ -401,7 +440,7 @@ static int launch(const CUtensorMap* maps, const Args& args, cudaStream_t stream
   if (tiles > 0x7fffffff) return -10;
   const int pairs = sm_count() / 2;
   const int grid = 2 * int(tiles < pairs ? tiles : pairs);
-  kern<<<grid, THREADS, SMEM_TOTAL, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], args);
+  kern<<<grid, THREADS, Smem<BACK>::TOTAL, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], args);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
