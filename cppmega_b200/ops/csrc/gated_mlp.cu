@@ -6,7 +6,7 @@
 // activation, linear this saves writing and reading dh, reading [g u] in the forward, and two launches.  Bound by the tensor cores:
 // 4096 x 3584 x 18944 forward 700 us at 94 % of the tensor pipe, backward 376 us at 89 %.
 //
-// Both kernels are the 256 x 256 x 64 tcgen05.mma.cta_group::2 pipeline of gemm_pair.cu (stages of 32 KB, two accumulators in TMEM,
+// Both kernels are the 256 x 256 x 64 tcgen05.mma.cta_group::2 pipeline of gemm_pair.cu (6 or 5 stages of 32 KB, two accumulators in TMEM,
 // every wait bounded, no multicast).  The first CTA of a pair loads the gate rows of w1 and the second the up rows, so that the tile is
 // one ordinary 256-column product.  The epilogue has eight warps, two to a TMEM quadrant: its exponentials, and in the backward its
 // loads of g and u, have to fit under the main loop of the next tile.
@@ -34,11 +34,11 @@ constexpr int A_BYTES = BM * BK * 2;
 constexpr int STAGE_BYTES = 2 * A_BYTES;
 constexpr int STORE_BYTES = 32 * 64;    // one warp's 32 rows x 32 columns of 16-bit values
 constexpr int STORE_BUFS = 2;
-// Shared memory: operand stages, store staging, and in the backward one chunk of g and u per epilogue warp on its way in.
-template <bool BACK>
+// Shared memory: operand stages, store staging, and with INBOX one chunk of g and u per epilogue warp on its way in.
+template <bool INBOX>
 struct Smem {
-  static constexpr int STAGES = BACK ? 5 : 6;
-  static constexpr int FETCH_BYTES = BACK ? 2 * STORE_BYTES : 0;
+  static constexpr int STAGES = INBOX ? 5 : 6;
+  static constexpr int FETCH_BYTES = INBOX ? 2 * STORE_BYTES : 0;
   static constexpr int STORE_OFF = STAGES * STAGE_BYTES;
   static constexpr int FETCH_OFF = STORE_OFF + EPI_WARPS * STORE_BUFS * STORE_BYTES;
   static constexpr int BAR_OFF = FETCH_OFF + EPI_WARPS * FETCH_BYTES;
@@ -142,11 +142,11 @@ struct Outbox {
 
 // BACK = false: A = x, B = w1 (rows of g and u), outputs h (tmO0), g (tmO1), u (tmO2).
 // BACK = true:  A = dy, B = w2 (reduction rows), outputs dg (tmO1), du (tmO2).
-template <bool BACK, int ACT>
+template <bool BACK, int ACT, bool INBOX>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmO0,
              const __grid_constant__ CUtensorMap tmO1, const __grid_constant__ CUtensorMap tmO2, const Args args) {
-  using S = Smem<BACK>;
+  using S = Smem<INBOX>;
   constexpr int STAGES = S::STAGES;
   extern __shared__ uint8_t smem_raw[];
   // the dynamic segment starts at the same offset in both CTAs, so the aligned offsets agree as the descriptors need
@@ -269,28 +269,32 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     const int part = (warp - 2) >> 2;                           // which half of the tile's columns
     Outbox out{smem + S::STORE_OFF + (warp - 2) * STORE_BUFS * STORE_BYTES, lane};
     const int c_begin = part * (cols >> 1), c_end = c_begin + (cols >> 1);
-    // Backward: g and u of the chunks (32 rows x 32 columns) of this warp's tiles, in the order in which they are needed and one ahead,
-    // over the ends of tiles too.  Four lanes copy a row (64-byte swizzle, as in the Outbox), so that an instruction touches 8 lines
-    // where a lane to a row touched 32; past the last row or column come zeros.  The 32 KB cost a sixth operand stage.  Against a lane to a
-    // row, loaded into registers: this kernel 88 us from 95 at 16384 x 1024 x 2048 and 78 from 87 at 4096 x 512 x 8192, the same at
-    // hidden sizes of 2048 and more, and 1.5 us more of 87 (forward and backward) at 100 x 4096 x 4096, where one tile fills no pipeline.
+    // Backward: g and u of the chunks (32 rows x 32 columns) of this warp's tiles are requested in the order in which they are needed and
+    // one ahead, over the ends of tiles too: a row to a lane into registers, or with INBOX a row to four lanes into shared memory (64-byte
+    // swizzle, as in the Outbox), where an instruction touches 8 lines instead of 32.  Past the last row or column come zeros.
     uint8_t* inbox = smem + S::FETCH_OFF + (warp - 2) * S::FETCH_BYTES;
     int ahead_tile = first_tile, ahead_c = c_begin;
     uint32_t powers = 0;                                        // of the chunk on its way: g's, u's << 8
+    uint4 gv[4], uv[4];                                         // the chunk on its way, without INBOX
     auto fetch = [&]() {
       if (ahead_tile < total) {
         int m0, n0;
         place(ahead_tile, m0, n0);
-        const int base = m0 + rank * BM + q * 32, col = n0 + ahead_c, piece = lane & 3;
+        const int base = m0 + rank * BM + q * 32, col = n0 + ahead_c;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const int r = v * 8 + (lane >> 2);
+          const int r = INBOX ? v * 8 + (lane >> 2) : lane, piece = INBOX ? lane & 3 : v;
           const bool on = base + r < args.M && col + 8 * piece < args.F;
           const __half* p = on ? args.kept.v + (long long)(base + r) * 2 * args.F + col + 8 * piece : args.kept.v;
-          const uint32_t dst = smem_u32(inbox + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(on ? 16 : 0) : "memory");
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + STORE_BYTES), "l"(on ? p + args.F : p), "r"(on ? 16 : 0)
-                       : "memory");
+          if constexpr (INBOX) {
+            const uint32_t dst = smem_u32(inbox + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(on ? 16 : 0) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + STORE_BYTES), "l"(on ? p + args.F : p), "r"(on ? 16 : 0)
+                         : "memory");
+          } else {
+            gv[v] = on ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+            uv[v] = on ? *reinterpret_cast<const uint4*>(p + args.F) : make_uint4(0, 0, 0, 0);
+          }
         }
         powers = 127u | 127u << 8;
         if (base + lane < args.M && col < args.F) {
@@ -300,7 +304,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         ahead_c += 32;
         if (ahead_c == c_end) { ahead_c = c_begin; ahead_tile += tile_step; }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      if constexpr (INBOX) asm volatile("cp.async.commit_group;" ::: "memory");
     };
     uint32_t acc = 0, acc_phase = 0;
     bool ok = *abort_flag == 0;
@@ -357,17 +361,19 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
           const bool any = row0 < args.M && n0 + c < args.F;     // the same in all lanes
           uint32_t d[32];
           if (any) tmem_ld_32x32(t_base + c, d);
-          asm volatile("cp.async.wait_group 0;" ::: "memory");
-          __syncwarp();
+          if constexpr (INBOX) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncwarp();
+          }
           uint4 gc[4], uc[4];
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const int at = lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4);
-            gc[v] = *reinterpret_cast<const uint4*>(inbox + at);
-            uc[v] = *reinterpret_cast<const uint4*>(inbox + STORE_BYTES + at);
+            gc[v] = INBOX ? *reinterpret_cast<const uint4*>(inbox + at) : gv[v];
+            uc[v] = INBOX ? *reinterpret_cast<const uint4*>(inbox + STORE_BYTES + at) : uv[v];
           }
           const float gi = inverse_power(powers & 255u), ui = inverse_power(powers >> 8);
-          __syncwarp();                                          // read by every lane: the next chunk may come
+          if constexpr (INBOX) __syncwarp();                     // read by every lane: the next chunk may come
           fetch();
           if (!any) continue;
           tmem_ld_wait();
@@ -396,7 +402,7 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
-    if constexpr (BACK) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if constexpr (INBOX) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
   }
@@ -427,12 +433,12 @@ static int make_out_map(CUtensorMap* out, void* base, long long rows, long long 
   return r == CUDA_SUCCESS ? 0 : int(r);
 }
 
-template <bool BACK, int ACT>
+template <bool BACK, int ACT, bool INBOX>
 static int launch(const CUtensorMap* maps, const Args& args, cudaStream_t stream) {
-  auto kern = gated_kernel<BACK, ACT>;
+  auto kern = gated_kernel<BACK, ACT, INBOX>;
   static PerDevice configured;
   if (configured.first()) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<BACK>::TOTAL) != cudaSuccess) return -2;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<INBOX>::TOTAL) != cudaSuccess) return -2;
     configured.done();
   }
   const int cols = BACK ? args.bn : args.bn / 2;
@@ -440,16 +446,29 @@ static int launch(const CUtensorMap* maps, const Args& args, cudaStream_t stream
   if (tiles > 0x7fffffff) return -10;
   const int pairs = sm_count() / 2;
   const int grid = 2 * int(tiles < pairs ? tiles : pairs);
-  kern<<<grid, THREADS, Smem<BACK>::TOTAL, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], args);
+  kern<<<grid, THREADS, Smem<INBOX>::TOTAL, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], args);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+// Up to this reduction the backward's epilogue is longer than a tile's main loop, and g and u come through shared memory; above it the main
+// loop is, and the operand stage that this costs counts more.  Registers against shared memory, us: 4096 x 512 x 8192 97 / 79, 16384 x 1024 x
+// 2048 101 / 85, 16384 x 1536 x 2048 109 / 93, 8192 x 2048 x 2048 70 / 64; 8192 x 3584 x 2048 96 / 97, 4096 x 4096 x 21504 501 / 509,
+// 100 x 4096 x 4096 23.3 / 24.5.
+constexpr int INBOX_K = 2560;
+template <bool BACK, int ACT>
+static int launch_in(const CUtensorMap* maps, const Args& args, cudaStream_t stream) {
+  if constexpr (BACK) {
+    if (args.K <= INBOX_K) return launch<true, ACT, true>(maps, args, stream);
+  }
+  return launch<BACK, ACT, false>(maps, args, stream);
 }
 
 template <bool BACK>
 static int launch_act(int act, const CUtensorMap* maps, const Args& args, cudaStream_t stream) {
   switch (act) {
-    case SILU: return launch<BACK, SILU>(maps, args, stream);
-    case GELU_TANH: return launch<BACK, GELU_TANH>(maps, args, stream);
-    case RELU: return launch<BACK, RELU>(maps, args, stream);
+    case SILU: return launch_in<BACK, SILU>(maps, args, stream);
+    case GELU_TANH: return launch_in<BACK, GELU_TANH>(maps, args, stream);
+    case RELU: return launch_in<BACK, RELU>(maps, args, stream);
   }
   return -10;
 }

@@ -391,6 +391,13 @@ def test_gated_mlp(name, lead, H, F, Ho):
     _check_mlp(x, w1, w2, name, y, dict(x=dx, w1=dw1, w2=dw2), dy)
 
 
+# More tiles than CTA pairs, so that a pair takes several, on both sides of the width at which the backward changes how it reads g and u.
+@pytest.mark.parametrize("name", ["silu", "gelu_tanh", "relu"])
+@pytest.mark.parametrize("T,H,F,Ho", [(2100, 40, 2344, 136), (2100, 40, 2344, 2560), (2100, 40, 2344, 2568), (5000, 264, 1000, 72), (200, 16, 40, 4104)])
+def test_gated_mlp_several_tiles_a_pair(name, T, H, F, Ho):
+    test_gated_mlp(name, (T,), H, F, Ho)
+
+
 @pytest.mark.parametrize("T", [1, 2, 3, 7, 8, 9, 15, 16, 17, 24, 31, 32, 33, 48, 63, 64, 65, 100, 128, 200, 256, 257])
 @pytest.mark.parametrize("H,F,Ho", [(1024, 2048, 1024), (520, 1000, 248), (24, 40, 16)])
 def test_gated_mlp_without_gradients(T, H, F, Ho):
