@@ -4,7 +4,7 @@
 //   gated_kernel, backward  dh = dy W2 stays in TMEM; the epilogue reads g and u and stores dg = dh u act'(g), du = dh act(g).
 // The other products (h W2^T, [dg du] w1, [dg du]^T x, dy^T h) are dense ones, with the last wave shared (gemm_split.cu).  Against linear,
 // activation, linear this saves writing and reading dh, reading [g u] in the forward, and two launches.  Bound by the tensor cores:
-// 4096 x 3584 x 18944 forward 700 us at 94 % of the tensor pipe, backward 376 us at 89 %.
+// 4096 x 3584 x 18944 forward 714 us at 95 % of the tensor pipe, backward 396 us at 91 % (at the clocks of a loop).
 //
 // Both kernels are the 256 x 256 x 64 tcgen05.mma.cta_group::2 pipeline of gemm_pair.cu (6 or 5 stages of 32 KB, two accumulators in TMEM,
 // every wait bounded, no multicast).  The first CTA of a pair loads the gate rows of w1 and the second the up rows, so that the tile is
