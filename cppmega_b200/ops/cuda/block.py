@@ -10,6 +10,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import cuda as _cu
@@ -72,6 +73,16 @@ def _first_order(fn):
     def backward(ctx, *grads):
         return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
     return backward
+
+
+def _bare(*tensors) -> bool:
+    """Whether the tensors are no more than the memory that a kernel reads: one inside a function transform (``vmap``, ``torch.func``)
+    has no storage, and the tangent of a forward-mode dual lies beside it."""
+    for t in tensors:
+        if t is not None and (not torch._C._has_storage(t)
+                              or forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None):
+            return False
+    return True
 
 
 @functools.lru_cache(maxsize=1024)
@@ -183,7 +194,7 @@ class GatedMLPFn(torch.autograd.Function):
 @_on_device
 def gated_mlp(x, w1, w2, activation):
     """None where the kernels do not apply: they take bf16 throughout and widths that are multiples of 8."""
-    if not (x.dtype == w1.dtype == w2.dtype == torch.bfloat16 and w1.is_contiguous() and w2.is_contiguous() and x.numel() > 0
+    if not (_bare(x, w1, w2) and x.dtype == w1.dtype == w2.dtype == torch.bfloat16 and w1.is_contiguous() and w2.is_contiguous() and x.numel() > 0
             and x.shape[-1] % 8 == 0 and w2.shape[0] % 8 == 0 and w2.shape[1] % 8 == 0 and w1.data_ptr() % 16 == 0
             and w2.data_ptr() % 16 == 0 and x.numel() // x.shape[-1] < 2 ** 30):
         return None
@@ -265,7 +276,8 @@ def residual_rmsnorm(y, residual, weight, post_weight, gate, scale, eps):
     """None where the kernels do not apply: one type for all tensors (bf16, fp16 or fp32), rows of at most 16384."""
     dt = y.dtype
     if (dt not in ROW_TYPES or residual.dtype != dt or weight.dtype != dt or (post_weight is not None and post_weight.dtype != dt)
-            or (gate is not None and gate.dtype != dt) or y.shape[-1] > MAX_WIDTH or y.numel() == 0):
+            or (gate is not None and gate.dtype != dt) or y.shape[-1] > MAX_WIDTH or y.numel() == 0
+            or not _bare(y, residual, weight, post_weight, gate)):
         return None
     weight = weight.contiguous()
     if post_weight is not None:
@@ -341,7 +353,7 @@ def rmsnorm_gated(x, weight, z, eps, group, norm_before_gate):
     most 65535 of them."""
     dt = x.dtype
     if (dt not in ROW_TYPES or weight.dtype != dt or (z is not None and z.dtype != dt) or group > MAX_WIDTH or x.numel() == 0
-            or x.shape[-1] // group > 65535):
+            or x.shape[-1] // group > 65535 or not _bare(x, weight, z)):
         return None
     weight = weight.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (z is not None and z.requires_grad)):

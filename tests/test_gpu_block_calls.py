@@ -1,0 +1,48 @@
+"""The operators around a dense block on the GPU: calls that reach them in less usual ways."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from cppmega_b200.ops import functional as F_
+from cppmega_b200.ops import reference as ref
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-5
+
+
+def _randn(*shape, dtype=torch.bfloat16, std=1.0, mean=0.0, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + 7919 * sum(shape))
+    return torch.empty(shape, device="cuda").normal_(mean, std, generator=g).to(dtype)
+
+
+def _norm_calls():
+    f32 = torch.float32
+    x, z, w = _randn(6, 64, dtype=f32), _randn(6, 64, dtype=f32, seed=1), _randn(64, dtype=f32, mean=1.0, std=0.1, seed=2)
+    return {"rmsnorm_gated": (F_.rmsnorm_gated, ref.rmsnorm_gated, (x, w, z)),
+            "residual_rmsnorm": (lambda *a: F_.residual_rmsnorm(*a)[0], lambda *a: ref.residual_rmsnorm(*a)[0], (x, z, w, w, w))}
+
+
+@pytest.mark.parametrize("name", ["rmsnorm_gated", "residual_rmsnorm"])
+def test_norms_carry_tangents_and_transforms(name):
+    """Forward mode, ``vmap`` and ``torch.func.grad`` give what the definition gives (it is what runs)."""
+    call, plain, args = _norm_calls()[name]
+    tangents = tuple(torch.full_like(t, 0.5) for t in args)
+    with forward_ad.dual_level():
+        got, want = (forward_ad.unpack_dual(f(*[forward_ad.make_dual(t, d) for t, d in zip(args, tangents)])).tangent for f in (call, plain))
+    assert torch.equal(got, want) and got.abs().max() > 0
+    for t in (torch.func.jvp(call, args, tangents)[1],):
+        assert torch.equal(t, want)
+    many = args[0].expand(3, 6, 64)
+    assert torch.equal(torch.func.vmap(lambda t: call(t, *args[1:]))(many), torch.func.vmap(lambda t: plain(t, *args[1:]))(many))
+    assert torch.equal(*(torch.func.grad(lambda t: f(t, *args[1:]).sum())(args[0]) for f in (call, plain)))
+
+
+def test_gated_mlp_refuses_tangents():
+    """The products have no forward-mode derivative, so that a call with tangents raises instead of losing them."""
+    x, w1, w2 = _randn(6, 64), _randn(48, 64), _randn(64, 24)
+    with forward_ad.dual_level():
+        for i in range(3):
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate((x, w1, w2))]
+            with pytest.raises(RuntimeError):
+                F_.gated_mlp(*args)
