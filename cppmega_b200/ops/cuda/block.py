@@ -15,6 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import cuda as _cu
 from .. import functional as F_
+from .. import reference as ref
 
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1, "relu": 2}
 ROW_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -316,13 +317,15 @@ class GatedRMSNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, z, eps, group, gate_first):
         y, x, z, rstd = _gated_forward(x, weight, z, eps, group, gate_first, keep=True)
         ctx.save_for_backward(x, weight, z, rstd)
-        ctx.group, ctx.gate_first = group, gate_first
+        ctx.eps, ctx.group, ctx.gate_first = eps, group, gate_first
         return y
 
     @staticmethod
     @_first_order
     def backward(ctx, dy):
         x, weight, z, rstd = ctx.saved_tensors
+        if not _bare(dy):
+            return _gated_by_definition(ctx, x, weight, z, dy)
         _, need_w, need_z = ctx.needs_input_grad[:3]
         W = x.shape[-1]
         R = x.numel() // W
@@ -345,6 +348,17 @@ class GatedRMSNormFn(torch.autograd.Function):
             _failed("cm_rmsnorm_gated_bwd", rc)
         F_.count_launch("rmsnorm_gated_bwd")
         return dx, dw, dz, None, None, None
+
+
+def _gated_by_definition(ctx, x, weight, z, dy):
+    """Gradients for a ``dy`` without memory of its own (a batch of them, under ``is_grads_batched``)."""
+    F_._miss("rmsnorm_gated_bwd(batched gradients)", x)
+    with torch.enable_grad():
+        leaves = [None if t is None else t.detach().requires_grad_(need) for t, need in zip((x, weight, z), ctx.needs_input_grad)]
+        y = ref.rmsnorm_gated(*leaves, ctx.eps, ctx.group, not ctx.gate_first)
+    wanted = [t for t in leaves if t is not None and t.requires_grad]
+    grads = iter(torch.autograd.grad(y, wanted, dy))
+    return (*(next(grads) if t is not None and t.requires_grad else None for t in leaves), None, None, None)
 
 
 @_on_device

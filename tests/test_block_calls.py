@@ -39,3 +39,22 @@ def test_kernels_leave_tangents_and_transforms_to_the_definitions(name, i):
     torch.func.grad(inside)(args[i])
     torch.func.vmap(inside)(args[i].expand(3, *args[i].shape))
     assert seen == [None, None]
+
+
+@pytest.mark.parametrize("before", [True, False])
+@pytest.mark.parametrize("gate", [True, False])
+def test_gated_norm_takes_a_batch_of_upstream_gradients(monkeypatch, before, gate):
+    """``is_grads_batched`` hands the backward gradients that have no memory a kernel could read."""
+    x, w, z = (t.requires_grad_() for t in (_r(5, 24), _r(24), _r(5, 24, seed=1)))
+
+    def forward(x, weight, z, eps, group, gate_first, keep):
+        return ref.rmsnorm_gated(x, weight, z, eps, group, not gate_first), x, z, torch.empty(0)
+
+    monkeypatch.setattr(block, "_gated_forward", forward)
+    ins = [x, w, z] if gate else [x, w]
+    many = _r(3, 5, 24, seed=2)
+    got = torch.autograd.grad(block.rmsnorm_gated(x, w, z if gate else None, 1e-5, 8, before), ins, many, is_grads_batched=True)
+    y = ref.rmsnorm_gated(x, w, z if gate else None, 1e-5, 8, before)
+    for i, dy in enumerate(many):
+        want = torch.autograd.grad(y, ins, dy, retain_graph=True)
+        assert all(torch.allclose(g[i], t, rtol=1e-5, atol=1e-6) for g, t in zip(got, want))

@@ -46,3 +46,15 @@ def test_gated_mlp_refuses_tangents():
             args = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate((x, w1, w2))]
             with pytest.raises(RuntimeError):
                 F_.gated_mlp(*args)
+
+
+@pytest.mark.parametrize("before", [True, False])
+def test_gated_norm_takes_a_batch_of_upstream_gradients(before):
+    """Each gradient of a batch is the one that the definition gives alone: the same fp32 expressions over another batch of rows."""
+    x, w, z = (t.requires_grad_() for t in _norm_calls()["rmsnorm_gated"][2])
+    many = _randn(3, 6, 64, dtype=torch.float32, seed=4)
+    got = torch.autograd.grad(F_.rmsnorm_gated(x, w, z, EPS, 16, before), [x, w, z], many, is_grads_batched=True)
+    y = ref.rmsnorm_gated(x, w, z, EPS, 16, before)
+    for i, dy in enumerate(many):
+        for g, t in zip(got, torch.autograd.grad(y, [x, w, z], dy, retain_graph=True)):
+            assert (g[i] - t).abs().max() <= 64 * 2 ** -24 * t.abs().max()
