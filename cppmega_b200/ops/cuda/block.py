@@ -115,6 +115,13 @@ def _rows(t: torch.Tensor):
     return _cu.fast_contiguous(t), t.shape[-1]
 
 
+def _given_back(t, dtype: torch.dtype, device: torch.device, packed: bool = True, align: int = 1):
+    """A saved tensor in the form in which the kernels read it, whatever form a saved-tensor hook gave its values back in."""
+    if t is None or (t.dtype == dtype and t.device == device and (not packed or t.is_contiguous() and t.data_ptr() % align == 0)):
+        return t
+    return torch.empty(t.shape, dtype=dtype, device=device).copy_(t)
+
+
 def _like(t: torch.Tensor) -> torch.Tensor:
     """A packed tensor of the same shape, type and device."""
     return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
@@ -162,8 +169,11 @@ class GatedMLPFn(torch.autograd.Function):
     @staticmethod
     @_first_order
     def backward(ctx, dy):
-        x, w1, w2, kept, h = ctx.saved_tensors
+        x, p1, p2, kept, h = ctx.saved_tensors
         need_x, need_w1, need_w2, _ = ctx.needs_input_grad
+        w1, w2, h = (_given_back(t, torch.bfloat16, dy.device, align=16) for t in (p1, p2, h))
+        kept = _given_back(kept, torch.uint8, dy.device, align=16)
+        x = _given_back(x, torch.bfloat16, dy.device, packed=False)
         H, F, Ho = w1.shape[1], w2.shape[1], w2.shape[0]
         dy, lddy = _tma_rows(dy)
         x, ldx = _tma_rows(x)
@@ -177,8 +187,8 @@ class GatedMLPFn(torch.autograd.Function):
                 return t
             return run
 
-        dw1 = _cu.wgrad_into_main_grad(w1, target(0, w1)) if need_w1 else None
-        dw2 = _cu.wgrad_into_main_grad(w2, target(1, w2)) if need_w2 else None
+        dw1 = _cu.wgrad_into_main_grad(p1, target(0, w1)) if need_w1 else None
+        dw2 = _cu.wgrad_into_main_grad(p2, target(1, w2)) if need_w2 else None
         dgu = x.new_empty(h.shape[0], 2 * F) if need_x or need_w1 else None
         L, M = _cu.lib(), h.shape[0]
         floats = _size("cm_gated_mlp_bwd_ws", x.get_device(), M, H, F, Ho)
@@ -231,7 +241,7 @@ class ResidualRMSNormFn(torch.autograd.Function):
         n, h, y, stats = _residual_forward(y, residual, weight, post, gate, scale, eps, keep=True)
         # the block's output is read again only where a norm or a gate stands between it and the stream
         ctx.save_for_backward(h, y if post is not None or gate is not None else None, weight, post, gate, stats)
-        ctx.scale = scale
+        ctx.scale, ctx.dtype = scale, y.dtype
         ctx.set_materialize_grads(False)
         return n, h
 
@@ -242,6 +252,10 @@ class ResidualRMSNormFn(torch.autograd.Function):
             return (None,) * 7
         h, y, weight, post, gate, stats = ctx.saved_tensors
         need_y, _, need_w, need_post, need_gate = ctx.needs_input_grad[:5]
+        dt, dev = ctx.dtype, (dh if dn is None else dn).device
+        h, weight, post, gate = (_given_back(t, dt, dev) for t in (h, weight, post, gate))
+        stats = _given_back(stats, torch.float32, dev)
+        y = _given_back(y, dt, dev, packed=False)
         W = h.shape[-1]
         R = h.numel() // W
         sy = sdn = sdh = 0
@@ -327,6 +341,8 @@ class GatedRMSNormFn(torch.autograd.Function):
         if not _bare(dy):
             return _gated_by_definition(ctx, x, weight, z, dy)
         _, need_w, need_z = ctx.needs_input_grad[:3]
+        weight, rstd = _given_back(weight, dy.dtype, dy.device), _given_back(rstd, torch.float32, dy.device)
+        x, z = (_given_back(t, dy.dtype, dy.device, packed=False) for t in (x, z))
         W = x.shape[-1]
         R = x.numel() // W
         x, sx = _rows(x)

@@ -58,3 +58,69 @@ def test_gated_norm_takes_a_batch_of_upstream_gradients(monkeypatch, before, gat
     for i, dy in enumerate(many):
         want = torch.autograd.grad(y, ins, dy, retain_graph=True)
         assert all(torch.allclose(g[i], t, rtol=1e-5, atol=1e-6) for g, t in zip(got, want))
+
+
+class _Recorder:
+    """Stands in for the kernel library: a backward entry leaves the bytes at each pointer of its arguments that is looked at."""
+
+    def __init__(self, look, sizes):
+        self.look, self.sizes, self.seen = look, sizes, None
+
+    def __getattr__(self, name):
+        import ctypes
+
+        def call(*args):
+            if name == self.look:
+                self.seen = {i: ctypes.string_at(args[i], n) for i, n in self.sizes.items()}
+            return 64 if name.endswith(("_ws", "_parts", "_kept")) else 0
+        return call
+
+
+def _bytes(t):
+    return t.detach().contiguous().reshape(-1).view(torch.uint8).numpy().tobytes()
+
+
+def _apart(t):                                   # the same values, every second element of a buffer
+    return t.new_empty(*t.shape, 2)[..., 0].copy_(t)
+
+
+def _wider(t):
+    return t.float() if t.dtype == torch.bfloat16 else t
+
+
+def _offset(t):                                  # packed, but not on 16 bytes
+    return t.new_empty(t.numel() + 1)[1:].view(t.shape).copy_(t)
+
+
+@pytest.mark.parametrize("form", [_apart, _wider, _offset])
+@pytest.mark.parametrize("name", ["gated_mlp", "residual_rmsnorm", "rmsnorm_gated"])
+def test_backward_reads_saved_tensors_in_any_form(monkeypatch, name, form):
+    """A saved-tensor hook may give the values back with other strides, in a wider type or at another address."""
+    bf = torch.bfloat16
+    r = lambda *s, seed=0: _r(*s, seed=seed, dtype=bf).requires_grad_()  # noqa: E731
+    calls = {                                    # call, entry, argument -> saved tensor behind it
+        "gated_mlp": (lambda: block.gated_mlp(r(4, 16), r(48, 16), r(16, 24), "silu"), "cm_gated_mlp_bwd", {2: 0, 4: 1, 5: 2, 6: 3, 7: 4}),
+        "residual_rmsnorm": (lambda: block.residual_rmsnorm(r(4, 16), r(4, 16, seed=1), r(16), r(16, seed=2), r(16, seed=3), 0.5, 1e-5)[0],
+                             "cm_residual_rmsnorm_bwd", {4: 0, 5: 1, 7: 2, 8: 3, 9: 4, 11: 5}),
+        "rmsnorm_gated": (lambda: block.rmsnorm_gated(r(4, 16), r(16), r(4, 16, seed=1), 1e-5, 16, True), "cm_rmsnorm_gated_bwd",
+                          {0: 0, 4: 1, 2: 2, 7: 3}),
+    }
+    call, entry, where = calls[name]
+    saved = []
+
+    def pack(t):
+        saved.append(t.detach().clone())
+        return form(t.detach())
+
+    library = _Recorder(entry, {})
+    monkeypatch.setattr(block._cu, "lib", lambda: library)
+    monkeypatch.setattr(block._cu, "err_word", lambda dev: torch.zeros(1))
+    monkeypatch.setattr(block._cu, "stream_ptr", lambda: None)
+    block._size.cache_clear()
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        y = call()
+    want = {arg: _bytes(saved[i]) for arg, i in where.items()}
+    library.sizes = {arg: len(b) for arg, b in want.items()}
+    y.backward(torch.ones_like(y))
+    block._size.cache_clear()
+    assert library.seen == want

@@ -58,3 +58,31 @@ def test_gated_norm_takes_a_batch_of_upstream_gradients(before):
     for i, dy in enumerate(many):
         for g, t in zip(got, torch.autograd.grad(y, [x, w, z], dy, retain_graph=True)):
             assert (g[i] - t).abs().max() <= 64 * 2 ** -24 * t.abs().max()
+
+
+@pytest.mark.parametrize("form", ["apart", "wider", "offset"])
+@pytest.mark.parametrize("name", ["gated_mlp", "residual_rmsnorm", "rmsnorm_gated"])
+def test_saved_tensors_given_back_in_another_form(name, form):
+    """Hooks that return the saved values every second element of a buffer, in fp32, or off the 16-byte grid."""
+    x, z, w = _randn(40, 64).requires_grad_(), _randn(40, 64, seed=1).requires_grad_(), _randn(64, mean=1.0, std=0.1, seed=2).requires_grad_()
+    w1, w2 = _randn(144, 64, std=0.1, seed=3).requires_grad_(), _randn(64, 72, std=0.1, seed=4).requires_grad_()
+    call, leaves = {"gated_mlp": (lambda: F_.gated_mlp(x, w1, w2), [x, w1, w2]),
+                    "residual_rmsnorm": (lambda: F_.residual_rmsnorm(x, z, w, w, w, 0.5)[0], [x, z, w]),
+                    "rmsnorm_gated": (lambda: F_.rmsnorm_gated(x, w, z, EPS, 16, False), [x, w, z])}[name]
+    dy = _randn(40, 64, std=0.1, seed=5)
+    want = torch.autograd.grad(call(), leaves, dy)
+
+    def pack(t):
+        if form == "apart":
+            return t.new_empty(*t.shape, 2)[..., 0].copy_(t.detach())
+        if form == "wider":
+            return t.detach().float() if t.dtype == torch.bfloat16 else t.detach()
+        return t.new_empty(t.numel() + 1)[1:].view(t.shape).copy_(t.detach())
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        y = call()
+    for a, b in zip(torch.autograd.grad(y, leaves, dy), want):
+        if form == "offset" and name != "gated_mlp":      # rows off the grid are summed in another order: one step of bf16, and fp32 sums
+            assert ((a.double() - b.double()).abs() <= 2 * 2 ** -8 * b.double().abs() + 2 ** -14 * b.double().abs().max()).all()
+        else:
+            assert torch.equal(a, b)
