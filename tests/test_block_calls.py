@@ -109,6 +109,8 @@ def test_backward_reads_saved_tensors_in_any_form(monkeypatch, name, form):
     saved = []
 
     def pack(t):
+        if t.is_floating_point():                # no kernel ran: what results hold may be NaN, whose bits a cast changes
+            t.detach().nan_to_num_()
         saved.append(t.detach().clone())
         return form(t.detach())
 
