@@ -6,6 +6,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from ..ops import functional as F_
 from ..parallel.state import ParallelContext
@@ -33,8 +34,10 @@ class RMSNorm(nn.Module):
         return F_.rmsnorm(x, self.weight, self.eps)
 
 
-def _hooked(m: nn.Module) -> bool:
-    return bool(m._forward_pre_hooks or m._forward_hooks or m._backward_hooks or m._backward_pre_hooks)
+def _stock(m: nn.Module, cls: type) -> bool:
+    """Whether calling ``m`` is nothing but ``cls.forward``: not replaced or wrapped, with no hooks of its own or of all modules."""
+    return (type(m) is cls and "forward" not in m.__dict__
+            and not (m._forward_pre_hooks or m._forward_hooks or m._backward_hooks or m._backward_pre_hooks or _has_any_global_hook()))
 
 
 class DenseMLP(nn.Module):
@@ -51,9 +54,10 @@ class DenseMLP(nn.Module):
                                             seed=seed_for(name + ".linear_fc2", seed), name=name + ".linear_fc2")
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        # as one operator where the two linears are plain products: no tensor parallelism, nothing hooked to them (a precision
-        # rule or a probe on one of them wants its calls), and no FP8 storage of what is kept for backward
-        if self.pc.tp == 1 and not (_hooked(self.linear_fc1) or _hooked(self.linear_fc2) or fp8_activations.packing()):
+        # as one operator where the two linears are plain products: no tensor parallelism, no other module in their place, nothing
+        # hooked to them (a precision rule or a probe on one of them wants its calls), and no FP8 storage of what is kept for backward
+        if (self.pc.tp == 1 and _stock(self.linear_fc1, ColumnParallelLinear) and _stock(self.linear_fc2, RowParallelLinear)
+                and not fp8_activations.packing()):
             return F_.gated_mlp(x, self.linear_fc1.weight, self.linear_fc2.weight)
         return self.linear_fc2(F_.swiglu(self.linear_fc1(x)))
 

@@ -122,3 +122,58 @@ def test_backward_reads_saved_tensors_in_any_form(monkeypatch, name, form):
         got, want = torch.frombuffer(bytearray(library.seen[arg]), dtype=saved[i].dtype), saved[i].reshape(-1)
         # no kernel ran: what results hold may be NaN, whose bits a cast changes
         assert torch.equal(got.nan_to_num(), want.nan_to_num()) if got.is_floating_point() else torch.equal(got, want)
+
+
+def _dense_mlp():
+    from cppmega_b200.models.common import DenseMLP
+    from cppmega_b200.parallel.state import single_process_context
+    return DenseMLP(32, 48, single_process_context(), std=0.1, out_std=0.1, dtype=torch.float32, seed=3)
+
+
+def test_dense_mlp_calls_a_child_that_is_not_a_stock_linear(monkeypatch):
+    """A module in the place of a linear, one with a bias, a forward of its own, a parametrised weight: what it computes counts."""
+    class Biased(torch.nn.Module):
+        def __init__(self, m):
+            super().__init__()
+            self.inner, self.weight, self.bias = m, m.weight, torch.ones(m.weight.shape[0])
+
+        def forward(self, x):
+            return self.inner(x) + self.bias
+
+    class Nameless(torch.nn.Module):                # no attribute ``weight``
+        def __init__(self, m):
+            super().__init__()
+            self.inner = m
+
+        def forward(self, x):
+            return 2 * self.inner(x)
+
+    x = _r(2, 5, 32)
+    for name in ("linear_fc1", "linear_fc2"):
+        for wrap in (Biased, Nameless):
+            m = _dense_mlp()
+            setattr(m, name, wrap(getattr(m, name)))
+            assert torch.equal(m(x), m.linear_fc2(F_.swiglu(m.linear_fc1(x))))
+        m = _dense_mlp()
+        child = getattr(m, name)
+        monkeypatch.setattr(child, "forward", lambda t, plain=child.forward: 3 * plain(t))
+        assert torch.equal(m(x), m.linear_fc2(F_.swiglu(m.linear_fc1(x))))
+        m = _dense_mlp()
+        want = m.linear_fc2(F_.swiglu(m.linear_fc1(x)))
+        torch.nn.utils.parametrize.register_parametrization(getattr(m, name), "weight", torch.nn.Identity())
+        assert torch.equal(m(x), want)
+
+
+def test_dense_mlp_shows_its_linears_to_global_hooks():
+    m, x, seen = _dense_mlp(), _r(2, 5, 32), []
+    hook = torch.nn.modules.module.register_module_forward_hook(lambda mod, args, out: seen.append(mod))
+    try:
+        m(x)
+    finally:
+        hook.remove()
+    assert m.linear_fc1 in seen and m.linear_fc2 in seen
+    calls = []
+    with pytest.MonkeyPatch.context() as patch:     # without hooks it is the operator again
+        patch.setattr(F_, "gated_mlp", lambda *a: calls.append(1) or x)
+        m(x)
+    assert calls == [1]
