@@ -6,6 +6,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 from torch.nn.modules.module import _has_any_global_hook
 
 from ..ops import functional as F_
@@ -38,6 +39,14 @@ def _stock(m: nn.Module, cls: type) -> bool:
     """Whether calling ``m`` is nothing but ``cls.forward``: not replaced or wrapped, with no hooks of its own or of all modules."""
     return (type(m) is cls and "forward" not in m.__dict__
             and not (m._forward_pre_hooks or m._forward_hooks or m._backward_hooks or m._backward_pre_hooks or _has_any_global_hook()))
+
+
+def gated_norm(norm: nn.Module, x: torch.Tensor, gate: torch.Tensor, norm_before_gate: bool = True) -> torch.Tensor:
+    """A mixer's output norm with its SiLU gate, as one operator where ``norm`` is a plain :class:`RMSNorm`; any other module in its
+    place, and one with hooks, is called with the norm's input alone."""
+    if _stock(norm, RMSNorm):
+        return norm(x, gate, norm_before_gate)
+    return norm(x) * F.silu(gate) if norm_before_gate else norm(x * F.silu(gate))
 
 
 class DenseMLP(nn.Module):

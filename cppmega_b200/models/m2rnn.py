@@ -17,7 +17,7 @@ import torch.nn.functional as F
 from ..config.model import M2RNNConfig
 from ..ops import functional as F_
 from ..parallel.state import ParallelContext
-from .common import RMSNorm, fp32_param, seed_for
+from .common import RMSNorm, fp32_param, gated_norm, seed_for
 
 
 class M2RNNMixer(nn.Module):
@@ -80,5 +80,5 @@ class M2RNNMixer(nn.Module):
         y = F_.m2rnn_scan(q, k, v, self.state_weight, f)                                       # [B,S,H,V]
         if self.D is not None:
             y = y + v * self.D
-        y = self.g_norm(y.flatten(-2, -1), gate=g, norm_before_gate=False)                     # g is read in place from proj
+        y = gated_norm(self.g_norm, y.flatten(-2, -1), g, norm_before_gate=False)              # g is read in place from proj
         return F_.linear(y, self.output_projection.weight)

@@ -27,7 +27,7 @@ from ..ops import functional as F_
 from ..ops import mimo_scan_ref
 from ..parallel.state import ParallelContext
 from ..parallel.tensor_parallel import ColumnParallelLinear, RowParallelLinear
-from .common import RMSNorm, fp32_param, seed_for
+from .common import RMSNorm, fp32_param, gated_norm, seed_for
 
 
 @dataclass(frozen=True)
@@ -125,7 +125,7 @@ class SSDMixer(nn.Module):
             Cm, Bm, xs.reshape(B_, S, H, P), ADT, DTt, trap_t, self.C_bias if v.bc_bias else zeros,
             self.B_bias if v.bc_bias else zeros, ones, None, ones, angles, self.D, None,
             self.cfg.mamba3.rotary_dim_divisor, max(self.cfg.mamba3.chunk_size, 32))
-        y = self.norm(y.reshape(B_, S, self.d_inner).to(x.dtype), gate=z)
+        y = gated_norm(self.norm, y.reshape(B_, S, self.d_inner).to(x.dtype), z)
         return self.out_proj(y)
 
 

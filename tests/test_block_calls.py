@@ -177,3 +177,35 @@ def test_dense_mlp_shows_its_linears_to_global_hooks():
         patch.setattr(F_, "gated_mlp", lambda *a: calls.append(1) or x)
         m(x)
     assert calls == [1]
+
+
+def _mixers():
+    from cppmega_b200.config.model import M2RNNConfig, nam56r_tiny
+    from cppmega_b200.models.m2rnn import M2RNNMixer
+    from cppmega_b200.models.mamba_variants import VARIANTS, SSDMixer
+    from cppmega_b200.parallel.state import single_process_context
+    cfg, pc = nam56r_tiny(), single_process_context()
+    return {"g_norm": M2RNNMixer(160, M2RNNConfig(), pc, 1),
+            "norm": SSDMixer(cfg, pc, 1, VARIANTS["ssd"], dtype=torch.float32, seed=3, out_std=0.1)}
+
+
+@pytest.mark.parametrize("name", ["g_norm", "norm"])
+def test_mixers_call_a_norm_that_is_not_the_stock_one(name):
+    """A norm without a gate argument in the place of the mixer's output norm, and hooks on it: called with its input alone."""
+    m = _mixers()[name]
+    x = _r(1, 64, m.input_projection.weight.shape[1] if name == "g_norm" else m.in_proj.weight.shape[1])
+    want, norm, seen = m(x), getattr(m, name), []
+
+    class Plain(torch.nn.Module):
+        def forward(self, t):
+            seen.append(t)
+            return F_.rmsnorm(t, norm.weight, norm.eps)
+
+    setattr(m, name, Plain())
+    got = m(x)
+    assert len(seen) == 1 and torch.allclose(got, want, rtol=1e-4, atol=1e-5)
+    setattr(m, name, norm)
+    hook = norm.register_forward_hook(lambda mod, args, out: seen.append(args[0]))
+    m(x)
+    hook.remove()
+    assert torch.allclose(seen[1], seen[0], rtol=1e-4, atol=1e-5)
