@@ -202,8 +202,9 @@ class _PackingContext(torch.autograd.graph.saved_tensors_hooks):
 
 def packing() -> bool:
     """Whether saved activations are being compressed: operators that keep them in a form of their own (bytes the hooks pass over)
-    step back for their plain composition then."""
-    return getattr(_state, "packing", 0) > 0 and not _disabled()
+    step back for their plain composition then.  Without gradients nothing is saved, so that both passes of a recomputed layer (the
+    second runs outside the context) take the same operators."""
+    return getattr(_state, "packing", 0) > 0 and torch.is_grad_enabled() and not _disabled()
 
 
 def fp8_activation_context(*, recipe: str = "mxfp8", n_layers: int = 0, bf16_first: int = 0, bf16_last: int = 0,

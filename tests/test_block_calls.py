@@ -209,3 +209,19 @@ def test_mixers_call_a_norm_that_is_not_the_stock_one(name):
     m(x)
     hook.remove()
     assert torch.allclose(seen[1], seen[0], rtol=1e-4, atol=1e-5)
+
+
+def test_recomputed_dense_mlp_takes_the_same_operator_in_both_passes(monkeypatch):
+    """FP8 storage of saved activations with recomputation: the first pass runs under the context, the replay outside it."""
+    from cppmega_b200.utils import fp8_activations as fa
+    from cppmega_b200.utils.recompute import checkpoint
+    m, x, calls = _dense_mlp(), _r(2, 5, 32).requires_grad_(), []
+    plain = F_.gated_mlp
+    monkeypatch.setattr(F_, "gated_mlp", lambda *a: calls.append(torch.is_grad_enabled()) or plain(*a))
+    with fa.fp8_activation_context():
+        y = checkpoint(m, x)
+        assert fa.packing()                      # tensors saved here are packed all the same
+        with torch.no_grad():
+            assert not fa.packing()
+    y.sum().backward()
+    assert calls == [False, True]
