@@ -121,8 +121,12 @@ class Fp8ActivationPacker:
         # one packed copy per distinct tensor: a normed activation that feeds three linears is saved three times
         self._seen: "weakref.WeakValueDictionary" = weakref.WeakValueDictionary()
 
+    def applies(self) -> bool:
+        """Whether tensors saved at this point are packed (as far as their type and size allow)."""
+        return not _disabled()
+
     def pack(self, t: Any) -> Any:
-        if (not isinstance(t, torch.Tensor) or _disabled() or t.dtype != torch.bfloat16 or t.numel() < self.min_elements
+        if (not isinstance(t, torch.Tensor) or not self.applies() or t.dtype != torch.bfloat16 or t.numel() < self.min_elements
                 or isinstance(t, torch.nn.Parameter) or _is_weight(t)):
             STATS["passed"] += 1
             return t
@@ -183,20 +187,21 @@ class LayerAwareFp8Packer(Fp8ActivationPacker):
         super().__init__(**kw)
         self.n_layers, self.bf16_first, self.bf16_last = n_layers, bf16_first, bf16_last
 
-    def pack(self, t: Any) -> Any:
-        if is_bf16_layer(current_layer_idx(), self.n_layers, self.bf16_first, self.bf16_last):
-            STATS["passed"] += 1
-            return t
-        return super().pack(t)
+    def applies(self) -> bool:
+        return super().applies() and not is_bf16_layer(current_layer_idx(), self.n_layers, self.bf16_first, self.bf16_last)
 
 
 class _PackingContext(torch.autograd.graph.saved_tensors_hooks):
+    def __init__(self, packer: Fp8ActivationPacker):
+        super().__init__(packer.pack, packer.unpack)
+        self.packer = packer
+
     def __enter__(self):
-        _state.packing = getattr(_state, "packing", 0) + 1
+        _state.packers = [*getattr(_state, "packers", ()), self.packer]
         return super().__enter__()
 
     def __exit__(self, *exc):
-        _state.packing -= 1
+        _state.packers = _state.packers[:-1]
         return super().__exit__(*exc)
 
 
@@ -204,7 +209,8 @@ def packing() -> bool:
     """Whether saved activations are being compressed: operators that keep them in a form of their own (bytes the hooks pass over)
     step back for their plain composition then.  Without gradients nothing is saved, so that both passes of a recomputed layer (the
     second runs outside the context) take the same operators."""
-    return getattr(_state, "packing", 0) > 0 and torch.is_grad_enabled() and not _disabled()
+    packers = getattr(_state, "packers", None)
+    return bool(packers) and torch.is_grad_enabled() and packers[-1].applies()
 
 
 def fp8_activation_context(*, recipe: str = "mxfp8", n_layers: int = 0, bf16_first: int = 0, bf16_last: int = 0,
@@ -217,4 +223,4 @@ def fp8_activation_context(*, recipe: str = "mxfp8", n_layers: int = 0, bf16_fir
                                                           min_elements=min_elements)
     else:
         packer = Fp8ActivationPacker(recipe=recipe, clamp=clamp, min_elements=min_elements)
-    return _PackingContext(packer.pack, packer.unpack)
+    return _PackingContext(packer)

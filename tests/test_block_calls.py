@@ -225,3 +225,21 @@ def test_recomputed_dense_mlp_takes_the_same_operator_in_both_passes(monkeypatch
             assert not fa.packing()
     y.sum().backward()
     assert calls == [False, True]
+
+
+def test_layers_that_stay_bf16_keep_the_fused_dense_mlp(monkeypatch):
+    """The first and last layers of a layer-aware storage pack nothing, so that nothing there has to step back for the packer."""
+    from cppmega_b200.utils import fp8_activations as fa
+    m, x, calls = _dense_mlp(), _r(2, 5, 32), []
+    monkeypatch.setattr(F_, "gated_mlp", lambda *a: calls.append(fa.current_layer_idx()) or x)
+    try:
+        for layer in range(5):
+            fa.set_current_layer_idx(layer)
+            with fa.fp8_activation_context(n_layers=5, bf16_first=1, bf16_last=2):
+                m(x)
+                with fa.fp8_activation_context():
+                    assert fa.packing()          # the inner context packs every layer
+                assert fa.packing() == (layer in (1, 2))
+    finally:
+        fa.set_current_layer_idx(-1)
+    assert calls == [0, 3, 4] and not fa.packing()
