@@ -318,6 +318,8 @@ def gated_mlp(x, w1, w2, activation: str = "silu"):
     if w1.dim() != 2 or w2.dim() != 2 or x.dim() < 1 or w1.shape[1] != x.shape[-1] or w1.shape[0] != 2 * w2.shape[1]:
         raise ValueError(f"gated_mlp: x {tuple(x.shape)}, w1 {tuple(w1.shape)}, w2 {tuple(w2.shape)}")
     _same_device("gated_mlp", x, w1, w2)
+    if x.numel() == 0 or w1.numel() == 0 or w2.numel() == 0:       # a sum over nothing is zero: no kernel has anything to read
+        return ref.gated_mlp(x, w1, w2, activation)
     fn = _cuda("gated_mlp", x) if _PRECISION_RECIPE == "bf16" else None
     if fn is not None:
         y = fn(x, w1, w2, activation)

@@ -243,3 +243,14 @@ def test_layers_that_stay_bf16_keep_the_fused_dense_mlp(monkeypatch):
     finally:
         fa.set_current_layer_idx(-1)
     assert calls == [0, 3, 4] and not fa.packing()
+
+
+@pytest.mark.parametrize("T,H,F,Ho", [(4, 16, 0, 16), (4, 16, 24, 0), (0, 16, 24, 16), (4, 0, 24, 16)])
+def test_gated_mlp_of_nothing_is_the_definition(monkeypatch, T, H, F, Ho):
+    """A width or a number of tokens of zero never asks for a kernel: the entries return without writing their results."""
+    monkeypatch.setattr(F_, "_cuda", lambda name, *t: pytest.fail(f"{name} asked for"))
+    leaves = [_r(*s, dtype=torch.bfloat16).requires_grad_() for s in ((T, H), (2 * F, H), (Ho, F))]
+    y = F_.gated_mlp(*leaves)
+    assert y.shape == (T, Ho) and y.dtype == torch.bfloat16 and (y == 0).all()
+    for g, t in zip(torch.autograd.grad(y, leaves, torch.ones_like(y)), leaves):
+        assert g.shape == t.shape and (g == 0).all()

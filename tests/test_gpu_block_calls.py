@@ -86,3 +86,17 @@ def test_saved_tensors_given_back_in_another_form(name, form):
             assert ((a.double() - b.double()).abs() <= 2 * 2 ** -8 * b.double().abs() + 2 ** -14 * b.double().abs().max()).all()
         else:
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T,H,F,Ho", [(4, 16, 0, 16), (4, 16, 24, 0), (0, 16, 24, 16), (4, 0, 24, 16), (300, 64, 0, 64)])
+def test_gated_mlp_of_nothing(T, H, F, Ho):
+    """A width or a number of tokens of zero: sums over nothing are zero, and so are their gradients."""
+    leaves = [_randn(*s).requires_grad_() for s in ((T, H), (2 * F, H), (Ho, F))]
+    junk = [torch.full((1 << 16,), float("nan"), device="cuda") for _ in range(8)]      # what unwritten results would hold
+    del junk
+    y = F_.gated_mlp(*leaves)
+    grads = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    with torch.no_grad():
+        again = F_.gated_mlp(*leaves)
+    assert y.shape == (T, Ho) and all(g.shape == t.shape for g, t in zip(grads, leaves))
+    assert all((t == 0).all() for t in (y, again, *grads))
