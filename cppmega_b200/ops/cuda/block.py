@@ -288,11 +288,12 @@ class ResidualRMSNormFn(torch.autograd.Function):
 
 @_on_device
 def residual_rmsnorm(y, residual, weight, post_weight, gate, scale, eps):
-    """None where the kernels do not apply: one type for all tensors (bf16, fp16 or fp32), rows of at most 16384."""
+    """None where the kernels do not apply: one type for all tensors (bf16, fp16 or fp32), rows of at most 16384, a scale that is a
+    number (a tensor may want a gradient)."""
     dt = y.dtype
     if (dt not in ROW_TYPES or residual.dtype != dt or weight.dtype != dt or (post_weight is not None and post_weight.dtype != dt)
             or (gate is not None and gate.dtype != dt) or y.shape[-1] > MAX_WIDTH or y.numel() == 0
-            or not _bare(y, residual, weight, post_weight, gate)):
+            or isinstance(scale, torch.Tensor) or not _bare(y, residual, weight, post_weight, gate)):
         return None
     weight = weight.contiguous()
     if post_weight is not None:

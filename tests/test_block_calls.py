@@ -254,3 +254,11 @@ def test_gated_mlp_of_nothing_is_the_definition(monkeypatch, T, H, F, Ho):
     assert y.shape == (T, Ho) and y.dtype == torch.bfloat16 and (y == 0).all()
     for g, t in zip(torch.autograd.grad(y, leaves, torch.ones_like(y)), leaves):
         assert g.shape == t.shape and (g == 0).all()
+
+
+def test_residual_rmsnorm_with_a_learnt_scale_is_the_definition():
+    """The kernels take the scale as a number: one that wants a gradient would not get it."""
+    x, w, scale = _r(4, 16), _r(16), torch.tensor(0.5, requires_grad=True)
+    assert block.residual_rmsnorm(x, x, w, None, None, scale, 1e-5) is None
+    n, h = F_.residual_rmsnorm(x, x, w, scale=scale)
+    assert torch.allclose(torch.autograd.grad(h.sum(), scale)[0], x.sum())

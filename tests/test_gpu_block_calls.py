@@ -100,3 +100,14 @@ def test_gated_mlp_of_nothing(T, H, F, Ho):
         again = F_.gated_mlp(*leaves)
     assert y.shape == (T, Ho) and all(g.shape == t.shape for g, t in zip(grads, leaves))
     assert all((t == 0).all() for t in (y, again, *grads))
+
+
+def test_residual_rmsnorm_with_a_learnt_scale():
+    """The gradient of a scale given as a tensor: sum of dh y over everything, 4096 fp32 products and their sum."""
+    y, x, w = _randn(64, 64, dtype=torch.float32), _randn(64, 64, dtype=torch.float32, seed=1), _randn(64, dtype=torch.float32, mean=1.0, std=0.1)
+    scale = torch.tensor(0.5, device="cuda", requires_grad=True)
+    dh = _randn(64, 64, dtype=torch.float32, seed=2)
+    _, h = F_.residual_rmsnorm(y, x, w, scale=scale)
+    (got,) = torch.autograd.grad(h, scale, dh)
+    terms = dh.double() * y.double()
+    assert abs(got.double() - terms.sum()) <= (64 + 4096) * 2 ** -24 * terms.abs().sum()
