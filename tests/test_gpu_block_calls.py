@@ -111,3 +111,38 @@ def test_residual_rmsnorm_with_a_learnt_scale():
     (got,) = torch.autograd.grad(h, scale, dh)
     terms = dh.double() * y.double()
     assert abs(got.double() - terms.sum()) <= (64 + 4096) * 2 ** -24 * terms.abs().sum()
+
+
+@pytest.mark.parametrize("before", [True, False])
+def test_gated_norm_in_fp32_far_out_gates(before):
+    """The gate's relative error does not grow with its distance from zero.  In units of 2^-24: the exponential 4 (2 ulp), 1 + e and the
+    quotient 1 each, the reciprocal root 5, products 1 each.  Rows of +-1 (with the gate first +-1 / silu(z)) have a mean square of one,
+    and 16 terms are summed without error (15 roundings with the gate first)."""
+    U = 2.0 ** -24
+    z = torch.linspace(-80, 2 if before else -1, 4096 * 16, device="cuda").reshape(4096, 16)
+    zd = z.double()
+    q = torch.sigmoid(zd)
+    a, slope = zd * q, q + zd * q * (1 - q)
+    sign = torch.where(torch.arange(16, device="cuda") % 2 == 0, 1.0, -1.0).expand(4096, 16)
+    x = (sign if before else sign / a.float()).contiguous().requires_grad_()
+    z, w = z.requires_grad_(), torch.ones(16, device="cuda")
+    dy = _randn(*z.shape, dtype=torch.float32, std=0.1, seed=3)
+    y = F_.rmsnorm_gated(x, w, z, EPS, None, before)
+    (dz,) = torch.autograd.grad(y, z, dy)
+    xd, e_slope = x.detach().double(), U * (7 * q + 16 * (zd * q).abs())
+    v = xd if before else xd * a
+    r = (v.square().mean(1, keepdim=True) + EPS).rsqrt()
+    if before:
+        want, bound = xd * r * a, 16 * U
+        wz = dy.double() * xd * r * slope
+        ez = 10 * U * wz.abs() + (dy.double() * xd * r).abs() * e_slope
+    else:
+        hat, g = v * r, dy.double()
+        want, bound = hat, 40 * U
+        m = (g * hat).mean(1, keepdim=True)
+        du = r * (g - hat * m)
+        wz = du * xd * slope
+        e_du = 60 * U * r * (g.abs() + 2 * hat.abs() * (g * hat).abs().mean(1, keepdim=True))
+        ez = 10 * U * wz.abs() + (du * xd).abs() * e_slope + e_du * (xd * slope).abs()
+    assert ((y.detach().double() - want).abs() <= bound * want.abs()).all()
+    assert ((dz.double() - wz).abs() <= ez).all()
