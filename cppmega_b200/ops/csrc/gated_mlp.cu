@@ -50,7 +50,9 @@ enum Act : int { SILU = 0, GELU_TANH = 1, RELU = 2 };
 
 // g and u are kept for the backward as 16-bit floats of 11 bits under one power of two per row and 32 columns: as bf16 they would bring a
 // third rounding of 2^-9 into dx and dw1, next to those of the products' operands and of the results (3.0e-3 against 2.4e-3 of the
-// gradients' norm).  The largest value of a group lies in [2^14, 2^15); what is 2^29 times smaller loses bits, and nothing overflows.
+// gradients' norm).  The largest value of a group lies in [2^14, 2^15); what is 2^29 times smaller loses bits, and nothing overflows.  Of a
+// gate that is closed, far out on its negative side, the size has no part in any gradient: it counts as closed_at, beyond which act and its
+// slope are zero in fp32, so that it does not take its neighbours' bits, and is kept as the lowest fp16 number where it has no room.
 //   kept = [M][2F] fp16 (g, then u), then [2][groups][M] bytes: the exponent field of the power that the values were multiplied with
 struct Kept {
   __half* v;
@@ -109,6 +111,18 @@ __device__ __forceinline__ void act_slope(Pair g, Pair& a, Pair& slope) {
     const Pair inner = b * pr_fma(b * b, pr(6.f * GELU_C * GELU_K), pr(2.f * GELU_C));
     slope = pr_fma(q * pr_fma(pr(-1.f), q, pr(1.f)), inner, q);        // q + q (1 - q) b 2 c (1 + 3 k b^2)
   }
+}
+
+// What a gate counts for in its group's power of two.
+template <int ACT>
+__device__ __forceinline__ float gate_size(float g) {
+  constexpr float closed_at = ACT == RELU ? 0.f : -128.f;
+  return fabsf(fmaxf(g, closed_at));
+}
+__device__ __forceinline__ uint32_t saturated_half2(float lo, float hi) {
+  uint32_t p;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+  return p;
 }
 
 // values 2 j and 2 j + 1 of an accumulator's row; two values as bf16
@@ -326,29 +340,28 @@ gated_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             tmem_ld_wait();
             uint32_t o[16];
             if (args.kept.v) {
-              auto keep = [&](const uint32_t (&v)[32], const CUtensorMap* map, uint8_t* power) {
+              auto keep = [&](const uint32_t (&v)[32], auto size, const CUtensorMap* map, uint8_t* power) {
                 float m = 0.f;
                 if (n0 + c + 32 <= args.F) {
 #pragma unroll
-                  for (int j = 0; j < 32; ++j) m = fmaxf(m, fabsf(__uint_as_float(v[j])));
+                  for (int j = 0; j < 32; ++j) m = fmaxf(m, size(__uint_as_float(v[j])));
                 } else {                                        // the gate's columns past the last are up's first rows: not of this group
 #pragma unroll
                   for (int j = 0; j < 32; ++j)
-                    if (n0 + c + j < args.F) m = fmaxf(m, fabsf(__uint_as_float(v[j])));
+                    if (n0 + c + j < args.F) m = fmaxf(m, size(__uint_as_float(v[j])));
                 }
                 const uint32_t field = power_for(m);
                 const float k = power_of(field);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                   const float2 f = pr_get(two(v, j) * pr(k));
-                  const __half2 p = __floats2half2_rn(f.x, f.y);
-                  o[j] = *reinterpret_cast<const uint32_t*>(&p);
+                  o[j] = saturated_half2(f.x, f.y);
                 }
                 out.put(map, o, n0 + c, row0);
                 if (row < args.M) power[(long long)((n0 + c) >> 5) * args.M + row] = uint8_t(field);
               };
-              keep(g, &tmO1, args.kept.power);
-              keep(u, &tmO2, args.kept.power + args.kept.plane);
+              keep(g, gate_size<ACT>, &tmO1, args.kept.power);
+              keep(u, [](float v) { return fabsf(v); }, &tmO2, args.kept.power + args.kept.plane);
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j) o[j] = bf16_of(act_of<ACT>(two(g, j)) * two(u, j));
@@ -574,10 +587,11 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_gate_kernel(const f
       lo[tok * F + f] = __float2bfloat16(isfinite(back) ? v - back : 0.f);
     }
     if (kept.v) {                             // a warp holds a group of 32 columns
-      const uint32_t gp = power_for(warp_max(fabsf(g[j]))), up = power_for(warp_max(fabsf(u[j])));
+      const uint32_t gp = power_for(warp_max(gate_size<ACT>(g[j]))), up = power_for(warp_max(fabsf(u[j])));
       if (col < F) {
-        kept.v[tok * 2 * F + f] = __float2half_rn(g[j] * power_of(gp));
-        kept.v[tok * 2 * F + F + f] = __float2half_rn(u[j] * power_of(up));
+        const uint32_t p = saturated_half2(g[j] * power_of(gp), u[j] * power_of(up));
+        kept.v[tok * 2 * F + f] = __ushort_as_half(uint16_t(p));
+        kept.v[tok * 2 * F + F + f] = __ushort_as_half(uint16_t(p >> 16));
       }
       if ((threadIdx.x & 31) == 0 && col < F) {
         uint8_t* e = kept.power + (long long)(f >> 5) * cut.tokens + tok;

@@ -146,3 +146,42 @@ def test_gated_norm_in_fp32_far_out_gates(before):
         ez = 10 * U * wz.abs() + (du * xd).abs() * e_slope + e_du * (xd * slope).abs()
     assert ((y.detach().double() - want).abs() <= bound * want.abs()).all()
     assert ((dz.double() - wz).abs() <= ez).all()
+
+
+@pytest.mark.parametrize("T", [20, 300])
+@pytest.mark.parametrize("ffn", [72, 200])
+@pytest.mark.parametrize("name,weight", [("relu", -3e38), ("relu", -1e12), ("silu", -1e30), ("silu", -1e12), ("gelu_tanh", -1e30)])
+def test_gated_mlp_closed_gate_leaves_its_neighbours_alone(T, ffn, name, weight):
+    """A gate far out on the negative side (the first overflows to -inf) is closed: results and gradients are those with a gate that is
+    closed at a moderate value, in its own column and in the 31 others that share its power of two."""
+    x, w1, w2 = _randn(T, 64), _randn(2 * ffn, 64, std=0.125, seed=1), _randn(64, ffn, std=0.1, seed=2)
+    x[:, 0] = 4.0
+    cols = [3, 40, ffn - 1]
+    w1[:ffn, 0] = 0.0
+    dy = _randn(T, 64, std=0.1, seed=3)
+    res = []
+    for closed in (weight, -256.0):                 # 4 * -256 and at most 64 * 4 * 0.6 beside it
+        w1[cols, 0] = closed
+        leaves = [t.detach().clone().requires_grad_() for t in (x, w1, w2)]
+        y = F_.gated_mlp(*leaves, name)
+        res.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+    (y, dx, dw1, dw2), (y2, *want) = res
+    assert torch.equal(y, y2) and torch.equal(dw1, want[1]) and torch.equal(dw2, want[2])
+    assert torch.equal(dx, want[0]) and want[1].abs().max() > 0
+
+
+@pytest.mark.parametrize("name", ["silu", "gelu_tanh", "relu"])
+@pytest.mark.parametrize("T", [20, 90])
+def test_gated_mlp_gradients_of_a_nan_row(T, name):
+    """A token that is NaN has gradients that are, and leaves the others' as they are."""
+    x, w1, w2 = _randn(T, 64), _randn(144, 64, std=0.125, seed=1), _randn(64, 72, std=0.1, seed=2)
+    dy, grads = _randn(T, 64, std=0.1, seed=3), []
+    for bad in (False, True):
+        leaf = x.clone()
+        if bad:
+            leaf[4, 7] = float("nan")
+        leaf.requires_grad_()
+        grads.append(torch.autograd.grad(F_.gated_mlp(leaf, w1, w2, name), leaf, dy)[0])
+    rest = torch.arange(T, device="cuda") != 4
+    assert torch.isnan(grads[1][4].float()).all()   # dg = dh u slope with u NaN, whatever the slope
+    assert torch.equal(grads[0][rest], grads[1][rest])
