@@ -207,7 +207,7 @@ static int gated_launch(const GatedArgs& a, bool back, int& blocks, cudaStream_t
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING) != cudaSuccess) return -2;             \
         configured[a.gate_first].done();                                                                                         \
       }                                                                                                                          \
-      static int resident[2];                                                                                                    \
+      static Resident resident[2];                                                                                                   \
       blocks = rv_blocks(kern, TB, RING, RPB, a.rows, a.width, groups, resident[a.gate_first]);                                                         \
       kern<<<dim3(blocks, groups), TB, RING, s>>>(a);                                                                            \
     } else {                                                                                                                     \

@@ -299,7 +299,7 @@ static int residual_launch(const ResidualArgs& a, bool back, int& blocks, cudaSt
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SLOT * (FULL ? 5 : 3)) != cudaSuccess) return -2; \
         configured.done();                                                                                                        \
       }                                                                                                                           \
-      static int resident[6];                                                                                                     \
+      static Resident resident[6];                                                                                                    \
       blocks = rv_blocks(kern, TB, SLOT * a.ring_ops, RPB, a.rows, a.width, 1, resident[a.ring_ops]);                                    \
       kern<<<blocks, TB, SLOT * a.ring_ops, s>>>(a);                                                                              \
     } else residual_norm_fwd<T, TPR, VPT, VEC, FULL><<<unsigned((a.rows + RPB - 1) / RPB), TB, 0, s>>>(a);                          \

@@ -6,6 +6,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "fp32_pair.cuh"
 
@@ -310,15 +312,24 @@ static inline long long rv_most_blocks(long long rows, int width, int share) {
   const long long most = ((long long)sm_count() * per_sm + share - 1) / share;
   return rows < most ? rows : most;
 }
-// `resident`: the runtime's answer for one kernel and amount of shared memory (0: not asked yet)
-template <typename K>
-static int rv_blocks(K kern, int threads, int smem, int rows_per_block, long long rows, int width, int share, int& resident) {
-  if (resident == 0) {
-    int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess || n < 1) n = 1;
-    resident = n;
+// Blocks of one kernel, with one amount of shared memory, that an SM holds: the runtime's answer, kept per device.  Backward passes on
+// several devices ask from several host threads.
+struct Resident {
+  std::atomic<int> kept[64] = {};
+  template <typename K>
+  int blocks(K kern, int threads, int smem) {
+    int dev = -1, n = 0;
+    const bool keep = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+    if (keep && (n = kept[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess || n < 1) return 1;
+    if (keep) kept[dev].store(n, std::memory_order_relaxed);
+    return n;
   }
-  const long long want = (rows + rows_per_block - 1) / rows_per_block, fit = ((long long)sm_count() * resident + share - 1) / share;
+};
+template <typename K>
+static int rv_blocks(K kern, int threads, int smem, int rows_per_block, long long rows, int width, int share, Resident& resident) {
+  const long long want = (rows + rows_per_block - 1) / rows_per_block;
+  const long long fit = ((long long)sm_count() * resident.blocks(kern, threads, smem) + share - 1) / share;
   const long long most = rv_most_blocks(rows, width, share), n = fit < most ? fit : most;
   return int(want < n ? want : n);
 }

@@ -262,3 +262,11 @@ def test_residual_rmsnorm_with_a_learnt_scale_is_the_definition():
     assert block.residual_rmsnorm(x, x, w, None, None, scale, 1e-5) is None
     n, h = F_.residual_rmsnorm(x, x, w, scale=scale)
     assert torch.allclose(torch.autograd.grad(h.sum(), scale)[0], x.sum())
+
+
+def test_launchers_keep_no_answer_of_one_device_for_all():
+    """What a launcher asks the runtime once, it asks per device; a plain static would serve every device and race between threads."""
+    import re
+    from cppmega_b200.ops.cuda.build import CSRC
+    for name in ("residual_norm.cu", "gated_norm.cu", "gated_mlp.cu", "few_rows.cu", "gemm_split.cu", "row_vec.cuh"):
+        assert not re.findall(r"\bstatic\s+(?:int|bool|long long|size_t)\s+\w+(?:\[\w+\])?\s*(?:=[^;()]*)?;", (CSRC / name).read_text()), name
