@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace cm {
 
 enum ErrorCode : int {
@@ -301,13 +303,19 @@ int sm_count();
 // Function attributes (the dynamic shared-memory limit) are per device: a flag per (call site, device) says whether the
 // current device has been configured.  Usage: `static PerDevice cfg; if (cfg.first()) { cudaFuncSetAttribute(...); cfg.done(); }`
 struct PerDevice {
-  bool set[64] = {};
-  int dev = -1;
-  bool first() {
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { dev = -1; return true; }
-    return !set[dev];
+  std::atomic<bool> set[64] = {};
+  static int current() {                  // -1: not kept, asked again
+    int dev = -1;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : -1;
   }
-  void done() { if (dev >= 0) set[dev] = true; }
+  bool first() {
+    const int dev = current();
+    return dev < 0 || !set[dev].load(std::memory_order_acquire);
+  }
+  void done() {
+    const int dev = current();
+    if (dev >= 0) set[dev].store(true, std::memory_order_release);
+  }
 };
 
 }  // namespace cm

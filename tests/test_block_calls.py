@@ -270,3 +270,32 @@ def test_launchers_keep_no_answer_of_one_device_for_all():
     from cppmega_b200.ops.cuda.build import CSRC
     for name in ("residual_norm.cu", "gated_norm.cu", "gated_mlp.cu", "few_rows.cu", "gemm_split.cu", "row_vec.cuh"):
         assert not re.findall(r"\bstatic\s+(?:int|bool|long long|size_t)\s+\w+(?:\[\w+\])?\s*(?:=[^;()]*)?;", (CSRC / name).read_text()), name
+
+
+def test_function_attributes_are_marked_on_the_device_that_was_set(tmp_path):
+    """Two host threads on two devices take turns between asking and marking: neither marks the other's device."""
+    import re
+    import subprocess
+    from cppmega_b200.ops.cuda.build import CSRC
+    struct = re.search(r"struct PerDevice \{.*?\n\};", (CSRC / "common.cuh").read_text(), re.S).group(0)
+    (tmp_path / "t.cpp").write_text("""#include <atomic>
+enum { cudaSuccess = 0 };
+static int current = 0;
+static int cudaGetDevice(int* d) { *d = current; return cudaSuccess; }
+%s
+int main() {
+  static PerDevice cfg;
+  bool a0 = cfg.first();           // thread A, device 0: sets its attribute ...
+  current = 1;
+  bool b0 = cfg.first();           // ... thread B, device 1, asks meanwhile ...
+  current = 0;
+  cfg.done();                      // ... and A marks device 0
+  bool a1 = cfg.first();
+  current = 1;
+  bool b1 = cfg.first();           // B has not marked device 1 yet
+  cfg.done();
+  return a0 && b0 && !a1 && b1 && !cfg.first() ? 0 : 1;
+}
+""" % struct)
+    subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "t"), str(tmp_path / "t.cpp")], check=True)
+    assert subprocess.run([str(tmp_path / "t")]).returncode == 0
