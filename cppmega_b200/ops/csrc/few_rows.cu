@@ -1,6 +1,6 @@
 // Weight matrix times few rows of activations: the weights are read once, at the memory's rate, and that is all of the time.
 //
-// The weights are the 128-row operand A of tcgen05.mma and the activations (up to 256 rows) its N side, so that one row costs the
+// The weights are the 128-row operand A of tcgen05.mma and the activations (up to 64 rows) its N side, so that one row costs the
 // tensor cores next to nothing.  What matters is that every SM streams the same number of weight bytes without a pause: the k blocks of
 // all tiles form one sequence that is cut into equal runs, one per block of a grid of one block per SM (a tile per block would leave
 // most SMs idle in the last wave: 336 tiles on 148 SMs are 2.3 waves), and the TMA ring holds all of shared memory (160 KB and more in
@@ -193,7 +193,7 @@ Cut cut_for(int tokens, int N, int K) {
 
 int launch_partials(const void* X, const void* X2, long long ldx, const void* W, float* part, const Cut& cut, int N, int K, bool early, int* err,
                     cudaStream_t stream) {
-  if (cut.tokens < 1 || cut.tokens > (X2 ? MAX_ROWS / 4 : MAX_ROWS) || cut.grid < 1) return -10;
+  if (cut.tokens < 1 || cut.tokens > MAX_ROWS || cut.grid < 1) return -10;
   Args a;
   a.cut = cut;
   a.tiles = (N + TILE - 1) / TILE;

@@ -5,7 +5,7 @@
 namespace cm {
 namespace few {
 
-constexpr int MAX_ROWS = 256;       // rows of activations
+constexpr int MAX_ROWS = 64;        // rows of activations
 constexpr int TILE = 128;           // weight rows of a tile
 
 // One product [tokens, N] = X [tokens, K] W [N, K]^T, cut into equal runs of 64-deep k blocks: block c of the grid works on the k blocks
@@ -46,8 +46,9 @@ inline int launch_early(void (*kern)(P...), dim3 grid, dim3 block, int smem, cud
   return cudaLaunchKernelEx(&cfg, kern, P(args)...) == cudaSuccess ? 0 : -3;
 }
 
-// X: row pitch ldx; X2: null, or what X lacks (X + X2 is multiplied; same pitch, tokens <= MAX_ROWS / 4); W: dense rows of K.  Bases and pitches on 16 bytes, K % 8 == 0, tokens <= MAX_ROWS.  early: X, and the work space's
-// last reader, are those of the kernel before it in the stream, and the weights are older: their loads start before that one has ended.
+// X: row pitch ldx; X2: null, or what X lacks (X + X2 is multiplied; same pitch); W: dense rows of K.  Bases and pitches on 16 bytes,
+// K % 8 == 0, tokens <= MAX_ROWS.  early: X, and the work space's last reader, are those of the kernel before it in the stream, and the
+// weights are older: their loads start before that one has ended.
 int launch_partials(const void* X, const void* X2, long long ldx, const void* W, float* part, const Cut& cut, int N, int K, bool early, int* err,
                     cudaStream_t stream);
 

@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(few::TILE * MAX_SHARE) few_sum_kernel(const fl
 //   3584 x 18944    76 / 101     77 /  83     82 /  86     91 /  90
 //   1024 x  2048    13 /  20     14 /  18     15 /  18     19 /  20
 //    256 x   512    11 /  10     11 /  10     12 /  10     11 /  11
-constexpr int FEW_TOKENS = few::MAX_ROWS / 4;
+constexpr int FEW_TOKENS = few::MAX_ROWS;
 
 // floats of the partial tiles, the larger of the two products', in whole 16 bytes; lo lies behind them
 static long long few_floats(const few::Cut& a, const few::Cut& b) { return a.floats() > b.floats() ? a.floats() : b.floats(); }

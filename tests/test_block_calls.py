@@ -299,3 +299,15 @@ int main() {
 """ % struct)
     subprocess.run(["g++", "-std=c++17", "-o", str(tmp_path / "t"), str(tmp_path / "t.cpp")], check=True)
     assert subprocess.run([str(tmp_path / "t")]).returncode == 0
+
+
+def test_few_row_products_take_what_the_feed_forward_gives_them():
+    """The limit of the streamed product is the dispatch's: no range that is accepted but never run."""
+    import re
+    from cppmega_b200.ops.cuda import lib
+    from cppmega_b200.ops.cuda.build import CSRC
+    most = int(re.search(r"MAX_ROWS = (\d+);", (CSRC / "few_rows.cuh").read_text()).group(1))
+    L, H, F = lib(), 1024, 2048
+    ws = [L.cm_gated_mlp_fwd_ws(m, H, F, H) for m in (most - 1, most, most + 1)]
+    # up to the limit the work space grows with the tokens: partial tiles, and h's second part of F / 2 floats a token
+    assert ws[1] > ws[0] > 0 and ws[2] != ws[1] + (ws[1] - ws[0])
