@@ -368,7 +368,8 @@ static inline int rv_team(int nvec, bool vec, bool by_warp) {
          : nvec <= 4096 ? 16 * 1024 + 4 : 0;
 }
 
-// CM_ROW_TEAM(team, vec, F): calls F(threads, vectors, vec) with compile-time values; -10 for a team that does not exist.
+// CM_ROW_TEAM(team, vec, F): calls F(threads, vectors, vec) with compile-time values; -10 for a team that does not exist.  Rows have up to
+// 16384 elements of type T: the largest team is one of 32-bit rows.
 #define CM_ROW_TEAMS(team, VEC, F)                     \
   switch (team) {                                      \
     case 16 * 8 + 1: return F(8, 1, VEC);              \
@@ -379,7 +380,9 @@ static inline int rv_team(int nvec, bool vec, bool by_warp) {
     case 16 * 256 + 2: return F(256, 2, VEC);          \
     case 16 * 512 + 2: return F(512, 2, VEC);          \
     case 16 * 1024 + 2: return F(1024, 2, VEC);        \
-    case 16 * 1024 + 4: return F(1024, 4, VEC);        \
+    case 16 * 1024 + 4:                                \
+      if constexpr (sizeof(T) == 4) return F(1024, 4, VEC); \
+      break;                                           \
   }
 #define CM_ROW_TEAM(team, vec, F)                      \
   if (vec) {                                           \

@@ -311,3 +311,18 @@ def test_few_row_products_take_what_the_feed_forward_gives_them():
     ws = [L.cm_gated_mlp_fwd_ws(m, H, F, H) for m in (most - 1, most, most + 1)]
     # up to the limit the work space grows with the tokens: partial tiles, and h's second part of F / 2 floats a token
     assert ws[1] > ws[0] > 0 and ws[2] != ws[1] + (ws[1] - ws[0])
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_norm_entries_refuse_rows_wider_than_the_operators(dtype):
+    """The C entries take the widths that the operators do, up to 16384; pointers are never looked at."""
+    from cppmega_b200.ops.cuda import lib
+    L = lib()
+    for W in (16392, 20000, 32768):
+        assert L.cm_residual_rmsnorm_fwd(16, W, 16, W, 16, None, None, 0, 16, 16, None, None, 2, W, 1.0, 1e-5, dtype, None) == -10
+        assert L.cm_residual_rmsnorm_fwd(16, W, 16, W, 16, 16, 16, 0, 16, 16, None, None, 2, W, 1.0, 1e-5, dtype, None) == -10
+        assert L.cm_residual_rmsnorm_bwd(16, W, None, 0, 16, None, 0, 16, None, None, 0, 16, 16, 16, None, None, None, None, None, None, 2, W, 1.0,
+                                         dtype, None) == -10
+        for gate_first in (0, 1):
+            assert L.cm_rmsnorm_gated_fwd(16, W, None, 0, 16, 16, None, 2, W, W, gate_first, 1e-5, dtype, None) == -10
+            assert L.cm_rmsnorm_gated_bwd(16, W, None, 0, 16, 16, W, 16, 16, None, None, None, 2, W, W, gate_first, dtype, None) == -10
