@@ -185,3 +185,36 @@ def test_gated_mlp_gradients_of_a_nan_row(T, name):
     rest = torch.arange(T, device="cuda") != 4
     assert torch.isnan(grads[1][4].float()).all()   # dg = dh u slope with u NaN, whatever the slope
     assert torch.equal(grads[0][rest], grads[1][rest])
+
+
+# ---- products whose first rows are done whole and whose last rows are split --------------------------------------------
+
+MIXED = {False: [(4408, 3080, 2056), (4112, 1032, 8200), (9480, 264, 2056), (1448, 3080, 8200)],
+         True: [(4112, 1032, 4104), (1448, 3080, 4104), (9736, 264, 4104), (4408, 1032, 4104)]}
+
+
+@pytest.mark.parametrize("a_mn", [False, True])
+@pytest.mark.parametrize("b_mn,M,N,K", [(b, *s) for b, shapes in MIXED.items() for s in shapes])
+@pytest.mark.parametrize("fp32,accumulate,pad", [(False, False, 0), (True, True, 4), (False, True, 3), (True, False, 5)])
+def test_gemm_split_after_whole_rows(a_mn, b_mn, M, N, K, fp32, accumulate, pad):
+    """Both parts of a mixed plan, every row of the result, in rows of any pitch.  One rounding to the result's type; K products and their
+    sums in fp32, in any order."""
+    import ctypes
+    from cppmega_b200.ops import cuda as cu
+    L = cu.lib()
+    plan = (ctypes.c_int * 4)()
+    floats = L.cm_gemm_split_plan(torch.cuda.get_device_properties(0).multi_processor_count, M, N, K, int(b_mn), plan)
+    assert 0 < plan[0] < M and plan[2] > 1 and floats > 0
+    a, b = _randn(*((K, M) if a_mn else (M, K))), _randn(*((K, N) if b_mn else (N, K)), seed=1)
+    c0 = _randn(M, N + pad, dtype=torch.float32 if fp32 else torch.bfloat16, seed=2)
+    c, ws = c0.clone(), torch.full((floats + 64,), float("nan"), device="cuda")
+    assert L.cm_gemm_split(a.data_ptr(), b.data_ptr(), c.data_ptr(), M, N, K, a.stride(0), b.stride(0), N + pad, int(a_mn), int(b_mn), int(fp32),
+                           int(accumulate), ws.data_ptr(), cu.err_word().data_ptr(), cu.stream_ptr()) == 0
+    torch.cuda.synchronize()
+    cu.check_errors()
+    x, y = (a.t() if a_mn else a).double(), (b if b_mn else b.t()).double()
+    before = c0[:, :N].double()
+    want = x @ y + (before if accumulate else 0)
+    size = x.abs() @ y.abs() + (before.abs() if accumulate else 0)
+    assert ((c[:, :N].double() - want).abs() <= (0 if fp32 else 2 ** -8) * want.abs() + (64 + K) * 2 ** -24 * size).all()
+    assert torch.equal(c[:, N:], c0[:, N:]) and ws[floats:].isnan().all() and not ws[:floats].isnan().any()
