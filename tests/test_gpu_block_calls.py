@@ -218,3 +218,78 @@ def test_gemm_split_after_whole_rows(a_mn, b_mn, M, N, K, fp32, accumulate, pad)
     size = x.abs() @ y.abs() + (before.abs() if accumulate else 0)
     assert ((c[:, :N].double() - want).abs() <= (0 if fp32 else 2 ** -8) * want.abs() + (64 + K) * 2 ** -24 * size).all()
     assert torch.equal(c[:, N:], c0[:, N:]) and ws[floats:].isnan().all() and not ws[:floats].isnan().any()
+
+
+# ---- many rows a block --------------------------------------------------------------------------------------------------
+
+def _against_chunks(call, rows, grads, shared):
+    """One call over all rows against calls over 100 rows each, where no block has a second one.  What belongs to a row has the same bits;
+    the gradients of what the rows share are the same fp32 terms in another order: at most 64 + rows / 100 additions on either side."""
+    def run(cut):
+        outs, leaves = call(cut)
+        return [t.detach() for t in outs], torch.autograd.grad(outs, leaves, [g[cut] for g in grads])
+
+    outs, back = run(slice(None))
+    parts = [run(slice(i, i + 100)) for i in range(0, rows, 100)]
+    for k, t in enumerate(outs):
+        assert torch.equal(t, torch.cat([p[0][k] for p in parts]))
+    for k, t in enumerate(back):
+        if k not in shared:
+            assert torch.equal(t, torch.cat([p[1][k] for p in parts])), k
+        elif t.dtype == torch.float32:
+            total, size = sum(p[1][k].double() for p in parts), shared[k]
+            assert ((t.double() - total).abs() <= 2 * (64 + rows / 100) * 2 ** -24 * size).all(), k
+    return outs, back
+
+
+MANY = [(12000, 816), (8000, 333), (40000, 64), (20001, 16), (3001, 4096), (2500, 8192), (6000, 2048)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("before", [True, False])
+@pytest.mark.parametrize("rows,group,groups", [(r, w, 1) for r, w in MANY] + [(9000, 1024, 8), (5000, 333, 3)])
+def test_gated_norm_with_many_rows_a_block(dtype, before, rows, group, groups):
+    import test_gpu_block as tb
+    D = group * groups
+    x, w, z = _randn(rows, D, dtype=dtype), _randn(D, dtype=dtype, mean=1.0, std=0.1, seed=1).requires_grad_(), _randn(rows, D, dtype=dtype, std=2.0, seed=2)
+    dy = _randn(rows, D, dtype=dtype, std=0.1, seed=3)
+
+    def call(cut):
+        ins = [x[cut].detach().requires_grad_(), w, z[cut].detach().requires_grad_()]
+        return [F_.rmsnorm_gated(*ins, EPS, group, before)], ins
+
+    xd, zd = x.double(), z.double()
+    a = zd * torch.sigmoid(zd)
+    v = (xd if before else xd * a).view(rows, groups, group)
+    hat = (v * (v.square().mean(-1, keepdim=True) + EPS).rsqrt()).view(rows, D)
+    terms = (dy.double() * hat * (a if before else 1)).abs().sum(0)
+    (y,), (dx, dw, dz) = _against_chunks(call, rows, [dy], {1: 1.01 * terms})
+    tb._check_gated(x, w, z, group, before, y, dict(x=dx, w=dw, z=dz), dy)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("post,gate,scale", [(False, "none", 1.0), (False, "none", 0.22), (True, "channel", 0.5), (True, "token", -0.5)])
+@pytest.mark.parametrize("rows,width", MANY)
+def test_residual_rmsnorm_with_many_rows_a_block(dtype, post, gate, scale, rows, width):
+    import test_gpu_block as tb
+    ins = tb._residual_inputs((rows,), width, dtype, post, gate)
+    names = list(ins)
+    dn, dh = (_randn(rows, width, dtype=dtype, std=0.1, seed=s) for s in (11, 12))
+
+    def call(cut):
+        leaves = {k: (t[cut] if t.dim() > 1 else t).detach().requires_grad_() for k, t in ins.items()}
+        n, h = F_.residual_rmsnorm(leaves["y"], leaves["residual"], leaves["weight"], leaves.get("post_weight"), leaves.get("gate"), scale, EPS)
+        return [n, h], list(leaves.values())
+
+    d = {k: t.double() for k, t in ins.items()}
+    y, one = d["y"], torch.ones(width, dtype=torch.float64, device="cuda")
+    hat = y * (y.square().mean(-1, keepdim=True) + EPS).rsqrt() if post else y
+    gs = scale * d.get("gate", one)
+    h = d["residual"] + gs * hat * d.get("post_weight", one)
+    rho = (h.square().mean(-1, keepdim=True) + EPS).rsqrt()
+    g = dn.double() * d["weight"]
+    full = rho * (g - h * rho * (g * h * rho).mean(-1, keepdim=True)) + dh.double()
+    sizes = {"weight": dn.double() * h * rho, "post_weight": gs * full * hat, "gate": scale * full * hat * d.get("post_weight", one)}
+    shared = {names.index(k): 1.01 * sizes[k].abs().sum(0) for k in sizes if k in ins and ins[k].dim() == 1}
+    (n, h), back = _against_chunks(call, rows, [dn, dh], shared)
+    tb._check_residual(ins, scale, n, h, dict(zip(names, back)), dn, dh)
