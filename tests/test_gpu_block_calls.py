@@ -293,3 +293,34 @@ def test_residual_rmsnorm_with_many_rows_a_block(dtype, post, gate, scale, rows,
     shared = {names.index(k): 1.01 * sizes[k].abs().sum(0) for k in sizes if k in ins and ins[k].dim() == 1}
     (n, h), back = _against_chunks(call, rows, [dn, dh], shared)
     tb._check_residual(ins, scale, n, h, dict(zip(names, back)), dn, dh)
+
+
+@pytest.mark.parametrize("name", ["relu", "gelu_tanh"])
+def test_gated_mlp_activations_against_differences(name):
+    """The gradient along a random direction against the formula's own difference; relu's gates stay on their side of the kink (+-8 with
+    a spread of one, moved by an eighth), where the block is a quadratic and a central difference exact."""
+    import test_gpu_block as tb
+    x, w1, w2 = (t.clone() for t in tb._mlp_inputs((64,), 64, 64, 64))
+    x[:, 0] = 4.0
+    if name == "relu":
+        w1[:64, 0] = 2.0 * torch.where(torch.arange(64, device="cuda") % 3 == 0, -1.0, 1.0).bfloat16()
+    v, dy = _randn(64, 64, seed=5), _randn(64, 64, seed=6)
+    v[:, 0] = 0
+    leaf = x.clone().requires_grad_()
+    (dx,) = torch.autograd.grad(F_.gated_mlp(leaf, w1, w2, name), leaf, dy)
+    xd, vd, w1d, w2d, dyd = (t.double() for t in (x, v, w1, w2, dy))
+
+    def exact(t):
+        gu = t @ w1d.t()
+        return ((tb._act(name, gu[:, :64])[0] * gu[:, 64:]) @ w2d.t() * dyd).sum()
+
+    def slope(e):
+        return (exact(xd + e * vd) - exact(xd - e * vd)) / (2 * e)
+
+    want, half = slope(2.0 ** -3), slope(2.0 ** -4)
+    g, up = (xd @ w1d.t()).split(64, 1)
+    a, s, _ = tb._act(name, g)
+    dh = dyd @ w2d
+    size = torch.cat([dh * up * s, dh * a], 1).abs() @ w1d.abs()
+    # bf16: the two gradients and the result (2^-8 each of what they are or are summed from); g and u with 11 bits: another 2^-8 at most
+    assert abs((dx.double() * vd).sum() - want) <= 2 * abs(want - half) + 4 * 2 ** -8 * (size * vd.abs()).sum()
