@@ -11,7 +11,6 @@ import functools
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from .. import cuda as _cu
 from .. import functional as F_
@@ -66,13 +65,31 @@ def _on_device(fn):
     return call
 
 
-def _first_order(fn):
-    """``backward`` without a graph of its own.  Only under ``create_graph`` does it go through the library's guard, which makes a second
-    derivative raise (the guard costs as much as a launch)."""
-    guarded = once_differentiable(fn)
+class _Undifferentiable(torch.autograd.Function):
+    """Passes its first ``n`` tensors on as results that depend on all of its tensors and refuse to be differentiated."""
 
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tuple(t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
     def backward(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+        raise RuntimeError("the kernels around a dense block have first derivatives only; ops.reference has the definitions, which can be "
+                           "differentiated again")
+
+
+def _first_order(fn):
+    """``backward`` without a graph of its own.  Under ``create_graph`` its results are tied to everything that they were computed from, so
+    that a second derivative raises on every way to it instead of missing a term."""
+    def backward(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return fn(ctx, *grads)
+        with torch.no_grad():
+            outs = fn(ctx, *grads)
+        own = [t for t in outs if t is not None]
+        roots = [t for t in (*ctx.saved_tensors, *grads) if t is not None and t.requires_grad]
+        tied = iter(_Undifferentiable.apply(len(own), *own, *roots))
+        return tuple(None if t is None else next(tied) for t in outs)
     return backward
 
 

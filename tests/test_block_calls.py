@@ -326,3 +326,30 @@ def test_norm_entries_refuse_rows_wider_than_the_operators(dtype):
         for gate_first in (0, 1):
             assert L.cm_rmsnorm_gated_fwd(16, W, None, 0, 16, 16, None, 2, W, W, gate_first, 1e-5, dtype, None) == -10
             assert L.cm_rmsnorm_gated_bwd(16, W, None, 0, 16, 16, W, 16, 16, None, None, None, 2, W, W, gate_first, dtype, None) == -10
+
+
+def _without_kernels(monkeypatch):
+    """Forward and backward of the wrappers with a library that computes nothing."""
+    library = _Recorder("", {})
+    monkeypatch.setattr(block._cu, "lib", lambda: library)
+    monkeypatch.setattr(block._cu, "err_word", lambda dev: torch.zeros(1))
+    monkeypatch.setattr(block._cu, "stream_ptr", lambda: None)
+    monkeypatch.setattr(block, "_size", lambda *a: 64)
+
+
+@pytest.mark.parametrize("name", ["gated_mlp", "residual_rmsnorm", "rmsnorm_gated"])
+def test_second_derivatives_raise_beside_other_terms(monkeypatch, name):
+    """A term that needs a second derivative may not go missing from a sum whose other terms have theirs: not with an upstream gradient
+    that is a constant, and not where only some leaves are asked for."""
+    _without_kernels(monkeypatch)
+    call, args = _block_calls()[name]
+    leaves = [t.requires_grad_() for t in args]
+    for asked in leaves:
+        y = call(*leaves)
+        y = y[0] if isinstance(y, tuple) else y
+        (g,) = torch.autograd.grad(y.sum(), leaves[0], create_graph=True)
+        assert g.requires_grad
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum() + asked.sum(), asked)
+        with pytest.raises(RuntimeError):
+            (g.sum() + asked.sum()).backward()
