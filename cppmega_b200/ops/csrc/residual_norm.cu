@@ -9,9 +9,9 @@
 // The second mean is linear in the first: with S1 = sum g hh, S2 = sum a yh (rho g + dh0), S3 = sum a yh hh it is
 // (S2 - rho S1 S3 / W) / W, so that a row is read once and reduced once.
 // Bound by memory: forward 4 rows moved, backward 4, with post norm or gate 6.  16384 x 4096 in bf16: forward 80 us and backward 94 (83 each
-// at the copy rate); with post norm and gate 88 and 162 (83, 125): there the backward is short of issue slots, at two blocks an SM for
-// its registers.  A team of threads holds a row (rv_team), so that it crosses memory once each way.  Sums over rows go through one partial row per block and a second
-// kernel in a fixed order: the same call gives the same bits.
+// at the copy rate); with post norm and gate 88 and 162 (83, 125): two blocks an SM, for its 128 registers, do not hide the time between a
+// row's sums and its results.  A team of threads holds a row (rv_team), so that it crosses memory once each way.  Sums over rows go through
+// one partial row per block and a second kernel in a fixed order: the same call gives the same bits.
 #include "row_vec.cuh"
 #define CM_ROW_TEAM_BY_WARP(team, F)
 

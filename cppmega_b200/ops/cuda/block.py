@@ -3,6 +3,7 @@
 
 The wrappers take their tensors as they come: leading dimensions of any number, rows of any pitch (column slices of a wider
 projection are read in place), widths that no vector divides.  Work space is allocated per call on the current stream.
+A kernel reads memory and gives first derivatives: what needs more than that is left to the definitions, or raises.
 """
 from __future__ import annotations
 

@@ -257,7 +257,8 @@ def rmsnorm(x, weight, eps: float = 1e-5):
 def rmsnorm_gated(x, weight, z=None, eps: float = 1e-5, group_size=None, norm_before_gate=True):
     """RMS norm of a mixer's output with a SiLU gate: ``rms(x) * weight * silu(z)``, or ``rms(x * silu(z)) * weight`` with
     ``norm_before_gate=False``; every ``group_size`` channels normalise apart (default: the whole row).  ``x``, ``z`` [..., D] of
-    one type, rows of any pitch (column slices of a projection are read in place), ``weight`` [D]."""
+    one type, rows of any pitch (column slices of a projection are read in place), ``weight`` [D].  The kernels have first derivatives;
+    forward mode, function transforms and batches of upstream gradients run the definition, ``reference.rmsnorm_gated``."""
     D = x.shape[-1]
     group = int(group_size) if group_size else D
     fn = _cuda("rmsnorm_gated", x)
@@ -276,7 +277,8 @@ def residual_rmsnorm(y, residual, weight, post_weight=None, gate=None, scale: fl
     """The step between two blocks: ``h = residual + scale * gate * p`` with ``p = rms(y) * post_weight`` (``y`` itself without a
     post norm), and the norm the next block reads, ``n = rms(h) * weight``.  Returns ``(n, h)``, both in the type of ``y``; ``n``
     is the norm of ``h`` as rounded to that type.  ``y``, ``residual`` [..., D]; ``gate`` [D] (one per channel, shared by all
-    rows) or the shape of ``y``; ``weight``, ``post_weight`` [D]."""
+    rows) or the shape of ``y``; ``weight``, ``post_weight`` [D].  The kernels take ``scale`` as a number and have first derivatives; a
+    scale that is a tensor, forward mode and function transforms run the definition, ``reference.residual_rmsnorm``."""
     row = y.shape[-1:]
     if residual.shape != y.shape:
         raise ValueError(f"residual_rmsnorm: block output {tuple(y.shape)}, residual {tuple(residual.shape)}")
@@ -311,8 +313,8 @@ def head_linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
 def gated_mlp(x, w1, w2, activation: str = "silu"):
     """Gated feed-forward block ``(act(x Wg^T) * (x Wu^T)) W2^T``: ``x`` [..., H], ``w1`` [2F, H] (the gate rows, then the up rows),
     ``w2`` [Ho, F]; ``activation`` is ``silu``, ``gelu_tanh`` or ``relu``.  In bf16 with widths that are multiples of 8 the
-    projections, the activation and the product are one kernel, and so are their gradients; under an FP8 recipe, and for anything
-    else, it is :func:`linear`, activation, :func:`linear`."""
+    projections, the activation and the product are one kernel, and so are their gradients (first derivatives); under an FP8 recipe,
+    and for anything else, it is :func:`linear`, activation, :func:`linear`."""
     if activation not in ref.GATED_ACTIVATIONS:
         raise ValueError(f"gated_mlp: unknown activation {activation!r}, one of {sorted(ref.GATED_ACTIVATIONS)}")
     if w1.dim() != 2 or w2.dim() != 2 or x.dim() < 1 or w1.shape[1] != x.shape[-1] or w1.shape[0] != 2 * w2.shape[1]:
