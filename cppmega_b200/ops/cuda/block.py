@@ -110,11 +110,10 @@ def _size(name: str, device: int, *args) -> int:
     return getattr(_cu.lib(), name)(*args)
 
 
-def _rows(t: torch.Tensor):
-    """``(tensor, elements between rows)`` of the [rows, width] view of a tensor whose rows are contiguous and evenly spaced; any
-    other tensor is copied."""
+def _pitch(t: torch.Tensor):
+    """Elements between rows of the [rows, width] view of a tensor whose rows are contiguous and evenly spaced; None for any other."""
     if t.is_contiguous():
-        return t, t.shape[-1]
+        return t.shape[-1]
     if t.stride(-1) == 1 or t.shape[-1] == 1:
         pitch = expect = None
         for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
@@ -123,14 +122,40 @@ def _rows(t: torch.Tensor):
             if pitch is None:
                 pitch = expect = s
             if s != expect:
-                pitch = 0
-                break
+                return None
             expect = s * n
         if pitch is None:
-            return t, t.shape[-1]
+            return t.shape[-1]
         if pitch >= t.shape[-1]:
-            return t, pitch
-    return _cu.fast_contiguous(t), t.shape[-1]
+            return pitch
+    return None
+
+
+def _rows(t: torch.Tensor):
+    """``(tensor, elements between rows)`` of the [rows, width] view; a tensor without one is copied."""
+    pitch = _pitch(t)
+    return (t, pitch) if pitch is not None else (_cu.fast_contiguous(t), t.shape[-1])
+
+
+class _Copied(torch.autograd.Function):
+    """A packed copy that stays tied to its original."""
+
+    @staticmethod
+    def forward(ctx, t):
+        return _cu.fast_copy_(torch.empty(t.shape, dtype=t.dtype, device=t.device), t)
+
+    @staticmethod
+    def backward(ctx, g):
+        return g
+
+
+def _readable(t, tma: bool = False):
+    """The tensor, or a copy where the kernels cannot read it in place: made before the operator's own function, which saves what it is
+    given, so that a second derivative finds its way from there to the original."""
+    if t is None:
+        return t
+    pitch = _pitch(t)
+    return t if pitch is not None and not (tma and (pitch % 8 or t.data_ptr() % 16)) else _Copied.apply(t)
 
 
 def _given_back(t, dtype: torch.dtype, device: torch.device, packed: bool = True, align: int = 1):
@@ -228,7 +253,7 @@ def gated_mlp(x, w1, w2, activation):
             and w2.data_ptr() % 16 == 0 and x.numel() // x.shape[-1] < 2 ** 30):
         return None
     if torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad):
-        return GatedMLPFn.apply(x, w1, w2, ACTIVATIONS[activation])
+        return GatedMLPFn.apply(_readable(x, tma=True), w1, w2, ACTIVATIONS[activation])
     return _mlp_forward(x, w1, w2, ACTIVATIONS[activation], keep=False)[0]
 
 
@@ -320,7 +345,7 @@ def residual_rmsnorm(y, residual, weight, post_weight, gate, scale, eps):
         gate = gate.contiguous()
     if torch.is_grad_enabled() and (y.requires_grad or residual.requires_grad or weight.requires_grad
                                     or (post_weight is not None and post_weight.requires_grad) or (gate is not None and gate.requires_grad)):
-        return ResidualRMSNormFn.apply(y, residual, weight, post_weight, gate, float(scale), float(eps))
+        return ResidualRMSNormFn.apply(_readable(y), residual, weight, post_weight, gate, float(scale), float(eps))
     return _residual_forward(y, residual, weight, post_weight, gate, float(scale), float(eps), keep=False)[:2]
 
 
@@ -406,7 +431,7 @@ def rmsnorm_gated(x, weight, z, eps, group, norm_before_gate):
         return None
     weight = weight.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (z is not None and z.requires_grad)):
-        return GatedRMSNormFn.apply(x, weight, z, float(eps), group, not norm_before_gate)
+        return GatedRMSNormFn.apply(_readable(x), weight, _readable(z), float(eps), group, not norm_before_gate)
     return _gated_forward(x, weight, z, float(eps), group, not norm_before_gate, keep=False)[0]
 
 

@@ -353,3 +353,17 @@ def test_second_derivatives_raise_beside_other_terms(monkeypatch, name):
             torch.autograd.grad(g.sum() + asked.sum(), asked)
         with pytest.raises(RuntimeError):
             (g.sum() + asked.sum()).backward()
+
+
+@pytest.mark.parametrize("name,i", [("gated_mlp", 0), ("residual_rmsnorm", 0), ("rmsnorm_gated", 0), ("rmsnorm_gated", 2)])
+def test_second_derivatives_raise_through_an_input_that_was_copied(monkeypatch, name, i):
+    """Columns that are not contiguous are copied for the kernels; the copy is still the caller's tensor, here the only one with a gradient."""
+    _without_kernels(monkeypatch)
+    call, args = _block_calls()[name]
+    leaf = args[i].t().contiguous().requires_grad_()
+    y = call(*[leaf.t() if j == i else t for j, t in enumerate(args)])
+    y = y[0] if isinstance(y, tuple) else y
+    (g,) = torch.autograd.grad(y.sum(), leaf, create_graph=True)
+    assert g.shape == leaf.shape
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum() + leaf.sum(), leaf)
