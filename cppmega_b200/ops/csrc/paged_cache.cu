@@ -1,0 +1,349 @@
+// Rows of a paged key-value cache: written (quantised on the way where the cache holds E4M3) and read back into packed sequences.
+//
+//   write   cache[slot / page, slot % page, h, :] = x[t, h, :]               16-bit caches: the same bits
+//           e4m3(x / 2^e), e = ceil(log2(max |x| / 448))                     E4M3 caches, one exponent byte e + 127 per row (token, head)
+//   read    y[t, h, :] = cache[table[s, p / page], p % page, h, :] (x 2^e)   t the p-th token of sequence s
+//
+// One power of two per row: multiplying by it is exact, so a value is rounded once, to the 4 bits of E4M3, and the attention that reads the
+// cache can leave the power out of its products.  The exponent's largest value is taken over the finite values of the row; what is not finite is
+// stored as NaN.
+//
+// Both are copies: bytes in and out at the memory's rate is all there is.  A row belongs to 8 or 16 lanes, 16 bytes of it to each (8 of an
+// E4M3 row), so rows of any stride move in whole sectors, and four rows of every lane group are in flight at once.
+//
+// Of tokens that are given the same slot the last one stays, whatever order the blocks run in: each block looks for its own slots among the
+// later tokens (a bit table in shared memory answers for almost all of them).  It reads the list of slots once per block, 5 % of the bytes
+// that move at 16384 tokens of 8 heads.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "paged.cuh"
+
+namespace cm {
+namespace paged {
+
+constexpr int THREADS = 256;
+constexpr int MAX_TOKENS = 128;              // tokens of one block
+constexpr int HASH_BITS = 8192;
+constexpr int ROWS_AHEAD = 4;
+
+struct Side {                                // keys or values
+  const uint8_t* x;                          // rows of the packed tensor
+  long long x_tok, x_head;                   // strides in bytes
+  uint8_t* cache;
+  long long c_page, c_tok, c_head;           // strides in bytes
+  uint8_t* scale;                            // [pages, page, heads] or null
+  int lanes, width;                          // lanes of a row, 16-byte pieces of the packed row (8 values each)
+};
+
+struct WriteArgs {
+  Side side[2];
+  int sides;
+  const void* slots;
+  long long total;                           // slots of the cache
+  int wide;                                  // slots are 64-bit
+  int T, heads, page, per_block;
+  int* err;
+};
+
+__device__ __forceinline__ long long slot_of(const WriteArgs& a, long long t) {
+  return a.wide ? reinterpret_cast<const long long*>(a.slots)[t] : (long long)reinterpret_cast<const int*>(a.slots)[t];
+}
+
+template <typename T>
+__device__ __forceinline__ float2 two(uint32_t v);
+template <>
+__device__ __forceinline__ float2 two<__nv_bfloat16>(uint32_t v) {
+  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+}
+template <>
+__device__ __forceinline__ float2 two<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t join(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t join<__nv_bfloat16>(float a, float b) { return pack_bf16(a, b); }
+template <>
+__device__ __forceinline__ uint32_t join<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// exponent byte of a row's largest magnitude: the smallest e with amax <= 448 * 2^e = 1.75 * 2^(e + 8), read off its bits
+__device__ __forceinline__ int exponent_byte(float amax) {
+  if (!(amax > 0.f)) return 127;
+  const uint32_t u = __float_as_uint(amax);
+  const int e = int(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u);
+  return e < 1 ? 1 : e;                      // at most 254 - 8 + 1
+}
+
+template <typename T>
+__device__ __forceinline__ uint2 quantised(const uint4& v, float inv) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t out[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = two<T>(w[i >> 1]);
+    const float x = (i & 1) ? f.y : f.x;
+    const uint32_t b = isfinite(x) ? (uint32_t)__nv_cvt_float_to_fp8(x * inv, __NV_SATFINITE, __NV_E4M3) : 0x7fu;
+    out[i >> 2] |= b << (8 * (i & 3));
+  }
+  return make_uint2(out[0], out[1]);
+}
+
+template <typename T>
+__device__ __forceinline__ float largest(const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = two<T>(w[i]);
+    if (isfinite(f.x)) m = fmaxf(m, fabsf(f.x));
+    if (isfinite(f.y)) m = fmaxf(m, fabsf(f.y));
+  }
+  return m;
+}
+
+// T: the packed rows' type; E4M3: what the cache holds (the same type otherwise)
+template <typename T, bool E4M3>
+__global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteArgs a) {
+  __shared__ uint32_t bits[HASH_BITS / 32];
+  __shared__ long long own[MAX_TOKENS];      // the slot, or -1: not written
+  __shared__ int lost[MAX_TOKENS];           // a later token has the same slot
+  const long long t0 = (long long)blockIdx.x * a.per_block;
+  const int n = (int)min((long long)a.per_block, a.T - t0);
+  for (int i = threadIdx.x; i < HASH_BITS / 32; i += THREADS) bits[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    long long s = slot_of(a, t0 + i);
+    if (s >= a.total) {
+      if (a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
+      s = -1;
+    }
+    own[i] = s < 0 ? -1 : s;
+    lost[i] = 0;
+    if (s >= 0) atomicOr(&bits[(s & (HASH_BITS - 1)) >> 5], 1u << (s & 31));
+  }
+  __syncthreads();
+  for (long long t = t0 + 1 + threadIdx.x; t < a.T; t += THREADS) {
+    const long long s = slot_of(a, t);
+    if (s >= 0 && (bits[(s & (HASH_BITS - 1)) >> 5] >> (s & 31) & 1)) {
+      const int before = (int)min((long long)n, t - t0);
+      for (int i = 0; i < before; ++i)
+        if (own[i] == s) lost[i] = 1;
+    }
+  }
+  __syncthreads();
+
+  for (int w = 0; w < a.sides; ++w) {
+    const Side& d = a.side[w];
+    const int group = threadIdx.x / d.lanes, part = threadIdx.x % d.lanes, groups = THREADS / d.lanes;
+    const int rows = n * a.heads;
+    // whole rounds, so that the lanes of a warp meet in the shuffles
+    for (int r0 = 0; r0 < rows; r0 += groups * ROWS_AHEAD) {
+      uint4 v[ROWS_AHEAD];
+      int tok[ROWS_AHEAD], head[ROWS_AHEAD];
+#pragma unroll
+      for (int u = 0; u < ROWS_AHEAD; ++u) {
+        const int r = r0 + u * groups + group;
+        v[u] = make_uint4(0, 0, 0, 0);
+        tok[u] = r / a.heads;
+        head[u] = r - tok[u] * a.heads;
+        if (r >= rows || own[tok[u]] < 0 || lost[tok[u]]) tok[u] = -1;
+        else if (part < d.width)
+          v[u] = __ldg(reinterpret_cast<const uint4*>(d.x + (t0 + tok[u]) * d.x_tok + head[u] * d.x_head) + part);
+      }
+#pragma unroll
+      for (int u = 0; u < ROWS_AHEAD; ++u) {
+        float m = 0.f;
+        if (E4M3) {
+          m = largest<T>(v[u]);
+          for (int o = d.lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        }
+        if (tok[u] < 0) continue;
+        const long long s = own[tok[u]], page = s / a.page;
+        uint8_t* row = d.cache + page * d.c_page + (s - page * a.page) * d.c_tok + head[u] * d.c_head;
+        if (E4M3) {
+          const int e = exponent_byte(m);
+          // 2^(127 - e): a subnormal for e = 254 alone, which exponent_byte does not reach
+          if (part < d.width) reinterpret_cast<uint2*>(row)[part] = quantised<T>(v[u], __uint_as_float((254u - e) << 23));
+          if (part == 0) d.scale[s * a.heads + head[u]] = (uint8_t)e;
+        } else if (part < d.width) {
+          reinterpret_cast<uint4*>(row)[part] = v[u];
+        }
+      }
+    }
+  }
+}
+
+struct ReadArgs {
+  Side side[2];                              // x: the packed rows that are written
+  int sides;
+  const int* table;
+  long long table_row;                       // elements between the table's rows
+  const int* ends;                           // [sequences + 1]
+  int sequences, columns, pages;
+  int T, heads, page, per_block;
+  int* err;
+};
+
+template <typename T, bool E4M3>
+__device__ __forceinline__ uint4 expanded(const uint8_t* row, int part, float scale) {
+  if (!E4M3) return __ldg(reinterpret_cast<const uint4*>(row) + part);
+  const uint2 v = __ldg(reinterpret_cast<const uint2*>(row) + part);
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((i < 2 ? v.x : v.y) >> (16 * (i & 1))), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    o[i] = join<T>(f.x * scale, f.y * scale);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+template <typename T, bool E4M3>
+__global__ void __launch_bounds__(THREADS) cache_read_kernel(const ReadArgs a) {
+  __shared__ int where[MAX_TOKENS][2];       // page and place in it, or -1: a row of zeros
+  const long long t0 = (long long)blockIdx.x * a.per_block;
+  const int n = (int)min((long long)a.per_block, a.T - t0);
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const int t = (int)t0 + i;
+    int lo = 0, hi = a.sequences;            // the last sequence that begins at or before t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(a.ends + mid) <= t) lo = mid;
+      else hi = mid;
+    }
+    int page = -1, at = 0;
+    const int begin = a.sequences > 0 ? __ldg(a.ends + lo) : 0;
+    if (a.sequences > 0 && begin >= 0 && begin <= t && t < __ldg(a.ends + lo + 1)) {
+      const int pos = t - begin, col = pos / a.page;
+      at = pos - col * a.page;
+      page = col < a.columns ? __ldg(a.table + lo * a.table_row + col) : -1;
+      if (page < 0 || page >= a.pages) {
+        page = -1;
+        if (a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
+      }
+    }
+    where[i][0] = page;
+    where[i][1] = at;
+  }
+  __syncthreads();
+  for (int w = 0; w < a.sides; ++w) {
+    const Side& d = a.side[w];
+    const int group = threadIdx.x / d.lanes, part = threadIdx.x % d.lanes, groups = THREADS / d.lanes;
+    if (part >= d.width) continue;
+    const int rows = n * a.heads;
+    for (int r0 = group; r0 < rows; r0 += groups * ROWS_AHEAD) {
+      uint4 v[ROWS_AHEAD];
+#pragma unroll
+      for (int u = 0; u < ROWS_AHEAD; ++u) {
+        const int r = r0 + u * groups;
+        v[u] = make_uint4(0, 0, 0, 0);
+        if (r >= rows) continue;
+        const int tok = r / a.heads, head = r - tok * a.heads, page = where[tok][0], at = where[tok][1];
+        if (page < 0) continue;
+        const uint8_t* row = d.cache + page * d.c_page + at * d.c_tok + head * d.c_head;
+        float scale = 1.f;
+        if (E4M3) scale = power_of(__ldg(d.scale + ((long long)page * a.page + at) * a.heads + head));
+        v[u] = expanded<T, E4M3>(row, part, scale);
+      }
+#pragma unroll
+      for (int u = 0; u < ROWS_AHEAD; ++u) {
+        const int r = r0 + u * groups;
+        if (r >= rows) continue;
+        const int tok = r / a.heads, head = r - tok * a.heads;
+        reinterpret_cast<uint4*>(const_cast<uint8_t*>(d.x) + (t0 + tok) * d.x_tok + head * d.x_head)[part] = v[u];
+      }
+    }
+  }
+}
+
+// Tokens of one block: enough blocks for four on every SM, and then as many tokens as the block's tables hold
+static int tokens_per_block(int T) {
+  const int sms = sm_count() > 0 ? sm_count() : 1;
+  const int n = (T + 4 * sms - 1) / (4 * sms);
+  return n < 1 ? 1 : n > MAX_TOKENS ? MAX_TOKENS : n;
+}
+
+static Side side_of(const void* x, const long long* xs, void* cache, const long long* cs, void* scale, int width, int esize) {
+  Side d;
+  d.x = (const uint8_t*)x;
+  d.x_tok = xs[0] * 2;
+  d.x_head = xs[1] * 2;
+  d.cache = (uint8_t*)cache;
+  d.c_page = cs[0] * esize;
+  d.c_tok = cs[1] * esize;
+  d.c_head = cs[2] * esize;
+  d.scale = (uint8_t*)scale;
+  d.width = width / 8;
+  d.lanes = 1;
+  while (d.lanes < d.width) d.lanes *= 2;
+  return d;
+}
+
+template <typename A, typename Kern>
+static int start(Kern kern, A& a, cudaStream_t stream) {
+  a.per_block = tokens_per_block(a.T);
+  kern<<<(a.T + a.per_block - 1) / a.per_block, THREADS, 0, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+}  // namespace paged
+}  // namespace cm
+
+using namespace cm;
+using namespace cm::paged;
+
+// k [T, heads, dim] with strides ks (elements) of its first two axes, v likewise or null; caches [pages, page, heads, dim] with strides kcs, vcs
+// of their first three.  kind: 0 bf16, 1 fp16; e4m3: the caches hold E4M3 and k_scale, v_scale [pages, page, heads] their exponent bytes.  slots
+// [T] of 32 or (wide) 64 bits: place page * (slots of a page) + offset, negative: left out.  Widths are multiples of 8 up to 256, rows on 16
+// bytes (8 in an E4M3 cache).
+extern "C" int cm_cache_write(const void* k, const long long* ks, const void* v, const long long* vs, void* kc, const long long* kcs, void* vc,
+                              const long long* vcs, void* k_scale, void* v_scale, const void* slots, int wide, int T, int heads, int dim,
+                              int vdim, int pages, int page, int kind, int e4m3, int* err, cudaStream_t stream) {
+  if (T <= 0 || heads <= 0) return 0;
+  if (dim < 8 || dim % 8 || dim > 256 || (v && (vdim < 8 || vdim % 8 || vdim > 256)) || page < 1 || pages < 0) return -10;
+  if (e4m3 && (!k_scale || (v && !v_scale))) return -10;
+  WriteArgs a;
+  a.side[0] = side_of(k, ks, kc, kcs, k_scale, dim, e4m3 ? 1 : 2);
+  a.sides = 1;
+  if (v) a.side[a.sides++] = side_of(v, vs, vc, vcs, v_scale, vdim, e4m3 ? 1 : 2);
+  a.slots = slots;
+  a.wide = wide;
+  a.total = (long long)pages * page;
+  a.T = T;
+  a.heads = heads;
+  a.page = page;
+  a.err = err;
+  if (kind == 0) return e4m3 ? start(cache_write_kernel<__nv_bfloat16, true>, a, stream) : start(cache_write_kernel<__nv_bfloat16, false>, a, stream);
+  return e4m3 ? start(cache_write_kernel<__half, true>, a, stream) : start(cache_write_kernel<__half, false>, a, stream);
+}
+
+// The other way: token t of the packed results (strides ks, vs) is the (t - ends[s])-th of the sequence s that holds it; tokens of no sequence
+// become zeros.  table [sequences, columns] of page numbers, table_row elements from row to row.
+extern "C" int cm_cache_read(void* k, const long long* ks, void* v, const long long* vs, const void* kc, const long long* kcs, const void* vc,
+                             const long long* vcs, const void* k_scale, const void* v_scale, const int* table, long long table_row,
+                             const int* ends, int sequences, int columns, int T, int heads, int dim, int vdim, int pages, int page, int kind,
+                             int e4m3, int* err, cudaStream_t stream) {
+  if (T <= 0 || heads <= 0) return 0;
+  if (dim < 8 || dim % 8 || dim > 256 || (v && (vdim < 8 || vdim % 8 || vdim > 256)) || page < 1 || sequences < 0) return -10;
+  if (e4m3 && (!k_scale || (v && !v_scale))) return -10;
+  ReadArgs a;
+  a.side[0] = side_of(k, ks, const_cast<void*>(kc), kcs, const_cast<void*>(k_scale), dim, e4m3 ? 1 : 2);
+  a.sides = 1;
+  if (v) a.side[a.sides++] = side_of(v, vs, const_cast<void*>(vc), vcs, const_cast<void*>(v_scale), vdim, e4m3 ? 1 : 2);
+  a.table = table;
+  a.table_row = table_row;
+  a.ends = ends;
+  a.sequences = sequences;
+  a.columns = columns;
+  a.pages = pages;
+  a.T = T;
+  a.heads = heads;
+  a.page = page;
+  a.err = err;
+  if (kind == 0) return e4m3 ? start(cache_read_kernel<__nv_bfloat16, true>, a, stream) : start(cache_read_kernel<__nv_bfloat16, false>, a, stream);
+  return e4m3 ? start(cache_read_kernel<__half, true>, a, stream) : start(cache_read_kernel<__half, false>, a, stream);
+}

@@ -371,6 +371,148 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, counts: Sequence[int]) -> tor
 
 
 # ---------------------------------------------------------------------------
+# attention over packed sequences and over a paged key-value cache
+# ---------------------------------------------------------------------------
+
+def _ends(name: str, ends: torch.Tensor, total: int) -> list:
+    """The host's copy of ``cu_seqlens``: starts at zero, never falls, stays inside the ``total`` rows."""
+    out = ends.tolist()
+    if not out or out[0] != 0 or any(b < a for a, b in zip(out, out[1:])) or out[-1] > total:
+        raise ValueError(f"{name}: sequence ends {out} do not start at 0 and rise to at most {total}")
+    return out
+
+
+def _softmax_or_nothing(scores: torch.Tensor) -> torch.Tensor:
+    """Softmax over the last axis; a row of nothing but -inf (or of no keys at all) gives zeros."""
+    if scores.shape[-1] == 0:
+        return scores
+    top = scores.detach().amax(-1, keepdim=True)
+    e = torch.exp(scores - torch.where(top == -math.inf, torch.zeros_like(top), top))
+    total = e.sum(-1, keepdim=True)
+    return e / torch.where(total == 0, torch.ones_like(total), total)
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float,
+                     cu_seqlens_k: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention inside each sequence of a packed batch; the queries are the last positions of their keys."""
+    ends = _ends("packed_attention", cu_seqlens, q.shape[0])
+    ends_k = _ends("packed_attention", cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, k.shape[0])
+    group = q.shape[1] // k.shape[1] if k.shape[1] else 1
+    outs = []
+    for a, b, c, d in zip(ends, ends[1:], ends_k, ends_k[1:]):
+        qs = q[a:b].float().transpose(0, 1)
+        ks, vs = (t[c:d].float().repeat_interleave(group, 1).transpose(0, 1) for t in (k, v))
+        last = torch.arange(b - a, device=q.device)[:, None] + (d - c) - (b - a)
+        seen = torch.arange(d - c, device=q.device)[None, :] <= last
+        scores = torch.where(seen, qs @ ks.transpose(1, 2) * scale, -math.inf)
+        outs.append((_softmax_or_nothing(scores) @ vs).transpose(0, 1))
+    outs.append(q.new_zeros(q.shape[0] - ends[-1], q.shape[1], v.shape[2], dtype=torch.float32))
+    return torch.cat(outs).to(q.dtype)
+
+
+def cache_row_quantize(x: torch.Tensor):
+    """One power of two per row: ``(payload float8_e4m3fn, exponent byte uint8)`` with ``x ~ payload * 2^(byte - 127)``.  The exponent is the
+    smallest ``e`` with ``amax <= 448 * 2^e`` over the finite values; a row of zeros has byte 127, other values are NaN."""
+    xf = x.float()
+    finite = torch.isfinite(xf)
+    amax = torch.where(finite, xf.abs(), torch.zeros_like(xf)).amax(-1)
+    m, e = torch.frexp(amax)
+    e = torch.where(amax > 0, (e - 9 + (m > 0.875).int()).clamp(min=-126), torch.zeros_like(e))
+    inv = ((127 - e).to(torch.int32) << 23).view(torch.float32)            # 2^-e, e <= 120
+    y = torch.where(finite, (xf * inv[..., None]).clamp(-E4M3_MAX, E4M3_MAX), torch.full_like(xf, math.nan))
+    return y.to(torch.float8_e4m3fn), (e + 127).to(torch.uint8)
+
+
+def cache_power(byte: torch.Tensor) -> torch.Tensor:
+    """``2^(byte - 127)`` in fp32; 0 is 2^-127, 255 infinity."""
+    b = byte.to(torch.int32)
+    return torch.where(b == 0, torch.full_like(b, 0x00400000), b << 23).view(torch.float32)
+
+
+def _cache_rows(cache: torch.Tensor, scale: Optional[torch.Tensor], page: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
+    """fp32 rows ``cache[page, at]``; pages outside the cache give rows of zeros."""
+    there = (page >= 0) & (page < cache.shape[0])
+    page = torch.where(there, page, torch.zeros_like(page))
+    if cache.dtype == torch.float8_e4m3fn:
+        rows = cache.view(torch.uint8)[page, at].view(torch.float8_e4m3fn).float()
+    else:
+        rows = cache[page, at].float()
+    if scale is not None:
+        rows = rows * cache_power(scale[page, at])[..., None]
+    return torch.where(there[..., None, None], rows, torch.zeros_like(rows))
+
+
+def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> None:
+    """Rows into a paged cache, in place; of equal slots the last row stays, negative slots are left out."""
+    page = k_cache.shape[1]
+    total = k_cache.shape[0] * page
+    slots = slots.long()
+    if slots.numel() and int(slots.max()) >= total:
+        raise ValueError(f"cache_write: slot {int(slots.max())} of a cache of {total}")
+    index = torch.arange(slots.numel(), device=slots.device)
+    used = slots >= 0
+    owner = torch.full((total,), -1, dtype=torch.long, device=slots.device)
+    owner.scatter_reduce_(0, slots[used], index[used], "amax")
+    keep = index[used][owner[slots[used]] == index[used]]
+    where = slots[keep]
+    for x, cache, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+        if x is None:
+            continue
+        rows = x.detach()[keep]
+        if scale is None:
+            cache[where // page, where % page] = rows
+        else:
+            payload, byte = cache_row_quantize(rows)
+            cache.view(torch.uint8)[where // page, where % page] = payload.view(torch.uint8)
+            scale[where // page, where % page] = byte
+
+
+def cache_read(k_cache, v_cache, block_table, cu_seqlens, total: int, k_scale=None, v_scale=None, dtype=None):
+    """Packed rows ``(k, v)`` of the first tokens of each sequence; rows of no sequence are zeros."""
+    page = k_cache.shape[1]
+    ends = _ends("cache_read", cu_seqlens, total)
+    lens = [b - a for a, b in zip(ends, ends[1:])]
+    if lens and max(lens) > block_table.shape[1] * page:
+        raise ValueError(f"cache_read: {max(lens)} tokens, and {block_table.shape[1]} pages of {page}")
+    dev = k_cache.device
+    n = torch.tensor(lens, dtype=torch.long, device=dev)
+    seq = torch.repeat_interleave(torch.arange(len(lens), device=dev), n)
+    pos = torch.arange(ends[-1], device=dev) - cu_seqlens.long()[seq]
+    pages = block_table[seq, pos // page].long() if seq.numel() else seq
+    if seq.numel() and not bool(((pages >= 0) & (pages < k_cache.shape[0])).all()):
+        raise ValueError(f"cache_read: a page outside the cache's {k_cache.shape[0]}")
+    outs = []
+    for cache, scale in ((k_cache, k_scale), (v_cache, v_scale)):
+        if cache is None:
+            outs.append(None)
+            continue
+        out = torch.zeros(total, *cache.shape[2:], dtype=dtype or cache.dtype, device=dev)
+        out[:ends[-1]] = _cache_rows(cache, scale, pages, pos % page).to(out.dtype)
+        outs.append(out)
+    return tuple(outs)
+
+
+def paged_attention(q, k_cache, v_cache, block_table, seq_lens, scale: float, k_scale=None, v_scale=None) -> torch.Tensor:
+    """One query token per sequence over the first ``seq_lens`` rows of its pages; no rows give zeros."""
+    B, Hq, _ = q.shape
+    pages, page, Hk, _ = k_cache.shape
+    room = block_table.shape[1] * page
+    if q.device.type == "cpu":
+        if B and not (0 <= int(seq_lens.min()) and int(seq_lens.max()) <= room):
+            raise ValueError(f"paged_attention: lengths {seq_lens.tolist()} in {room} places")
+        used = torch.arange(room)[None, ::page] < seq_lens[:, None]
+        if bool((used & ((block_table < 0) | (block_table >= pages))).any()):
+            raise ValueError(f"paged_attention: a page outside the cache's {pages}")
+    pos = torch.arange(room, device=q.device)
+    table = block_table.long()[:, pos // page]
+    k, v = (_cache_rows(c, s, table, (pos % page).expand_as(table)).transpose(1, 2) for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
+    seen = ((pos < seq_lens[:, None]) & (table >= 0) & (table < pages))[:, None, :, None]
+    scores = q.float().view(B, Hk, Hq // Hk if Hk else 1, -1) @ torch.where(seen, k, torch.zeros_like(k)).transpose(2, 3) * scale
+    p = _softmax_or_nothing(torch.where(seen.transpose(2, 3), scores, -math.inf))
+    return (p @ torch.where(seen, v, torch.zeros_like(v))).reshape(B, Hq, v.shape[-1]).to(q.dtype)
+
+
+# ---------------------------------------------------------------------------
 # MXFP8 (E4M3 payload + E8M0 1x32 scales)
 # ---------------------------------------------------------------------------
 
