@@ -1,0 +1,1239 @@
+// Causal attention over sequences of different lengths packed into one buffer, with grouped heads; forward and backward on tcgen05 with the
+// scores in TMEM.
+//
+//   s[i, j] = scale * q[i] . k[j]   (j <= i + Lk - L inside the sequence)     p = softmax_j(s)     o[i] = sum_j p[i, j] v[j]
+//   delta[i] = do[i] . o[i]    ds = p (do v' - delta)    dq = scale ds k    dk = scale ds' q    dv = p' do
+//
+// Rows.  A query tile is 128 rows of (token, head of a group), so one tile of keys serves all heads of a group, a short sequence fills a
+// tile with its heads, the key gradients of a group add up inside one accumulator, and the tile of a causal diagonal is 128 / heads tokens
+// high.  Groups that do not divide 128 leave the last rows of a tile idle.  Tensor maps over [width, heads, tokens] read the rows where
+// they lie, whatever the strides, and give zeros behind a width that is no multiple of 64.
+//
+// Sequences.  A block finds its own tile: with f(p) = the number of tiles at place p or later of their sequences, block u works on the
+// place p with f(p + 1) <= u < f(p).  So the tiles with the longest loops of ALL sequences start first, and neither the host nor another kernel
+// lays out a plan.  The grid is the bound that the host knows (rows / tile + sequences); the blocks left over fill the rows behind the
+// last sequence with zeros.  Rows of a tile behind its sequence's end belong to somebody else: as rows of the result they are not
+// stored, as summed rows (V; K of dq; Q and dO of the key gradients) they are set to zero in shared memory, since a weight of zero does not
+// silence a NaN.
+//
+// Forward: one block per pair of query tiles.  A warp loads, one thread issues the products, a warpgroup per query tile (thread <-> row <->
+// TMEM lane) does the softmax: P goes back to TMEM as an operand, O stays there and is rescaled only when a row's maximum has grown by 2^8.
+// Backward: two kernels with seven products instead of one with five.  One kernel has a fixed set of columns too few (S, dP, dK, dV and dQ of 128
+// columns are 640 of 512) and adds dQ across blocks with atomics, in an order that changes from run to run; in two, P and dS of either
+// orientation are operands in TMEM that never pass through shared memory, every sum has one owner, and the bits are the same each time.
+//   dq     block per query tile, loops over key tiles:   S = Q K', dP = dO V', dQ += dS K
+//   dk dv  block per key tile, loops over query tiles:   S' = K Q', dP' = V dO', dV += P' dO, dK += dS' Q
+// The issuing thread polls what each product waits for and issues whichever is ready, so the products of one tile fill the pauses of
+// another; a product that overwrites columns is issued only after the commit of the one that reads them.
+// Query tiles of the key gradients run from the last one down: blocks of one sequence then read the same rows at the same time, out of L2.
+//
+// Roundings to 16 bits: P and dS, as operands of their products.  Maxima, sums, scores, deltas and all accumulators are fp32.  fp16's range
+// is too short for dS of any size: it is scaled by a power of two, from the row's largest |do| for dq, from the call's for dk.
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace cm {
+namespace packed {
+namespace {
+
+constexpr int TILE = 128;
+constexpr int SLAB = 128 * 128;              // bytes of one [128 rows x 64 columns] slab, 128-byte swizzle
+constexpr float RESCALE_AT = 8.f;            // log2
+
+// ---- products --------------------------------------------------------------------------------------------------------
+__host__ __device__ constexpr uint32_t idesc(bool half, int n, bool b_mn) {        // M 128, A K-major
+  return (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(TILE >> 4) << 24);
+}
+// 16-column step k of a K-major operand whose slabs lie one after the other
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int k) { return umma_desc_sw128(tile + (k >> 2) * SLAB + (k & 3) * 32, 16, 1024); }
+// 16-row step k of the same slabs read MN-major
+__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int k) { return umma_desc_sw128(tile + k * 2048, SLAB, 1024); }
+// A in TMEM (row = lane, two 16-bit values of K per column)
+__device__ __forceinline__ void umma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool HALF>
+__device__ __forceinline__ uint32_t pair(float lo, float hi) {
+  if (!HALF) return pack_bf16(lo, hi);
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <bool HALF>
+__device__ __forceinline__ float2 unpair(uint32_t v) {
+  if (!HALF) return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+__device__ __forceinline__ void tma_rows(void* dst, const CUtensorMap* map, uint64_t* bar, int col, int head, int row) {
+  tma_load_3d(dst, map, bar, col, head, row);
+}
+
+// ---- waits -----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ bool ready(uint64_t* bar, int parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
+}
+// Bounds a loop that polls: false once it has turned for too long without anything becoming ready, or another role has given up
+struct Patience {
+  unsigned long long since = 0;
+  uint32_t idle = 0;
+  __device__ __forceinline__ bool more(bool moved, volatile int* abort_flag, int* err) {
+    if (moved) { idle = 0; since = 0; return true; }
+    if ((++idle & 63u) != 0) return true;
+    if (*abort_flag) return false;
+    if (err && *reinterpret_cast<volatile int*>(err) != 0) { *abort_flag = 1; return false; }
+    const unsigned long long now = cm_globaltimer();
+    if (!since) { since = now; return true; }
+    if (now - since <= CM_WAIT_NS) return true;
+    *abort_flag = 1;
+    if (err) atomicCAS(err, 0, ERR_WAIT_TMEM_FULL);
+    return false;
+  }
+};
+
+// ---- sequences -------------------------------------------------------------------------------------------------------
+struct Args {
+  const int *cu_q, *cu_k;
+  int n, T, Tk;                              // sequences, rows of queries and of keys
+  int heads, kv_heads;
+  int hb, chunks, tok;                       // heads of a tile, tiles of heads in a group, tokens of a tile
+  int dim, vdim;
+  int units;                                 // blocks per (key head, chunk)
+  float scale, scale_log2;
+  void* out;                                 // forward: o [T, heads, vdim]; backward: dq [T, heads, dim] or dk [Tk, kv_heads, dim]
+  void* out2;                                // dv [Tk, kv_heads, vdim]
+  const void *o, *go;                        // backward, for delta: o and do with their strides
+  long long o_tok, o_head, go_tok, go_head;
+  float* lse;                                // [T, heads]: log2 of the sum of weights; +inf without keys; null: not wanted
+  float* delta;                              // [T, heads]
+  uint32_t* top;                             // largest |do| of the call as bits (fp16)
+  int* err;
+};
+
+struct Unit {
+  int seq, place, total;                     // total: tiles of all sequences
+  bool bad;
+};
+
+// Which tile is block u's?  One warp; `per` rows a tile of the sequences in cu.
+__device__ Unit find_unit(const Args& a, const int* cu, int per, int u, int lane) {
+  constexpr int KEPT = 4;
+  Unit r;
+  r.bad = lane == 0 && (__ldg(a.cu_q) != 0 || __ldg(a.cu_k) != 0);
+  int kept[KEPT], most = 0;
+  auto tiles = [&](int i) { return (__ldg(cu + i + 1) - __ldg(cu + i) + per - 1) / per; };
+  for (int i = lane; i < a.n; i += 32) {
+    const int q0 = __ldg(a.cu_q + i), q1 = __ldg(a.cu_q + i + 1), k0 = __ldg(a.cu_k + i), k1 = __ldg(a.cu_k + i + 1);
+    r.bad |= q0 < 0 || q1 < q0 || q1 > a.T || k0 < 0 || k1 < k0 || k1 > a.Tk;
+  }
+  r.bad = __any_sync(0xffffffffu, r.bad);
+  r.seq = r.place = r.total = 0;
+  if (r.bad) return r;
+#pragma unroll
+  for (int c = 0; c < KEPT; ++c) kept[c] = c * 32 + lane < a.n ? tiles(c * 32 + lane) : 0;
+  auto after = [&](int p) {                  // tiles at place p or later
+    int s = 0;
+#pragma unroll
+    for (int c = 0; c < KEPT; ++c) s += max(0, kept[c] - p);
+    for (int i = KEPT * 32 + lane; i < a.n; i += 32) s += max(0, tiles(i) - p);
+    return __reduce_add_sync(0xffffffffu, s);
+  };
+#pragma unroll
+  for (int c = 0; c < KEPT; ++c) most = max(most, kept[c]);
+  for (int i = KEPT * 32 + lane; i < a.n; i += 32) most = max(most, tiles(i));
+  most = __reduce_max_sync(0xffffffffu, most);
+  r.total = after(0);
+  if (u >= r.total) return r;
+  int lo = 0, hi = most;                     // after(lo) > u >= after(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (after(mid) > u) lo = mid;
+    else hi = mid;
+  }
+  r.place = lo;
+  int rank = u - after(lo + 1);
+  for (int c = 0, i0 = 0; i0 < a.n; i0 += 32, ++c) {
+    int t = 0;
+    if (c == 0) t = kept[0];
+    else if (c == 1) t = kept[1];
+    else if (c == 2) t = kept[2];
+    else if (c == 3) t = kept[3];
+    else if (i0 + lane < a.n) t = tiles(i0 + lane);
+    const unsigned has = __ballot_sync(0xffffffffu, t > lo);
+    if (rank < __popc(has)) {
+      r.seq = i0 + __fns(has, 0, rank + 1);
+      break;
+    }
+    rank -= __popc(has);
+  }
+  return r;
+}
+
+// The blocks left over: zeros into the rows [begin, rows) of a [rows, heads, width] result, columns of `heads` heads from head0 on
+__device__ void clear_rows(void* out, int begin, int rows, int all_heads, int head0, int heads, int width, int part, int parts) {
+  const int pieces = heads * width / 8;
+  for (long long r = begin + part; r < rows; r += parts) {
+    uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + (r * all_heads + head0) * width);
+    for (int i = threadIdx.x; i < pieces; i += blockDim.x) dst[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// rows [from, 128) of `slabs` slabs set to zero by one warp
+__device__ __forceinline__ void clear_tail(uint8_t* tile, int slabs, int from, int lane) {
+  for (int s = 0; s < slabs; ++s)
+    for (int i = from * 8 + lane; i < TILE * 8; i += 32) reinterpret_cast<uint4*>(tile + s * SLAB)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// copies in flight land before the shared memory is released
+__device__ __forceinline__ void settle(volatile int* abort_flag) {
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+    __syncthreads();
+  }
+}
+
+// 32 accumulator columns times f as 16-bit values to a row (16-byte stores; `left` columns exist)
+template <bool HALF>
+__device__ __forceinline__ void store_columns(uint16_t* row, const uint32_t (&x)[32], float f, int left) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint4 o;
+    o.x = pair<HALF>(__uint_as_float(x[q * 8]) * f, __uint_as_float(x[q * 8 + 1]) * f);
+    o.y = pair<HALF>(__uint_as_float(x[q * 8 + 2]) * f, __uint_as_float(x[q * 8 + 3]) * f);
+    o.z = pair<HALF>(__uint_as_float(x[q * 8 + 4]) * f, __uint_as_float(x[q * 8 + 5]) * f);
+    o.w = pair<HALF>(__uint_as_float(x[q * 8 + 6]) * f, __uint_as_float(x[q * 8 + 7]) * f);
+    if (q * 8 < left) reinterpret_cast<uint4*>(row)[q] = o;
+  }
+}
+
+struct Masked { static constexpr bool value = true; };
+struct Whole { static constexpr bool value = false; };
+
+// ---- forward ---------------------------------------------------------------------------------------------------------
+constexpr int THREADS = 320;                 // eight compute warps, one that issues products, one that loads
+constexpr int MMA_WARP = 8, TMA_WARP = 9;
+
+template <int D, int DV>
+struct Fwd {
+  static constexpr int KS = D / 64, VS = DV / 64;
+  static constexpr int K_SLOTS = 3, V_SLOTS = DV == 128 ? 2 : 3;
+  static constexpr bool P_OVER_S = DV == 128;                 // no columns left for P: it takes the place of the scores it came from
+  struct Shared {
+    uint64_t q_full[2], k_full[K_SLOTS], k_empty[K_SLOTS], v_full[V_SLOTS], v_empty[V_SLOTS], tail;
+    uint64_t s_full[2], s_free[2], p_full[2], o_done[2];
+    Unit unit;
+    uint32_t tmem_slot;
+    int abort_flag;
+  };
+  static constexpr int SMEM = (2 * KS + K_SLOTS * KS + V_SLOTS * VS) * SLAB + (int)sizeof(Shared) + 1024;
+};
+
+template <bool HALF, int D, int DV>
+__global__ void __launch_bounds__(THREADS, 1)
+packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const Args a) {
+  using F = Fwd<D, DV>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + 2 * F::KS * SLAB;
+  uint8_t* sV = sK + F::K_SLOTS * F::KS * SLAB;
+  auto* sh = reinterpret_cast<typename F::Shared*>(sV + F::V_SLOTS * F::VS * SLAB);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hh = a.kv_heads * a.chunks, u = blockIdx.x / hh, kvh = (blockIdx.x % hh) / a.chunks, chunk = blockIdx.x % a.chunks;
+  const int head0 = kvh * (a.heads / a.kv_heads) + chunk * a.hb;
+  volatile int* abort_flag = &sh->abort_flag;
+  if (warp == 0) {
+    const Unit r = find_unit(a, a.cu_q, 2 * a.tok, u, lane);
+    if (lane == 0) sh->unit = r;
+  }
+  if (tid == 32) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sh->q_full[t], 1);
+      mbar_init(&sh->s_full[t], 1);
+      mbar_init(&sh->s_free[t], 4);
+      mbar_init(&sh->p_full[t], 4);
+      mbar_init(&sh->o_done[t], 1);
+    }
+    for (int s = 0; s < F::K_SLOTS; ++s) { mbar_init(&sh->k_full[s], 1); mbar_init(&sh->k_empty[s], 1); }
+    for (int s = 0; s < F::V_SLOTS; ++s) { mbar_init(&sh->v_full[s], 1); mbar_init(&sh->v_empty[s], 1); }
+    mbar_init(&sh->tail, 1);
+    sh->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == MMA_WARP) { tmem_alloc(&sh->tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  const bool drain = setup_barrier(a.err);
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem_slot;       // S_t at 128 t, O_t at 256 + DV t, P_t over S_t or at 384 + 64 t
+  const Unit unit = sh->unit;
+  if (drain || unit.bad || u >= unit.total) {
+    if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
+    if (drain) return;
+    if (unit.bad) {
+      if (tid == 0 && a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
+      return;
+    }
+    clear_rows(a.out, __ldg(a.cu_q + a.n), a.T, a.heads, head0, a.hb, a.vdim, u - unit.total, a.units - unit.total);
+    return;
+  }
+  const int q0 = __ldg(a.cu_q + unit.seq), L = __ldg(a.cu_q + unit.seq + 1) - q0;
+  const int k0 = __ldg(a.cu_k + unit.seq), Lk = __ldg(a.cu_k + unit.seq + 1) - k0;
+  const int off = Lk - L;                    // query i sees the keys up to i + off
+  const int rows = a.hb * a.tok;
+  // key tiles of query tile t, and the first of them that the mask cuts
+  int n[2], whole[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int first = (2 * unit.place + t) * a.tok, last = min(L, first + a.tok) - 1;
+    n[t] = first < L && off + last >= 0 ? (off + last) / TILE + 1 : 0;
+    whole[t] = off + first + 1 > 0 ? (off + first + 1) / TILE : 0;
+  }
+  const int most = max(n[0], n[1]);
+
+  if (warp == TMA_WARP) {
+    // ------------------------------ loads ------------------------------
+    bool ok = true;
+    auto load_q = [&](int t) {
+      if (n[t] == 0 || lane != 0) return;
+      mbar_expect_tx(&sh->q_full[t], F::KS * rows * 128);
+      for (int s = 0; s < F::KS; ++s)
+        tma_rows(sQ + (t * F::KS + s) * SLAB, &tmQ, &sh->q_full[t], s * 64, head0, q0 + (2 * unit.place + t) * a.tok);
+    };
+    load_q(0);
+    for (int j = 0; j < most && ok; ++j) {
+      const int ks = j % F::K_SLOTS, vs = j % F::V_SLOTS;
+      ok = warp_wait(&sh->k_empty[ks], ((j / F::K_SLOTS) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(&sh->k_full[ks], F::KS * SLAB);
+        for (int s = 0; s < F::KS; ++s) tma_rows(sK + (ks * F::KS + s) * SLAB, &tmK, &sh->k_full[ks], s * 64, kvh, k0 + j * TILE);
+      }
+      if (j == 0) load_q(1);
+      ok = warp_wait(&sh->v_empty[vs], ((j / F::V_SLOTS) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY);
+      if (!ok) break;
+      const bool cut = (j + 1) * TILE > Lk;                   // the sequence's last tile: the rows behind its end are set to zero
+      uint64_t* bar = cut ? &sh->tail : &sh->v_full[vs];
+      if (lane == 0) {
+        mbar_expect_tx(bar, F::VS * SLAB);
+        for (int s = 0; s < F::VS; ++s) tma_rows(sV + (vs * F::VS + s) * SLAB, &tmV, bar, s * 64, kvh, k0 + j * TILE);
+      }
+      if (cut) {
+        ok = warp_wait(bar, 0, abort_flag, a.err, ERR_WAIT_FULL);
+        if (!ok) break;
+        clear_tail(sV + vs * F::VS * SLAB, F::VS, Lk - j * TILE, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->v_full[vs]);
+      }
+    }
+  } else if (warp == MMA_WARP) {
+    // ------------------------------ products ------------------------------
+    if (elect_one()) {
+      constexpr uint32_t id_s = idesc(HALF, TILE, false), id_o = idesc(HALF, DV, true);
+      int s_next[2] = {0, 0}, p_next[2] = {0, 0}, k_freed = 0, v_freed = 0;
+      Patience patience;
+      bool moved = true;
+      while ((p_next[0] < n[0] || p_next[1] < n[1]) && patience.more(moved, abort_flag, a.err)) {
+        moved = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int i = p_next[t], vs = i % F::V_SLOTS;
+          if (i < s_next[t] && ready(&sh->p_full[t], i & 1) && ready(&sh->v_full[vs], (i / F::V_SLOTS) & 1)) {
+            tc_fence_after();
+            const uint32_t aV = smem_u32(sV + vs * F::VS * SLAB), tP = F::P_OVER_S ? tmem + t * 128 : tmem + 384 + t * 64;
+#pragma unroll
+            for (int k = 0; k < TILE / 16; ++k) umma_ta(tmem + 256 + t * DV, tP + k * 8, desc_mn(aV, k), id_o, (i | k) != 0);
+            umma_commit(&sh->o_done[t]);
+            ++p_next[t];
+            if ((p_next[0] > v_freed || v_freed >= n[0]) && (p_next[1] > v_freed || v_freed >= n[1])) {
+              umma_commit(&sh->v_empty[v_freed % F::V_SLOTS]);
+              ++v_freed;
+            }
+            moved = true;
+          }
+          const int j = s_next[t], ks = j % F::K_SLOTS;
+          if (j < n[t] && ready(&sh->k_full[ks], (j / F::K_SLOTS) & 1) &&
+              (j == 0 ? ready(&sh->q_full[t], 0) : ready(F::P_OVER_S ? &sh->o_done[t] : &sh->s_free[t], (j - 1) & 1))) {
+            tc_fence_after();
+            const uint32_t aQ = smem_u32(sQ + t * F::KS * SLAB), aK = smem_u32(sK + ks * F::KS * SLAB);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) umma_f16(tmem + t * 128, desc_k(aQ, k), desc_k(aK, k), id_s, k != 0);
+            umma_commit(&sh->s_full[t]);
+            ++s_next[t];
+            if ((s_next[0] > k_freed || k_freed >= n[0]) && (s_next[1] > k_freed || k_freed >= n[1])) {
+              umma_commit(&sh->k_empty[k_freed % F::K_SLOTS]);
+              ++k_freed;
+            }
+            moved = true;
+          }
+        }
+      }
+    }
+  } else {
+    // ------------------------------ softmax of query tile t ------------------------------
+    const int t = warp >> 2, r = tid & 127, tok = r / a.hb, qt = 2 * unit.place + t;
+    const int pos = qt * a.tok + tok;                         // position of this row's query
+    const bool mine = r < rows && pos < L;
+    const int last = mine ? off + pos : -1;                   // last key it sees
+    const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + t * 128 + lane_addr, tO = tmem + 256 + t * DV + lane_addr;
+    const uint32_t tP = F::P_OVER_S ? tS : tmem + 384 + t * 64 + lane_addr;
+    float m_ref = -INFINITY, l = 0.f;
+    auto tile = [&](int j, auto where) {
+      constexpr bool MASK = decltype(where)::value;
+      const int lim = last - j * TILE;                        // columns up to lim are seen
+      bool ok = warp_wait(&sh->s_full[t], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
+      if (!ok) return false;
+      tc_fence_after();
+      // first pass over the row: its maximum.  The first half of the row is read last and kept for the second pass.
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      uint32_t s0[32], s1[32], s2[32];
+#pragma unroll
+      for (int c = 1; c >= 0; --c) {
+        tmem_ld_32x32(tS + c * 64, s0);
+        tmem_ld_32x32(tS + c * 64 + 32, s1);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          if (!MASK || c * 64 + e <= lim) top[e & 1] = fmaxf(top[e & 1], __uint_as_float(s0[e]));
+          if (!MASK || c * 64 + 32 + e <= lim) top[2 + (e & 1)] = fmaxf(top[2 + (e & 1)], __uint_as_float(s1[e]));
+        }
+      }
+      float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if (m_new != -INFINITY) m_new *= a.scale_log2;          // a scale of zero leaves "nothing seen" as it is
+      float alpha = 1.f;
+      if (m_new > m_ref + RESCALE_AT) {                       // also from -inf
+        alpha = ex2(m_ref - m_new);
+        m_ref = m_new;
+        l *= alpha;
+      }
+      if (j > 0) {
+        if (!F::P_OVER_S) {                                   // P_t and O_t are free (P over S: S_t was issued after O_t was done)
+          ok = warp_wait(&sh->o_done[t], (j - 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
+          if (!ok) return false;
+          tc_fence_after();
+        }
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+          for (int c = 0; c < DV / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(tO + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st(tO + c * 32, o);
+          }
+        }
+      }
+      const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // nothing seen so far
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t p[32];
+      auto quarter = [&](const uint32_t (&sc)[32], int col0, int at) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float x = ex2(fmaf(__uint_as_float(sc[2 * e]), a.scale_log2, -ref));
+          float y = ex2(fmaf(__uint_as_float(sc[2 * e + 1]), a.scale_log2, -ref));
+          if (MASK) {
+            x = col0 + 2 * e <= lim ? x : 0.f;
+            y = col0 + 2 * e + 1 <= lim ? y : 0.f;
+          }
+          sum[(2 * e) & 3] += x;
+          sum[(2 * e + 1) & 3] += y;
+          p[at + e] = pair<HALF>(x, y);
+        }
+      };
+      quarter(s0, 0, 0);
+      quarter(s1, 32, 16);
+      tmem_st(tP, p);
+      tmem_ld_32x32(tS + 64, s2);
+      tmem_ld_32x32(tS + 96, s1);
+      tmem_ld_wait();
+      if (!F::P_OVER_S) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->s_free[t]);
+      }
+      quarter(s2, 64, 0);
+      quarter(s1, 96, 16);
+      tmem_st(tP + 32, p);
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->p_full[t]);
+      return true;
+    };
+    const int count = t ? n[1] : n[0], open = t ? whole[1] : whole[0];
+    bool ok = true;
+    for (int j = 0; j < min(count, open) && ok; ++j) ok = tile(j, Whole{});
+    for (int j = min(count, open); j < count && ok; ++j) ok = tile(j, Masked{});
+    if (ok && count > 0) ok = warp_wait(&sh->o_done[t], (count - 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
+    if (ok) {
+      tc_fence_after();
+      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;               // a NaN stays
+      const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
+      uint16_t* row = reinterpret_cast<uint16_t*>(a.out) + at * a.vdim;
+#pragma unroll
+      for (int c = 0; c < DV / 32; ++c) {
+        uint32_t o[32];
+        if (count > 0) {
+          tmem_ld_32x32(tO + c * 32, o);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = last >= 0 ? o[e] : 0u;            // a row without keys
+        if (mine) store_columns<HALF>(row + c * 32, o, last >= 0 ? inv : 0.f, a.vdim - c * 32);
+      }
+      if (mine && a.lse) a.lse[at] = l == 0.f ? INFINITY : m_ref + log2f(l);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  settle(abort_flag);
+  if (warp == MMA_WARP) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// ---- backward: query gradients, and delta ------------------------------------------------------------------------------
+template <int D, int DV>
+struct Dq {
+  static constexpr int KS = D / 64, VS = DV / 64, K_SLOTS = 3, V_SLOTS = 2;
+  struct Shared {
+    uint64_t q_full, k_full[K_SLOTS], k_empty[K_SLOTS], v_full[V_SLOTS], v_empty[V_SLOTS], tail;
+    uint64_t s_full[2], dp_full, dp_free, ds_full[2], dq_done[2], acc_done;
+    Unit unit;
+    uint32_t tmem_slot;
+    int abort_flag;
+  };
+  static constexpr int SMEM = (KS + VS + K_SLOTS * KS + V_SLOTS * VS) * SLAB + (int)sizeof(Shared) + 1024;
+};
+
+template <bool HALF, int D, int DV>
+__global__ void __launch_bounds__(THREADS, 1)
+packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const __grid_constant__ CUtensorMap tmG, const Args a) {
+  using F = Dq<D, DV>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sG = sQ + F::KS * SLAB;
+  uint8_t* sK = sG + F::VS * SLAB;
+  uint8_t* sV = sK + F::K_SLOTS * F::KS * SLAB;
+  auto* sh = reinterpret_cast<typename F::Shared*>(sV + F::V_SLOTS * F::VS * SLAB);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hh = a.kv_heads * a.chunks, u = blockIdx.x / hh, kvh = (blockIdx.x % hh) / a.chunks, chunk = blockIdx.x % a.chunks;
+  const int head0 = kvh * (a.heads / a.kv_heads) + chunk * a.hb;
+  volatile int* abort_flag = &sh->abort_flag;
+  if (warp == 0) {
+    const Unit r = find_unit(a, a.cu_q, a.tok, u, lane);
+    if (lane == 0) sh->unit = r;
+  }
+  if (tid == 32) {
+    mbar_init(&sh->q_full, 1);
+    for (int s = 0; s < F::K_SLOTS; ++s) { mbar_init(&sh->k_full[s], 1); mbar_init(&sh->k_empty[s], 1); }
+    for (int s = 0; s < F::V_SLOTS; ++s) { mbar_init(&sh->v_full[s], 1); mbar_init(&sh->v_empty[s], 1); }
+    mbar_init(&sh->tail, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sh->s_full[b], 1);
+      mbar_init(&sh->ds_full[b], 8);
+      mbar_init(&sh->dq_done[b], 1);
+    }
+    mbar_init(&sh->dp_full, 1);
+    mbar_init(&sh->dp_free, 8);
+    mbar_init(&sh->acc_done, 1);
+    sh->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == MMA_WARP) { tmem_alloc(&sh->tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before();
+  const bool drain = setup_barrier(a.err);
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem_slot;       // S of even and odd key tiles at 0 and 128 (dS over them), dP at 256, dQ at 384
+  const Unit unit = sh->unit;
+  if (drain || unit.bad || u >= unit.total) {
+    if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
+    if (drain) return;
+    if (unit.bad) {
+      if (tid == 0 && a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
+      return;
+    }
+    clear_rows(a.out, __ldg(a.cu_q + a.n), a.T, a.heads, head0, a.hb, a.dim, u - unit.total, a.units - unit.total);
+    return;
+  }
+  const int q0 = __ldg(a.cu_q + unit.seq), L = __ldg(a.cu_q + unit.seq + 1) - q0;
+  const int k0 = __ldg(a.cu_k + unit.seq), Lk = __ldg(a.cu_k + unit.seq + 1) - k0;
+  const int off = Lk - L, rows = a.hb * a.tok, first = unit.place * a.tok, end = min(L, first + a.tok);
+  const int n = off + end - 1 >= 0 ? (off + end - 1) / TILE + 1 : 0;
+  const int open = off + first + 1 > 0 ? min(n, (off + first + 1) / TILE) : 0;
+
+  if (warp == TMA_WARP) {
+    bool ok = true;
+    if (n > 0 && lane == 0) {
+      mbar_expect_tx(&sh->q_full, (F::KS + F::VS) * rows * 128);
+      for (int s = 0; s < F::KS; ++s) tma_rows(sQ + s * SLAB, &tmQ, &sh->q_full, s * 64, head0, q0 + first);
+      for (int s = 0; s < F::VS; ++s) tma_rows(sG + s * SLAB, &tmG, &sh->q_full, s * 64, head0, q0 + first);
+    }
+    for (int j = 0; j < n && ok; ++j) {
+      const int ks = j % F::K_SLOTS, vs = j % F::V_SLOTS;
+      ok = warp_wait(&sh->k_empty[ks], ((j / F::K_SLOTS) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY);
+      if (!ok) break;
+      const bool cut = (j + 1) * TILE > Lk;                   // K is summed over its rows: those behind the sequence's end become zero
+      uint64_t* bar = cut ? &sh->tail : &sh->k_full[ks];
+      if (lane == 0) {
+        mbar_expect_tx(bar, F::KS * SLAB);
+        for (int s = 0; s < F::KS; ++s) tma_rows(sK + (ks * F::KS + s) * SLAB, &tmK, bar, s * 64, kvh, k0 + j * TILE);
+      }
+      if (cut) {
+        ok = warp_wait(bar, 0, abort_flag, a.err, ERR_WAIT_FULL);
+        if (!ok) break;
+        clear_tail(sK + ks * F::KS * SLAB, F::KS, Lk - j * TILE, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->k_full[ks]);
+      }
+      ok = warp_wait(&sh->v_empty[vs], ((j / F::V_SLOTS) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(&sh->v_full[vs], F::VS * SLAB);
+        for (int s = 0; s < F::VS; ++s) tma_rows(sV + (vs * F::VS + s) * SLAB, &tmV, &sh->v_full[vs], s * 64, kvh, k0 + j * TILE);
+      }
+    }
+  } else if (warp == MMA_WARP) {
+    if (elect_one()) {
+      constexpr uint32_t id_s = idesc(HALF, TILE, false), id_q = idesc(HALF, D, true);
+      const uint32_t aQ = smem_u32(sQ), aG = smem_u32(sG);
+      int is = 0, ip = 0, iq = 0;
+      bool there = false;
+      Patience patience;
+      bool moved = true;
+      while (iq < n && patience.more(moved, abort_flag, a.err)) {
+        moved = false;
+        if (!there) {
+          there = moved = ready(&sh->q_full, 0);
+          continue;
+        }
+        if (is < n && ready(&sh->k_full[is % F::K_SLOTS], (is / F::K_SLOTS) & 1) &&
+            (is < 2 || ready(&sh->dq_done[is & 1], ((is >> 1) - 1) & 1))) {
+          tc_fence_after();
+          const uint32_t aK = smem_u32(sK + (is % F::K_SLOTS) * F::KS * SLAB);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) umma_f16(tmem + (is & 1) * 128, desc_k(aQ, k), desc_k(aK, k), id_s, k != 0);
+          umma_commit(&sh->s_full[is & 1]);
+          ++is;
+          moved = true;
+        }
+        if (ip < n && ready(&sh->v_full[ip % F::V_SLOTS], (ip / F::V_SLOTS) & 1) && (ip == 0 || ready(&sh->dp_free, (ip - 1) & 1))) {
+          tc_fence_after();
+          const uint32_t aV = smem_u32(sV + (ip % F::V_SLOTS) * F::VS * SLAB);
+#pragma unroll
+          for (int k = 0; k < DV / 16; ++k) umma_f16(tmem + 256, desc_k(aG, k), desc_k(aV, k), id_s, k != 0);
+          umma_commit(&sh->dp_full);
+          umma_commit(&sh->v_empty[ip % F::V_SLOTS]);
+          ++ip;
+          moved = true;
+        }
+        if (iq < is && ready(&sh->ds_full[iq & 1], (iq >> 1) & 1)) {
+          tc_fence_after();
+          const uint32_t aK = smem_u32(sK + (iq % F::K_SLOTS) * F::KS * SLAB), tdS = tmem + (iq & 1) * 128;
+#pragma unroll
+          for (int k = 0; k < TILE / 16; ++k)                 // the halves of dS lie over the halves of S that they came from
+            umma_ta(tmem + 384, tdS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(aK, k), id_q, (iq | k) != 0);
+          umma_commit(&sh->dq_done[iq & 1]);
+          umma_commit(&sh->k_empty[iq % F::K_SLOTS]);
+          ++iq;
+          moved = true;
+        }
+      }
+      if (n > 0 && iq == n) umma_commit(&sh->acc_done);
+    }
+  } else {
+    const int half = warp >> 2, r = tid & 127, tok = r / a.hb, pos = first + tok;
+    const bool mine = r < rows && pos < L;
+    const int last = mine ? off + pos : -1, head = head0 + (r - tok * a.hb);
+    const long long at = (long long)(q0 + pos) * a.heads + head;
+    // delta, and the power of two that brings the row's largest |do| to 2^-4; both threads of a row add it up whole
+    float delta = 0.f, big = 0.f;
+    if (mine) {
+      const uint4* ov = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o) + (q0 + pos) * a.o_tok + head * a.o_head);
+      const uint4* gv = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.go) + (q0 + pos) * a.go_tok + head * a.go_head);
+#pragma unroll
+      for (int c = 0; c < DV / 8; ++c) {
+        if (c * 8 >= a.vdim) break;
+        const uint4 x = __ldg(ov + c), y = __ldg(gv + c);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpair<HALF>(xs[e]), g = unpair<HALF>(ys[e]);
+          delta = fmaf(f.x, g.x, fmaf(f.y, g.y, delta));
+          if (HALF) big = fmaxf(big, fmaxf(fabsf(g.x), fabsf(g.y)));
+        }
+      }
+    }
+    float up = 1.f, down = 1.f;
+    if (HALF) {
+      if (big > 0.f && isfinite(big)) {
+        const int e = 127 - 4 - int(__float_as_uint(big) >> 23);
+        up = __uint_as_float(uint32_t(127 + e) << 23);
+        down = __uint_as_float(uint32_t(127 - e) << 23);
+      }
+      if (half == 0) {
+        const uint32_t all = __reduce_max_sync(0xffffffffu, mine && isfinite(big) ? __float_as_uint(big) : 0u);
+        if (lane == 0 && all) atomicMax(a.top, all);
+      }
+    }
+    const float lse = mine ? a.lse[at] : INFINITY;
+    if (mine && half == 0) a.delta[at] = delta;
+    const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
+    const float delta_up = delta * up;
+    auto tile = [&](int j, auto where) {
+      constexpr bool MASK = decltype(where)::value;
+      const int lim = last - j * TILE - half * 64;
+      const uint32_t tS = tmem + (j & 1) * 128 + half * 64 + lane_addr, tdP = tmem + 256 + half * 64 + lane_addr;
+      if (!warp_wait(&sh->s_full[j & 1], (j >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
+      tc_fence_after();
+      float p[64];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32];
+        tmem_ld_32x32(tS + c * 32, s);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float x = ex2(fmaf(__uint_as_float(s[e]), a.scale_log2, -lse));
+          p[c * 32 + e] = !MASK || c * 32 + e <= lim ? x : 0.f;
+        }
+      }
+      if (!warp_wait(&sh->dp_full, j & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
+      tc_fence_after();
+      uint32_t ds[32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t d[32];
+        tmem_ld_32x32(tdP + c * 32, d);
+        tmem_ld_wait();
+        if (c == 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->dp_free);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int i = c * 32 + 2 * e;
+          float x = p[i] * (HALF ? fmaf(__uint_as_float(d[2 * e]), up, -delta_up) : __uint_as_float(d[2 * e]) - delta);
+          float y = p[i + 1] * (HALF ? fmaf(__uint_as_float(d[2 * e + 1]), up, -delta_up) : __uint_as_float(d[2 * e + 1]) - delta);
+          if (MASK) {                                         // what is not seen may be anything, a NaN too
+            x = i <= lim ? x : 0.f;
+            y = i + 1 <= lim ? y : 0.f;
+          }
+          ds[c * 16 + e] = pair<HALF>(x, y);
+        }
+      }
+      tmem_st(tS, ds);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->ds_full[j & 1]);
+      return true;
+    };
+    bool ok = true;
+    for (int j = 0; j < open && ok; ++j) ok = tile(j, Whole{});
+    for (int j = open; j < n && ok; ++j) ok = tile(j, Masked{});
+    if (ok && n > 0) ok = warp_wait(&sh->acc_done, 0, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
+    if (ok) {
+      tc_fence_after();
+      uint16_t* row = reinterpret_cast<uint16_t*>(a.out) + at * a.dim;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        const int col = half * (D / 2) + c * 32;
+        uint32_t x[32];
+        if (n > 0) {
+          tmem_ld_32x32(tmem + 384 + col + lane_addr, x);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = last >= 0 ? x[e] : 0u;
+        if (mine) store_columns<HALF>(row + col, x, last >= 0 ? a.scale * down : 0.f, a.dim - col);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  settle(abort_flag);
+  if (warp == MMA_WARP) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// ---- backward: key and value gradients ---------------------------------------------------------------------------------
+template <int D, int DV>
+struct Dkv {
+  static constexpr int KS = D / 64, VS = DV / 64, STAGES = 2;
+  struct Shared {
+    uint64_t kv_full, q_full[STAGES], stat_full[STAGES], q_empty[STAGES], tail;
+    uint64_t s_full, dp_full, p_full, ds_full, dv_done, dk_done, acc_done;
+    Unit unit;
+    uint32_t tmem_slot;
+    int abort_flag;
+    float lse[STAGES][TILE], delta[STAGES][TILE];
+  };
+  static constexpr int SMEM = (1 + STAGES) * (KS + VS) * SLAB + (int)sizeof(Shared) + 1024;
+};
+
+template <bool HALF, int D, int DV>
+__global__ void __launch_bounds__(THREADS, 1)
+packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ CUtensorMap tmG, const Args a) {
+  using F = Dkv<D, DV>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = sK + F::KS * SLAB;
+  uint8_t* sQ = sV + F::VS * SLAB;           // stages of Q, then dO
+  constexpr int STAGE = (F::KS + F::VS) * SLAB;
+  auto* sh = reinterpret_cast<typename F::Shared*>(sQ + F::STAGES * STAGE);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int u = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads, group0 = kvh * (a.heads / a.kv_heads);
+  const int rows = a.hb * a.tok;
+  volatile int* abort_flag = &sh->abort_flag;
+  if (warp == 0) {
+    const Unit r = find_unit(a, a.cu_k, TILE, u, lane);
+    if (lane == 0) sh->unit = r;
+  }
+  if (tid == 32) {
+    mbar_init(&sh->kv_full, 1);
+    for (int s = 0; s < F::STAGES; ++s) {
+      mbar_init(&sh->q_full[s], 1);
+      mbar_init(&sh->stat_full[s], 1);
+      mbar_init(&sh->q_empty[s], 1);
+    }
+    mbar_init(&sh->tail, 1);
+    mbar_init(&sh->s_full, 1);
+    mbar_init(&sh->dp_full, 1);
+    mbar_init(&sh->p_full, 8);
+    mbar_init(&sh->ds_full, 8);
+    mbar_init(&sh->dv_done, 1);
+    mbar_init(&sh->dk_done, 1);
+    mbar_init(&sh->acc_done, 1);
+    sh->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == MMA_WARP) { tmem_alloc(&sh->tmem_slot, 512); tmem_relinquish(); }
+  if (warp == TMA_WARP && rows < TILE) {     // rows that no copy ever fills are summed too
+    for (int s = 0; s < F::STAGES; ++s) clear_tail(sQ + s * STAGE, F::KS + F::VS, rows, lane);
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  const bool drain = setup_barrier(a.err);
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem_slot;       // S' at 0 (P' over it), dP' at 128 (dS' over it), dV at 256, dK at 384
+  const Unit unit = sh->unit;
+  if (drain || unit.bad || u >= unit.total) {
+    if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
+    if (drain) return;
+    if (unit.bad) {
+      if (tid == 0 && a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
+      return;
+    }
+    clear_rows(a.out, __ldg(a.cu_k + a.n), a.Tk, a.kv_heads, kvh, 1, a.dim, u - unit.total, a.units - unit.total);
+    clear_rows(a.out2, __ldg(a.cu_k + a.n), a.Tk, a.kv_heads, kvh, 1, a.vdim, u - unit.total, a.units - unit.total);
+    return;
+  }
+  const int q0 = __ldg(a.cu_q + unit.seq), L = __ldg(a.cu_q + unit.seq + 1) - q0;
+  const int k0 = __ldg(a.cu_k + unit.seq), Lk = __ldg(a.cu_k + unit.seq + 1) - k0;
+  const int off = Lk - L;
+  // place 0 is the last key tile of its sequence, which few queries see: the longest loops come first
+  const int kt = (Lk + TILE - 1) / TILE - 1 - unit.place, key0 = kt * TILE;
+  const int q_tiles = (L + a.tok - 1) / a.tok, q_first = max(0, key0 - off) / a.tok;
+  const int per_chunk = max(0, q_tiles - q_first), n = per_chunk * a.chunks;
+  auto tile_of = [&](int i) { return q_tiles - 1 - i % per_chunk; };          // query tile of step i, the last one first
+  float up = 1.f, down = 1.f;                // power of two that brings the call's largest |do| to 2^-4
+  if (HALF) {
+    const uint32_t top = *a.top;
+    if (top) {
+      const int e = 127 - 4 - int(top >> 23);
+      up = __uint_as_float(uint32_t(127 + e) << 23);
+      down = __uint_as_float(uint32_t(127 - e) << 23);
+    }
+  }
+
+  if (warp == TMA_WARP) {
+    bool ok = true;
+    if (n > 0 && lane == 0) {
+      mbar_expect_tx(&sh->kv_full, (F::KS + F::VS) * SLAB);
+      for (int s = 0; s < F::KS; ++s) tma_rows(sK + s * SLAB, &tmK, &sh->kv_full, s * 64, kvh, k0 + key0);
+      for (int s = 0; s < F::VS; ++s) tma_rows(sV + s * SLAB, &tmV, &sh->kv_full, s * 64, kvh, k0 + key0);
+    }
+    uint32_t cuts = 0;
+    for (int i = 0; i < n && ok; ++i) {
+      const int s = i % F::STAGES, first = tile_of(i) * a.tok, head0 = group0 + i / per_chunk * a.hb;
+      ok = warp_wait(&sh->q_empty[s], ((i / F::STAGES) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY);
+      if (!ok) break;
+      const bool cut = first + a.tok > L;                     // Q and dO are summed over their rows
+      uint64_t* bar = cut ? &sh->tail : &sh->q_full[s];
+      uint8_t* st = sQ + s * STAGE;
+      if (lane == 0) {
+        mbar_expect_tx(bar, (F::KS + F::VS) * rows * 128);
+        for (int c = 0; c < F::KS; ++c) tma_rows(st + c * SLAB, &tmQ, bar, c * 64, head0, q0 + first);
+        for (int c = 0; c < F::VS; ++c) tma_rows(st + (F::KS + c) * SLAB, &tmG, bar, c * 64, head0, q0 + first);
+      }
+      for (int r = lane; r < TILE; r += 32) {
+        const int tok = r / a.hb, pos = first + tok;
+        const bool mine = r < rows && pos < L;
+        const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
+        sh->lse[s][r] = mine ? a.lse[at] : INFINITY;
+        sh->delta[s][r] = mine ? a.delta[at] * up : 0.f;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->stat_full[s]);
+      if (cut) {
+        ok = warp_wait(bar, cuts & 1, abort_flag, a.err, ERR_WAIT_FULL);
+        ++cuts;
+        if (!ok) break;
+        clear_tail(st, F::KS + F::VS, (L - first) * a.hb, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->q_full[s]);
+      }
+    }
+  } else if (warp == MMA_WARP) {
+    if (elect_one()) {
+      constexpr uint32_t id_s = idesc(HALF, TILE, false), id_v = idesc(HALF, DV, true), id_k = idesc(HALF, D, true);
+      const uint32_t aK = smem_u32(sK), aV = smem_u32(sV);
+      int is = 0, ip = 0, iv = 0, ik = 0, freed = 0;
+      bool there = false;
+      Patience patience;
+      bool moved = true;
+      auto stage_free = [&]() {
+        if (iv > freed && ik > freed) {
+          umma_commit(&sh->q_empty[freed % F::STAGES]);
+          ++freed;
+        }
+      };
+      while (ik < n && patience.more(moved, abort_flag, a.err)) {
+        moved = false;
+        if (!there) {
+          there = moved = ready(&sh->kv_full, 0);
+          continue;
+        }
+        if (is < n && ready(&sh->q_full[is % F::STAGES], (is / F::STAGES) & 1) && (is == 0 || ready(&sh->dv_done, (is - 1) & 1))) {
+          tc_fence_after();
+          const uint32_t aQ = smem_u32(sQ + (is % F::STAGES) * STAGE);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) umma_f16(tmem, desc_k(aK, k), desc_k(aQ, k), id_s, k != 0);
+          umma_commit(&sh->s_full);
+          ++is;
+          moved = true;
+        }
+        if (iv < is && ready(&sh->p_full, iv & 1)) {
+          tc_fence_after();
+          const uint32_t aG = smem_u32(sQ + (iv % F::STAGES) * STAGE + F::KS * SLAB);
+#pragma unroll
+          for (int k = 0; k < TILE / 16; ++k) umma_ta(tmem + 256, tmem + (k >> 2) * 64 + (k & 3) * 8, desc_mn(aG, k), id_v, (iv | k) != 0);
+          umma_commit(&sh->dv_done);
+          ++iv;
+          stage_free();
+          moved = true;
+        }
+        if (ip < n && ready(&sh->q_full[ip % F::STAGES], (ip / F::STAGES) & 1) && (ip == 0 || ready(&sh->dk_done, (ip - 1) & 1))) {
+          tc_fence_after();
+          const uint32_t aG = smem_u32(sQ + (ip % F::STAGES) * STAGE + F::KS * SLAB);
+#pragma unroll
+          for (int k = 0; k < DV / 16; ++k) umma_f16(tmem + 128, desc_k(aV, k), desc_k(aG, k), id_s, k != 0);
+          umma_commit(&sh->dp_full);
+          ++ip;
+          moved = true;
+        }
+        if (ik < ip && ready(&sh->ds_full, ik & 1)) {
+          tc_fence_after();
+          const uint32_t aQ = smem_u32(sQ + (ik % F::STAGES) * STAGE);
+#pragma unroll
+          for (int k = 0; k < TILE / 16; ++k) umma_ta(tmem + 384, tmem + 128 + (k >> 2) * 64 + (k & 3) * 8, desc_mn(aQ, k), id_k, (ik | k) != 0);
+          umma_commit(&sh->dk_done);
+          ++ik;
+          stage_free();
+          moved = true;
+        }
+      }
+      if (n > 0 && ik == n) umma_commit(&sh->acc_done);
+    }
+  } else {
+    const int half = warp >> 2, r = tid & 127;
+    const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + half * 64 + lane_addr, tdP = tmem + 128 + half * 64 + lane_addr;
+    auto step = [&](int i, auto where) {
+      constexpr bool MASK = decltype(where)::value;
+      const int s = i % F::STAGES, first = tile_of(i) * a.tok;
+      // columns [from, to) see this key: queries at or behind it, of this sequence
+      const int from = max(0, key0 + r - off - first) * a.hb - half * 64, to = min(a.tok, L - first) * a.hb - half * 64;
+      if (!warp_wait(&sh->stat_full[s], (i / F::STAGES) & 1, abort_flag, a.err, ERR_WAIT_FULL)) return false;
+      if (!warp_wait(&sh->s_full, i & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
+      tc_fence_after();
+      float p[64];
+      uint32_t w[32];
+      const float4* lse = reinterpret_cast<const float4*>(&sh->lse[s][half * 64]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t x[32];
+        tmem_ld_32x32(tS + c * 32, x);
+        tmem_ld_wait();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float4 m = lse[c * 8 + q];
+          const float ms[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int col = c * 32 + q * 4 + e;
+            const float y = ex2(fmaf(__uint_as_float(x[q * 4 + e]), a.scale_log2, -ms[e]));
+            p[col] = !MASK || (col >= from && col < to) ? y : 0.f;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[c * 16 + e] = pair<HALF>(p[c * 32 + 2 * e], p[c * 32 + 2 * e + 1]);
+      }
+      tmem_st(tS, w);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->p_full);
+      if (!warp_wait(&sh->dp_full, i & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
+      tc_fence_after();
+      const float4* delta = reinterpret_cast<const float4*>(&sh->delta[s][half * 64]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t x[32];
+        tmem_ld_32x32(tdP + c * 32, x);
+        tmem_ld_wait();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float4 m = delta[c * 8 + q];
+          const float ms[4] = {m.x, m.y, m.z, m.w};
+          float d[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int col = c * 32 + q * 4 + e;
+            const float y = p[col] * (HALF ? fmaf(__uint_as_float(x[q * 4 + e]), up, -ms[e]) : __uint_as_float(x[q * 4 + e]) - ms[e]);
+            d[e] = !MASK || (col >= from && col < to) ? y : 0.f;
+          }
+          w[c * 16 + q * 2] = pair<HALF>(d[0], d[1]);
+          w[c * 16 + q * 2 + 1] = pair<HALF>(d[2], d[3]);
+        }
+      }
+      tmem_st(tdP, w);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->ds_full);
+      return true;
+    };
+    bool ok = true;
+    for (int i = 0; i < n && ok; ++i) {
+      const int first = tile_of(i) * a.tok;
+      ok = key0 + TILE - 1 > off + first || first + a.tok > L ? step(i, Masked{}) : step(i, Whole{});
+    }
+    if (ok && n > 0) ok = warp_wait(&sh->acc_done, 0, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
+    if (ok) {
+      tc_fence_after();
+      const bool mine = key0 + r < Lk;
+      const long long at = (long long)(k0 + key0 + r) * a.kv_heads + kvh;
+      uint16_t* krow = reinterpret_cast<uint16_t*>(a.out) + at * a.dim;
+      uint16_t* vrow = reinterpret_cast<uint16_t*>(a.out2) + at * a.vdim;
+#pragma unroll
+      for (int c = 0; c < (D + DV) / 64; ++c) {
+        const bool k = c < D / 64;
+        const int col = k ? half * (D / 2) + c * 32 : half * (DV / 2) + (c - D / 64) * 32;
+        uint32_t x[32];
+        if (n > 0) {
+          tmem_ld_32x32(tmem + (k ? 384 : 256) + col + lane_addr, x);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = 0u;
+        }
+        if (mine) store_columns<HALF>((k ? krow : vrow) + col, x, k ? a.scale * down : 1.f, (k ? a.dim : a.vdim) - col);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  settle(abort_flag);
+  if (warp == MMA_WARP) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// ---- launches --------------------------------------------------------------------------------------------------------
+// [rows, heads, width] with strides (elements) of rows and heads; boxes of 64 columns, `box_heads` heads, `box_rows` rows
+int map_rows(CUtensorMap* out, const void* base, int rows, int heads, int width, const long long* strides, int box_heads, int box_rows, bool half) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) return -1;
+  // a stride that no step takes may be anything: one that the encoder accepts stands in its place
+  const long long plain = (long long)width * 2;
+  cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t st[2] = {(cuuint64_t)(heads > 1 ? strides[1] * 2 : plain), (cuuint64_t)(rows > 1 ? strides[0] * 2 : plain * heads)};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows}, es[3] = {1, 1, 1};
+  const CUresult r = enc(out, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, st, box,
+                         es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : int(r);
+}
+
+static_assert(Fwd<128, 128>::SMEM <= 227 * 1024 && Fwd<128, 64>::SMEM <= 227 * 1024 && Dq<128, 128>::SMEM <= 227 * 1024 &&
+                  Dkv<128, 128>::SMEM <= 227 * 1024,
+              "shared memory of a block");
+
+template <typename K>
+int configure(K kern, int smem, PerDevice& cfg) {
+  if (cfg.first()) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2;
+    cfg.done();
+  }
+  return 0;
+}
+
+// Tiles of the sequences are at most rows / per + n, since each begins at most one part-filled tile; one block more for the rows behind them
+long long units_of(int rows, int n, int per) { return rows / per + (long long)n + 1; }
+
+int shape(Args& a) {
+  if (a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads || a.dim < 8 || a.dim % 8 || a.dim > 128 || a.vdim < 8 || a.vdim % 8 || a.vdim > 128 ||
+      a.T < 1 || a.Tk < 1 || a.n < 0 || !(a.scale >= 0.f) || a.T > (1 << 30) || a.Tk > (1 << 30) || a.n > (1 << 30))
+    return -10;
+  // Heads of a tile: all of a group where they fill 15/16 of its rows or more, else the largest divisor of the group that does (96 heads: three
+  // tiles of 32 heads of 4 tokens rather than one of a single token that leaves a quarter idle).  One head always does.
+  const int group = a.heads / a.kv_heads;
+  a.hb = group < TILE ? group : TILE;
+  while (group % a.hb || TILE / a.hb * a.hb < TILE * 15 / 16) --a.hb;
+  a.chunks = group / a.hb;
+  a.tok = TILE / a.hb;
+  return 0;
+}
+
+struct Inputs {
+  const void *q, *k, *v, *g;
+  const long long *qs, *ks, *vs, *gs;
+};
+
+int maps(CUtensorMap (&m)[4], const Inputs& i, const Args& a, bool half) {
+  int rc = map_rows(&m[0], i.q, a.T, a.heads, a.dim, i.qs, a.hb, a.tok, half);
+  if (!rc) rc = map_rows(&m[1], i.k, a.Tk, a.kv_heads, a.dim, i.ks, 1, TILE, half);
+  if (!rc) rc = map_rows(&m[2], i.v, a.Tk, a.kv_heads, a.vdim, i.vs, 1, TILE, half);
+  if (!rc && i.g) rc = map_rows(&m[3], i.g, a.T, a.heads, a.vdim, i.gs, a.hb, a.tok, half);
+  return rc;
+}
+
+template <bool HALF, int D, int DV>
+int forward(const Inputs& in, Args a, cudaStream_t stream) {
+  CUtensorMap m[4];
+  int rc = maps(m, in, a, HALF);
+  static PerDevice cfg;
+  if (!rc) rc = configure(packed_fwd_kernel<HALF, D, DV>, Fwd<D, DV>::SMEM, cfg);
+  if (rc) return rc;
+  const long long units = units_of(a.T, a.n, 2 * a.tok), grid = units * a.kv_heads * a.chunks;
+  if (grid > 0x7fffffffLL) return -10;
+  a.units = (int)units;
+  packed_fwd_kernel<HALF, D, DV><<<(unsigned)grid, THREADS, Fwd<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+template <bool HALF, int D, int DV>
+int backward(const Inputs& in, Args a, void* dq, void* dk, void* dv, cudaStream_t stream) {
+  CUtensorMap m[4];
+  int rc = maps(m, in, a, HALF);
+  static PerDevice cfg_q, cfg_k;
+  if (!rc) rc = configure(packed_dq_kernel<HALF, D, DV>, Dq<D, DV>::SMEM, cfg_q);
+  if (!rc) rc = configure(packed_dkv_kernel<HALF, D, DV>, Dkv<D, DV>::SMEM, cfg_k);
+  if (rc) return rc;
+  const long long uq = units_of(a.T, a.n, a.tok), uk = units_of(a.Tk, a.n, TILE);
+  if (uq * a.kv_heads * a.chunks > 0x7fffffffLL || uk * a.kv_heads > 0x7fffffffLL) return -10;
+  if (HALF && cudaMemsetAsync(a.top, 0, sizeof(uint32_t), stream) != cudaSuccess) return -3;
+  a.units = (int)uq;
+  a.out = dq;
+  packed_dq_kernel<HALF, D, DV><<<(unsigned)(uq * a.kv_heads * a.chunks), THREADS, Dq<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], m[3], a);
+  if (cudaGetLastError() != cudaSuccess) return -3;
+  a.units = (int)uk;
+  a.out = dk;
+  a.out2 = dv;
+  packed_dkv_kernel<HALF, D, DV><<<(unsigned)(uk * a.kv_heads), THREADS, Dkv<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], m[3], a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+}  // namespace
+}  // namespace packed
+}  // namespace cm
+
+using namespace cm;
+using namespace cm::packed;
+
+// q [T, heads, dim], k [Tk, kv_heads, dim], v [Tk, kv_heads, vdim] with strides (elements) of their first two axes, rows on 16 bytes; cu_q,
+// cu_k [n + 1]; o [T, heads, vdim] packed; lse [T, heads] or null.  kind: 0 bf16, 1 fp16.  dim, vdim multiples of 8 up to 128; scale not negative.
+extern "C" int cm_packed_attention_fwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs,
+                                       const int* cu_q, const int* cu_k, void* o, float* lse, int n, int T, int Tk, int heads, int kv_heads, int dim,
+                                       int vdim, float scale, int kind, int* err, cudaStream_t stream) {
+  Args a = {};
+  a.cu_q = cu_q; a.cu_k = cu_k;
+  a.n = n; a.T = T; a.Tk = Tk;
+  a.heads = heads; a.kv_heads = kv_heads;
+  a.dim = dim; a.vdim = vdim;
+  a.scale = scale; a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = o;
+  a.lse = lse;
+  a.err = err;
+  const int rc = shape(a);
+  if (rc) return rc;
+  const Inputs in = {q, k, v, nullptr, qs, ks, vs, nullptr};
+  if (kind == 0) {
+    if (vdim > 64) return forward<false, 128, 128>(in, a, stream);
+    return dim > 64 ? forward<false, 128, 64>(in, a, stream) : forward<false, 64, 64>(in, a, stream);
+  }
+  if (vdim > 64) return forward<true, 128, 128>(in, a, stream);
+  return dim > 64 ? forward<true, 128, 64>(in, a, stream) : forward<true, 64, 64>(in, a, stream);
+}
+
+// o and go (the gradient of o) [T, heads, vdim] with strides as q's; lse from the forward; delta: scratch of T * heads + 1 floats;
+// dq [T, heads, dim], dk [Tk, kv_heads, dim], dv [Tk, kv_heads, vdim] packed, all written whole.
+extern "C" int cm_packed_attention_bwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs,
+                                       const void* o, const long long* os, const void* go, const long long* gs, const int* cu_q, const int* cu_k,
+                                       const float* lse, float* delta, void* dq, void* dk, void* dv, int n, int T, int Tk, int heads, int kv_heads,
+                                       int dim, int vdim, float scale, int kind, int* err, cudaStream_t stream) {
+  Args a = {};
+  a.cu_q = cu_q; a.cu_k = cu_k;
+  a.n = n; a.T = T; a.Tk = Tk;
+  a.heads = heads; a.kv_heads = kv_heads;
+  a.dim = dim; a.vdim = vdim;
+  a.scale = scale; a.scale_log2 = scale * 1.4426950408889634f;
+  a.o = o; a.go = go;
+  a.o_tok = os[0]; a.o_head = os[1];
+  a.go_tok = gs[0]; a.go_head = gs[1];
+  a.lse = const_cast<float*>(lse);
+  a.delta = delta;
+  a.top = reinterpret_cast<uint32_t*>(delta + (long long)T * heads);
+  a.err = err;
+  const int rc = shape(a);
+  if (rc) return rc;
+  const Inputs in = {q, k, v, go, qs, ks, vs, gs};
+  if (kind == 0) {
+    if (vdim > 64) return backward<false, 128, 128>(in, a, dq, dk, dv, stream);
+    return dim > 64 ? backward<false, 128, 64>(in, a, dq, dk, dv, stream) : backward<false, 64, 64>(in, a, dq, dk, dv, stream);
+  }
+  if (vdim > 64) return backward<true, 128, 128>(in, a, dq, dk, dv, stream);
+  return dim > 64 ? backward<true, 128, 64>(in, a, dq, dk, dv, stream) : backward<true, 64, 64>(in, a, dq, dk, dv, stream);
+}

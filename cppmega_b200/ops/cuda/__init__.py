@@ -62,11 +62,12 @@ def _declare(L: ctypes.CDLL) -> None:
         if fn is not None:
             fn.argtypes = args
             fn.restype = i32
-    from . import attention, block, extra, kernels4, paged
+    from . import attention, block, extra, kernels4, packed, paged
     extra.declare(L)
     kernels4.declare(L)
     attention.declare(L)
     block.declare(L)
+    packed.declare(L)
     paged.declare(L)
 
 
@@ -391,11 +392,12 @@ def _register() -> None:
     F_.register_cuda("rmsnorm", rmsnorm)
     F_.register_cuda("swiglu", swiglu)
     F_.register_cuda("adamw_shard", adamw_shard)
-    from . import attention, block, extra, kernels4, paged
+    from . import attention, block, extra, kernels4, packed, paged
     extra.register()
     kernels4.register()
     attention.register()
     block.register()
+    packed.register()
     paged.register()
 
 

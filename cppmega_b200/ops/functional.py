@@ -457,8 +457,8 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, cu_seqlens_k=None):
     query without keys gives zeros, and so do the rows behind the last sequence, whatever they hold.  Within a sequence a key that is not finite
     reaches earlier queries too where it shares a tile with them (a weight of zero times infinity).
 
-    bf16 and fp16 with ``D`` and ``Dv`` multiples of 8 up to 128 and up to 128 heads a group run on the kernels, in training with their
-    gradients (first derivatives; the same call gives the same bits); strided tensors are read in place where rows lie on 16 bytes.
+    bf16 and fp16 with ``D`` and ``Dv`` multiples of 8 up to 128 run on the kernels, in training with their gradients (first
+    derivatives; the same call gives the same bits); strided tensors are read in place where rows lie on 16 bytes.
     Anything else, forward mode and function transforms run the definition, ``reference.packed_attention``.  No call waits for the device: ends
     that fall or run over the buffer are reported by ``ops.cuda.check_errors``."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape[:2] != v.shape[:2] or q.shape[2] != k.shape[2]:
