@@ -27,7 +27,9 @@
 // another; a product that overwrites columns is issued only after the commit of the one that reads them.
 // Query tiles of the key gradients run from the last one down: blocks of one sequence then read the same rows at the same time, out of L2.
 //
-// Roundings to 16 bits: P and dS, as operands of their products.  Maxima, sums, scores, deltas and all accumulators are fp32.  fp16's range
+// Roundings to 16 bits: P and dS, as operands of their products.  delta takes o before its rounding (the forward keeps what that takes away,
+// in 16 bits more): with the rounded o, an error of 2^-9 of |do||o| is added to every ds of a row with one sign, and dq and dk were off by 4.4e-3
+// of their norms instead of 2.4e-3.  Maxima, sums, scores, deltas and all accumulators are fp32.  fp16's range
 // is too short for dS of any size: it is scaled by a power of two, from the row's largest |do| for dq, from the call's for dk.
 #include <cuda_fp16.h>
 
@@ -125,9 +127,9 @@ struct Args {
   int units;                                 // blocks per (key head, chunk)
   float scale, scale_log2;
   void* out;                                 // forward: o [T, heads, vdim]; backward: dq [T, heads, dim] or dk [Tk, kv_heads, dim]
-  void* out2;                                // dv [Tk, kv_heads, vdim]
-  const void *o, *go;                        // backward, for delta: o and do with their strides
-  long long o_tok, o_head, go_tok, go_head;
+  void* out2;                                // forward: what rounding took from o, or null; backward: dv [Tk, kv_heads, vdim]
+  const void *o, *o_rest, *go;               // backward, for delta: o, what rounding took from it (both packed), do with its strides
+  long long go_tok, go_head;
   float* lse;                                // [T, heads]: log2 of the sum of weights; +inf without keys; null: not wanted
   float* delta;                              // [T, heads]
   uint32_t* top;                             // largest |do| of the call as bits (fp16)
@@ -228,6 +230,12 @@ __device__ __forceinline__ void store_columns(uint16_t* row, const uint32_t (&x)
     o.w = pair<HALF>(__uint_as_float(x[q * 8 + 6]) * f, __uint_as_float(x[q * 8 + 7]) * f);
     if (q * 8 < left) reinterpret_cast<uint4*>(row)[q] = o;
   }
+}
+
+// What the rounding of store_columns takes away, to as many bits again
+template <bool HALF>
+__device__ __forceinline__ float rest(float x) {
+  return HALF ? x - __half2float(__float2half_rn(x)) : x - __bfloat162float(__float2bfloat16_rn(x));
 }
 
 struct Masked { static constexpr bool value = true; };
@@ -507,7 +515,13 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = last >= 0 ? o[e] : 0u;            // a row without keys
-        if (mine) store_columns<HALF>(row + c * 32, o, last >= 0 ? inv : 0.f, a.vdim - c * 32);
+        const float f = last >= 0 ? inv : 0.f;
+        if (mine) store_columns<HALF>(row + c * 32, o, f, a.vdim - c * 32);
+        if (a.out2) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(rest<HALF>(__uint_as_float(o[e]) * f));
+          if (mine) store_columns<HALF>(reinterpret_cast<uint16_t*>(a.out2) + at * a.vdim + c * 32, o, 1.f, a.vdim - c * 32);
+        }
       }
       if (mine && a.lse) a.lse[at] = l == 0.f ? INFINITY : m_ref + log2f(l);
     }
@@ -678,17 +692,18 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     // delta, and the power of two that brings the row's largest |do| to 2^-4; both threads of a row add it up whole
     float delta = 0.f, big = 0.f;
     if (mine) {
-      const uint4* ov = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o) + (q0 + pos) * a.o_tok + head * a.o_head);
+      const uint4* ov = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o) + at * a.vdim);
+      const uint4* rv = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o_rest) + at * a.vdim);
       const uint4* gv = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.go) + (q0 + pos) * a.go_tok + head * a.go_head);
 #pragma unroll
       for (int c = 0; c < DV / 8; ++c) {
         if (c * 8 >= a.vdim) break;
-        const uint4 x = __ldg(ov + c), y = __ldg(gv + c);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        const uint4 x = __ldg(ov + c), z = __ldg(rv + c), y = __ldg(gv + c);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, zs[4] = {z.x, z.y, z.z, z.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 f = unpair<HALF>(xs[e]), g = unpair<HALF>(ys[e]);
-          delta = fmaf(f.x, g.x, fmaf(f.y, g.y, delta));
+          const float2 f = unpair<HALF>(xs[e]), h = unpair<HALF>(zs[e]), g = unpair<HALF>(ys[e]);
+          delta = fmaf(f.x + h.x, g.x, fmaf(f.y + h.y, g.y, delta));
           if (HALF) big = fmaxf(big, fmaxf(fabsf(g.x), fabsf(g.y)));
         }
       }
@@ -898,12 +913,19 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         for (int c = 0; c < F::KS; ++c) tma_rows(st + c * SLAB, &tmQ, bar, c * 64, head0, q0 + first);
         for (int c = 0; c < F::VS; ++c) tma_rows(st + (F::KS + c) * SLAB, &tmG, bar, c * 64, head0, q0 + first);
       }
-      for (int r = lane; r < TILE; r += 32) {
-        const int tok = r / a.hb, pos = first + tok;
+      float lse[TILE / 32], delta[TILE / 32];                 // all on their way before the first is put down
+#pragma unroll
+      for (int c = 0; c < TILE / 32; ++c) {
+        const int r = c * 32 + lane, tok = r / a.hb, pos = first + tok;
         const bool mine = r < rows && pos < L;
         const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
-        sh->lse[s][r] = mine ? a.lse[at] : INFINITY;
-        sh->delta[s][r] = mine ? a.delta[at] * up : 0.f;
+        lse[c] = mine ? __ldg(a.lse + at) : INFINITY;
+        delta[c] = mine ? __ldg(a.delta + at) * up : 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < TILE / 32; ++c) {
+        sh->lse[s][c * 32 + lane] = lse[c];
+        sh->delta[s][c * 32 + lane] = delta[c];
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->stat_full[s]);
@@ -1183,57 +1205,55 @@ int backward(const Inputs& in, Args a, void* dq, void* dk, void* dv, cudaStream_
 using namespace cm;
 using namespace cm::packed;
 
-// q [T, heads, dim], k [Tk, kv_heads, dim], v [Tk, kv_heads, vdim] with strides (elements) of their first two axes, rows on 16 bytes; cu_q,
-// cu_k [n + 1]; o [T, heads, vdim] packed; lse [T, heads] or null.  kind: 0 bf16, 1 fp16.  dim, vdim multiples of 8 up to 128; scale not negative.
-extern "C" int cm_packed_attention_fwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs,
-                                       const int* cu_q, const int* cu_k, void* o, float* lse, int n, int T, int Tk, int heads, int kv_heads, int dim,
-                                       int vdim, float scale, int kind, int* err, cudaStream_t stream) {
-  Args a = {};
+// Sizes and strides (elements) come in n: strides of tokens and heads of q, k, v (and of go, in the backward); sequences, T, Tk, heads, kv_heads,
+// dim, vdim, kind (0 bf16, 1 fp16).  dim, vdim multiples of 8 up to 128; rows on 16 bytes; scale not negative.
+static int arguments(Args& a, const int* cu_q, const int* cu_k, float scale, const long long* n, int* err) {
   a.cu_q = cu_q; a.cu_k = cu_k;
-  a.n = n; a.T = T; a.Tk = Tk;
-  a.heads = heads; a.kv_heads = kv_heads;
-  a.dim = dim; a.vdim = vdim;
+  a.n = (int)n[8]; a.T = (int)n[9]; a.Tk = (int)n[10];
+  a.heads = (int)n[11]; a.kv_heads = (int)n[12];
+  a.dim = (int)n[13]; a.vdim = (int)n[14];
   a.scale = scale; a.scale_log2 = scale * 1.4426950408889634f;
-  a.out = o;
-  a.lse = lse;
   a.err = err;
-  const int rc = shape(a);
-  if (rc) return rc;
-  const Inputs in = {q, k, v, nullptr, qs, ks, vs, nullptr};
-  if (kind == 0) {
-    if (vdim > 64) return forward<false, 128, 128>(in, a, stream);
-    return dim > 64 ? forward<false, 128, 64>(in, a, stream) : forward<false, 64, 64>(in, a, stream);
-  }
-  if (vdim > 64) return forward<true, 128, 128>(in, a, stream);
-  return dim > 64 ? forward<true, 128, 64>(in, a, stream) : forward<true, 64, 64>(in, a, stream);
+  return shape(a);
 }
 
-// o and go (the gradient of o) [T, heads, vdim] with strides as q's; lse from the forward; delta: scratch of T * heads + 1 floats;
-// dq [T, heads, dim], dk [Tk, kv_heads, dim], dv [Tk, kv_heads, vdim] packed, all written whole.
-extern "C" int cm_packed_attention_bwd(const void* q, const long long* qs, const void* k, const long long* ks, const void* v, const long long* vs,
-                                       const void* o, const long long* os, const void* go, const long long* gs, const int* cu_q, const int* cu_k,
-                                       const float* lse, float* delta, void* dq, void* dk, void* dv, int n, int T, int Tk, int heads, int kv_heads,
-                                       int dim, int vdim, float scale, int kind, int* err, cudaStream_t stream) {
+// q [T, heads, dim], k [Tk, kv_heads, dim], v [Tk, kv_heads, vdim]; cu_q, cu_k [sequences + 1]; o [T, heads, vdim] packed; for a backward pass
+// o_rest, as o, and lse [T, heads], else null
+extern "C" int cm_packed_attention_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, void* o_rest,
+                                       float* lse, const long long* n, float scale, int* err, cudaStream_t stream) {
   Args a = {};
-  a.cu_q = cu_q; a.cu_k = cu_k;
-  a.n = n; a.T = T; a.Tk = Tk;
-  a.heads = heads; a.kv_heads = kv_heads;
-  a.dim = dim; a.vdim = vdim;
-  a.scale = scale; a.scale_log2 = scale * 1.4426950408889634f;
-  a.o = o; a.go = go;
-  a.o_tok = os[0]; a.o_head = os[1];
-  a.go_tok = gs[0]; a.go_head = gs[1];
+  const int rc = arguments(a, cu_q, cu_k, scale, n, err);
+  if (rc) return rc;
+  a.out = o;
+  a.out2 = o_rest;
+  a.lse = lse;
+  const Inputs in = {q, k, v, nullptr, n, n + 2, n + 4, nullptr};
+  if (n[15] == 0) {
+    if (a.vdim > 64) return forward<false, 128, 128>(in, a, stream);
+    return a.dim > 64 ? forward<false, 128, 64>(in, a, stream) : forward<false, 64, 64>(in, a, stream);
+  }
+  if (a.vdim > 64) return forward<true, 128, 128>(in, a, stream);
+  return a.dim > 64 ? forward<true, 128, 64>(in, a, stream) : forward<true, 64, 64>(in, a, stream);
+}
+
+// o, o_rest and lse from the forward; go (the gradient of o) [T, heads, vdim]; delta: scratch of T * heads + 1 floats;
+// dq [T, heads, dim], dk [Tk, kv_heads, dim], dv [Tk, kv_heads, vdim] packed, all written whole
+extern "C" int cm_packed_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* go, const int* cu_q,
+                                       const int* cu_k, const float* lse, float* delta, void* dq, void* dk, void* dv, const long long* n, float scale,
+                                       int* err, cudaStream_t stream) {
+  Args a = {};
+  const int rc = arguments(a, cu_q, cu_k, scale, n, err);
+  if (rc) return rc;
+  a.o = o; a.o_rest = o_rest; a.go = go;
+  a.go_tok = n[6]; a.go_head = n[7];
   a.lse = const_cast<float*>(lse);
   a.delta = delta;
-  a.top = reinterpret_cast<uint32_t*>(delta + (long long)T * heads);
-  a.err = err;
-  const int rc = shape(a);
-  if (rc) return rc;
-  const Inputs in = {q, k, v, go, qs, ks, vs, gs};
-  if (kind == 0) {
-    if (vdim > 64) return backward<false, 128, 128>(in, a, dq, dk, dv, stream);
-    return dim > 64 ? backward<false, 128, 64>(in, a, dq, dk, dv, stream) : backward<false, 64, 64>(in, a, dq, dk, dv, stream);
+  a.top = reinterpret_cast<uint32_t*>(delta + (long long)a.T * a.heads);
+  const Inputs in = {q, k, v, go, n, n + 2, n + 4, n + 6};
+  if (n[15] == 0) {
+    if (a.vdim > 64) return backward<false, 128, 128>(in, a, dq, dk, dv, stream);
+    return a.dim > 64 ? backward<false, 128, 64>(in, a, dq, dk, dv, stream) : backward<false, 64, 64>(in, a, dq, dk, dv, stream);
   }
-  if (vdim > 64) return backward<true, 128, 128>(in, a, dq, dk, dv, stream);
-  return dim > 64 ? backward<true, 128, 64>(in, a, dq, dk, dv, stream) : backward<true, 64, 64>(in, a, dq, dk, dv, stream);
+  if (a.vdim > 64) return backward<true, 128, 128>(in, a, dq, dk, dv, stream);
+  return a.dim > 64 ? backward<true, 128, 64>(in, a, dq, dk, dv, stream) : backward<true, 64, 64>(in, a, dq, dk, dv, stream);
 }

@@ -679,48 +679,48 @@ extern "C" long long cm_paged_attention_ws(int sequences, int kv_heads, int grou
   return layout_of(sequences, kv_heads, group, dim, vdim, columns, page).floats;
 }
 
-// q [sequences, kv_heads * group, dim] with strides qs (elements) of its first two axes; caches as in cm_cache_write; table [sequences, columns],
-// lens [sequences]; out [sequences, kv_heads * group, vdim] packed; ws: cm_paged_attention_ws floats.  kind: 0 bf16, 1 fp16 (a 16-bit cache
-// has the same type).  dim, vdim multiples of 8 (16 in an E4M3 cache) up to 128, group up to 128.
-extern "C" int cm_paged_attention(const void* q, const long long* qs, const void* k, const long long* kcs, const void* v, const long long* vcs,
-                                  const void* k_scale, const void* v_scale, const int* table, long long table_row, const int* lens, void* out,
-                                  float* ws, int sequences, int kv_heads, int group, int columns, int pages, int page, int dim, int vdim,
-                                  float scale, int kind, int e4m3, int* err, cudaStream_t stream) {
+// q [sequences, kv_heads * group, dim]; caches [pages, page, kv_heads, .], E4M3 ones with their exponent bytes; table [sequences, columns],
+// lens [sequences]; out [sequences, kv_heads * group, vdim] packed; ws: cm_paged_attention_ws floats.  Sizes and strides (elements) come in n:
+//   strides of q's sequences and heads, of pages, tokens and heads of the key cache, then of the value cache, of the table's rows;
+//   sequences, kv_heads, group, columns, pages, page, dim, vdim, kind (0 bf16, 1 fp16; a 16-bit cache has the same type), e4m3.
+// dim, vdim multiples of 8 (16 in an E4M3 cache) up to 128, group up to 128.
+extern "C" int cm_paged_attention(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale, const int* table,
+                                  const int* lens, void* out, float* ws, const long long* n, float scale, int* err, cudaStream_t stream) {
+  const long long sequences = n[9], kv_heads = n[10], group = n[11], columns = n[12], pages = n[13], page = n[14], dim = n[15], vdim = n[16];
+  const bool e4m3 = n[18];
   if (sequences <= 0 || kv_heads <= 0) return 0;
-  const int step = e4m3 ? 16 : 8;
+  const int step = e4m3 ? 16 : 8, es = e4m3 ? 1 : 2;
   if (group < 1 || group > 128 || dim < step || dim > 128 || dim % step || vdim < step || vdim > 128 || vdim % step || page < 1 || columns < 0 ||
-      (long long)columns * page > 0x7fffffffLL - KEYS || (long long)sequences * kv_heads * group > 0x7fffffffLL)
+      columns * page > 0x7fffffffLL - KEYS || sequences * kv_heads * group > 0x7fffffffLL)
     return -10;
-  const Layout s = layout_of(sequences, kv_heads, group, dim, vdim, columns, page);
-  const int es = e4m3 ? 1 : 2;
+  const Layout s = layout_of((int)sequences, (int)kv_heads, (int)group, (int)dim, (int)vdim, (int)columns, (int)page);
   Args a;
   a.q = (const uint8_t*)q;
-  a.q_seq = qs[0] * 2;
-  a.q_head = qs[1] * 2;
+  a.q_seq = n[0] * 2; a.q_head = n[1] * 2;
   a.k = (const uint8_t*)k;
   a.v = (const uint8_t*)v;
-  a.k_page = kcs[0] * es; a.k_tok = kcs[1] * es; a.k_head = kcs[2] * es;
-  a.v_page = vcs[0] * es; a.v_tok = vcs[1] * es; a.v_head = vcs[2] * es;
+  a.k_page = n[2] * es; a.k_tok = n[3] * es; a.k_head = n[4] * es;
+  a.v_page = n[5] * es; a.v_tok = n[6] * es; a.v_head = n[7] * es;
   a.k_scale = (const uint8_t*)k_scale;
   a.v_scale = (const uint8_t*)v_scale;
   a.table = table;
-  a.table_row = table_row;
+  a.table_row = n[8];
   a.lens = lens;
   a.out = out;
   a.part = ws;
-  a.sequences = sequences;
-  a.kv_heads = kv_heads;
-  a.group = group;
-  a.columns = columns;
-  a.pages = pages;
-  a.page = page;
-  a.dim = dim;
-  a.vdim = vdim;
+  a.sequences = (int)sequences;
+  a.kv_heads = (int)kv_heads;
+  a.group = (int)group;
+  a.columns = (int)columns;
+  a.pages = (int)pages;
+  a.page = (int)page;
+  a.dim = (int)dim;
+  a.vdim = (int)vdim;
   a.runs = s.grid > 0 ? s.grid * WARPS / s.tiles : 1;
   a.tiles = s.tiles;
   a.rows = s.rows;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.err = err;
-  if (kind == 0) return e4m3 ? pick<true, true>(a, s, stream) : pick<true, false>(a, s, stream);
+  if (n[17] == 0) return e4m3 ? pick<true, true>(a, s, stream) : pick<true, false>(a, s, stream);
   return e4m3 ? pick<false, true>(a, s, stream) : pick<false, false>(a, s, stream);
 }

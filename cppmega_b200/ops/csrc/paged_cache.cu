@@ -26,6 +26,7 @@ constexpr int THREADS = 256;
 constexpr int MAX_TOKENS = 128;              // tokens of one block
 constexpr int HASH_BITS = 8192;
 constexpr int ROWS_AHEAD = 4;
+constexpr int SCAN = 8;                      // later slots that a thread has on their way at once
 
 struct Side {                                // keys or values
   const uint8_t* x;                          // rows of the packed tensor
@@ -126,13 +127,17 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteArgs a)
     if (s >= 0) atomicOr(&bits[(s & (HASH_BITS - 1)) >> 5], 1u << (s & 31));
   }
   __syncthreads();
-  for (long long t = t0 + 1 + threadIdx.x; t < a.T; t += THREADS) {
-    const long long s = slot_of(a, t);
-    if (s >= 0 && (bits[(s & (HASH_BITS - 1)) >> 5] >> (s & 31) & 1)) {
-      const int before = (int)min((long long)n, t - t0);
-      for (int i = 0; i < before; ++i)
-        if (own[i] == s) lost[i] = 1;
-    }
+  for (long long t = t0 + 1 + threadIdx.x; t < a.T; t += SCAN * THREADS) {
+    long long s[SCAN];
+#pragma unroll
+    for (int c = 0; c < SCAN; ++c) s[c] = t + c * THREADS < a.T ? slot_of(a, t + c * THREADS) : -1;
+#pragma unroll
+    for (int c = 0; c < SCAN; ++c)
+      if (s[c] >= 0 && (bits[(s[c] & (HASH_BITS - 1)) >> 5] >> (s[c] & 31) & 1)) {
+        const int before = (int)min((long long)n, t + c * THREADS - t0);
+        for (int i = 0; i < before; ++i)
+          if (own[i] == s[c]) lost[i] = 1;
+      }
   }
   __syncthreads();
 
@@ -260,10 +265,10 @@ __global__ void __launch_bounds__(THREADS) cache_read_kernel(const ReadArgs a) {
   }
 }
 
-// Tokens of one block: enough blocks for four on every SM, and then as many tokens as the block's tables hold
-static int tokens_per_block(int T) {
+// Tokens of one block: enough blocks for `resident` on every SM, and then as many tokens as the block's tables hold
+static int tokens_per_block(int T, int resident) {
   const int sms = sm_count() > 0 ? sm_count() : 1;
-  const int n = (T + 4 * sms - 1) / (4 * sms);
+  const int n = (T + resident * sms - 1) / (resident * sms);
   return n < 1 ? 1 : n > MAX_TOKENS ? MAX_TOKENS : n;
 }
 
@@ -284,8 +289,8 @@ static Side side_of(const void* x, const long long* xs, void* cache, const long 
 }
 
 template <typename A, typename Kern>
-static int start(Kern kern, A& a, cudaStream_t stream) {
-  a.per_block = tokens_per_block(a.T);
+static int start(Kern kern, A& a, int resident, cudaStream_t stream) {
+  a.per_block = tokens_per_block(a.T, resident);
   kern<<<(a.T + a.per_block - 1) / a.per_block, THREADS, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
@@ -296,54 +301,55 @@ static int start(Kern kern, A& a, cudaStream_t stream) {
 using namespace cm;
 using namespace cm::paged;
 
-// k [T, heads, dim] with strides ks (elements) of its first two axes, v likewise or null; caches [pages, page, heads, dim] with strides kcs, vcs
-// of their first three.  kind: 0 bf16, 1 fp16; e4m3: the caches hold E4M3 and k_scale, v_scale [pages, page, heads] their exponent bytes.  slots
-// [T] of 32 or (wide) 64 bits: place page * (slots of a page) + offset, negative: left out.  Widths are multiples of 8 up to 256, rows on 16
-// bytes (8 in an E4M3 cache).
-extern "C" int cm_cache_write(const void* k, const long long* ks, const void* v, const long long* vs, void* kc, const long long* kcs, void* vc,
-                              const long long* vcs, void* k_scale, void* v_scale, const void* slots, int wide, int T, int heads, int dim,
-                              int vdim, int pages, int page, int kind, int e4m3, int* err, cudaStream_t stream) {
-  if (T <= 0 || heads <= 0) return 0;
-  if (dim < 8 || dim % 8 || dim > 256 || (v && (vdim < 8 || vdim % 8 || vdim > 256)) || page < 1 || pages < 0) return -10;
-  if (e4m3 && (!k_scale || (v && !v_scale))) return -10;
-  WriteArgs a;
-  a.side[0] = side_of(k, ks, kc, kcs, k_scale, dim, e4m3 ? 1 : 2);
+// Sizes and strides come in one array of 64-bit numbers, strides in elements:
+//   k_tok, k_head, v_tok, v_head of the packed rows; page, token and head strides of the key cache, then of the value cache;
+//   T, heads, dim, vdim (0: no values), pages, page, kind (0 bf16, 1 fp16), e4m3, then what the function says.
+// Packed rows k [T, heads, dim], v [T, heads, vdim]; caches [pages, page, heads, .]; with e4m3 the caches hold E4M3 and k_scale, v_scale
+// [pages, page, heads] their exponent bytes.  Widths are multiples of 8 up to 256; rows on 16 bytes (8 in an E4M3 cache).
+template <typename A>
+static int common(A& a, void* k, void* v, void* kc, void* vc, void* k_scale, void* v_scale, const long long* n) {
+  const int es = n[17] ? 1 : 2, dim = (int)n[12], vdim = (int)n[13];
+  if (dim < 8 || dim % 8 || dim > 256 || vdim < 0 || vdim % 8 || vdim > 256 || n[15] < 1 || n[14] < 0) return -10;
+  if (n[17] && (!k_scale || (vdim && !v_scale))) return -10;
+  a.side[0] = side_of(k, n, kc, n + 4, k_scale, dim, es);
   a.sides = 1;
-  if (v) a.side[a.sides++] = side_of(v, vs, vc, vcs, v_scale, vdim, e4m3 ? 1 : 2);
-  a.slots = slots;
-  a.wide = wide;
-  a.total = (long long)pages * page;
-  a.T = T;
-  a.heads = heads;
-  a.page = page;
-  a.err = err;
-  if (kind == 0) return e4m3 ? start(cache_write_kernel<__nv_bfloat16, true>, a, stream) : start(cache_write_kernel<__nv_bfloat16, false>, a, stream);
-  return e4m3 ? start(cache_write_kernel<__half, true>, a, stream) : start(cache_write_kernel<__half, false>, a, stream);
+  if (vdim) a.side[a.sides++] = side_of(v, n + 2, vc, n + 7, v_scale, vdim, es);
+  a.T = (int)n[10];
+  a.heads = (int)n[11];
+  a.page = (int)n[15];
+  return 0;
 }
 
-// The other way: token t of the packed results (strides ks, vs) is the (t - ends[s])-th of the sequence s that holds it; tokens of no sequence
-// become zeros.  table [sequences, columns] of page numbers, table_row elements from row to row.
-extern "C" int cm_cache_read(void* k, const long long* ks, void* v, const long long* vs, const void* kc, const long long* kcs, const void* vc,
-                             const long long* vcs, const void* k_scale, const void* v_scale, const int* table, long long table_row,
-                             const int* ends, int sequences, int columns, int T, int heads, int dim, int vdim, int pages, int page, int kind,
-                             int e4m3, int* err, cudaStream_t stream) {
-  if (T <= 0 || heads <= 0) return 0;
-  if (dim < 8 || dim % 8 || dim > 256 || (v && (vdim < 8 || vdim % 8 || vdim > 256)) || page < 1 || sequences < 0) return -10;
-  if (e4m3 && (!k_scale || (v && !v_scale))) return -10;
-  ReadArgs a;
-  a.side[0] = side_of(k, ks, const_cast<void*>(kc), kcs, const_cast<void*>(k_scale), dim, e4m3 ? 1 : 2);
-  a.sides = 1;
-  if (v) a.side[a.sides++] = side_of(v, vs, const_cast<void*>(vc), vcs, const_cast<void*>(v_scale), vdim, e4m3 ? 1 : 2);
-  a.table = table;
-  a.table_row = table_row;
-  a.ends = ends;
-  a.sequences = sequences;
-  a.columns = columns;
-  a.pages = pages;
-  a.T = T;
-  a.heads = heads;
-  a.page = page;
+// Then: slots are 64-bit numbers.  slots [T]: page * (slots of a page) + offset, negative: left out.
+extern "C" int cm_cache_write(const void* k, const void* v, void* kc, void* vc, void* k_scale, void* v_scale, const void* slots, const long long* n,
+                              int* err, cudaStream_t stream) {
+  if (n[10] <= 0 || n[11] <= 0) return 0;
+  WriteArgs a;
+  const int rc = common(a, const_cast<void*>(k), const_cast<void*>(v), kc, vc, k_scale, v_scale, n);
+  if (rc) return rc;
+  a.slots = slots;
+  a.wide = (int)n[18];
+  a.total = n[14] * n[15];
   a.err = err;
-  if (kind == 0) return e4m3 ? start(cache_read_kernel<__nv_bfloat16, true>, a, stream) : start(cache_read_kernel<__nv_bfloat16, false>, a, stream);
-  return e4m3 ? start(cache_read_kernel<__half, true>, a, stream) : start(cache_read_kernel<__half, false>, a, stream);
+  if (n[16] == 0) return n[17] ? start(cache_write_kernel<__nv_bfloat16, true>, a, 4, stream) : start(cache_write_kernel<__nv_bfloat16, false>, a, 4, stream);
+  return n[17] ? start(cache_write_kernel<__half, true>, a, 4, stream) : start(cache_write_kernel<__half, false>, a, 4, stream);
+}
+
+// Then: elements between the rows of the table, sequences, columns of the table.  Token t of the packed results is the (t - ends[s])-th of the
+// sequence s that holds it; tokens of no sequence become zeros.
+extern "C" int cm_cache_read(void* k, void* v, const void* kc, const void* vc, const void* k_scale, const void* v_scale, const int* table,
+                             const int* ends, const long long* n, int* err, cudaStream_t stream) {
+  if (n[10] <= 0 || n[11] <= 0) return 0;
+  ReadArgs a;
+  const int rc = common(a, k, v, const_cast<void*>(kc), const_cast<void*>(vc), const_cast<void*>(k_scale), const_cast<void*>(v_scale), n);
+  if (rc) return rc;
+  a.table = table;
+  a.table_row = n[18];
+  a.ends = ends;
+  a.sequences = (int)n[19];
+  a.columns = (int)n[20];
+  a.pages = (int)n[14];
+  a.err = err;
+  if (n[16] == 0) return n[17] ? start(cache_read_kernel<__nv_bfloat16, true>, a, 8, stream) : start(cache_read_kernel<__nv_bfloat16, false>, a, 8, stream);
+  return n[17] ? start(cache_read_kernel<__half, true>, a, 8, stream) : start(cache_read_kernel<__half, false>, a, 8, stream);
 }

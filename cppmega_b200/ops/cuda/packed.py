@@ -8,23 +8,27 @@ import torch
 from .. import cuda as _cu
 from .. import functional as F_
 from .block import _Copied, _bare, _failed, _first_order, _given_back, _on_device, _ptr
-from .paged import TYPES, _rows_on, _strides, _width_ok
+from .paged import TYPES, Plan, planned, rows_on, strides, width_ok
 
 
 def declare(L: ctypes.CDLL) -> None:
     vp, i32, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
     sig = {
-        "cm_packed_attention_fwd": [vp] * 10 + [i32] * 7 + [f32, i32, vp, vp],
-        "cm_packed_attention_bwd": [vp] * 17 + [i32] * 7 + [f32, i32, vp, vp],
+        "cm_packed_attention_fwd": [vp] * 9 + [f32, vp, vp],
+        "cm_packed_attention_bwd": [vp] * 14 + [f32, vp, vp],
     }
     for name, args in sig.items():
         if hasattr(L, name):
             getattr(L, name).argtypes, getattr(L, name).restype = args, i32
 
 
-def _in_place(t: torch.Tensor) -> bool:
+def _strides_ok(t: torch.Tensor) -> bool:
     """Whether a tensor map can read the rows where they are: on 16 bytes, and no step of zero."""
-    return _rows_on(t, 16) and all(n == 1 or 0 < s < 2 ** 38 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    return rows_on(t, 16) and all(n == 1 or 0 < s < 2 ** 38 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+
+
+def _in_place(t: torch.Tensor) -> bool:
+    return t.data_ptr() % 16 == 0 and _strides_ok(t)
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
@@ -36,24 +40,37 @@ def _packed(t: torch.Tensor) -> torch.Tensor:
     return t if _in_place(t) else t.clone(memory_format=torch.contiguous_format)
 
 
-def _forward(q, k, v, cu_q, cu_k, scale, keep):
+def _numbers(q, k, v, cu_q, go=None):
     T, H, D = q.shape
-    o = torch.empty(T, H, v.shape[2], dtype=q.dtype, device=q.device)
-    lse = torch.empty(T, H, dtype=torch.float32, device=q.device) if keep else None
-    rc = _cu.lib().cm_packed_attention_fwd(
-        q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _ptr(lse),
-        cu_q.numel() - 1, T, k.shape[0], H, k.shape[1], D, v.shape[2], scale, TYPES[q.dtype], _cu.err_word(q.device).data_ptr(), _cu.stream_ptr())
+    return [*strides(q), *strides(k), *strides(v), *strides(go, 2), cu_q.numel() - 1, T, k.shape[0], H, k.shape[1], D, v.shape[2], TYPES[q.dtype]]
+
+
+def _plan(q, k, v, cu_q, cu_k):
+    if not (q.dtype in TYPES and width_ok(q, 8, 128) and width_ok(v, 8, 128) and 0 < q.shape[0] < 2 ** 30 and 0 < k.shape[0] < 2 ** 30
+            and q.shape[1] > 0):
+        return False
+    return Plan(_numbers(q, k, v, cu_q), shape=(q.shape[0], q.shape[1], v.shape[2]), like=q.is_contiguous() and q.shape[2] == v.shape[2],
+                copy=not (_strides_ok(q) and _strides_ok(k) and _strides_ok(v) and cu_q.is_contiguous() and (cu_k is None or cu_k.is_contiguous())))
+
+
+def _forward(plan, q, k, v, cu_q, cu_k, scale, keep):
+    dev = q.device
+    o = torch.empty_like(q) if plan.like else torch.empty(plan.shape, dtype=q.dtype, device=dev)
+    rest = torch.empty_like(o) if keep else None
+    lse = torch.empty(plan.shape[:2], dtype=torch.float32, device=dev) if keep else None
+    rc = _cu.lib().cm_packed_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _ptr(rest),
+                                           _ptr(lse), plan.at, scale, _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
     if rc:
         _failed("cm_packed_attention_fwd", rc)
     F_.count_launch("packed_attention")
-    return o, lse
+    return o, rest, lse
 
 
 class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, cu_q, cu_k, scale):
-        o, lse = _forward(q, k, v, cu_q, cu_k, scale, keep=True)
-        ctx.save_for_backward(q, k, v, cu_q, cu_k, o, lse)
+    def forward(ctx, q, k, v, cu_q, cu_k, scale, plan):
+        o, rest, lse = _forward(plan, q, k, v, cu_q, cu_k, scale, keep=True)
+        ctx.save_for_backward(q, k, v, cu_q, cu_k, o, rest, lse)
         ctx.scale, ctx.dtype = scale, q.dtype
         return o
 
@@ -61,39 +78,42 @@ class PackedAttentionFn(torch.autograd.Function):
     @_first_order
     def backward(ctx, go):
         dt, dev = ctx.dtype, go.device
-        q, k, v, cu_q, cu_k, o, lse = ctx.saved_tensors
-        q, k, v, o = (_packed(_given_back(t, dt, dev, packed=False)) for t in (q, k, v, o))
+        q, k, v, cu_q, cu_k, o, rest, lse = ctx.saved_tensors
+        q, k, v = (_packed(_given_back(t, dt, dev, packed=False)) for t in (q, k, v))
+        o, rest = (_given_back(t, dt, dev, align=16) for t in (o, rest))
         cu_q, cu_k = (_given_back(t, torch.int32, dev) for t in (cu_q, cu_k))
         lse = _given_back(lse, torch.float32, dev)
         go = _packed(go)
-        T, H, D = q.shape
-        Tk, G, V = v.shape
-        dq = torch.empty(T, H, D, dtype=dt, device=dev)
-        dk, dv = torch.empty(Tk, G, D, dtype=dt, device=dev), torch.empty(Tk, G, V, dtype=dt, device=dev)
-        delta = torch.empty(T * H + 1, dtype=torch.float32, device=dev)
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+        delta = torch.empty(lse.numel() + 1, dtype=torch.float32, device=dev)
+        plan = planned((F_.layout_of("packed_attention_bwd", q, k, v, go, cu_q)), lambda: Plan(_numbers(q, k, v, cu_q, go)))
         rc = _cu.lib().cm_packed_attention_bwd(
-            q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), o.data_ptr(), _strides(o), go.data_ptr(), _strides(go),
-            cu_q.data_ptr(), cu_k.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu_q.numel() - 1, T, Tk,
-            H, G, D, V, ctx.scale, TYPES[dt], _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(), go.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
+            lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), plan.at, ctx.scale,
+            _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
         if rc:
             _failed("cm_packed_attention_bwd", rc)
         F_.count_launch("packed_attention_bwd", 2)
-        return dq, dk, dv, None, None, None
+        return dq, dk, dv, None, None, None, None
 
 
 @_on_device
-def packed_attention(q, k, v, cu_q, scale, cu_k):
+def packed_attention(q, k, v, cu_q, scale, cu_k, layout):
     """None where the kernels do not apply."""
-    if not (q.dtype in TYPES and not isinstance(scale, torch.Tensor) and _bare(q, k, v, cu_q, cu_k) and _width_ok(q, 8, 128) and _width_ok(v, 8, 128)
-            and 0 < q.shape[0] < 2 ** 30 and 0 < k.shape[0] < 2 ** 30 and q.shape[1] > 0 and abs(scale) < 2.0 ** 64):
+    plan = planned(layout, lambda: _plan(q, k, v, cu_q, cu_k))
+    if not plan or isinstance(scale, torch.Tensor) or not abs(scale) < 2.0 ** 64 or not _bare(q, k, v, cu_q, cu_k):
         return None
-    cu_q = cu_q.contiguous()
-    cu_k = cu_q if cu_k is None else cu_k.contiguous()
-    if scale < 0:          # the kernels take the largest product of a row for its reference: the sign goes into q, exactly
-        q, scale = -q, -scale
+    if scale < 0 or plan.copy or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        if scale < 0:      # the kernels take the largest product of a row for its reference: the sign goes into q, exactly
+            q, scale = -q, -scale
+        q, k, v, cu_q = _readable(q), _readable(k), _readable(v), cu_q.contiguous()
+        cu_k = None if cu_k is None else cu_k.contiguous()
+        return packed_attention(q, k, v, cu_q, scale, cu_k, F_.layout_of("packed_attention", q, k, v, cu_q, cu_k))
+    if cu_k is None:
+        cu_k = cu_q
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return PackedAttentionFn.apply(_readable(q), _readable(k), _readable(v), cu_q, cu_k, float(scale))
-    return _forward(_packed(q), _packed(k), _packed(v), cu_q, cu_k, float(scale), keep=False)[0]
+        return PackedAttentionFn.apply(q, k, v, cu_q, cu_k, float(scale), plan)
+    return _forward(plan, q, k, v, cu_q, cu_k, float(scale), keep=False)[0]
 
 
 def register() -> None:

@@ -2,6 +2,9 @@
 
 Tensors are read where they are: strides of a cache are free as long as a row (the last axis) is contiguous and lies on 16 bytes.
 Work space is allocated per call on the current stream, and nothing waits for the device.
+
+A call's sizes and strides, as the library takes them, are worked out once per layout (shapes, strides, types, devices) and kept: a step of
+generation makes the same call again and again, and on the host its checks would cost more than its kernels do on the device.
 """
 from __future__ import annotations
 
@@ -20,9 +23,9 @@ E4M3 = torch.float8_e4m3fn
 def declare(L: ctypes.CDLL) -> None:
     vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
     sig = {
-        "cm_cache_write": [vp] * 11 + [i32] * 9 + [vp, vp],
-        "cm_cache_read": [vp] * 11 + [i64, vp] + [i32] * 10 + [vp, vp],
-        "cm_paged_attention": [vp] * 9 + [i64, vp, vp, vp] + [i32] * 8 + [f32, i32, i32, vp, vp],
+        "cm_cache_write": [vp] * 10,
+        "cm_cache_read": [vp] * 11,
+        "cm_paged_attention": [vp] * 10 + [f32, vp, vp],
     }
     for name, args in sig.items():
         if hasattr(L, name):
@@ -31,25 +34,43 @@ def declare(L: ctypes.CDLL) -> None:
         L.cm_paged_attention_ws.argtypes, L.cm_paged_attention_ws.restype = [i32] * 7, i64
 
 
-def _strides(t):
-    """Strides of all axes but the last, as the library takes them."""
-    return None if t is None else (ctypes.c_longlong * (t.dim() - 1))(*t.stride()[:-1])
+class Plan:
+    """What a layout's calls have in common: the library's array of sizes and strides, and what else the wrapper needs."""
+
+    __slots__ = ("numbers", "at", "copy", "shape", "work", "like")
+
+    def __init__(self, numbers, copy=False, shape=None, work=0, like=False):
+        self.numbers = (ctypes.c_longlong * len(numbers))(*numbers)
+        self.at = ctypes.addressof(self.numbers)
+        self.copy, self.shape, self.work, self.like = copy, shape, work, like
 
 
-def _rows_on(t, align: int) -> bool:
-    """Whether every row of the tensor is contiguous and begins on ``align`` bytes."""
+_plans: dict = {}
+
+
+def planned(layout, make):
+    """The plan of a layout, or False where the kernels do not apply."""
+    plan = _plans.get(layout)
+    if plan is None:
+        if len(_plans) >= 4096:
+            _plans.clear()
+        plan = _plans[layout] = make()
+    return plan
+
+
+def strides(t, n=None):
+    return list(t.stride()[:-1]) if t is not None else [0] * n
+
+
+def rows_on(t, align: int) -> bool:
+    """Whether every row of the tensor is contiguous and lies on ``align`` bytes, as far as the strides go."""
     if t is None:
         return True
     es = t.element_size()
-    return (t.shape[-1] == 1 or t.stride(-1) == 1) and t.data_ptr() % align == 0 and all(s * es % align == 0 for s in t.stride()[:-1])
+    return (t.shape[-1] == 1 or t.stride(-1) == 1) and all(s * es % align == 0 for s in t.stride()[:-1])
 
 
-def _packed_rows(t, align: int = 16):
-    """A few rows: copied where the kernels cannot read them in place."""
-    return t if t is None or _rows_on(t, align) else t.clone(memory_format=torch.contiguous_format)
-
-
-def _width_ok(t, step: int, most: int) -> bool:
+def width_ok(t, step: int, most: int) -> bool:
     return t is None or (t.shape[-1] % step == 0 and step <= t.shape[-1] <= most)
 
 
@@ -58,82 +79,111 @@ def _scales(t):
     return t is None or t.is_contiguous()
 
 
-@_on_device
-def cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale) -> bool:
-    """False where the kernel does not apply."""
+def _caches_ok(k_cache, v_cache, k_scale, v_scale, align, step, most):
+    return (rows_on(k_cache, align) and rows_on(v_cache, align) and width_ok(k_cache, step, most) and width_ok(v_cache, step, most)
+            and _scales(k_scale) and _scales(v_scale) and k_cache.shape[0] < 2 ** 31 and k_cache.shape[1] < 2 ** 31)
+
+
+def _plan_write(k, v, k_cache, v_cache, slots, k_scale, v_scale):
     q = k_cache.dtype == E4M3
-    if not (k.dtype in TYPES and _bare(k, v, k_cache, v_cache, slots) and _width_ok(k, 8, 256) and _width_ok(v, 8, 256)
-            and _rows_on(k_cache, 8 if q else 16) and _rows_on(v_cache, 8 if q else 16) and _scales(k_scale) and _scales(v_scale)
-            and k.shape[0] * max(1, k.shape[1]) < 2 ** 30 and k_cache.shape[0] < 2 ** 31 and k_cache.shape[1] < 2 ** 31):
-        return False
     T, heads, dim = k.shape
-    if T == 0 or heads == 0:
-        return True
-    k, v, slots = _packed_rows(k.detach()), _packed_rows(None if v is None else v.detach()), slots.contiguous()
-    rc = _cu.lib().cm_cache_write(
-        k.data_ptr(), _strides(k), _ptr(v), _strides(v), k_cache.data_ptr(), _strides(k_cache), _ptr(v_cache), _strides(v_cache),
-        _ptr(k_scale), _ptr(v_scale), slots.data_ptr(), int(slots.dtype == torch.int64), T, heads, dim, 0 if v is None else v.shape[2],
-        k_cache.shape[0], k_cache.shape[1], TYPES[k.dtype], int(q), _cu.err_word(k.device).data_ptr(), _cu.stream_ptr())
+    if not (k.dtype in TYPES and _caches_ok(k_cache, v_cache, k_scale, v_scale, 8 if q else 16, 8, 256) and T * max(1, heads) < 2 ** 30):
+        return False
+    return Plan([*strides(k), *strides(v, 2), *strides(k_cache), *strides(v_cache, 3), T, heads, dim, 0 if v is None else v.shape[2],
+                 k_cache.shape[0], k_cache.shape[1], TYPES[k.dtype], int(q), int(slots.dtype == torch.int64)],
+                copy=not (rows_on(k, 16) and rows_on(v, 16) and slots.is_contiguous()))
+
+
+@_on_device
+def cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout) -> bool:
+    """False where the kernel does not apply."""
+    plan = planned(layout, lambda: _plan_write(k, v, k_cache, v_cache, slots, k_scale, v_scale))
+    if not plan or not _bare(k, v, k_cache, v_cache, slots, k_scale, v_scale):
+        return False
+    at, kp, vp, kcp, vcp = slots.data_ptr(), k.data_ptr(), _ptr(v), k_cache.data_ptr(), _ptr(v_cache)
+    if (kcp | (vcp or 0)) & (7 if k_scale is not None else 15):
+        return False
+    if plan.copy or (kp | (vp or 0)) & 15:                # a few rows
+        k, v = (None if t is None else t.detach().clone(memory_format=torch.contiguous_format) for t in (k, v))
+        slots = slots.contiguous()
+        return cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, F_.layout_of("cache_write", k, v, k_cache, v_cache, slots, k_scale, v_scale))
+    rc = _cu.lib().cm_cache_write(kp, vp, kcp, vcp, _ptr(k_scale), _ptr(v_scale), at, plan.at, _cu.err_word(k.device).data_ptr(), _cu.stream_ptr())
     if rc:
         _failed("cm_cache_write", rc)
     F_.count_launch("cache_write")
     return True
 
 
-@_on_device
-def cache_read(k_cache, v_cache, table, ends, total, k_scale, v_scale, dtype):
-    """None where the kernel does not apply."""
+def _plan_read(k_cache, v_cache, table, ends, total, k_scale, v_scale, dtype):
     q = k_cache.dtype == E4M3
-    heads = k_cache.shape[2]
-    if not (dtype in TYPES and _bare(k_cache, v_cache, table, ends) and _width_ok(k_cache, 8, 256) and _width_ok(v_cache, 8, 256)
-            and _rows_on(k_cache, 8 if q else 16) and _rows_on(v_cache, 8 if q else 16) and _scales(k_scale) and _scales(v_scale)
-            and not (torch.is_grad_enabled() and (k_cache.requires_grad or (v_cache is not None and v_cache.requires_grad)))
-            and total * max(1, heads) < 2 ** 30 and k_cache.shape[0] < 2 ** 31):
+    heads, dim, vdim = k_cache.shape[2], k_cache.shape[3], 0 if v_cache is None else v_cache.shape[3]
+    if not (dtype in TYPES and _caches_ok(k_cache, v_cache, k_scale, v_scale, 8 if q else 16, 8, 256) and total * max(1, heads) < 2 ** 30):
+        return False
+    return Plan([heads * dim, dim, heads * vdim, vdim, *strides(k_cache), *strides(v_cache, 3), total, heads, dim, vdim, k_cache.shape[0],
+                 k_cache.shape[1], TYPES[dtype], int(q), table.stride(0), table.shape[0], table.shape[1]],
+                copy=not ((table.stride(-1) == 1 or table.shape[1] <= 1) and ends.is_contiguous()),
+                shape=((total, heads, dim), (total, heads, vdim)))
+
+
+@_on_device
+def cache_read(k_cache, v_cache, table, ends, total, k_scale, v_scale, dtype, layout):
+    """None where the kernel does not apply."""
+    plan = planned(layout, lambda: _plan_read(k_cache, v_cache, table, ends, total, k_scale, v_scale, dtype))
+    if (not plan or not _bare(k_cache, v_cache, table, ends, k_scale, v_scale)
+            or (torch.is_grad_enabled() and (k_cache.requires_grad or (v_cache is not None and v_cache.requires_grad)))):
         return None
-    k = torch.empty(total, heads, k_cache.shape[3], dtype=dtype, device=k_cache.device)
-    v = None if v_cache is None else torch.empty(total, heads, v_cache.shape[3], dtype=dtype, device=k_cache.device)
-    if total == 0 or heads == 0:
-        return k, v
-    if table.stride(-1) != 1:
-        table = table.contiguous()
-    ends = ends.contiguous()
-    rc = _cu.lib().cm_cache_read(
-        k.data_ptr(), _strides(k), _ptr(v), _strides(v), k_cache.data_ptr(), _strides(k_cache), _ptr(v_cache), _strides(v_cache),
-        _ptr(k_scale), _ptr(v_scale), table.data_ptr(), table.stride(0), ends.data_ptr(), table.shape[0], table.shape[1], total, heads,
-        k.shape[2], 0 if v is None else v.shape[2], k_cache.shape[0], k_cache.shape[1], TYPES[dtype], int(q),
-        _cu.err_word(k.device).data_ptr(), _cu.stream_ptr())
+    kcp, vcp = k_cache.data_ptr(), _ptr(v_cache)
+    if (kcp | (vcp or 0)) & (7 if k_scale is not None else 15):
+        return None
+    if plan.copy:
+        table, ends = table.contiguous(), ends.contiguous()
+        layout = (F_.layout_of("cache_read", k_cache, v_cache, table, ends, k_scale, v_scale), total, dtype)
+        return cache_read(k_cache, v_cache, table, ends, total, k_scale, v_scale, dtype, layout)
+    dev = k_cache.device
+    k = torch.empty(plan.shape[0], dtype=dtype, device=dev)
+    v = None if v_cache is None else torch.empty(plan.shape[1], dtype=dtype, device=dev)
+    rc = _cu.lib().cm_cache_read(k.data_ptr(), _ptr(v), kcp, vcp, _ptr(k_scale), _ptr(v_scale), table.data_ptr(), ends.data_ptr(), plan.at,
+                                 _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
     if rc:
         _failed("cm_cache_read", rc)
     F_.count_launch("cache_read")
     return k, v
 
 
-@_on_device
-def paged_attention(q, k_cache, v_cache, table, lens, scale, k_scale, v_scale):
-    """None where the kernels do not apply."""
+def _plan_attention(q, k_cache, v_cache, table, lens, k_scale, v_scale):
     e4m3 = k_cache.dtype == E4M3
     B, H, dim = q.shape
     pages, page, heads, vdim = v_cache.shape
-    step = 16 if e4m3 else 8
-    if not (q.dtype in TYPES and (e4m3 or k_cache.dtype == q.dtype) and not isinstance(scale, torch.Tensor)
-            and _bare(q, k_cache, v_cache, table, lens) and _width_ok(k_cache, step, 128) and _width_ok(v_cache, step, 128)
-            and H // heads <= 128 and _rows_on(k_cache, 16) and _rows_on(v_cache, 16) and _scales(k_scale) and _scales(v_scale)
-            and table.shape[1] * page < 2 ** 31 - 16 and B * H < 2 ** 31 and pages < 2 ** 31):
+    group, columns = H // heads, table.shape[1]
+    if not (q.dtype in TYPES and (e4m3 or k_cache.dtype == q.dtype) and _caches_ok(k_cache, v_cache, k_scale, v_scale, 16, 16 if e4m3 else 8, 128)
+            and 0 < group <= 128 and columns * page < 2 ** 31 - 16 and B * H < 2 ** 31):
+        return False
+    return Plan([*strides(q), *strides(k_cache), *strides(v_cache), table.stride(0), B, heads, group, columns, pages, page, dim, vdim,
+                 TYPES[q.dtype], int(e4m3)],
+                copy=not (rows_on(q, 16) and (table.stride(-1) == 1 or columns <= 1) and lens.is_contiguous()), shape=(B, H, vdim),
+                work=_cu.lib().cm_paged_attention_ws(B, heads, group, dim, vdim, columns, page) if B else 0,
+                like=q.is_contiguous() and vdim == dim)
+
+
+@_on_device
+def paged_attention(q, k_cache, v_cache, table, lens, scale, k_scale, v_scale, layout):
+    """None where the kernels do not apply."""
+    plan = planned(layout, lambda: _plan_attention(q, k_cache, v_cache, table, lens, k_scale, v_scale))
+    if (not plan or isinstance(scale, torch.Tensor) or not _bare(q, k_cache, v_cache, table, lens, k_scale, v_scale)
+            or (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad))):
         return None
-    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+    qp, kp, vp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    if (kp | vp) & 15:
         return None
-    out = torch.empty(B, H, vdim, dtype=q.dtype, device=q.device)
-    if B == 0 or H == 0:
-        return out
-    q, lens = _packed_rows(q), lens.contiguous()
-    if table.stride(-1) != 1:
-        table = table.contiguous()
-    L, group, columns = _cu.lib(), H // heads, table.shape[1]
-    ws = torch.empty(L.cm_paged_attention_ws(B, heads, group, dim, vdim, columns, page), dtype=torch.float32, device=q.device)
-    rc = L.cm_paged_attention(
-        q.data_ptr(), _strides(q), k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(), _strides(v_cache), _ptr(k_scale), _ptr(v_scale),
-        table.data_ptr(), table.stride(0), lens.data_ptr(), out.data_ptr(), ws.data_ptr(), B, heads, group, columns, pages, page, dim, vdim,
-        float(scale), TYPES[q.dtype], int(e4m3), _cu.err_word(q.device).data_ptr(), _cu.stream_ptr())
+    if plan.copy or qp & 15:
+        q, table, lens = q.clone(memory_format=torch.contiguous_format), table.contiguous(), lens.contiguous()
+        return paged_attention(q, k_cache, v_cache, table, lens, scale, k_scale, v_scale,
+                               F_.layout_of("paged_attention", q, k_cache, v_cache, table, lens, k_scale, v_scale))
+    dev = q.device
+    out = torch.empty_like(q) if plan.like else torch.empty(plan.shape, dtype=q.dtype, device=dev)
+    ws = torch.empty(plan.work, dtype=torch.float32, device=dev)
+    rc = _cu.lib().cm_paged_attention(qp, kp, vp, _ptr(k_scale), _ptr(v_scale), table.data_ptr(), lens.data_ptr(), out.data_ptr(), ws.data_ptr(),
+                                      plan.at, float(scale), _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
     if rc:
         _failed("cm_paged_attention", rc)
     F_.count_launch("paged_attention")

@@ -441,10 +441,42 @@ def causal_attention_library(q, k, v, scale: float):
     return o.transpose(1, 2)[..., :dv]
 
 
+_CHECKED: set = set()
+
+
+def layout_of(name: str, *tensors):
+    """Everything about a call's tensors but their addresses and values: what its checks and its plan go by."""
+    return (name, *[None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors])
+
+
+def _checked(layout) -> None:
+    """Calls of this layout pass their checks."""
+    if len(_CHECKED) >= 4096:
+        _CHECKED.clear()
+    _CHECKED.add(layout)
+
+
 def _sequence_ends(name: str, ends, like: torch.Tensor) -> None:
     if ends.dtype != torch.int32 or ends.dim() != 1 or ends.numel() < 1:
         raise ValueError(f"{name}: sequence ends are int32 [sequences + 1], got {ends.dtype} {tuple(ends.shape)}")
     _same_device(name, like, ends)
+
+
+def _check_packed(q, k, v, cu_seqlens, cu_seqlens_k) -> None:
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape[:2] != v.shape[:2] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"packed_attention: {q.shape[1]} query heads over {k.shape[1]} key heads")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError(f"packed_attention: q {q.dtype}, k {k.dtype}, v {v.dtype}")
+    _same_device("packed_attention", q, k, v)
+    _sequence_ends("packed_attention", cu_seqlens, q)
+    if cu_seqlens_k is not None:
+        _sequence_ends("packed_attention", cu_seqlens_k, q)
+        if cu_seqlens_k.shape != cu_seqlens.shape:
+            raise ValueError(f"packed_attention: {cu_seqlens.numel() - 1} sequences of queries, {cu_seqlens_k.numel() - 1} of keys")
+    elif k.shape[0] != q.shape[0]:
+        raise ValueError(f"packed_attention: {q.shape[0]} queries and {k.shape[0]} keys without cu_seqlens_k")
 
 
 def packed_attention(q, k, v, cu_seqlens, scale: float, cu_seqlens_k=None):
@@ -461,23 +493,13 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, cu_seqlens_k=None):
     derivatives; the same call gives the same bits); strided tensors are read in place where rows lie on 16 bytes.
     Anything else, forward mode and function transforms run the definition, ``reference.packed_attention``.  No call waits for the device: ends
     that fall or run over the buffer are reported by ``ops.cuda.check_errors``."""
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k.shape[:2] != v.shape[:2] or q.shape[2] != k.shape[2]:
-        raise ValueError(f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"packed_attention: {q.shape[1]} query heads over {k.shape[1]} key heads")
-    if q.dtype != k.dtype or q.dtype != v.dtype:
-        raise ValueError(f"packed_attention: q {q.dtype}, k {k.dtype}, v {v.dtype}")
-    _same_device("packed_attention", q, k, v)
-    _sequence_ends("packed_attention", cu_seqlens, q)
-    if cu_seqlens_k is not None:
-        _sequence_ends("packed_attention", cu_seqlens_k, q)
-        if cu_seqlens_k.shape != cu_seqlens.shape:
-            raise ValueError(f"packed_attention: {cu_seqlens.numel() - 1} sequences of queries, {cu_seqlens_k.numel() - 1} of keys")
-    elif k.shape[0] != q.shape[0]:
-        raise ValueError(f"packed_attention: {q.shape[0]} queries and {k.shape[0]} keys without cu_seqlens_k")
+    layout = layout_of("packed_attention", q, k, v, cu_seqlens, cu_seqlens_k)
+    if layout not in _CHECKED:
+        _check_packed(q, k, v, cu_seqlens, cu_seqlens_k)
+        _checked(layout)
     fn = _cuda("packed_attention", q)
     if fn is not None:
-        o = fn(q, k, v, cu_seqlens, scale, cu_seqlens_k)
+        o = fn(q, k, v, cu_seqlens, scale, cu_seqlens_k, layout)
         if o is not None:
             return o
         _miss("packed_attention(shape/dtype)", q)
@@ -507,16 +529,7 @@ def _check_table(name: str, table, sequences: int, k_cache) -> None:
     _same_device(name, k_cache, table)
 
 
-def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> None:
-    """Writes the keys ``k`` [T, G, D] and values ``v`` [T, G, Dv] of new tokens into a paged cache ``k_cache`` [pages, page, G, D], ``v_cache``
-    [pages, page, G, Dv], in place.  ``slots`` [T] (int32 or int64): page number times page size plus place in the page; a negative slot is
-    left out (padding), of equal slots the last token's row stays.  ``v`` and ``v_cache`` may both be None (values that are columns of the
-    key rows).
-
-    A ``float8_e4m3fn`` cache holds each row divided by a power of two, whose exponent byte (127 + exponent, as in MXFP8) goes to ``k_scale``,
-    ``v_scale`` (uint8 [pages, page, G]): the smallest with which the row's largest finite magnitude is at most 448; values that are not
-    finite become NaN.  A 16-bit cache holds the rows as they are.  Values only: no gradient passes through a cache.  A slot behind the
-    cache's end is skipped and reported by ``ops.cuda.check_errors``."""
+def _check_write(k, v, k_cache, v_cache, slots, k_scale, v_scale) -> None:
     if (v is None) != (v_cache is None):
         raise ValueError("cache_write: values and their cache come together")
     _check_cache("cache_write", k_cache, v_cache, k_scale, v_scale)
@@ -527,16 +540,32 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> No
             raise ValueError(f"cache_write: rows {tuple(x.shape)} and slots {tuple(slots.shape)} for a cache of {tuple(cache.shape)}")
         if x.dtype != cache.dtype and cache.dtype != torch.float8_e4m3fn:
             raise ValueError(f"cache_write: rows of {x.dtype} into a cache of {cache.dtype}")
-        if cache.requires_grad:
-            raise ValueError("cache_write: a cache has no gradient")
     if v is not None and v.dtype != k.dtype:
         raise ValueError(f"cache_write: k {k.dtype}, v {v.dtype}")
     if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"cache_write: slots {slots.dtype} {tuple(slots.shape)}")
     _same_device("cache_write", k, v, k_cache, slots)
+
+
+def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> None:
+    """Writes the keys ``k`` [T, G, D] and values ``v`` [T, G, Dv] of new tokens into a paged cache ``k_cache`` [pages, page, G, D], ``v_cache``
+    [pages, page, G, Dv], in place.  ``slots`` [T] (int32 or int64): page number times page size plus place in the page; a negative slot is
+    left out (padding), of equal slots the last token's row stays.  ``v`` and ``v_cache`` may both be None (values that are columns of the
+    key rows).
+
+    A ``float8_e4m3fn`` cache holds each row divided by a power of two, whose exponent byte (127 + exponent, as in MXFP8) goes to ``k_scale``,
+    ``v_scale`` (uint8 [pages, page, G]): the smallest with which the row's largest finite magnitude is at most 448; values that are not
+    finite become NaN.  A 16-bit cache holds the rows as they are.  Values only: no gradient passes through a cache.  A slot behind the
+    cache's end is skipped and reported by ``ops.cuda.check_errors``."""
+    layout = layout_of("cache_write", k, v, k_cache, v_cache, slots, k_scale, v_scale)
+    if layout not in _CHECKED:
+        _check_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
+        _checked(layout)
+    if k_cache.requires_grad or (v_cache is not None and v_cache.requires_grad):
+        raise ValueError("cache_write: a cache has no gradient")
     fn = _cuda("cache_write", k)
     if fn is not None:
-        if fn(k, v, k_cache, v_cache, slots, k_scale, v_scale):
+        if fn(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout):
             return
         _miss("cache_write(shape/dtype)", k)
     with torch.no_grad():
@@ -550,9 +579,12 @@ def cache_read(k_cache, v_cache, block_table, cu_seqlens, total: int, k_scale=No
     ``v_cache`` may be None (then so is the second result).  ``dtype``: type of the rows (bf16 by default out of an E4M3 cache, whose
     rows are multiplied by their powers of two; a 16-bit cache keeps its own).  Pages outside the cache give rows of zeros and are reported
     by ``ops.cuda.check_errors``."""
-    _check_cache("cache_read", k_cache, v_cache, k_scale, v_scale)
-    _sequence_ends("cache_read", cu_seqlens, k_cache)
-    _check_table("cache_read", block_table, cu_seqlens.numel() - 1, k_cache)
+    layout = layout_of("cache_read", k_cache, v_cache, block_table, cu_seqlens, k_scale, v_scale)
+    if layout not in _CHECKED:
+        _check_cache("cache_read", k_cache, v_cache, k_scale, v_scale)
+        _sequence_ends("cache_read", cu_seqlens, k_cache)
+        _check_table("cache_read", block_table, cu_seqlens.numel() - 1, k_cache)
+        _checked(layout)
     if total < 0:
         raise ValueError(f"cache_read: {total} rows")
     if dtype is None:
@@ -561,11 +593,23 @@ def cache_read(k_cache, v_cache, block_table, cu_seqlens, total: int, k_scale=No
         raise ValueError(f"cache_read: a cache of {k_cache.dtype} read as {dtype}")
     fn = _cuda("cache_read", k_cache)
     if fn is not None:
-        out = fn(k_cache, v_cache, block_table, cu_seqlens, total, k_scale, v_scale, dtype)
+        out = fn(k_cache, v_cache, block_table, cu_seqlens, total, k_scale, v_scale, dtype, (layout, total, dtype))
         if out is not None:
             return out
         _miss("cache_read(shape/dtype)", k_cache)
     return ref.cache_read(k_cache, v_cache, block_table, cu_seqlens, total, k_scale, v_scale, dtype)
+
+
+def _check_paged(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale) -> None:
+    _check_cache("paged_attention", k_cache, v_cache, k_scale, v_scale)
+    if v_cache is None or q.dim() != 3 or q.shape[2] != k_cache.shape[3]:
+        raise ValueError(f"paged_attention: q {tuple(q.shape)} over caches {tuple(k_cache.shape)}, {None if v_cache is None else tuple(v_cache.shape)}")
+    if k_cache.shape[2] == 0 or q.shape[1] % k_cache.shape[2]:
+        raise ValueError(f"paged_attention: {q.shape[1]} query heads over {k_cache.shape[2]} key heads")
+    _check_table("paged_attention", block_table, q.shape[0], k_cache)
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != q.shape[:1]:
+        raise ValueError(f"paged_attention: lengths {seq_lens.dtype} {tuple(seq_lens.shape)} for {q.shape[0]} sequences (int32)")
+    _same_device("paged_attention", q, k_cache, seq_lens)
 
 
 def paged_attention(q, k_cache, v_cache, block_table, seq_lens, scale: float, k_scale=None, v_scale=None):
@@ -577,18 +621,13 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, scale: float, k_
     bf16 and fp16 queries with a cache of the same type or of E4M3, widths that are multiples of 8 (E4M3: 16) up to 128 and up to 128 heads a
     group run on the kernels; anything else, and calls that need a gradient, run the definition, ``reference.paged_attention``.
     Lengths outside the table and pages outside the cache are left out and reported by ``ops.cuda.check_errors``."""
-    _check_cache("paged_attention", k_cache, v_cache, k_scale, v_scale)
-    if v_cache is None or q.dim() != 3 or q.shape[2] != k_cache.shape[3]:
-        raise ValueError(f"paged_attention: q {tuple(q.shape)} over caches {tuple(k_cache.shape)}, {None if v_cache is None else tuple(v_cache.shape)}")
-    if k_cache.shape[2] == 0 or q.shape[1] % k_cache.shape[2]:
-        raise ValueError(f"paged_attention: {q.shape[1]} query heads over {k_cache.shape[2]} key heads")
-    _check_table("paged_attention", block_table, q.shape[0], k_cache)
-    if seq_lens.dtype != torch.int32 or seq_lens.shape != q.shape[:1]:
-        raise ValueError(f"paged_attention: lengths {seq_lens.dtype} {tuple(seq_lens.shape)} for {q.shape[0]} sequences (int32)")
-    _same_device("paged_attention", q, k_cache, seq_lens)
+    layout = layout_of("paged_attention", q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale)
+    if layout not in _CHECKED:
+        _check_paged(q, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale)
+        _checked(layout)
     fn = _cuda("paged_attention", q)
     if fn is not None:
-        o = fn(q, k_cache, v_cache, block_table, seq_lens, scale, k_scale, v_scale)
+        o = fn(q, k_cache, v_cache, block_table, seq_lens, scale, k_scale, v_scale, layout)
         if o is not None:
             return o
         _miss("paged_attention(shape/dtype)", q)
