@@ -5,21 +5,25 @@
 // where row j lies in page table[b, j / page], and an E4M3 cache holds rows divided by a power of two each.
 //
 // What bounds it: the cache is read once, and that is all of the time.  So every SM streams the same number of bytes without a pause:
-// the keys of all (sequence, key head) pairs form one sequence of steps of 16 keys, cut into equal runs, one per warp (lengths are known
-// on the device alone, so each warp adds them up for itself).  A warp works alone: no barrier, its own ring of asynchronous copies (24 KB a warp,
-// 192 KB an SM), its own running maximum and sum, its own accumulators.  Where a run ends inside a pair, the warp leaves its maximum, sum and
-// accumulators in a work space, and a second kernel joins them in a fixed order; a pair that lies inside one run is finished at once.
+// the keys of all sequences form one sequence of steps of 16 keys, cut into equal runs (lengths are known on the device alone, so each
+// warp adds them up for itself).  A run belongs to up to 16 neighbouring warps, one per key head: they read the same tokens at the same
+// time, so that memory is read in whole token rows.  A warp works alone: no barrier, its own ring of asynchronous copies (96 KB and
+// more on their way per SM), its own running maximum and sum, its own accumulators.  Where a run ends inside a pair, the warp leaves its maximum,
+// sum and accumulators in a work space, and a second kernel joins them in a fixed order; a pair that lies inside one run is finished at once.
 //
-// The products are 16 x 8 x 16 matrix instructions with the heads of a group as rows: with 4 to 16 heads a key, plain multiply-adds
-// would take longer than the memory does.  Any order of the summed index and any order of the value columns will do as long as both factors agree, so a
-// lane copies exactly the 16-byte pieces it needs for its fragments, in global order, and reads back only what it copied itself: no
-// transposition, no swizzle, no synchronisation inside a warp.  E4M3 becomes fp16 in one conversion per two values, exactly; the query is scaled to
-// fp16's range by a power of two per head, the key's power goes into the score, and the value's power into the exponent of its weight,
-// whose reference is a maximum of its own: weights never leave fp16's range, whatever the powers are.
+// The products are 16 x 8 x 16 matrix instructions with 16 keys (then 16 value columns) as rows and the heads of a group as columns, eight
+// at a time: S' = K q', o' = V' p'.  With the heads as rows, half of each instruction, of the exponentials and of the accumulators would belong
+// to nobody at 4 to 8 heads a key.  Any order of the summed index and any order of the value columns will do as long as both factors
+// agree, so a fragment is read from shared memory as the 16 bytes that lie together in a row.  A warp copies whole rows (a lane that copied its own fragments
+// would ask for 16 bytes each of four rows, and every sector of V came twice), to places from which both sides of the
+// exchange find their eight lanes in eight banks; the weights alone are transposed, 8 x 8 at a time.
+// E4M3 becomes fp16 in one conversion per two values, exactly; the query is scaled to fp16's range by a power of two per head, the key's power
+// goes into the score, and the value's power into the exponent of its weight, whose reference is a maximum of its own: weights never leave
+// fp16's range, whatever the powers are.
 // Weights are rounded to the type of the products (bf16 or fp16: half a step of the result's own type, averaged over the keys);
 // scores, maxima, sums and accumulators are fp32.
 //
-// The reference value of a row's softmax follows its maximum only when that has grown by 2^8, so that accumulators are rarely rescaled.
+// The reference value of a head's softmax follows its maximum only when that has grown by 2^8, so that accumulators are rarely rescaled.
 #include <cuda_fp16.h>
 
 #include "few_rows.cuh"
@@ -29,10 +33,9 @@ namespace cm {
 namespace paged {
 namespace {
 
-constexpr int WARPS = 8;
 constexpr int KEYS = 16;                     // keys of one step
-constexpr int WARP_BYTES = 24 * 1024;        // ring of one warp
-constexpr int SHORTEST_RUN = 4;              // steps: fewer would be all set-up, and more pieces to join
+constexpr int RING_BYTES = 192 * 1024;       // the rings of a block's warps
+constexpr int SHORTEST_RUN = 2;              // steps: fewer would be all set-up, and more pieces to join
 constexpr float RESCALE_AT = 8.f;            // log2
 
 struct Args {
@@ -48,6 +51,8 @@ struct Args {
   float* part;                               // pieces of [rows][DV + 4]: weights' sum, maximum, two unused, accumulators
   int sequences, kv_heads, group, columns, pages, page, dim, vdim;
   int runs, tiles, rows;                     // runs of the sequence of steps; head tiles of a group (1, 2, 4, 8); rows of a piece
+  int aligned;                               // a step lies inside one page
+  int side, chunks;                          // key heads of a run, and how often a sequence is gone through for all of them
   float scale_log2;
   int* err;
 };
@@ -57,11 +62,9 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-template <int BYTES>
 __device__ __forceinline__ void copy_piece(uint32_t dst, const uint8_t* src, bool there) {
-  const int n = there ? BYTES : 0;           // what is not there becomes zeros
-  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  // what is not there becomes zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -115,59 +118,86 @@ __device__ __forceinline__ int length_of(const Args& a, int b, bool& bad) {
 }
 __device__ __forceinline__ int steps_of(int len) { return (len + KEYS - 1) / KEYS; }
 
-// steps of all pairs, and the run length that cuts them; the same in every warp of both kernels
+// steps of all (sequence, chunk of key heads) pairs, and the run length that cuts them; the same in every warp of both kernels
 __device__ __forceinline__ long long all_steps(const Args& a, int lane, bool& bad) {
   long long n = 0;
   for (int b = lane; b < a.sequences; b += 32) n += steps_of(length_of(a, b, bad));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n * a.kv_heads;
+  return n * a.chunks;
 }
 __device__ __forceinline__ long long run_length(const Args& a, long long total) {
   const long long q = (total + a.runs - 1) / a.runs;
   return q < SHORTEST_RUN ? SHORTEST_RUN : q;
 }
 
-template <bool BF16, bool E4M3, int D, int DV>
+// Warps of a block (one block per SM): as many as its registers hold, with a ring of two steps or more for each.  Per thread: 16 query
+// registers and 4 DV / 16 accumulators for eight heads, and about 70 others.
+__host__ __device__ constexpr int warps_of(bool e4m3, int dim, int vdim, int nt) {
+  return nt == 4 ? 8 : nt == 2 ? 12 : (e4m3 ? dim + vdim : 2 * (dim + vdim)) > 384 ? 12 : 16;
+}
+
+template <bool BF16, bool E4M3, int D, int DV, int NT>
 struct Form {
+  static constexpr int WARPS = warps_of(E4M3, D, DV, NT);
   static constexpr bool MMA_BF16 = BF16 && !E4M3;
   static constexpr int K_ROW = E4M3 ? D : 2 * D, V_ROW = E4M3 ? DV : 2 * DV;       // bytes
   static constexpr int K_PIECES = K_ROW / 64;                 // 16-byte pieces of a key row to a lane (4 lanes a row)
   static constexpr int V_BYTES = V_ROW / 8 < 16 ? 8 : 16;     // a piece of a value row (8 lanes a row)
   static constexpr int V_PIECES = V_ROW / 8 / V_BYTES;
   static constexpr int STAGE = KEYS * (K_ROW + V_ROW);
-  static constexpr int STAGES = WARP_BYTES / STAGE > 6 ? 6 : WARP_BYTES / STAGE;
+  static constexpr int FIT = RING_BYTES / WARPS / STAGE;
+  static constexpr int STAGES = FIT > 6 ? 6 : FIT;
   static constexpr int SPAN = V_BYTES / (E4M3 ? 1 : 2);       // neighbouring value columns of a lane's piece
   static constexpr int RING = STAGES * STAGE + (E4M3 ? STAGES * KEYS * 8 : 0);
+  static_assert(STAGES >= 2 && WARPS * RING <= 227 * 1024, "a ring of two steps or more");
 };
 
 // A place in the sequence of steps
 struct Place {
-  int b, h, step, steps, len;
+  int b, c, step, steps, len;                // sequence, chunk of its key heads
 };
 __device__ __forceinline__ void advance(const Args& a, Place& p, bool& bad) {
   if (++p.step < p.steps) return;
   p.step = 0;
-  if (++p.h < a.kv_heads) return;
-  p.h = 0;
+  if (++p.c < a.chunks) return;
+  p.c = 0;
   do {
     if (++p.b >= a.sequences) { p.steps = p.len = 0; return; }
     p.len = length_of(a, p.b, bad);
     p.steps = steps_of(p.len);
   } while (p.steps == 0);
 }
+// 8 x 8 values of 16 bits (row = lane / 4, two columns a lane) -> their transpose
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// over the eight lanes that hold the keys of one pair of heads
+__device__ __forceinline__ float max8(float t) {
+  t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+  t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+  return fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+}
+__device__ __forceinline__ float sum8(float t) {
+  t += __shfl_xor_sync(0xffffffffu, t, 4);
+  t += __shfl_xor_sync(0xffffffffu, t, 8);
+  return t + __shfl_xor_sync(0xffffffffu, t, 16);
+}
 
-// BF16: type of the query and the result (fp16 otherwise; a 16-bit cache has the same); MT: 16-row tiles of heads that a warp multiplies
-template <bool BF16, bool E4M3, int D, int DV, int MT>
-__global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Args a) {
-  using F = Form<BF16, E4M3, D, DV>;
+// BF16: type of the query and the result (fp16 otherwise; a 16-bit cache has the same); NT: tiles of eight heads that a warp multiplies
+template <bool BF16, bool E4M3, int D, int DV, int NT>
+__global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_attention_kernel(const Args a) {
+  using F = Form<BF16, E4M3, D, DV, NT>;
   constexpr bool MB = F::MMA_BF16;
-  constexpr int VT = DV / 8;                                  // 8-column tiles of the result
+  constexpr int VT = DV / 16;                                 // 16-column tiles of the result
   extern __shared__ __align__(128) uint8_t smem_raw[];
   few::let_next_start();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, row8 = lane >> 2;
-  const int worker = blockIdx.x * WARPS + warp, run = worker / a.tiles, tile = worker % a.tiles;
-  const int head0 = tile * 16 * MT;                           // first head of this warp inside its group
+  const int worker = blockIdx.x * F::WARPS + warp, lanes_of_run = a.side * a.tiles, run = worker / lanes_of_run;
+  const int side = worker % lanes_of_run / a.tiles, tile = worker % a.tiles;
+  const int head0 = tile * 8 * NT;                            // first head of this warp inside its group
   if (head0 >= a.group || run >= a.runs) return;
   bool bad = false;
   const long long total = all_steps(a, lane, bad), q = run_length(a, total), begin = run * q;
@@ -181,7 +211,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Ar
     long long before = 0;                                     // steps of the sequences before a chunk of 32
     for (int b0 = 0;; b0 += 32) {
       const int len = b0 + lane < a.sequences ? length_of(a, b0 + lane, bad) : 0;
-      const long long mine = (long long)steps_of(len) * a.kv_heads;
+      const long long mine = (long long)steps_of(len) * a.chunks;
       long long upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -195,8 +225,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Ar
         at.len = __shfl_sync(0xffffffffu, len, src);
         at.steps = steps_of(at.len);
         at.b = b0 + src;
-        at.h = (int)(off / at.steps);
-        at.step = (int)(off - (long long)at.h * at.steps);
+        at.c = (int)(off / at.steps);
+        at.step = (int)(off - (long long)at.c * at.steps);
         break;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
@@ -210,54 +240,80 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Ar
   // ---- copies, STAGES - 1 steps ahead ----
   Place to = at;
   int left = count;                                           // steps not yet issued
-  auto page_at = [&](const Place& p) {                        // lane < 16: the page of that key
-    const int pos = p.step * KEYS + lane;
-    return lane < KEYS && pos < p.len ? __ldg(a.table + p.b * a.table_row + pos / a.page) : -1;
+  int col = 0, in = 0, page = -1;                             // table column, place in the page, page: of the step's first key, or of key `lane`
+  auto find_page = [&]() {                                    // for a place reached by a jump
+    const int pos = to.step * KEYS + (a.aligned ? 0 : lane & 15);
+    col = pos / a.page;
+    in = pos - col * a.page;
   };
-  int page = page_at(to);
+  auto load_page = [&]() {
+    page = to.step * KEYS + (a.aligned ? 0 : lane & 15) < to.len ? __ldg(a.table + to.b * a.table_row + col) : -1;
+  };
+  find_page();
+  load_page();
+  constexpr int KC = F::K_ROW / 16, VC = F::V_ROW / 16;       // 16-byte pieces of a row; 32 / KC rows to an instruction
+  const int kc = lane % KC, kr = lane / KC, vc = lane % VC, vr = lane / VC;
+  const bool k_exists = kc * 16 < a.dim * (E4M3 ? 1 : 2), v_exists = vc * 16 < a.vdim * (E4M3 ? 1 : 2);
+  // where the copies go: K by (eight keys, piece of four lanes), V by (row of a lane's fragment, piece of eight lanes)
+  const uint32_t k_dst = (kc >> 2) * 512 + ((kr * 4 + (kc & 3)) ^ ((kc >> 2 & 1) * 4)) * 16;
+  auto v_dst = [&](int i) {
+    const int key = i * (32 / VC) + vr, quad_of = key >> 1 & 3, y = (key & 1) | (key >> 3 << 1);
+    return F::V_BYTES == 16 ? ((y * F::V_PIECES + (vc >> 3)) * 32 + quad_of * 8 + ((vc & 7) ^ (2 * quad_of))) * 16
+                            : y * 256 + ((vc >> 1) * 8 + quad_of * 2 + (vc & 1)) * 16;
+  };
   auto issue = [&](int stage) {
     if (left > 0) {
-      const int pos = to.step * KEYS + lane;
-      long long ko = -1, vo = -1;
-      if (lane < KEYS && pos < to.len) {
-        if (page >= 0 && page < a.pages) {
-          const int in = pos % a.page;
-          ko = page * a.k_page + in * a.k_tok + to.h * a.k_head;
-          vo = page * a.v_page + in * a.v_tok + to.h * a.v_head;
-          if (E4M3) rows_of[stage * KEYS + lane] = ((long long)page * a.page + in) * a.kv_heads + to.h;
-        } else {
-          if (E4M3) rows_of[stage * KEYS + lane] = -1;
-          if (a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
+      const int head = to.c * a.side + side, room = to.len - to.step * KEYS;          // key head; keys of the step
+      const bool known = page >= 0 && page < a.pages;
+      const uint32_t k_to = ring_s + stage * F::STAGE + k_dst, v_to = ring_s + stage * F::STAGE + KEYS * F::K_ROW;
+      if (a.aligned) {
+        if (!known && a.err && lane == 0) atomicCAS(a.err, 0, ERR_BAD_ARG);
+        const int keys = known ? room : 0;
+        const uint8_t* ks = known ? a.k + page * a.k_page + (in + kr) * a.k_tok + head * a.k_head + kc * 16 : a.k;
+        const uint8_t* vs = known ? a.v + page * a.v_page + (in + vr) * a.v_tok + head * a.v_head + vc * 16 : a.v;
+        if (E4M3 && lane < KEYS) rows_of[stage * KEYS + lane] = lane < keys ? ((long long)page * a.page + in + lane) * a.kv_heads + head : -1;
+#pragma unroll
+        for (int i = 0; i < KC / 2; ++i) {
+          const bool there = k_exists && i * (32 / KC) + kr < keys;
+          copy_piece(k_to + (i * (32 / KC) >> 3) * F::K_PIECES * 512 + (i * (32 / KC) & 7) * 64, there ? ks + i * (32 / KC) * a.k_tok : a.k, there);
         }
-      } else if (E4M3 && lane < KEYS) {
-        rows_of[stage * KEYS + lane] = -1;
-      }
-      uint32_t dst = ring_s + stage * F::STAGE + lane * 16;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const long long o = __shfl_sync(0xffffffffu, ko, t * 8 + row8);
+        for (int i = 0; i < VC / 2; ++i) {
+          const bool there = v_exists && i * (32 / VC) + vr < keys;
+          copy_piece(v_to + v_dst(i), there ? vs + i * (32 / VC) * a.v_tok : a.v, there);
+        }
+      } else {
+        const bool there = (lane & 15) < room && known;
+        const long long ko = there ? page * a.k_page + in * a.k_tok + head * a.k_head : -1;
+        const long long vo = there ? page * a.v_page + in * a.v_tok + head * a.v_head : -1;
+        if (!known && (lane & 15) < room && a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
+        if (E4M3 && lane < KEYS) rows_of[stage * KEYS + lane] = there ? ((long long)page * a.page + in) * a.kv_heads + head : -1;
 #pragma unroll
-        for (int j = 0; j < F::K_PIECES; ++j, dst += 512) {
-          const int byte = j * 64 + quad * 16;
-          const bool there = o >= 0 && byte < a.dim * (E4M3 ? 1 : 2);
-          copy_piece<16>(dst, a.k + (there ? o + byte : 0), there);
+        for (int i = 0; i < KC / 2; ++i) {
+          const long long o = __shfl_sync(0xffffffffu, ko, i * (32 / KC) + kr);
+          const bool here = k_exists && o >= 0;
+          copy_piece(k_to + (i * (32 / KC) >> 3) * F::K_PIECES * 512 + (i * (32 / KC) & 7) * 64, here ? a.k + o + kc * 16 : a.k, here);
+        }
+#pragma unroll
+        for (int i = 0; i < VC / 2; ++i) {
+          const long long o = __shfl_sync(0xffffffffu, vo, i * (32 / VC) + vr);
+          const bool here = v_exists && o >= 0;
+          copy_piece(v_to + v_dst(i), here ? a.v + o + vc * 16 : a.v, here);
         }
       }
-      dst = ring_s + stage * F::STAGE + KEYS * F::K_ROW + lane * F::V_BYTES;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const long long o = __shfl_sync(0xffffffffu, vo, quad * 2 + (i & 1) + (i >> 1) * 8);
-#pragma unroll
-        for (int j = 0; j < F::V_PIECES; ++j, dst += 32 * F::V_BYTES) {
-          const int byte = j * 128 + row8 * F::V_BYTES;
-          const bool there = o >= 0 && byte < a.vdim * (E4M3 ? 1 : 2);
-          copy_piece<F::V_BYTES>(dst, a.v + (there ? o + byte : 0), there);
-        }
-      }
-      --left;
-      if (left > 0) {
+      if (--left > 0) {
+        const int before = to.step;
         advance(a, to, bad);
-        page = page_at(to);
+        if (to.step == before + 1 && a.page >= KEYS) {        // the next sixteen keys of the same pair
+          in += KEYS;
+          if (in >= a.page) {
+            in -= a.page;
+            ++col;
+          }
+        } else {
+          find_page();
+        }
+        load_page();
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -276,68 +332,72 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Ar
     }
   };
 
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < F::STAGES - 1; ++s) issue(s);
   float kf_next, vl_next;
   scales_at(0, kf_next, vl_next);
 
-  uint32_t qf[MT][D / 16][4];                                 // query fragments
-  float factor[MT][2];                                        // score factor of the rows lane / 4 and lane / 4 + 8
-  float o[MT][VT][4], m[MT][2], mv[MT][2], l[MT][2];          // mv: reference of the weights that multiply V (E4M3: their own)
+  uint32_t qf[NT][D / 16][2];                                 // query fragments: head = lane / 4
+  float factor[NT][2];                                        // score factor of the heads 2 quad and 2 quad + 1, as all that follows
+  float o[NT][VT][4], m[NT][2], mv[NT][2], l[NT][2];          // mv: reference of the weights that multiply V (E4M3: their own)
+  const float size = fabsf(a.scale_log2);                     // the sign goes into the query, so that the largest product is the largest score
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
   auto load_query = [&](const Place& p) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
+    for (int t = 0; t < NT; ++t) {
+      const int head = head0 + t * 8 + row8;
+      const uint8_t* src = a.q + p.b * a.q_seq + ((long long)(p.c * a.side + side) * a.group + head) * a.q_head;
+      const bool row = head < a.group;
+      if (!E4M3) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int head = head0 + t * 16 + half * 8 + row8;
-        const uint8_t* src = a.q + p.b * a.q_seq + ((long long)p.h * a.group + head) * a.q_head;
-        const bool row = head < a.group;
-        if (!E4M3) {
+        for (int j = 0; j < D / 32; ++j) {
+          const int at_dim = j * 32 + quad * 8;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (row && at_dim < a.dim) v = __ldg(reinterpret_cast<const uint4*>(src + at_dim * 2));
+          qf[t][2 * j][0] = v.x ^ flip;
+          qf[t][2 * j][1] = v.y ^ flip;
+          qf[t][2 * j + 1][0] = v.z ^ flip;
+          qf[t][2 * j + 1][1] = v.w ^ flip;
+        }
+        factor[t][0] = factor[t][1] = size;
+      } else {
+        float big = 0.f;
 #pragma unroll
-          for (int j = 0; j < D / 32; ++j) {
-            const int at_dim = j * 32 + quad * 8;
+        for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int at_dim = j * 64 + quad * 16 + c * 8;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (row && at_dim < a.dim) v = __ldg(reinterpret_cast<const uint4*>(src + at_dim * 2));
-            qf[t][2 * j][half] = v.x;
-            qf[t][2 * j][2 + half] = v.y;
-            qf[t][2 * j + 1][half] = v.z;
-            qf[t][2 * j + 1][2 + half] = v.w;
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              qf[t][4 * j + 2 * c + (e >> 1)][e & 1] = w[e] ^ flip;
+              const float2 f = unpair<BF16>(w[e]);
+              big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
           }
-          factor[t][half] = a.scale_log2;
-        } else {
-          uint32_t raw[D / 64][8];
-          float big = 0.f;
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        // largest magnitude into [2^14, 2^15): what falls below fp16's smallest step is 2^-39 of it
+        int up = 14 + 127 - (int)(__float_as_uint(big) >> 23);
+        up = big > 0.f && isfinite(big) ? (up > 100 ? 100 : up < -100 ? -100 : up) : 0;
+        const float by = __uint_as_float(uint32_t(127 + up) << 23);
 #pragma unroll
-          for (int j = 0; j < D / 64; ++j)
+        for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int at_dim = j * 64 + quad * 16 + c * 8;
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (row && at_dim < a.dim) v = __ldg(reinterpret_cast<const uint4*>(src + at_dim * 2));
-              raw[j][c * 4] = v.x; raw[j][c * 4 + 1] = v.y; raw[j][c * 4 + 2] = v.z; raw[j][c * 4 + 3] = v.w;
+          for (int e = 0; e < 2; ++e) {
+            const float2 f = unpair<BF16>(qf[t][k][e]);
+            qf[t][k][e] = pair<false>(f.x * by, f.y * by);
+          }
+        const float mine = size * __uint_as_float(uint32_t(127 - up) << 23);
+        factor[t][0] = __shfl_sync(0xffffffffu, mine, quad * 8);
+        factor[t][1] = __shfl_sync(0xffffffffu, mine, quad * 8 + 4);
+      }
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = unpair<BF16>(raw[j][c * 4 + e]);
-                big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-              }
-            }
-          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-          // largest magnitude into [2^14, 2^15): what falls below fp16's smallest step is 2^-39 of it
-          int up = 14 + 127 - (int)(__float_as_uint(big) >> 23);
-          up = big > 0.f && isfinite(big) ? (up > 100 ? 100 : up < -100 ? -100 : up) : 0;
-          const float by = __uint_as_float(uint32_t(127 + up) << 23);
-#pragma unroll
-          for (int j = 0; j < D / 64; ++j)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 f = unpair<BF16>(raw[j][e]);
-              qf[t][4 * j + (e >> 1)][(e & 1) * 2 + half] = pair<false>(f.x * by, f.y * by);
-            }
-          factor[t][half] = a.scale_log2 * __uint_as_float(uint32_t(127 - up) << 23);
-        }
-        m[t][half] = mv[t][half] = -INFINITY;
-        l[t][half] = 0.f;
+      for (int c = 0; c < 2; ++c) {
+        m[t][c] = mv[t][c] = -INFINITY;
+        l[t][c] = 0.f;
       }
 #pragma unroll
       for (int c = 0; c < VT; ++c) o[t][c][0] = o[t][c][1] = o[t][c][2] = o[t][c][3] = 0.f;
@@ -348,47 +408,44 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Ar
   auto leave = [&](const Place& p, int first, long long piece) {
     const bool whole = first == 0 && p.step == p.steps - 1;
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float sum = l[t][half];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const int row = t * 16 + half * 8 + row8, head = head0 + row;
+      for (int c = 0; c < 2; ++c) {
+        const float sum = sum8(l[t][c]);
+        const int row = t * 8 + quad * 2 + c, head = head0 + row;
         if (head >= a.group) continue;
-        float f = E4M3 && m[t][half] != -INFINITY ? ex2(mv[t][half] - m[t][half]) : 1.f;
+        float f = E4M3 && m[t][c] != -INFINITY ? ex2(mv[t][c] - m[t][c]) : 1.f;
         if (whole) {
           f = sum > 0.f ? f / sum : sum == 0.f ? 0.f : sum;   // a NaN stays
-          uint8_t* dst = reinterpret_cast<uint8_t*>(a.out) + (((long long)p.b * a.kv_heads + p.h) * a.group + head) * a.vdim * 2;
+          uint8_t* dst = reinterpret_cast<uint8_t*>(a.out) + (((long long)p.b * a.kv_heads + p.c * a.side + side) * a.group + head) * a.vdim * 2;
 #pragma unroll
-          for (int j = 0; j < VT / F::SPAN; ++j)
+          for (int j = 0; j < DV / 8 / F::SPAN; ++j)
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int e = 0; e < F::SPAN; e += 8) {
+              const int column = (j * 8 + row8) * F::SPAN + e;
+              uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < F::SPAN; e += 8) {
-                const int col = (j * 8 + quad * 2 + c) * F::SPAN + e;
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  w[i] = pair<BF16>(o[t][j * F::SPAN + e + 2 * i][half * 2 + c] * f, o[t][j * F::SPAN + e + 2 * i + 1][half * 2 + c] * f);
-                if (col < a.vdim) *reinterpret_cast<uint4*>(dst + col * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int i = 0; i < 4; ++i) {
+                const int n = (j * F::SPAN + e) / 2 + i;
+                w[i] = pair<BF16>(o[t][n][c] * f, o[t][n][2 + c] * f);
               }
+              if (column < a.vdim) *reinterpret_cast<uint4*>(dst + column * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         } else {
-          float* dst = a.part + ((piece * a.tiles + tile) * a.rows + row) * (DV + 4);
-          if (quad == 0) {
+          float* dst = a.part + (((piece * a.side + side) * a.tiles + tile) * a.rows + row) * (DV + 4);
+          if (row8 == 0) {
             dst[0] = sum;
-            dst[1] = m[t][half];
+            dst[1] = m[t][c];
           }
           dst += 4;
 #pragma unroll
-          for (int j = 0; j < VT / F::SPAN; ++j)
+          for (int j = 0; j < DV / 8 / F::SPAN; ++j)
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int e = 0; e < F::SPAN; e += 4) {
-                const int col = (j * 8 + quad * 2 + c) * F::SPAN + e, n = j * F::SPAN + e, k = half * 2 + c;
-                *reinterpret_cast<float4*>(dst + col) = make_float4(o[t][n][k] * f, o[t][n + 1][k] * f, o[t][n + 2][k] * f, o[t][n + 3][k] * f);
-              }
+            for (int e = 0; e < F::SPAN; e += 4) {
+              const int n = (j * F::SPAN + e) / 2;
+              *reinterpret_cast<float4*>(dst + (j * 8 + row8) * F::SPAN + e) =
+                  make_float4(o[t][n][c] * f, o[t][n][2 + c] * f, o[t][n + 1][c] * f, o[t][n + 1][2 + c] * f);
+            }
         }
       }
   };
@@ -397,116 +454,129 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Ar
   load_query(at);
   for (int i = 0; i < count; ++i) {
     copies_but<F::STAGES - 2>();
+    __syncwarp();                                             // the step's rows are there, and the stage before has been read
     issue(stage == 0 ? F::STAGES - 1 : stage - 1);            // into the stage that was read last
     const float kf = kf_next, vl = vl_next;
     const int next = stage + 1 == F::STAGES ? 0 : stage + 1;
     if (E4M3 && i + 1 < count) scales_at(next, kf_next, vl_next);
     const uint32_t base = ring_s + stage * F::STAGE;
 
-    // ---- scores ----
-    float s[MT][2][4];
+    // ---- scores: keys lane / 4 and lane / 4 + 8 of the heads 2 quad and 2 quad + 1 ----
+    float s[NT][4], s2[NT][4];                                // two sums, so that a product does not wait for the one before
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int x = 0; x < MT; ++x) s[x][t][0] = s[x][t][1] = s[x][t][2] = s[x][t][3] = 0.f;
+      for (int c = 0; c < 4; ++c) s[x][c] = s2[x][c] = 0.f;
 #pragma unroll
-      for (int j = 0; j < F::K_PIECES; ++j) {
-        const uint4 kv = lds16(base + (t * F::K_PIECES + j) * 512 + lane * 16);
-        if (!E4M3) {
+    for (int j = 0; j < F::K_PIECES; ++j) {
+      const uint32_t place = base + (lane ^ ((j & 1) * 4)) * 16;
+      const uint4 lo = lds16(place + j * 512), hi = lds16(place + (F::K_PIECES + j) * 512);
+      if (!E4M3) {
+        const uint32_t k0[4] = {lo.x, hi.x, lo.y, hi.y}, k1[4] = {lo.z, hi.z, lo.w, hi.w};
 #pragma unroll
-          for (int x = 0; x < MT; ++x) {
-            mma<MB>(s[x][t], qf[x][2 * j], kv.x, kv.y);
-            mma<MB>(s[x][t], qf[x][2 * j + 1], kv.z, kv.w);
-          }
-        } else {
-          const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
+        for (int x = 0; x < NT; ++x) {
+          mma<MB>(s[x], k0, qf[x][2 * j][0], qf[x][2 * j][1]);
+          mma<MB>(s2[x], k1, qf[x][2 * j + 1][0], qf[x][2 * j + 1][1]);
+        }
+      } else {
+        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t lo = expand_lo(w[e]), hi = expand_hi(w[e]);
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t k[4] = {expand_lo(wl[e]), expand_lo(wh[e]), expand_hi(wl[e]), expand_hi(wh[e])};
 #pragma unroll
-            for (int x = 0; x < MT; ++x) mma<MB>(s[x][t], qf[x][4 * j + e], lo, hi);
-          }
+          for (int x = 0; x < NT; ++x) mma<MB>(e & 1 ? s2[x] : s[x], k, qf[x][4 * j + e][0], qf[x][4 * j + e][1]);
         }
       }
     }
-    const int room = at.len - at.step * KEYS - quad * 2;      // keys of this lane: quad * 2 + {0, 1}, + 8
-    float vlog[2][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float kp = E4M3 ? __shfl_sync(0xffffffffu, kf, t * 8 + quad * 2 + c) : 1.f;
-        vlog[t][c] = E4M3 ? __shfl_sync(0xffffffffu, vl, t * 8 + quad * 2 + c) : 0.f;
-        const bool there = t * 8 + c < room;
+      for (int c = 0; c < 4; ++c) s[x][c] += s2[x][c];
+    float vlog[2] = {0.f, 0.f};                               // of the two keys
+    if (E4M3) {
+      const float k0 = __shfl_sync(0xffffffffu, kf, row8), k1 = __shfl_sync(0xffffffffu, kf, 8 + row8);
+      vlog[0] = __shfl_sync(0xffffffffu, vl, row8);
+      vlog[1] = __shfl_sync(0xffffffffu, vl, 8 + row8);
 #pragma unroll
-        for (int x = 0; x < MT; ++x) {
-          s[x][t][c] = there ? s[x][t][c] * factor[x][0] * kp : -INFINITY;
-          s[x][t][2 + c] = there ? s[x][t][2 + c] * factor[x][1] * kp : -INFINITY;
-        }
+      for (int x = 0; x < NT; ++x) {
+        s[x][0] *= k0; s[x][1] *= k0;
+        s[x][2] *= k1; s[x][3] *= k1;
       }
+    }
+    const int room = at.len - at.step * KEYS;
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      s[x][0] *= factor[x][0]; s[x][1] *= factor[x][1];
+      s[x][2] *= factor[x][0]; s[x][3] *= factor[x][1];
+    }
+    if (room < KEYS) {                                        // the last step of a pair
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        if (row8 >= room) s[x][0] = s[x][1] = -INFINITY;
+        if (row8 + 8 >= room) s[x][2] = s[x][3] = -INFINITY;
+      }
+    }
 
     // ---- reference values ----
     bool grown = false;
-    float top[MT][2], topv[MT][2];
+    float top[NT][2], topv[NT][2];
 #pragma unroll
-    for (int x = 0; x < MT; ++x)
+    for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int k = half * 2;
-        top[x][half] = fmaxf(fmaxf(s[x][0][k], s[x][0][k + 1]), fmaxf(s[x][1][k], s[x][1][k + 1]));
-        grown |= top[x][half] > m[x][half] + RESCALE_AT;
+      for (int c = 0; c < 2; ++c) {
+        top[x][c] = fmaxf(s[x][c], s[x][2 + c]);
+        grown |= top[x][c] > m[x][c] + RESCALE_AT;
         if (E4M3) {
-          topv[x][half] = fmaxf(fmaxf(s[x][0][k] + vlog[0][0], s[x][0][k + 1] + vlog[0][1]),
-                                fmaxf(s[x][1][k] + vlog[1][0], s[x][1][k + 1] + vlog[1][1]));
-          grown |= topv[x][half] > mv[x][half] + RESCALE_AT;
+          topv[x][c] = fmaxf(s[x][c] + vlog[0], s[x][2 + c] + vlog[1]);
+          grown |= topv[x][c] > mv[x][c] + RESCALE_AT;
         }
       }
     if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-      for (int x = 0; x < MT; ++x)
+      for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int c = 0; c < 2; ++c) {
           auto raise = [&](float& ref, float t) {             // the factor that takes sums to the new reference
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+            t = max8(t);
             if (!(t > ref)) return 1.f;
             const float by = ex2(ref - t);
             ref = t;
             return by;
           };
-          const float by = raise(m[x][half], top[x][half]);
-          l[x][half] *= by;
-          const float byv = E4M3 ? raise(mv[x][half], topv[x][half]) : by;
+          const float by = raise(m[x][c], top[x][c]);
+          l[x][c] *= by;
+          const float byv = E4M3 ? raise(mv[x][c], topv[x][c]) : by;
 #pragma unroll
-          for (int c = 0; c < VT; ++c) {
-            o[x][c][half * 2] *= byv;
-            o[x][c][half * 2 + 1] *= byv;
+          for (int n = 0; n < VT; ++n) {
+            o[x][n][c] *= byv;
+            o[x][n][2 + c] *= byv;
           }
         }
     }
 
     // ---- weights ----
-    uint32_t p[MT][4];
+    uint32_t p[NT][2];                                        // keys 2 quad, + 1 (and + 8) of head lane / 4
 #pragma unroll
-    for (int x = 0; x < MT; ++x)
+    for (int x = 0; x < NT; ++x) {
+      float w[4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const float ref = m[x][half] == -INFINITY ? 0.f : m[x][half];
-        const float refv = mv[x][half] == -INFINITY ? 0.f : mv[x][half];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const float u = s[x][t][half * 2], w = s[x][t][half * 2 + 1];
-          const float pu = ex2(u - ref), pw = ex2(w - ref);
-          l[x][half] += pu + pw;
-          p[x][t * 2 + half] = E4M3 ? pair<MB>(ex2(u + vlog[t][0] - refv), ex2(w + vlog[t][1] - refv)) : pair<MB>(pu, pw);
-        }
+      for (int c = 0; c < 2; ++c) {
+        const float ref = m[x][c] == -INFINITY ? 0.f : m[x][c], refv = mv[x][c] == -INFINITY ? 0.f : mv[x][c];
+        const float u = ex2(s[x][c] - ref), y = ex2(s[x][2 + c] - ref);
+        l[x][c] += u + y;
+        w[c] = E4M3 ? ex2(s[x][c] + vlog[0] - refv) : u;
+        w[2 + c] = E4M3 ? ex2(s[x][2 + c] + vlog[1] - refv) : y;
       }
+      p[x][0] = transposed(pair<MB>(w[0], w[1]));
+      p[x][1] = transposed(pair<MB>(w[2], w[3]));
+    }
 
-    // ---- weights times values ----
-    const uint32_t vb = base + KEYS * F::K_ROW + lane * F::V_BYTES;
+    // ---- values times weights ----
+    const uint32_t vb = base + KEYS * F::K_ROW +
+                        (F::V_BYTES == 16 ? (quad * 8 + (row8 ^ (2 * quad))) * 16 : ((row8 >> 2) * 8 + quad * 2 + (row8 >> 1 & 1)) * 16 + (row8 & 1) * 8);
 #pragma unroll
     for (int j = 0; j < F::V_PIECES; ++j) {
-      uint32_t r[4][4];
+      uint32_t r[4][4];                                       // keys 2 quad, + 1, + 8, + 9
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const uint32_t ad = vb + (y * F::V_PIECES + j) * 32 * F::V_BYTES;
@@ -521,28 +591,26 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Ar
 #pragma unroll
       for (int w = 0; w < F::V_BYTES / 4; ++w) {
         if (!E4M3) {
-          const uint32_t b0 = __byte_perm(r[0][w], r[1][w], 0x5410), b1 = __byte_perm(r[2][w], r[3][w], 0x5410);
-          const uint32_t c0 = __byte_perm(r[0][w], r[1][w], 0x7632), c1 = __byte_perm(r[2][w], r[3][w], 0x7632);
+          const uint32_t v[4] = {__byte_perm(r[0][w], r[1][w], 0x5410), __byte_perm(r[0][w], r[1][w], 0x7632),
+                                 __byte_perm(r[2][w], r[3][w], 0x5410), __byte_perm(r[2][w], r[3][w], 0x7632)};
 #pragma unroll
-          for (int x = 0; x < MT; ++x) {
-            mma<MB>(o[x][j * F::SPAN + 2 * w], p[x], b0, b1);
-            mma<MB>(o[x][j * F::SPAN + 2 * w + 1], p[x], c0, c1);
-          }
+          for (int x = 0; x < NT; ++x) mma<MB>(o[x][j * F::SPAN / 2 + w], v, p[x][0], p[x][1]);
         } else {
           const uint32_t e0 = __byte_perm(r[0][w], r[1][w], 0x5140), e1 = __byte_perm(r[2][w], r[3][w], 0x5140);
           const uint32_t f0 = __byte_perm(r[0][w], r[1][w], 0x7362), f1 = __byte_perm(r[2][w], r[3][w], 0x7362);
-          const uint32_t b[4][2] = {{expand_lo(e0), expand_lo(e1)}, {expand_hi(e0), expand_hi(e1)},
-                                    {expand_lo(f0), expand_lo(f1)}, {expand_hi(f0), expand_hi(f1)}};
+          const uint32_t v0[4] = {expand_lo(e0), expand_hi(e0), expand_lo(e1), expand_hi(e1)};
+          const uint32_t v1[4] = {expand_lo(f0), expand_hi(f0), expand_lo(f1), expand_hi(f1)};
 #pragma unroll
-          for (int x = 0; x < MT; ++x)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) mma<MB>(o[x][j * F::SPAN + 4 * w + c], p[x], b[c][0], b[c][1]);
+          for (int x = 0; x < NT; ++x) {
+            mma<MB>(o[x][j * F::SPAN / 2 + 2 * w], v0, p[x][0], p[x][1]);
+            mma<MB>(o[x][j * F::SPAN / 2 + 2 * w + 1], v1, p[x][0], p[x][1]);
+          }
         }
       }
     }
 
     const bool last = i + 1 == count;
-    if (last || at.step == at.steps - 1) leave(at, first, run + (long long)at.b * a.kv_heads + at.h);
+    if (last || at.step == at.steps - 1) leave(at, first, run + (long long)at.b * a.chunks + at.c);
     if (!last) {
       const bool other = at.step == at.steps - 1;
       advance(a, at, bad);
@@ -556,12 +624,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const Ar
   copies_but<0>();
 }
 
-constexpr int JOIN_WARPS = 4;
+constexpr int JOIN_WARPS = 8;
+constexpr int JOIN_PIECES = 256;             // pieces weighed at once
 
 // The pieces of each pair become its result: a block per (sequence, head).  Piece numbers: run r leaves piece r + s of pair s, which no other
-// pair of r and s shares along the sequence of steps.
+// pair of r and s shares along the sequence of steps.  All maxima are read first, so that the accumulators come without waiting for one another.
 template <bool BF16, int DV>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const Args a, int tile_rows) {
+  constexpr int C = DV / 32, AHEAD = 4;      // columns of a lane
+  __shared__ float part[JOIN_WARPS][DV], weight[JOIN_PIECES], tops[JOIN_WARPS], sums[JOIN_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / (a.kv_heads * a.group), hq = blockIdx.x % (a.kv_heads * a.group), h = hq / a.group, head = hq % a.group;
   bool bad = false;
@@ -570,102 +641,128 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const Args a, int
   for (int i = lane; i < b; i += 32) before += steps_of(length_of(a, i, bad));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  const int steps = steps_of(length_of(a, b, bad));
-  const long long s0 = before * a.kv_heads + (long long)h * steps;
+  const int steps = steps_of(length_of(a, b, bad)), chunk = h / a.side;
+  const long long s0 = before * a.chunks + (long long)chunk * steps;
   const int r0 = (int)(s0 / q), r1 = steps ? (int)((s0 + steps - 1) / q) : r0;
   few::wait_for_input();                     // by every block: the next kernel of the stream counts on this one having waited
   if (steps && r0 == r1) return;             // finished by the one run that holds it
 
-  constexpr int C = DV / 32;                 // columns of a lane
-  __shared__ float part[JOIN_WARPS][DV + 2];
   float top = -INFINITY, sum = 0.f, acc[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) acc[c] = 0.f;
-  if (steps) {
-    const int tile = head / tile_rows, row = head % tile_rows;
-    const long long pair_no = (long long)b * a.kv_heads + h;
-    for (int r = r0 + warp; r <= r1; r += JOIN_WARPS) {
-      const float* src = a.part + (((r + pair_no) * a.tiles + tile) * a.rows + row) * (DV + 4);
-      const float n = src[0], ref = src[1];
-      float v[C];
+  // a piece of the next run lies `pitch` floats behind
+  const long long pitch = (long long)a.side * a.tiles * a.rows * (DV + 4);
+  const float* base = a.part + (long long)(b * (long long)a.chunks + chunk + r0) * pitch +
+                      ((h - chunk * a.side) * a.tiles + head / tile_rows) * (long long)a.rows * (DV + 4) + (head % tile_rows) * (DV + 4);
+  const int n = steps ? r1 - r0 + 1 : 0;
+  for (int i0 = 0; i0 < n; i0 += JOIN_PIECES) {
+    const int i = i0 + threadIdx.x, here = min(JOIN_PIECES, n - i0);
+    const float ref = i < n ? base[i * pitch + 1] : -INFINITY, mass = i < n ? base[i * pitch] : 0.f;
+    const float most = warp_max(ref);
+    __syncthreads();                         // the weights before have been used
+    if (lane == 0) tops[warp] = most;
+    __syncthreads();
+    float now = top;
+    for (int w = 0; w < JOIN_WARPS; ++w) now = fmaxf(now, tops[w]);
+    const float by = ref == -INFINITY ? 0.f : ex2(ref - now), old = top == -INFINITY ? 0.f : ex2(top - now);
+    weight[threadIdx.x] = by;
+    sum = sum * old + mass * by;
+    top = now;
 #pragma unroll
-      for (int c = 0; c < C; ++c) v[c] = src[4 + lane * C + c];
-      const float t = fmaxf(top, ref);
-      const float old = top == -INFINITY ? 0.f : ex2(top - t), by = ref == -INFINITY ? 0.f : ex2(ref - t);
-      sum = sum * old + n * by;
+    for (int c = 0; c < C; ++c) acc[c] *= old;
+    __syncthreads();
+    for (int k = warp; k < here; k += JOIN_WARPS * AHEAD) {
+      float v[AHEAD][C], w[AHEAD];
 #pragma unroll
-      for (int c = 0; c < C; ++c) acc[c] = acc[c] * old + v[c] * by;
-      top = t;
+      for (int u = 0; u < AHEAD; ++u) {
+        const int at = k + u * JOIN_WARPS;
+        w[u] = at < here ? weight[at] : 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) v[u][c] = at < here ? base[(i0 + at) * pitch + 4 + lane * C + c] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] += v[u][c] * w[u];
     }
   }
-  if (lane == 0) {
-    part[warp][DV] = sum;
-    part[warp][DV + 1] = top;
-  }
+  sum = warp_sum(sum);
+  if (lane == 0) sums[warp] = sum;
 #pragma unroll
   for (int c = 0; c < C; ++c) part[warp][lane * C + c] = acc[c];
   __syncthreads();
   const int col = threadIdx.x * 2;
   if (col >= a.vdim) return;
-  top = -INFINITY;
-  for (int w = 0; w < JOIN_WARPS; ++w) top = fmaxf(top, part[w][DV + 1]);
-  float n = 0.f, x = 0.f, y = 0.f;
+  float mass = 0.f, x = 0.f, y = 0.f;
   for (int w = 0; w < JOIN_WARPS; ++w) {
-    const float by = part[w][DV + 1] == -INFINITY ? 0.f : ex2(part[w][DV + 1] - top);
-    n += part[w][DV] * by;
-    x += part[w][col] * by;
-    y += part[w][col + 1] * by;
+    mass += sums[w];
+    x += part[w][col];
+    y += part[w][col + 1];
   }
-  const float inv = n > 0.f ? 1.f / n : n == 0.f ? 0.f : n;
+  const float inv = mass > 0.f ? 1.f / mass : mass == 0.f ? 0.f : mass;
   reinterpret_cast<uint32_t*>(a.out)[((long long)blockIdx.x * a.vdim + col) >> 1] = pair<BF16>(x * inv, y * inv);
 }
 
 struct Layout {
-  int mt, tiles, rows, grid, dv;
+  int nt, tiles, rows, grid, warps, dim, vdim, side, chunks, runs;
   long long floats;
 };
 
-// Heads of a group in tiles of 16 rows: two tiles a warp where the accumulators leave registers for them (64 value columns), else one; more
-// tiles than that go to neighbouring warps, which read the same keys at the same time, out of L2.
-Layout layout_of(int sequences, int kv_heads, int group, int dim, int vdim, int columns, int page) {
+// Heads of a group in tiles of eight: up to four tiles a warp with 64 value columns, two with 128 (its registers hold no more); more go to
+// neighbouring warps, which read the same keys at the same time, out of L2.
+Layout layout_of(int sequences, int kv_heads, int group, int dim, int vdim, int columns, int page, bool e4m3) {
   Layout s;
-  s.dv = vdim <= 64 && (dim <= 128) ? 64 : 128;
-  s.mt = s.dv == 64 && group > 16 ? 2 : 1;
+  s.vdim = vdim <= 64 ? 64 : 128;
+  s.dim = dim <= 64 && s.vdim == 64 ? 64 : 128;
+  s.nt = group <= 8 ? 1 : group <= 16 || s.vdim == 128 ? 2 : 4;
   s.tiles = 1;
-  while (s.tiles * 16 * s.mt < group) s.tiles *= 2;
-  s.rows = group < 16 * s.mt ? group : 16 * s.mt;
-  const long long steps = (long long)sequences * kv_heads * (((long long)columns * page + KEYS - 1) / KEYS);
-  const long long want = (steps + SHORTEST_RUN - 1) / SHORTEST_RUN * s.tiles, sms = sm_count() > 0 ? sm_count() : 1;
-  const long long blocks = (want + WARPS - 1) / WARPS;
+  while (s.tiles * 8 * s.nt < group) s.tiles *= 2;
+  s.warps = warps_of(e4m3, s.dim, s.vdim, s.nt);
+  s.rows = group < 8 * s.nt ? group : 8 * s.nt;
+  s.side = kv_heads < 16 ? kv_heads : 16;                     // the largest divisor of the key heads up to 16
+  while (kv_heads % s.side) --s.side;
+  s.chunks = kv_heads / s.side;
+  const long long steps = (long long)sequences * s.chunks * (((long long)columns * page + KEYS - 1) / KEYS);
+  const long long want = (steps + SHORTEST_RUN - 1) / SHORTEST_RUN * s.tiles * s.side, sms = sm_count() > 0 ? sm_count() : 1;
+  const long long blocks = (want + s.warps - 1) / s.warps;
   s.grid = int(blocks < sms ? blocks : sms);
-  s.floats = (s.grid * WARPS / s.tiles + (long long)sequences * kv_heads) * s.tiles * s.rows * (s.dv + 4);
+  s.runs = s.grid * s.warps / (s.side * s.tiles);
+  if (s.runs == 0) {                                          // a device of few SMs: one run all the same
+    s.runs = 1;
+    s.grid = steps > 0 ? (s.side * s.tiles + s.warps - 1) / s.warps : 0;
+  }
+  s.floats = (s.runs + (long long)sequences * s.chunks) * s.side * s.tiles * s.rows * (s.vdim + 4);
   return s;
 }
 
-template <bool BF16, bool E4M3, int D, int DV, int MT>
+template <bool BF16, bool E4M3, int D, int DV, int NT>
 int start(const Args& a, int grid, cudaStream_t stream) {
-  auto kern = paged_attention_kernel<BF16, E4M3, D, DV, MT>;
-  constexpr int smem = WARPS * Form<BF16, E4M3, D, DV>::RING;
+  using F = Form<BF16, E4M3, D, DV, NT>;
+  auto kern = paged_attention_kernel<BF16, E4M3, D, DV, NT>;
+  constexpr int smem = F::WARPS * F::RING;
   if (grid > 0) {
     static PerDevice cfg;
     if (cfg.first()) {
       if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2;
       cfg.done();
     }
-    kern<<<grid, WARPS * 32, smem, stream>>>(a);
+    kern<<<grid, F::WARPS * 32, smem, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return -3;
   }
   const dim3 blocks((unsigned)(a.sequences * a.kv_heads * a.group));
-  return few::launch_early(join_kernel<BF16, DV>, blocks, dim3(JOIN_WARPS * 32), 0, stream, a, 16 * MT);
+  return few::launch_early(join_kernel<BF16, DV>, blocks, dim3(JOIN_WARPS * 32), 0, stream, a, 8 * NT);
 }
 
 template <bool BF16, bool E4M3>
 int pick(const Args& a, const Layout& s, cudaStream_t stream) {
-  if (s.dv == 64) {
-    if (a.dim <= 64) return s.mt == 2 ? start<BF16, E4M3, 64, 64, 2>(a, s.grid, stream) : start<BF16, E4M3, 64, 64, 1>(a, s.grid, stream);
-    return s.mt == 2 ? start<BF16, E4M3, 128, 64, 2>(a, s.grid, stream) : start<BF16, E4M3, 128, 64, 1>(a, s.grid, stream);
-  }
-  return start<BF16, E4M3, 128, 128, 1>(a, s.grid, stream);
+  if (s.vdim == 128) return s.nt == 1 ? start<BF16, E4M3, 128, 128, 1>(a, s.grid, stream) : start<BF16, E4M3, 128, 128, 2>(a, s.grid, stream);
+  if (s.dim == 128)
+    return s.nt == 1   ? start<BF16, E4M3, 128, 64, 1>(a, s.grid, stream)
+           : s.nt == 2 ? start<BF16, E4M3, 128, 64, 2>(a, s.grid, stream)
+                       : start<BF16, E4M3, 128, 64, 4>(a, s.grid, stream);
+  return s.nt == 1   ? start<BF16, E4M3, 64, 64, 1>(a, s.grid, stream)
+         : s.nt == 2 ? start<BF16, E4M3, 64, 64, 2>(a, s.grid, stream)
+                     : start<BF16, E4M3, 64, 64, 4>(a, s.grid, stream);
 }
 
 }  // namespace
@@ -675,8 +772,8 @@ int pick(const Args& a, const Layout& s, cudaStream_t stream) {
 using namespace cm;
 using namespace cm::paged;
 
-extern "C" long long cm_paged_attention_ws(int sequences, int kv_heads, int group, int dim, int vdim, int columns, int page) {
-  return layout_of(sequences, kv_heads, group, dim, vdim, columns, page).floats;
+extern "C" long long cm_paged_attention_ws(int sequences, int kv_heads, int group, int dim, int vdim, int columns, int page, int e4m3) {
+  return layout_of(sequences, kv_heads, group, dim, vdim, columns, page, e4m3).floats;
 }
 
 // q [sequences, kv_heads * group, dim]; caches [pages, page, kv_heads, .], E4M3 ones with their exponent bytes; table [sequences, columns],
@@ -693,7 +790,7 @@ extern "C" int cm_paged_attention(const void* q, const void* k, const void* v, c
   if (group < 1 || group > 128 || dim < step || dim > 128 || dim % step || vdim < step || vdim > 128 || vdim % step || page < 1 || columns < 0 ||
       columns * page > 0x7fffffffLL - KEYS || sequences * kv_heads * group > 0x7fffffffLL)
     return -10;
-  const Layout s = layout_of((int)sequences, (int)kv_heads, (int)group, (int)dim, (int)vdim, (int)columns, (int)page);
+  const Layout s = layout_of((int)sequences, (int)kv_heads, (int)group, (int)dim, (int)vdim, (int)columns, (int)page, e4m3);
   Args a;
   a.q = (const uint8_t*)q;
   a.q_seq = n[0] * 2; a.q_head = n[1] * 2;
@@ -716,7 +813,10 @@ extern "C" int cm_paged_attention(const void* q, const void* k, const void* v, c
   a.page = (int)page;
   a.dim = (int)dim;
   a.vdim = (int)vdim;
-  a.runs = s.grid > 0 ? s.grid * WARPS / s.tiles : 1;
+  a.runs = s.runs;
+  a.side = s.side;
+  a.chunks = s.chunks;
+  a.aligned = page % KEYS == 0;
   a.tiles = s.tiles;
   a.rows = s.rows;
   a.scale_log2 = scale * 1.4426950408889634f;

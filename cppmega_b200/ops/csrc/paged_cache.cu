@@ -17,6 +17,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace cm {
@@ -27,6 +29,13 @@ constexpr int MAX_TOKENS = 128;              // tokens of one block
 constexpr int HASH_BITS = 8192;
 constexpr int ROWS_AHEAD = 4;
 constexpr int SCAN = 8;                      // later slots that a thread has on their way at once
+
+// r / n for r < 128 n: by a product where that is exact (r n < 2^32), by a division else
+struct Divide {
+  uint32_t n, magic;
+  __host__ Divide(int heads = 1) : n(heads), magic(heads > 1 && heads < 5000 ? uint32_t(((1ull << 32) + heads - 1) / heads) : 0) {}
+  __device__ __forceinline__ int operator()(int r) const { return n == 1 ? r : magic ? int(__umulhi(uint32_t(r), magic)) : int(uint32_t(r) / n); }
+};
 
 struct Side {                                // keys or values
   const uint8_t* x;                          // rows of the packed tensor
@@ -44,6 +53,7 @@ struct WriteArgs {
   long long total;                           // slots of the cache
   int wide;                                  // slots are 64-bit
   int T, heads, page, per_block;
+  Divide by_heads;
   int* err;
 };
 
@@ -79,22 +89,34 @@ __device__ __forceinline__ int exponent_byte(float amax) {
   return e < 1 ? 1 : e;                      // at most 254 - 8 + 1
 }
 
+// eight values times a power of two as E4M3; infinities and NaN (of which a row that has any says so) become NaN
 template <typename T>
-__device__ __forceinline__ uint2 quantised(const uint4& v, float inv) {
+__device__ __forceinline__ uint2 quantised(const uint4& v, float inv, bool all_finite) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   uint32_t out[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = two<T>(w[i >> 1]);
-    const float x = (i & 1) ? f.y : f.x;
-    const uint32_t b = isfinite(x) ? (uint32_t)__nv_cvt_float_to_fp8(x * inv, __NV_SATFINITE, __NV_E4M3) : 0x7fu;
-    out[i >> 2] |= b << (8 * (i & 3));
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = two<T>(w[i]);
+    uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(f.x * inv, f.y * inv), __NV_SATFINITE, __NV_E4M3);
+    if (!all_finite) {
+      if (!isfinite(f.x)) b = (b & 0xff00u) | 0x7fu;
+      if (!isfinite(f.y)) b = (b & 0x00ffu) | 0x7f00u;
+    }
+    out[i >> 1] |= b << (16 * (i & 1));
   }
   return make_uint2(out[0], out[1]);
 }
 
+// Magnitudes of 16-bit floats order as their bits do without the sign: the largest of eight, two to an instruction
+__device__ __forceinline__ uint32_t largest_bits(const uint4& v) {
+  const uint32_t m = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(v.x & m, v.y & m), __vmaxu2(v.z & m, v.w & m));
+}
 template <typename T>
-__device__ __forceinline__ float largest(const uint4& v) {
+constexpr uint32_t first_not_finite() { return std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u; }
+
+template <typename T>
+__device__ float largest_finite(const uint4& v) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   float m = 0.f;
 #pragma unroll
@@ -108,9 +130,10 @@ __device__ __forceinline__ float largest(const uint4& v) {
 
 // T: the packed rows' type; E4M3: what the cache holds (the same type otherwise)
 template <typename T, bool E4M3>
-__global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(THREADS, 4) cache_write_kernel(const WriteArgs a) {
   __shared__ uint32_t bits[HASH_BITS / 32];
   __shared__ long long own[MAX_TOKENS];      // the slot, or -1: not written
+  __shared__ long long base[2][MAX_TOKENS];  // and where it begins in the caches
   __shared__ int lost[MAX_TOKENS];           // a later token has the same slot
   const long long t0 = (long long)blockIdx.x * a.per_block;
   const int n = (int)min((long long)a.per_block, a.T - t0);
@@ -124,7 +147,11 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteArgs a)
     }
     own[i] = s < 0 ? -1 : s;
     lost[i] = 0;
-    if (s >= 0) atomicOr(&bits[(s & (HASH_BITS - 1)) >> 5], 1u << (s & 31));
+    if (s >= 0) {
+      atomicOr(&bits[(s & (HASH_BITS - 1)) >> 5], 1u << (s & 31));
+      const long long page = s / a.page, in = s - page * a.page;
+      for (int w = 0; w < a.sides; ++w) base[w][i] = page * a.side[w].c_page + in * a.side[w].c_tok;
+    }
   }
   __syncthreads();
   for (long long t = t0 + 1 + threadIdx.x; t < a.T; t += SCAN * THREADS) {
@@ -153,7 +180,7 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteArgs a)
       for (int u = 0; u < ROWS_AHEAD; ++u) {
         const int r = r0 + u * groups + group;
         v[u] = make_uint4(0, 0, 0, 0);
-        tok[u] = r / a.heads;
+        tok[u] = a.by_heads(r);
         head[u] = r - tok[u] * a.heads;
         if (r >= rows || own[tok[u]] < 0 || lost[tok[u]]) tok[u] = -1;
         else if (part < d.width)
@@ -162,18 +189,25 @@ __global__ void __launch_bounds__(THREADS) cache_write_kernel(const WriteArgs a)
 #pragma unroll
       for (int u = 0; u < ROWS_AHEAD; ++u) {
         float m = 0.f;
+        bool all_finite = true;
         if (E4M3) {
-          m = largest<T>(v[u]);
-          for (int o = d.lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          uint32_t x = largest_bits(v[u]);
+          for (int o = d.lanes >> 1; o > 0; o >>= 1) x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, o));
+          x = max(x & 0xffffu, x >> 16);
+          all_finite = x < first_not_finite<T>();
+          m = two<T>(x).x;
+          if (!__all_sync(0xffffffffu, all_finite)) {         // the row's largest finite one
+            m = largest_finite<T>(v[u]);
+            for (int o = d.lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          }
         }
         if (tok[u] < 0) continue;
-        const long long s = own[tok[u]], page = s / a.page;
-        uint8_t* row = d.cache + page * d.c_page + (s - page * a.page) * d.c_tok + head[u] * d.c_head;
+        uint8_t* row = d.cache + base[w][tok[u]] + head[u] * d.c_head;
         if (E4M3) {
           const int e = exponent_byte(m);
           // 2^(127 - e): a subnormal for e = 254 alone, which exponent_byte does not reach
-          if (part < d.width) reinterpret_cast<uint2*>(row)[part] = quantised<T>(v[u], __uint_as_float((254u - e) << 23));
-          if (part == 0) d.scale[s * a.heads + head[u]] = (uint8_t)e;
+          if (part < d.width) reinterpret_cast<uint2*>(row)[part] = quantised<T>(v[u], __uint_as_float((254u - e) << 23), all_finite);
+          if (part == 0) d.scale[own[tok[u]] * a.heads + head[u]] = (uint8_t)e;
         } else if (part < d.width) {
           reinterpret_cast<uint4*>(row)[part] = v[u];
         }
@@ -190,6 +224,7 @@ struct ReadArgs {
   const int* ends;                           // [sequences + 1]
   int sequences, columns, pages;
   int T, heads, page, per_block;
+  Divide by_heads;
   int* err;
 };
 
@@ -208,8 +243,9 @@ __device__ __forceinline__ uint4 expanded(const uint8_t* row, int part, float sc
 }
 
 template <typename T, bool E4M3>
-__global__ void __launch_bounds__(THREADS) cache_read_kernel(const ReadArgs a) {
-  __shared__ int where[MAX_TOKENS][2];       // page and place in it, or -1: a row of zeros
+__global__ void __launch_bounds__(THREADS, 6) cache_read_kernel(const ReadArgs a) {
+  __shared__ long long own[MAX_TOKENS];      // page * (slots of a page) + place, or -1: a row of zeros
+  __shared__ long long base[2][MAX_TOKENS];  // and where it begins in the caches
   const long long t0 = (long long)blockIdx.x * a.per_block;
   const int n = (int)min((long long)a.per_block, a.T - t0);
   for (int i = threadIdx.x; i < n; i += THREADS) {
@@ -231,8 +267,8 @@ __global__ void __launch_bounds__(THREADS) cache_read_kernel(const ReadArgs a) {
         if (a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
       }
     }
-    where[i][0] = page;
-    where[i][1] = at;
+    own[i] = page < 0 ? -1 : (long long)page * a.page + at;
+    for (int w = 0; w < a.sides; ++w) base[w][i] = page * a.side[w].c_page + at * a.side[w].c_tok;
   }
   __syncthreads();
   for (int w = 0; w < a.sides; ++w) {
@@ -247,18 +283,18 @@ __global__ void __launch_bounds__(THREADS) cache_read_kernel(const ReadArgs a) {
         const int r = r0 + u * groups;
         v[u] = make_uint4(0, 0, 0, 0);
         if (r >= rows) continue;
-        const int tok = r / a.heads, head = r - tok * a.heads, page = where[tok][0], at = where[tok][1];
-        if (page < 0) continue;
-        const uint8_t* row = d.cache + page * d.c_page + at * d.c_tok + head * d.c_head;
+        const int tok = a.by_heads(r), head = r - tok * a.heads;
+        if (own[tok] < 0) continue;
+        const uint8_t* row = d.cache + base[w][tok] + head * d.c_head;
         float scale = 1.f;
-        if (E4M3) scale = power_of(__ldg(d.scale + ((long long)page * a.page + at) * a.heads + head));
+        if (E4M3) scale = power_of(__ldg(d.scale + own[tok] * a.heads + head));
         v[u] = expanded<T, E4M3>(row, part, scale);
       }
 #pragma unroll
       for (int u = 0; u < ROWS_AHEAD; ++u) {
         const int r = r0 + u * groups;
         if (r >= rows) continue;
-        const int tok = r / a.heads, head = r - tok * a.heads;
+        const int tok = a.by_heads(r), head = r - tok * a.heads;
         reinterpret_cast<uint4*>(const_cast<uint8_t*>(d.x) + (t0 + tok) * d.x_tok + head * d.x_head)[part] = v[u];
       }
     }
@@ -316,6 +352,7 @@ static int common(A& a, void* k, void* v, void* kc, void* vc, void* k_scale, voi
   if (vdim) a.side[a.sides++] = side_of(v, n + 2, vc, n + 7, v_scale, vdim, es);
   a.T = (int)n[10];
   a.heads = (int)n[11];
+  a.by_heads = Divide(a.heads);
   a.page = (int)n[15];
   return 0;
 }

@@ -31,7 +31,7 @@ def declare(L: ctypes.CDLL) -> None:
         if hasattr(L, name):
             getattr(L, name).argtypes, getattr(L, name).restype = args, i32
     if hasattr(L, "cm_paged_attention_ws"):
-        L.cm_paged_attention_ws.argtypes, L.cm_paged_attention_ws.restype = [i32] * 7, i64
+        L.cm_paged_attention_ws.argtypes, L.cm_paged_attention_ws.restype = [i32] * 8, i64
 
 
 class Plan:
@@ -161,7 +161,7 @@ def _plan_attention(q, k_cache, v_cache, table, lens, k_scale, v_scale):
     return Plan([*strides(q), *strides(k_cache), *strides(v_cache), table.stride(0), B, heads, group, columns, pages, page, dim, vdim,
                  TYPES[q.dtype], int(e4m3)],
                 copy=not (rows_on(q, 16) and (table.stride(-1) == 1 or columns <= 1) and lens.is_contiguous()), shape=(B, H, vdim),
-                work=_cu.lib().cm_paged_attention_ws(B, heads, group, dim, vdim, columns, page) if B else 0,
+                work=_cu.lib().cm_paged_attention_ws(B, heads, group, dim, vdim, columns, page, int(e4m3)) if B else 0,
                 like=q.is_contiguous() and vdim == dim)
 
 
