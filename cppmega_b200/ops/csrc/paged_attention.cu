@@ -42,7 +42,8 @@ struct Args {
   const uint8_t* q;                          // [sequences, heads, dim]
   long long q_seq, q_head;                   // bytes
   const uint8_t *k, *v;                      // [pages, page, kv_heads, .]
-  long long k_page, k_tok, k_head, v_page, v_tok, v_head;      // bytes
+  long long k_page, v_page;                  // bytes
+  int k_tok, k_head, v_tok, v_head;          // bytes
   const uint8_t *k_scale, *v_scale;          // [pages, page, kv_heads] or null
   const int* table;
   long long table_row;
@@ -65,6 +66,9 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ void copy_piece(uint32_t dst, const uint8_t* src, bool there) {
   // what is not there becomes zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_whole(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -255,6 +259,7 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
   const int kc = lane % KC, kr = lane / KC, vc = lane % VC, vr = lane / VC;
   const bool k_exists = kc * 16 < a.dim * (E4M3 ? 1 : 2), v_exists = vc * 16 < a.vdim * (E4M3 ? 1 : 2);
   // where the copies go: K by (eight keys, piece of four lanes), V by (row of a lane's fragment, piece of eight lanes)
+  const uint8_t *k_lane = a.k + kr * a.k_tok + kc * 16, *v_lane = a.v + vr * a.v_tok + vc * 16;
   const uint32_t k_dst = (kc >> 2) * 512 + ((kr * 4 + (kc & 3)) ^ ((kc >> 2 & 1) * 4)) * 16;
   auto v_dst = [&](int i) {
     const int key = i * (32 / VC) + vr, quad_of = key >> 1 & 3, y = (key & 1) | (key >> 3 << 1);
@@ -269,23 +274,31 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
       if (a.aligned) {
         if (!known && a.err && lane == 0) atomicCAS(a.err, 0, ERR_BAD_ARG);
         const int keys = known ? room : 0;
-        const uint8_t* ks = known ? a.k + page * a.k_page + (in + kr) * a.k_tok + head * a.k_head + kc * 16 : a.k;
-        const uint8_t* vs = known ? a.v + page * a.v_page + (in + vr) * a.v_tok + head * a.v_head + vc * 16 : a.v;
+        const uint8_t* ks = k_lane + page * a.k_page + (long long)in * a.k_tok + (long long)head * a.k_head;
+        const uint8_t* vs = v_lane + page * a.v_page + (long long)in * a.v_tok + (long long)head * a.v_head;
         if (E4M3 && lane < KEYS) rows_of[stage * KEYS + lane] = lane < keys ? ((long long)page * a.page + in + lane) * a.kv_heads + head : -1;
+        if (keys >= KEYS && a.dim == D && a.vdim == DV) {     // nothing to leave out
 #pragma unroll
-        for (int i = 0; i < KC / 2; ++i) {
-          const bool there = k_exists && i * (32 / KC) + kr < keys;
-          copy_piece(k_to + (i * (32 / KC) >> 3) * F::K_PIECES * 512 + (i * (32 / KC) & 7) * 64, there ? ks + i * (32 / KC) * a.k_tok : a.k, there);
-        }
+          for (int i = 0; i < KC / 2; ++i, ks += 32 / KC * a.k_tok)
+            copy_whole(k_to + (i * (32 / KC) >> 3) * F::K_PIECES * 512 + (i * (32 / KC) & 7) * 64, ks);
 #pragma unroll
-        for (int i = 0; i < VC / 2; ++i) {
-          const bool there = v_exists && i * (32 / VC) + vr < keys;
-          copy_piece(v_to + v_dst(i), there ? vs + i * (32 / VC) * a.v_tok : a.v, there);
+          for (int i = 0; i < VC / 2; ++i, vs += 32 / VC * a.v_tok) copy_whole(v_to + v_dst(i), vs);
+        } else {
+#pragma unroll
+          for (int i = 0; i < KC / 2; ++i, ks += 32 / KC * a.k_tok) {
+            const bool there = k_exists && i * (32 / KC) + kr < keys;
+            copy_piece(k_to + (i * (32 / KC) >> 3) * F::K_PIECES * 512 + (i * (32 / KC) & 7) * 64, there ? ks : a.k, there);
+          }
+#pragma unroll
+          for (int i = 0; i < VC / 2; ++i, vs += 32 / VC * a.v_tok) {
+            const bool there = v_exists && i * (32 / VC) + vr < keys;
+            copy_piece(v_to + v_dst(i), there ? vs : a.v, there);
+          }
         }
       } else {
         const bool there = (lane & 15) < room && known;
-        const long long ko = there ? page * a.k_page + in * a.k_tok + head * a.k_head : -1;
-        const long long vo = there ? page * a.v_page + in * a.v_tok + head * a.v_head : -1;
+        const long long ko = there ? page * a.k_page + (long long)in * a.k_tok + (long long)head * a.k_head : -1;
+        const long long vo = there ? page * a.v_page + (long long)in * a.v_tok + (long long)head * a.v_head : -1;
         if (!known && (lane & 15) < room && a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
         if (E4M3 && lane < KEYS) rows_of[stage * KEYS + lane] = there ? ((long long)page * a.page + in) * a.kv_heads + head : -1;
 #pragma unroll
@@ -624,14 +637,12 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
   copies_but<0>();
 }
 
-constexpr int JOIN_WARPS = 8;
-constexpr int JOIN_PIECES = 256;             // pieces weighed at once
-
 // The pieces of each pair become its result: a block per (sequence, head).  Piece numbers: run r leaves piece r + s of pair s, which no other
 // pair of r and s shares along the sequence of steps.  All maxima are read first, so that the accumulators come without waiting for one another.
-template <bool BF16, int DV>
+template <bool BF16, int DV, int JOIN_WARPS>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const Args a, int tile_rows) {
-  constexpr int C = DV / 32, AHEAD = 4;      // columns of a lane
+  constexpr int C = DV / 32, AHEAD = 8;      // columns of a lane
+  constexpr int JOIN_PIECES = JOIN_WARPS * 32;                // pieces weighed at once
   __shared__ float part[JOIN_WARPS][DV], weight[JOIN_PIECES], tops[JOIN_WARPS], sums[JOIN_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / (a.kv_heads * a.group), hq = blockIdx.x % (a.kv_heads * a.group), h = hq / a.group, head = hq % a.group;
@@ -677,8 +688,14 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const Args a, int
       for (int u = 0; u < AHEAD; ++u) {
         const int at = k + u * JOIN_WARPS;
         w[u] = at < here ? weight[at] : 0.f;
-#pragma unroll
-        for (int c = 0; c < C; ++c) v[u][c] = at < here ? base[(i0 + at) * pitch + 4 + lane * C + c] : 0.f;
+        const float* src = base + (i0 + (at < here ? at : 0)) * pitch + 4 + lane * C;
+        if (C == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src);
+          v[u][0] = x.x; v[u][1] = x.y; v[u][C - 2] = x.z; v[u][C - 1] = x.w;
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(src);
+          v[u][0] = x.x; v[u][1] = x.y;
+        }
       }
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u)
@@ -703,6 +720,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const Args a, int
   reinterpret_cast<uint32_t*>(a.out)[((long long)blockIdx.x * a.vdim + col) >> 1] = pair<BF16>(x * inv, y * inv);
 }
 
+constexpr bool NT2 = true;
 struct Layout {
   int nt, tiles, rows, grid, warps, dim, vdim, side, chunks, runs;
   long long floats;
@@ -714,7 +732,7 @@ Layout layout_of(int sequences, int kv_heads, int group, int dim, int vdim, int 
   Layout s;
   s.vdim = vdim <= 64 ? 64 : 128;
   s.dim = dim <= 64 && s.vdim == 64 ? 64 : 128;
-  s.nt = group <= 8 ? 1 : group <= 16 || s.vdim == 128 ? 2 : 4;
+  s.nt = group <= 8 ? 1 : group <= 16 || s.vdim == 128 || NT2 ? 2 : 4;
   s.tiles = 1;
   while (s.tiles * 8 * s.nt < group) s.tiles *= 2;
   s.warps = warps_of(e4m3, s.dim, s.vdim, s.nt);
@@ -749,8 +767,10 @@ int start(const Args& a, int grid, cudaStream_t stream) {
     kern<<<grid, F::WARPS * 32, smem, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return -3;
   }
-  const dim3 blocks((unsigned)(a.sequences * a.kv_heads * a.group));
-  return few::launch_early(join_kernel<BF16, DV>, blocks, dim3(JOIN_WARPS * 32), 0, stream, a, 8 * NT);
+  // few blocks have many pieces each: 16 warps read them side by side (131071 tokens, 222 pieces: JOINLONG), many blocks have few
+  const int blocks = a.sequences * a.kv_heads * a.group;
+  if (blocks <= 2 * sm_count()) return few::launch_early(join_kernel<BF16, DV, 16>, dim3(blocks), dim3(512), 0, stream, a, 8 * NT);
+  return few::launch_early(join_kernel<BF16, DV, 4>, dim3(blocks), dim3(128), 0, stream, a, 8 * NT);
 }
 
 template <bool BF16, bool E4M3>
@@ -780,7 +800,7 @@ extern "C" long long cm_paged_attention_ws(int sequences, int kv_heads, int grou
 // lens [sequences]; out [sequences, kv_heads * group, vdim] packed; ws: cm_paged_attention_ws floats.  Sizes and strides (elements) come in n:
 //   strides of q's sequences and heads, of pages, tokens and heads of the key cache, then of the value cache, of the table's rows;
 //   sequences, kv_heads, group, columns, pages, page, dim, vdim, kind (0 bf16, 1 fp16; a 16-bit cache has the same type), e4m3.
-// dim, vdim multiples of 8 (16 in an E4M3 cache) up to 128, group up to 128.
+// dim, vdim multiples of 8 (16 in an E4M3 cache) up to 128, group up to 128; steps between tokens and heads below 2^31 bytes.
 extern "C" int cm_paged_attention(const void* q, const void* k, const void* v, const void* k_scale, const void* v_scale, const int* table,
                                   const int* lens, void* out, float* ws, const long long* n, float scale, int* err, cudaStream_t stream) {
   const long long sequences = n[9], kv_heads = n[10], group = n[11], columns = n[12], pages = n[13], page = n[14], dim = n[15], vdim = n[16];
@@ -790,14 +810,16 @@ extern "C" int cm_paged_attention(const void* q, const void* k, const void* v, c
   if (group < 1 || group > 128 || dim < step || dim > 128 || dim % step || vdim < step || vdim > 128 || vdim % step || page < 1 || columns < 0 ||
       columns * page > 0x7fffffffLL - KEYS || sequences * kv_heads * group > 0x7fffffffLL)
     return -10;
+  for (int i : {3, 4, 6, 7})
+    if (n[i] < -(1ll << 30) || n[i] >= 1ll << 30) return -10;
   const Layout s = layout_of((int)sequences, (int)kv_heads, (int)group, (int)dim, (int)vdim, (int)columns, (int)page, e4m3);
   Args a;
   a.q = (const uint8_t*)q;
   a.q_seq = n[0] * 2; a.q_head = n[1] * 2;
   a.k = (const uint8_t*)k;
   a.v = (const uint8_t*)v;
-  a.k_page = n[2] * es; a.k_tok = n[3] * es; a.k_head = n[4] * es;
-  a.v_page = n[5] * es; a.v_tok = n[6] * es; a.v_head = n[7] * es;
+  a.k_page = n[2] * es; a.k_tok = int(n[3] * es); a.k_head = int(n[4] * es);
+  a.v_page = n[5] * es; a.v_tok = int(n[6] * es); a.v_head = int(n[7] * es);
   a.k_scale = (const uint8_t*)k_scale;
   a.v_scale = (const uint8_t*)v_scale;
   a.table = table;

@@ -12,8 +12,8 @@
 // E4M3 row), so rows of any stride move in whole sectors, and four rows of every lane group are in flight at once.
 //
 // Of tokens that are given the same slot the last one stays, whatever order the blocks run in: each block looks for its own slots among the
-// later tokens (a bit table in shared memory answers for almost all of them).  It reads the list of slots once per block, 5 % of the bytes
-// that move at 16384 tokens of 8 heads.
+// later tokens (a hash table of its own in shared memory).  It reads the list of slots once per block, 5 % of the bytes that move at 16384
+// tokens of 8 heads.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -26,7 +26,8 @@ namespace paged {
 
 constexpr int THREADS = 256;
 constexpr int MAX_TOKENS = 128;              // tokens of one block
-constexpr int HASH_BITS = 8192;
+constexpr int TABLE = 2048;                  // places of the hash table
+constexpr int FREE = -1, SHARED = -2;        // a place that no slot, or more than one, falls to
 constexpr int ROWS_AHEAD = 4;
 constexpr int SCAN = 8;                      // later slots that a thread has on their way at once
 
@@ -39,12 +40,15 @@ struct Divide {
 
 struct Side {                                // keys or values
   const uint8_t* x;                          // rows of the packed tensor
-  long long x_tok, x_head;                   // strides in bytes
   uint8_t* cache;
-  long long c_page, c_tok, c_head;           // strides in bytes
   uint8_t* scale;                            // [pages, page, heads] or null
-  int lanes, width;                          // lanes of a row, 16-byte pieces of the packed row (8 values each)
+  long long c_page;                          // strides in bytes
+  int x_tok, x_head, c_tok, c_head;
+  int lanes, width;                          // lanes of a row (8, 16 or 32), 16-byte pieces of the packed row (8 values each)
 };
+
+__device__ __forceinline__ uint32_t place_of(long long slot) { return (uint32_t(slot) * 2654435769u) >> 21; }
+static_assert(TABLE == 1 << 11, "place_of");
 
 struct WriteArgs {
   Side side[2];
@@ -128,16 +132,64 @@ __device__ float largest_finite(const uint4& v) {
   return m;
 }
 
-// T: the packed rows' type; E4M3: what the cache holds (the same type otherwise)
+// T: the packed rows' type; E4M3: what the cache holds (the same type otherwise); LANES: of a row.  The block's tokens of one side.
+template <typename T, bool E4M3, int LANES>
+__device__ __forceinline__ void write_rows(const Side& d, const Divide& by_heads, int heads, int n, long long t0, const long long* own, const int* lost,
+                                           const long long* base) {
+  constexpr int GROUPS = THREADS / LANES;
+  const int group = threadIdx.x / LANES, part = threadIdx.x % LANES, rows = n * heads;
+  const uint8_t* x = d.x + t0 * d.x_tok + part * 16;
+  uint8_t* cache = d.cache + part * (E4M3 ? 8 : 16);
+  const bool exists = part < d.width;
+  // whole rounds, so that the lanes of a warp meet in the shuffles
+  for (int r0 = group; r0 - group < rows; r0 += GROUPS * ROWS_AHEAD) {
+    uint4 v[ROWS_AHEAD];
+    int tok[ROWS_AHEAD], head[ROWS_AHEAD];
+#pragma unroll
+    for (int u = 0; u < ROWS_AHEAD; ++u) {
+      const int r = r0 + u * GROUPS;
+      v[u] = make_uint4(0, 0, 0, 0);
+      tok[u] = by_heads(r);
+      head[u] = r - tok[u] * heads;
+      if (r >= rows || own[tok[u]] < 0 || lost[tok[u]]) tok[u] = -1;
+      else if (exists) v[u] = __ldg(reinterpret_cast<const uint4*>(x + (long long)tok[u] * d.x_tok + (long long)head[u] * d.x_head));
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS_AHEAD; ++u) {
+      uint8_t* row = cache + base[tok[u] < 0 ? 0 : tok[u]] + (long long)head[u] * d.c_head;
+      if (!E4M3) {
+        if (tok[u] >= 0 && exists) *reinterpret_cast<uint4*>(row) = v[u];
+        continue;
+      }
+      uint32_t most = largest_bits(v[u]);
+#pragma unroll
+      for (int o = LANES >> 1; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+      most = max(most & 0xffffu, most >> 16);
+      const bool all_finite = most < first_not_finite<T>();
+      float m = two<T>(most).x;
+      if (!__all_sync(0xffffffffu, all_finite)) {             // the row's largest finite one
+        m = largest_finite<T>(v[u]);
+#pragma unroll
+        for (int o = LANES >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      }
+      if (tok[u] < 0) continue;
+      const int e = exponent_byte(m);
+      // 2^(127 - e): a subnormal for e = 254 alone, which exponent_byte does not reach
+      if (exists) *reinterpret_cast<uint2*>(row) = quantised<T>(v[u], __uint_as_float((254u - e) << 23), all_finite);
+      if (part == 0) d.scale[own[tok[u]] * heads + head[u]] = (uint8_t)e;
+    }
+  }
+}
+
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(THREADS, 4) cache_write_kernel(const WriteArgs a) {
-  __shared__ uint32_t bits[HASH_BITS / 32];
+  __shared__ int table[TABLE];               // hash place -> token of this block
   __shared__ long long own[MAX_TOKENS];      // the slot, or -1: not written
   __shared__ long long base[2][MAX_TOKENS];  // and where it begins in the caches
   __shared__ int lost[MAX_TOKENS];           // a later token has the same slot
   const long long t0 = (long long)blockIdx.x * a.per_block;
   const int n = (int)min((long long)a.per_block, a.T - t0);
-  for (int i = threadIdx.x; i < HASH_BITS / 32; i += THREADS) bits[i] = 0;
+  for (int i = threadIdx.x; i < TABLE; i += THREADS) table[i] = FREE;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += THREADS) {
     long long s = slot_of(a, t0 + i);
@@ -148,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 4) cache_write_kernel(const WriteArgs
     own[i] = s < 0 ? -1 : s;
     lost[i] = 0;
     if (s >= 0) {
-      atomicOr(&bits[(s & (HASH_BITS - 1)) >> 5], 1u << (s & 31));
+      if (atomicCAS(&table[place_of(s)], FREE, i) != FREE) table[place_of(s)] = SHARED;
       const long long page = s / a.page, in = s - page * a.page;
       for (int w = 0; w < a.sides; ++w) base[w][i] = page * a.side[w].c_page + in * a.side[w].c_tok;
     }
@@ -159,60 +211,22 @@ __global__ void __launch_bounds__(THREADS, 4) cache_write_kernel(const WriteArgs
 #pragma unroll
     for (int c = 0; c < SCAN; ++c) s[c] = t + c * THREADS < a.T ? slot_of(a, t + c * THREADS) : -1;
 #pragma unroll
-    for (int c = 0; c < SCAN; ++c)
-      if (s[c] >= 0 && (bits[(s[c] & (HASH_BITS - 1)) >> 5] >> (s[c] & 31) & 1)) {
-        const int before = (int)min((long long)n, t + c * THREADS - t0);
+    for (int c = 0; c < SCAN; ++c) {
+      const int at = s[c] < 0 ? FREE : table[place_of(s[c])], before = (int)min((long long)n, t + c * THREADS - t0);
+      if (at >= 0) {
+        if (at < before && own[at] == s[c]) lost[at] = 1;
+      } else if (at == SHARED) {
         for (int i = 0; i < before; ++i)
           if (own[i] == s[c]) lost[i] = 1;
       }
+    }
   }
   __syncthreads();
-
   for (int w = 0; w < a.sides; ++w) {
     const Side& d = a.side[w];
-    const int group = threadIdx.x / d.lanes, part = threadIdx.x % d.lanes, groups = THREADS / d.lanes;
-    const int rows = n * a.heads;
-    // whole rounds, so that the lanes of a warp meet in the shuffles
-    for (int r0 = 0; r0 < rows; r0 += groups * ROWS_AHEAD) {
-      uint4 v[ROWS_AHEAD];
-      int tok[ROWS_AHEAD], head[ROWS_AHEAD];
-#pragma unroll
-      for (int u = 0; u < ROWS_AHEAD; ++u) {
-        const int r = r0 + u * groups + group;
-        v[u] = make_uint4(0, 0, 0, 0);
-        tok[u] = a.by_heads(r);
-        head[u] = r - tok[u] * a.heads;
-        if (r >= rows || own[tok[u]] < 0 || lost[tok[u]]) tok[u] = -1;
-        else if (part < d.width)
-          v[u] = __ldg(reinterpret_cast<const uint4*>(d.x + (t0 + tok[u]) * d.x_tok + head[u] * d.x_head) + part);
-      }
-#pragma unroll
-      for (int u = 0; u < ROWS_AHEAD; ++u) {
-        float m = 0.f;
-        bool all_finite = true;
-        if (E4M3) {
-          uint32_t x = largest_bits(v[u]);
-          for (int o = d.lanes >> 1; o > 0; o >>= 1) x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, o));
-          x = max(x & 0xffffu, x >> 16);
-          all_finite = x < first_not_finite<T>();
-          m = two<T>(x).x;
-          if (!__all_sync(0xffffffffu, all_finite)) {         // the row's largest finite one
-            m = largest_finite<T>(v[u]);
-            for (int o = d.lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          }
-        }
-        if (tok[u] < 0) continue;
-        uint8_t* row = d.cache + base[w][tok[u]] + head[u] * d.c_head;
-        if (E4M3) {
-          const int e = exponent_byte(m);
-          // 2^(127 - e): a subnormal for e = 254 alone, which exponent_byte does not reach
-          if (part < d.width) reinterpret_cast<uint2*>(row)[part] = quantised<T>(v[u], __uint_as_float((254u - e) << 23), all_finite);
-          if (part == 0) d.scale[own[tok[u]] * a.heads + head[u]] = (uint8_t)e;
-        } else if (part < d.width) {
-          reinterpret_cast<uint4*>(row)[part] = v[u];
-        }
-      }
-    }
+    if (d.lanes == 8) write_rows<T, E4M3, 8>(d, a.by_heads, a.heads, n, t0, own, lost, base[w]);
+    else if (d.lanes == 16) write_rows<T, E4M3, 16>(d, a.by_heads, a.heads, n, t0, own, lost, base[w]);
+    else write_rows<T, E4M3, 32>(d, a.by_heads, a.heads, n, t0, own, lost, base[w]);
   }
 }
 
@@ -228,10 +242,10 @@ struct ReadArgs {
   int* err;
 };
 
-template <typename T, bool E4M3>
-__device__ __forceinline__ uint4 expanded(const uint8_t* row, int part, float scale) {
-  if (!E4M3) return __ldg(reinterpret_cast<const uint4*>(row) + part);
-  const uint2 v = __ldg(reinterpret_cast<const uint2*>(row) + part);
+// eight E4M3 values (x, y) times the power of their exponent byte (z)
+template <typename T>
+__device__ __forceinline__ uint4 expanded(const uint4& v) {
+  const float scale = power_of(v.z);
   uint32_t o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -240,6 +254,43 @@ __device__ __forceinline__ uint4 expanded(const uint8_t* row, int part, float sc
     o[i] = join<T>(f.x * scale, f.y * scale);
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+template <typename T, bool E4M3, int LANES>
+__device__ __forceinline__ void read_rows(const Side& d, const Divide& by_heads, int heads, int n, long long t0, const long long* own,
+                                          const long long* base) {
+  constexpr int GROUPS = THREADS / LANES;
+  const int group = threadIdx.x / LANES, part = threadIdx.x % LANES, rows = n * heads;
+  if (part >= d.width) return;
+  uint8_t* x = const_cast<uint8_t*>(d.x) + t0 * d.x_tok + part * 16;
+  const uint8_t* cache = d.cache + part * (E4M3 ? 8 : 16);
+  for (int r0 = group; r0 < rows; r0 += GROUPS * ROWS_AHEAD) {
+    uint4 v[ROWS_AHEAD];                     // of an E4M3 row: eight values and its exponent byte
+    int tok[ROWS_AHEAD], head[ROWS_AHEAD];
+#pragma unroll
+    for (int u = 0; u < ROWS_AHEAD; ++u) {
+      const int r = r0 + u * GROUPS;
+      v[u] = make_uint4(0, 0, 127, 0);
+      if (!E4M3) v[u].z = 0;
+      tok[u] = by_heads(r);
+      head[u] = r - tok[u] * heads;
+      if (r >= rows || own[tok[u]] < 0) continue;
+      const uint8_t* row = cache + base[tok[u]] + (long long)head[u] * d.c_head;
+      if (E4M3) {
+        const uint2 b = __ldg(reinterpret_cast<const uint2*>(row));
+        v[u].x = b.x;
+        v[u].y = b.y;
+        v[u].z = __ldg(d.scale + own[tok[u]] * heads + head[u]);
+      } else {
+        v[u] = __ldg(reinterpret_cast<const uint4*>(row));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS_AHEAD; ++u) {
+      if (r0 + u * GROUPS >= rows) continue;
+      *reinterpret_cast<uint4*>(x + (long long)tok[u] * d.x_tok + (long long)head[u] * d.x_head) = E4M3 ? expanded<T>(v[u]) : v[u];
+    }
+  }
 }
 
 template <typename T, bool E4M3>
@@ -273,31 +324,9 @@ __global__ void __launch_bounds__(THREADS, 6) cache_read_kernel(const ReadArgs a
   __syncthreads();
   for (int w = 0; w < a.sides; ++w) {
     const Side& d = a.side[w];
-    const int group = threadIdx.x / d.lanes, part = threadIdx.x % d.lanes, groups = THREADS / d.lanes;
-    if (part >= d.width) continue;
-    const int rows = n * a.heads;
-    for (int r0 = group; r0 < rows; r0 += groups * ROWS_AHEAD) {
-      uint4 v[ROWS_AHEAD];
-#pragma unroll
-      for (int u = 0; u < ROWS_AHEAD; ++u) {
-        const int r = r0 + u * groups;
-        v[u] = make_uint4(0, 0, 0, 0);
-        if (r >= rows) continue;
-        const int tok = a.by_heads(r), head = r - tok * a.heads;
-        if (own[tok] < 0) continue;
-        const uint8_t* row = d.cache + base[w][tok] + head * d.c_head;
-        float scale = 1.f;
-        if (E4M3) scale = power_of(__ldg(d.scale + own[tok] * a.heads + head));
-        v[u] = expanded<T, E4M3>(row, part, scale);
-      }
-#pragma unroll
-      for (int u = 0; u < ROWS_AHEAD; ++u) {
-        const int r = r0 + u * groups;
-        if (r >= rows) continue;
-        const int tok = a.by_heads(r), head = r - tok * a.heads;
-        reinterpret_cast<uint4*>(const_cast<uint8_t*>(d.x) + (t0 + tok) * d.x_tok + head * d.x_head)[part] = v[u];
-      }
-    }
+    if (d.lanes == 8) read_rows<T, E4M3, 8>(d, a.by_heads, a.heads, n, t0, own, base[w]);
+    else if (d.lanes == 16) read_rows<T, E4M3, 16>(d, a.by_heads, a.heads, n, t0, own, base[w]);
+    else read_rows<T, E4M3, 32>(d, a.by_heads, a.heads, n, t0, own, base[w]);
   }
 }
 
@@ -311,16 +340,15 @@ static int tokens_per_block(int T, int resident) {
 static Side side_of(const void* x, const long long* xs, void* cache, const long long* cs, void* scale, int width, int esize) {
   Side d;
   d.x = (const uint8_t*)x;
-  d.x_tok = xs[0] * 2;
-  d.x_head = xs[1] * 2;
+  d.x_tok = int(xs[0] * 2);
+  d.x_head = int(xs[1] * 2);
   d.cache = (uint8_t*)cache;
   d.c_page = cs[0] * esize;
-  d.c_tok = cs[1] * esize;
-  d.c_head = cs[2] * esize;
+  d.c_tok = int(cs[1] * esize);
+  d.c_head = int(cs[2] * esize);
   d.scale = (uint8_t*)scale;
   d.width = width / 8;
-  d.lanes = 1;
-  while (d.lanes < d.width) d.lanes *= 2;
+  d.lanes = d.width <= 8 ? 8 : d.width <= 16 ? 16 : 32;
   return d;
 }
 
@@ -341,12 +369,15 @@ using namespace cm::paged;
 //   k_tok, k_head, v_tok, v_head of the packed rows; page, token and head strides of the key cache, then of the value cache;
 //   T, heads, dim, vdim (0: no values), pages, page, kind (0 bf16, 1 fp16), e4m3, then what the function says.
 // Packed rows k [T, heads, dim], v [T, heads, vdim]; caches [pages, page, heads, .]; with e4m3 the caches hold E4M3 and k_scale, v_scale
-// [pages, page, heads] their exponent bytes.  Widths are multiples of 8 up to 256; rows on 16 bytes (8 in an E4M3 cache).
+// [pages, page, heads] their exponent bytes.  Widths are multiples of 8 up to 256; rows on 16 bytes (8 in an E4M3 cache); all strides but
+// those of pages below 2^31 bytes.
 template <typename A>
 static int common(A& a, void* k, void* v, void* kc, void* vc, void* k_scale, void* v_scale, const long long* n) {
   const int es = n[17] ? 1 : 2, dim = (int)n[12], vdim = (int)n[13];
   if (dim < 8 || dim % 8 || dim > 256 || vdim < 0 || vdim % 8 || vdim > 256 || n[15] < 1 || n[14] < 0) return -10;
   if (n[17] && (!k_scale || (vdim && !v_scale))) return -10;
+  for (int i : {0, 1, 2, 3, 5, 6, 8, 9})
+    if (n[i] < -(1ll << 30) || n[i] >= 1ll << 30) return -10;
   a.side[0] = side_of(k, n, kc, n + 4, k_scale, dim, es);
   a.sides = 1;
   if (vdim) a.side[a.sides++] = side_of(v, n + 2, vc, n + 7, v_scale, vdim, es);

@@ -67,7 +67,12 @@ def rows_on(t, align: int) -> bool:
     if t is None:
         return True
     es = t.element_size()
-    return (t.shape[-1] == 1 or t.stride(-1) == 1) and all(s * es % align == 0 for s in t.stride()[:-1])
+    return (t.shape[-1] == 1 or t.stride(-1) == 1) and all(s * es % align == 0 for s in t.stride()[:-1]) and near(t)
+
+
+def near(t) -> bool:
+    """Steps between tokens and heads are 32-bit numbers of bytes in the kernels; those between pages are not."""
+    return all(s < 2 ** 30 for s in (t.stride()[1:] if t.dim() == 4 else t.stride()))
 
 
 def width_ok(t, step: int, most: int) -> bool:
