@@ -23,8 +23,9 @@
 // orientation are operands in TMEM that never pass through shared memory, every sum has one owner, and the bits are the same each time.
 //   dq     block per query tile, loops over key tiles:   S = Q K', dP = dO V', dQ += dS K
 //   dk dv  block per key tile, loops over query tiles:   S' = K Q', dP' = V dO', dV += P' dO, dK += dS' Q
-// The issuing thread polls what each product waits for and issues whichever is ready, so the products of one tile fill the pauses of
-// another; a product that overwrites columns is issued only after the commit of the one that reads them.
+// The issuing threads take the products in a fixed order (the bits are the same each time) in which each has its operands before the one in front
+// of it is done; a product that overwrites columns is issued after the commit of the one that reads them.  One thread that polled for
+// whatever was ready first spent more time on polling than the products took (forward 2100 cycles a 128 x 128 tile).
 // Query tiles of the key gradients run from the last one down: blocks of one sequence then read the same rows at the same time, out of L2.
 //
 // Roundings to 16 bits: P and dS, as operands of their products.  delta takes o before its rounding (the forward keeps what that takes away,
@@ -40,6 +41,7 @@ namespace packed {
 namespace {
 
 constexpr int TILE = 128;
+constexpr int PART = 64;                     // columns of scores that are multiplied and waited for as one
 constexpr int SLAB = 128 * 128;              // bytes of one [128 rows x 64 columns] slab, 128-byte swizzle
 constexpr float RESCALE_AT = 8.f;            // log2
 
@@ -47,10 +49,12 @@ constexpr float RESCALE_AT = 8.f;            // log2
 __host__ __device__ constexpr uint32_t idesc(bool half, int n, bool b_mn) {        // M 128, A K-major
   return (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(TILE >> 4) << 24);
 }
-// 16-column step k of a K-major operand whose slabs lie one after the other
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int k) { return umma_desc_sw128(tile + (k >> 2) * SLAB + (k & 3) * 32, 16, 1024); }
-// 16-row step k of the same slabs read MN-major
-__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int k) { return umma_desc_sw128(tile + k * 2048, SLAB, 1024); }
+// Descriptors of a slab, to whose low word the steps below are added: one base for an operand, since both orientations have the same row pitch
+__device__ __forceinline__ uint64_t base_k(uint32_t tile) { return umma_desc_sw128(tile, 16, 1024); }
+__device__ __forceinline__ uint64_t base_mn(uint32_t tile) { return umma_desc_sw128(tile, SLAB, 1024); }
+// 16-column step k of a K-major operand whose slabs lie one after the other; 16-row step k of the same slabs read MN-major
+__device__ __forceinline__ constexpr uint32_t step_k(int k) { return uint32_t((k >> 2) * SLAB + (k & 3) * 32) >> 4; }
+__device__ __forceinline__ constexpr uint32_t step_mn(int k) { return uint32_t(k * 2048) >> 4; }
 // A in TMEM (row = lane, two 16-bit values of K per column)
 __device__ __forceinline__ void umma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
   asm volatile(
@@ -89,31 +93,15 @@ __device__ __forceinline__ void tma_rows(void* dst, const CUtensorMap* map, uint
 }
 
 // ---- waits -----------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ bool ready(uint64_t* bar, int parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-  return ok;
-}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
 }
-// Bounds a loop that polls: false once it has turned for too long without anything becoming ready, or another role has given up
-struct Patience {
-  unsigned long long since = 0;
-  uint32_t idle = 0;
-  __device__ __forceinline__ bool more(bool moved, volatile int* abort_flag, int* err) {
-    if (moved) { idle = 0; since = 0; return true; }
-    if ((++idle & 63u) != 0) return true;
-    if (*abort_flag) return false;
-    if (err && *reinterpret_cast<volatile int*>(err) != 0) { *abort_flag = 1; return false; }
-    const unsigned long long now = cm_globaltimer();
-    if (!since) { since = now; return true; }
-    if (now - since <= CM_WAIT_NS) return true;
-    *abort_flag = 1;
-    if (err) atomicCAS(err, 0, ERR_WAIT_TMEM_FULL);
-    return false;
+// A place in a ring of slots, and the parity of its round
+template <int SLOTS>
+struct Ring {
+  int at = 0, round = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == SLOTS) { at = 0; round ^= 1; }
   }
 };
 
@@ -244,15 +232,15 @@ struct Whole { static constexpr bool value = false; };
 // ---- forward ---------------------------------------------------------------------------------------------------------
 constexpr int THREADS = 320;                 // eight compute warps, one that issues products, one that loads
 constexpr int MMA_WARP = 8, TMA_WARP = 9;
+constexpr int FWD_THREADS = 352, FWD_TMA_WARP = 10;           // forward: an issuing warp for each query tile (8 and 9)
 
 template <int D, int DV>
 struct Fwd {
   static constexpr int KS = D / 64, VS = DV / 64;
   static constexpr int K_SLOTS = 3, V_SLOTS = DV == 128 ? 2 : 3;
-  static constexpr bool P_OVER_S = DV == 128;                 // no columns left for P: it takes the place of the scores it came from
   struct Shared {
     uint64_t q_full[2], k_full[K_SLOTS], k_empty[K_SLOTS], v_full[V_SLOTS], v_empty[V_SLOTS], tail;
-    uint64_t s_full[2], s_free[2], p_full[2], o_done[2];
+    uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];       // query tile, half of the key tile
     Unit unit;
     uint32_t tmem_slot;
     int abort_flag;
@@ -261,7 +249,7 @@ struct Fwd {
 };
 
 template <bool HALF, int D, int DV>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(FWD_THREADS, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const Args a) {
   using F = Fwd<D, DV>;
@@ -282,13 +270,14 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (tid == 32) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh->q_full[t], 1);
-      mbar_init(&sh->s_full[t], 1);
-      mbar_init(&sh->s_free[t], 4);
-      mbar_init(&sh->p_full[t], 4);
-      mbar_init(&sh->o_done[t], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&sh->s_full[t][b], 1);
+        mbar_init(&sh->p_full[t][b], 4);
+        mbar_init(&sh->pv_done[t][b], 1);
+      }
     }
-    for (int s = 0; s < F::K_SLOTS; ++s) { mbar_init(&sh->k_full[s], 1); mbar_init(&sh->k_empty[s], 1); }
-    for (int s = 0; s < F::V_SLOTS; ++s) { mbar_init(&sh->v_full[s], 1); mbar_init(&sh->v_empty[s], 1); }
+    for (int s = 0; s < F::K_SLOTS; ++s) { mbar_init(&sh->k_full[s], 1); mbar_init(&sh->k_empty[s], 2); }
+    for (int s = 0; s < F::V_SLOTS; ++s) { mbar_init(&sh->v_full[s], 1); mbar_init(&sh->v_empty[s], 2); }
     mbar_init(&sh->tail, 1);
     sh->abort_flag = 0;
     fence_mbar_init();
@@ -297,7 +286,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   tc_fence_before();
   const bool drain = setup_barrier(a.err);
   tc_fence_after();
-  const uint32_t tmem = sh->tmem_slot;       // S_t at 128 t, O_t at 256 + DV t, P_t over S_t or at 384 + 64 t
+  const uint32_t tmem = sh->tmem_slot;       // S_t at 128 t, one half of it after the other, P over the half it came from; O_t at 256 + DV t
   const Unit unit = sh->unit;
   if (drain || unit.bad || u >= unit.total) {
     if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
@@ -313,17 +302,17 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int k0 = __ldg(a.cu_k + unit.seq), Lk = __ldg(a.cu_k + unit.seq + 1) - k0;
   const int off = Lk - L;                    // query i sees the keys up to i + off
   const int rows = a.hb * a.tok;
-  // key tiles of query tile t, and the first of them that the mask cuts
+  // halves of key tiles (64 keys) of query tile t, and the first of them that the mask cuts
   int n[2], whole[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int first = (2 * unit.place + t) * a.tok, last = min(L, first + a.tok) - 1;
-    n[t] = first < L && off + last >= 0 ? (off + last) / TILE + 1 : 0;
-    whole[t] = off + first + 1 > 0 ? (off + first + 1) / TILE : 0;
+    n[t] = first < L && off + last >= 0 ? (off + last) / PART + 1 : 0;
+    whole[t] = off + first + 1 > 0 ? (off + first + 1) / PART : 0;
   }
-  const int most = max(n[0], n[1]);
+  const int most = (max(n[0], n[1]) + 1) / 2;
 
-  if (warp == TMA_WARP) {
+  if (warp == FWD_TMA_WARP) {
     // ------------------------------ loads ------------------------------
     bool ok = true;
     auto load_q = [&](int t) {
@@ -359,47 +348,59 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (lane == 0) mbar_arrive(&sh->v_full[vs]);
       }
     }
-  } else if (warp == MMA_WARP) {
-    // ------------------------------ products ------------------------------
+  } else if (warp >= MMA_WARP) {
+    // ------------------------------ products of query tile t ------------------------------
     if (elect_one()) {
-      constexpr uint32_t id_s = idesc(HALF, TILE, false), id_o = idesc(HALF, DV, true);
-      int s_next[2] = {0, 0}, p_next[2] = {0, 0}, k_freed = 0, v_freed = 0;
-      Patience patience;
-      bool moved = true;
-      while ((p_next[0] < n[0] || p_next[1] < n[1]) && patience.more(moved, abort_flag, a.err)) {
-        moved = false;
+      constexpr uint32_t id_s = idesc(HALF, PART, false), id_o = idesc(HALF, DV, true);
+      const int t = warp - MMA_WARP, count = t ? n[1] : n[0];
+      const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * DV;
+      const uint64_t dQ = base_k(smem_u32(sQ + t * F::KS * SLAB)), dK = base_k(smem_u32(sK)), dV = base_mn(smem_u32(sV));
+      Ring<F::K_SLOTS> rk;
+      Ring<F::V_SLOTS> rv;
+      bool ok = true;
+      auto scores = [&](int j) {             // S(j) = Q K(j)', 64 keys; a key tile is let go after its second half
+        if (!(j & 1)) ok = mbar_wait(&sh->k_full[rk.at], rk.round, abort_flag, a.err, ERR_WAIT_FULL);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t d = dK + rk.at * (F::KS * SLAB >> 4) + (j & 1) * (SLAB / 2 >> 4);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int i = p_next[t], vs = i % F::V_SLOTS;
-          if (i < s_next[t] && ready(&sh->p_full[t], i & 1) && ready(&sh->v_full[vs], (i / F::V_SLOTS) & 1)) {
-            tc_fence_after();
-            const uint32_t aV = smem_u32(sV + vs * F::VS * SLAB), tP = F::P_OVER_S ? tmem + t * 128 : tmem + 384 + t * 64;
-#pragma unroll
-            for (int k = 0; k < TILE / 16; ++k) umma_ta(tmem + 256 + t * DV, tP + k * 8, desc_mn(aV, k), id_o, (i | k) != 0);
-            umma_commit(&sh->o_done[t]);
-            ++p_next[t];
-            if ((p_next[0] > v_freed || v_freed >= n[0]) && (p_next[1] > v_freed || v_freed >= n[1])) {
-              umma_commit(&sh->v_empty[v_freed % F::V_SLOTS]);
-              ++v_freed;
-            }
-            moved = true;
-          }
-          const int j = s_next[t], ks = j % F::K_SLOTS;
-          if (j < n[t] && ready(&sh->k_full[ks], (j / F::K_SLOTS) & 1) &&
-              (j == 0 ? ready(&sh->q_full[t], 0) : ready(F::P_OVER_S ? &sh->o_done[t] : &sh->s_free[t], (j - 1) & 1))) {
-            tc_fence_after();
-            const uint32_t aQ = smem_u32(sQ + t * F::KS * SLAB), aK = smem_u32(sK + ks * F::KS * SLAB);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) umma_f16(tmem + t * 128, desc_k(aQ, k), desc_k(aK, k), id_s, k != 0);
-            umma_commit(&sh->s_full[t]);
-            ++s_next[t];
-            if ((s_next[0] > k_freed || k_freed >= n[0]) && (s_next[1] > k_freed || k_freed >= n[1])) {
-              umma_commit(&sh->k_empty[k_freed % F::K_SLOTS]);
-              ++k_freed;
-            }
-            moved = true;
-          }
+        for (int k = 0; k < D / 16; ++k) umma_f16(tS + (j & 1) * 64, dQ + step_k(k), d + step_k(k), id_s, k != 0);
+        umma_commit(&sh->s_full[t][j & 1]);
+        if ((j & 1) || j + 1 == count) {
+          umma_commit(&sh->k_empty[rk.at]);
+          rk.next();
         }
+      };
+      if (count > 0) ok = mbar_wait(&sh->q_full[t], 0, abort_flag, a.err, ERR_WAIT_FULL);
+      if (ok && count > 0) scores(0);
+      if (ok && count > 1) scores(1);
+      for (int j = 0; j < count && ok; ++j) {
+        if (!(j & 1)) ok = mbar_wait(&sh->v_full[rv.at], rv.round, abort_flag, a.err, ERR_WAIT_FULL);
+        ok = ok && mbar_wait(&sh->p_full[t][j & 1], (j >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t d = dV + rv.at * (F::VS * SLAB >> 4) + (j & 1) * step_mn(4);
+#pragma unroll
+        for (int k = 0; k < PART / 16; ++k) umma_ta(tO, tS + (j & 1) * 64 + k * 8, d + step_mn(k), id_o, (j | k) != 0);
+        umma_commit(&sh->pv_done[t][j & 1]);
+        if ((j & 1) || j + 1 == count) {
+          umma_commit(&sh->v_empty[rv.at]);
+          rv.next();
+        }
+        if (j + 2 < count) {                 // over the columns of P(j)
+          ok = mbar_wait(&sh->pv_done[t][j & 1], (j >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+          if (ok) scores(j + 2);
+        }
+      }
+      // key tiles that the other query tile alone looks at
+      for (int j = (count + 1) / 2; j < most && ok; ++j) {
+        ok = mbar_wait(&sh->k_full[rk.at], rk.round, abort_flag, a.err, ERR_WAIT_FULL) &&
+             mbar_wait(&sh->v_full[rv.at], rv.round, abort_flag, a.err, ERR_WAIT_FULL);
+        if (!ok) break;
+        mbar_arrive(&sh->k_empty[rk.at]);
+        mbar_arrive(&sh->v_empty[rv.at]);
+        rk.next();
+        rv.next();
       }
     }
   } else {
@@ -409,28 +410,23 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const bool mine = r < rows && pos < L;
     const int last = mine ? off + pos : -1;                   // last key it sees
     const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + t * 128 + lane_addr, tO = tmem + 256 + t * DV + lane_addr;
-    const uint32_t tP = F::P_OVER_S ? tS : tmem + 384 + t * 64 + lane_addr;
+    const uint32_t tO = tmem + 256 + t * DV + lane_addr;
     float m_ref = -INFINITY, l = 0.f;
-    auto tile = [&](int j, auto where) {
+    auto part = [&](int j, auto where) {
       constexpr bool MASK = decltype(where)::value;
-      const int lim = last - j * TILE;                        // columns up to lim are seen
-      bool ok = warp_wait(&sh->s_full[t], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
-      if (!ok) return false;
+      const int lim = last - j * PART;                        // columns up to lim are seen
+      const uint32_t tS = tmem + t * 128 + (j & 1) * 64 + lane_addr;
+      if (!warp_wait(&sh->s_full[t][j & 1], (j >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
       tc_fence_after();
-      // first pass over the row: its maximum.  The first half of the row is read last and kept for the second pass.
+      uint32_t s0[32], s1[32];
+      tmem_ld_32x32(tS, s0);
+      tmem_ld_32x32(tS + 32, s1);
+      tmem_ld_wait();
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      uint32_t s0[32], s1[32], s2[32];
 #pragma unroll
-      for (int c = 1; c >= 0; --c) {
-        tmem_ld_32x32(tS + c * 64, s0);
-        tmem_ld_32x32(tS + c * 64 + 32, s1);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          if (!MASK || c * 64 + e <= lim) top[e & 1] = fmaxf(top[e & 1], __uint_as_float(s0[e]));
-          if (!MASK || c * 64 + 32 + e <= lim) top[2 + (e & 1)] = fmaxf(top[2 + (e & 1)], __uint_as_float(s1[e]));
-        }
+      for (int e = 0; e < 32; ++e) {
+        if (!MASK || e <= lim) top[e & 1] = fmaxf(top[e & 1], __uint_as_float(s0[e]));
+        if (!MASK || 32 + e <= lim) top[2 + (e & 1)] = fmaxf(top[2 + (e & 1)], __uint_as_float(s1[e]));
       }
       float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
       if (m_new != -INFINITY) m_new *= a.scale_log2;          // a scale of zero leaves "nothing seen" as it is
@@ -440,22 +436,17 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         m_ref = m_new;
         l *= alpha;
       }
-      if (j > 0) {
-        if (!F::P_OVER_S) {                                   // P_t and O_t are free (P over S: S_t was issued after O_t was done)
-          ok = warp_wait(&sh->o_done[t], (j - 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
-          if (!ok) return false;
-          tc_fence_after();
-        }
-        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+      if (__any_sync(0xffffffffu, alpha != 1.f) && j > 0) {   // O of all parts before this one
+        if (!warp_wait(&sh->pv_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
+        tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < DV / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32(tO + c * 32, o);
-            tmem_ld_wait();
+        for (int c = 0; c < DV / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32(tO + c * 32, o);
+          tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st(tO + c * 32, o);
-          }
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st(tO + c * 32, o);
         }
       }
       const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // nothing seen so far
@@ -477,30 +468,19 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       };
       quarter(s0, 0, 0);
       quarter(s1, 32, 16);
-      tmem_st(tP, p);
-      tmem_ld_32x32(tS + 64, s2);
-      tmem_ld_32x32(tS + 96, s1);
-      tmem_ld_wait();
-      if (!F::P_OVER_S) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->s_free[t]);
-      }
-      quarter(s2, 64, 0);
-      quarter(s1, 96, 16);
-      tmem_st(tP + 32, p);
+      tmem_st(tS, p);
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->p_full[t]);
+      if (lane == 0) mbar_arrive(&sh->p_full[t][j & 1]);
       return true;
     };
     const int count = t ? n[1] : n[0], open = t ? whole[1] : whole[0];
     bool ok = true;
-    for (int j = 0; j < min(count, open) && ok; ++j) ok = tile(j, Whole{});
-    for (int j = min(count, open); j < count && ok; ++j) ok = tile(j, Masked{});
-    if (ok && count > 0) ok = warp_wait(&sh->o_done[t], (count - 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
+    for (int j = 0; j < min(count, open) && ok; ++j) ok = part(j, Whole{});
+    for (int j = min(count, open); j < count && ok; ++j) ok = part(j, Masked{});
+    if (ok && count > 0) ok = warp_wait(&sh->pv_done[t][(count - 1) & 1], ((count - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
     if (ok) {
       tc_fence_after();
       const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;               // a NaN stays
@@ -537,8 +517,8 @@ template <int D, int DV>
 struct Dq {
   static constexpr int KS = D / 64, VS = DV / 64, K_SLOTS = 3, V_SLOTS = 2;
   struct Shared {
-    uint64_t q_full, k_full[K_SLOTS], k_empty[K_SLOTS], v_full[V_SLOTS], v_empty[V_SLOTS], tail;
-    uint64_t s_full[2], dp_full, dp_free, ds_full[2], dq_done[2], acc_done;
+    uint64_t q_full, rows_in, k_full[K_SLOTS], k_empty[K_SLOTS], v_full[V_SLOTS], v_empty[V_SLOTS], tail;
+    uint64_t s_full[2], s_free[2], dp_full[2], ds_full[2], dq_done[2], acc_done;        // half of the key tile
     Unit unit;
     uint32_t tmem_slot;
     int abort_flag;
@@ -570,14 +550,15 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     mbar_init(&sh->q_full, 1);
     for (int s = 0; s < F::K_SLOTS; ++s) { mbar_init(&sh->k_full[s], 1); mbar_init(&sh->k_empty[s], 1); }
     for (int s = 0; s < F::V_SLOTS; ++s) { mbar_init(&sh->v_full[s], 1); mbar_init(&sh->v_empty[s], 1); }
+    mbar_init(&sh->rows_in, 8);
     mbar_init(&sh->tail, 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh->s_full[b], 1);
-      mbar_init(&sh->ds_full[b], 8);
+      mbar_init(&sh->s_free[b], 4);
+      mbar_init(&sh->dp_full[b], 1);
+      mbar_init(&sh->ds_full[b], 4);
       mbar_init(&sh->dq_done[b], 1);
     }
-    mbar_init(&sh->dp_full, 1);
-    mbar_init(&sh->dp_free, 8);
     mbar_init(&sh->acc_done, 1);
     sh->abort_flag = 0;
     fence_mbar_init();
@@ -586,7 +567,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   tc_fence_before();
   const bool drain = setup_barrier(a.err);
   tc_fence_after();
-  const uint32_t tmem = sh->tmem_slot;       // S of even and odd key tiles at 0 and 128 (dS over them), dP at 256, dQ at 384
+  const uint32_t tmem = sh->tmem_slot;       // S at 0, dP at 128 (halves of 64 columns, dS over those of dP), dQ at 256; Q at 384, dO at 448
   const Unit unit = sh->unit;
   if (drain || unit.bad || u >= unit.total) {
     if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
@@ -638,51 +619,62 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
   } else if (warp == MMA_WARP) {
     if (elect_one()) {
-      constexpr uint32_t id_s = idesc(HALF, TILE, false), id_q = idesc(HALF, D, true);
-      const uint32_t aQ = smem_u32(sQ), aG = smem_u32(sG);
-      int is = 0, ip = 0, iq = 0;
-      bool there = false;
-      Patience patience;
-      bool moved = true;
-      while (iq < n && patience.more(moved, abort_flag, a.err)) {
-        moved = false;
-        if (!there) {
-          there = moved = ready(&sh->q_full, 0);
-          continue;
-        }
-        if (is < n && ready(&sh->k_full[is % F::K_SLOTS], (is / F::K_SLOTS) & 1) &&
-            (is < 2 || ready(&sh->dq_done[is & 1], ((is >> 1) - 1) & 1))) {
-          tc_fence_after();
-          const uint32_t aK = smem_u32(sK + (is % F::K_SLOTS) * F::KS * SLAB);
+      constexpr uint32_t id_s = idesc(HALF, PART, false), id_q = idesc(HALF, D, true);
+      const uint64_t dK = base_k(smem_u32(sK)), dKt = base_mn(smem_u32(sK)), dV = base_k(smem_u32(sV));
+      Ring<F::K_SLOTS> rs, rq;
+      Ring<F::V_SLOTS> rv;
+      bool ok = n == 0 || mbar_wait(&sh->rows_in, 0, abort_flag, a.err, ERR_WAIT_FULL);
+      auto scores = [&](int h) {             // half h of S = Q K'
+        const uint64_t d = dK + rs.at * (F::KS * SLAB >> 4) + h * (SLAB / 2 >> 4);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) umma_f16(tmem + (is & 1) * 128, desc_k(aQ, k), desc_k(aK, k), id_s, k != 0);
-          umma_commit(&sh->s_full[is & 1]);
-          ++is;
-          moved = true;
-        }
-        if (ip < n && ready(&sh->v_full[ip % F::V_SLOTS], (ip / F::V_SLOTS) & 1) && (ip == 0 || ready(&sh->dp_free, (ip - 1) & 1))) {
-          tc_fence_after();
-          const uint32_t aV = smem_u32(sV + (ip % F::V_SLOTS) * F::VS * SLAB);
+        for (int k = 0; k < D / 16; ++k) umma_ta(tmem + h * 64, tmem + 384 + k * 8, d + step_k(k), id_s, k != 0);
+        umma_commit(&sh->s_full[h]);
+      };
+      auto weights = [&](int h) {            // half h of dP = dO V'
+        const uint64_t d = dV + rv.at * (F::VS * SLAB >> 4) + h * (SLAB / 2 >> 4);
 #pragma unroll
-          for (int k = 0; k < DV / 16; ++k) umma_f16(tmem + 256, desc_k(aG, k), desc_k(aV, k), id_s, k != 0);
-          umma_commit(&sh->dp_full);
-          umma_commit(&sh->v_empty[ip % F::V_SLOTS]);
-          ++ip;
-          moved = true;
+        for (int k = 0; k < DV / 16; ++k) umma_ta(tmem + 128 + h * 64, tmem + 448 + k * 8, d + step_k(k), id_s, k != 0);
+        umma_commit(&sh->dp_full[h]);
+      };
+      for (int j = -1; j < n && ok; ++j) {
+        // S(j + 1) as soon as the compute warps hold S(j), dQ(j) when dS(j) is there, dP(j + 1) over the columns of dS(j)
+        if (j + 1 < n) {
+          ok = mbar_wait(&sh->k_full[rs.at], rs.round, abort_flag, a.err, ERR_WAIT_FULL);
+          for (int h = 0; h < 2 && ok; ++h) {
+            ok = j < 0 || mbar_wait(&sh->s_free[h], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
+            scores(h);
+          }
+          rs.next();
         }
-        if (iq < is && ready(&sh->ds_full[iq & 1], (iq >> 1) & 1)) {
+        for (int h = 0; h < 2 && ok && j >= 0; ++h) {
+          ok = mbar_wait(&sh->ds_full[h], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t aK = smem_u32(sK + (iq % F::K_SLOTS) * F::KS * SLAB), tdS = tmem + (iq & 1) * 128;
+          const uint64_t d = dKt + rq.at * (F::KS * SLAB >> 4) + h * step_mn(4);
 #pragma unroll
-          for (int k = 0; k < TILE / 16; ++k)                 // the halves of dS lie over the halves of S that they came from
-            umma_ta(tmem + 384, tdS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(aK, k), id_q, (iq | k) != 0);
-          umma_commit(&sh->dq_done[iq & 1]);
-          umma_commit(&sh->k_empty[iq % F::K_SLOTS]);
-          ++iq;
-          moved = true;
+          for (int k = 0; k < PART / 16; ++k) umma_ta(tmem + 256, tmem + 128 + h * 64 + k * 8, d + step_mn(k), id_q, (j | h | k) != 0);
+          umma_commit(&sh->dq_done[h]);
+        }
+        if (!ok) break;
+        if (j >= 0) {
+          umma_commit(&sh->k_empty[rq.at]);
+          rq.next();
+        }
+        if (j + 1 < n) {
+          ok = mbar_wait(&sh->v_full[rv.at], rv.round, abort_flag, a.err, ERR_WAIT_FULL);
+          for (int h = 0; h < 2 && ok; ++h) {
+            ok = j < 0 || mbar_wait(&sh->dq_done[h], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
+            weights(h);
+          }
+          if (ok) umma_commit(&sh->v_empty[rv.at]);
+          rv.next();
         }
       }
-      if (n > 0 && iq == n) umma_commit(&sh->acc_done);
+      if (ok && n > 0) umma_commit(&sh->acc_done);
     }
   } else {
     const int half = warp >> 2, r = tid & 127, tok = r / a.hb, pos = first + tok;
@@ -724,11 +716,30 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (mine && half == 0) a.delta[at] = delta;
     const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
     const float delta_up = delta * up;
+    bool ok = n == 0 || warp_wait(&sh->q_full, 0, abort_flag, a.err, ERR_WAIT_FULL);
+    if (ok && n > 0) {                       // Q and dO go to TMEM, half a row from each of its two threads
+      auto fill = [&](const uint8_t* tile, int slabs, uint32_t to) {
+        if (half >= slabs) return;
+        uint32_t x[32];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint4 v = *reinterpret_cast<const uint4*>(tile + half * SLAB + r * 128 + ((c ^ (r & 7)) << 4));
+          x[c * 4] = v.x; x[c * 4 + 1] = v.y; x[c * 4 + 2] = v.z; x[c * 4 + 3] = v.w;
+        }
+        tmem_st(to + half * 32 + lane_addr, x);
+      };
+      fill(sQ, F::KS, tmem + 384);
+      fill(sG, F::VS, tmem + 448);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->rows_in);
+    }
     auto tile = [&](int j, auto where) {
       constexpr bool MASK = decltype(where)::value;
       const int lim = last - j * TILE - half * 64;
-      const uint32_t tS = tmem + (j & 1) * 128 + half * 64 + lane_addr, tdP = tmem + 256 + half * 64 + lane_addr;
-      if (!warp_wait(&sh->s_full[j & 1], (j >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
+      const uint32_t tS = tmem + half * 64 + lane_addr, tdP = tmem + 128 + half * 64 + lane_addr;
+      if (!warp_wait(&sh->s_full[half], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
       tc_fence_after();
       float p[64];
 #pragma unroll
@@ -736,13 +747,18 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         uint32_t s[32];
         tmem_ld_32x32(tS + c * 32, s);
         tmem_ld_wait();
+        if (c == 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->s_free[half]);
+        }
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const float x = ex2(fmaf(__uint_as_float(s[e]), a.scale_log2, -lse));
           p[c * 32 + e] = !MASK || c * 32 + e <= lim ? x : 0.f;
         }
       }
-      if (!warp_wait(&sh->dp_full, j & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
+      if (!warp_wait(&sh->dp_full[half], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
       tc_fence_after();
       uint32_t ds[32];
 #pragma unroll
@@ -750,11 +766,6 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         uint32_t d[32];
         tmem_ld_32x32(tdP + c * 32, d);
         tmem_ld_wait();
-        if (c == 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->dp_free);
-        }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int i = c * 32 + 2 * e;
@@ -767,14 +778,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           ds[c * 16 + e] = pair<HALF>(x, y);
         }
       }
-      tmem_st(tS, ds);
+      tmem_st(tdP, ds);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->ds_full[j & 1]);
+      if (lane == 0) mbar_arrive(&sh->ds_full[half]);
       return true;
     };
-    bool ok = true;
     for (int j = 0; j < open && ok; ++j) ok = tile(j, Whole{});
     for (int j = open; j < n && ok; ++j) ok = tile(j, Masked{});
     if (ok && n > 0) ok = warp_wait(&sh->acc_done, 0, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
@@ -786,7 +796,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const int col = half * (D / 2) + c * 32;
         uint32_t x[32];
         if (n > 0) {
-          tmem_ld_32x32(tmem + 384 + col + lane_addr, x);
+          tmem_ld_32x32(tmem + 256 + col + lane_addr, x);
           tmem_ld_wait();
         }
 #pragma unroll
@@ -942,63 +952,54 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   } else if (warp == MMA_WARP) {
     if (elect_one()) {
       constexpr uint32_t id_s = idesc(HALF, TILE, false), id_v = idesc(HALF, DV, true), id_k = idesc(HALF, D, true);
-      const uint32_t aK = smem_u32(sK), aV = smem_u32(sV);
-      int is = 0, ip = 0, iv = 0, ik = 0, freed = 0;
-      bool there = false;
-      Patience patience;
-      bool moved = true;
-      auto stage_free = [&]() {
-        if (iv > freed && ik > freed) {
-          umma_commit(&sh->q_empty[freed % F::STAGES]);
-          ++freed;
-        }
+      const uint64_t dK = base_k(smem_u32(sK)), dV = base_k(smem_u32(sV)), dQ = base_k(smem_u32(sQ)), dQt = base_mn(smem_u32(sQ));
+      const uint64_t dG = dQ + (F::KS * SLAB >> 4), dGt = dQt + (F::KS * SLAB >> 4);
+      Ring<F::STAGES> next, now;             // of the scores, of the gradients
+      bool ok = n == 0 || mbar_wait(&sh->kv_full, 0, abort_flag, a.err, ERR_WAIT_FULL);
+      auto scores = [&](int i) {             // S' = K Q', over the columns of P' before
+        ok = mbar_wait(&sh->q_full[next.at], next.round, abort_flag, a.err, ERR_WAIT_FULL) &&
+             (i == 0 || mbar_wait(&sh->dv_done, (i - 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY));
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t d = dQ + next.at * (STAGE >> 4);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) umma_f16(tmem, dK + step_k(k), d + step_k(k), id_s, k != 0);
+        umma_commit(&sh->s_full);
       };
-      while (ik < n && patience.more(moved, abort_flag, a.err)) {
-        moved = false;
-        if (!there) {
-          there = moved = ready(&sh->kv_full, 0);
-          continue;
-        }
-        if (is < n && ready(&sh->q_full[is % F::STAGES], (is / F::STAGES) & 1) && (is == 0 || ready(&sh->dv_done, (is - 1) & 1))) {
-          tc_fence_after();
-          const uint32_t aQ = smem_u32(sQ + (is % F::STAGES) * STAGE);
+      auto weights = [&](int i) {            // dP' = V dO', over the columns of dS' before
+        ok = i == 0 || mbar_wait(&sh->dk_done, (i - 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t d = dG + next.at * (STAGE >> 4);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) umma_f16(tmem, desc_k(aK, k), desc_k(aQ, k), id_s, k != 0);
-          umma_commit(&sh->s_full);
-          ++is;
-          moved = true;
-        }
-        if (iv < is && ready(&sh->p_full, iv & 1)) {
-          tc_fence_after();
-          const uint32_t aG = smem_u32(sQ + (iv % F::STAGES) * STAGE + F::KS * SLAB);
-#pragma unroll
-          for (int k = 0; k < TILE / 16; ++k) umma_ta(tmem + 256, tmem + (k >> 2) * 64 + (k & 3) * 8, desc_mn(aG, k), id_v, (iv | k) != 0);
-          umma_commit(&sh->dv_done);
-          ++iv;
-          stage_free();
-          moved = true;
-        }
-        if (ip < n && ready(&sh->q_full[ip % F::STAGES], (ip / F::STAGES) & 1) && (ip == 0 || ready(&sh->dk_done, (ip - 1) & 1))) {
-          tc_fence_after();
-          const uint32_t aG = smem_u32(sQ + (ip % F::STAGES) * STAGE + F::KS * SLAB);
-#pragma unroll
-          for (int k = 0; k < DV / 16; ++k) umma_f16(tmem + 128, desc_k(aV, k), desc_k(aG, k), id_s, k != 0);
-          umma_commit(&sh->dp_full);
-          ++ip;
-          moved = true;
-        }
-        if (ik < ip && ready(&sh->ds_full, ik & 1)) {
-          tc_fence_after();
-          const uint32_t aQ = smem_u32(sQ + (ik % F::STAGES) * STAGE);
-#pragma unroll
-          for (int k = 0; k < TILE / 16; ++k) umma_ta(tmem + 384, tmem + 128 + (k >> 2) * 64 + (k & 3) * 8, desc_mn(aQ, k), id_k, (ik | k) != 0);
-          umma_commit(&sh->dk_done);
-          ++ik;
-          stage_free();
-          moved = true;
-        }
+        for (int k = 0; k < DV / 16; ++k) umma_f16(tmem + 128, dV + step_k(k), d + step_k(k), id_s, k != 0);
+        umma_commit(&sh->dp_full);
+        next.next();
+      };
+      if (ok && n > 0) {
+        scores(0);
+        if (ok) weights(0);
       }
-      if (n > 0 && ik == n) umma_commit(&sh->acc_done);
+      for (int i = 0; i < n && ok; ++i) {
+        ok = mbar_wait(&sh->p_full, i & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t g = dGt + now.at * (STAGE >> 4), q = dQt + now.at * (STAGE >> 4);
+#pragma unroll
+        for (int k = 0; k < TILE / 16; ++k) umma_ta(tmem + 256, tmem + (k >> 2) * 64 + (k & 3) * 8, g + step_mn(k), id_v, (i | k) != 0);
+        umma_commit(&sh->dv_done);
+        if (i + 1 < n) scores(i + 1);
+        ok = ok && mbar_wait(&sh->ds_full, i & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < TILE / 16; ++k) umma_ta(tmem + 384, tmem + 128 + (k >> 2) * 64 + (k & 3) * 8, q + step_mn(k), id_k, (i | k) != 0);
+        umma_commit(&sh->dk_done);
+        umma_commit(&sh->q_empty[now.at]);
+        now.next();
+        if (i + 1 < n) weights(i + 1);
+      }
+      if (ok && n > 0) umma_commit(&sh->acc_done);
     }
   } else {
     const int half = warp >> 2, r = tid & 127;
@@ -1172,7 +1173,7 @@ int forward(const Inputs& in, Args a, cudaStream_t stream) {
   const long long units = units_of(a.T, a.n, 2 * a.tok), grid = units * a.kv_heads * a.chunks;
   if (grid > 0x7fffffffLL) return -10;
   a.units = (int)units;
-  packed_fwd_kernel<HALF, D, DV><<<(unsigned)grid, THREADS, Fwd<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], a);
+  packed_fwd_kernel<HALF, D, DV><<<(unsigned)grid, FWD_THREADS, Fwd<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], a);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
