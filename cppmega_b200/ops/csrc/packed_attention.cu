@@ -34,7 +34,7 @@
 // is too short for dS of any size: it is scaled by a power of two, from the row's largest |do| for dq, from the call's for dk.
 #include <cuda_fp16.h>
 
-#include "common.cuh"
+#include "fp32_pair.cuh"
 
 namespace cm {
 namespace packed {
@@ -111,6 +111,7 @@ struct Args {
   int n, T, Tk;                              // sequences, rows of queries and of keys
   int heads, kv_heads;
   int hb, chunks, tok;                       // heads of a tile, tiles of heads in a group, tokens of a tile
+  int by_hb;                                 // r / hb is r * by_hb >> 16 for r < 128
   int dim, vdim;
   int units;                                 // blocks per (key head, chunk)
   float scale, scale_log2;
@@ -125,60 +126,74 @@ struct Args {
 };
 
 struct Unit {
-  int seq, place, total;                     // total: tiles of all sequences
-  bool bad;
+  int place, total;                          // place of the tile in its sequence; tiles of all sequences
+  int q0, L, k0, Lk;                         // the sequence's queries and keys
+  int bad;
 };
 
-// Which tile is block u's?  One warp; `per` rows a tile of the sequences in cu.
-__device__ Unit find_unit(const Args& a, const int* cu, int per, int u, int lane) {
-  constexpr int KEPT = 4;
-  Unit r;
-  r.bad = lane == 0 && (__ldg(a.cu_q) != 0 || __ldg(a.cu_k) != 0);
-  int kept[KEPT], most = 0;
-  auto tiles = [&](int i) { return (__ldg(cu + i + 1) - __ldg(cu + i) + per - 1) / per; };
-  for (int i = lane; i < a.n; i += 32) {
-    const int q0 = __ldg(a.cu_q + i), q1 = __ldg(a.cu_q + i + 1), k0 = __ldg(a.cu_k + i), k1 = __ldg(a.cu_k + i + 1);
-    r.bad |= q0 < 0 || q1 < q0 || q1 > a.T || k0 < 0 || k1 < k0 || k1 > a.Tk;
-  }
-  r.bad = __any_sync(0xffffffffu, r.bad);
-  r.seq = r.place = r.total = 0;
-  if (r.bad) return r;
+// Which tile is block u's?  One warp; `per` rows a tile of the sequences' queries or (of_keys) keys.
+__device__ Unit find_unit(const Args& a, bool of_keys, int per, int u, int lane) {
+  constexpr int KEPT = 4;                    // sequences that a lane keeps the tiles of; more are counted again each time
+  Unit r = {};
+  bool bad = false;
+  int kept[KEPT], q0 = 0, L = 0, k0 = 0, Lk = 0;              // of sequence `lane`
+  auto tiles = [&](int rows) { return int(unsigned(rows + per - 1) / unsigned(per)); };
+  const int* cu = of_keys ? a.cu_k : a.cu_q;
+  auto tiles_of = [&](int i) { return tiles(__ldg(cu + i + 1) - __ldg(cu + i)); };
 #pragma unroll
-  for (int c = 0; c < KEPT; ++c) kept[c] = c * 32 + lane < a.n ? tiles(c * 32 + lane) : 0;
+  for (int c = 0; c < KEPT; ++c) {
+    const int i = c * 32 + lane;
+    kept[c] = 0;
+    if (c * 32 >= a.n) continue;
+    if (i < a.n) {
+      const int x0 = __ldg(a.cu_q + i), x1 = __ldg(a.cu_q + i + 1), y0 = __ldg(a.cu_k + i), y1 = __ldg(a.cu_k + i + 1);
+      bad |= x0 < 0 || x1 < x0 || x1 > a.T || y0 < 0 || y1 < y0 || y1 > a.Tk || (i == 0 && (x0 != 0 || y0 != 0));
+      kept[c] = tiles(of_keys ? y1 - y0 : x1 - x0);
+      if (c == 0) { q0 = x0; L = x1 - x0; k0 = y0; Lk = y1 - y0; }
+    }
+  }
+  if (a.n == 0) bad = __ldg(a.cu_q) != 0 || __ldg(a.cu_k) != 0;
+  for (int i = KEPT * 32 + lane; i < a.n; i += 32) {
+    const int x0 = __ldg(a.cu_q + i), x1 = __ldg(a.cu_q + i + 1), y0 = __ldg(a.cu_k + i), y1 = __ldg(a.cu_k + i + 1);
+    bad |= x0 < 0 || x1 < x0 || x1 > a.T || y0 < 0 || y1 < y0 || y1 > a.Tk;
+  }
+  r.bad = __any_sync(0xffffffffu, bad);
+  if (r.bad) return r;
   auto after = [&](int p) {                  // tiles at place p or later
     int s = 0;
 #pragma unroll
     for (int c = 0; c < KEPT; ++c) s += max(0, kept[c] - p);
-    for (int i = KEPT * 32 + lane; i < a.n; i += 32) s += max(0, tiles(i) - p);
+    for (int i = KEPT * 32 + lane; i < a.n; i += 32) s += max(0, tiles_of(i) - p);
     return __reduce_add_sync(0xffffffffu, s);
   };
-#pragma unroll
-  for (int c = 0; c < KEPT; ++c) most = max(most, kept[c]);
-  for (int i = KEPT * 32 + lane; i < a.n; i += 32) most = max(most, tiles(i));
-  most = __reduce_max_sync(0xffffffffu, most);
+  int most = max(max(kept[0], kept[1]), max(kept[2], kept[3]));
+  for (int i = KEPT * 32 + lane; i < a.n; i += 32) most = max(most, tiles_of(i));
   r.total = after(0);
   if (u >= r.total) return r;
-  int lo = 0, hi = most;                     // after(lo) > u >= after(hi)
+  int lo = 0, hi = __reduce_max_sync(0xffffffffu, most), from_hi = 0;         // after(lo) > u >= after(hi)
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (after(mid) > u) lo = mid;
-    else hi = mid;
+    const int mid = (lo + hi) >> 1, f = after(mid);
+    if (f > u) lo = mid;
+    else { hi = mid; from_hi = f; }
   }
   r.place = lo;
-  int rank = u - after(lo + 1);
+  int rank = u - from_hi, seq = 0;           // hi is lo + 1: the rank-th of the sequences that have a tile at this place
   for (int c = 0, i0 = 0; i0 < a.n; i0 += 32, ++c) {
-    int t = 0;
-    if (c == 0) t = kept[0];
-    else if (c == 1) t = kept[1];
-    else if (c == 2) t = kept[2];
-    else if (c == 3) t = kept[3];
-    else if (i0 + lane < a.n) t = tiles(i0 + lane);
+    const int t = c == 0 ? kept[0] : c == 1 ? kept[1] : c == 2 ? kept[2] : c == 3 ? kept[3] : i0 + lane < a.n ? tiles_of(i0 + lane) : 0;
     const unsigned has = __ballot_sync(0xffffffffu, t > lo);
     if (rank < __popc(has)) {
-      r.seq = i0 + __fns(has, 0, rank + 1);
+      const bool it = t > lo && __popc(has & ((1u << lane) - 1)) == rank;
+      seq = i0 + __ffs(__ballot_sync(0xffffffffu, it)) - 1;
       break;
     }
     rank -= __popc(has);
+  }
+  if (seq < 32) {
+    r.q0 = __shfl_sync(0xffffffffu, q0, seq); r.L = __shfl_sync(0xffffffffu, L, seq);
+    r.k0 = __shfl_sync(0xffffffffu, k0, seq); r.Lk = __shfl_sync(0xffffffffu, Lk, seq);
+  } else {
+    r.q0 = __ldg(a.cu_q + seq); r.L = __ldg(a.cu_q + seq + 1) - r.q0;
+    r.k0 = __ldg(a.cu_k + seq); r.Lk = __ldg(a.cu_k + seq + 1) - r.k0;
   }
   return r;
 }
@@ -206,9 +221,10 @@ __device__ __forceinline__ void settle(volatile int* abort_flag) {
   }
 }
 
-// 32 accumulator columns times f as 16-bit values to a row (16-byte stores; `left` columns exist)
+// 32 accumulator columns times f as 16-bit values, to columns col .. col + 31 of row r of slabs in shared memory
 template <bool HALF>
-__device__ __forceinline__ void store_columns(uint16_t* row, const uint32_t (&x)[32], float f, int left) {
+__device__ __forceinline__ void put_columns(uint8_t* slabs, int r, int col, const uint32_t (&x)[32], float f) {
+  uint8_t* row = slabs + (col >> 6) * SLAB + r * 128;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint4 o;
@@ -216,11 +232,28 @@ __device__ __forceinline__ void store_columns(uint16_t* row, const uint32_t (&x)
     o.y = pair<HALF>(__uint_as_float(x[q * 8 + 2]) * f, __uint_as_float(x[q * 8 + 3]) * f);
     o.z = pair<HALF>(__uint_as_float(x[q * 8 + 4]) * f, __uint_as_float(x[q * 8 + 5]) * f);
     o.w = pair<HALF>(__uint_as_float(x[q * 8 + 6]) * f, __uint_as_float(x[q * 8 + 7]) * f);
-    if (q * 8 < left) reinterpret_cast<uint4*>(row)[q] = o;
+    *reinterpret_cast<uint4*>(row + ((((col >> 3) + q) & 7) ^ (r & 7)) * 16) = o;
   }
 }
+// The warp's 32 rows of those slabs, columns begin .. begin + COLS - 1 (of `width` that exist), to global rows `row_of(r)` (null: not stored):
+// whole lines, where each thread for itself would store 16 bytes of 32 rows at a time
+template <int COLS, typename RowOf>
+__device__ __forceinline__ void send_rows(const uint8_t* slabs, int row0, int begin, int width, int lane, RowOf row_of) {
+  constexpr int LANES = COLS / 8, ROWS = 32 / LANES;
+  __syncwarp();
+  const int piece = begin / 8 + lane % LANES;
+#pragma unroll 4
+  for (int i = 0; i < 32; i += ROWS) {
+    const int r = row0 + i + lane / LANES;
+    uint16_t* dst = row_of(r);
+    if (dst && piece * 8 < width)
+      reinterpret_cast<uint4*>(dst)[piece] =
+          *reinterpret_cast<const uint4*>(slabs + (piece >> 3) * SLAB + r * 128 + (((piece & 7) ^ (r & 7)) << 4));
+  }
+  __syncwarp();
+}
 
-// What the rounding of store_columns takes away, to as many bits again
+// What the rounding of put_columns takes away, to as many bits again
 template <bool HALF>
 __device__ __forceinline__ float rest(float x) {
   return HALF ? x - __half2float(__float2half_rn(x)) : x - __bfloat162float(__float2bfloat16_rn(x));
@@ -264,7 +297,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int head0 = kvh * (a.heads / a.kv_heads) + chunk * a.hb;
   volatile int* abort_flag = &sh->abort_flag;
   if (warp == 0) {
-    const Unit r = find_unit(a, a.cu_q, 2 * a.tok, u, lane);
+    const Unit r = find_unit(a, false, 2 * a.tok, u, lane);
     if (lane == 0) sh->unit = r;
   }
   if (tid == 32) {
@@ -298,8 +331,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     clear_rows(a.out, __ldg(a.cu_q + a.n), a.T, a.heads, head0, a.hb, a.vdim, u - unit.total, a.units - unit.total);
     return;
   }
-  const int q0 = __ldg(a.cu_q + unit.seq), L = __ldg(a.cu_q + unit.seq + 1) - q0;
-  const int k0 = __ldg(a.cu_k + unit.seq), Lk = __ldg(a.cu_k + unit.seq + 1) - k0;
+  const int q0 = unit.q0, L = unit.L, k0 = unit.k0, Lk = unit.Lk;
   const int off = Lk - L;                    // query i sees the keys up to i + off
   const int rows = a.hb * a.tok;
   // halves of key tiles (64 keys) of query tile t, and the first of them that the mask cuts
@@ -405,7 +437,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
   } else {
     // ------------------------------ softmax of query tile t ------------------------------
-    const int t = warp >> 2, r = tid & 127, tok = r / a.hb, qt = 2 * unit.place + t;
+    const int t = warp >> 2, r = tid & 127, tok = r * a.by_hb >> 16, qt = 2 * unit.place + t;
     const int pos = qt * a.tok + tok;                         // position of this row's query
     const bool mine = r < rows && pos < L;
     const int last = mine ? off + pos : -1;                   // last key it sees
@@ -450,26 +482,25 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
       const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // nothing seen so far
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      Pair sum[2] = {pr(0.f), pr(0.f)};
       uint32_t p[32];
       auto quarter = [&](const uint32_t (&sc)[32], int col0, int at) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float x = ex2(fmaf(__uint_as_float(sc[2 * e]), a.scale_log2, -ref));
-          float y = ex2(fmaf(__uint_as_float(sc[2 * e + 1]), a.scale_log2, -ref));
+          const float2 z = pr_get(pr_fma(pr(__uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1])), pr(a.scale_log2), pr(-ref)));
+          float x = ex2(z.x), y = ex2(z.y);
           if (MASK) {
             x = col0 + 2 * e <= lim ? x : 0.f;
             y = col0 + 2 * e + 1 <= lim ? y : 0.f;
           }
-          sum[(2 * e) & 3] += x;
-          sum[(2 * e + 1) & 3] += y;
+          sum[e & 1] = sum[e & 1] + pr(x, y);
           p[at + e] = pair<HALF>(x, y);
         }
       };
       quarter(s0, 0, 0);
       quarter(s1, 32, 16);
       tmem_st(tS, p);
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += pr_sum(sum[0] + sum[1]);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -485,23 +516,32 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tc_fence_after();
       const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;               // a NaN stays
       const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
-      uint16_t* row = reinterpret_cast<uint16_t*>(a.out) + at * a.vdim;
+      const float f = last >= 0 ? inv : 0.f;
+      uint8_t* stage = sQ + t * F::KS * SLAB;                 // Q_t has been used
+      auto rows_of = [&](void* out) {
+        return [&, out](int r) -> uint16_t* {
+          const int tok = r * a.by_hb >> 16, pos = qt * a.tok + tok;
+          return r < rows && pos < L ? reinterpret_cast<uint16_t*>(out) + ((long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb)) * a.vdim : nullptr;
+        };
+      };
 #pragma unroll
-      for (int c = 0; c < DV / 32; ++c) {
-        uint32_t o[32];
-        if (count > 0) {
-          tmem_ld_32x32(tO + c * 32, o);
-          tmem_ld_wait();
+      for (int pass = 0; pass < 2; ++pass) {                  // o, then what its rounding takes away
+        if (pass == 1 && !a.out2) break;
+#pragma unroll
+        for (int c = 0; c < DV / 32; ++c) {
+          uint32_t o[32];
+          if (count > 0) {
+            tmem_ld_32x32(tO + c * 32, o);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            o[e] = last >= 0 ? o[e] : 0u;                     // a row without keys
+            if (pass == 1) o[e] = __float_as_uint(rest<HALF>(__uint_as_float(o[e]) * f));
+          }
+          put_columns<HALF>(stage, r, c * 32, o, pass ? 1.f : f);
         }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = last >= 0 ? o[e] : 0u;            // a row without keys
-        const float f = last >= 0 ? inv : 0.f;
-        if (mine) store_columns<HALF>(row + c * 32, o, f, a.vdim - c * 32);
-        if (a.out2) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(rest<HALF>(__uint_as_float(o[e]) * f));
-          if (mine) store_columns<HALF>(reinterpret_cast<uint16_t*>(a.out2) + at * a.vdim + c * 32, o, 1.f, a.vdim - c * 32);
-        }
+        send_rows<DV>(stage, (warp & 3) * 32, 0, a.vdim, lane, rows_of(pass ? a.out2 : a.out));
       }
       if (mine && a.lse) a.lse[at] = l == 0.f ? INFINITY : m_ref + log2f(l);
     }
@@ -522,6 +562,7 @@ struct Dq {
     Unit unit;
     uint32_t tmem_slot;
     int abort_flag;
+    float delta[TILE], big[TILE];
   };
   static constexpr int SMEM = (KS + VS + K_SLOTS * KS + V_SLOTS * VS) * SLAB + (int)sizeof(Shared) + 1024;
 };
@@ -543,7 +584,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const int head0 = kvh * (a.heads / a.kv_heads) + chunk * a.hb;
   volatile int* abort_flag = &sh->abort_flag;
   if (warp == 0) {
-    const Unit r = find_unit(a, a.cu_q, a.tok, u, lane);
+    const Unit r = find_unit(a, false, a.tok, u, lane);
     if (lane == 0) sh->unit = r;
   }
   if (tid == 32) {
@@ -579,8 +620,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     clear_rows(a.out, __ldg(a.cu_q + a.n), a.T, a.heads, head0, a.hb, a.dim, u - unit.total, a.units - unit.total);
     return;
   }
-  const int q0 = __ldg(a.cu_q + unit.seq), L = __ldg(a.cu_q + unit.seq + 1) - q0;
-  const int k0 = __ldg(a.cu_k + unit.seq), Lk = __ldg(a.cu_k + unit.seq + 1) - k0;
+  const int q0 = unit.q0, L = unit.L, k0 = unit.k0, Lk = unit.Lk;
   const int off = Lk - L, rows = a.hb * a.tok, first = unit.place * a.tok, end = min(L, first + a.tok);
   const int n = off + end - 1 >= 0 ? (off + end - 1) / TILE + 1 : 0;
   const int open = off + first + 1 > 0 ? min(n, (off + first + 1) / TILE) : 0;
@@ -677,29 +717,54 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (ok && n > 0) umma_commit(&sh->acc_done);
     }
   } else {
-    const int half = warp >> 2, r = tid & 127, tok = r / a.hb, pos = first + tok;
+    const int half = warp >> 2, r = tid & 127, tok = r * a.by_hb >> 16, pos = first + tok;
     const bool mine = r < rows && pos < L;
     const int last = mine ? off + pos : -1, head = head0 + (r - tok * a.hb);
     const long long at = (long long)(q0 + pos) * a.heads + head;
-    // delta, and the power of two that brings the row's largest |do| to 2^-4; both threads of a row add it up whole
-    float delta = 0.f, big = 0.f;
-    if (mine) {
-      const uint4* ov = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o) + at * a.vdim);
-      const uint4* rv = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o_rest) + at * a.vdim);
-      const uint4* gv = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.go) + (q0 + pos) * a.go_tok + head * a.go_head);
+    // delta, and the power of two that brings the row's largest |do| to 2^-4: DV / 8 lanes a row, four rows of a lane on their way at once
+    {
+      constexpr int LANES = DV / 8, ROWS = 32 / LANES, AHEAD = 4;
+      const int piece = lane % LANES;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 16; i0 += ROWS * AHEAD) {
+        uint4 x[AHEAD], z[AHEAD], y[AHEAD];
 #pragma unroll
-      for (int c = 0; c < DV / 8; ++c) {
-        if (c * 8 >= a.vdim) break;
-        const uint4 x = __ldg(ov + c), z = __ldg(rv + c), y = __ldg(gv + c);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, zs[4] = {z.x, z.y, z.z, z.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        for (int i = 0; i < AHEAD; ++i) {
+          const int row = warp * 16 + i0 + i * ROWS + lane / LANES, tok = row * a.by_hb >> 16, pos = first + tok, head = head0 + (row - tok * a.hb);
+          const bool there = row < rows && pos < L && piece * 8 < a.vdim;
+          const long long at = ((long long)(q0 + pos) * a.heads + head) * a.vdim + piece * 8;
+          x[i] = z[i] = y[i] = make_uint4(0, 0, 0, 0);
+          if (there) {
+            x[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o) + at));
+            z[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o_rest) + at));
+            y[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.go) + (q0 + pos) * a.go_tok + head * a.go_head + piece * 8));
+          }
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpair<HALF>(xs[e]), h = unpair<HALF>(zs[e]), g = unpair<HALF>(ys[e]);
-          delta = fmaf(f.x + h.x, g.x, fmaf(f.y + h.y, g.y, delta));
-          if (HALF) big = fmaxf(big, fmaxf(fabsf(g.x), fabsf(g.y)));
+        for (int i = 0; i < AHEAD; ++i) {
+          const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, zs[4] = {z[i].x, z[i].y, z[i].z, z[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+          float dot = 0.f, big = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpair<HALF>(xs[e]), h = unpair<HALF>(zs[e]), g = unpair<HALF>(ys[e]);
+            dot = fmaf(f.x + h.x, g.x, fmaf(f.y + h.y, g.y, dot));
+            if (HALF) big = fmaxf(big, fmaxf(fabsf(g.x), fabsf(g.y)));
+          }
+#pragma unroll
+          for (int o = LANES >> 1; o > 0; o >>= 1) {
+            dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            if (HALF) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+          }
+          if (piece == 0) {
+            const int row = warp * 16 + i0 + i * ROWS + lane / LANES;
+            sh->delta[row] = dot;
+            if (HALF) sh->big[row] = big;
+          }
         }
       }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
     }
+    const float delta = sh->delta[r], big = HALF ? sh->big[r] : 0.f;
     float up = 1.f, down = 1.f;
     if (HALF) {
       if (big > 0.f && isfinite(big)) {
@@ -753,9 +818,11 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (lane == 0) mbar_arrive(&sh->s_free[half]);
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float x = ex2(fmaf(__uint_as_float(s[e]), a.scale_log2, -lse));
-          p[c * 32 + e] = !MASK || c * 32 + e <= lim ? x : 0.f;
+        for (int e = 0; e < 16; ++e) {
+          const float2 x = pr_get(pr_fma(pr(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), pr(a.scale_log2), pr(-lse)));
+          const int i = c * 32 + 2 * e;
+          p[i] = !MASK || i <= lim ? ex2(x.x) : 0.f;
+          p[i + 1] = !MASK || i + 1 <= lim ? ex2(x.y) : 0.f;
         }
       }
       if (!warp_wait(&sh->dp_full[half], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
@@ -769,8 +836,9 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int i = c * 32 + 2 * e;
-          float x = p[i] * (HALF ? fmaf(__uint_as_float(d[2 * e]), up, -delta_up) : __uint_as_float(d[2 * e]) - delta);
-          float y = p[i + 1] * (HALF ? fmaf(__uint_as_float(d[2 * e + 1]), up, -delta_up) : __uint_as_float(d[2 * e + 1]) - delta);
+          const Pair dp = pr(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1]));
+          const float2 xy = pr_get(pr(p[i], p[i + 1]) * (HALF ? pr_fma(dp, pr(up), pr(-delta_up)) : dp + pr(-delta)));
+          float x = xy.x, y = xy.y;
           if (MASK) {                                         // what is not seen may be anything, a NaN too
             x = i <= lim ? x : 0.f;
             y = i + 1 <= lim ? y : 0.f;
@@ -790,7 +858,6 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (ok && n > 0) ok = warp_wait(&sh->acc_done, 0, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
     if (ok) {
       tc_fence_after();
-      uint16_t* row = reinterpret_cast<uint16_t*>(a.out) + at * a.dim;
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
         const int col = half * (D / 2) + c * 32;
@@ -801,8 +868,12 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
 #pragma unroll
         for (int e = 0; e < 32; ++e) x[e] = last >= 0 ? x[e] : 0u;
-        if (mine) store_columns<HALF>(row + col, x, last >= 0 ? a.scale * down : 0.f, a.dim - col);
+        put_columns<HALF>(sQ, r, col, x, last >= 0 ? a.scale * down : 0.f);   // Q is in TMEM
       }
+      send_rows<D / 2>(sQ, (warp & 3) * 32, half * (D / 2), a.dim, lane, [&](int r) -> uint16_t* {
+        const int tok = r * a.by_hb >> 16, pos = first + tok;
+        return r < rows && pos < L ? reinterpret_cast<uint16_t*>(a.out) + ((long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb)) * a.dim : nullptr;
+      });
     }
   }
   tc_fence_before();
@@ -821,7 +892,7 @@ struct Dkv {
     Unit unit;
     uint32_t tmem_slot;
     int abort_flag;
-    float lse[STAGES][TILE], delta[STAGES][TILE];
+    alignas(16) float lse[STAGES][TILE], delta[STAGES][TILE];             // their negatives; read four at a time
   };
   static constexpr int SMEM = (1 + STAGES) * (KS + VS) * SLAB + (int)sizeof(Shared) + 1024;
 };
@@ -843,7 +914,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int rows = a.hb * a.tok;
   volatile int* abort_flag = &sh->abort_flag;
   if (warp == 0) {
-    const Unit r = find_unit(a, a.cu_k, TILE, u, lane);
+    const Unit r = find_unit(a, true, TILE, u, lane);
     if (lane == 0) sh->unit = r;
   }
   if (tid == 32) {
@@ -885,8 +956,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     clear_rows(a.out2, __ldg(a.cu_k + a.n), a.Tk, a.kv_heads, kvh, 1, a.vdim, u - unit.total, a.units - unit.total);
     return;
   }
-  const int q0 = __ldg(a.cu_q + unit.seq), L = __ldg(a.cu_q + unit.seq + 1) - q0;
-  const int k0 = __ldg(a.cu_k + unit.seq), Lk = __ldg(a.cu_k + unit.seq + 1) - k0;
+  const int q0 = unit.q0, L = unit.L, k0 = unit.k0, Lk = unit.Lk;
   const int off = Lk - L;
   // place 0 is the last key tile of its sequence, which few queries see: the longest loops come first
   const int kt = (Lk + TILE - 1) / TILE - 1 - unit.place, key0 = kt * TILE;
@@ -926,11 +996,11 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       float lse[TILE / 32], delta[TILE / 32];                 // all on their way before the first is put down
 #pragma unroll
       for (int c = 0; c < TILE / 32; ++c) {
-        const int r = c * 32 + lane, tok = r / a.hb, pos = first + tok;
+        const int r = c * 32 + lane, tok = r * a.by_hb >> 16, pos = first + tok;
         const bool mine = r < rows && pos < L;
         const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
-        lse[c] = mine ? __ldg(a.lse + at) : INFINITY;
-        delta[c] = mine ? __ldg(a.delta + at) * up : 0.f;
+        lse[c] = mine ? -__ldg(a.lse + at) : -INFINITY;
+        delta[c] = mine ? __ldg(a.delta + at) * -up : 0.f;
       }
 #pragma unroll
       for (int c = 0; c < TILE / 32; ++c) {
@@ -1023,13 +1093,14 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         tmem_ld_wait();
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          const float4 m = lse[c * 8 + q];
-          const float ms[4] = {m.x, m.y, m.z, m.w};
+          const float4 m = lse[c * 8 + q];                    // as they are subtracted
+          const float2 u = pr_get(pr_fma(pr(__uint_as_float(x[q * 4]), __uint_as_float(x[q * 4 + 1])), pr(a.scale_log2), pr(m.x, m.y)));
+          const float2 v = pr_get(pr_fma(pr(__uint_as_float(x[q * 4 + 2]), __uint_as_float(x[q * 4 + 3])), pr(a.scale_log2), pr(m.z, m.w)));
+          const float es[4] = {ex2(u.x), ex2(u.y), ex2(v.x), ex2(v.y)};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int col = c * 32 + q * 4 + e;
-            const float y = ex2(fmaf(__uint_as_float(x[q * 4 + e]), a.scale_log2, -ms[e]));
-            p[col] = !MASK || (col >= from && col < to) ? y : 0.f;
+            p[col] = !MASK || (col >= from && col < to) ? es[e] : 0.f;
           }
         }
 #pragma unroll
@@ -1051,13 +1122,15 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           const float4 m = delta[c * 8 + q];
-          const float ms[4] = {m.x, m.y, m.z, m.w};
-          float d[4];
+          const int at = c * 32 + q * 4;
+          const Pair d0 = pr(__uint_as_float(x[q * 4]), __uint_as_float(x[q * 4 + 1])), d1 = pr(__uint_as_float(x[q * 4 + 2]), __uint_as_float(x[q * 4 + 3]));
+          const float2 u = pr_get(pr(p[at], p[at + 1]) * (HALF ? pr_fma(d0, pr(up), pr(m.x, m.y)) : d0 + pr(m.x, m.y)));
+          const float2 v = pr_get(pr(p[at + 2], p[at + 3]) * (HALF ? pr_fma(d1, pr(up), pr(m.z, m.w)) : d1 + pr(m.z, m.w)));
+          float d[4] = {u.x, u.y, v.x, v.y};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int col = c * 32 + q * 4 + e;
-            const float y = p[col] * (HALF ? fmaf(__uint_as_float(x[q * 4 + e]), up, -ms[e]) : __uint_as_float(x[q * 4 + e]) - ms[e]);
-            d[e] = !MASK || (col >= from && col < to) ? y : 0.f;
+            const int col = at + e;
+            if (MASK && !(col >= from && col < to)) d[e] = 0.f;
           }
           w[c * 16 + q * 2] = pair<HALF>(d[0], d[1]);
           w[c * 16 + q * 2 + 1] = pair<HALF>(d[2], d[3]);
@@ -1078,10 +1151,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (ok && n > 0) ok = warp_wait(&sh->acc_done, 0, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
     if (ok) {
       tc_fence_after();
-      const bool mine = key0 + r < Lk;
-      const long long at = (long long)(k0 + key0 + r) * a.kv_heads + kvh;
-      uint16_t* krow = reinterpret_cast<uint16_t*>(a.out) + at * a.dim;
-      uint16_t* vrow = reinterpret_cast<uint16_t*>(a.out2) + at * a.vdim;
+      uint8_t* stage = sQ;                                    // the first stage has been used
 #pragma unroll
       for (int c = 0; c < (D + DV) / 64; ++c) {
         const bool k = c < D / 64;
@@ -1094,8 +1164,15 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = 0u;
         }
-        if (mine) store_columns<HALF>((k ? krow : vrow) + col, x, k ? a.scale * down : 1.f, (k ? a.dim : a.vdim) - col);
+        put_columns<HALF>(k ? stage : stage + F::KS * SLAB, r, col, x, k ? a.scale * down : 1.f);
       }
+      auto rows_of = [&](void* out, int width) {
+        return [&, out, width](int r) -> uint16_t* {
+          return key0 + r < Lk ? reinterpret_cast<uint16_t*>(out) + ((long long)(k0 + key0 + r) * a.kv_heads + kvh) * width : nullptr;
+        };
+      };
+      send_rows<D / 2>(stage, (warp & 3) * 32, half * (D / 2), a.dim, lane, rows_of(a.out, a.dim));
+      send_rows<DV / 2>(stage + F::KS * SLAB, (warp & 3) * 32, half * (DV / 2), a.vdim, lane, rows_of(a.out2, a.vdim));
     }
   }
   tc_fence_before();
@@ -1147,6 +1224,7 @@ int shape(Args& a) {
   while (group % a.hb || TILE / a.hb * a.hb < TILE * 15 / 16) --a.hb;
   a.chunks = group / a.hb;
   a.tok = TILE / a.hb;
+  a.by_hb = (65536 + a.hb - 1) / a.hb;       // too large by less than hb / 65536 a step: r hb < 65536
   return 0;
 }
 
