@@ -72,6 +72,12 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[32])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// eight floats in a row of shared memory times four, on their way before the next wait
+__device__ __forceinline__ void lds_row(float4 (&v)[8], const float* src) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[i].x), "=f"(v[i].y), "=f"(v[i].z), "=f"(v[i].w) : "r"(smem_u32(src + 4 * i)) : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -221,34 +227,38 @@ __device__ __forceinline__ void settle(volatile int* abort_flag) {
   }
 }
 
-// 32 accumulator columns times f as 16-bit values, to columns col .. col + 31 of row r of slabs in shared memory
+// 32 fp32 columns as 16-bit values, to columns col .. col + 31 of row r of slabs in shared memory
 template <bool HALF>
-__device__ __forceinline__ void put_columns(uint8_t* slabs, int r, int col, const uint32_t (&x)[32], float f) {
+__device__ __forceinline__ void put_columns(uint8_t* slabs, int r, int col, const uint32_t (&x)[32]) {
   uint8_t* row = slabs + (col >> 6) * SLAB + r * 128;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint4 o;
-    o.x = pair<HALF>(__uint_as_float(x[q * 8]) * f, __uint_as_float(x[q * 8 + 1]) * f);
-    o.y = pair<HALF>(__uint_as_float(x[q * 8 + 2]) * f, __uint_as_float(x[q * 8 + 3]) * f);
-    o.z = pair<HALF>(__uint_as_float(x[q * 8 + 4]) * f, __uint_as_float(x[q * 8 + 5]) * f);
-    o.w = pair<HALF>(__uint_as_float(x[q * 8 + 6]) * f, __uint_as_float(x[q * 8 + 7]) * f);
+    o.x = pair<HALF>(__uint_as_float(x[q * 8]), __uint_as_float(x[q * 8 + 1]));
+    o.y = pair<HALF>(__uint_as_float(x[q * 8 + 2]), __uint_as_float(x[q * 8 + 3]));
+    o.z = pair<HALF>(__uint_as_float(x[q * 8 + 4]), __uint_as_float(x[q * 8 + 5]));
+    o.w = pair<HALF>(__uint_as_float(x[q * 8 + 6]), __uint_as_float(x[q * 8 + 7]));
     *reinterpret_cast<uint4*>(row + ((((col >> 3) + q) & 7) ^ (r & 7)) * 16) = o;
   }
 }
-// The warp's 32 rows of those slabs, columns begin .. begin + COLS - 1 (of `width` that exist), to global rows `row_of(r)` (null: not stored):
-// whole lines, where each thread for itself would store 16 bytes of 32 rows at a time
+// The warp's 32 rows of one slab, its columns as columns begin .. begin + COLS - 1 (of `width` that exist) of global rows `row_of(r)` (null: not
+// stored): whole lines, where each thread for itself would store 16 bytes of 32 rows at a time.  A slab holds 64 columns: begin counts on from it.
 template <int COLS, typename RowOf>
-__device__ __forceinline__ void send_rows(const uint8_t* slabs, int row0, int begin, int width, int lane, RowOf row_of) {
+__device__ __forceinline__ void send_rows(const uint8_t* slab, int row0, int begin, int width, int lane, RowOf row_of) {
   constexpr int LANES = COLS / 8, ROWS = 32 / LANES;
   __syncwarp();
   const int piece = begin / 8 + lane % LANES;
-#pragma unroll 4
-  for (int i = 0; i < 32; i += ROWS) {
-    const int r = row0 + i + lane / LANES;
-    uint16_t* dst = row_of(r);
-    if (dst && piece * 8 < width)
-      reinterpret_cast<uint4*>(dst)[piece] =
-          *reinterpret_cast<const uint4*>(slabs + (piece >> 3) * SLAB + r * 128 + (((piece & 7) ^ (r & 7)) << 4));
+  const bool exists = piece * 8 < width;
+  uint4 v[32 / ROWS];
+#pragma unroll
+  for (int i = 0; i < 32 / ROWS; ++i) {
+    const int r = row0 + i * ROWS + lane / LANES;
+    v[i] = *reinterpret_cast<const uint4*>(slab + r * 128 + (((piece & 7) ^ (r & 7)) << 4));
+  }
+#pragma unroll
+  for (int i = 0; i < 32 / ROWS; ++i) {
+    uint16_t* dst = row_of(row0 + i * ROWS + lane / LANES);
+    if (dst && exists) reinterpret_cast<uint4*>(dst)[piece] = v[i];
   }
   __syncwarp();
 }
@@ -524,8 +534,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           return r < rows && pos < L ? reinterpret_cast<uint16_t*>(out) + ((long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb)) * a.vdim : nullptr;
         };
       };
+      // o to one slab and what its rounding takes away to the other, 64 columns at a time; where Q_t has one slab alone (width 64) one after the other
+      constexpr int PASSES = F::KS == 1 ? 2 : 1;
 #pragma unroll
-      for (int pass = 0; pass < 2; ++pass) {                  // o, then what its rounding takes away
+      for (int pass = 0; pass < PASSES; ++pass) {
         if (pass == 1 && !a.out2) break;
 #pragma unroll
         for (int c = 0; c < DV / 32; ++c) {
@@ -535,13 +547,19 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tmem_ld_wait();
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            o[e] = last >= 0 ? o[e] : 0u;                     // a row without keys
-            if (pass == 1) o[e] = __float_as_uint(rest<HALF>(__uint_as_float(o[e]) * f));
+          for (int e = 0; e < 32; ++e) o[e] = last >= 0 ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;            // a row without keys
+          if (pass == 0) put_columns<HALF>(stage, r, (c & 1) * 32, o);
+          if (a.out2 && pass == PASSES - 1) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(rest<HALF>(__uint_as_float(o[e])));
+            put_columns<HALF>(stage + (PASSES == 1 ? SLAB : 0), r, (c & 1) * 32, o);
           }
-          put_columns<HALF>(stage, r, c * 32, o, pass ? 1.f : f);
+          if (c & 1) {
+            const int begin = (c - 1) * 32;
+            if (pass == 0) send_rows<64>(stage, (warp & 3) * 32, begin, a.vdim, lane, rows_of(a.out));
+            if (a.out2 && pass == PASSES - 1) send_rows<64>(stage + (PASSES == 1 ? SLAB : 0), (warp & 3) * 32, begin, a.vdim, lane, rows_of(a.out2));
+          }
         }
-        send_rows<DV>(stage, (warp & 3) * 32, 0, a.vdim, lane, rows_of(pass ? a.out2 : a.out));
       }
       if (mine && a.lse) a.lse[at] = l == 0.f ? INFINITY : m_ref + log2f(l);
     }
@@ -807,23 +825,19 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (!warp_wait(&sh->s_full[half], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
       tc_fence_after();
       float p[64];
+      uint32_t s0[32], s1[32];
+      tmem_ld_32x32(tS, s0);
+      tmem_ld_32x32(tS + 32, s1);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->s_free[half]);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t s[32];
-        tmem_ld_32x32(tS + c * 32, s);
-        tmem_ld_wait();
-        if (c == 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh->s_free[half]);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float2 x = pr_get(pr_fma(pr(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), pr(a.scale_log2), pr(-lse)));
-          const int i = c * 32 + 2 * e;
-          p[i] = !MASK || i <= lim ? ex2(x.x) : 0.f;
-          p[i + 1] = !MASK || i + 1 <= lim ? ex2(x.y) : 0.f;
-        }
+      for (int e = 0; e < 32; ++e) {
+        const uint32_t (&s)[32] = e < 16 ? s0 : s1;
+        const float2 x = pr_get(pr_fma(pr(__uint_as_float(s[2 * (e & 15)]), __uint_as_float(s[2 * (e & 15) + 1])), pr(a.scale_log2), pr(-lse)));
+        p[2 * e] = !MASK || 2 * e <= lim ? ex2(x.x) : 0.f;
+        p[2 * e + 1] = !MASK || 2 * e + 1 <= lim ? ex2(x.y) : 0.f;
       }
       if (!warp_wait(&sh->dp_full[half], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
       tc_fence_after();
@@ -867,10 +881,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           tmem_ld_wait();
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = last >= 0 ? x[e] : 0u;
-        put_columns<HALF>(sQ, r, col, x, last >= 0 ? a.scale * down : 0.f);   // Q is in TMEM
+        for (int e = 0; e < 32; ++e) x[e] = last >= 0 ? __float_as_uint(__uint_as_float(x[e]) * (a.scale * down)) : 0u;
+        put_columns<HALF>(sQ, r, col, x);                     // Q is in TMEM
       }
-      send_rows<D / 2>(sQ, (warp & 3) * 32, half * (D / 2), a.dim, lane, [&](int r) -> uint16_t* {
+      send_rows<D / 2>(sQ + (D == 128 ? half * SLAB : 0), (warp & 3) * 32, half * (D / 2), a.dim, lane, [&](int r) -> uint16_t* {
         const int tok = r * a.by_hb >> 16, pos = first + tok;
         return r < rows && pos < L ? reinterpret_cast<uint16_t*>(a.out) + ((long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb)) * a.dim : nullptr;
       });
@@ -1085,17 +1099,20 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tc_fence_after();
       float p[64];
       uint32_t w[32];
-      const float4* lse = reinterpret_cast<const float4*>(&sh->lse[s][half * 64]);
+      uint32_t x0[32], x1[32];
+      float4 m[8];
+      tmem_ld_32x32(tS, x0);
+      tmem_ld_32x32(tS + 32, x1);
+      lds_row(m, &sh->lse[s][half * 64]);
+      tmem_ld_wait();
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t x[32];
-        tmem_ld_32x32(tS + c * 32, x);
-        tmem_ld_wait();
+        if (c == 1) lds_row(m, &sh->lse[s][half * 64 + 32]);
+        const uint32_t (&x)[32] = c ? x1 : x0;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float4 m = lse[c * 8 + q];                    // as they are subtracted
-          const float2 u = pr_get(pr_fma(pr(__uint_as_float(x[q * 4]), __uint_as_float(x[q * 4 + 1])), pr(a.scale_log2), pr(m.x, m.y)));
-          const float2 v = pr_get(pr_fma(pr(__uint_as_float(x[q * 4 + 2]), __uint_as_float(x[q * 4 + 3])), pr(a.scale_log2), pr(m.z, m.w)));
+        for (int q = 0; q < 8; ++q) {                         // lse and delta lie there as they are subtracted
+          const float2 u = pr_get(pr_fma(pr(__uint_as_float(x[q * 4]), __uint_as_float(x[q * 4 + 1])), pr(a.scale_log2), pr(m[q].x, m[q].y)));
+          const float2 v = pr_get(pr_fma(pr(__uint_as_float(x[q * 4 + 2]), __uint_as_float(x[q * 4 + 3])), pr(a.scale_log2), pr(m[q].z, m[q].w)));
           const float es[4] = {ex2(u.x), ex2(u.y), ex2(v.x), ex2(v.y)};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -1113,19 +1130,18 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (lane == 0) mbar_arrive(&sh->p_full);
       if (!warp_wait(&sh->dp_full, i & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
       tc_fence_after();
-      const float4* delta = reinterpret_cast<const float4*>(&sh->delta[s][half * 64]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t x[32];
         tmem_ld_32x32(tdP + c * 32, x);
+        lds_row(m, &sh->delta[s][half * 64 + c * 32]);
         tmem_ld_wait();
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          const float4 m = delta[c * 8 + q];
           const int at = c * 32 + q * 4;
           const Pair d0 = pr(__uint_as_float(x[q * 4]), __uint_as_float(x[q * 4 + 1])), d1 = pr(__uint_as_float(x[q * 4 + 2]), __uint_as_float(x[q * 4 + 3]));
-          const float2 u = pr_get(pr(p[at], p[at + 1]) * (HALF ? pr_fma(d0, pr(up), pr(m.x, m.y)) : d0 + pr(m.x, m.y)));
-          const float2 v = pr_get(pr(p[at + 2], p[at + 3]) * (HALF ? pr_fma(d1, pr(up), pr(m.z, m.w)) : d1 + pr(m.z, m.w)));
+          const float2 u = pr_get(pr(p[at], p[at + 1]) * (HALF ? pr_fma(d0, pr(up), pr(m[q].x, m[q].y)) : d0 + pr(m[q].x, m[q].y)));
+          const float2 v = pr_get(pr(p[at + 2], p[at + 3]) * (HALF ? pr_fma(d1, pr(up), pr(m[q].z, m[q].w)) : d1 + pr(m[q].z, m[q].w)));
           float d[4] = {u.x, u.y, v.x, v.y};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -1164,15 +1180,19 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = 0u;
         }
-        put_columns<HALF>(k ? stage : stage + F::KS * SLAB, r, col, x, k ? a.scale * down : 1.f);
+        if (k) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * (a.scale * down));
+        }
+        put_columns<HALF>(k ? stage : stage + F::KS * SLAB, r, col, x);
       }
       auto rows_of = [&](void* out, int width) {
         return [&, out, width](int r) -> uint16_t* {
           return key0 + r < Lk ? reinterpret_cast<uint16_t*>(out) + ((long long)(k0 + key0 + r) * a.kv_heads + kvh) * width : nullptr;
         };
       };
-      send_rows<D / 2>(stage, (warp & 3) * 32, half * (D / 2), a.dim, lane, rows_of(a.out, a.dim));
-      send_rows<DV / 2>(stage + F::KS * SLAB, (warp & 3) * 32, half * (DV / 2), a.vdim, lane, rows_of(a.out2, a.vdim));
+      send_rows<D / 2>(stage + (D == 128 ? half * SLAB : 0), (warp & 3) * 32, half * (D / 2), a.dim, lane, rows_of(a.out, a.dim));
+      send_rows<DV / 2>(stage + (F::KS + (DV == 128 ? half : 0)) * SLAB, (warp & 3) * 32, half * (DV / 2), a.vdim, lane, rows_of(a.out2, a.vdim));
     }
   }
   tc_fence_before();
