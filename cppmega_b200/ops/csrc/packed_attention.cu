@@ -18,9 +18,10 @@
 //
 // Forward: one block per pair of query tiles.  A warp loads, one thread issues the products, a warpgroup per query tile (thread <-> row <->
 // TMEM lane) does the softmax: P goes back to TMEM as an operand, O stays there and is rescaled only when a row's maximum has grown by 2^8.
-// Backward: two kernels with seven products instead of one with five.  One kernel has a fixed set of columns too few (S, dP, dK, dV and dQ of 128
+// Backward: two kernels with seven products, after a small one for delta, instead of one with five.  One kernel has a fixed set of columns too few (S, dP, dK, dV and dQ of 128
 // columns are 640 of 512) and adds dQ across blocks with atomics, in an order that changes from run to run; in two, P and dS of either
 // orientation are operands in TMEM that never pass through shared memory, every sum has one owner, and the bits are the same each time.
+//   delta  rows of o and do, read once
 //   dq     block per query tile, loops over key tiles:   S = Q K', dP = dO V', dQ += dS K
 //   dk dv  block per key tile, loops over query tiles:   S' = K Q', dP' = V dO', dV += P' dO, dK += dS' Q
 // The issuing threads take the products in a fixed order (the bits are the same each time) in which each has its operands before the one in front
@@ -127,6 +128,7 @@ struct Args {
   long long go_tok, go_head;
   float* lse;                                // [T, heads]: log2 of the sum of weights; +inf without keys; null: not wanted
   float* delta;                              // [T, heads]
+  float* big;                                // [T, heads]: largest |do| of a row (fp16)
   uint32_t* top;                             // largest |do| of the call as bits (fp16)
   int* err;
 };
@@ -570,7 +572,63 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (warp == MMA_WARP) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
-// ---- backward: query gradients, and delta ------------------------------------------------------------------------------
+// ---- backward: delta -----------------------------------------------------------------------------------------------------
+// delta[i] = do[i] . o[i] before its rounding, in fp16 also the row's largest |do| and the call's.  DV / 8 lanes a row, four rows of a lane on their way
+// at once: three reads of a row's width at the memory's rate.  Inside the dq kernel, whose blocks have an SM to themselves, nothing would
+// run meanwhile (9000 cycles a block, 120 us at 16384 x 32 rows of 128; here 65).
+constexpr int DELTA_THREADS = 256, DELTA_AHEAD = 4;
+
+template <bool HALF, int LANES>
+__global__ void __launch_bounds__(DELTA_THREADS, 4) packed_delta_kernel(const Args a) {
+  constexpr int ROWS = DELTA_THREADS / LANES;
+  const int piece = threadIdx.x % LANES;
+  // what lies behind the last sequence counts for nothing
+  const long long rows = (long long)min(max(__ldg(a.cu_q + a.n), 0), a.T) * a.heads, base = (long long)blockIdx.x * (ROWS * DELTA_AHEAD);
+  const long long row0 = base + threadIdx.x / LANES, tok0 = base / a.heads;
+  const unsigned head0 = unsigned(base - tok0 * a.heads) + threadIdx.x / LANES;
+  uint4 x[DELTA_AHEAD], z[DELTA_AHEAD], y[DELTA_AHEAD];
+#pragma unroll
+  for (int i = 0; i < DELTA_AHEAD; ++i) {
+    const long long row = row0 + i * ROWS;
+    x[i] = z[i] = y[i] = make_uint4(0, 0, 0, 0);
+    if (row < rows && piece * 8 < a.vdim) {
+      const unsigned more = (head0 + i * ROWS) / unsigned(a.heads), head = head0 + i * ROWS - more * a.heads;
+      const long long tok = tok0 + more;
+      x[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o) + row * a.vdim) + piece);
+      z[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o_rest) + row * a.vdim) + piece);
+      y[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.go) + tok * a.go_tok + head * a.go_head) + piece);
+    }
+  }
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < DELTA_AHEAD; ++i) {
+    const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, zs[4] = {z[i].x, z[i].y, z[i].z, z[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+    float dot = 0.f, big = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpair<HALF>(xs[e]), h = unpair<HALF>(zs[e]), g = unpair<HALF>(ys[e]);
+      dot = fmaf(f.x + h.x, g.x, fmaf(f.y + h.y, g.y, dot));
+      if (HALF) big = fmaxf(big, fmaxf(fabsf(g.x), fabsf(g.y)));
+    }
+#pragma unroll
+    for (int o = LANES >> 1; o > 0; o >>= 1) {
+      dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if (HALF) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+    }
+    const long long row = row0 + i * ROWS;
+    if (piece == 0 && row < rows) {
+      a.delta[row] = dot;
+      if (HALF) a.big[row] = big;
+    }
+    if (HALF && isfinite(big)) most = fmaxf(most, big);
+  }
+  if (HALF) {                                // the largest is the same in any order
+    const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+    if ((threadIdx.x & 31) == 0 && all) atomicMax(a.top, all);
+  }
+}
+
+// ---- backward: query gradients -------------------------------------------------------------------------------------------
 template <int D, int DV>
 struct Dq {
   static constexpr int KS = D / 64, VS = DV / 64, K_SLOTS = 3, V_SLOTS = 2;
@@ -580,7 +638,6 @@ struct Dq {
     Unit unit;
     uint32_t tmem_slot;
     int abort_flag;
-    float delta[TILE], big[TILE];
   };
   static constexpr int SMEM = (KS + VS + K_SLOTS * KS + V_SLOTS * VS) * SLAB + (int)sizeof(Shared) + 1024;
 };
@@ -739,68 +796,11 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const bool mine = r < rows && pos < L;
     const int last = mine ? off + pos : -1, head = head0 + (r - tok * a.hb);
     const long long at = (long long)(q0 + pos) * a.heads + head;
-    // delta, and the power of two that brings the row's largest |do| to 2^-4: DV / 8 lanes a row, four rows of a lane on their way at once
-    {
-      constexpr int LANES = DV / 8, ROWS = 32 / LANES, AHEAD = 4;
-      const int piece = lane % LANES;
-#pragma unroll 1
-      for (int i0 = 0; i0 < 16; i0 += ROWS * AHEAD) {
-        uint4 x[AHEAD], z[AHEAD], y[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          const int row = warp * 16 + i0 + i * ROWS + lane / LANES, tok = row * a.by_hb >> 16, pos = first + tok, head = head0 + (row - tok * a.hb);
-          const bool there = row < rows && pos < L && piece * 8 < a.vdim;
-          const long long at = ((long long)(q0 + pos) * a.heads + head) * a.vdim + piece * 8;
-          x[i] = z[i] = y[i] = make_uint4(0, 0, 0, 0);
-          if (there) {
-            x[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o) + at));
-            z[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.o_rest) + at));
-            y[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.go) + (q0 + pos) * a.go_tok + head * a.go_head + piece * 8));
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, zs[4] = {z[i].x, z[i].y, z[i].z, z[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
-          float dot = 0.f, big = 0.f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = unpair<HALF>(xs[e]), h = unpair<HALF>(zs[e]), g = unpair<HALF>(ys[e]);
-            dot = fmaf(f.x + h.x, g.x, fmaf(f.y + h.y, g.y, dot));
-            if (HALF) big = fmaxf(big, fmaxf(fabsf(g.x), fabsf(g.y)));
-          }
-#pragma unroll
-          for (int o = LANES >> 1; o > 0; o >>= 1) {
-            dot += __shfl_xor_sync(0xffffffffu, dot, o);
-            if (HALF) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-          }
-          if (piece == 0) {
-            const int row = warp * 16 + i0 + i * ROWS + lane / LANES;
-            sh->delta[row] = dot;
-            if (HALF) sh->big[row] = big;
-          }
-        }
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-    }
-    const float delta = sh->delta[r], big = HALF ? sh->big[r] : 0.f;
-    float up = 1.f, down = 1.f;
-    if (HALF) {
-      if (big > 0.f && isfinite(big)) {
-        const int e = 127 - 4 - int(__float_as_uint(big) >> 23);
-        up = __uint_as_float(uint32_t(127 + e) << 23);
-        down = __uint_as_float(uint32_t(127 - e) << 23);
-      }
-      if (half == 0) {
-        const uint32_t all = __reduce_max_sync(0xffffffffu, mine && isfinite(big) ? __float_as_uint(big) : 0u);
-        if (lane == 0 && all) atomicMax(a.top, all);
-      }
-    }
+    const float delta = mine ? a.delta[at] : 0.f;
     const float lse = mine ? a.lse[at] : INFINITY;
-    if (mine && half == 0) a.delta[at] = delta;
     const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
-    const float delta_up = delta * up;
     bool ok = n == 0 || warp_wait(&sh->q_full, 0, abort_flag, a.err, ERR_WAIT_FULL);
-    if (ok && n > 0) {                       // Q and dO go to TMEM, half a row from each of its two threads
+    if (ok && n > 0) {                       // half a row from each of its two threads
       auto fill = [&](const uint8_t* tile, int slabs, uint32_t to) {
         if (half >= slabs) return;
         uint32_t x[32];
@@ -818,6 +818,16 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->rows_in);
     }
+    float up = 1.f, down = 1.f;              // fp16: the power of two that brings the row's largest |do| to 2^-4
+    if (HALF) {
+      const float big = mine ? a.big[at] : 0.f;
+      if (big > 0.f && isfinite(big)) {
+        const int e = 127 - 4 - int(__float_as_uint(big) >> 23);
+        up = __uint_as_float(uint32_t(127 + e) << 23);
+        down = __uint_as_float(uint32_t(127 - e) << 23);
+      }
+    }
+    const float delta_up = delta * up;
     auto tile = [&](int j, auto where) {
       constexpr bool MASK = decltype(where)::value;
       const int lim = last - j * TILE - half * 64;
@@ -1286,6 +1296,13 @@ int backward(const Inputs& in, Args a, void* dq, void* dk, void* dv, cudaStream_
   const long long uq = units_of(a.T, a.n, a.tok), uk = units_of(a.Tk, a.n, TILE);
   if (uq * a.kv_heads * a.chunks > 0x7fffffffLL || uk * a.kv_heads > 0x7fffffffLL) return -10;
   if (HALF && cudaMemsetAsync(a.top, 0, sizeof(uint32_t), stream) != cudaSuccess) return -3;
+  {
+    constexpr int LANES = DV / 8, ROWS = DELTA_THREADS / LANES * DELTA_AHEAD;
+    const long long blocks = ((long long)a.T * a.heads + ROWS - 1) / ROWS;
+    if (blocks > 0x7fffffffLL) return -10;
+    packed_delta_kernel<HALF, LANES><<<(unsigned)blocks, DELTA_THREADS, 0, stream>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return -3;
+  }
   a.units = (int)uq;
   a.out = dq;
   packed_dq_kernel<HALF, D, DV><<<(unsigned)(uq * a.kv_heads * a.chunks), THREADS, Dq<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], m[3], a);
@@ -1335,7 +1352,7 @@ extern "C" int cm_packed_attention_fwd(const void* q, const void* k, const void*
   return a.dim > 64 ? forward<true, 128, 64>(in, a, stream) : forward<true, 64, 64>(in, a, stream);
 }
 
-// o, o_rest and lse from the forward; go (the gradient of o) [T, heads, vdim]; delta: scratch of T * heads + 1 floats;
+// o, o_rest and lse from the forward; go (the gradient of o) [T, heads, vdim]; delta: scratch of T * heads floats, fp16: 2 T heads + 1;
 // dq [T, heads, dim], dk [Tk, kv_heads, dim], dv [Tk, kv_heads, vdim] packed, all written whole
 extern "C" int cm_packed_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* go, const int* cu_q,
                                        const int* cu_k, const float* lse, float* delta, void* dq, void* dk, void* dv, const long long* n, float scale,
@@ -1347,7 +1364,8 @@ extern "C" int cm_packed_attention_bwd(const void* q, const void* k, const void*
   a.go_tok = n[6]; a.go_head = n[7];
   a.lse = const_cast<float*>(lse);
   a.delta = delta;
-  a.top = reinterpret_cast<uint32_t*>(delta + (long long)a.T * a.heads);
+  a.big = delta + (long long)a.T * a.heads;
+  a.top = reinterpret_cast<uint32_t*>(a.big + (long long)a.T * a.heads);
   const Inputs in = {q, k, v, go, n, n + 2, n + 4, n + 6};
   if (n[15] == 0) {
     if (a.vdim > 64) return backward<false, 128, 128>(in, a, dq, dk, dv, stream);

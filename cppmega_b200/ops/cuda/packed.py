@@ -85,7 +85,7 @@ class PackedAttentionFn(torch.autograd.Function):
         lse = _given_back(lse, torch.float32, dev)
         go = _packed(go)
         dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
-        delta = torch.empty(lse.numel() + 1, dtype=torch.float32, device=dev)
+        delta = torch.empty(lse.numel() if dt == torch.bfloat16 else 2 * lse.numel() + 1, dtype=torch.float32, device=dev)
         plan = planned((F_.layout_of("packed_attention_bwd", q, k, v, go, cu_q)), lambda: Plan(_numbers(q, k, v, cu_q, go)))
         rc = _cu.lib().cm_packed_attention_bwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(), go.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
@@ -93,7 +93,7 @@ class PackedAttentionFn(torch.autograd.Function):
             _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
         if rc:
             _failed("cm_packed_attention_bwd", rc)
-        F_.count_launch("packed_attention_bwd", 2)
+        F_.count_launch("packed_attention_bwd", 3)
         return dq, dk, dv, None, None, None, None
 
 
