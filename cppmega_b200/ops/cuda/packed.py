@@ -53,6 +53,15 @@ def _plan(q, k, v, cu_q, cu_k):
                 copy=not (_strides_ok(q) and _strides_ok(k) and _strides_ok(v) and cu_q.is_contiguous() and (cu_k is None or cu_k.is_contiguous())))
 
 
+def _plan_backward(dt, q, k, v, cu_q, cu_k, o, rest, lse, go):
+    """False where a tensor is not in the form in which the forward left it, or an upstream gradient has to be copied."""
+    if not (all(t.dtype == dt and t.device == go.device for t in (q, k, v, o, rest, go)) and all(_strides_ok(t) for t in (q, k, v, go))
+            and all(t.is_contiguous() and t.device == go.device for t in (cu_q, cu_k, o, rest, lse))
+            and cu_q.dtype == cu_k.dtype == torch.int32 and lse.dtype == torch.float32):
+        return False
+    return Plan(_numbers(q, k, v, cu_q, go), work=lse.numel() if dt == torch.bfloat16 else 2 * lse.numel() + 1)
+
+
 def _forward(plan, q, k, v, cu_q, cu_k, scale, keep):
     dev = q.device
     o = torch.empty_like(q) if plan.like else torch.empty(plan.shape, dtype=q.dtype, device=dev)
@@ -77,16 +86,20 @@ class PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     @_first_order
     def backward(ctx, go):
-        dt, dev = ctx.dtype, go.device
-        q, k, v, cu_q, cu_k, o, rest, lse = ctx.saved_tensors
-        q, k, v = (_packed(_given_back(t, dt, dev, packed=False)) for t in (q, k, v))
-        o, rest = (_given_back(t, dt, dev, align=16) for t in (o, rest))
-        cu_q, cu_k = (_given_back(t, torch.int32, dev) for t in (cu_q, cu_k))
-        lse = _given_back(lse, torch.float32, dev)
-        go = _packed(go)
+        saved = ctx.saved_tensors
+        layout = F_.layout_of("packed_attention_bwd", *saved, go)
+        plan = planned(layout, lambda: _plan_backward(ctx.dtype, *saved, go))
+        q, k, v, cu_q, cu_k, o, rest, lse = saved
+        if not plan or (q.data_ptr() | k.data_ptr() | v.data_ptr() | o.data_ptr() | rest.data_ptr() | go.data_ptr()) & 15:
+            dt, dev = ctx.dtype, go.device     # whatever form a saved-tensor hook gave the values back in
+            q, k, v = (_packed(_given_back(t, dt, dev, packed=False)) for t in (q, k, v))
+            o, rest = (_given_back(t, dt, dev, align=16) for t in (o, rest))
+            cu_q, cu_k = (_given_back(t, torch.int32, dev) for t in (cu_q, cu_k))
+            lse, go = _given_back(lse, torch.float32, dev), _packed(go)
+            plan = _plan_backward(dt, q, k, v, cu_q, cu_k, o, rest, lse, go)
+        dev = go.device
         dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
-        delta = torch.empty(lse.numel() if dt == torch.bfloat16 else 2 * lse.numel() + 1, dtype=torch.float32, device=dev)
-        plan = planned((F_.layout_of("packed_attention_bwd", q, k, v, go, cu_q)), lambda: Plan(_numbers(q, k, v, cu_q, go)))
+        delta = torch.empty(plan.work, dtype=torch.float32, device=dev)
         rc = _cu.lib().cm_packed_attention_bwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(), go.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
             lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), plan.at, ctx.scale,
