@@ -243,32 +243,44 @@ __device__ __forceinline__ void put_columns(uint8_t* slabs, int r, int col, cons
     *reinterpret_cast<uint4*>(row + ((((col >> 3) + q) & 7) ^ (r & 7)) * 16) = o;
   }
 }
-// The warp's 32 rows of one slab, its columns as columns begin .. begin + COLS - 1 (of `width` that exist) of global rows `row_of(r)` (null: not
-// stored): whole lines, where each thread for itself would store 16 bytes of 32 rows at a time.  A slab holds 64 columns: begin counts on from it.
-template <int COLS, typename RowOf>
-__device__ __forceinline__ void send_rows(const uint8_t* slab, int row0, int begin, int width, int lane, RowOf row_of) {
-  constexpr int LANES = COLS / 8, ROWS = 32 / LANES;
+// Which rows of a tile a lane sends with LANES lanes a row: their places behind the tile's first row of the result in steps of the result's width,
+// -1 for those that are not stored
+template <int LANES, typename PlaceOf>
+__device__ __forceinline__ void places(int (&at)[LANES], int row0, int lane, PlaceOf place_of) {
+#pragma unroll
+  for (int i = 0; i < LANES; ++i) at[i] = place_of(row0 + i * (32 / LANES) + lane / LANES);
+}
+// The warp's 32 rows of one slab (64 columns), its columns as columns begin .. begin + 8 LANES - 1 of the result, of whose `width` that exist: whole
+// lines, where each thread for itself would store 16 bytes of 32 rows at a time
+template <int LANES>
+__device__ __forceinline__ void send_rows(const uint8_t* slab, int row0, int begin, int width, int lane, const int (&at)[LANES], uint16_t* out) {
   __syncwarp();
   const int piece = begin / 8 + lane % LANES;
   const bool exists = piece * 8 < width;
-  uint4 v[32 / ROWS];
+  uint4 v[LANES];
 #pragma unroll
-  for (int i = 0; i < 32 / ROWS; ++i) {
-    const int r = row0 + i * ROWS + lane / LANES;
+  for (int i = 0; i < LANES; ++i) {
+    const int r = row0 + i * (32 / LANES) + lane / LANES;
     v[i] = *reinterpret_cast<const uint4*>(slab + r * 128 + (((piece & 7) ^ (r & 7)) << 4));
   }
+  out += piece * 8;
 #pragma unroll
-  for (int i = 0; i < 32 / ROWS; ++i) {
-    uint16_t* dst = row_of(row0 + i * ROWS + lane / LANES);
-    if (dst && exists) reinterpret_cast<uint4*>(dst)[piece] = v[i];
-  }
+  for (int i = 0; i < LANES; ++i)
+    if (at[i] >= 0 && exists) *reinterpret_cast<uint4*>(out + (long long)at[i] * width) = v[i];
   __syncwarp();
 }
 
-// What the rounding of put_columns takes away, to as many bits again
+// 32 fp32 columns less what put_columns makes of them
 template <bool HALF>
-__device__ __forceinline__ float rest(float x) {
-  return HALF ? x - __half2float(__float2half_rn(x)) : x - __bfloat162float(__float2bfloat16_rn(x));
+__device__ __forceinline__ void take_rest(uint32_t (&x)[32]) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    const float2 v = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+    const uint32_t w = pair<HALF>(v.x, v.y);
+    const float2 u = HALF ? unpair<HALF>(w) : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    x[e] = __float_as_uint(v.x - u.x);
+    x[e + 1] = __float_as_uint(v.y - u.y);
+  }
 }
 
 struct Masked { static constexpr bool value = true; };
@@ -328,6 +340,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     fence_mbar_init();
   }
   if (warp == MMA_WARP) { tmem_alloc(&sh->tmem_slot, 512); tmem_relinquish(); }
+  if (warp == FWD_TMA_WARP && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
   tc_fence_before();
   const bool drain = setup_barrier(a.err);
   tc_fence_after();
@@ -530,12 +547,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
       const float f = last >= 0 ? inv : 0.f;
       uint8_t* stage = sQ + t * F::KS * SLAB;                 // Q_t has been used
-      auto rows_of = [&](void* out) {
-        return [&, out](int r) -> uint16_t* {
-          const int tok = r * a.by_hb >> 16, pos = qt * a.tok + tok;
-          return r < rows && pos < L ? reinterpret_cast<uint16_t*>(out) + ((long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb)) * a.vdim : nullptr;
-        };
-      };
+      int places_at[8];
+      places(places_at, (warp & 3) * 32, lane, [&](int r) {
+        const int tok = r * a.by_hb >> 16;
+        return r < rows && qt * a.tok + tok < L ? tok * a.heads + (r - tok * a.hb) : -1;
+      });
+      const long long first = ((long long)(q0 + qt * a.tok) * a.heads + head0) * a.vdim;
       // o to one slab and what its rounding takes away to the other, 64 columns at a time; where Q_t has one slab alone (width 64) one after the other
       constexpr int PASSES = F::KS == 1 ? 2 : 1;
 #pragma unroll
@@ -552,14 +569,14 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int e = 0; e < 32; ++e) o[e] = last >= 0 ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;            // a row without keys
           if (pass == 0) put_columns<HALF>(stage, r, (c & 1) * 32, o);
           if (a.out2 && pass == PASSES - 1) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(rest<HALF>(__uint_as_float(o[e])));
+            take_rest<HALF>(o);
             put_columns<HALF>(stage + (PASSES == 1 ? SLAB : 0), r, (c & 1) * 32, o);
           }
           if (c & 1) {
             const int begin = (c - 1) * 32;
-            if (pass == 0) send_rows<64>(stage, (warp & 3) * 32, begin, a.vdim, lane, rows_of(a.out));
-            if (a.out2 && pass == PASSES - 1) send_rows<64>(stage + (PASSES == 1 ? SLAB : 0), (warp & 3) * 32, begin, a.vdim, lane, rows_of(a.out2));
+            if (pass == 0) send_rows(stage, (warp & 3) * 32, begin, a.vdim, lane, places_at, reinterpret_cast<uint16_t*>(a.out) + first);
+            if (a.out2 && pass == PASSES - 1) 
+              send_rows(stage + (PASSES == 1 ? SLAB : 0), (warp & 3) * 32, begin, a.vdim, lane, places_at, reinterpret_cast<uint16_t*>(a.out2) + first);
           }
         }
       }
@@ -894,10 +911,13 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         for (int e = 0; e < 32; ++e) x[e] = last >= 0 ? __float_as_uint(__uint_as_float(x[e]) * (a.scale * down)) : 0u;
         put_columns<HALF>(sQ, r, col, x);                     // Q is in TMEM
       }
-      send_rows<D / 2>(sQ + (D == 128 ? half * SLAB : 0), (warp & 3) * 32, half * (D / 2), a.dim, lane, [&](int r) -> uint16_t* {
-        const int tok = r * a.by_hb >> 16, pos = first + tok;
-        return r < rows && pos < L ? reinterpret_cast<uint16_t*>(a.out) + ((long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb)) * a.dim : nullptr;
+      int places_at[D / 16];
+      places(places_at, (warp & 3) * 32, lane, [&](int r) {
+        const int tok = r * a.by_hb >> 16;
+        return r < rows && first + tok < L ? tok * a.heads + (r - tok * a.hb) : -1;
       });
+      send_rows(sQ + (D == 128 ? half * SLAB : 0), (warp & 3) * 32, half * (D / 2), a.dim, lane, places_at,
+                reinterpret_cast<uint16_t*>(a.out) + ((long long)(q0 + first) * a.heads + head0) * a.dim);
     }
   }
   tc_fence_before();
@@ -1196,13 +1216,14 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         put_columns<HALF>(k ? stage : stage + F::KS * SLAB, r, col, x);
       }
-      auto rows_of = [&](void* out, int width) {
-        return [&, out, width](int r) -> uint16_t* {
-          return key0 + r < Lk ? reinterpret_cast<uint16_t*>(out) + ((long long)(k0 + key0 + r) * a.kv_heads + kvh) * width : nullptr;
-        };
-      };
-      send_rows<D / 2>(stage + (D == 128 ? half * SLAB : 0), (warp & 3) * 32, half * (D / 2), a.dim, lane, rows_of(a.out, a.dim));
-      send_rows<DV / 2>(stage + (F::KS + (DV == 128 ? half : 0)) * SLAB, (warp & 3) * 32, half * (DV / 2), a.vdim, lane, rows_of(a.out2, a.vdim));
+      auto place_of = [&](int r) { return key0 + r < Lk ? r * a.kv_heads : -1; };
+      const long long first = (long long)(k0 + key0) * a.kv_heads + kvh;
+      int k_at[D / 16], v_at[DV / 16];
+      places(k_at, (warp & 3) * 32, lane, place_of);
+      places(v_at, (warp & 3) * 32, lane, place_of);
+      send_rows(stage + (D == 128 ? half * SLAB : 0), (warp & 3) * 32, half * (D / 2), a.dim, lane, k_at, reinterpret_cast<uint16_t*>(a.out) + first * a.dim);
+      send_rows(stage + (F::KS + (DV == 128 ? half : 0)) * SLAB, (warp & 3) * 32, half * (DV / 2), a.vdim, lane, v_at,
+                reinterpret_cast<uint16_t*>(a.out2) + first * a.vdim);
     }
   }
   tc_fence_before();
