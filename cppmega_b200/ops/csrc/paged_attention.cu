@@ -261,11 +261,16 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
   // where the copies go: K by (eight keys, piece of four lanes), V by (row of a lane's fragment, piece of eight lanes)
   const uint8_t *k_lane = a.k + kr * a.k_tok + kc * 16, *v_lane = a.v + vr * a.v_tok + vc * 16;
   const uint32_t k_dst = (kc >> 2) * 512 + ((kr * 4 + (kc & 3)) ^ ((kc >> 2 & 1) * 4)) * 16;
-  auto v_dst = [&](int i) {
+  uint32_t v_dst[VC / 2];
+#pragma unroll
+  for (int i = 0; i < VC / 2; ++i) {
     const int key = i * (32 / VC) + vr, quad_of = key >> 1 & 3, y = (key & 1) | (key >> 3 << 1);
-    return F::V_BYTES == 16 ? ((y * F::V_PIECES + (vc >> 3)) * 32 + quad_of * 8 + ((vc & 7) ^ (2 * quad_of))) * 16
-                            : y * 256 + ((vc >> 1) * 8 + quad_of * 2 + (vc & 1)) * 16;
-  };
+    v_dst[i] = F::V_BYTES == 16 ? ((y * F::V_PIECES + (vc >> 3)) * 32 + quad_of * 8 + ((vc & 7) ^ (2 * quad_of))) * 16
+                                : y * 256 + ((vc >> 1) * 8 + quad_of * 2 + (vc & 1)) * 16;
+  }
+  const uint8_t *k_row = k_lane, *v_row = v_lane;             // aligned: this lane's first rows of the step
+  long long scale_row = 0;                                    // and the place of its first key's exponents
+  bool turned = true;                                         // the step lies in another page than the one before
   auto issue = [&](int stage) {
     if (left > 0) {
       const int head = to.c * a.side + side, room = to.len - to.step * KEYS;          // key head; keys of the step
@@ -274,15 +279,23 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
       if (a.aligned) {
         if (!known && a.err && lane == 0) atomicCAS(a.err, 0, ERR_BAD_ARG);
         const int keys = known ? room : 0;
-        const uint8_t* ks = k_lane + page * a.k_page + (long long)in * a.k_tok + (long long)head * a.k_head;
-        const uint8_t* vs = v_lane + page * a.v_page + (long long)in * a.v_tok + (long long)head * a.v_head;
-        if (E4M3 && lane < KEYS) rows_of[stage * KEYS + lane] = lane < keys ? ((long long)page * a.page + in + lane) * a.kv_heads + head : -1;
+        if (turned) {
+          k_row = k_lane + page * a.k_page + (long long)in * a.k_tok + (long long)head * a.k_head;
+          v_row = v_lane + page * a.v_page + (long long)in * a.v_tok + (long long)head * a.v_head;
+          if (E4M3) scale_row = ((long long)page * a.page + in + lane) * a.kv_heads + head;
+        } else {
+          k_row += KEYS * a.k_tok;
+          v_row += KEYS * a.v_tok;
+          if (E4M3) scale_row += KEYS * a.kv_heads;
+        }
+        const uint8_t *ks = k_row, *vs = v_row;
+        if (E4M3 && lane < KEYS) rows_of[stage * KEYS + lane] = lane < keys ? scale_row : -1;
         if (keys >= KEYS && a.dim == D && a.vdim == DV) {     // nothing to leave out
 #pragma unroll
           for (int i = 0; i < KC / 2; ++i, ks += 32 / KC * a.k_tok)
             copy_whole(k_to + (i * (32 / KC) >> 3) * F::K_PIECES * 512 + (i * (32 / KC) & 7) * 64, ks);
 #pragma unroll
-          for (int i = 0; i < VC / 2; ++i, vs += 32 / VC * a.v_tok) copy_whole(v_to + v_dst(i), vs);
+          for (int i = 0; i < VC / 2; ++i, vs += 32 / VC * a.v_tok) copy_whole(v_to + v_dst[i], vs);
         } else {
 #pragma unroll
           for (int i = 0; i < KC / 2; ++i, ks += 32 / KC * a.k_tok) {
@@ -292,7 +305,7 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
 #pragma unroll
           for (int i = 0; i < VC / 2; ++i, vs += 32 / VC * a.v_tok) {
             const bool there = v_exists && i * (32 / VC) + vr < keys;
-            copy_piece(v_to + v_dst(i), there ? vs : a.v, there);
+            copy_piece(v_to + v_dst[i], there ? vs : a.v, there);
           }
         }
       } else {
@@ -311,22 +324,24 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
         for (int i = 0; i < VC / 2; ++i) {
           const long long o = __shfl_sync(0xffffffffu, vo, i * (32 / VC) + vr);
           const bool here = v_exists && o >= 0;
-          copy_piece(v_to + v_dst(i), here ? a.v + o + vc * 16 : a.v, here);
+          copy_piece(v_to + v_dst[i], here ? a.v + o + vc * 16 : a.v, here);
         }
       }
       if (--left > 0) {
         const int before = to.step;
         advance(a, to, bad);
+        turned = true;
         if (to.step == before + 1 && a.page >= KEYS) {        // the next sixteen keys of the same pair
           in += KEYS;
-          if (in >= a.page) {
+          turned = in >= a.page;
+          if (turned) {
             in -= a.page;
             ++col;
           }
         } else {
           find_page();
         }
-        load_page();
+        if (turned || !a.aligned) load_page();
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -720,19 +735,19 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const Args a, int
   reinterpret_cast<uint32_t*>(a.out)[((long long)blockIdx.x * a.vdim + col) >> 1] = pair<BF16>(x * inv, y * inv);
 }
 
-constexpr bool NT2 = true;
 struct Layout {
   int nt, tiles, rows, grid, warps, dim, vdim, side, chunks, runs;
   long long floats;
 };
 
 // Heads of a group in tiles of eight: up to four tiles a warp with 64 value columns, two with 128 (its registers hold no more); more go to
-// neighbouring warps, which read the same keys at the same time, out of L2.
+// neighbouring warps, which read the same keys at the same time, out of L2 (32 heads on one key head of 128 and 64, 48 sequences of 32768: 121 us
+// with four tiles a warp, 143 with two warps of two).
 Layout layout_of(int sequences, int kv_heads, int group, int dim, int vdim, int columns, int page, bool e4m3) {
   Layout s;
   s.vdim = vdim <= 64 ? 64 : 128;
   s.dim = dim <= 64 && s.vdim == 64 ? 64 : 128;
-  s.nt = group <= 8 ? 1 : group <= 16 || s.vdim == 128 || NT2 ? 2 : 4;
+  s.nt = group <= 8 ? 1 : group <= 16 || s.vdim == 128 ? 2 : 4;
   s.tiles = 1;
   while (s.tiles * 8 * s.nt < group) s.tiles *= 2;
   s.warps = warps_of(e4m3, s.dim, s.vdim, s.nt);
@@ -767,7 +782,8 @@ int start(const Args& a, int grid, cudaStream_t stream) {
     kern<<<grid, F::WARPS * 32, smem, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return -3;
   }
-  // few blocks have many pieces each: 16 warps read them side by side (131071 tokens, 222 pieces: JOINLONG), many blocks have few
+  // few blocks have many pieces each: 16 warps read them side by side (131071 tokens, 222 pieces,
+  // both kernels: 95 us, 107 with 8 warps); many blocks have few
   const int blocks = a.sequences * a.kv_heads * a.group;
   if (blocks <= 2 * sm_count()) return few::launch_early(join_kernel<BF16, DV, 16>, dim3(blocks), dim3(512), 0, stream, a, 8 * NT);
   return few::launch_early(join_kernel<BF16, DV, 4>, dim3(blocks), dim3(128), 0, stream, a, 8 * NT);

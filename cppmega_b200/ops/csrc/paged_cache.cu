@@ -45,6 +45,7 @@ struct Side {                                // keys or values
   long long c_page;                          // strides in bytes
   int x_tok, x_head, c_tok, c_head;
   int lanes, width;                          // lanes of a row (8, 16 or 32), 16-byte pieces of the packed row (8 values each)
+  int wide;                                  // an E4M3 cache whose rows are whole 16-byte pieces
 };
 
 __device__ __forceinline__ uint32_t place_of(long long slot) { return (uint32_t(slot) * 2654435769u) >> 21; }
@@ -112,9 +113,14 @@ __device__ __forceinline__ uint2 quantised(const uint4& v, float inv, bool all_f
 }
 
 // Magnitudes of 16-bit floats order as their bits do without the sign: the largest of eight, two to an instruction
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 __device__ __forceinline__ uint32_t largest_bits(const uint4& v) {
   const uint32_t m = 0x7fff7fffu;
-  return __vmaxu2(__vmaxu2(v.x & m, v.y & m), __vmaxu2(v.z & m, v.w & m));
+  return max2(max2(v.x & m, v.y & m), max2(v.z & m, v.w & m));
 }
 template <typename T>
 constexpr uint32_t first_not_finite() { return std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u; }
@@ -132,50 +138,67 @@ __device__ float largest_finite(const uint4& v) {
   return m;
 }
 
-// T: the packed rows' type; E4M3: what the cache holds (the same type otherwise); LANES: of a row.  The block's tokens of one side.
-template <typename T, bool E4M3, int LANES>
+// T: the packed rows' type; E4M3: what the cache holds (the same type otherwise); LANES: of a row; PIECES: of 16 bytes to a lane.  The block's tokens
+// of one side.  Two pieces a lane where rows are quantised and lie on 16 bytes: what is done once per lane (the row's place, its largest value,
+// its exponent) then serves 16 values, and 16 bytes are stored at once.
+template <typename T, bool E4M3, int LANES, int PIECES>
 __device__ __forceinline__ void write_rows(const Side& d, const Divide& by_heads, int heads, int n, long long t0, const long long* own, const int* lost,
                                            const long long* base) {
-  constexpr int GROUPS = THREADS / LANES;
+  constexpr int GROUPS = THREADS / LANES, AHEAD = ROWS_AHEAD / PIECES;
   const int group = threadIdx.x / LANES, part = threadIdx.x % LANES, rows = n * heads;
-  const uint8_t* x = d.x + t0 * d.x_tok + part * 16;
-  uint8_t* cache = d.cache + part * (E4M3 ? 8 : 16);
-  const bool exists = part < d.width;
+  const uint8_t* x = d.x + t0 * d.x_tok + part * PIECES * 16;
+  uint8_t* cache = d.cache + part * PIECES * (E4M3 ? 8 : 16);
+  const bool exists = part * PIECES < d.width;
   // whole rounds, so that the lanes of a warp meet in the shuffles
-  for (int r0 = group; r0 - group < rows; r0 += GROUPS * ROWS_AHEAD) {
-    uint4 v[ROWS_AHEAD];
-    int tok[ROWS_AHEAD], head[ROWS_AHEAD];
+  for (int r0 = group; r0 - group < rows; r0 += GROUPS * AHEAD) {
+    uint4 v[AHEAD][PIECES];
+    int tok[AHEAD], head[AHEAD];
 #pragma unroll
-    for (int u = 0; u < ROWS_AHEAD; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       const int r = r0 + u * GROUPS;
-      v[u] = make_uint4(0, 0, 0, 0);
       tok[u] = by_heads(r);
       head[u] = r - tok[u] * heads;
       if (r >= rows || own[tok[u]] < 0 || lost[tok[u]]) tok[u] = -1;
-      else if (exists) v[u] = __ldg(reinterpret_cast<const uint4*>(x + (long long)tok[u] * d.x_tok + (long long)head[u] * d.x_head));
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) v[u][i] = make_uint4(0, 0, 0, 0);
+      if (tok[u] >= 0 && exists) {
+        const uint4* src = reinterpret_cast<const uint4*>(x + (long long)tok[u] * d.x_tok + (long long)head[u] * d.x_head);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) v[u][i] = __ldg(src + i);
+      }
     }
 #pragma unroll
-    for (int u = 0; u < ROWS_AHEAD; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       uint8_t* row = cache + base[tok[u] < 0 ? 0 : tok[u]] + (long long)head[u] * d.c_head;
       if (!E4M3) {
-        if (tok[u] >= 0 && exists) *reinterpret_cast<uint4*>(row) = v[u];
+        if (tok[u] >= 0 && exists) *reinterpret_cast<uint4*>(row) = v[u][0];
         continue;
       }
-      uint32_t most = largest_bits(v[u]);
+      uint32_t most = largest_bits(v[u][0]);
+      if (PIECES == 2) most = max2(most, largest_bits(v[u][PIECES - 1]));
 #pragma unroll
-      for (int o = LANES >> 1; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+      for (int o = LANES >> 1; o > 0; o >>= 1) most = max2(most, __shfl_xor_sync(0xffffffffu, most, o));
       most = max(most & 0xffffu, most >> 16);
       const bool all_finite = most < first_not_finite<T>();
       float m = two<T>(most).x;
       if (!__all_sync(0xffffffffu, all_finite)) {             // the row's largest finite one
-        m = largest_finite<T>(v[u]);
+        m = largest_finite<T>(v[u][0]);
+        if (PIECES == 2) m = fmaxf(m, largest_finite<T>(v[u][PIECES - 1]));
 #pragma unroll
         for (int o = LANES >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       }
       if (tok[u] < 0) continue;
       const int e = exponent_byte(m);
-      // 2^(127 - e): a subnormal for e = 254 alone, which exponent_byte does not reach
-      if (exists) *reinterpret_cast<uint2*>(row) = quantised<T>(v[u], __uint_as_float((254u - e) << 23), all_finite);
+      if (exists) {
+        const float inv = __uint_as_float((254u - e) << 23);  // 2^(127 - e): a subnormal for e = 254 alone, which exponent_byte does not reach
+        const uint2 y = quantised<T>(v[u][0], inv, all_finite);
+        if (PIECES == 2) {
+          const uint2 z = quantised<T>(v[u][PIECES - 1], inv, all_finite);
+          *reinterpret_cast<uint4*>(row) = make_uint4(y.x, y.y, z.x, z.y);
+        } else {
+          *reinterpret_cast<uint2*>(row) = y;
+        }
+      }
       if (part == 0) d.scale[own[tok[u]] * heads + head[u]] = (uint8_t)e;
     }
   }
@@ -224,9 +247,10 @@ __global__ void __launch_bounds__(THREADS, 4) cache_write_kernel(const WriteArgs
   __syncthreads();
   for (int w = 0; w < a.sides; ++w) {
     const Side& d = a.side[w];
-    if (d.lanes == 8) write_rows<T, E4M3, 8>(d, a.by_heads, a.heads, n, t0, own, lost, base[w]);
-    else if (d.lanes == 16) write_rows<T, E4M3, 16>(d, a.by_heads, a.heads, n, t0, own, lost, base[w]);
-    else write_rows<T, E4M3, 32>(d, a.by_heads, a.heads, n, t0, own, lost, base[w]);
+    if (E4M3 && d.wide && d.width <= 16) write_rows<T, E4M3, 8, 2>(d, a.by_heads, a.heads, n, t0, own, lost, base[w]);
+    else if (d.lanes == 8) write_rows<T, E4M3, 8, 1>(d, a.by_heads, a.heads, n, t0, own, lost, base[w]);
+    else if (d.lanes == 16) write_rows<T, E4M3, 16, 1>(d, a.by_heads, a.heads, n, t0, own, lost, base[w]);
+    else write_rows<T, E4M3, 32, 1>(d, a.by_heads, a.heads, n, t0, own, lost, base[w]);
   }
 }
 
@@ -348,6 +372,7 @@ static Side side_of(const void* x, const long long* xs, void* cache, const long 
   d.c_head = int(cs[2] * esize);
   d.scale = (uint8_t*)scale;
   d.width = width / 8;
+  d.wide = esize == 1 && width % 16 == 0 && ((reinterpret_cast<uintptr_t>(cache) | d.c_page | d.c_tok | d.c_head) & 15) == 0;
   d.lanes = d.width <= 8 ? 8 : d.width <= 16 ? 16 : 32;
   return d;
 }
