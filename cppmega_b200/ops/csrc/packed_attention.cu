@@ -287,9 +287,10 @@ struct Masked { static constexpr bool value = true; };
 struct Whole { static constexpr bool value = false; };
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
-constexpr int THREADS = 320;                 // eight compute warps, one that issues products, one that loads
-constexpr int MMA_WARP = 8, TMA_WARP = 9;
-constexpr int FWD_THREADS = 352, FWD_TMA_WARP = 10;           // forward: an issuing warp for each query tile (8 and 9)
+// Eight compute warps, two that issue products, one that loads.  One issuing thread for all products of a block was the longest chain of the backward:
+// a wait that has nothing to wait for and eight products cost it 250 cycles beside the compute warps (dq 2110 cycles a 128 x 128 tile, ONEDQ with two).
+constexpr int THREADS = 352;
+constexpr int MMA_WARP = 8, TMA_WARP = 10;
 
 template <int D, int DV>
 struct Fwd {
@@ -306,7 +307,7 @@ struct Fwd {
 };
 
 template <bool HALF, int D, int DV>
-__global__ void __launch_bounds__(FWD_THREADS, 1)
+__global__ void __launch_bounds__(THREADS, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const Args a) {
   using F = Fwd<D, DV>;
@@ -340,7 +341,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     fence_mbar_init();
   }
   if (warp == MMA_WARP) { tmem_alloc(&sh->tmem_slot, 512); tmem_relinquish(); }
-  if (warp == FWD_TMA_WARP && lane == 0) {
+  if (warp == TMA_WARP && lane == 0) {
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -373,7 +374,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
   const int most = (max(n[0], n[1]) + 1) / 2;
 
-  if (warp == FWD_TMA_WARP) {
+  if (warp == TMA_WARP) {
     // ------------------------------ loads ------------------------------
     bool ok = true;
     auto load_q = [&](int t) {
@@ -750,49 +751,49 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
     }
   } else if (warp == MMA_WARP) {
+    // ------------------------------ S = Q K', each half as soon as its compute warps hold the one before ------------------------------
     if (elect_one()) {
-      constexpr uint32_t id_s = idesc(HALF, PART, false), id_q = idesc(HALF, D, true);
-      const uint64_t dK = base_k(smem_u32(sK)), dKt = base_mn(smem_u32(sK)), dV = base_k(smem_u32(sV));
-      Ring<F::K_SLOTS> rs, rq;
-      Ring<F::V_SLOTS> rv;
+      constexpr uint32_t id_s = idesc(HALF, PART, false);
+      const uint64_t dK = base_k(smem_u32(sK));
+      Ring<F::K_SLOTS> rk;
       bool ok = n == 0 || mbar_wait(&sh->rows_in, 0, abort_flag, a.err, ERR_WAIT_FULL);
-      auto scores = [&](int h) {             // half h of S = Q K'
-        const uint64_t d = dK + rs.at * (F::KS * SLAB >> 4) + h * (SLAB / 2 >> 4);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) umma_ta(tmem + h * 64, tmem + 384 + k * 8, d + step_k(k), id_s, k != 0);
-        umma_commit(&sh->s_full[h]);
-      };
-      auto weights = [&](int h) {            // half h of dP = dO V'
-        const uint64_t d = dV + rv.at * (F::VS * SLAB >> 4) + h * (SLAB / 2 >> 4);
-#pragma unroll
-        for (int k = 0; k < DV / 16; ++k) umma_ta(tmem + 128 + h * 64, tmem + 448 + k * 8, d + step_k(k), id_s, k != 0);
-        umma_commit(&sh->dp_full[h]);
-      };
-      for (int j = -1; j < n && ok; ++j) {
-        // S(j + 1) as soon as the compute warps hold S(j), dQ(j) when dS(j) is there, dP(j + 1) over the columns of dS(j)
-        if (j + 1 < n) {
-          ok = mbar_wait(&sh->k_full[rs.at], rs.round, abort_flag, a.err, ERR_WAIT_FULL);
-          for (int h = 0; h < 2 && ok; ++h) {
-            ok = j < 0 || mbar_wait(&sh->s_free[h], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
-            if (!ok) break;
-            tc_fence_after();
-            scores(h);
-          }
-          rs.next();
-        }
-        for (int h = 0; h < 2 && ok && j >= 0; ++h) {
-          ok = mbar_wait(&sh->ds_full[h], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+      for (int j = 0; j < n && ok; ++j) {
+        ok = mbar_wait(&sh->k_full[rk.at], rk.round, abort_flag, a.err, ERR_WAIT_FULL);
+        for (int h = 0; h < 2 && ok; ++h) {
+          ok = j == 0 || mbar_wait(&sh->s_free[h], (j - 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t d = dKt + rq.at * (F::KS * SLAB >> 4) + h * step_mn(4);
+          const uint64_t d = dK + rk.at * (F::KS * SLAB >> 4) + h * (SLAB / 2 >> 4);
 #pragma unroll
-          for (int k = 0; k < PART / 16; ++k) umma_ta(tmem + 256, tmem + 128 + h * 64 + k * 8, d + step_mn(k), id_q, (j | h | k) != 0);
-          umma_commit(&sh->dq_done[h]);
+          for (int k = 0; k < D / 16; ++k) umma_ta(tmem + h * 64, tmem + 384 + k * 8, d + step_k(k), id_s, k != 0);
+          umma_commit(&sh->s_full[h]);
         }
-        if (!ok) break;
+        rk.next();
+      }
+    }
+  } else if (warp == MMA_WARP + 1) {
+    // ------------------------------ dQ += dS K, then dP = dO V' of the next tile over the columns of dS ------------------------------
+    if (elect_one()) {
+      constexpr uint32_t id_s = idesc(HALF, PART, false), id_q = idesc(HALF, D, true);
+      const uint64_t dK = base_mn(smem_u32(sK)), dV = base_k(smem_u32(sV));
+      Ring<F::K_SLOTS> rk;
+      Ring<F::V_SLOTS> rv;
+      bool ok = n == 0 || mbar_wait(&sh->rows_in, 0, abort_flag, a.err, ERR_WAIT_FULL);
+      for (int j = -1; j < n && ok; ++j) {
         if (j >= 0) {
-          umma_commit(&sh->k_empty[rq.at]);
-          rq.next();
+          ok = mbar_wait(&sh->k_full[rk.at], rk.round, abort_flag, a.err, ERR_WAIT_FULL);
+          for (int h = 0; h < 2 && ok; ++h) {
+            ok = mbar_wait(&sh->ds_full[h], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t d = dK + rk.at * (F::KS * SLAB >> 4) + h * step_mn(4);
+#pragma unroll
+            for (int k = 0; k < PART / 16; ++k) umma_ta(tmem + 256, tmem + 128 + h * 64 + k * 8, d + step_mn(k), id_q, (j | h | k) != 0);
+            umma_commit(&sh->dq_done[h]);
+          }
+          if (!ok) break;
+          umma_commit(&sh->k_empty[rk.at]);
+          rk.next();
         }
         if (j + 1 < n) {
           ok = mbar_wait(&sh->v_full[rv.at], rv.round, abort_flag, a.err, ERR_WAIT_FULL);
@@ -800,7 +801,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             ok = j < 0 || mbar_wait(&sh->dq_done[h], j & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
             if (!ok) break;
             tc_fence_after();
-            weights(h);
+            const uint64_t d = dV + rv.at * (F::VS * SLAB >> 4) + h * (SLAB / 2 >> 4);
+#pragma unroll
+            for (int k = 0; k < DV / 16; ++k) umma_ta(tmem + 128 + h * 64, tmem + 448 + k * 8, d + step_k(k), id_s, k != 0);
+            umma_commit(&sh->dp_full[h]);
           }
           if (ok) umma_commit(&sh->v_empty[rv.at]);
           rv.next();
@@ -932,7 +936,7 @@ struct Dkv {
   static constexpr int KS = D / 64, VS = DV / 64, STAGES = 2;
   struct Shared {
     uint64_t kv_full, q_full[STAGES], stat_full[STAGES], q_empty[STAGES], tail;
-    uint64_t s_full, dp_full, p_full, ds_full, dv_done, dk_done, acc_done;
+    uint64_t s_full[2], dp_full[2], p_full[2], ds_full[2], dv_done[2], dk_done[2], acc_done;      // half of the query tile
     Unit unit;
     uint32_t tmem_slot;
     int abort_flag;
@@ -966,16 +970,18 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int s = 0; s < F::STAGES; ++s) {
       mbar_init(&sh->q_full[s], 1);
       mbar_init(&sh->stat_full[s], 1);
-      mbar_init(&sh->q_empty[s], 1);
+      mbar_init(&sh->q_empty[s], 2);
     }
     mbar_init(&sh->tail, 1);
-    mbar_init(&sh->s_full, 1);
-    mbar_init(&sh->dp_full, 1);
-    mbar_init(&sh->p_full, 8);
-    mbar_init(&sh->ds_full, 8);
-    mbar_init(&sh->dv_done, 1);
-    mbar_init(&sh->dk_done, 1);
-    mbar_init(&sh->acc_done, 1);
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(&sh->s_full[h], 1);
+      mbar_init(&sh->dp_full[h], 1);
+      mbar_init(&sh->p_full[h], 4);
+      mbar_init(&sh->ds_full[h], 4);
+      mbar_init(&sh->dv_done[h], 1);
+      mbar_init(&sh->dk_done[h], 1);
+    }
+    mbar_init(&sh->acc_done, 2);
     sh->abort_flag = 0;
     fence_mbar_init();
   }
@@ -1063,55 +1069,48 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (lane == 0) mbar_arrive(&sh->q_full[s]);
       }
     }
-  } else if (warp == MMA_WARP) {
+  } else if (warp >= MMA_WARP) {
+    // The first issuing warp: dV += P' dO, then S' = K Q' of the next query tile over the columns of P'; the second: dK += dS' Q, then dP' = V dO'
+    // over the columns of dS'.  Half by half, so that the scores of one half are multiplied while the other half is still being used.
     if (elect_one()) {
-      constexpr uint32_t id_s = idesc(HALF, TILE, false), id_v = idesc(HALF, DV, true), id_k = idesc(HALF, D, true);
-      const uint64_t dK = base_k(smem_u32(sK)), dV = base_k(smem_u32(sV)), dQ = base_k(smem_u32(sQ)), dQt = base_mn(smem_u32(sQ));
-      const uint64_t dG = dQ + (F::KS * SLAB >> 4), dGt = dQt + (F::KS * SLAB >> 4);
+      const bool second = warp > MMA_WARP;
+      constexpr uint32_t id_s = idesc(HALF, PART, false);
+      const uint32_t id_g = second ? idesc(HALF, D, true) : idesc(HALF, DV, true), tS = tmem + (second ? 128 : 0), tG = tmem + (second ? 384 : 256);
+      const uint32_t q = smem_u32(sQ), g = smem_u32(sQ + F::KS * SLAB);
+      const uint64_t dA = base_k(smem_u32(second ? sV : sK)), dB = base_k(second ? g : q), dG = base_mn(second ? q : g);
+      uint64_t *scored = second ? sh->dp_full : sh->s_full, *given = second ? sh->ds_full : sh->p_full, *used = second ? sh->dk_done : sh->dv_done;
+      const int steps = (second ? DV : D) / 16;
       Ring<F::STAGES> next, now;             // of the scores, of the gradients
       bool ok = n == 0 || mbar_wait(&sh->kv_full, 0, abort_flag, a.err, ERR_WAIT_FULL);
-      auto scores = [&](int i) {             // S' = K Q', over the columns of P' before
-        ok = mbar_wait(&sh->q_full[next.at], next.round, abort_flag, a.err, ERR_WAIT_FULL) &&
-             (i == 0 || mbar_wait(&sh->dv_done, (i - 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY));
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t d = dQ + next.at * (STAGE >> 4);
+      for (int i = -1; i < n && ok; ++i) {
+        if (i >= 0) {
+          const uint64_t d = dG + now.at * (STAGE >> 4);
+          for (int h = 0; h < 2 && ok; ++h) {
+            ok = mbar_wait(&given[h], i & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) umma_f16(tmem, dK + step_k(k), d + step_k(k), id_s, k != 0);
-        umma_commit(&sh->s_full);
-      };
-      auto weights = [&](int i) {            // dP' = V dO', over the columns of dS' before
-        ok = i == 0 || mbar_wait(&sh->dk_done, (i - 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t d = dG + next.at * (STAGE >> 4);
+            for (int k = 0; k < PART / 16; ++k) umma_ta(tG, tS + h * 64 + k * 8, d + h * step_mn(4) + step_mn(k), id_g, (i | h | k) != 0);
+            umma_commit(&used[h]);
+          }
+          if (!ok) break;
+          umma_commit(&sh->q_empty[now.at]);
+          now.next();
+        }
+        if (i + 1 < n) {
+          ok = mbar_wait(&sh->q_full[next.at], next.round, abort_flag, a.err, ERR_WAIT_FULL);
+          for (int h = 0; h < 2 && ok; ++h) {
+            ok = i < 0 || mbar_wait(&used[h], i & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t d = dB + next.at * (STAGE >> 4) + h * (SLAB / 2 >> 4);
 #pragma unroll
-        for (int k = 0; k < DV / 16; ++k) umma_f16(tmem + 128, dV + step_k(k), d + step_k(k), id_s, k != 0);
-        umma_commit(&sh->dp_full);
-        next.next();
-      };
-      if (ok && n > 0) {
-        scores(0);
-        if (ok) weights(0);
-      }
-      for (int i = 0; i < n && ok; ++i) {
-        ok = mbar_wait(&sh->p_full, i & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t g = dGt + now.at * (STAGE >> 4), q = dQt + now.at * (STAGE >> 4);
-#pragma unroll
-        for (int k = 0; k < TILE / 16; ++k) umma_ta(tmem + 256, tmem + (k >> 2) * 64 + (k & 3) * 8, g + step_mn(k), id_v, (i | k) != 0);
-        umma_commit(&sh->dv_done);
-        if (i + 1 < n) scores(i + 1);
-        ok = ok && mbar_wait(&sh->ds_full, i & 1, abort_flag, a.err, ERR_WAIT_TMEM_EMPTY);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < TILE / 16; ++k) umma_ta(tmem + 384, tmem + 128 + (k >> 2) * 64 + (k & 3) * 8, q + step_mn(k), id_k, (i | k) != 0);
-        umma_commit(&sh->dk_done);
-        umma_commit(&sh->q_empty[now.at]);
-        now.next();
-        if (i + 1 < n) weights(i + 1);
+            for (int k = 0; k < D / 16; ++k)
+              if (k < steps) umma_f16(tS + h * 64, dA + step_k(k), d + step_k(k), id_s, k != 0);
+            umma_commit(&scored[h]);
+          }
+          next.next();
+        }
       }
       if (ok && n > 0) umma_commit(&sh->acc_done);
     }
@@ -1125,7 +1124,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       // columns [from, to) see this key: queries at or behind it, of this sequence
       const int from = max(0, key0 + r - off - first) * a.hb - half * 64, to = min(a.tok, L - first) * a.hb - half * 64;
       if (!warp_wait(&sh->stat_full[s], (i / F::STAGES) & 1, abort_flag, a.err, ERR_WAIT_FULL)) return false;
-      if (!warp_wait(&sh->s_full, i & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
+      if (!warp_wait(&sh->s_full[half], i & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
       tc_fence_after();
       float p[64];
       uint32_t w[32];
@@ -1157,8 +1156,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->p_full);
-      if (!warp_wait(&sh->dp_full, i & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
+      if (lane == 0) mbar_arrive(&sh->p_full[half]);
+      if (!warp_wait(&sh->dp_full[half], i & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -1186,7 +1185,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->ds_full);
+      if (lane == 0) mbar_arrive(&sh->ds_full[half]);
       return true;
     };
     bool ok = true;
@@ -1302,7 +1301,7 @@ int forward(const Inputs& in, Args a, cudaStream_t stream) {
   const long long units = units_of(a.T, a.n, 2 * a.tok), grid = units * a.kv_heads * a.chunks;
   if (grid > 0x7fffffffLL) return -10;
   a.units = (int)units;
-  packed_fwd_kernel<HALF, D, DV><<<(unsigned)grid, FWD_THREADS, Fwd<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], a);
+  packed_fwd_kernel<HALF, D, DV><<<(unsigned)grid, THREADS, Fwd<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], a);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
