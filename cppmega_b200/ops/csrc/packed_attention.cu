@@ -29,9 +29,12 @@
 // whatever was ready first spent more time on polling than the products took (forward 2100 cycles a 128 x 128 tile).
 // Query tiles of the key gradients run from the last one down: blocks of one sequence then read the same rows at the same time, out of L2.
 //
-// Roundings to 16 bits: P and dS, as operands of their products.  delta takes o before its rounding (the forward keeps what that takes away,
-// in 16 bits more): with the rounded o, an error of 2^-9 of |do||o| is added to every ds of a row with one sign, and dq and dk were off by 4.4e-3
-// of their norms instead of 2.4e-3.  Maxima, sums, scores, deltas and all accumulators are fp32.  fp16's range
+// Roundings to 16 bits: P and dS, as operands of their products.  o is divided by the sum of the weights as rounded, so that what a rounding
+// adds to one weight moves o only by that weight's distance from it; the largest weight, which is not 1 while the maximum that it is taken
+// against lags, otherwise moves a row that settles on one key by 2^-9 of itself (6 % of the forward's time).  delta takes o before its rounding
+// (the forward keeps what that takes away, in 16 bits more).  Both because an error of o is added to every ds of a row with one sign: dq and
+// dk of rows that settle on few keys are off by 2.45e-3 of their norms, where the roundings of dS and of the result itself make 2.4e-3;
+// 3.0e-3 with the sum of unrounded weights, 4.0e-3 with the rounded o too.  Maxima, sums, scores, deltas and all accumulators are fp32.  fp16's range
 // is too short for dS of any size: it is scaled by a power of two, from the row's largest |do| for dq, from the call's for dk.
 #include <cuda_fp16.h>
 
@@ -288,7 +291,7 @@ struct Whole { static constexpr bool value = false; };
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
 // Eight compute warps, two that issue products, one that loads.  One issuing thread for all products of a block was the longest chain of the backward:
-// a wait that has nothing to wait for and eight products cost it 250 cycles beside the compute warps (dq 2110 cycles a 128 x 128 tile, ONEDQ with two).
+// a wait that has nothing to wait for and eight products cost it 250 cycles beside the compute warps (dq 2110 cycles a 128 x 128 tile, 1800 with two).
 constexpr int THREADS = 352;
 constexpr int MMA_WARP = 8, TMA_WARP = 10;
 
@@ -473,7 +476,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int last = mine ? off + pos : -1;                   // last key it sees
     const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tO = tmem + 256 + t * DV + lane_addr;
-    float m_ref = -INFINITY, l = 0.f;
+    float m_ref = -INFINITY, l = 0.f, l_taken = 0.f;          // sums of the weights, and of the weights as rounded
     auto part = [&](int j, auto where) {
       constexpr bool MASK = decltype(where)::value;
       const int lim = last - j * PART;                        // columns up to lim are seen
@@ -497,6 +500,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         alpha = ex2(m_ref - m_new);
         m_ref = m_new;
         l *= alpha;
+        l_taken *= alpha;
       }
       if (__any_sync(0xffffffffu, alpha != 1.f) && j > 0) {   // O of all parts before this one
         if (!warp_wait(&sh->pv_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
@@ -512,7 +516,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
       const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // nothing seen so far
-      Pair sum[2] = {pr(0.f), pr(0.f)};
+      Pair sum[2] = {pr(0.f), pr(0.f)}, taken[2] = {pr(0.f), pr(0.f)};
       uint32_t p[32];
       auto quarter = [&](const uint32_t (&sc)[32], int col0, int at) {
 #pragma unroll
@@ -525,12 +529,15 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           sum[e & 1] = sum[e & 1] + pr(x, y);
           p[at + e] = pair<HALF>(x, y);
+          const float2 w = unpair<HALF>(p[at + e]);
+          taken[e & 1] = taken[e & 1] + pr(w.x, w.y);
         }
       };
       quarter(s0, 0, 0);
       quarter(s1, 32, 16);
       tmem_st(tS, p);
       l += pr_sum(sum[0] + sum[1]);
+      l_taken += pr_sum(taken[0] + taken[1]);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -544,7 +551,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (ok && count > 0) ok = warp_wait(&sh->pv_done[t][(count - 1) & 1], ((count - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
     if (ok) {
       tc_fence_after();
-      const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;               // a NaN stays
+      const float inv = l_taken > 0.f ? 1.f / l_taken : l_taken == 0.f ? 0.f : l_taken;            // a NaN stays
       const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
       const float f = last >= 0 ? inv : 0.f;
       uint8_t* stage = sQ + t * F::KS * SLAB;                 // Q_t has been used
@@ -576,7 +583,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (c & 1) {
             const int begin = (c - 1) * 32;
             if (pass == 0) send_rows(stage, (warp & 3) * 32, begin, a.vdim, lane, places_at, reinterpret_cast<uint16_t*>(a.out) + first);
-            if (a.out2 && pass == PASSES - 1) 
+            if (a.out2 && pass == PASSES - 1)
               send_rows(stage + (PASSES == 1 ? SLAB : 0), (warp & 3) * 32, begin, a.vdim, lane, places_at, reinterpret_cast<uint16_t*>(a.out2) + first);
           }
         }
@@ -593,7 +600,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 // ---- backward: delta -----------------------------------------------------------------------------------------------------
 // delta[i] = do[i] . o[i] before its rounding, in fp16 also the row's largest |do| and the call's.  DV / 8 lanes a row, four rows of a lane on their way
 // at once: three reads of a row's width at the memory's rate.  Inside the dq kernel, whose blocks have an SM to themselves, nothing would
-// run meanwhile (9000 cycles a block, 120 us at 16384 x 32 rows of 128; here 65).
+// run meanwhile (9000 cycles a block, 120 us at 16384 x 32 rows of 128; here 71).
 constexpr int DELTA_THREADS = 256, DELTA_AHEAD = 4;
 
 template <bool HALF, int LANES>

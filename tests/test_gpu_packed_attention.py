@@ -2,7 +2,7 @@
 
 Tolerances from the exact values, with u half a step of the type (2^-8 in bf16, 2^-11 in fp16) and e the error of a weight's exponent, twice the
 error of a score (its fp32 sum over D products, D 2^-23 of their magnitudes in any order, and roundings of scale and maximum): a weight p is off
-by p (u + e); o by |p||v| (u + e) and its own rounding; delta and dP by fp32 sums over the value columns of do, v and o as rounded; ds by
+by p (u + e); o, divided by the sum of the weights as rounded, by sum p |v - o| (u + e) <= (|p||v| + |o|) (u + e) and its own rounding; delta and dP by fp32 sums over the value columns of do, v and o as rounded; ds by
 its rounding u and by the errors of p and of dP - delta; a gradient by its operands' errors, its fp32 sum and its own rounding.  In fp16 what is
 below the range is lost: 2^-25 of a weight of up to 2^8, and of ds scaled so that |do| is at most 2^-4.
 """
@@ -64,7 +64,7 @@ def _compare(q, k, v, ends, ends_k, scale, o, go=None, grads=None):
             lost = 2.0 ** -17 * p.amax(1, keepdim=True) * (p > 0) if fp16 else 0.0
             ep = p * (u + e) + lost
             out, eo = p @ vh, ep @ vh.abs()
-            _check(o[a:b, h], out, eo * (1 + u) + u * out.abs() + tiny, "o")
+            _check(o[a:b, h], out, (eo + ep.sum(1, keepdim=True) * out.abs()) * (1 + u) + u * out.abs() + tiny, "o")
             if go is None:
                 continue
             g = go[a:b, h].double()
@@ -129,6 +129,27 @@ WIDTHS = [(128, 128), (128, 64), (64, 64), (64, 128), (96, 80), (8, 16)]
 @pytest.mark.parametrize("lens", [[1], [128], [127, 129], [5, 0, 300, 64, 1, 0], [256, 255, 257], [700, 33]])
 def test_one_head(lens, D, V, dtype):
     _run(lens, 1, 1, D, V, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,V", [(128, 128), (64, 64)])
+def test_rows_that_settle_on_few_keys(D, V, dtype):
+    """o = sum p (1 + d) v / sum p (1 + d) with |d| <= u + e is off by at most sum p |v - o| (u + e) / (1 - u - e), and its rounding: nearly nothing
+    but the rounding where one weight is nearly all of a row, although that weight is no power of two while the maximum lags."""
+    L, u = 400, HALF_STEP[dtype]
+    q, k, v = _randn(L, 1, D, dtype=dtype, std=1.5), _randn(L, 1, D, dtype=dtype, seed=1), _randn(L, 1, V, dtype=dtype, seed=2)
+    k[70::100] *= 4
+    o = F_.packed_attention(q, k, v, _i32([0, L]), D ** -0.5)[:, 0].double()
+    qh, kh, vh = q[:, 0].double(), k[:, 0].double(), v[:, 0].double()
+    hidden = torch.ones(L, L, dtype=torch.bool, device="cuda").triu(1)
+    p = torch.softmax((qh @ kh.T * D ** -0.5).masked_fill(hidden, -math.inf), 1)
+    assert (p.amax(1) > 0.99).sum() > 10
+    mags = (qh.abs() @ kh.abs().T * D ** -0.5).masked_fill(hidden, 0.0)
+    e = 2 * (((D + 8) * 2.0 ** -23) * mags).amax(1, keepdim=True) + 2.0 ** -19 + L * 2.0 ** -23
+    out = p @ vh
+    spread = (p[:, :, None] * (vh[None] - out[:, None]).abs()).sum(1)
+    lost = 2.0 ** -17 * p.amax(1, keepdim=True) * vh.abs().sum(0, keepdim=True) if dtype == torch.float16 else 0.0
+    _check(o, out, spread * (u + e) / (1 - u - e) + lost + u * out.abs() * (1 + u) + 2.0 ** -24 * L * (p @ vh.abs()), "o")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
