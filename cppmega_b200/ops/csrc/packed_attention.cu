@@ -31,7 +31,7 @@
 //
 // Roundings to 16 bits: P and dS, as operands of their products.  o is divided by the sum of the weights as rounded, so that what a rounding
 // adds to one weight moves o only by that weight's distance from it; the largest weight, which is not 1 while the maximum that it is taken
-// against lags, otherwise moves a row that settles on one key by 2^-9 of itself (6 % of the forward's time).  delta takes o before its rounding
+// against lags, otherwise moves a row that settles on one key by 2^-9 of itself (8 % of the forward's time).  delta takes o before its rounding
 // (the forward keeps what that takes away, in 16 bits more).  Both because an error of o is added to every ds of a row with one sign: dq and
 // dk of rows that settle on few keys are off by 2.45e-3 of their norms, where the roundings of dS and of the result itself make 2.4e-3;
 // 3.0e-3 with the sum of unrounded weights, 4.0e-3 with the rounded o too.  Maxima, sums, scores, deltas and all accumulators are fp32.  fp16's range

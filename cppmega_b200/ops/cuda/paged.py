@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import cuda as _cu
 from .. import functional as F_
@@ -116,6 +117,7 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout) -> bool
     if rc:
         _failed("cm_cache_write", rc)
     F_.count_launch("cache_write")
+    increment_version([t for t in (k_cache, v_cache, k_scale, v_scale) if t is not None])        # whoever saved them for a gradient is told
     return True
 
 
@@ -174,7 +176,7 @@ def _plan_attention(q, k_cache, v_cache, table, lens, k_scale, v_scale):
 def paged_attention(q, k_cache, v_cache, table, lens, scale, k_scale, v_scale, layout):
     """None where the kernels do not apply."""
     plan = planned(layout, lambda: _plan_attention(q, k_cache, v_cache, table, lens, k_scale, v_scale))
-    if (not plan or isinstance(scale, torch.Tensor) or not _bare(q, k_cache, v_cache, table, lens, k_scale, v_scale)
+    if (not plan or isinstance(scale, torch.Tensor) or not abs(scale) < 2.0 ** 64 or not _bare(q, k_cache, v_cache, table, lens, k_scale, v_scale)
             or (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad))):
         return None
     qp, kp, vp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()

@@ -491,7 +491,8 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, cu_seqlens_k=None):
 
     bf16 and fp16 with ``D`` and ``Dv`` multiples of 8 up to 128 run on the kernels, in training with their gradients (first
     derivatives; the same call gives the same bits); strided tensors are read in place where rows lie on 16 bytes.
-    Anything else, forward mode and function transforms run the definition, ``reference.packed_attention``.  No call waits for the device: ends
+    Anything else, forward mode and function transforms run the definition, ``reference.packed_attention``.  A CUDA graph takes forward and
+    backward together, while no eager graph of the same leaves is alive (autograd would add to those on the eager stream).  No call waits for the device: ends
     that fall or run over the buffer are reported by ``ops.cuda.check_errors``."""
     layout = layout_of("packed_attention", q, k, v, cu_seqlens, cu_seqlens_k)
     if layout not in _CHECKED:
@@ -533,17 +534,19 @@ def _check_write(k, v, k_cache, v_cache, slots, k_scale, v_scale) -> None:
     if (v is None) != (v_cache is None):
         raise ValueError("cache_write: values and their cache come together")
     _check_cache("cache_write", k_cache, v_cache, k_scale, v_scale)
+    if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"cache_write: slots {slots.dtype} {tuple(slots.shape)}")
     for x, cache in ((k, k_cache), (v, v_cache)):
         if x is None:
             continue
+        if any(n > 1 and s == 0 for n, s in zip(cache.shape, cache.stride())):
+            raise ValueError(f"cache_write: the rows of a cache are written once each, those of {tuple(cache.shape)} with strides {cache.stride()} overlap")
         if x.dim() != 3 or x.shape[0] != slots.shape[0] or x.shape[1:] != cache.shape[2:]:
             raise ValueError(f"cache_write: rows {tuple(x.shape)} and slots {tuple(slots.shape)} for a cache of {tuple(cache.shape)}")
         if x.dtype != cache.dtype and cache.dtype != torch.float8_e4m3fn:
             raise ValueError(f"cache_write: rows of {x.dtype} into a cache of {cache.dtype}")
     if v is not None and v.dtype != k.dtype:
         raise ValueError(f"cache_write: k {k.dtype}, v {v.dtype}")
-    if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"cache_write: slots {slots.dtype} {tuple(slots.shape)}")
     _same_device("cache_write", k, v, k_cache, slots)
 
 

@@ -399,7 +399,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ends_k = _ends("packed_attention", cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, k.shape[0])
     group = q.shape[1] // k.shape[1] if k.shape[1] else 1
     outs = []
-    for a, b, c, d in zip(ends, ends[1:], ends_k, ends_k[1:]):
+    for a, b, c, d in zip([0, *ends], ends, [0, *ends_k], ends_k):           # from an empty one on: no sequences give gradients of zeros
         qs = q[a:b].float().transpose(0, 1)
         ks, vs = (t[c:d].float().repeat_interleave(group, 1).transpose(0, 1) for t in (k, v))
         last = torch.arange(b - a, device=q.device)[:, None] + (d - c) - (b - a)
@@ -507,7 +507,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, scale: float, k_
     table = block_table.long()[:, pos // page]
     k, v = (_cache_rows(c, s, table, (pos % page).expand_as(table)).transpose(1, 2) for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
     seen = ((pos < seq_lens[:, None]) & (table >= 0) & (table < pages))[:, None, :, None]
-    scores = q.float().view(B, Hk, Hq // Hk if Hk else 1, -1) @ torch.where(seen, k, torch.zeros_like(k)).transpose(2, 3) * scale
+    scores = q.float().view(B, Hk, Hq // Hk if Hk else 1, q.shape[2]) @ torch.where(seen, k, torch.zeros_like(k)).transpose(2, 3) * scale
     p = _softmax_or_nothing(torch.where(seen.transpose(2, 3), scores, -math.inf))
     return (p @ torch.where(seen, v, torch.zeros_like(v))).reshape(B, Hq, v.shape[-1]).to(q.dtype)
 

@@ -396,3 +396,59 @@ def test_a_prompt_continued_from_a_cache_and_then_generated():
         at = torch.tensor([ends[0] + n - 1, ends[1] + n - 1, ends[2] + n - 1], device="cuda")
         one = F_.paged_attention(q[at], kc, vc, table, _i32([n, n, n]), 0.125).float()
         assert ((one - want[at]).abs() <= 4 * 2.0 ** -8 * size).all()
+
+
+def test_calls_of_nothing():
+    for T, n in ((3, 0), (200, 0), (0, 0)):
+        leaves = [_randn(T, 2, 64, seed=s).requires_grad_() for s in range(3)]
+        o = F_.packed_attention(*leaves, _i32([0] * (n + 1)), 1.0)
+        assert o.shape == (T, 2, 64) and (o == 0).all()
+        assert all((g == 0).all() for g in torch.autograd.grad(o, leaves, torch.ones_like(o)))
+    q, none = _randn(3, 2, 64).requires_grad_(), _randn(0, 2, 64)
+    o = F_.packed_attention(q, none, none, _i32([0, 3]), 1.0, _i32([0, 0]))
+    assert (o == 0).all()
+    from cppmega_b200.ops import cuda as cu_
+    cu_.check_errors()
+
+
+def test_tensors_behind_32_bits():
+    """More than 2^31 elements of q, o and their gradients: the last sequences against the same ones by themselves, bit for bit."""
+    T, H, D = 131200, 128, 128
+    assert T * H * D > 2 ** 31
+    ends = [*range(0, T - 200, 1000), T - 150, T - 20, T]
+    q, go = torch.empty(T, H, D, dtype=torch.bfloat16, device="cuda"), torch.empty(T, H, D, dtype=torch.bfloat16, device="cuda")
+    for t, seed in ((q, 1), (go, 2)):
+        t.normal_(generator=torch.Generator(device="cuda").manual_seed(seed))
+    k, v = _randn(T, 4, D, seed=3), _randn(T, 4, D, seed=4)
+    at = ends[-4]
+    few = [e - at for e in ends[-4:]]
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = F_.packed_attention(*leaves, _i32(ends), 0.09)
+    got = [o.detach()[at:], *[g[at:] for g in torch.autograd.grad(o, leaves, go)]]
+    del o
+    leaves = [t.detach()[at:].requires_grad_() for t in leaves]
+    o = F_.packed_attention(*leaves, _i32(few), 0.09)
+    assert all(torch.equal(a, b) for a, b in zip(got, [o.detach(), *torch.autograd.grad(o, leaves, go[at:])]))
+
+
+def test_two_calls_at_once():
+    """Forward and backward on two streams at the same time, each with its own data, leave each other alone."""
+    cu = _i32([0, 700, 1500])
+    data = [[_randn(1500, n, 64, dtype=torch.float16, seed=10 * i + s).requires_grad_() for s, n in ((0, 8), (1, 4), (2, 4))] for i in range(2)]
+    go = [_randn(1500, 8, 64, dtype=torch.float16, std=10.0 ** (-2 * i), seed=77) for i in range(2)]
+
+    def once(i):
+        o = F_.packed_attention(*data[i], cu, 0.125)
+        return [o.detach(), *torch.autograd.grad(o, data[i], go[i])]
+
+    want = [once(0), once(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, once(i)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i, x in got for a, b in zip(x, want[i]))

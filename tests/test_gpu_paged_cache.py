@@ -330,6 +330,67 @@ def test_a_step_of_generation_captured_and_replayed():
     assert int(lens.max()) == 70 <= most
 
 
+def test_calls_of_nothing():
+    for store in (torch.bfloat16, E4M3):
+        (kc, ks), (vc, vs) = _blank(3, 16, 2, 64, store), _blank(3, 16, 2, 64, store)
+        none = torch.zeros(0, 3, dtype=torch.int32, device="cuda")
+        F_.cache_write(_randn(0, 2, 64), _randn(0, 2, 64), kc, vc, torch.zeros(0, dtype=torch.int64, device="cuda"), ks, vs)
+        assert F_.cache_read(kc, vc, none, _i32([0]), 0, ks, vs)[0].shape == (0, 2, 64)
+        assert all((t == 0).all() for t in F_.cache_read(kc, vc, none, _i32([0]), 70, ks, vs))
+        assert F_.paged_attention(_randn(0, 4, 64), kc, vc, none, _i32([]), 0.1, ks, vs).shape == (0, 4, 64)
+        assert (F_.paged_attention(_randn(2, 4, 64), kc, vc, none.new_zeros(2, 0), _i32([0, 0]), 0.1, ks, vs) == 0).all()
+        assert (F_.paged_attention(_randn(2, 4, 64), kc, vc, none.new_zeros(2, 3), _i32([0, 0]), 0.1, ks, vs) == 0).all()
+    from cppmega_b200.ops import cuda as cu
+    cu.check_errors()
+
+
+def test_sequences_that_share_pages():
+    """One table row for several sequences (a common beginning), broadcast, at different lengths."""
+    kc, vc, table, _, _ = _filled([300], 16, 2, 128, 128, torch.bfloat16, torch.bfloat16)
+    lens = [300, 17, 300, 16]
+    _check(_randn(4, 8, 128, seed=9), kc, vc, table.expand(4, -1), lens, 0.09)
+    k, v = F_.cache_read(kc, vc, table.expand(2, -1), _i32([0, 300, 317]), 317)
+    assert torch.equal(k[300:], k[:17]) and torch.equal(v[300:], v[:17])
+
+
+def test_two_calls_at_once():
+    lens = [3000, 1, 700]
+    kc, vc, table, ks, vs = _filled(lens, 16, 4, 128, 128, E4M3, torch.bfloat16)
+    qs, n = [_randn(3, 32, 128, seed=s) for s in (5, 6)], _i32(lens)
+    want = [F_.paged_attention(q, kc, vc, table, n, 0.1, ks, vs) for q in qs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(30):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, F_.paged_attention(qs[i], kc, vc, table, n, 0.1, ks, vs)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i, o in got)
+
+
+def test_a_cache_that_was_saved_for_a_gradient_and_written():
+    kc, vc, table, _, _ = _filled([20], 16, 2, 64, 64, torch.bfloat16, torch.bfloat16)
+    q = _randn(1, 4, 64).requires_grad_()
+    o = F_.paged_attention(q, kc, vc, table, _i32([20]), 0.1)
+    before = kc._version
+    F_.cache_write(_randn(1, 2, 64), _randn(1, 2, 64), kc, vc, torch.tensor([3], device="cuda"))
+    assert kc._version == before + 1 and o.isfinite().all()
+    with torch.inference_mode():
+        a, b = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+        F_.cache_write(_randn(1, 2, 64), _randn(1, 2, 64), a, b, torch.tensor([3], device="cuda"))
+        assert a.abs().sum() > 0
+
+
+@pytest.mark.parametrize("scale", [math.inf, math.nan])
+def test_scales_that_are_not_finite_run_the_definition(scale):
+    kc, vc, table, _, _ = _filled([20], 16, 2, 64, 64, torch.bfloat16, torch.bfloat16)
+    F_.reset_counters()
+    assert F_.paged_attention(_randn(1, 4, 64), kc, vc, table, _i32([20]), scale).isnan().any()
+    assert F_.fallback_counts() == {"paged_attention(shape/dtype)": 1}
+
+
 def test_paged_attention_for_a_gradient_is_the_definition():
     lens = [20, 3]
     kc, vc, table, _, _ = _filled(lens, 16, 2, 64, 64, torch.bfloat16, torch.bfloat16)

@@ -160,7 +160,7 @@ def test_packed_attention_refuses(change):
     dict(k=torch.zeros(3, 2, 16)), dict(k=torch.zeros(3, 1, 8)), dict(k=torch.zeros(3, 2, 8, dtype=torch.float16)), dict(v=None),
     dict(slots=torch.tensor([0, 1])), dict(slots=torch.tensor([0.0, 1, 2])), dict(slots=torch.tensor([0, 1, 8])), dict(ks=torch.zeros(2, 4, 2, dtype=torch.uint8)),
     dict(kc=torch.zeros(2, 4, 2, 8, dtype=torch.uint8).view(E4M3)), dict(vc=torch.zeros(2, 5, 2, 8)), dict(kc=torch.zeros(8, 2, 8)),
-    dict(kc=torch.zeros(2, 4, 2, 8, requires_grad=True)),
+    dict(kc=torch.zeros(2, 4, 2, 8, requires_grad=True)), dict(kc=torch.zeros(1, 4, 2, 8).expand(2, 4, 2, 8)), dict(slots=torch.tensor(3)),
 ])
 def test_cache_write_refuses(change):
     args = dict(k=torch.ones(3, 2, 8), v=torch.ones(3, 2, 8), kc=torch.zeros(2, 4, 2, 8), vc=torch.zeros(2, 4, 2, 8), slots=torch.tensor([0, 5, 7]),
@@ -194,3 +194,27 @@ def test_paged_attention_refuses(change):
     args.update(change)
     with pytest.raises(ValueError):
         F_.paged_attention(args["q"], args["kc"], args["vc"], args["table"], args["lens"], 1.0)
+
+
+def test_calls_of_nothing():
+    """No sequences, no tokens, no columns, no rows to read."""
+    for T, Tk in ((3, 3), (0, 0)):
+        o = F_.packed_attention(torch.ones(T, 2, 8), torch.ones(Tk, 2, 8), torch.ones(Tk, 2, 8), _i32(0), 1.0)
+        assert o.shape == (T, 2, 8) and (o == 0).all()
+        leaves = [torch.ones(n, 2, 8, requires_grad=True) for n in (T, Tk, Tk)]
+        assert all((g == 0).all() for g in torch.autograd.grad(F_.packed_attention(*leaves, _i32(0), 1.0).sum(), leaves))
+    assert (F_.packed_attention(torch.ones(3, 2, 8), torch.ones(0, 2, 8), torch.ones(0, 2, 8), _i32(0, 3), 1.0, _i32(0, 0)) == 0).all()
+    kc, vc = torch.ones(2, 4, 2, 8), torch.ones(2, 4, 2, 8)
+    F_.cache_write(torch.zeros(0, 2, 8), torch.zeros(0, 2, 8), kc, vc, torch.zeros(0, dtype=torch.int64))
+    assert (kc == 1).all() and (vc == 1).all()
+    none = torch.zeros(0, 3, dtype=torch.int32)
+    assert F_.cache_read(kc, vc, none, _i32(0), 0)[0].shape == (0, 2, 8) and (F_.cache_read(kc, vc, none, _i32(0), 5)[1] == 0).all()
+    assert F_.paged_attention(torch.ones(0, 4, 8), kc, vc, none, _i32(), 1.0).shape == (0, 4, 8)
+    assert (F_.paged_attention(torch.ones(2, 4, 8), kc, vc, none.new_zeros(2, 0), _i32(0, 0), 1.0) == 0).all()
+
+
+def test_a_cache_that_was_saved_for_a_gradient_and_written():
+    kc, vc, q = torch.ones(2, 4, 2, 8), torch.ones(2, 4, 2, 8), torch.ones(1, 4, 8, requires_grad=True)
+    before = kc._version, vc._version
+    F_.cache_write(torch.zeros(1, 2, 8), torch.zeros(1, 2, 8), kc, vc, torch.tensor([5]))
+    assert kc._version > before[0] and vc._version > before[1]
