@@ -20,8 +20,10 @@
 // E4M3 becomes fp16 in one conversion per two values, exactly; the query is scaled to fp16's range by a power of two per head, the key's power
 // goes into the score, and the value's power into the exponent of its weight, whose reference is a maximum of its own: weights never leave
 // fp16's range, whatever the powers are.
-// Weights are rounded to the type of the products (bf16 or fp16: half a step of the result's own type, averaged over the keys);
-// scores, maxima, sums and accumulators are fp32.
+// Weights are rounded to the type of the products (bf16 or fp16: half a step of the result's own type, averaged over the keys).  Over a 16-bit cache
+// the sum that divides the result is that of the rounded weights: a row that settles on few keys does not take their rounding into its result
+// (1000 keys, one in fifty three times as large: off by 1.7e-3 of its norm, 2.3e-3 with the sum of the others).  Over an E4M3 cache the weights that are rounded have the
+// values' powers in them, and the sum is that of the unrounded ones.  Scores, maxima, sums and accumulators are fp32.
 //
 // The reference value of a head's softmax follows its maximum only when that has grown by 2^8, so that accumulators are rarely rescaled.
 #include <cuda_fp16.h>
@@ -52,7 +54,7 @@ struct Args {
   float* part;                               // pieces of [rows][DV + 4]: weights' sum, maximum, two unused, accumulators
   int sequences, kv_heads, group, columns, pages, page, dim, vdim;
   int runs, tiles, rows;                     // runs of the sequence of steps; head tiles of a group (1, 2, 4, 8); rows of a piece
-  int aligned;                               // a step lies inside one page
+  int aligned;                               // a step lies inside one page, and its keys within 2^31 bytes
   int side, chunks;                          // key heads of a run, and how often a sequence is gone through for all of them
   float scale_log2;
   int* err;
@@ -102,6 +104,8 @@ __device__ __forceinline__ float2 unpair(uint32_t v) {
   if (BF16) return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
   return __half22float2(*reinterpret_cast<__half2*>(&v));
 }
+template <bool BF16>
+__device__ __forceinline__ float rounded(float x) { return unpair<BF16>(pair<BF16>(x, 0.f)).x; }
 // two E4M3 bytes (the lower or the upper half of a word) -> two fp16
 __device__ __forceinline__ uint32_t expand_lo(uint32_t w) {
   uint32_t r;
@@ -259,7 +263,7 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
   const int kc = lane % KC, kr = lane / KC, vc = lane % VC, vr = lane / VC;
   const bool k_exists = kc * 16 < a.dim * (E4M3 ? 1 : 2), v_exists = vc * 16 < a.vdim * (E4M3 ? 1 : 2);
   // where the copies go: K by (eight keys, piece of four lanes), V by (row of a lane's fragment, piece of eight lanes)
-  const uint8_t *k_lane = a.k + kr * a.k_tok + kc * 16, *v_lane = a.v + vr * a.v_tok + vc * 16;
+  const uint8_t *k_lane = a.k + kr * a.k_tok + kc * 16, *v_lane = a.v + vr * a.v_tok + vc * 16;          // aligned: within 2^31 bytes
   const uint32_t k_dst = (kc >> 2) * 512 + ((kr * 4 + (kc & 3)) ^ ((kc >> 2 & 1) * 4)) * 16;
   uint32_t v_dst[VC / 2];
 #pragma unroll
@@ -590,7 +594,11 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const float ref = m[x][c] == -INFINITY ? 0.f : m[x][c], refv = mv[x][c] == -INFINITY ? 0.f : mv[x][c];
-        const float u = ex2(s[x][c] - ref), y = ex2(s[x][2 + c] - ref);
+        float u = ex2(s[x][c] - ref), y = ex2(s[x][2 + c] - ref);
+        if (!E4M3) {                                          // the sum of what V is multiplied by
+          u = rounded<MB>(u);
+          y = rounded<MB>(y);
+        }
         l[x][c] += u + y;
         w[c] = E4M3 ? ex2(s[x][c] + vlog[0] - refv) : u;
         w[2 + c] = E4M3 ? ex2(s[x][2 + c] + vlog[1] - refv) : y;
@@ -854,7 +862,7 @@ extern "C" int cm_paged_attention(const void* q, const void* k, const void* v, c
   a.runs = s.runs;
   a.side = s.side;
   a.chunks = s.chunks;
-  a.aligned = page % KEYS == 0;
+  a.aligned = page % KEYS == 0 && llabs((long long)a.k_tok) * KEYS < 1ll << 31 && llabs((long long)a.v_tok) * KEYS < 1ll << 31;
   a.tiles = s.tiles;
   a.rows = s.rows;
   a.scale_log2 = scale * 1.4426950408889634f;

@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, 6) cache_read_kernel(const ReadArgs a
       }
     }
     own[i] = page < 0 ? -1 : (long long)page * a.page + at;
-    for (int w = 0; w < a.sides; ++w) base[w][i] = page * a.side[w].c_page + at * a.side[w].c_tok;
+    for (int w = 0; w < a.sides; ++w) base[w][i] = page * a.side[w].c_page + (long long)at * a.side[w].c_tok;
   }
   __syncthreads();
   for (int w = 0; w < a.sides; ++w) {

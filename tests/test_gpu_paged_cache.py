@@ -183,7 +183,9 @@ def _check(q, kc, vc, table, lens, scale, ks=None, vs=None, got=None):
     half = HALF_STEP[q.dtype]
     weight = 2.0 ** -11 if ks is not None else half
     n = max(max(lens), 1)
-    bound = half * want.abs() + (1 + half) * (size * (weight + 2 * e_score + 2.0 ** -20 + 4 * n * 2.0 ** -24) + (lost if ks is not None else 0))
+    # over a 16-bit cache the sum is that of the rounded weights: sum p (1 + d) v / sum p (1 + d) is off by sum p d (v - o), |d| <= weight
+    own = half * want.abs() if ks is not None else (half + weight) * want.abs()
+    bound = own + (1 + half) * (size * (weight + 2 * e_score + 2.0 ** -20 + 4 * n * 2.0 ** -24) + (lost if ks is not None else 0))
     bound = bound + torch.finfo(q.dtype).smallest_normal
     assert got.dtype == q.dtype and ((got.double() - want).abs() <= bound).all(), ((got.double() - want).abs() / bound).max()
     return got
@@ -273,6 +275,39 @@ def test_paged_attention_of_a_cache_behind_32_bits(store):
     _check(_randn(1, 32, D, seed=2), kc, vc, table, lens, D ** -0.5, ks, vs)
     got = F_.cache_read(kc, vc, table, _i32([0, 150]), 150, ks, vs)
     assert all(torch.equal(a, b) for a, b in zip(got, ref.cache_read(kc, vc, table, _i32([0, 150]), 150, ks, vs, torch.bfloat16)))
+
+
+@pytest.mark.parametrize("form", ["long pages", "places first"])
+def test_places_of_a_page_far_apart(form):
+    """Tokens of one page more than 2^31 bytes apart: pages of a million tokens, and a cache laid out [page, pages, heads, width]."""
+    G, D = 8, 128
+    if form == "long pages":
+        page, pages = 1050000, 2
+        kc, vc = (torch.empty(pages, page, G, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        lens, ends, table, first = [page + 70], [0, page + 70], _i32([[1, 0]]), page - 100
+    else:
+        page, pages = 32, 70000
+        kc, vc = (torch.empty(page, pages, G, D, dtype=torch.bfloat16, device="cuda").transpose(0, 1) for _ in range(2))
+        lens, ends, table, first = [100], [0, 100], _i32([[pages - 1, 0, 3, pages - 2]]), 0
+    assert (page - 1) * kc.stride(1) * 2 > 2 ** 31
+    n = lens[0] - first                                       # the tokens that are written; the others hold zeros
+    if first:
+        kc.zero_()
+        vc.zero_()
+    k, v = _randn(n, G, D), _randn(n, G, D, seed=1)
+    pos = torch.arange(first, lens[0], device="cuda")
+    F_.cache_write(k, v, kc, vc, table[0].long()[pos // page] * page + pos % page)
+    got = F_.cache_read(kc, vc, table, _i32(ends), lens[0])
+    assert torch.equal(got[0][first:], k) and torch.equal(got[1][first:], v) and not got[0][:first].any()
+    q = _randn(1, 32, D, seed=2)
+    o = F_.paged_attention(q, kc, vc, table, _i32(lens), 0.5)
+    (k_all, v_all), heads = (t.double() for t in got), q[0].double().view(G, 4, D)
+    for g in range(G):
+        s = heads[g] @ k_all[:, g].T * 0.5
+        p = torch.softmax(s, 1)
+        e = 2 * ((D + 8) * 2.0 ** -23 * (heads[g].abs() @ k_all[:, g].abs().T * 0.5)).amax(1, keepdim=True) + 2.0 ** -19 + lens[0] * 2.0 ** -23
+        want, size = p @ v_all[:, g], p @ v_all[:, g].abs()
+        assert ((o[0].view(G, 4, D)[g].double() - want).abs() <= (2.0 ** -8 + e) * 2 * size + 2.0 ** -8 * want.abs()).all()
 
 
 def test_paged_attention_same_bits_and_other_stream():
