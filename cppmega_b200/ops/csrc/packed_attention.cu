@@ -9,8 +9,8 @@
 // high.  Groups that do not divide 128 leave the last rows of a tile idle.  Tensor maps over [width, heads, tokens] read the rows where
 // they lie, whatever the strides, and give zeros behind a width that is no multiple of 64.
 //
-// Sequences.  A block finds its own tile: with f(p) = the number of tiles at place p or later of their sequences, block u works on the
-// place p with f(p + 1) <= u < f(p).  So the tiles with the longest loops of ALL sequences start first, and neither the host nor another kernel
+// Sequences.  A block finds its own tile: with f(p) = the number of tiles at place p or later of their sequences (counted in tiles from the first
+// key that a sequence's queries see), block u works on the place p with f(p + 1) <= u < f(p).  So the tiles with the longest loops of ALL sequences start first, and neither the host nor another kernel
 // lays out a plan.  The grid is the bound that the host knows (rows / tile + sequences); the blocks left over fill the rows behind the
 // last sequence with zeros.  Rows of a tile behind its sequence's end belong to somebody else: as rows of the result they are not
 // stored, as summed rows (V; K of dq; Q and dO of the key gradients) they are set to zero in shared memory, since a weight of zero does not
@@ -147,19 +147,23 @@ __device__ Unit find_unit(const Args& a, bool of_keys, int per, int u, int lane)
   constexpr int KEPT = 4;                    // sequences that a lane keeps the tiles of; more are counted again each time
   Unit r = {};
   bool bad = false;
-  int kept[KEPT], q0 = 0, L = 0, k0 = 0, Lk = 0;              // of sequence `lane`
+  int kept[KEPT], ahead[KEPT], q0 = 0, L = 0, k0 = 0, Lk = 0;              // of sequence `lane`
   auto tiles = [&](int rows) { return int(unsigned(rows + per - 1) / unsigned(per)); };
   const int* cu = of_keys ? a.cu_k : a.cu_q;
   auto tiles_of = [&](int i) { return tiles(__ldg(cu + i + 1) - __ldg(cu + i)); };
+  // a sequence's first place: the keys before its first query, in tiles
+  auto first_of = [&](int rows, int keys) { return of_keys || keys <= rows ? 0 : int(unsigned(keys - rows) / unsigned(per)); };
+  auto first_at = [&](int i) { return first_of(__ldg(a.cu_q + i + 1) - __ldg(a.cu_q + i), __ldg(a.cu_k + i + 1) - __ldg(a.cu_k + i)); };
 #pragma unroll
   for (int c = 0; c < KEPT; ++c) {
     const int i = c * 32 + lane;
-    kept[c] = 0;
+    kept[c] = ahead[c] = 0;
     if (c * 32 >= a.n) continue;
     if (i < a.n) {
       const int x0 = __ldg(a.cu_q + i), x1 = __ldg(a.cu_q + i + 1), y0 = __ldg(a.cu_k + i), y1 = __ldg(a.cu_k + i + 1);
       bad |= x0 < 0 || x1 < x0 || x1 > a.T || y0 < 0 || y1 < y0 || y1 > a.Tk || (i == 0 && (x0 != 0 || y0 != 0));
       kept[c] = tiles(of_keys ? y1 - y0 : x1 - x0);
+      ahead[c] = first_of(x1 - x0, y1 - y0);
       if (c == 0) { q0 = x0; L = x1 - x0; k0 = y0; Lk = y1 - y0; }
     }
   }
@@ -173,12 +177,12 @@ __device__ Unit find_unit(const Args& a, bool of_keys, int per, int u, int lane)
   auto after = [&](int p) {                  // tiles at place p or later
     int s = 0;
 #pragma unroll
-    for (int c = 0; c < KEPT; ++c) s += max(0, kept[c] - p);
-    for (int i = KEPT * 32 + lane; i < a.n; i += 32) s += max(0, tiles_of(i) - p);
+    for (int c = 0; c < KEPT; ++c) s += min(kept[c], max(0, ahead[c] + kept[c] - p));
+    for (int i = KEPT * 32 + lane; i < a.n; i += 32) s += min(tiles_of(i), max(0, first_at(i) + tiles_of(i) - p));
     return __reduce_add_sync(0xffffffffu, s);
   };
-  int most = max(max(kept[0], kept[1]), max(kept[2], kept[3]));
-  for (int i = KEPT * 32 + lane; i < a.n; i += 32) most = max(most, tiles_of(i));
+  int most = max(max(ahead[0] + kept[0], ahead[1] + kept[1]), max(ahead[2] + kept[2], ahead[3] + kept[3]));
+  for (int i = KEPT * 32 + lane; i < a.n; i += 32) most = max(most, first_at(i) + tiles_of(i));
   r.total = after(0);
   if (u >= r.total) return r;
   int lo = 0, hi = __reduce_max_sync(0xffffffffu, most), from_hi = 0;         // after(lo) > u >= after(hi)
@@ -187,14 +191,17 @@ __device__ Unit find_unit(const Args& a, bool of_keys, int per, int u, int lane)
     if (f > u) lo = mid;
     else { hi = mid; from_hi = f; }
   }
-  r.place = lo;
   int rank = u - from_hi, seq = 0;           // hi is lo + 1: the rank-th of the sequences that have a tile at this place
   for (int c = 0, i0 = 0; i0 < a.n; i0 += 32, ++c) {
-    const int t = c == 0 ? kept[0] : c == 1 ? kept[1] : c == 2 ? kept[2] : c == 3 ? kept[3] : i0 + lane < a.n ? tiles_of(i0 + lane) : 0;
-    const unsigned has = __ballot_sync(0xffffffffu, t > lo);
+    const bool there = i0 + lane < a.n;
+    const int t = c == 0 ? kept[0] : c == 1 ? kept[1] : c == 2 ? kept[2] : c == 3 ? kept[3] : there ? tiles_of(i0 + lane) : 0;
+    const int f = c == 0 ? ahead[0] : c == 1 ? ahead[1] : c == 2 ? ahead[2] : c == 3 ? ahead[3] : there ? first_at(i0 + lane) : 0;
+    const bool at = f <= lo && lo < f + t;
+    const unsigned has = __ballot_sync(0xffffffffu, at);
     if (rank < __popc(has)) {
-      const bool it = t > lo && __popc(has & ((1u << lane) - 1)) == rank;
-      seq = i0 + __ffs(__ballot_sync(0xffffffffu, it)) - 1;
+      const int src = __ffs(__ballot_sync(0xffffffffu, at && __popc(has & ((1u << lane) - 1)) == rank)) - 1;
+      seq = i0 + src;
+      r.place = lo - __shfl_sync(0xffffffffu, f, src);
       break;
     }
     rank -= __popc(has);
