@@ -29,13 +29,14 @@
 // whatever was ready first spent more time on polling than the products took (forward 2100 cycles a 128 x 128 tile).
 // Query tiles of the key gradients run from the last one down: blocks of one sequence then read the same rows at the same time, out of L2.
 //
-// Roundings to 16 bits: P and dS, as operands of their products.  o is divided by the sum of the weights as rounded, so that what a rounding
-// adds to one weight moves o only by that weight's distance from it; the largest weight, which is not 1 while the maximum that it is taken
-// against lags, otherwise moves a row that settles on one key by 2^-9 of itself (8 % of the forward's time).  delta takes o before its rounding
-// (the forward keeps what that takes away, in 16 bits more).  Both because an error of o is added to every ds of a row with one sign: dq and
-// dk of rows that settle on few keys are off by 2.45e-3 of their norms, where the roundings of dS and of the result itself make 2.4e-3;
-// 3.0e-3 with the sum of unrounded weights, 4.0e-3 with the rounded o too.  Maxima, sums, scores, deltas and all accumulators are fp32.  fp16's range
-// is too short for dS of any size: it is scaled by a power of two, from the row's largest |do| for dq, from the call's for dk.
+// Roundings to 16 bits: P and dS, as operands of their products.  o is divided by a sum in which the largest weight of every 64 keys counts as it
+// was rounded, so that what rounding adds to it moves o only by that key's distance from it: no weight is 1 while the maximum that it is taken
+// against lags, and a row that settles on one key was off by up to 2^-9 of itself.  (The sum of all weights as rounded gives the same errors to
+// within 1 % and takes 20 % more of the forward's time.)  delta takes o before its rounding (the forward keeps what that takes away, in 16 bits
+// more).  Both because an error of o is added to every ds of a row with one sign: dq and dk of rows that settle on few keys are off by 2.45e-3 of
+// their norms, where the roundings of dS and of the result itself make 2.4e-3; 3.0e-3 with the sum of unrounded weights, 4.0e-3 with the
+// rounded o too.  Maxima, sums, scores, deltas and all accumulators are fp32.  fp16's range is too short for dS of any size: it is scaled by a
+// power of two, from the row's largest |do| for dq, from the call's for dk.
 #include <cuda_fp16.h>
 
 #include "fp32_pair.cuh"
@@ -86,6 +87,11 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
+  return d;
 }
 template <bool HALF>
 __device__ __forceinline__ uint32_t pair(float lo, float hi) {
@@ -483,7 +489,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int last = mine ? off + pos : -1;                   // last key it sees
     const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tO = tmem + 256 + t * DV + lane_addr;
-    float m_ref = -INFINITY, l = 0.f, l_taken = 0.f;          // sums of the weights, and of the weights as rounded
+    float m_ref = -INFINITY, l = 0.f, gained = 0.f;           // sums of the weights, and of what rounding adds to the largest ones
     auto part = [&](int j, auto where) {
       constexpr bool MASK = decltype(where)::value;
       const int lim = last - j * PART;                        // columns up to lim are seen
@@ -496,18 +502,20 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tmem_ld_wait();
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        if (!MASK || e <= lim) top[e & 1] = fmaxf(top[e & 1], __uint_as_float(s0[e]));
-        if (!MASK || 32 + e <= lim) top[2 + (e & 1)] = fmaxf(top[2 + (e & 1)], __uint_as_float(s1[e]));
+      for (int e = 0; e < 32; e += 2) {
+        const int to = e >> 1 & 1;
+        top[to] = max3(top[to], !MASK || e <= lim ? __uint_as_float(s0[e]) : -INFINITY, !MASK || e + 1 <= lim ? __uint_as_float(s0[e + 1]) : -INFINITY);
+        top[2 + to] = max3(top[2 + to], !MASK || 32 + e <= lim ? __uint_as_float(s1[e]) : -INFINITY,
+                           !MASK || 33 + e <= lim ? __uint_as_float(s1[e + 1]) : -INFINITY);
       }
-      float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      if (m_new != -INFINITY) m_new *= a.scale_log2;          // a scale of zero leaves "nothing seen" as it is
+      const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      const float m_new = largest != -INFINITY ? largest * a.scale_log2 : -INFINITY;            // a scale of zero leaves "nothing seen" as it is
       float alpha = 1.f;
       if (m_new > m_ref + RESCALE_AT) {                       // also from -inf
         alpha = ex2(m_ref - m_new);
         m_ref = m_new;
         l *= alpha;
-        l_taken *= alpha;
+        gained *= alpha;
       }
       if (__any_sync(0xffffffffu, alpha != 1.f) && j > 0) {   // O of all parts before this one
         if (!warp_wait(&sh->pv_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
@@ -523,7 +531,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
       const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // nothing seen so far
-      Pair sum[2] = {pr(0.f), pr(0.f)}, taken[2] = {pr(0.f), pr(0.f)};
+      Pair sum[2] = {pr(0.f), pr(0.f)};
       uint32_t p[32];
       auto quarter = [&](const uint32_t (&sc)[32], int col0, int at) {
 #pragma unroll
@@ -536,15 +544,16 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           sum[e & 1] = sum[e & 1] + pr(x, y);
           p[at + e] = pair<HALF>(x, y);
-          const float2 w = unpair<HALF>(p[at + e]);
-          taken[e & 1] = taken[e & 1] + pr(w.x, w.y);
         }
       };
       quarter(s0, 0, 0);
       quarter(s1, 32, 16);
       tmem_st(tS, p);
       l += pr_sum(sum[0] + sum[1]);
-      l_taken += pr_sum(taken[0] + taken[1]);
+      if (largest != -INFINITY) {                             // the part's largest weight, as above
+        const float x = ex2(fmaf(largest, a.scale_log2, -ref));
+        gained += unpair<HALF>(pair<HALF>(x, 0.f)).x - x;
+      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -558,7 +567,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (ok && count > 0) ok = warp_wait(&sh->pv_done[t][(count - 1) & 1], ((count - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
     if (ok) {
       tc_fence_after();
-      const float inv = l_taken > 0.f ? 1.f / l_taken : l_taken == 0.f ? 0.f : l_taken;            // a NaN stays
+      const float taken = l + gained, inv = taken > 0.f ? 1.f / taken : taken == 0.f ? 0.f : taken;            // a NaN stays
       const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
       const float f = last >= 0 ? inv : 0.f;
       uint8_t* stage = sQ + t * F::KS * SLAB;                 // Q_t has been used

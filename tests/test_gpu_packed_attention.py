@@ -2,7 +2,8 @@
 
 Tolerances from the exact values, with u half a step of the type (2^-8 in bf16, 2^-11 in fp16) and e the error of a weight's exponent, twice the
 error of a score (its fp32 sum over D products, D 2^-23 of their magnitudes in any order, and roundings of scale and maximum): a weight p is off
-by p (u + e); o, divided by the sum of the weights as rounded, by sum p |v - o| (u + e) <= (|p||v| + |o|) (u + e) and its own rounding; delta and dP by fp32 sums over the value columns of do, v and o as rounded; ds by
+by p (u + e); o, whose sum of weights has the largest of every 64 keys as rounded, by p |v - o| (u + e) for those and p |v| (u + e) for the others,
+at most (|p||v| + |o|) (u + e), and its own rounding; delta and dP by fp32 sums over the value columns of do, v and o as rounded; ds by
 its rounding u and by the errors of p and of dP - delta; a gradient by its operands' errors, its fp32 sum and its own rounding.  In fp16 what is
 below the range is lost: 2^-25 of a weight of up to 2^8, and of ds scaled so that |do| is at most 2^-4.
 """
@@ -134,8 +135,9 @@ def test_one_head(lens, D, V, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D,V", [(128, 128), (64, 64)])
 def test_rows_that_settle_on_few_keys(D, V, dtype):
-    """o = sum p (1 + d) v / sum p (1 + d) with |d| <= u + e is off by at most sum p |v - o| (u + e) / (1 - u - e), and its rounding: nearly nothing
-    but the rounding where one weight is nearly all of a row, although that weight is no power of two while the maximum lags."""
+    """o = sum p (1 + d) v / sum p (1 + d'), |d| <= u + e, where d' is d for the largest weight of every 64 keys and without u for the others, is off by at most
+    the sum of p |v - o| (u + e) over those and of p (|v| u + |v - o| e) over the others, each over 1 - u - e, and its rounding: nearly nothing but the rounding
+    where one weight is nearly all of a row, although that weight is no power of two while the maximum lags."""
     L, u = 400, HALF_STEP[dtype]
     q, k, v = _randn(L, 1, D, dtype=dtype, std=1.5), _randn(L, 1, D, dtype=dtype, seed=1), _randn(L, 1, V, dtype=dtype, seed=2)
     k[70::100] *= 4
@@ -147,7 +149,10 @@ def test_rows_that_settle_on_few_keys(D, V, dtype):
     mags = (qh.abs() @ kh.abs().T * D ** -0.5).masked_fill(hidden, 0.0)
     e = 2 * (((D + 8) * 2.0 ** -23) * mags).amax(1, keepdim=True) + 2.0 ** -19 + L * 2.0 ** -23
     out = p @ vh
-    spread = (p[:, :, None] * (vh[None] - out[:, None]).abs()).sum(1)
+    parts = torch.nn.functional.pad(p, (0, -L % 64)).view(L, -1, 64)
+    largest = (parts == parts.amax(2, keepdim=True)).view(L, -1)[:, :L]
+    away = (vh[None] - out[:, None]).abs()
+    spread = (p[:, :, None] * torch.where(largest[:, :, None], away, torch.maximum(away, vh.abs()[None]))).sum(1)
     lost = 2.0 ** -17 * p.amax(1, keepdim=True) * vh.abs().sum(0, keepdim=True) if dtype == torch.float16 else 0.0
     _check(o, out, spread * (u + e) / (1 - u - e) + lost + u * out.abs() * (1 + u) + 2.0 ** -24 * L * (p @ vh.abs()), "o")
 
