@@ -39,6 +39,7 @@
 // power of two, from the row's largest |do| for dq, from the call's for dk.
 #include <cuda_fp16.h>
 
+#include "few_rows.cuh"
 #include "fp32_pair.cuh"
 
 namespace cm {
@@ -130,6 +131,8 @@ struct Args {
   int by_hb;                                 // r / hb is r * by_hb >> 16 for r < 128
   int dim, vdim;
   int units;                                 // blocks per (key head, chunk)
+  int splits;                                // forward: blocks that share the keys of a pair of query tiles
+  float* part;                               // what each of them leaves: [unit, key head, chunk][split][tile][DV + 3][128 rows]
   float scale, scale_log2;
   void* out;                                 // forward: o [T, heads, vdim]; backward: dq [T, heads, dim] or dk [Tk, kv_heads, dim]
   void* out2;                                // forward: what rounding took from o, or null; backward: dv [Tk, kv_heads, vdim]
@@ -308,6 +311,22 @@ struct Whole { static constexpr bool value = false; };
 constexpr int THREADS = 352;
 constexpr int MMA_WARP = 8, TMA_WARP = 10;
 
+// Few rows on many keys: the key tiles of a pair of query tiles are shared out among neighbouring blocks, no fewer than four to each, and
+// join_kernel makes one result of what they leave.
+struct Share {
+  int begin, tiles, pieces;                  // first key tile, key tiles of a block, blocks that have any
+};
+constexpr int FEWEST_TILES = 4;              // 512 keys: about as long as a block's set-up and what it leaves take
+__device__ __forceinline__ Share share_of(const Args& a, const Unit& unit, int split) {
+  const int last = min(unit.L, 2 * (unit.place + 1) * a.tok) - 1 + unit.Lk - unit.L;       // last key that the pair sees
+  const int all = last >= 0 ? last / TILE + 1 : 0;
+  Share s;
+  s.tiles = a.splits == 1 ? max(all, 1) : max(FEWEST_TILES, (all + a.splits - 1) / a.splits);
+  s.pieces = max(1, (all + s.tiles - 1) / s.tiles);
+  s.begin = split * s.tiles;
+  return s;
+}
+
 template <int D, int DV>
 struct Fwd {
   static constexpr int KS = D / 64, VS = DV / 64;
@@ -334,7 +353,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint8_t* sV = sK + F::K_SLOTS * F::KS * SLAB;
   auto* sh = reinterpret_cast<typename F::Shared*>(sV + F::V_SLOTS * F::VS * SLAB);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int hh = a.kv_heads * a.chunks, u = blockIdx.x / hh, kvh = (blockIdx.x % hh) / a.chunks, chunk = blockIdx.x % a.chunks;
+  few::let_next_start();
+  const int tiles = blockIdx.x / a.splits, split = blockIdx.x % a.splits;             // two query tiles; a share of their keys
+  const int hh = a.kv_heads * a.chunks, u = tiles / hh, kvh = (tiles % hh) / a.chunks, chunk = tiles % a.chunks;
   const int head0 = kvh * (a.heads / a.kv_heads) + chunk * a.hb;
   volatile int* abort_flag = &sh->abort_flag;
   if (warp == 0) {
@@ -374,18 +395,24 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (tid == 0 && a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
       return;
     }
-    clear_rows(a.out, __ldg(a.cu_q + a.n), a.T, a.heads, head0, a.hb, a.vdim, u - unit.total, a.units - unit.total);
+    if (split == 0) clear_rows(a.out, __ldg(a.cu_q + a.n), a.T, a.heads, head0, a.hb, a.vdim, u - unit.total, a.units - unit.total);
     return;
   }
-  const int q0 = unit.q0, L = unit.L, k0 = unit.k0, Lk = unit.Lk;
+  // this block's key tiles; from here on the keys are counted from the first of them
+  const Share share = share_of(a, unit, split);
+  const int q0 = unit.q0, L = unit.L, k0 = unit.k0 + share.begin * TILE, Lk = unit.Lk - share.begin * TILE;
   const int off = Lk - L;                    // query i sees the keys up to i + off
   const int rows = a.hb * a.tok;
+  if (split > 0 && split >= share.pieces) {
+    if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
+    return;
+  }
   // halves of key tiles (64 keys) of query tile t, and the first of them that the mask cuts
   int n[2], whole[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int first = (2 * unit.place + t) * a.tok, last = min(L, first + a.tok) - 1;
-    n[t] = first < L && off + last >= 0 ? (off + last) / PART + 1 : 0;
+    n[t] = first < L && off + last >= 0 ? min((off + last) / PART + 1, 2 * share.tiles) : 0;
     whole[t] = off + first + 1 > 0 ? (off + first + 1) / PART : 0;
   }
   const int most = (max(n[0], n[1]) + 1) / 2;
@@ -567,21 +594,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (ok && count > 0) ok = warp_wait(&sh->pv_done[t][(count - 1) & 1], ((count - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL);
     if (ok) {
       tc_fence_after();
-      const float taken = l + gained, inv = taken > 0.f ? 1.f / taken : taken == 0.f ? 0.f : taken;            // a NaN stays
-      const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
-      const float f = last >= 0 ? inv : 0.f;
-      uint8_t* stage = sQ + t * F::KS * SLAB;                 // Q_t has been used
-      int places_at[8];
-      places(places_at, (warp & 3) * 32, lane, [&](int r) {
-        const int tok = r * a.by_hb >> 16;
-        return r < rows && qt * a.tok + tok < L ? tok * a.heads + (r - tok * a.hb) : -1;
-      });
-      const long long first = ((long long)(q0 + qt * a.tok) * a.heads + head0) * a.vdim;
-      // o to one slab and what its rounding takes away to the other, 64 columns at a time; where Q_t has one slab alone (width 64) one after the other
-      constexpr int PASSES = F::KS == 1 ? 2 : 1;
-#pragma unroll
-      for (int pass = 0; pass < PASSES; ++pass) {
-        if (pass == 1 && !a.out2) break;
+      if (share.pieces > 1) {
+        float* to = a.part + (((long long)blockIdx.x * 2 + t) * (DV + 3)) * TILE + r;
+        to[0] = m_ref;
+        to[TILE] = l;
+        to[2 * TILE] = l + gained;
 #pragma unroll
         for (int c = 0; c < DV / 32; ++c) {
           uint32_t o[32];
@@ -590,27 +607,99 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tmem_ld_wait();
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = last >= 0 ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;            // a row without keys
-          if (pass == 0) put_columns<HALF>(stage, r, (c & 1) * 32, o);
-          if (a.out2 && pass == PASSES - 1) {
-            take_rest<HALF>(o);
-            put_columns<HALF>(stage + (PASSES == 1 ? SLAB : 0), r, (c & 1) * 32, o);
-          }
-          if (c & 1) {
-            const int begin = (c - 1) * 32;
-            if (pass == 0) send_rows(stage, (warp & 3) * 32, begin, a.vdim, lane, places_at, reinterpret_cast<uint16_t*>(a.out) + first);
-            if (a.out2 && pass == PASSES - 1)
-              send_rows(stage + (PASSES == 1 ? SLAB : 0), (warp & 3) * 32, begin, a.vdim, lane, places_at, reinterpret_cast<uint16_t*>(a.out2) + first);
+          for (int e = 0; e < 32; ++e) to[(3 + c * 32 + e) * TILE] = last >= 0 ? __uint_as_float(o[e]) : 0.f;            // nothing seen here
+        }
+      } else {
+        const float taken = l + gained, inv = taken > 0.f ? 1.f / taken : taken == 0.f ? 0.f : taken;            // a NaN stays
+        const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
+        const float f = last >= 0 ? inv : 0.f;
+        uint8_t* stage = sQ + t * F::KS * SLAB;                 // Q_t has been used
+        int places_at[8];
+        places(places_at, (warp & 3) * 32, lane, [&](int r) {
+          const int tok = r * a.by_hb >> 16;
+          return r < rows && qt * a.tok + tok < L ? tok * a.heads + (r - tok * a.hb) : -1;
+        });
+        const long long first = ((long long)(q0 + qt * a.tok) * a.heads + head0) * a.vdim;
+        // o to one slab and what its rounding takes away to the other, 64 columns at a time; where Q_t has one slab alone (width 64) one after the other
+        constexpr int PASSES = F::KS == 1 ? 2 : 1;
+  #pragma unroll
+        for (int pass = 0; pass < PASSES; ++pass) {
+          if (pass == 1 && !a.out2) break;
+  #pragma unroll
+          for (int c = 0; c < DV / 32; ++c) {
+            uint32_t o[32];
+            if (count > 0) {
+              tmem_ld_32x32(tO + c * 32, o);
+              tmem_ld_wait();
+            }
+  #pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = last >= 0 ? __float_as_uint(__uint_as_float(o[e]) * f) : 0u;            // a row without keys
+            if (pass == 0) put_columns<HALF>(stage, r, (c & 1) * 32, o);
+            if (a.out2 && pass == PASSES - 1) {
+              take_rest<HALF>(o);
+              put_columns<HALF>(stage + (PASSES == 1 ? SLAB : 0), r, (c & 1) * 32, o);
+            }
+            if (c & 1) {
+              const int begin = (c - 1) * 32;
+              if (pass == 0) send_rows(stage, (warp & 3) * 32, begin, a.vdim, lane, places_at, reinterpret_cast<uint16_t*>(a.out) + first);
+              if (a.out2 && pass == PASSES - 1)
+                send_rows(stage + (PASSES == 1 ? SLAB : 0), (warp & 3) * 32, begin, a.vdim, lane, places_at, reinterpret_cast<uint16_t*>(a.out2) + first);
+            }
           }
         }
+        if (mine && a.lse) a.lse[at] = l == 0.f ? INFINITY : m_ref + log2f(l);
       }
-      if (mine && a.lse) a.lse[at] = l == 0.f ? INFINITY : m_ref + log2f(l);
     }
   }
   tc_fence_before();
   __syncthreads();
   settle(abort_flag);
   if (warp == MMA_WARP) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// What the blocks of a pair of query tiles left, in the order of their keys.  A block per tile and eight columns, a thread per row.
+template <bool HALF, int DV>
+__global__ void __launch_bounds__(TILE) packed_join_kernel(const Args a) {
+  constexpr int COLUMNS = 8, STEP = (DV + 3) * TILE * 2;
+  __shared__ Unit found;
+  const int chunks_of = DV / COLUMNS, c0 = blockIdx.x % chunks_of * COLUMNS, t = blockIdx.x / chunks_of % 2, tiles = blockIdx.x / chunks_of / 2;
+  const int hh = a.kv_heads * a.chunks, u = tiles / hh, kvh = (tiles % hh) / a.chunks, chunk = tiles % a.chunks, r = threadIdx.x;
+  if (threadIdx.x < 32) {
+    const Unit f = find_unit(a, false, 2 * a.tok, u, threadIdx.x);
+    if (threadIdx.x == 0) found = f;
+  }
+  __syncthreads();
+  const Unit unit = found;
+  few::wait_for_input();                     // by every block: the next kernel of the stream counts on this one having waited
+  if (unit.bad || u >= unit.total || c0 >= a.vdim) return;
+  const int pieces = share_of(a, unit, 0).pieces, tok = r * a.by_hb >> 16, pos = (2 * unit.place + t) * a.tok + tok;
+  if (pieces == 1 || r >= a.hb * a.tok || pos >= unit.L) return;
+  const float* from = a.part + ((long long)tiles * a.splits * 2 + t) * (DV + 3) * TILE + r;
+  float m = -INFINITY, l = 0.f, taken = 0.f, o[COLUMNS] = {};
+  for (int s = 0; s < pieces; ++s) m = fmaxf(m, from[(long long)s * STEP]);
+  const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 2
+  for (int s = 0; s < pieces; ++s) {
+    const float* x = from + (long long)s * STEP;
+    const float by = ex2(x[0] - ref);
+    l += by * x[TILE];
+    taken += by * x[2 * TILE];
+#pragma unroll
+    for (int c = 0; c < COLUMNS; ++c) o[c] += by * x[(3 + c0 + c) * TILE];
+  }
+  const float inv = taken > 0.f ? 1.f / taken : taken == 0.f ? 0.f : taken;               // a NaN stays
+  const long long at = (long long)(unit.q0 + pos) * a.heads + kvh * (a.heads / a.kv_heads) + chunk * a.hb + (r - tok * a.hb);
+  uint32_t w[4], rest[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const float x = o[2 * c] * inv, y = o[2 * c + 1] * inv;
+    w[c] = pair<HALF>(x, y);
+    const float2 f = unpair<HALF>(w[c]);
+    rest[c] = pair<HALF>(x - f.x, y - f.y);
+  }
+  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + at * a.vdim + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (a.out2) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out2) + at * a.vdim + c0) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+  if (a.lse && c0 == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
 // ---- backward: delta -----------------------------------------------------------------------------------------------------
@@ -1301,6 +1390,15 @@ int shape(Args& a) {
   return 0;
 }
 
+// Blocks that share the keys of a pair of query tiles in the forward: as many as there are SMs for, where half of them or more would have nothing to do
+// (64 new tokens on 8128 keys, 4 heads over 1: 20 us, 112 unshared; 512 on 7680, 32 heads over 8, two shares: 71 us, 108 unshared).
+int splits_of(const Args& a) {
+  const long long pairs = (a.T / (2 * a.tok) + (long long)a.n) * a.kv_heads * a.chunks, sms = sm_count() > 0 ? sm_count() : 1;
+  const long long most = a.Tk / (FEWEST_TILES * TILE);
+  if (pairs < 1 || 2 * pairs > sms || most < 2) return 1;
+  return int(sms / pairs < most ? sms / pairs : most);
+}
+
 struct Inputs {
   const void *q, *k, *v, *g;
   const long long *qs, *ks, *vs, *gs;
@@ -1321,11 +1419,14 @@ int forward(const Inputs& in, Args a, cudaStream_t stream) {
   static PerDevice cfg;
   if (!rc) rc = configure(packed_fwd_kernel<HALF, D, DV>, Fwd<D, DV>::SMEM, cfg);
   if (rc) return rc;
-  const long long units = units_of(a.T, a.n, 2 * a.tok), grid = units * a.kv_heads * a.chunks;
-  if (grid > 0x7fffffffLL) return -10;
+  const long long units = units_of(a.T, a.n, 2 * a.tok), pairs = units * a.kv_heads * a.chunks;
+  a.splits = a.part ? splits_of(a) : 1;
+  if (pairs * a.splits > 0x7fffffffLL) return -10;
   a.units = (int)units;
-  packed_fwd_kernel<HALF, D, DV><<<(unsigned)grid, THREADS, Fwd<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], a);
-  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+  packed_fwd_kernel<HALF, D, DV><<<(unsigned)(pairs * a.splits), THREADS, Fwd<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], a);
+  if (cudaGetLastError() != cudaSuccess) return -3;
+  if (a.splits == 1) return 0;
+  return few::launch_early(packed_join_kernel<HALF, DV>, dim3((unsigned)(pairs * 2 * (DV / 8))), dim3(TILE), 0, stream, a);
 }
 
 template <bool HALF, int D, int DV>
@@ -1376,16 +1477,25 @@ static int arguments(Args& a, const int* cu_q, const int* cu_k, float scale, con
   return shape(a);
 }
 
+// Floats of work space that the forward wants for these sizes (as below) on the current device; 0: none
+extern "C" long long cm_packed_attention_ws(const long long* n) {
+  Args a = {};
+  if (arguments(a, nullptr, nullptr, 0.f, n, nullptr)) return 0;
+  const int splits = splits_of(a);
+  return splits == 1 ? 0 : units_of(a.T, a.n, 2 * a.tok) * a.kv_heads * a.chunks * splits * 2 * ((a.vdim > 64 ? 128 : 64) + 3) * TILE;
+}
+
 // q [T, heads, dim], k [Tk, kv_heads, dim], v [Tk, kv_heads, vdim]; cu_q, cu_k [sequences + 1]; o [T, heads, vdim] packed; for a backward pass
-// o_rest, as o, and lse [T, heads], else null
+// o_rest, as o, and lse [T, heads], else null; ws: cm_packed_attention_ws floats, or null
 extern "C" int cm_packed_attention_fwd(const void* q, const void* k, const void* v, const int* cu_q, const int* cu_k, void* o, void* o_rest,
-                                       float* lse, const long long* n, float scale, int* err, cudaStream_t stream) {
+                                       float* lse, float* ws, const long long* n, float scale, int* err, cudaStream_t stream) {
   Args a = {};
   const int rc = arguments(a, cu_q, cu_k, scale, n, err);
   if (rc) return rc;
   a.out = o;
   a.out2 = o_rest;
   a.lse = lse;
+  a.part = ws;
   const Inputs in = {q, k, v, nullptr, n, n + 2, n + 4, nullptr};
   if (n[15] == 0) {
     if (a.vdim > 64) return forward<false, 128, 128>(in, a, stream);

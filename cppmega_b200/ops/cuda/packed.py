@@ -14,12 +14,14 @@ from .paged import TYPES, Plan, planned, rows_on, strides, width_ok
 def declare(L: ctypes.CDLL) -> None:
     vp, i32, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
     sig = {
-        "cm_packed_attention_fwd": [vp] * 9 + [f32, vp, vp],
+        "cm_packed_attention_fwd": [vp] * 10 + [f32, vp, vp],
         "cm_packed_attention_bwd": [vp] * 14 + [f32, vp, vp],
     }
     for name, args in sig.items():
         if hasattr(L, name):
             getattr(L, name).argtypes, getattr(L, name).restype = args, i32
+    if hasattr(L, "cm_packed_attention_ws"):
+        L.cm_packed_attention_ws.argtypes, L.cm_packed_attention_ws.restype = [vp], ctypes.c_longlong
 
 
 def _strides_ok(t: torch.Tensor) -> bool:
@@ -49,8 +51,10 @@ def _plan(q, k, v, cu_q, cu_k):
     if not (q.dtype in TYPES and width_ok(q, 8, 128) and width_ok(v, 8, 128) and 0 < q.shape[0] < 2 ** 30 and 0 < k.shape[0] < 2 ** 30
             and q.shape[1] > 0):
         return False
-    return Plan(_numbers(q, k, v, cu_q), shape=(q.shape[0], q.shape[1], v.shape[2]), like=q.is_contiguous() and q.shape[2] == v.shape[2],
+    plan = Plan(_numbers(q, k, v, cu_q), shape=(q.shape[0], q.shape[1], v.shape[2]), like=q.is_contiguous() and q.shape[2] == v.shape[2],
                 copy=not (_strides_ok(q) and _strides_ok(k) and _strides_ok(v) and cu_q.is_contiguous() and (cu_k is None or cu_k.is_contiguous())))
+    plan.work = _cu.lib().cm_packed_attention_ws(plan.at)
+    return plan
 
 
 def _plan_backward(dt, q, k, v, cu_q, cu_k, o, rest, lse, go):
@@ -67,8 +71,9 @@ def _forward(plan, q, k, v, cu_q, cu_k, scale, keep):
     o = torch.empty_like(q) if plan.like else torch.empty(plan.shape, dtype=q.dtype, device=dev)
     rest = torch.empty_like(o) if keep else None
     lse = torch.empty(plan.shape[:2], dtype=torch.float32, device=dev) if keep else None
+    ws = torch.empty(plan.work, dtype=torch.float32, device=dev) if plan.work else None
     rc = _cu.lib().cm_packed_attention_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), o.data_ptr(), _ptr(rest),
-                                           _ptr(lse), plan.at, scale, _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
+                                           _ptr(lse), _ptr(ws), plan.at, scale, _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
     if rc:
         _failed("cm_packed_attention_fwd", rc)
     F_.count_launch("packed_attention")

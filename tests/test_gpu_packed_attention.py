@@ -173,6 +173,36 @@ def test_keys_with_their_own_ends(lens, lens_k, D, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,V", [(128, 128), (96, 48), (64, 64)])
+@pytest.mark.parametrize("lens,lens_k,H,G", [
+    ([64], [5000], 8, 2), ([1], [3001], 4, 1), ([3, 33, 1, 70], [4000, 33, 0, 640], 4, 2), ([200], [1100], 3, 1), ([2, 0, 300], [1, 50, 2500], 1, 1),
+    ([900], [900], 2, 1),
+])
+def test_few_rows_on_many_keys(lens, lens_k, H, G, D, V, dtype):
+    """Keys shared out among blocks: shares that end inside a tile's mask, that some rows do not reach, sequences too short to be shared."""
+    _run(lens, H, G, D, V, dtype, lens_k=lens_k, tail=2, train=lens[0] != 64)
+
+
+def test_few_rows_on_many_keys_captured():
+    """The same graph for lengths that are shared out and for lengths that are not."""
+    q, k, v = (_randn(n, h, 64, seed=s) for s, n, h in ((0, 40, 4), (1, 3000, 2), (2, 3000, 2)))
+    cu, cu_k = _i32([0, 20, 40]), _i32([0, 1500, 3000])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        F_.packed_attention(q, k, v, cu, 0.125, cu_k)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = F_.packed_attention(q, k, v, cu, 0.125, cu_k)
+    for ends, ends_k in (([0, 20, 40], [0, 1500, 3000]), ([0, 1, 40], [0, 2990, 3000]), ([0, 40, 40], [0, 100, 100]), ([0, 0, 7], [0, 2000, 2700])):
+        cu.copy_(_i32(ends))
+        cu_k.copy_(_i32(ends_k))
+        g.replay()
+        _compare(q, k, v, ends, ends_k, 0.125, o.clone())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_long_sequences(dtype):
     _run([2500, 1300], 4, 2, 128, 128, dtype)
 
