@@ -548,13 +548,17 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (!warp_wait(&sh->pv_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL)) return false;
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < DV / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32(tO + c * 32, o);
+        for (int c = 0; c < DV / 32; c += 2) {
+          uint32_t o[2][32];
+          tmem_ld_32x32(tO + c * 32, o[0]);
+          tmem_ld_32x32(tO + c * 32 + 32, o[1]);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st(tO + c * 32, o);
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[h][e] = __float_as_uint(__uint_as_float(o[h][e]) * alpha);
+            tmem_st(tO + (c + h) * 32, o[h]);
+          }
         }
       }
       const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // nothing seen so far
