@@ -9,7 +9,9 @@
 // stored as NaN.
 //
 // Both are copies: bytes in and out at the memory's rate is all there is.  A row belongs to 8 or 16 lanes, 16 bytes of it to each (8 of an
-// E4M3 row), so rows of any stride move in whole sectors, and four rows of every lane group are in flight at once.
+// E4M3 row), so rows of any stride move in whole sectors, and four rows of every lane group are in flight at once.  Measured: 4095 tokens of 32
+// heads, 128 + 64 wide in bf16: write 22 us, read 16 (15 each at the copy rate, though much of it stays in L2); 16384 tokens of 8 heads, 128 + 128 into
+// E4M3: write 35 us of 16 (67 % of the instructions that an SM can issue: a row's maximum, the exponent, two conversions a pair), back 20 of 16.
 //
 // Of tokens that are given the same slot the last one stays, whatever order the blocks run in: each block looks for its own slots among the
 // later tokens (a hash table of its own in shared memory).  It reads the list of slots once per block, 5 % of the bytes that move at 16384

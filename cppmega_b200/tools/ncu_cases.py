@@ -1,6 +1,6 @@
 """Small, self-terminating workloads for Nsight Compute captures of single kernels.
 
-    python -m cppmega_b200.tools.ncu_cases {gemm,gemm_wgrad,attention,head_linear,scan_fwd,scan_bwd,m2rnn,m2rnn_bwd,sparse_mla,indexer,ce,rmsnorm,rmsnorm_bwd,adamw,quantize,strided_copy,moe_local,mxfp8_gemm,residual_norm,gated_norm,gated_mlp,gated_mlp_few,gated_mlp_shared}
+    python -m cppmega_b200.tools.ncu_cases {gemm,gemm_wgrad,attention,head_linear,scan_fwd,scan_bwd,m2rnn,m2rnn_bwd,sparse_mla,indexer,ce,rmsnorm,rmsnorm_bwd,adamw,quantize,strided_copy,moe_local,mxfp8_gemm,residual_norm,gated_norm,gated_mlp,gated_mlp_few,gated_mlp_shared,packed_attention,paged_attention,paged_attention_e4m3,paged_cache}
 
 Each case launches its kernel three times on inputs that exceed the 126 MB L2 but hold at most a few GB, so a
 ``--set full`` capture of one launch finishes in a minute or two:
@@ -306,12 +306,65 @@ def case_gated_mlp(tokens: int = 4096, hidden: int = 3584, ffn: int = 18944):
     cu.check_errors()
 
 
+def case_packed_attention():
+    """Documents of different lengths in one buffer, 32 heads over 8, 128 wide (forward and backward)."""
+    from cppmega_b200.ops import cuda as cu
+    from cppmega_b200.ops import functional as F_
+    ends = torch.tensor([0, 6000, 11000, 14500, 16383, 16384], dtype=torch.int32, device="cuda")
+    q, k, v = (torch.randn(16384, heads, 128, device="cuda").bfloat16().requires_grad_() for heads in (32, 8, 8))
+    for _ in range(3):
+        F_.packed_attention(q, k, v, ends, 128 ** -0.5).backward(q.detach())
+    torch.cuda.synchronize()
+    cu.check_errors()
+
+
+def _paged_cache(sequences: int, tokens: int, quantised: bool):
+    """(keys, values, their exponents or None, block table, lengths) of a cache of 8 heads, 128 wide, pages of 64."""
+    pages = sequences * (tokens // 64)
+    caches = [torch.randn(pages, 64, 8, 128, device="cuda").bfloat16() for _ in range(2)]
+    scales = [None, None]
+    if quantised:
+        caches = [c.to(torch.float8_e4m3fn) for c in caches]
+        scales = [torch.full((pages, 64, 8), 127, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    table = torch.randperm(pages, device="cuda").int().view(sequences, -1)
+    return *caches, *scales, table, torch.full((sequences,), tokens, dtype=torch.int32, device="cuda")
+
+
+def case_paged_attention(quantised: bool = False):
+    """One token for each of 64 sequences of 8192 (E4M3: 16384) over a paged cache, 32 heads over 8."""
+    from cppmega_b200.ops import cuda as cu
+    from cppmega_b200.ops import functional as F_
+    kc, vc, ks, vs, table, lens = _paged_cache(64, 16384 if quantised else 8192, quantised)
+    q = torch.randn(64, 32, 128, device="cuda").bfloat16()
+    for _ in range(3):
+        F_.paged_attention(q, kc, vc, table, lens, 128 ** -0.5, ks, vs)
+    torch.cuda.synchronize()
+    cu.check_errors()
+
+
+def case_paged_cache():
+    """65536 tokens of 8 heads, 128 wide, quantised into a paged cache and read back."""
+    from cppmega_b200.ops import cuda as cu
+    from cppmega_b200.ops import functional as F_
+    kc, vc, ks, vs, table, lens = _paged_cache(32, 2048, True)
+    k, v = (torch.randn(65536, 8, 128, device="cuda").bfloat16() for _ in range(2))
+    slots = (table.long()[:, :, None] * 64 + torch.arange(64, device="cuda")).view(-1)
+    ends = torch.arange(0, 65537, 2048, dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        F_.cache_write(k, v, kc, vc, slots, ks, vs)
+        F_.cache_read(kc, vc, table, ends, 65536, ks, vs)
+    torch.cuda.synchronize()
+    cu.check_errors()
+
+
 CASES = {"gemm": case_gemm, "attention": case_attention, "head_linear": case_head_linear, "gemm_wgrad": lambda: case_gemm(True, True), "scan_fwd": case_scan_fwd,
          "scan_bwd": case_scan_bwd, "m2rnn": case_m2rnn, "ce": case_ce, "rmsnorm": case_rmsnorm, "mxfp8_gemm": case_mxfp8_gemm,
          "m2rnn_bwd": case_m2rnn_bwd, "sparse_mla": case_sparse_mla, "indexer": case_indexer,
          "rmsnorm_bwd": case_rmsnorm_bwd, "adamw": case_adamw, "quantize": case_quantize, "strided_copy": case_strided_copy, "moe_local": case_moe_local,
          "residual_norm": case_residual_norm, "gated_norm": case_gated_norm, "gated_mlp": case_gated_mlp,
-         "gated_mlp_few": lambda: case_gated_mlp(24), "gated_mlp_shared": lambda: case_gated_mlp(16384, 4096, 1024)}
+         "gated_mlp_few": lambda: case_gated_mlp(24), "gated_mlp_shared": lambda: case_gated_mlp(16384, 4096, 1024),
+         "packed_attention": case_packed_attention, "paged_attention": case_paged_attention,
+         "paged_attention_e4m3": lambda: case_paged_attention(True), "paged_cache": case_paged_cache}
 
 if __name__ == "__main__":
     name = sys.argv[1] if len(sys.argv) > 1 else ""
