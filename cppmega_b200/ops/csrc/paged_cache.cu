@@ -11,16 +11,17 @@
 // Both are copies: bytes in and out at the memory's rate is all there is.  A row belongs to 8 or 16 lanes, 16 bytes of it to each (8 of an
 // E4M3 row), so rows of any stride move in whole sectors, and four rows of every lane group are in flight at once.  Measured: 4095 tokens of 32
 // heads, 128 + 64 wide in bf16: write 22 us, read 16 (15 each at the copy rate, though much of it stays in L2); 16384 tokens of 8 heads, 128 + 128 into
-// E4M3: write 35 us of 16 (67 % of the instructions that an SM can issue: a row's maximum, the exponent, two conversions a pair), back 20 of 16.
+// E4M3: write 26 us of 16 (issue slots: a row's maximum, its exponent, four instructions a pair of values), back 20 of 16.
 //
 // Of tokens that are given the same slot the last one stays, whatever order the blocks run in: each block looks for its own slots among the
-// later tokens (a hash table of its own in shared memory).  It reads the list of slots once per block, 5 % of the bytes that move at 16384
-// tokens of 8 heads.
+// later tokens (a hash table of its own in shared memory, slots of one place in a chain).  It reads the list of slots once per block: 4 us of the
+// 26 at 16384 tokens of 8 heads, 10 of 98 at 65536.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <type_traits>
 
+#include "fp32_pair.cuh"
 #include "paged.cuh"
 
 namespace cm {
@@ -29,7 +30,7 @@ namespace paged {
 constexpr int THREADS = 256;
 constexpr int MAX_TOKENS = 128;              // tokens of one block
 constexpr int TABLE = 2048;                  // places of the hash table
-constexpr int FREE = -1, SHARED = -2;        // a place that no slot, or more than one, falls to
+constexpr int NONE = -1;                     // a place that no slot falls to, the end of a chain
 constexpr int ROWS_AHEAD = 4;
 constexpr int SCAN = 8;                      // later slots that a thread has on their way at once
 
@@ -96,16 +97,16 @@ __device__ __forceinline__ int exponent_byte(float amax) {
   return e < 1 ? 1 : e;                      // at most 254 - 8 + 1
 }
 
-// eight values times a power of two as E4M3; infinities and NaN (of which a row that has any says so) become NaN
-template <typename T>
-__device__ __forceinline__ uint2 quantised(const uint4& v, float inv, bool all_finite) {
+// eight values times a power of two as E4M3; infinities and NaN (which a warp's rows have or have not) become NaN
+template <typename T, bool FINITE>
+__device__ __forceinline__ uint2 quantised(const uint4& v, float inv) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   uint32_t out[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = two<T>(w[i]);
-    uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(f.x * inv, f.y * inv), __NV_SATFINITE, __NV_E4M3);
-    if (!all_finite) {
+    uint32_t b = __nv_cvt_float2_to_fp8x2(pr_get(pr(f.x, f.y) * pr(inv)), __NV_SATFINITE, __NV_E4M3);
+    if (!FINITE) {
       if (!isfinite(f.x)) b = (b & 0xff00u) | 0x7fu;
       if (!isfinite(f.y)) b = (b & 0x00ffu) | 0x7f00u;
     }
@@ -181,9 +182,9 @@ __device__ __forceinline__ void write_rows(const Side& d, const Divide& by_heads
 #pragma unroll
       for (int o = LANES >> 1; o > 0; o >>= 1) most = max2(most, __shfl_xor_sync(0xffffffffu, most, o));
       most = max(most & 0xffffu, most >> 16);
-      const bool all_finite = most < first_not_finite<T>();
+      const bool finite = __all_sync(0xffffffffu, most < first_not_finite<T>());             // all values of the warp's rows
       float m = two<T>(most).x;
-      if (!__all_sync(0xffffffffu, all_finite)) {             // the row's largest finite one
+      if (!finite) {                                          // the row's largest finite one
         m = largest_finite<T>(v[u][0]);
         if (PIECES == 2) m = fmaxf(m, largest_finite<T>(v[u][PIECES - 1]));
 #pragma unroll
@@ -193,9 +194,10 @@ __device__ __forceinline__ void write_rows(const Side& d, const Divide& by_heads
       const int e = exponent_byte(m);
       if (exists) {
         const float inv = __uint_as_float((254u - e) << 23);  // 2^(127 - e): a subnormal for e = 254 alone, which exponent_byte does not reach
-        const uint2 y = quantised<T>(v[u][0], inv, all_finite);
+        const uint2 y = finite ? quantised<T, true>(v[u][0], inv) : quantised<T, false>(v[u][0], inv);
         if (PIECES == 2) {
-          const uint2 z = quantised<T>(v[u][PIECES - 1], inv, all_finite);
+          const uint4& w = v[u][PIECES - 1];
+          const uint2 z = finite ? quantised<T, true>(w, inv) : quantised<T, false>(w, inv);
           *reinterpret_cast<uint4*>(row) = make_uint4(y.x, y.y, z.x, z.y);
         } else {
           *reinterpret_cast<uint2*>(row) = y;
@@ -208,13 +210,14 @@ __device__ __forceinline__ void write_rows(const Side& d, const Divide& by_heads
 
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(THREADS, 4) cache_write_kernel(const WriteArgs a) {
-  __shared__ int table[TABLE];               // hash place -> token of this block
+  __shared__ int table[TABLE];               // hash place -> a token of this block
+  __shared__ int next[MAX_TOKENS];           // -> another one whose slot falls to the same place
   __shared__ long long own[MAX_TOKENS];      // the slot, or -1: not written
   __shared__ long long base[2][MAX_TOKENS];  // and where it begins in the caches
   __shared__ int lost[MAX_TOKENS];           // a later token has the same slot
   const long long t0 = (long long)blockIdx.x * a.per_block;
   const int n = (int)min((long long)a.per_block, a.T - t0);
-  for (int i = threadIdx.x; i < TABLE; i += THREADS) table[i] = FREE;
+  for (int i = threadIdx.x; i < TABLE; i += THREADS) table[i] = NONE;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += THREADS) {
     long long s = slot_of(a, t0 + i);
@@ -225,7 +228,7 @@ __global__ void __launch_bounds__(THREADS, 4) cache_write_kernel(const WriteArgs
     own[i] = s < 0 ? -1 : s;
     lost[i] = 0;
     if (s >= 0) {
-      if (atomicCAS(&table[place_of(s)], FREE, i) != FREE) table[place_of(s)] = SHARED;
+      next[i] = atomicExch(&table[place_of(s)], i);
       const long long page = s / a.page, in = s - page * a.page;
       for (int w = 0; w < a.sides; ++w) base[w][i] = page * a.side[w].c_page + in * a.side[w].c_tok;
     }
@@ -237,13 +240,9 @@ __global__ void __launch_bounds__(THREADS, 4) cache_write_kernel(const WriteArgs
     for (int c = 0; c < SCAN; ++c) s[c] = t + c * THREADS < a.T ? slot_of(a, t + c * THREADS) : -1;
 #pragma unroll
     for (int c = 0; c < SCAN; ++c) {
-      const int at = s[c] < 0 ? FREE : table[place_of(s[c])], before = (int)min((long long)n, t + c * THREADS - t0);
-      if (at >= 0) {
+      const int before = (int)min((long long)n, t + c * THREADS - t0);
+      for (int at = s[c] < 0 ? NONE : table[place_of(s[c])]; at != NONE; at = next[at])
         if (at < before && own[at] == s[c]) lost[at] = 1;
-      } else if (at == SHARED) {
-        for (int i = 0; i < before; ++i)
-          if (own[i] == s[c]) lost[i] = 1;
-      }
     }
   }
   __syncthreads();
