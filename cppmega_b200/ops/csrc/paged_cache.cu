@@ -324,6 +324,12 @@ __global__ void __launch_bounds__(THREADS, 6) cache_read_kernel(const ReadArgs a
   __shared__ long long base[2][MAX_TOKENS];  // and where it begins in the caches
   const long long t0 = (long long)blockIdx.x * a.per_block;
   const int n = (int)min((long long)a.per_block, a.T - t0);
+  if (blockIdx.x == 0)                       // ends that do not rise from 0 to at most T are reported; no row comes from outside the cache for them
+    for (int i = threadIdx.x; i <= a.sequences; i += THREADS) {
+      const int end = __ldg(a.ends + i);
+      if ((i == 0 ? end != 0 : end < __ldg(a.ends + i - 1)) || end > a.T)
+        if (a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
+    }
   for (int i = threadIdx.x; i < n; i += THREADS) {
     const int t = (int)t0 + i;
     int lo = 0, hi = a.sequences;            // the last sequence that begins at or before t

@@ -580,8 +580,8 @@ def cache_read(k_cache, v_cache, block_table, cu_seqlens, total: int, k_scale=No
     ``s`` gives its tokens ``0 .. cu_seqlens[s + 1] - cu_seqlens[s] - 1`` to the rows from ``cu_seqlens[s]`` on (int32 [n + 1], from 0),
     token ``p`` from place ``p % page`` of page ``block_table[s, p // page]`` (int32 [n, columns]); rows behind the last sequence are zeros.
     ``v_cache`` may be None (then so is the second result).  ``dtype``: type of the rows (bf16 by default out of an E4M3 cache, whose
-    rows are multiplied by their powers of two; a 16-bit cache keeps its own).  Pages outside the cache give rows of zeros and are reported
-    by ``ops.cuda.check_errors``."""
+    rows are multiplied by their powers of two; a 16-bit cache keeps its own).  Pages outside the cache give rows of zeros; they, and ends
+    that do not rise from 0 to at most ``total``, are reported by ``ops.cuda.check_errors``."""
     layout = layout_of("cache_read", k_cache, v_cache, block_table, cu_seqlens, k_scale, v_scale)
     if layout not in _CHECKED:
         _check_cache("cache_read", k_cache, v_cache, k_scale, v_scale)

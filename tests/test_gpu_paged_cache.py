@@ -464,6 +464,14 @@ def test_lengths_outside_the_table_are_reported(n):
     assert got.isfinite().all()
 
 
+@pytest.mark.parametrize("ends", [[0, 40, 30], [0, 40, 89], [1, 40, 80], [-3, 40, 80], [0, 2 ** 31 - 1, 80], [0, 40, -2 ** 31]])
+def test_read_with_ends_that_do_not_hold_is_reported(ends):
+    kc, vc = _randn(5, 16, 2, 64), _randn(5, 16, 2, 64, seed=1)
+    k, v = F_.cache_read(kc, vc, _i32([[1, 4, 3], [0, 2, 4]]), _i32(ends), 88)
+    _reported()
+    assert k.isfinite().all() and v.isfinite().all()
+
+
 @pytest.mark.parametrize("slot", [32, 2 ** 40])
 def test_slots_behind_the_cache_are_skipped_and_reported(slot):
     kc = torch.zeros(2, 16, 1, 8, dtype=torch.bfloat16, device="cuda")
