@@ -130,6 +130,11 @@ struct Ring {
   }
 };
 
+// setup_barrier, where warp 0 looks for the block's tile: another warp reads the error word meanwhile
+__device__ __forceinline__ bool set_up(const int* err) {
+  return __syncthreads_or(threadIdx.x == 64 && err && *reinterpret_cast<const volatile int*>(err) != 0);
+}
+
 // ---- sequences -------------------------------------------------------------------------------------------------------
 struct Args {
   const int *cu_q, *cu_k;
@@ -392,7 +397,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tma_prefetch_desc(&tmV);
   }
   tc_fence_before();
-  const bool drain = setup_barrier(a.err);
+  const bool drain = set_up(a.err);
   tc_fence_after();
   const uint32_t tmem = sh->tmem_slot;       // S_t at 128 t, one half of it after the other, P over the half it came from; O_t at 256 + DV t
   const Unit unit = sh->unit;
@@ -823,7 +828,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
   if (warp == MMA_WARP) { tmem_alloc(&sh->tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before();
-  const bool drain = setup_barrier(a.err);
+  const bool drain = set_up(a.err);
   tc_fence_after();
   const uint32_t tmem = sh->tmem_slot;       // S at 0, dP at 128 (halves of 64 columns, dS over those of dP), dQ at 256; Q at 384, dO at 448
   const Unit unit = sh->unit;
@@ -1115,7 +1120,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     fence_proxy_async_smem();
   }
   tc_fence_before();
-  const bool drain = setup_barrier(a.err);
+  const bool drain = set_up(a.err);
   tc_fence_after();
   const uint32_t tmem = sh->tmem_slot;       // S' at 0 (P' over it), dP' at 128 (dS' over it), dV at 256, dK at 384
   const Unit unit = sh->unit;
