@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
   constexpr bool MB = F::MMA_BF16;
   constexpr int VT = DV / 16;                                 // 16-column tiles of the result
   extern __shared__ __align__(128) uint8_t smem_raw[];
+  few::wait_for_input();                     // by every block, and before the next kernel may start: it counts on all older kernels having ended
   few::let_next_start();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, row8 = lane >> 2;
   const int worker = blockIdx.x * F::WARPS + warp, lanes_of_run = a.side * a.tiles, run = worker / lanes_of_run;
@@ -683,7 +684,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const Args a, int
   const int steps = steps_of(length_of(a, b, bad)), chunk = h / a.side;
   const long long s0 = before * a.chunks + (long long)chunk * steps;
   const int r0 = (int)(s0 / q), r1 = steps ? (int)((s0 + steps - 1) / q) : r0;
-  few::wait_for_input();                     // by every block: the next kernel of the stream counts on this one having waited
+  few::wait_for_input();                     // by every block, as above
+  few::let_next_start();
   if (steps && r0 == r1) return;             // finished by the one run that holds it
 
   float top = -INFINITY, sum = 0.f, acc[C];
@@ -792,8 +794,8 @@ int start(const Args& a, int grid, cudaStream_t stream) {
       if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -2;
       cfg.done();
     }
-    kern<<<grid, F::WARPS * 32, smem, stream>>>(a);
-    if (cudaGetLastError() != cudaSuccess) return -3;
+    // set up while the kernel before it ends (48 sequences of 500 to 8000, 32 heads on one row, call after call: 27 us, 29 without)
+    if (few::launch_early(kern, dim3(grid), dim3(F::WARPS * 32), smem, stream, a)) return -3;
   }
   // few blocks have many pieces each: 16 warps read them side by side (131071 tokens, 222 pieces,
   // both kernels: 95 us, 107 with 8 warps); many blocks have few
