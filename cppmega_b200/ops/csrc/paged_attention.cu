@@ -27,10 +27,10 @@
 //
 // The reference value of a head's softmax follows its maximum only when that has grown by 2^8, so that accumulators are rarely rescaled.
 //
-// Measured, both kernels: bf16, one sequence of 131071 tokens, 64 heads over 8, 128 wide 94 us (82 at the copy rate; 64 sequences of 8192 tokens, 32
-// heads over 8: 6.7 TB/s).  E4M3, 64 sequences of 100 to 16000 tokens, 32 heads over 8: 102 us (63 at the copy rate; 5.0 TB/s at 16384 each): half
+// Measured, both kernels: bf16, one sequence of 131071 tokens, 64 heads over 8, 128 wide 93 us (82 at the copy rate; 64 sequences of 8192 tokens, 32
+// heads over 8: 6.7 TB/s).  E4M3, 64 sequences of 100 to 16000 tokens, 32 heads over 8: 100 us (63 at the copy rate; 5.0 TB/s at 16384 each): half
 // the bytes of a key, the same chain of steps, and the conversions.  Short calls are set-up (the lengths, the table, the first rows: 5 us) and the
-// second kernel: 1000 tokens 9.5 us in a graph.
+// second kernel: 1000 tokens 9.1 us in a graph.
 #include <cuda_fp16.h>
 
 #include "few_rows.cuh"
