@@ -117,7 +117,8 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout) -> bool
     if rc:
         _failed("cm_cache_write", rc)
     F_.count_launch("cache_write")
-    increment_version([t for t in (k_cache, v_cache, k_scale, v_scale) if t is not None])        # whoever saved them for a gradient is told
+    # whoever saved them for a gradient is told (tensors of inference mode cannot be saved and have no count)
+    increment_version([t for t in (k_cache, v_cache, k_scale, v_scale) if t is not None and not t.is_inference()])
     return True
 
 

@@ -416,6 +416,10 @@ def test_a_cache_that_was_saved_for_a_gradient_and_written():
         a, b = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
         F_.cache_write(_randn(1, 2, 64), _randn(1, 2, 64), a, b, torch.tensor([3], device="cuda"))
         assert a.abs().sum() > 0
+    F_.cache_write(_randn(1, 2, 64), _randn(1, 2, 64), a, b, torch.tensor([9], device="cuda"))       # and outside of that mode
+    assert a.view(32, -1).abs().sum(1).nonzero().flatten().tolist() == [3, 9]
+    q = _randn(1, 4, 64)
+    assert F_.paged_attention(q, a, b, _i32([[0]]), _i32([10]), 0.1).isfinite().all()
 
 
 @pytest.mark.parametrize("scale", [math.inf, math.nan])
