@@ -43,8 +43,13 @@
 // within 1 % and takes 20 % more of the forward's time.)  delta takes o before its rounding (the forward keeps what that takes away, in 16 bits
 // more).  Both because an error of o is added to every ds of a row with one sign: dq and dk of rows that settle on few keys are off by 2.45e-3 of
 // their norms, where the roundings of dS and of the result itself make 2.4e-3; 3.0e-3 with the sum of unrounded weights, 4.0e-3 with the
-// rounded o too.  Maxima, sums, scores, deltas and all accumulators are fp32.  fp16's range is too short for dS of any size: it is scaled by a
-// power of two, from the row's largest |do| for dq, from the call's for dk.
+// rounded o too.  Maxima, sums, scores, deltas and all accumulators are fp32.
+//
+// fp16's range is too short for p and dS of any size: both are scaled by powers of two to all of it.  p <= 1 counts 2^14 times.  do v' and delta,
+// an average of them, are at most |do| max |v| (Euclidean norms, the keys of the row's sequence and key head), so dS is below 2^14 with the power
+// that brings twice that bound under one: |do| is the row's own for dq, and for dk, whose sum goes over rows, the largest of the sequence and key
+// head.  A factor of nearly four is left below 65504 for what roundings add, and what falls below the range is less than 2^-37 of |do| max |v|.  No
+// sequence and no key head depends on another's gradients.
 #include <cuda_fp16.h>
 
 #include "few_rows.cuh"
@@ -153,13 +158,15 @@ struct Args {
   long long go_tok, go_head;
   float* lse;                                // [T, heads]: log2 of the sum of weights; +inf without keys; null: not wanted
   float* delta;                              // [T, heads]
-  float* big;                                // [T, heads]: largest |do| of a row (fp16)
-  uint32_t* top;                             // largest |do| of the call as bits (fp16)
+  const void* v;                             // backward in fp16, for the bounds of dS: the values with their strides
+  long long v_tok, v_head;
+  float* big;                                // [T, heads]: |do| of a row
+  uint32_t *top, *vtop;                      // [sequences, kv_heads]: the largest finite |do| and |v|, as bits
   int* err;
 };
 
 struct Unit {
-  int place, total;                          // place of the tile in its sequence; tiles of all sequences
+  int seq, place, total;                     // sequence; place of the tile in it; tiles of all sequences
   int q0, L, k0, Lk;                         // the sequence's queries and keys
   int bad;
 };
@@ -228,6 +235,7 @@ __device__ Unit find_unit(const Args& a, bool of_keys, int per, int u, int lane)
     }
     rank -= __popc(has);
   }
+  r.seq = seq;
   if (seq < 32) {
     r.q0 = __shfl_sync(0xffffffffu, q0, seq); r.L = __shfl_sync(0xffffffffu, L, seq);
     r.k0 = __shfl_sync(0xffffffffu, k0, seq); r.Lk = __shfl_sync(0xffffffffu, Lk, seq);
@@ -720,10 +728,35 @@ __global__ void __launch_bounds__(TILE) packed_join_kernel(const Args a) {
 }
 
 // ---- backward: delta -----------------------------------------------------------------------------------------------------
-// delta[i] = do[i] . o[i] before its rounding, in fp16 also the row's largest |do| and the call's.  DV / 8 lanes a row, four rows of a lane on their way
-// at once: three reads of a row's width at the memory's rate.  Inside the dq kernel, whose blocks have an SM to themselves, nothing would
+// delta[i] = do[i] . o[i] before its rounding, in fp16 also |do| of the row and the largest of its sequence and key head.  DV / 8 lanes a row, four rows of a
+// lane on their way at once: three reads of a row's width at the memory's rate.  Inside the dq kernel, whose blocks have an SM to themselves, nothing would
 // run meanwhile (9000 cycles a block, 120 us at 16384 x 32 rows of 128; here 71).
 constexpr int DELTA_THREADS = 256, DELTA_AHEAD = 4;
+
+// the last sequence that begins at or before row `tok`, of n > 0
+__device__ __forceinline__ int sequence_of(const int* cu, int n, int tok) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(cu + mid) <= tok) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+// The largest is the same in any order.  Most rows are not above what they find there.
+__device__ __forceinline__ void raise_to(uint32_t* at, float x) {
+  const uint32_t bits = __float_as_uint(x);
+  if (isfinite(x) && bits > *reinterpret_cast<const volatile uint32_t*>(at)) atomicMax(at, bits);
+}
+// 2^14 p is rounded to fp16, and p (do v' - delta) with it
+constexpr float P_UP = 14.f, P_DOWN = 1.f / 16384;
+// For 2 `bound` in [2^e, 2^(e + 1)): the power 2^-(e + 1), under which it is in [1/2, 1), and its inverse
+__device__ __forceinline__ void powers_for(float bound, float& up, float& down) {
+  const int e = int(__float_as_uint(2.f * bound) >> 23) - 127;
+  const bool usable = bound > 0.f && e > -100 && e < 100;     // |do| and |v| of fp16 rows: 2^-47 to 2^41
+  up = usable ? __uint_as_float(uint32_t(126 - e) << 23) : 1.f;
+  down = usable ? __uint_as_float(uint32_t(128 + e) << 23) : 1.f;
+}
 
 template <bool HALF, int LANES>
 __global__ void __launch_bounds__(DELTA_THREADS, 4) packed_delta_kernel(const Args a) {
@@ -746,7 +779,6 @@ __global__ void __launch_bounds__(DELTA_THREADS, 4) packed_delta_kernel(const Ar
       y[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.go) + tok * a.go_tok + head * a.go_head) + piece);
     }
   }
-  float most = 0.f;
 #pragma unroll
   for (int i = 0; i < DELTA_AHEAD; ++i) {
     const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, zs[4] = {z[i].x, z[i].y, z[i].z, z[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
@@ -755,23 +787,54 @@ __global__ void __launch_bounds__(DELTA_THREADS, 4) packed_delta_kernel(const Ar
     for (int e = 0; e < 4; ++e) {
       const float2 f = unpair<HALF>(xs[e]), h = unpair<HALF>(zs[e]), g = unpair<HALF>(ys[e]);
       dot = fmaf(f.x + h.x, g.x, fmaf(f.y + h.y, g.y, dot));
-      if (HALF) big = fmaxf(big, fmaxf(fabsf(g.x), fabsf(g.y)));
+      if (HALF) big = fmaf(g.x, g.x, fmaf(g.y, g.y, big));
     }
 #pragma unroll
     for (int o = LANES >> 1; o > 0; o >>= 1) {
       dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      if (HALF) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      if (HALF) big += __shfl_xor_sync(0xffffffffu, big, o);
     }
     const long long row = row0 + i * ROWS;
     if (piece == 0 && row < rows) {
       a.delta[row] = dot;
-      if (HALF) a.big[row] = big;
+      if (HALF) {
+        big = sqrtf(big);
+        a.big[row] = big;
+        const unsigned more = (head0 + i * ROWS) / unsigned(a.heads), head = head0 + i * ROWS - more * a.heads;
+        raise_to(a.top + (long long)sequence_of(a.cu_q, a.n, int(tok0 + more)) * a.kv_heads + head / unsigned(a.heads / a.kv_heads), big);
+      }
     }
-    if (HALF && isfinite(big)) most = fmaxf(most, big);
   }
-  if (HALF) {                                // the largest is the same in any order
-    const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-    if ((threadIdx.x & 31) == 0 && all) atomicMax(a.top, all);
+}
+
+// fp16: the largest |v| of each sequence and key head.  Rows as above.
+template <int LANES>
+__global__ void __launch_bounds__(DELTA_THREADS) packed_sizes_kernel(const Args a) {
+  constexpr int ROWS = DELTA_THREADS / LANES;
+  const int piece = threadIdx.x % LANES;
+  const long long rows = (long long)min(max(__ldg(a.cu_k + a.n), 0), a.Tk) * a.kv_heads;
+  const long long row0 = (long long)blockIdx.x * (ROWS * DELTA_AHEAD) + threadIdx.x / LANES;
+  uint4 x[DELTA_AHEAD];
+#pragma unroll
+  for (int i = 0; i < DELTA_AHEAD; ++i) {
+    const long long row = row0 + i * ROWS, tok = row / a.kv_heads, head = row - tok * a.kv_heads;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (row < rows && piece * 8 < a.vdim)
+      x[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.v) + tok * a.v_tok + head * a.v_head) + piece);
+  }
+#pragma unroll
+  for (int i = 0; i < DELTA_AHEAD; ++i) {
+    const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    float big = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpair<true>(xs[e]);
+      big = fmaf(f.x, f.x, fmaf(f.y, f.y, big));
+    }
+#pragma unroll
+    for (int o = LANES >> 1; o > 0; o >>= 1) big += __shfl_xor_sync(0xffffffffu, big, o);
+    const long long row = row0 + i * ROWS, tok = row / a.kv_heads;
+    if (piece == 0 && row < rows) raise_to(a.vtop + (long long)sequence_of(a.cu_k, a.n, int(tok)) * a.kv_heads + (row - tok * a.kv_heads), sqrtf(big));
   }
 }
 
@@ -947,7 +1010,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int last = mine ? off + pos : -1, head = head0 + (r - tok * a.hb);
     const long long at = (long long)(q0 + pos) * a.heads + head;
     const float delta = mine ? a.delta[at] : 0.f;
-    const float lse = mine ? a.lse[at] : INFINITY;
+    const float lse = (mine ? a.lse[at] : INFINITY) - (HALF ? P_UP : 0.f);
     const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
     bool ok = n == 0 || warp_wait(&sh->q_full, 0, abort_flag, a.err, ERR_WAIT_FULL);
     if (ok && n > 0) {                       // half a row from each of its two threads
@@ -968,14 +1031,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->rows_in);
     }
-    float up = 1.f, down = 1.f;              // fp16: the power of two that brings the row's largest |do| to 2^-4
+    float up = 1.f, down = 1.f;              // fp16: of the row's own bound
     if (HALF) {
-      const float big = mine ? a.big[at] : 0.f;
-      if (big > 0.f && isfinite(big)) {
-        const int e = 127 - 4 - int(__float_as_uint(big) >> 23);
-        up = __uint_as_float(uint32_t(127 + e) << 23);
-        down = __uint_as_float(uint32_t(127 - e) << 23);
-      }
+      powers_for(mine ? a.big[at] * __uint_as_float(a.vtop[(long long)unit.seq * a.kv_heads + kvh]) : 0.f, up, down);
+      down *= P_DOWN;
     }
     const float delta_up = delta * up;
     auto tile = [&](int j, auto where) {
@@ -1142,14 +1201,11 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int q_tiles = (L + a.tok - 1) / a.tok, q_first = max(0, key0 - off) / a.tok;
   const int per_chunk = max(0, q_tiles - q_first), n = per_chunk * a.chunks;
   auto tile_of = [&](int i) { return q_tiles - 1 - i % per_chunk; };          // query tile of step i, the last one first
-  float up = 1.f, down = 1.f;                // power of two that brings the call's largest |do| to 2^-4
+  float up = 1.f, down = 1.f;                // fp16: of the bound of the sequence and key head
   if (HALF) {
-    const uint32_t top = *a.top;
-    if (top) {
-      const int e = 127 - 4 - int(top >> 23);
-      up = __uint_as_float(uint32_t(127 + e) << 23);
-      down = __uint_as_float(uint32_t(127 - e) << 23);
-    }
+    const long long at = (long long)unit.seq * a.kv_heads + kvh;
+    powers_for(__uint_as_float(a.top[at]) * __uint_as_float(a.vtop[at]), up, down);
+    down *= P_DOWN;
   }
 
   if (warp == TMA_WARP) {
@@ -1178,7 +1234,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const int r = c * 32 + lane, tok = r * a.by_hb >> 16, pos = first + tok;
         const bool mine = r < rows && pos < L;
         const long long at = (long long)(q0 + pos) * a.heads + head0 + (r - tok * a.hb);
-        lse[c] = mine ? -__ldg(a.lse + at) : -INFINITY;
+        lse[c] = mine ? (HALF ? P_UP : 0.f) - __ldg(a.lse + at) : -INFINITY;
         delta[c] = mine ? __ldg(a.delta + at) * -up : 0.f;
       }
 #pragma unroll
@@ -1341,6 +1397,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (k) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * (a.scale * down));
+        } else if (HALF) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * P_DOWN);
         }
         put_columns<HALF>(k ? stage : stage + F::KS * SLAB, r, col, x);
       }
@@ -1456,11 +1515,15 @@ int backward(const Inputs& in, Args a, void* dq, void* dk, void* dv, cudaStream_
   if (rc) return rc;
   const long long uq = units_of(a.T, a.n, a.tok), uk = units_of(a.Tk, a.n, TILE);
   if (uq * a.kv_heads * a.chunks > 0x7fffffffLL || uk * a.kv_heads > 0x7fffffffLL) return -10;
-  if (HALF && cudaMemsetAsync(a.top, 0, sizeof(uint32_t), stream) != cudaSuccess) return -3;
   {
     constexpr int LANES = DV / 8, ROWS = DELTA_THREADS / LANES * DELTA_AHEAD;
-    const long long blocks = ((long long)a.T * a.heads + ROWS - 1) / ROWS;
-    if (blocks > 0x7fffffffLL) return -10;
+    const long long blocks = ((long long)a.T * a.heads + ROWS - 1) / ROWS, v_blocks = ((long long)a.Tk * a.kv_heads + ROWS - 1) / ROWS;
+    if (blocks > 0x7fffffffLL || v_blocks > 0x7fffffffLL) return -10;
+    if (HALF) {
+      if (cudaMemsetAsync(a.top, 0, 2 * sizeof(uint32_t) * a.n * a.kv_heads, stream) != cudaSuccess) return -3;
+      packed_sizes_kernel<LANES><<<(unsigned)v_blocks, DELTA_THREADS, 0, stream>>>(a);
+      if (cudaGetLastError() != cudaSuccess) return -3;
+    }
     packed_delta_kernel<HALF, LANES><<<(unsigned)blocks, DELTA_THREADS, 0, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return -3;
   }
@@ -1522,7 +1585,7 @@ extern "C" int cm_packed_attention_fwd(const void* q, const void* k, const void*
   return a.dim > 64 ? forward<true, 128, 64>(in, a, stream) : forward<true, 64, 64>(in, a, stream);
 }
 
-// o, o_rest and lse from the forward; go (the gradient of o) [T, heads, vdim]; delta: scratch of T * heads floats, fp16: 2 T heads + 1;
+// o, o_rest and lse from the forward; go (the gradient of o) [T, heads, vdim]; delta: scratch of T * heads floats, fp16: 2 (T heads + sequences kv_heads);
 // dq [T, heads, dim], dk [Tk, kv_heads, dim], dv [Tk, kv_heads, vdim] packed, all written whole
 extern "C" int cm_packed_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* go, const int* cu_q,
                                        const int* cu_k, const float* lse, float* delta, void* dq, void* dk, void* dv, const long long* n, float scale,
@@ -1536,6 +1599,8 @@ extern "C" int cm_packed_attention_bwd(const void* q, const void* k, const void*
   a.delta = delta;
   a.big = delta + (long long)a.T * a.heads;
   a.top = reinterpret_cast<uint32_t*>(a.big + (long long)a.T * a.heads);
+  a.vtop = a.top + (long long)a.n * a.kv_heads;
+  a.v = v; a.v_tok = n[4]; a.v_head = n[5];
   const Inputs in = {q, k, v, go, n, n + 2, n + 4, n + 6};
   if (n[15] == 0) {
     if (a.vdim > 64) return backward<false, 128, 128>(in, a, dq, dk, dv, stream);

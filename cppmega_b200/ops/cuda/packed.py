@@ -63,7 +63,7 @@ def _plan_backward(dt, q, k, v, cu_q, cu_k, o, rest, lse, go):
             and all(t.is_contiguous() and t.device == go.device for t in (cu_q, cu_k, o, rest, lse))
             and cu_q.dtype == cu_k.dtype == torch.int32 and lse.dtype == torch.float32):
         return False
-    return Plan(_numbers(q, k, v, cu_q, go), work=lse.numel() if dt == torch.bfloat16 else 2 * lse.numel() + 1)
+    return Plan(_numbers(q, k, v, cu_q, go), work=lse.numel() if dt == torch.bfloat16 else 2 * (lse.numel() + (cu_q.numel() - 1) * k.shape[1]))
 
 
 def _forward(plan, q, k, v, cu_q, cu_k, scale, keep):
@@ -111,7 +111,7 @@ class PackedAttentionFn(torch.autograd.Function):
             _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
         if rc:
             _failed("cm_packed_attention_bwd", rc)
-        F_.count_launch("packed_attention_bwd", 3)
+        F_.count_launch("packed_attention_bwd", 3 if ctx.dtype == torch.bfloat16 else 4)
         return dq, dk, dv, None, None, None, None
 
 
