@@ -19,7 +19,8 @@
 // exchange find their eight lanes in eight banks; the weights alone are transposed, 8 x 8 at a time.
 // E4M3 becomes fp16 in one conversion per two values, exactly; the query is scaled to fp16's range by a power of two per head, the key's power
 // goes into the score, and the value's power into the exponent of its weight, whose reference is a maximum of its own: weights never leave
-// fp16's range, whatever the powers are.
+// fp16's range, whatever the powers are.  A row of zeros has no power (its byte says 1): it sets no reference, under which the weights of the
+// others would fall out of the range (a key far above the rest whose values are zero and theirs 0.05: the result was off by a quarter).
 // Weights are rounded to the type of the products (bf16 or fp16: half a step of the result's own type, averaged over the keys).  Over a 16-bit cache
 // the sum that divides the result is that of the rounded weights: a row that settles on few keys does not take their rounding into its result
 // (1000 keys, one in fifty three times as large: off by 1.7e-3 of its norm, 2.3e-3 with the sum of the others).  Over an E4M3 cache the weights that are rounded have the
@@ -569,7 +570,35 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
           grown |= topv[x][c] > mv[x][c] + RESCALE_AT;
         }
       }
+    const uint32_t vb = base + KEYS * F::K_ROW +
+                        (F::V_BYTES == 16 ? (quad * 8 + (row8 ^ (2 * quad))) * 16 : ((row8 >> 2) * 8 + quad * 2 + (row8 >> 1 & 1)) * 16 + (row8 & 1) * 8);
     if (__any_sync(0xffffffffu, grown)) {
+      if (E4M3) {                                             // rows of zeros: weight 0, no reference
+        unsigned some = 0;                                    // a bit for each key that has values
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {                         // keys 2 quad, + 1, + 8, + 9
+          uint32_t any = 0;
+#pragma unroll
+          for (int j = 0; j < F::V_PIECES; ++j) {
+            const uint32_t ad = vb + (y * F::V_PIECES + j) * 32 * F::V_BYTES;
+            if (F::V_BYTES == 16) {
+              const uint4 v = lds16(ad);
+              any |= v.x | v.y | v.z | v.w;
+            } else {
+              const uint2 v = lds8(ad);
+              any |= v.x | v.y;
+            }
+          }
+          some |= unsigned((any & 0x7f7f7f7fu) != 0) << (2 * quad + (y & 1) + (y >> 1) * 8);
+        }
+        some = __reduce_or_sync(0xffffffffu, some);
+        if (!(some >> row8 & 1)) vlog[0] = -INFINITY;
+        if (!(some >> (row8 + 8) & 1)) vlog[1] = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) topv[x][c] = fmaxf(s[x][c] + vlog[0], s[x][2 + c] + vlog[1]);
+      }
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -614,8 +643,6 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
     }
 
     // ---- values times weights ----
-    const uint32_t vb = base + KEYS * F::K_ROW +
-                        (F::V_BYTES == 16 ? (quad * 8 + (row8 ^ (2 * quad))) * 16 : ((row8 >> 2) * 8 + quad * 2 + (row8 >> 1 & 1)) * 16 + (row8 & 1) * 8);
 #pragma unroll
     for (int j = 0; j < F::V_PIECES; ++j) {
       uint32_t r[4][4];                                       // keys 2 quad, + 1, + 8, + 9
