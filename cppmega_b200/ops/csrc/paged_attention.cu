@@ -282,13 +282,17 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
   const uint8_t *k_row = k_lane, *v_row = v_lane;             // aligned: this lane's first rows of the step
   long long scale_row = 0;                                    // and the place of its first key's exponents
   bool turned = true;                                         // the step lies in another page than the one before
+  bool holes = false;                                         // pages outside the cache have been met
   auto issue = [&](int stage) {
     if (left > 0) {
       const int head = to.c * a.side + side, room = to.len - to.step * KEYS;          // key head; keys of the step
       const bool known = page >= 0 && page < a.pages;
       const uint32_t k_to = ring_s + stage * F::STAGE + k_dst, v_to = ring_s + stage * F::STAGE + KEYS * F::K_ROW;
       if (a.aligned) {
-        if (!known && a.err && lane == 0) atomicCAS(a.err, 0, ERR_BAD_ARG);
+        if (!known) {
+          holes = true;
+          if (a.err && lane == 0) atomicCAS(a.err, 0, ERR_BAD_ARG);
+        }
         const int keys = known ? room : 0;
         if (turned) {
           k_row = k_lane + page * a.k_page + (long long)in * a.k_tok + (long long)head * a.k_head;
@@ -324,6 +328,7 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
         const long long ko = there ? page * a.k_page + (long long)in * a.k_tok + (long long)head * a.k_head : -1;
         const long long vo = there ? page * a.v_page + (long long)in * a.v_tok + (long long)head * a.v_head : -1;
         if (!known && (lane & 15) < room && a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);
+        holes |= __any_sync(0xffffffffu, !known && (lane & 15) < room);
         if (E4M3 && lane < KEYS) rows_of[stage * KEYS + lane] = there ? ((long long)page * a.page + in) * a.kv_heads + head : -1;
 #pragma unroll
         for (int i = 0; i < KC / 2; ++i) {
@@ -553,6 +558,16 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
       for (int x = 0; x < NT; ++x) {
         if (row8 >= room) s[x][0] = s[x][1] = -INFINITY;
         if (row8 + 8 >= room) s[x][2] = s[x][3] = -INFINITY;
+      }
+    }
+    if (holes) {                                              // those pages have no keys; nothing is kept for this case, the table is read again
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int pos = at.step * KEYS + row8 + 8 * u;
+        const int p = pos < at.len ? __ldg(a.table + at.b * a.table_row + pos / a.page) : 0;
+        if (p >= 0 && p < a.pages) continue;
+#pragma unroll
+        for (int x = 0; x < NT; ++x) s[x][2 * u] = s[x][2 * u + 1] = -INFINITY;
       }
     }
 

@@ -69,3 +69,47 @@ def test_a_cache_of_keys_without_values_gives_zeros():
     kc, vc, ks, vs = _caches(4, 16, 1, (64, 64), E4M3)
     F_.cache_write(_randn(50, 1, 64), torch.zeros(50, 1, 64, dtype=torch.bfloat16, device="cuda"), kc, vc, torch.arange(50, device="cuda"), ks, vs)
     assert (F_.paged_attention(_randn(1, 4, 64), kc, vc, _i32([[0, 1, 2, 3]]), _i32([50]), 0.125, ks, vs) == 0).all()
+
+
+def _reported():
+    from cppmega_b200.ops import cuda as cu
+    with pytest.raises(cu.KernelError, match="bad argument"):
+        cu.check_errors()
+    cu.check_errors()
+
+
+@pytest.mark.parametrize("bad", [-1, 40, 2 ** 31 - 1, -2 ** 31])
+@pytest.mark.parametrize("page", [16, 64, 24, 7, 1])
+@pytest.mark.parametrize("store", [torch.bfloat16, E4M3])
+def test_keys_of_pages_outside_the_cache_have_no_weight(store, page, bad):
+    """The attention over the other keys, as if those of the page were not there: pages of whole steps, of parts of steps, first, last, and all of
+    them."""
+    heads, H, D, pages = 2, 8, 64, 40
+    caches = _caches(pages, page, heads, (D, D), store)
+    n = pages * page
+    k, v = _randn(n, heads, D, std=0.3), _randn(n, heads, D, seed=1) + 2
+    F_.cache_write(k, v, caches[0], caches[1], torch.arange(n, device="cuda"), *caches[2:])
+    if store == E4M3:
+        k, v = (t.bfloat16() for t in F_.cache_read(*caches[:2], torch.arange(pages, device="cuda").int()[None], _i32([0, n]), n, *caches[2:]))
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(page)).tolist()
+    table = [[*order[:5], bad, *order[5:9]], [bad, *order[10:19]], [*order[20:28], bad, bad], [bad] * 10, order[:10]]
+    lens = [10 * page, 10 * page - page // 2, 9 * page + 1, 10 * page, 10 * page]
+    q = _randn(5, H, D, seed=2)
+    got = F_.paged_attention(q, *caches[:2], _i32(table), _i32(lens), 1.0, *caches[2:])
+    _reported()
+    kd, vd, half = k.double().view(pages, page, heads, D), v.double().view(pages, page, heads, D), 2.0 ** -8
+    for b, (row, length) in enumerate(zip(table, lens)):
+        pos = torch.arange(length, device="cuda")
+        pos = pos[torch.tensor([row[p // page] != bad for p in pos.tolist()], device="cuda")]
+        at = torch.tensor(row, device="cuda")[pos // page], pos % page
+        for h in range(H):
+            kh, vh, qh = kd[at[0], at[1], h // 4], vd[at[0], at[1], h // 4], q[b, h].double()
+            if len(pos) == 0:
+                assert (got[b] == 0).all()
+                continue
+            s = kh @ qh
+            p = torch.softmax(s, 0)
+            e = 2 * ((D + 4) * 2.0 ** -23 * (kh.abs() @ qh.abs()).amax() + 2.0 ** -22 * s.abs().amax()) + 2.0 ** -20 + 4 * length * 2.0 ** -24
+            want, size = p @ vh, p @ vh.abs()
+            bound = 2 * half * want.abs() + (1 + half) * size * (half + e) + length * 2.0 ** -15 * float(store == E4M3) * (p * vh.abs().amax(1)).amax()
+            assert ((got[b, h].double() - want).abs() <= bound).all(), float(((got[b, h].double() - want).abs() / bound).max())
