@@ -38,12 +38,12 @@ def declare(L: ctypes.CDLL) -> None:
 class Plan:
     """What a layout's calls have in common: the library's array of sizes and strides, and what else the wrapper needs."""
 
-    __slots__ = ("numbers", "at", "copy", "shape", "work", "like")
+    __slots__ = ("numbers", "at", "copy", "shape", "work", "like", "spans")
 
-    def __init__(self, numbers, copy=False, shape=None, work=0, like=False):
+    def __init__(self, numbers, copy=False, shape=None, work=0, like=False, spans=None):
         self.numbers = (ctypes.c_longlong * len(numbers))(*numbers)
         self.at = ctypes.addressof(self.numbers)
-        self.copy, self.shape, self.work, self.like = copy, shape, work, like
+        self.copy, self.shape, self.work, self.like, self.spans = copy, shape, work, like, spans
 
 
 _plans: dict = {}
@@ -97,7 +97,12 @@ def _plan_write(k, v, k_cache, v_cache, slots, k_scale, v_scale):
         return False
     return Plan([*strides(k), *strides(v, 2), *strides(k_cache), *strides(v_cache, 3), T, heads, dim, 0 if v is None else v.shape[2],
                  k_cache.shape[0], k_cache.shape[1], TYPES[k.dtype], int(q), int(slots.dtype == torch.int64)],
-                copy=not (rows_on(k, 16) and rows_on(v, 16) and slots.is_contiguous()))
+                copy=not (rows_on(k, 16) and rows_on(v, 16) and slots.is_contiguous()), spans=[F_.bytes_spanned(t) for t in (k, v, k_cache, v_cache)])
+
+
+def _meet(a, a_bytes, b, b_bytes) -> bool:
+    """Whether two ranges of memory have bytes in common."""
+    return a < b + b_bytes and b < a + a_bytes
 
 
 @_on_device
@@ -109,7 +114,10 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout) -> bool
     at, kp, vp, kcp, vcp = slots.data_ptr(), k.data_ptr(), _ptr(v), k_cache.data_ptr(), _ptr(v_cache)
     if (kcp | (vcp or 0)) & (7 if k_scale is not None else 15):
         return False
-    if plan.copy or (kp | (vp or 0)) & 15:                # a few rows
+    k_bytes, v_bytes, kc_bytes, vc_bytes = plan.spans
+    inside = _meet(kp, k_bytes, kcp, kc_bytes) or vp and (
+        _meet(kp, k_bytes, vcp, vc_bytes) or _meet(vp, v_bytes, kcp, kc_bytes) or _meet(vp, v_bytes, vcp, vc_bytes))
+    if plan.copy or inside or (kp | (vp or 0)) & 15:      # a few rows; or rows of the cache itself, read before any is overwritten
         k, v = (None if t is None else t.detach().clone(memory_format=torch.contiguous_format) for t in (k, v))
         slots = slots.contiguous()
         return cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, F_.layout_of("cache_write", k, v, k_cache, v_cache, slots, k_scale, v_scale))

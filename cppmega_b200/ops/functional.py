@@ -456,6 +456,13 @@ def _checked(layout) -> None:
     _CHECKED.add(layout)
 
 
+def bytes_spanned(t) -> int:
+    """Bytes from a tensor's first element to the end of its last one."""
+    if t is None or t.numel() == 0:
+        return 0
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 def _sequence_ends(name: str, ends, like: torch.Tensor) -> None:
     if ends.dtype != torch.int32 or ends.dim() != 1 or ends.numel() < 1:
         raise ValueError(f"{name}: sequence ends are int32 [sequences + 1], got {ends.dtype} {tuple(ends.shape)}")
@@ -554,7 +561,7 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> No
     """Writes the keys ``k`` [T, G, D] and values ``v`` [T, G, Dv] of new tokens into a paged cache ``k_cache`` [pages, page, G, D], ``v_cache``
     [pages, page, G, Dv], in place.  ``slots`` [T] (int32 or int64): page number times page size plus place in the page; a negative slot is
     left out (padding), of equal slots the last token's row stays.  ``v`` and ``v_cache`` may both be None (values that are columns of the
-    key rows).
+    key rows).  ``k`` and ``v`` may lie in the cache itself (tokens moved inside it): they count as they were before the call.
 
     A ``float8_e4m3fn`` cache holds each row divided by a power of two, whose exponent byte (127 + exponent, as in MXFP8) goes to ``k_scale``,
     ``v_scale`` (uint8 [pages, page, G]): the smallest with which the row's largest finite magnitude is at most 448; values that are not

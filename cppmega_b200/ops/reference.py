@@ -455,10 +455,10 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> No
     owner.scatter_reduce_(0, slots[used], index[used], "amax")
     keep = index[used][owner[slots[used]] == index[used]]
     where = slots[keep]
-    for x, cache, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
-        if x is None:
+    taken = [None if x is None else x.detach()[keep] for x in (k, v)]       # of both, before a cache changes that they may lie in
+    for rows, cache, scale in zip(taken, (k_cache, v_cache), (k_scale, v_scale)):
+        if rows is None:
             continue
-        rows = x.detach()[keep]
         if scale is None:
             cache[where // page, where % page] = rows
         else:

@@ -113,3 +113,14 @@ def test_keys_of_pages_outside_the_cache_have_no_weight(store, page, bad):
             want, size = p @ vh, p @ vh.abs()
             bound = 2 * half * want.abs() + (1 + half) * size * (half + e) + length * 2.0 ** -15 * float(store == E4M3) * (p * vh.abs().amax(1)).amax()
             assert ((got[b, h].double() - want).abs() <= bound).all(), float(((got[b, h].double() - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("swap", [False, True])
+def test_tokens_moved_inside_a_cache(swap):
+    """Every token one place further, keys to keys or to values, in one call over many blocks."""
+    kc, vc = _randn(1000, 16, 4, 64), _randn(1000, 16, 4, 64, seed=1)
+    was = [t.clone().view(16000, 4, 64) for t in (kc, vc)]
+    k, v = (t.view(16000, 4, 64)[:15999] for t in ((vc, kc) if swap else (kc, vc)))
+    F_.cache_write(k, v, kc, vc, torch.arange(1, 16000, device="cuda"))
+    for got, rows, old in zip((kc, vc), reversed(was) if swap else was, was):
+        assert torch.equal(got.view(16000, 4, 64)[1:], rows[:15999]) and torch.equal(got.view(16000, 4, 64)[0], old[0])
