@@ -97,7 +97,7 @@ def _plan_write(k, v, k_cache, v_cache, slots, k_scale, v_scale):
         return False
     return Plan([*strides(k), *strides(v, 2), *strides(k_cache), *strides(v_cache, 3), T, heads, dim, 0 if v is None else v.shape[2],
                  k_cache.shape[0], k_cache.shape[1], TYPES[k.dtype], int(q), int(slots.dtype == torch.int64)],
-                copy=not (rows_on(k, 16) and rows_on(v, 16) and slots.is_contiguous()), spans=[F_.bytes_spanned(t) for t in (k, v, k_cache, v_cache)])
+                copy=not (rows_on(k, 16) and rows_on(v, 16) and slots.is_contiguous()), spans=[F_.bytes_spanned(t) for t in (k, v, k_cache, v_cache, k_scale, v_scale)])
 
 
 def _meet(a, a_bytes, b, b_bytes) -> bool:
@@ -111,17 +111,21 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout) -> bool
     plan = planned(layout, lambda: _plan_write(k, v, k_cache, v_cache, slots, k_scale, v_scale))
     if not plan or not _bare(k, v, k_cache, v_cache, slots, k_scale, v_scale):
         return False
-    at, kp, vp, kcp, vcp = slots.data_ptr(), k.data_ptr(), _ptr(v), k_cache.data_ptr(), _ptr(v_cache)
+    at, kp, vp, kcp, vcp, ksp, vsp = slots.data_ptr(), k.data_ptr(), _ptr(v), k_cache.data_ptr(), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale)
     if (kcp | (vcp or 0)) & (7 if k_scale is not None else 15):
         return False
-    k_bytes, v_bytes, kc_bytes, vc_bytes = plan.spans
+    k_bytes, v_bytes, kc_bytes, vc_bytes, ks_bytes, vs_bytes = plan.spans
+    if vcp and _meet(kcp, kc_bytes, vcp, vc_bytes):
+        F_.check_apart(layout, k_cache, v_cache)
+    if vsp and _meet(ksp, ks_bytes, vsp, vs_bytes):
+        F_.check_apart(layout, k_scale, v_scale)
     inside = _meet(kp, k_bytes, kcp, kc_bytes) or vp and (
         _meet(kp, k_bytes, vcp, vc_bytes) or _meet(vp, v_bytes, kcp, kc_bytes) or _meet(vp, v_bytes, vcp, vc_bytes))
     if plan.copy or inside or (kp | (vp or 0)) & 15:      # a few rows; or rows of the cache itself, read before any is overwritten
         k, v = (None if t is None else t.detach().clone(memory_format=torch.contiguous_format) for t in (k, v))
         slots = slots.contiguous()
         return cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, F_.layout_of("cache_write", k, v, k_cache, v_cache, slots, k_scale, v_scale))
-    rc = _cu.lib().cm_cache_write(kp, vp, kcp, vcp, _ptr(k_scale), _ptr(v_scale), at, plan.at, _cu.err_word(k.device).data_ptr(), _cu.stream_ptr())
+    rc = _cu.lib().cm_cache_write(kp, vp, kcp, vcp, ksp, vsp, at, plan.at, _cu.err_word(k.device).data_ptr(), _cu.stream_ptr())
     if rc:
         _failed("cm_cache_write", rc)
     F_.count_launch("cache_write")

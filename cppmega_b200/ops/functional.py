@@ -463,6 +463,52 @@ def bytes_spanned(t) -> int:
     return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
+def _axes(t) -> list:
+    """(bytes of a step, steps) of the axes that have any, the widest first."""
+    return sorted(((s * t.element_size(), n) for n, s in zip(t.shape, t.stride()) if n > 1), reverse=True)
+
+
+def _nested(t) -> bool:
+    """Whether every axis steps over all that the narrower ones reach: no two elements share memory."""
+    reach = t.element_size()
+    for step, n in reversed(_axes(t)):
+        if step < reach:
+            return False
+        reach += (n - 1) * step
+    return True
+
+
+def _share_memory(a, b) -> bool:
+    """Whether two nested tensors have bytes in common.  Their axes are gone through from the widest in; where that would take long (steps that
+    do not match, lying in one another many times) they count as if they had."""
+    budget = 4096
+
+    def meet(x, y, off) -> bool:               # elements of x from 0 on, of y from `off` on
+        nonlocal budget
+        budget -= 1
+        x_reach, y_reach = (sum((n - 1) * s for s, n in axes) + e for axes, e in ((x, a.element_size()), (y, b.element_size())))
+        if off >= x_reach or off + y_reach <= 0:
+            return False
+        if not (x or y) or budget < 0:
+            return True
+        if x and y and x[0][0] == y[0][0]:     # a step of one against a step of the other: only their difference counts
+            (step, nx), (_, ny) = x[0], y[0]
+            x_in, y_in = x_reach - (nx - 1) * step, y_reach - (ny - 1) * step
+            first, last = max(1 - nx, (-off - y_in) // step + 1), min(ny - 1, -((off - x_in) // step) - 1)
+            return any(meet(x[1:], y[1:], off + i * step) for i in range(first, last + 1))
+        if not y or (x and x[0] > y[0]):
+            step, n = x[0]
+            inside = x_reach - (n - 1) * step
+            first, last = max(0, (off - inside) // step + 1), min(n - 1, -((-off - y_reach) // step) - 1)
+            return any(meet(x[1:], y, off - i * step) for i in range(first, last + 1))
+        step, n = y[0]
+        inside = y_reach - (n - 1) * step
+        first, last = max(0, (-off - inside) // step + 1), min(n - 1, -((off - x_reach) // step) - 1)
+        return any(meet(x, y[1:], off + i * step) for i in range(first, last + 1))
+
+    return a.numel() > 0 and b.numel() > 0 and meet(_axes(a), _axes(b), b.data_ptr() - a.data_ptr())
+
+
 def _sequence_ends(name: str, ends, like: torch.Tensor) -> None:
     if ends.dtype != torch.int32 or ends.dim() != 1 or ends.numel() < 1:
         raise ValueError(f"{name}: sequence ends are int32 [sequences + 1], got {ends.dtype} {tuple(ends.shape)}")
@@ -543,11 +589,12 @@ def _check_write(k, v, k_cache, v_cache, slots, k_scale, v_scale) -> None:
     _check_cache("cache_write", k_cache, v_cache, k_scale, v_scale)
     if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"cache_write: slots {slots.dtype} {tuple(slots.shape)}")
-    for x, cache in ((k, k_cache), (v, v_cache)):
+    for x, cache, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
         if x is None:
             continue
-        if any(n > 1 and s == 0 for n, s in zip(cache.shape, cache.stride())):
-            raise ValueError(f"cache_write: the rows of a cache are written once each, those of {tuple(cache.shape)} with strides {cache.stride()} overlap")
+        for t in (cache, scale):
+            if t is not None and t.numel() and not _nested(t):
+                raise ValueError(f"cache_write: the rows of a cache are written once each, those of {tuple(t.shape)} with strides {t.stride()} overlap")
         if x.dim() != 3 or x.shape[0] != slots.shape[0] or x.shape[1:] != cache.shape[2:]:
             raise ValueError(f"cache_write: rows {tuple(x.shape)} and slots {tuple(slots.shape)} for a cache of {tuple(cache.shape)}")
         if x.dtype != cache.dtype and cache.dtype != torch.float8_e4m3fn:
@@ -555,6 +602,17 @@ def _check_write(k, v, k_cache, v_cache, slots, k_scale, v_scale) -> None:
     if v is not None and v.dtype != k.dtype:
         raise ValueError(f"cache_write: k {k.dtype}, v {v.dtype}")
     _same_device("cache_write", k, v, k_cache, slots)
+
+
+def check_apart(layout, a, b) -> None:
+    """The keys' memory is not the values'.  That goes by addresses too, so every call looks; the kernels' wrapper asks only where the ranges meet."""
+    if b is None or not (torch._C._has_storage(a) and torch._C._has_storage(b)):
+        return
+    place = ("apart", b.data_ptr() - a.data_ptr(), b.shape, layout)
+    if place not in _CHECKED:
+        if _share_memory(a, b):
+            raise ValueError(f"cache_write: keys {tuple(a.shape)} and values {tuple(b.shape)} share memory")
+        _checked(place)
 
 
 def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> None:
@@ -566,7 +624,7 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> No
     A ``float8_e4m3fn`` cache holds each row divided by a power of two, whose exponent byte (127 + exponent, as in MXFP8) goes to ``k_scale``,
     ``v_scale`` (uint8 [pages, page, G]): the smallest with which the row's largest finite magnitude is at most 448; values that are not
     finite become NaN.  A 16-bit cache holds the rows as they are.  Values only: no gradient passes through a cache.  A slot behind the
-    cache's end is skipped and reported by ``ops.cuda.check_errors``."""
+    cache's end is skipped and reported by ``ops.cuda.check_errors``.  Caches whose rows overlap one another, or the other cache's, are refused."""
     layout = layout_of("cache_write", k, v, k_cache, v_cache, slots, k_scale, v_scale)
     if layout not in _CHECKED:
         _check_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
@@ -578,6 +636,8 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> No
         if fn(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout):
             return
         _miss("cache_write(shape/dtype)", k)
+    check_apart(layout, k_cache, v_cache)
+    check_apart(layout, k_scale, v_scale)
     with torch.no_grad():
         ref.cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
 

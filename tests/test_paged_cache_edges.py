@@ -72,3 +72,96 @@ def test_the_definition_takes_rows_of_the_cache_as_they_were(swap):
     F_.cache_write(k, v, kc, vc, torch.arange(1, 32))
     for got, rows, old in zip((kc, vc), reversed(was) if swap else was, was):
         assert torch.equal(got.view(32, 2, 16)[1:], rows[:31]) and torch.equal(got.view(32, 2, 16)[0], old[0])
+
+
+# ---- caches whose rows share memory ----------------------------------------------------------------------------------------
+
+def _bytes_of(t):
+    """Every byte that a tensor's elements hold, as often as they hold it."""
+    at = torch.zeros(1, dtype=torch.long)
+    for n, s in zip(t.shape, t.stride()):
+        at = (at[:, None] + torch.arange(n) * s).view(-1)
+    es = t.element_size()
+    return (t.data_ptr() + at[:, None] * es + torch.arange(es)).view(-1).tolist()
+
+
+def test_memory_that_two_tensors_share():
+    """Against the bytes themselves, for views of one buffer with any steps: nothing that shares memory is missed, and views whose axes have the
+    same steps, or lie in one piece inside each other's, are told exactly."""
+    g = torch.Generator().manual_seed(5)
+    buffers = {torch.int16: torch.zeros(600, dtype=torch.int16), torch.uint8: torch.zeros(1200, dtype=torch.uint8)}
+    nested = same = 0
+    for _ in range(4000):
+        dtype = torch.int16 if torch.rand(1, generator=g) < 0.7 else torch.uint8
+        views = []
+        steps = [int(torch.randint(0, 40, (1,), generator=g)) for _ in range(3)] + [1]
+        for i in range(2):
+            if i and torch.rand(1, generator=g) < 0.5:
+                steps = [int(torch.randint(0, 40, (1,), generator=g)) for _ in range(3)] + [1]
+            shape = torch.randint(1, 5, (4,), generator=g).tolist()
+            views.append(buffers[dtype].as_strided(shape, steps, int(torch.randint(0, 150, (1,), generator=g))))
+        a, b = views
+        for t in views:
+            held = _bytes_of(t)
+            if F_._nested(t):
+                nested += 1
+                assert len(set(held)) == len(held)
+        meet = bool(set(_bytes_of(a)) & set(_bytes_of(b)))
+        if F_._nested(a) and F_._nested(b):
+            same += meet
+            assert F_._share_memory(a, b) == meet and F_._share_memory(b, a) == meet
+    assert nested > 500 and same > 50
+
+
+@pytest.mark.parametrize("case", ["heads overlap", "tokens overlap", "one cache for both", "columns of one another", "shifted by a row", "scales of both",
+                                  "scale broadcast"])
+def test_caches_that_share_memory_are_refused(case):
+    e4m3 = torch.float8_e4m3fn
+    k = v = torch.ones(3, 2, 16)
+    kc, vc, ks, vs = torch.zeros(4, 8, 2, 16), torch.zeros(4, 8, 2, 16), None, None
+    if case == "heads overlap":
+        kc = torch.zeros(600).as_strided((4, 8, 2, 16), (128, 16, 8, 1))
+    elif case == "tokens overlap":
+        kc = torch.zeros(4000).as_strided((4, 8, 2, 16), (512, 24, 16, 1))
+    elif case == "one cache for both":
+        vc = kc
+    elif case == "columns of one another":
+        v, vc = v[..., :8], kc[..., 8:]
+    elif case == "shifted by a row":
+        both = torch.zeros(5, 8, 2, 16)
+        kc, vc = both[:4], both.view(40, 2, 16)[1:33].view(4, 8, 2, 16)
+    else:
+        kc, vc = (torch.zeros(4, 8, 2, 16, dtype=torch.uint8).view(e4m3) for _ in range(2))
+        ks = vs = torch.zeros(4, 8, 2, dtype=torch.uint8)
+        if case == "scale broadcast":
+            ks, vs = torch.zeros(4, 8, 1, dtype=torch.uint8).expand(4, 8, 2), vs.clone()
+    for _ in range(2):
+        with pytest.raises(ValueError, match="overlap|share memory"):
+            F_.cache_write(k, v, kc, vc, torch.tensor([0, 5, 7]), ks, vs)
+
+
+@pytest.mark.parametrize("case", ["stacked in a page", "columns side by side", "heads side by side", "blocks of a page in two orders", "places first",
+                                  "one buffer, two halves"])
+def test_caches_that_lie_between_one_another_are_taken(case):
+    k, v = torch.ones(3, 2, 16), torch.full((3, 2, 16), 2.0)
+    if case == "stacked in a page":
+        both = torch.zeros(4, 2, 8, 2, 16)
+        kc, vc = both[:, 0], both[:, 1]
+    elif case == "columns side by side":
+        both = torch.zeros(4, 8, 2, 40)
+        kc, vc = both[..., :16], both[..., 24:]
+    elif case == "heads side by side":
+        both = torch.zeros(4, 8, 5, 16)
+        kc, vc = both[:, :, :2], both[:, :, 3:]
+    elif case == "blocks of a page in two orders":
+        both = torch.zeros(4, 512)
+        kc, vc = both[:, :256].view(4, 8, 2, 16), both[:, 256:].view(4, 2, 8, 16).transpose(1, 2)
+    elif case == "places first":
+        both = torch.zeros(8, 4, 2, 2, 16)
+        kc, vc = both[:, :, 0].transpose(0, 1), both[:, :, 1].transpose(0, 1)
+    else:
+        both = torch.zeros(8, 8, 2, 16)
+        kc, vc = both[:4], both[4:]
+    for _ in range(2):
+        F_.cache_write(k, v, kc, vc, torch.tensor([0, 9, 31]))
+    assert float(kc.sum()) == k.numel() and float(vc.sum()) == 2 * v.numel() and float(both.sum()) == 3 * k.numel()
