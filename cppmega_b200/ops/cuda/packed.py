@@ -7,6 +7,7 @@ import torch
 
 from .. import cuda as _cu
 from .. import functional as F_
+from .. import reference as ref
 from .block import _Copied, _bare, _failed, _first_order, _given_back, _on_device, _ptr
 from .paged import TYPES, Plan, planned, rows_on, strides, width_ok
 
@@ -92,6 +93,8 @@ class PackedAttentionFn(torch.autograd.Function):
     @_first_order
     def backward(ctx, go):
         saved = ctx.saved_tensors
+        if not _bare(go):
+            return _by_definition(ctx, *saved[:5], go)
         layout = F_.layout_of("packed_attention_bwd", *saved, go)
         plan = planned(layout, lambda: _plan_backward(ctx.dtype, *saved, go))
         q, k, v, cu_q, cu_k, o, rest, lse = saved
@@ -113,6 +116,18 @@ class PackedAttentionFn(torch.autograd.Function):
             _failed("cm_packed_attention_bwd", rc)
         F_.count_launch("packed_attention_bwd", 3 if ctx.dtype == torch.bfloat16 else 4)
         return dq, dk, dv, None, None, None, None
+
+
+def _by_definition(ctx, q, k, v, cu_q, cu_k, go):
+    """Gradients for a ``go`` without memory of its own (a batch of them, under ``is_grads_batched``)."""
+    F_._miss("packed_attention_bwd(batched gradients)", q)
+    q, k, v = (_given_back(t, ctx.dtype, go.device, packed=False) for t in (q, k, v))
+    cu_q, cu_k = (_given_back(t, torch.int32, go.device, packed=False) for t in (cu_q, cu_k))
+    with torch.enable_grad():
+        leaves = [t.detach().requires_grad_(need) for t, need in zip((q, k, v), ctx.needs_input_grad)]
+        o = ref.packed_attention(*leaves, cu_q, ctx.scale, cu_k)
+    grads = iter(torch.autograd.grad(o, [t for t in leaves if t.requires_grad], go))
+    return (*(next(grads) if t.requires_grad else None for t in leaves), None, None, None, None)
 
 
 @_on_device

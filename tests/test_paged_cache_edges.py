@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from cppmega_b200.ops import functional as F_
+from cppmega_b200.ops import reference as ref
 from cppmega_b200.ops.cuda import packed, paged
 
 
@@ -165,3 +166,23 @@ def test_caches_that_lie_between_one_another_are_taken(case):
     for _ in range(2):
         F_.cache_write(k, v, kc, vc, torch.tensor([0, 9, 31]))
     assert float(kc.sum()) == k.numel() and float(vc.sum()) == 2 * v.numel() and float(both.sum()) == 3 * k.numel()
+
+
+# ---- attention over packed sequences -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("wanted", [[0, 1, 2], [1], [0, 2]])
+def test_batched_upstream_gradients_of_the_packed_attention(kernels, wanted):
+    """Under ``is_grads_batched`` the upstream gradient has no memory that a kernel could read: the definition's gradients, one row of the batch
+    after the other."""
+    kernels.cm_packed_attention_ws = lambda at: 0
+    kernels.cm_packed_attention_fwd = lambda *args: 0
+    ends, ends_k = _i32(0, 5, 9), _i32(0, 7, 11)
+    leaves = [_randn(n, h, 16, seed=s).requires_grad_(s in wanted) for s, n, h in ((0, 9, 4), (1, 11, 2), (2, 11, 2))]
+    some = [leaves[i] for i in wanted]
+    go = _randn(3, 9, 4, 16, seed=3)
+    o = F_.packed_attention(*leaves, ends, 0.25, ends_k)
+    got = torch.autograd.grad(o, some, go, is_grads_batched=True)
+    for i in range(3):
+        want = torch.autograd.grad(ref.packed_attention(*leaves, ends, 0.25, ends_k), some, go[i])
+        # the same sums in another order in fp32, then one rounding
+        assert all(((a[i].double() - b.double()).abs() <= 2.0 ** -7 * b.double().abs() + 2.0 ** -16).all() for a, b in zip(got, want))
