@@ -728,6 +728,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const Args a, int
   const int r0 = (int)(s0 / q), r1 = steps ? (int)((s0 + steps - 1) / q) : r0;
   few::wait_for_input();                     // by every block, as above
   few::let_next_start();
+  if (bad && blockIdx.x == 0 && a.err) atomicCAS(a.err, 0, ERR_BAD_ARG);   // of a table of no columns nobody else has looked at the lengths
   if (steps && r0 == r1) return;             // finished by the one run that holds it
 
   float top = -INFINITY, sum = 0.f, acc[C];

@@ -124,3 +124,11 @@ def test_tokens_moved_inside_a_cache(swap):
     F_.cache_write(k, v, kc, vc, torch.arange(1, 16000, device="cuda"))
     for got, rows, old in zip((kc, vc), reversed(was) if swap else was, was):
         assert torch.equal(got.view(16000, 4, 64)[1:], rows[:15999]) and torch.equal(got.view(16000, 4, 64)[0], old[0])
+
+
+@pytest.mark.parametrize("lens", [[0, 1], [-1, 0], [2 ** 31 - 1, 0]])
+def test_lengths_over_a_table_of_no_columns_are_reported(lens):
+    kc, vc = _randn(5, 16, 2, 64), _randn(5, 16, 2, 64, seed=1)
+    got = F_.paged_attention(_randn(2, 4, 64), kc, vc, torch.zeros(2, 0, dtype=torch.int32, device="cuda"), _i32(lens), 0.1)
+    _reported()
+    assert (got == 0).all()
