@@ -387,7 +387,8 @@ static Side side_of(const void* x, const long long* xs, void* cache, const long 
 template <typename A, typename Kern>
 static int start(Kern kern, A& a, int resident, cudaStream_t stream) {
   a.per_block = tokens_per_block(a.T, resident);
-  kern<<<(a.T + a.per_block - 1) / a.per_block, THREADS, 0, stream>>>(a);
+  const int blocks = (a.T + a.per_block - 1) / a.per_block;
+  kern<<<blocks > 0 ? blocks : 1, THREADS, 0, stream>>>(a);   // of no tokens and of no heads what is given is looked at all the same
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -407,7 +408,7 @@ template <typename A>
 static int common(A& a, void* k, void* v, void* kc, void* vc, void* k_scale, void* v_scale, const long long* n) {
   const int es = n[17] ? 1 : 2, dim = (int)n[12], vdim = (int)n[13];
   if (dim < 8 || dim % 8 || dim > 256 || vdim < 0 || vdim % 8 || vdim > 256 || n[15] < 1 || n[14] < 0) return -10;
-  if (n[17] && (!k_scale || (vdim && !v_scale))) return -10;
+  if (n[17] && n[11] && n[14] && (!k_scale || (vdim && !v_scale))) return -10;             // a cache of nothing may lie nowhere
   for (int i : {0, 1, 2, 3, 5, 6, 8, 9})
     if (n[i] < -(1ll << 30) || n[i] >= 1ll << 30) return -10;
   a.side[0] = side_of(k, n, kc, n + 4, k_scale, dim, es);
@@ -423,7 +424,8 @@ static int common(A& a, void* k, void* v, void* kc, void* vc, void* k_scale, voi
 // Then: slots are 64-bit numbers.  slots [T]: page * (slots of a page) + offset, negative: left out.
 extern "C" int cm_cache_write(const void* k, const void* v, void* kc, void* vc, void* k_scale, void* v_scale, const void* slots, const long long* n,
                               int* err, cudaStream_t stream) {
-  if (n[10] <= 0 || n[11] <= 0) return 0;
+  if (n[10] == 0) return 0;
+  if (n[10] < 0 || n[11] < 0) return -10;
   WriteArgs a;
   const int rc = common(a, const_cast<void*>(k), const_cast<void*>(v), kc, vc, k_scale, v_scale, n);
   if (rc) return rc;
@@ -439,7 +441,7 @@ extern "C" int cm_cache_write(const void* k, const void* v, void* kc, void* vc, 
 // sequence s that holds it; tokens of no sequence become zeros.
 extern "C" int cm_cache_read(void* k, void* v, const void* kc, const void* vc, const void* k_scale, const void* v_scale, const int* table,
                              const int* ends, const long long* n, int* err, cudaStream_t stream) {
-  if (n[10] <= 0 || n[11] <= 0) return 0;
+  if (n[10] < 0 || n[11] < 0) return -10;
   ReadArgs a;
   const int rc = common(a, k, v, const_cast<void*>(kc), const_cast<void*>(vc), const_cast<void*>(k_scale), const_cast<void*>(v_scale), n);
   if (rc) return rc;

@@ -132,3 +132,32 @@ def test_lengths_over_a_table_of_no_columns_are_reported(lens):
     got = F_.paged_attention(_randn(2, 4, 64), kc, vc, torch.zeros(2, 0, dtype=torch.int32, device="cuda"), _i32(lens), 0.1)
     _reported()
     assert (got == 0).all()
+
+
+@pytest.mark.parametrize("store", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("heads", [2, 0])
+@pytest.mark.parametrize("ends", [[0, 1], [1, 0], [0, -1], [-1, 0]])
+def test_ends_of_a_read_of_no_rows_are_reported(ends, heads, store):
+    kc, vc, ks, vs = _caches(5, 16, heads, (64, 64), store)
+    k, v = F_.cache_read(kc, vc, _i32([[1, 4, 3]]), _i32(ends), 0, ks, vs)
+    _reported()
+    assert k.shape == v.shape == (0, heads, 64)
+    k, _ = F_.cache_read(kc, vc, _i32([[1, 4, 3]]), _i32([0, 0]), 0, ks, vs)
+    from cppmega_b200.ops import cuda as cu
+    cu.check_errors()
+
+
+@pytest.mark.parametrize("store", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("pages,heads", [(5, 0), (0, 2)])
+def test_pages_and_slots_of_a_cache_of_nothing_are_reported(pages, heads, store):
+    kc, vc, ks, vs = _caches(pages, 16, heads, (64, 64), store)
+    k, v = F_.cache_read(kc, vc, _i32([[1, 5, 3]]), _i32([0, 40]), 40, ks, vs)
+    _reported()
+    assert k.shape == v.shape == (40, heads, 64) and (k == 0).all() and (v == 0).all()
+    F_.cache_write(_randn(2, heads, 64), _randn(2, heads, 64), kc, vc, torch.tensor([3, 80], device="cuda"), ks, vs)
+    _reported()
+    slots = [3, -1] if pages else [-1, -1]
+    F_.cache_write(_randn(2, heads, 64), _randn(2, heads, 64), kc, vc, torch.tensor(slots, device="cuda"), ks, vs)
+    F_.cache_write(_randn(0, heads, 64), _randn(0, heads, 64), kc, vc, torch.zeros(0, dtype=torch.int32, device="cuda"), ks, vs)
+    from cppmega_b200.ops import cuda as cu
+    cu.check_errors()
