@@ -202,7 +202,8 @@ def paged_attention(q, k_cache, v_cache, table, lens, scale, k_scale, v_scale, l
     dev = q.device
     out = torch.empty_like(q) if plan.like else torch.empty(plan.shape, dtype=q.dtype, device=dev)
     ws = torch.empty(plan.work, dtype=torch.float32, device=dev)
-    rc = _cu.lib().cm_paged_attention(qp, kp, vp, _ptr(k_scale), _ptr(v_scale), table.data_ptr(), lens.data_ptr(), out.data_ptr(), ws.data_ptr(),
+    # a cache of no pages lies nowhere: the copies of no bytes that stand for its rows name the query's memory
+    rc = _cu.lib().cm_paged_attention(qp, kp or qp, vp or qp, _ptr(k_scale), _ptr(v_scale), table.data_ptr(), lens.data_ptr(), out.data_ptr(), ws.data_ptr(),
                                       plan.at, float(scale), _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
     if rc:
         _failed("cm_paged_attention", rc)

@@ -161,3 +161,15 @@ def test_pages_and_slots_of_a_cache_of_nothing_are_reported(pages, heads, store)
     F_.cache_write(_randn(0, heads, 64), _randn(0, heads, 64), kc, vc, torch.zeros(0, dtype=torch.int32, device="cuda"), ks, vs)
     from cppmega_b200.ops import cuda as cu
     cu.check_errors()
+
+
+@pytest.mark.parametrize("store", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("page", [16, 7])
+def test_attention_over_a_cache_of_no_pages(page, store):
+    kc, vc, ks, vs = _caches(0, page, 2, (64, 64), store)
+    table = torch.zeros(2, 30, dtype=torch.int32, device="cuda")
+    assert (F_.paged_attention(_randn(2, 4, 64), kc, vc, table, _i32([0, 0]), 0.1, ks, vs) == 0).all()
+    from cppmega_b200.ops import cuda as cu
+    cu.check_errors()
+    assert (F_.paged_attention(_randn(2, 4, 64), kc, vc, table, _i32([0, 200]), 0.1, ks, vs) == 0).all()
+    _reported()

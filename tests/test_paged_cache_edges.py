@@ -186,3 +186,14 @@ def test_batched_upstream_gradients_of_the_packed_attention(kernels, wanted):
         want = torch.autograd.grad(ref.packed_attention(*leaves, ends, 0.25, ends_k), some, go[i])
         # the same sums in another order in fp32, then one rounding
         assert all(((a[i].double() - b.double()).abs() <= 2.0 ** -7 * b.double().abs() + 2.0 ** -16).all() for a, b in zip(got, want))
+
+
+# ---- caches and calls of nothing ---------------------------------------------------------------------------------------------
+
+def test_paged_attention_over_a_cache_of_no_pages_names_memory_that_is_there(kernels):
+    seen = []
+    kernels.cm_paged_attention_ws = lambda *sizes: 0
+    kernels.cm_paged_attention = lambda *args: seen.append(args) or 0
+    q, none = _randn(2, 4, 16), torch.zeros(0, 8, 2, 16, dtype=torch.bfloat16)
+    F_.paged_attention(q, none, none, torch.zeros(2, 3, dtype=torch.int32), _i32(5, 0), 0.25)
+    assert seen[0][:3] == (q.data_ptr(),) * 3
