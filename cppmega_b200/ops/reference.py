@@ -431,6 +431,8 @@ def cache_power(byte: torch.Tensor) -> torch.Tensor:
 
 def _cache_rows(cache: torch.Tensor, scale: Optional[torch.Tensor], page: torch.Tensor, at: torch.Tensor) -> torch.Tensor:
     """fp32 rows ``cache[page, at]``; pages outside the cache give rows of zeros."""
+    if cache.shape[0] == 0:
+        return torch.zeros(*page.shape, *cache.shape[2:], dtype=torch.float32, device=cache.device)
     there = (page >= 0) & (page < cache.shape[0])
     page = torch.where(there, page, torch.zeros_like(page))
     if cache.dtype == torch.float8_e4m3fn:

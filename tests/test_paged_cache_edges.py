@@ -197,3 +197,19 @@ def test_paged_attention_over_a_cache_of_no_pages_names_memory_that_is_there(ker
     q, none = _randn(2, 4, 16), torch.zeros(0, 8, 2, 16, dtype=torch.bfloat16)
     F_.paged_attention(q, none, none, torch.zeros(2, 3, dtype=torch.int32), _i32(5, 0), 0.25)
     assert seen[0][:3] == (q.data_ptr(),) * 3
+
+
+@pytest.mark.parametrize("store", [torch.float32, torch.float8_e4m3fn])
+def test_the_definitions_over_a_cache_of_no_pages(store):
+    """No page is looked up, in a table that has columns either."""
+    kc, vc = (torch.zeros(0, 8, 2, n, dtype=torch.uint8).view(store) if store != torch.float32 else torch.zeros(0, 8, 2, n) for n in (16, 24))
+    ks = vs = None if store == torch.float32 else torch.zeros(0, 8, 2, dtype=torch.uint8)
+    table = torch.tensor([[0, -1, 3], [5, 5, 5]], dtype=torch.int32)
+    q = _randn(2, 4, 16, dtype=torch.float32).requires_grad_()
+    o = F_.paged_attention(q, kc, vc, table, _i32(0, 0), 1.0, ks, vs)
+    assert o.shape == (2, 4, 24) and (o == 0).all() and (torch.autograd.grad(o.sum(), q)[0] == 0).all()
+    k, v = F_.cache_read(kc, vc, table, _i32(0, 0, 0), 5, ks, vs)
+    assert k.shape == (5, 2, 16) and v.shape == (5, 2, 24) and not k.any() and not v.any()
+    F_.cache_write(torch.ones(3, 2, 16), torch.ones(3, 2, 24), kc, vc, torch.full((3,), -1), ks, None if vs is None else vs.clone())
+    with pytest.raises(ValueError, match="outside the cache"):
+        F_.paged_attention(q, kc, vc, table, _i32(0, 1), 1.0, ks, vs)
