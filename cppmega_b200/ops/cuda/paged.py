@@ -80,6 +80,11 @@ def width_ok(t, step: int, most: int) -> bool:
     return t is None or (t.shape[-1] % step == 0 and step <= t.shape[-1] <= most)
 
 
+def _rows_of_pages(table) -> bool:
+    """Whether the rows of a block table can be read in place; one without entries never is."""
+    return table.numel() == 0 or table.shape[1] == 1 or table.stride(1) == 1
+
+
 def _scales(t):
     """Exponent bytes are read and written through one index."""
     return t is None or t.is_contiguous()
@@ -141,7 +146,7 @@ def _plan_read(k_cache, v_cache, table, ends, total, k_scale, v_scale, dtype):
         return False
     return Plan([heads * dim, dim, heads * vdim, vdim, *strides(k_cache), *strides(v_cache, 3), total, heads, dim, vdim, k_cache.shape[0],
                  k_cache.shape[1], TYPES[dtype], int(q), table.stride(0), table.shape[0], table.shape[1]],
-                copy=not ((table.stride(-1) == 1 or table.shape[1] <= 1) and ends.is_contiguous()),
+                copy=not (_rows_of_pages(table) and ends.is_contiguous()),
                 shape=((total, heads, dim), (total, heads, vdim)))
 
 
@@ -180,7 +185,7 @@ def _plan_attention(q, k_cache, v_cache, table, lens, k_scale, v_scale):
         return False
     return Plan([*strides(q), *strides(k_cache), *strides(v_cache), table.stride(0), B, heads, group, columns, pages, page, dim, vdim,
                  TYPES[q.dtype], int(e4m3)],
-                copy=not (rows_on(q, 16) and (table.stride(-1) == 1 or columns <= 1) and lens.is_contiguous()), shape=(B, H, vdim),
+                copy=not (rows_on(q, 16) and _rows_of_pages(table) and lens.is_contiguous()), shape=(B, H, vdim),
                 work=_cu.lib().cm_paged_attention_ws(B, heads, group, dim, vdim, columns, page, int(e4m3)) if B else 0,
                 like=q.is_contiguous() and vdim == dim)
 

@@ -213,3 +213,19 @@ def test_the_definitions_over_a_cache_of_no_pages(store):
     F_.cache_write(torch.ones(3, 2, 16), torch.ones(3, 2, 24), kc, vc, torch.full((3,), -1), ks, None if vs is None else vs.clone())
     with pytest.raises(ValueError, match="outside the cache"):
         F_.paged_attention(q, kc, vc, table, _i32(0, 1), 1.0, ks, vs)
+
+
+@pytest.mark.parametrize("shape", [(0, 4), (3, 0), (0, 0), (2, 4)])
+def test_tables_whose_entries_lie_apart(kernels, shape):
+    """Every other column of a wider table: copied, and where it has no entries there is nothing to copy."""
+    seen = []
+    kernels.cm_paged_attention_ws = lambda *sizes: 0
+    kernels.cm_paged_attention = lambda *args: seen.append(args) or 0
+    kernels.cm_cache_read = lambda *args: seen.append(args) or 0
+    kc = _randn(4, 8, 2, 16)
+    n, columns = shape
+    table = torch.arange(4 * 10, dtype=torch.int32).view(4, 10)[:n, :2 * columns:2]
+    assert F_.paged_attention(_randn(n, 4, 32)[..., 8:24], kc, kc, table, torch.zeros(2 * n, dtype=torch.int32)[::2], 0.25).shape == (n, 4, 16)
+    ends = torch.zeros(n + 1, dtype=torch.int32)
+    assert F_.cache_read(kc, kc, table, ends, 3)[0].shape == (3, 2, 16)
+    assert len(seen) == 2
