@@ -12,6 +12,7 @@ that has a GPU, the first CUDA call raises instead of silently falling back.
 from __future__ import annotations
 
 import collections
+import operator
 from typing import Callable, Dict, Optional
 
 import torch
@@ -655,6 +656,7 @@ def cache_read(k_cache, v_cache, block_table, cu_seqlens, total: int, k_scale=No
         _sequence_ends("cache_read", cu_seqlens, k_cache)
         _check_table("cache_read", block_table, cu_seqlens.numel() - 1, k_cache)
         _checked(layout)
+    total = operator.index(total)              # a number: plans are kept by it
     if total < 0:
         raise ValueError(f"cache_read: {total} rows")
     if dtype is None:

@@ -229,3 +229,14 @@ def test_tables_whose_entries_lie_apart(kernels, shape):
     ends = torch.zeros(n + 1, dtype=torch.int32)
     assert F_.cache_read(kc, kc, table, ends, 3)[0].shape == (3, 2, 16)
     assert len(seen) == 2
+
+
+def test_a_number_of_rows_that_changes_in_place(kernels):
+    """A tensor of no axes may say how many rows are read: its value at the call counts, not the tensor."""
+    kernels.cm_cache_read = lambda *args: 0
+    kc, total = _randn(4, 8, 2, 16), torch.tensor(3)
+    for rows in (3, 7):
+        total.fill_(rows)
+        assert F_.cache_read(kc, None, torch.zeros(1, 2, dtype=torch.int32), _i32(0, 2), total)[0].shape == (rows, 2, 16)
+    with pytest.raises(TypeError):
+        F_.cache_read(kc, None, torch.zeros(1, 2, dtype=torch.int32), _i32(0, 2), 3.0)
