@@ -233,10 +233,12 @@ def test_tables_whose_entries_lie_apart(kernels, shape):
 
 def test_a_number_of_rows_that_changes_in_place(kernels):
     """A tensor of no axes may say how many rows are read: its value at the call counts, not the tensor."""
-    kernels.cm_cache_read = lambda *args: 0
+    seen = []
+    kernels.cm_cache_read = lambda *args: seen.append((ctypes.c_longlong * 11).from_address(args[8])[10]) or 0
     kc, total = _randn(4, 8, 2, 16), torch.tensor(3)
     for rows in (3, 7):
         total.fill_(rows)
         assert F_.cache_read(kc, None, torch.zeros(1, 2, dtype=torch.int32), _i32(0, 2), total)[0].shape == (rows, 2, 16)
+    assert seen == [3, 7]                                       # the rows that the kernel is told to write
     with pytest.raises(TypeError):
         F_.cache_read(kc, None, torch.zeros(1, 2, dtype=torch.int32), _i32(0, 2), 3.0)
