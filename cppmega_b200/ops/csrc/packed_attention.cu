@@ -1419,6 +1419,16 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (warp == MMA_WARP) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
+// Calls without rows of queries or of keys: their ends are looked at all the same
+__global__ void packed_ends_kernel(const int* cu_q, const int* cu_k, int n, int T, int Tk, int* err) {
+  bool bad = false;
+  for (int i = threadIdx.x; i <= n; i += blockDim.x) {
+    const int x = __ldg(cu_q + i), y = __ldg(cu_k + i);
+    bad |= x > T || y > Tk || (i == 0 ? x != 0 || y != 0 : x < __ldg(cu_q + i - 1) || y < __ldg(cu_k + i - 1));
+  }
+  if (bad && err) atomicCAS(err, 0, ERR_BAD_ARG);
+}
+
 // ---- launches --------------------------------------------------------------------------------------------------------
 // [rows, heads, width] with strides (elements) of rows and heads; boxes of 64 columns, `box_heads` heads, `box_rows` rows
 int map_rows(CUtensorMap* out, const void* base, int rows, int heads, int width, const long long* strides, int box_heads, int box_rows, bool half) {
@@ -1608,4 +1618,11 @@ extern "C" int cm_packed_attention_bwd(const void* q, const void* k, const void*
   }
   if (a.vdim > 64) return backward<true, 128, 128>(in, a, dq, dk, dv, stream);
   return a.dim > 64 ? backward<true, 128, 64>(in, a, dq, dk, dv, stream) : backward<true, 64, 64>(in, a, dq, dk, dv, stream);
+}
+
+// For T, Tk or heads of zero, where there is nothing to compute: reports ends that do not rise from 0 to at most T and Tk
+extern "C" int cm_packed_attention_ends(const int* cu_q, const int* cu_k, long long n, long long T, long long Tk, int* err, cudaStream_t stream) {
+  if (n < 0 || T < 0 || Tk < 0 || n >= 1ll << 31 || T >= 1ll << 31 || Tk >= 1ll << 31) return -10;
+  packed_ends_kernel<<<1, 256, 0, stream>>>(cu_q, cu_k, (int)n, (int)T, (int)Tk, err);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }

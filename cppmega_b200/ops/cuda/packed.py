@@ -13,16 +13,20 @@ from .paged import TYPES, Plan, planned, rows_on, strides, width_ok
 
 
 def declare(L: ctypes.CDLL) -> None:
-    vp, i32, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+    vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
     sig = {
         "cm_packed_attention_fwd": [vp] * 10 + [f32, vp, vp],
         "cm_packed_attention_bwd": [vp] * 14 + [f32, vp, vp],
+        "cm_packed_attention_ends": [vp, vp, i64, i64, i64, vp, vp],
     }
     for name, args in sig.items():
         if hasattr(L, name):
             getattr(L, name).argtypes, getattr(L, name).restype = args, i32
     if hasattr(L, "cm_packed_attention_ws"):
         L.cm_packed_attention_ws.argtypes, L.cm_packed_attention_ws.restype = [vp], ctypes.c_longlong
+
+
+NOTHING = -1               # work of a call without rows of queries, or of keys, or heads
 
 
 def _strides_ok(t: torch.Tensor) -> bool:
@@ -49,9 +53,10 @@ def _numbers(q, k, v, cu_q, go=None):
 
 
 def _plan(q, k, v, cu_q, cu_k):
-    if not (q.dtype in TYPES and width_ok(q, 8, 128) and width_ok(v, 8, 128) and 0 < q.shape[0] < 2 ** 30 and 0 < k.shape[0] < 2 ** 30
-            and q.shape[1] > 0):
+    if not (q.dtype in TYPES and width_ok(q, 8, 128) and width_ok(v, 8, 128) and q.shape[0] < 2 ** 30 and k.shape[0] < 2 ** 30):
         return False
+    if not (q.shape[0] and k.shape[0] and q.shape[1]):
+        return Plan([], shape=(q.shape[0], q.shape[1], v.shape[2]), work=NOTHING)
     plan = Plan(_numbers(q, k, v, cu_q), shape=(q.shape[0], q.shape[1], v.shape[2]), like=q.is_contiguous() and q.shape[2] == v.shape[2],
                 copy=not (_strides_ok(q) and _strides_ok(k) and _strides_ok(v) and cu_q.is_contiguous() and (cu_k is None or cu_k.is_contiguous())))
     plan.work = _cu.lib().cm_packed_attention_ws(plan.at)
@@ -118,6 +123,16 @@ class PackedAttentionFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None
 
 
+def _nothing(plan, q, k, v, cu_q, cu_k):
+    """Zeros that depend on the inputs, whose gradients are zeros too; the ends are checked on the device as those of any call."""
+    rc = _cu.lib().cm_packed_attention_ends(cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, q.shape[0], k.shape[0],
+                                            _cu.err_word(q.device).data_ptr(), _cu.stream_ptr())
+    if rc:
+        _failed("cm_packed_attention_ends", rc)
+    F_.count_launch("packed_attention")
+    return q.new_zeros(plan.shape) + sum(t[:0].sum() for t in (q, k, v))
+
+
 def _by_definition(ctx, q, k, v, cu_q, cu_k, go):
     """Gradients for a ``go`` without memory of its own (a batch of them, under ``is_grads_batched``)."""
     F_._miss("packed_attention_bwd(batched gradients)", q)
@@ -136,6 +151,8 @@ def packed_attention(q, k, v, cu_q, scale, cu_k, layout):
     plan = planned(layout, lambda: _plan(q, k, v, cu_q, cu_k))
     if not plan or isinstance(scale, torch.Tensor) or not abs(scale) < 2.0 ** 64 or not _bare(q, k, v, cu_q, cu_k):
         return None
+    if plan.work == NOTHING:
+        return _nothing(plan, q, k, v, cu_q.contiguous(), cu_q.contiguous() if cu_k is None else cu_k.contiguous())
     if scale < 0 or plan.copy or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
         if scale < 0:      # the kernels take the largest product of a row for its reference: the sign goes into q, exactly
             q, scale = -q, -scale

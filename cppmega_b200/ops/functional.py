@@ -545,9 +545,10 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, cu_seqlens_k=None):
 
     bf16 and fp16 with ``D`` and ``Dv`` multiples of 8 up to 128 run on the kernels, in training with their gradients (first
     derivatives; the same call gives the same bits); strided tensors are read in place where rows lie on 16 bytes.
-    Anything else, forward mode and function transforms run the definition, ``reference.packed_attention``.  A CUDA graph takes forward and
-    backward together, while no eager graph of the same leaves is alive (autograd would add to those on the eager stream).  No call waits for the device: ends
-    that fall or run over the buffer are reported by ``ops.cuda.check_errors``."""
+    Anything else, forward mode and function transforms run the definition, ``reference.packed_attention``, which reads the ends on the host.  A CUDA
+    graph takes forward and backward together, while no eager graph of the same leaves is alive (autograd would add to those on the eager stream).  The
+    kernels' calls, those without queries, keys or heads among them, wait for nothing: ends that fall or run over the buffer are reported by
+    ``ops.cuda.check_errors``."""
     layout = layout_of("packed_attention", q, k, v, cu_seqlens, cu_seqlens_k)
     if layout not in _CHECKED:
         _check_packed(q, k, v, cu_seqlens, cu_seqlens_k)

@@ -31,3 +31,48 @@ def test_batched_upstream_gradients(dtype):
         for a, b in zip(got, torch.autograd.grad(o, leaves, go[i], retain_graph=True)):
             a, b = a[i].double(), b.double()
             assert (a - b).norm() <= 8 * torch.finfo(dtype).eps / 2 * b.norm()
+
+
+NOTHING = [(0, 0, 2, 2), (0, 7, 2, 2), (7, 0, 4, 2), (7, 7, 0, 2)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,Tk,H,G", NOTHING)
+def test_calls_of_nothing_wait_for_nothing(T, Tk, H, G, dtype):
+    """No rows of queries, of keys, or no heads: zeros, and gradients of zeros, also in a captured graph, whose ends change in place."""
+    leaves = [_randn(n, h, 64, dtype=dtype, seed=s).requires_grad_() for s, n, h in ((0, T, H), (1, Tk, G), (2, Tk, G))]
+    cu, cu_k = _i32([0, T // 2, T]), _i32([0, Tk, Tk])
+
+    def once():
+        o = F_.packed_attention(*leaves, cu, -0.125, cu_k)
+        return [o.detach(), *torch.autograd.grad(o, leaves, torch.ones_like(o))]
+
+    F_.reset_counters()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager = once()
+    torch.cuda.current_stream().wait_stream(side)
+    assert F_.launch_counts() == {"packed_attention": 1} and not F_.fallback_counts()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = once()
+    g.replay()
+    from cppmega_b200.ops import cuda as cu_
+    cu_.check_errors()
+    for outs in (eager, captured):
+        assert outs[0].shape == (T, H, 64) and outs[0].dtype == dtype
+        assert all(a.shape == b.shape and (a == 0).all() for a, b in zip(outs[1:], leaves)) and (outs[0] == 0).all()
+    for ends, ends_k in (([0, T // 2, T + 1], [0, 0, Tk]), ([0, 0, T], [1, 1, 1]), ([0, -1, 0], [0, 0, 0]), ([0, 0, 0], [0, 5, 4])):
+        cu.copy_(_i32(ends))
+        cu_k.copy_(_i32(ends_k))
+        g.replay()
+        with pytest.raises(cu_.KernelError, match="bad argument"):
+            cu_.check_errors()
+
+
+def test_calls_of_nothing_can_be_differentiated_again():
+    leaves = [_randn(n, 2, 64, seed=s).requires_grad_() for s, n in ((0, 5), (1, 0), (2, 0))]
+    o = F_.packed_attention(*leaves, _i32([0, 5]), 0.1, _i32([0, 0]))
+    (g,) = torch.autograd.grad(o.sum() + leaves[0].square().sum(), leaves[0], create_graph=True)
+    assert torch.equal(torch.autograd.grad(g.sum(), leaves[0])[0], torch.full_like(leaves[0], 2))

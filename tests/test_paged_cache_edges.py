@@ -242,3 +242,16 @@ def test_a_number_of_rows_that_changes_in_place(kernels):
     assert seen == [3, 7]                                       # the rows that the kernel is told to write
     with pytest.raises(TypeError):
         F_.cache_read(kc, None, torch.zeros(1, 2, dtype=torch.int32), _i32(0, 2), 3.0)
+
+
+@pytest.mark.parametrize("T,Tk,H", [(0, 0, 4), (0, 7, 4), (7, 0, 4), (7, 7, 0)])
+def test_packed_attention_of_nothing_looks_at_its_ends_on_the_device(kernels, monkeypatch, T, Tk, H):
+    """No rows of queries, of keys, or no heads: one look at the ends, zeros, and nothing that waits for their values."""
+    seen = []
+    kernels.cm_packed_attention_ends = lambda *args: seen.append(args) or 0
+    monkeypatch.setattr(F_.ref, "packed_attention", None)
+    cu, cu_k = torch.tensor([0, -9, 0, -9, T], dtype=torch.int32)[::2], _i32(0, 0, Tk)
+    leaves = [_randn(n, h, 16, seed=s).requires_grad_() for s, n, h in ((0, T, H), (1, Tk, 2), (2, Tk, 2))]
+    o = F_.packed_attention(*leaves, cu, -0.5, cu_k)
+    assert len(seen) == 1 and seen[0][2:5] == (2, T, Tk) and o.shape == (T, H, 16) and not o.any()
+    assert all(g.shape == t.shape and not g.any() for g, t in zip(torch.autograd.grad(o.sum(), leaves), leaves))
