@@ -1537,10 +1537,13 @@ int backward(const Inputs& in, Args a, void* dq, void* dk, void* dv, cudaStream_
     packed_delta_kernel<HALF, LANES><<<(unsigned)blocks, DELTA_THREADS, 0, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return -3;
   }
-  a.units = (int)uq;
-  a.out = dq;
-  packed_dq_kernel<HALF, D, DV><<<(unsigned)(uq * a.kv_heads * a.chunks), THREADS, Dq<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], m[3], a);
-  if (cudaGetLastError() != cudaSuccess) return -3;
+  if (dq) {
+    a.units = (int)uq;
+    a.out = dq;
+    packed_dq_kernel<HALF, D, DV><<<(unsigned)(uq * a.kv_heads * a.chunks), THREADS, Dq<D, DV>::SMEM, stream>>>(m[0], m[1], m[2], m[3], a);
+    if (cudaGetLastError() != cudaSuccess) return -3;
+  }
+  if (!dk) return 0;
   a.units = (int)uk;
   a.out = dk;
   a.out2 = dv;
@@ -1596,7 +1599,7 @@ extern "C" int cm_packed_attention_fwd(const void* q, const void* k, const void*
 }
 
 // o, o_rest and lse from the forward; go (the gradient of o) [T, heads, vdim]; delta: scratch of T * heads floats, fp16: 2 (T heads + sequences kv_heads);
-// dq [T, heads, dim], dk [Tk, kv_heads, dim], dv [Tk, kv_heads, vdim] packed, all written whole
+// dq [T, heads, dim], dk [Tk, kv_heads, dim], dv [Tk, kv_heads, vdim] packed, all written whole; dq may be null, or dk and dv together
 extern "C" int cm_packed_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* go, const int* cu_q,
                                        const int* cu_k, const float* lse, float* delta, void* dq, void* dk, void* dv, const long long* n, float scale,
                                        int* err, cudaStream_t stream) {

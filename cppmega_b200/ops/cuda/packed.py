@@ -111,16 +111,18 @@ class PackedAttentionFn(torch.autograd.Function):
             lse, go = _given_back(lse, torch.float32, dev), _packed(go)
             plan = _plan_backward(dt, q, k, v, cu_q, cu_k, o, rest, lse, go)
         dev = go.device
-        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+        need_q, need_k, need_v = ctx.needs_input_grad[:3]           # dk and dv come from one kernel
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) if need else None
+                      for t, need in ((q, need_q), (k, need_k or need_v), (v, need_k or need_v)))
         delta = torch.empty(plan.work, dtype=torch.float32, device=dev)
         rc = _cu.lib().cm_packed_attention_bwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr(), go.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
-            lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), plan.at, ctx.scale,
+            lse.data_ptr(), delta.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), plan.at, ctx.scale,
             _cu.err_word(dev).data_ptr(), _cu.stream_ptr())
         if rc:
             _failed("cm_packed_attention_bwd", rc)
-        F_.count_launch("packed_attention_bwd", 3 if ctx.dtype == torch.bfloat16 else 4)
-        return dq, dk, dv, None, None, None, None
+        F_.count_launch("packed_attention_bwd", (1 if ctx.dtype == torch.bfloat16 else 2) + need_q + (need_k or need_v))
+        return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
 
 
 def _nothing(plan, q, k, v, cu_q, cu_k):

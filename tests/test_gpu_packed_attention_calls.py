@@ -76,3 +76,19 @@ def test_calls_of_nothing_can_be_differentiated_again():
     o = F_.packed_attention(*leaves, _i32([0, 5]), 0.1, _i32([0, 0]))
     (g,) = torch.autograd.grad(o.sum() + leaves[0].square().sum(), leaves[0], create_graph=True)
     assert torch.equal(torch.autograd.grad(g.sum(), leaves[0])[0], torch.full_like(leaves[0], 2))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("wanted,kernels", [([0], 1), ([1], 1), ([2], 1), ([1, 2], 1), ([0, 1], 2), ([0, 2], 2), ([0, 1, 2], 2)])
+def test_gradients_that_nobody_asks_for_are_not_computed(wanted, kernels, dtype):
+    """One large kernel for dq, one for dk and dv; the gradients that are asked for have the same bits."""
+    cu = _i32([0, 60, 190])
+    leaves = [_randn(190, n, 64, dtype=dtype, seed=s) for s, n in ((0, 4), (1, 2), (2, 2))]
+    go = _randn(190, 4, 64, dtype=dtype, seed=3)
+    every = [t.clone().requires_grad_() for t in leaves]
+    want = torch.autograd.grad(F_.packed_attention(*every, cu, 0.125), every, go)
+    some = [t.clone().requires_grad_(i in wanted) for i, t in enumerate(leaves)]
+    F_.reset_counters()
+    got = torch.autograd.grad(F_.packed_attention(*some, cu, 0.125), [some[i] for i in wanted], go)
+    assert all(torch.equal(a, want[i]) for a, i in zip(got, wanted))
+    assert F_.launch_counts()["packed_attention_bwd"] == kernels + (1 if dtype == torch.bfloat16 else 2)

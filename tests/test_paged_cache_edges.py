@@ -255,3 +255,17 @@ def test_packed_attention_of_nothing_looks_at_its_ends_on_the_device(kernels, mo
     o = F_.packed_attention(*leaves, cu, -0.5, cu_k)
     assert len(seen) == 1 and seen[0][2:5] == (2, T, Tk) and o.shape == (T, H, 16) and not o.any()
     assert all(g.shape == t.shape and not g.any() for g, t in zip(torch.autograd.grad(o.sum(), leaves), leaves))
+
+
+@pytest.mark.parametrize("wanted", [[0], [1], [2], [0, 2], [0, 1, 2]])
+def test_packed_gradients_that_nobody_asks_for_have_no_memory(kernels, wanted):
+    seen = []
+    kernels.cm_packed_attention_ws = lambda at: 0
+    kernels.cm_packed_attention_fwd = lambda *args: 0
+    kernels.cm_packed_attention_bwd = lambda *args: seen.append(args[10:13]) or 0
+    leaves = [_randn(9, h, 16, seed=s).requires_grad_(s in wanted) for s, h in ((0, 4), (1, 2), (2, 2))]
+    o = F_.packed_attention(*leaves, _i32(0, 5, 9), 0.25)
+    grads = torch.autograd.grad(o, [leaves[i] for i in wanted], torch.ones_like(o))
+    (dq, dk, dv), = seen
+    assert (dq is not None) == (0 in wanted) and (dk is not None) == (dv is not None) == bool({1, 2} & set(wanted))
+    assert [g.shape for g in grads] == [leaves[i].shape for i in wanted]
