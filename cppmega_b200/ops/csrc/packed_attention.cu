@@ -63,6 +63,7 @@ constexpr int TILE = 128;
 constexpr int PART = 64;                     // columns of scores that are multiplied and waited for as one
 constexpr int SLAB = 128 * 128;              // bytes of one [128 rows x 64 columns] slab, 128-byte swizzle
 constexpr float RESCALE_AT = 8.f;            // log2
+constexpr float FP16_UP = 7.f;               // log2: fp16 weights lie this far above their reference's, for more of the range below them (2^15 at most)
 
 // ---- products --------------------------------------------------------------------------------------------------------
 __host__ __device__ constexpr uint32_t idesc(bool half, int n, bool b_mn) {        // M 128, A K-major
@@ -559,9 +560,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
       const float m_new = largest != -INFINITY ? largest * a.scale_log2 : -INFINITY;            // a scale of zero leaves "nothing seen" as it is
       float alpha = 1.f;
-      if (m_new > m_ref + RESCALE_AT) {                       // also from -inf
-        alpha = ex2(m_ref - m_new);
-        m_ref = m_new;
+      constexpr float UP = HALF ? FP16_UP : 0.f;
+      if (m_new > m_ref + (RESCALE_AT + UP)) {                // also from -inf
+        alpha = ex2(m_ref - (m_new - UP));
+        m_ref = m_new - UP;
         l *= alpha;
         gained *= alpha;
       }

@@ -26,7 +26,9 @@
 // (1000 keys, one in fifty three times as large: off by 1.7e-3 of its norm, 2.3e-3 with the sum of the others).  Over an E4M3 cache the weights that are rounded have the
 // values' powers in them, and the sum is that of the unrounded ones.  Scores, maxima, sums and accumulators are fp32.
 //
-// The reference value of a head's softmax follows its maximum only when that has grown by 2^8, so that accumulators are rarely rescaled.
+// The reference value of a head's softmax follows its maximum only when that has grown by 2^8, so that accumulators are rarely rescaled.  In fp16 it
+// stays 2^7 below the maximum: with weights of 1 at the most, those of keys that one key stands far above fall among the subnormals (14 above,
+// its values zero: half a step is up to 4 % of such a weight).
 //
 // Measured, both kernels: bf16, one sequence of 131071 tokens, 64 heads over 8, 128 wide 93 us (82 at the copy rate; 64 sequences of 8192 tokens, 32
 // heads over 8: 6.7 TB/s).  E4M3, 64 sequences of 100 to 16000 tokens, 32 heads over 8: 100 us (63 at the copy rate; 5.0 TB/s at 16384 each): half
@@ -45,6 +47,7 @@ constexpr int KEYS = 16;                     // keys of one step
 constexpr int RING_BYTES = 192 * 1024;       // the rings of a block's warps
 constexpr int SHORTEST_RUN = 2;              // steps: fewer would be all set-up, and more pieces to join
 constexpr float RESCALE_AT = 8.f;            // log2
+constexpr float FP16_UP = 7.f;               // log2: fp16 weights lie this far above their reference's, for more of the range below them (2^15 at most)
 
 struct Args {
   const uint8_t* q;                          // [sequences, heads, dim]
@@ -205,6 +208,7 @@ template <bool BF16, bool E4M3, int D, int DV, int NT>
 __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_attention_kernel(const Args a) {
   using F = Form<BF16, E4M3, D, DV, NT>;
   constexpr bool MB = F::MMA_BF16;
+  constexpr float UP = MB ? 0.f : FP16_UP;
   constexpr int VT = DV / 16;                                 // 16-column tiles of the result
   extern __shared__ __align__(128) uint8_t smem_raw[];
   few::wait_for_input();                     // by every block, and before the next kernel may start: it counts on all older kernels having ended
@@ -579,10 +583,10 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         top[x][c] = fmaxf(s[x][c], s[x][2 + c]);
-        grown |= top[x][c] > m[x][c] + RESCALE_AT;
+        grown |= top[x][c] > m[x][c] + (RESCALE_AT + UP);
         if (E4M3) {
           topv[x][c] = fmaxf(s[x][c] + vlog[0], s[x][2 + c] + vlog[1]);
-          grown |= topv[x][c] > mv[x][c] + RESCALE_AT;
+          grown |= topv[x][c] > mv[x][c] + (RESCALE_AT + UP);
         }
       }
     const uint32_t vb = base + KEYS * F::K_ROW +
@@ -619,7 +623,7 @@ __global__ void __launch_bounds__(warps_of(E4M3, D, DV, NT) * 32, 1) paged_atten
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           auto raise = [&](float& ref, float t) {             // the factor that takes sums to the new reference
-            t = max8(t);
+            t = max8(t) - UP;
             if (!(t > ref)) return 1.f;
             const float by = ex2(ref - t);
             ref = t;

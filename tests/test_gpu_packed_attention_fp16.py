@@ -136,3 +136,21 @@ def test_no_sequences_and_empty_ones():
         assert all((g == 0).all() for g in grads)
     from cppmega_b200.ops import cuda as cu_
     cu_.check_errors()
+
+
+def test_keys_far_below_one_without_values():
+    """Weights that one key (its values zero) pushes 10 to 17 below it, the same for all the others, so that their roundings add up: 2^-11 of each, and
+    2^-25 under the 2^7 that the largest counts at the least."""
+    n, D = 300, 64
+    q, k = torch.zeros(n, 1, D, device="cuda").half(), torch.zeros(n, 1, D, device="cuda").half()
+    q[:, 0, 0] = torch.linspace(10, 17, n, device="cuda")
+    k[0, 0, 0] = 1
+    v = torch.full((n, 1, D), 8.0, device="cuda").half()
+    v[0] = 0
+    o = F_.packed_attention(q, k, v, _i32([0, n]), 1.0)[:, 0].double()
+    s = (q[:, 0].double() @ k[:, 0].double().T).masked_fill(torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+    p = torch.softmax(s, 1)
+    e = 2 * ((D + 8) * 2.0 ** -23) * s.masked_fill(s == -math.inf, 0).abs().amax(1, keepdim=True) + 2.0 ** -19 + n * 2.0 ** -23
+    want = p @ v[:, 0].double()
+    bound = (p * (U + e) + 2.0 ** -32 * (p > 0)) @ v[:, 0].double() + want * (U + e + U) + 2.0 ** -25
+    _check(o, want, bound * (1 + U), "o")

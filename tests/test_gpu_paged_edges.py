@@ -173,3 +173,29 @@ def test_attention_over_a_cache_of_no_pages(page, store):
     cu.check_errors()
     assert (F_.paged_attention(_randn(2, 4, 64), kc, vc, table, _i32([0, 200]), 0.1, ks, vs) == 0).all()
     _reported()
+
+
+@pytest.mark.parametrize("store", [torch.float16, E4M3])
+@pytest.mark.parametrize("group", [1, 12])
+def test_keys_far_below_one_with_few_values(store, group):
+    """Weights that one key pushes 10 to 17 below it, the same for all the others, so that their roundings add up: 2^-11 of each, and 2^-25 under the 2^7 that
+    the largest (over E4M3 times its values' power, which is 2^-20 for that key) counts at the least."""
+    n, D, page, dtype = 300, 64, 16, torch.float16
+    kc, vc, ks, vs = _caches(20, page, 1, (D, D), store)
+    q, k = torch.zeros(64, group, D, device="cuda").half(), torch.zeros(n, 1, D, device="cuda").half()
+    q[:, :, 0] = torch.linspace(10, 17, 64 * group, device="cuda").view(64, group)
+    k[40, 0, 0] = 1
+    v = torch.full((n, 1, D), 7.0, device="cuda").half()
+    v[40] = 7 * 2.0 ** -20 if store == E4M3 else 0
+    F_.cache_write(k, v, kc, vc, torch.arange(n, device="cuda"), ks, vs)
+    table = torch.arange(20, device="cuda").int()[None].expand(64, -1)
+    got = F_.paged_attention(q, kc, vc, table, _i32([n] * 64), 1.0, ks, vs).double()
+    s = q.double() @ k[:, 0].double().T
+    p = torch.softmax(s, -1)
+    e = 2 * ((D + 4) * 2.0 ** -23 + 2.0 ** -22) * 17 + 2.0 ** -20 + 4 * n * 2.0 ** -24
+    rows = v[:, 0].double()
+    want = p @ rows
+    lost = 2.0 ** -32 * (rows if store != E4M3 else (p[..., None] * rows).amax(-2, keepdim=True).expand(-1, -1, n, -1)).sum(-2)
+    u = 2.0 ** -11
+    bound = (p * (u + e)) @ rows + lost + want * (u + e + u) + 2.0 ** -25
+    assert ((got - want).abs() <= bound * (1 + u)).all(), float(((got - want).abs() / bound).max())
