@@ -199,3 +199,25 @@ def test_keys_far_below_one_with_few_values(store, group):
     u = 2.0 ** -11
     bound = (p * (u + e)) @ rows + lost + want * (u + e + u) + 2.0 ** -25
     assert ((got - want).abs() <= bound * (1 + u)).all(), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("store", [torch.bfloat16, E4M3])
+def test_equal_slots_among_slots_of_one_hash_place(store):
+    """Blocks of 128 tokens whose slots fall to three places of the hash table, 20 different ones to each and some often: chains of 40 and more, in which
+    equal slots and others follow one another.  Of equal slots the last row stays."""
+    slots = torch.arange(1 << 17, dtype=torch.int64)
+    place = (slots * 2654435769 % (1 << 32)) >> 21             # as the kernel has it
+    some = torch.cat([slots[place == p][:20] for p in (0, 777, 2047)])
+    assert len(some) == 60
+    T = 80000
+    g = torch.Generator().manual_seed(1)
+    drawn = some[torch.randint(0, 60, (T,), generator=g)]
+    drawn[::7] = -1
+    drawn[::13] = torch.randint(0, 1 << 17, (len(drawn[::13]),), generator=g)
+    drawn = drawn.cuda()
+    k = _randn(T, 1, 16)
+    (kc, _, ks, _), (wk, _, wks, _) = _caches(1 << 13, 16, 1, (16, 8), store), _caches(1 << 13, 16, 1, (16, 8), store)
+    F_.cache_write(k, None, kc, None, drawn, ks)
+    ref.cache_write(k, None, wk, None, drawn, wks)
+    assert torch.equal(kc.view(torch.uint8 if store == E4M3 else torch.int16), wk.view(torch.uint8 if store == E4M3 else torch.int16))
+    assert ks is None or torch.equal(ks, wks)
