@@ -730,8 +730,7 @@ __global__ void __launch_bounds__(TILE) packed_join_kernel(const Args a) {
 }
 
 // ---- backward: delta -----------------------------------------------------------------------------------------------------
-// delta[i] = do[i] . o[i] before its rounding, in fp16 also |do| of the row and the largest of its sequence and key head.  DV / 8 lanes a row, four rows of a
-// lane on their way at once: three reads of a row's width at the memory's rate.  Inside the dq kernel, whose blocks have an SM to themselves, nothing would
+// delta[i] = do[i] . o[i] before its rounding, in fp16 also |do| of the row.  DV / 8 lanes a row, four rows of a lane on their way at once: three reads of a row's width at the memory's rate.  Inside the dq kernel, whose blocks have an SM to themselves, nothing would
 // run meanwhile (9000 cycles a block, 120 us at 16384 x 32 rows of 128; here 71).
 constexpr int DELTA_THREADS = 256, DELTA_AHEAD = 4;
 
@@ -744,11 +743,6 @@ __device__ __forceinline__ int sequence_of(const int* cu, int n, int tok) {
     else hi = mid;
   }
   return lo;
-}
-// The largest is the same in any order.  Most rows are not above what they find there.
-__device__ __forceinline__ void raise_to(uint32_t* at, float x) {
-  const uint32_t bits = __float_as_uint(x);
-  if (isfinite(x) && bits > *reinterpret_cast<const volatile uint32_t*>(at)) atomicMax(at, bits);
 }
 // 2^14 p is rounded to fp16, and p (do v' - delta) with it
 constexpr float P_UP = 14.f, P_DOWN = 1.f / 16384;
@@ -799,44 +793,58 @@ __global__ void __launch_bounds__(DELTA_THREADS, 4) packed_delta_kernel(const Ar
     const long long row = row0 + i * ROWS;
     if (piece == 0 && row < rows) {
       a.delta[row] = dot;
-      if (HALF) {
-        big = sqrtf(big);
-        a.big[row] = big;
-        const unsigned more = (head0 + i * ROWS) / unsigned(a.heads), head = head0 + i * ROWS - more * a.heads;
-        raise_to(a.top + (long long)sequence_of(a.cu_q, a.n, int(tok0 + more)) * a.kv_heads + head / unsigned(a.heads / a.kv_heads), big);
-      }
+      if (HALF) a.big[row] = sqrtf(big);
     }
   }
 }
 
-// fp16: the largest |v| of each sequence and key head.  Rows as above.
+// fp16: the largest |v| and |do| of each sequence and key head.  A warp takes 32 tokens of a key head, most often of one sequence, and reports once for
+// each sequence among them (row by row, the few words that all rows ask for took 50 us at 8192 x 32 rows).
 template <int LANES>
 __global__ void __launch_bounds__(DELTA_THREADS) packed_sizes_kernel(const Args a) {
-  constexpr int ROWS = DELTA_THREADS / LANES;
-  const int piece = threadIdx.x % LANES;
-  const long long rows = (long long)min(max(__ldg(a.cu_k + a.n), 0), a.Tk) * a.kv_heads;
-  const long long row0 = (long long)blockIdx.x * (ROWS * DELTA_AHEAD) + threadIdx.x / LANES;
-  uint4 x[DELTA_AHEAD];
+  constexpr int AT_ONCE = 32 / LANES;
+  const int lane = threadIdx.x & 31, piece = lane % LANES, group = a.heads / a.kv_heads;
+  const long long warp = (long long)blockIdx.x * (DELTA_THREADS / 32) + (threadIdx.x >> 5), of_v = (long long)((a.Tk + 31) / 32) * a.kv_heads;
+  const bool v = warp < of_v;                // the others look at |do|
+  const long long mine = v ? warp : warp - of_v;
+  const int first = int(mine / a.kv_heads) * 32, kvh = int(mine % a.kv_heads), tok = first + lane;
+  const int* cu = v ? a.cu_k : a.cu_q;
+  const int rows = min(max(__ldg(cu + a.n), 0), v ? a.Tk : a.T);
+  if (first >= rows) return;
+  float big = 0.f;
+  if (v) {
 #pragma unroll
-  for (int i = 0; i < DELTA_AHEAD; ++i) {
-    const long long row = row0 + i * ROWS, tok = row / a.kv_heads, head = row - tok * a.kv_heads;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (row < rows && piece * 8 < a.vdim)
-      x[i] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.v) + tok * a.v_tok + head * a.v_head) + piece);
-  }
+    for (int i = 0; i < LANES; ++i) {
+      const int t = first + i * AT_ONCE + lane / LANES;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (t < rows && piece * 8 < a.vdim)
+        x = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.v) + t * a.v_tok + kvh * a.v_head) + piece);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+      float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < DELTA_AHEAD; ++i) {
-    const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-    float big = 0.f;
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpair<true>(xs[e]);
+        sum = fmaf(f.x, f.x, fmaf(f.y, f.y, sum));
+      }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = unpair<true>(xs[e]);
-      big = fmaf(f.x, f.x, fmaf(f.y, f.y, big));
+      for (int o = LANES >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float own = __shfl_sync(0xffffffffu, sum, (lane % AT_ONCE) * LANES);
+      if (lane / AT_ONCE == i) big = sqrtf(own);
     }
-#pragma unroll
-    for (int o = LANES >> 1; o > 0; o >>= 1) big += __shfl_xor_sync(0xffffffffu, big, o);
-    const long long row = row0 + i * ROWS, tok = row / a.kv_heads;
-    if (piece == 0 && row < rows) raise_to(a.vtop + (long long)sequence_of(a.cu_k, a.n, int(tok)) * a.kv_heads + (row - tok * a.kv_heads), sqrtf(big));
+  } else if (tok < rows) {
+    for (int h = 0; h < group; ++h) {
+      const float x = a.big[(long long)tok * a.heads + kvh * group + h];
+      if (isfinite(x)) big = fmaxf(big, x);
+    }
+  }
+  const int seq = tok < rows ? sequence_of(cu, a.n, tok) : -1;
+  const uint32_t bits = isfinite(big) ? __float_as_uint(big) : 0u;
+  for (unsigned todo = __ballot_sync(0xffffffffu, seq >= 0); todo;) {
+    const int s = __shfl_sync(0xffffffffu, seq, __ffs(todo) - 1);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, seq == s ? bits : 0u);
+    uint32_t* at = (v ? a.vtop : a.top) + (long long)s * a.kv_heads + kvh;
+    if (lane == 0 && most > *reinterpret_cast<volatile uint32_t*>(at)) atomicMax(at, most);            // the same in any order
+    todo &= ~__ballot_sync(0xffffffffu, seq == s);
   }
 }
 
@@ -1529,15 +1537,16 @@ int backward(const Inputs& in, Args a, void* dq, void* dk, void* dv, cudaStream_
   if (uq * a.kv_heads * a.chunks > 0x7fffffffLL || uk * a.kv_heads > 0x7fffffffLL) return -10;
   {
     constexpr int LANES = DV / 8, ROWS = DELTA_THREADS / LANES * DELTA_AHEAD;
-    const long long blocks = ((long long)a.T * a.heads + ROWS - 1) / ROWS, v_blocks = ((long long)a.Tk * a.kv_heads + ROWS - 1) / ROWS;
-    if (blocks > 0x7fffffffLL || v_blocks > 0x7fffffffLL) return -10;
-    if (HALF) {
-      if (cudaMemsetAsync(a.top, 0, 2 * sizeof(uint32_t) * a.n * a.kv_heads, stream) != cudaSuccess) return -3;
-      packed_sizes_kernel<LANES><<<(unsigned)v_blocks, DELTA_THREADS, 0, stream>>>(a);
-      if (cudaGetLastError() != cudaSuccess) return -3;
-    }
+    const long long blocks = ((long long)a.T * a.heads + ROWS - 1) / ROWS;
+    const long long warps = ((long long)(a.T + 31) / 32 + (a.Tk + 31) / 32) * a.kv_heads, sizes = (warps + DELTA_THREADS / 32 - 1) / (DELTA_THREADS / 32);
+    if (blocks > 0x7fffffffLL || sizes > 0x7fffffffLL) return -10;
     packed_delta_kernel<HALF, LANES><<<(unsigned)blocks, DELTA_THREADS, 0, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return -3;
+    if (HALF) {
+      if (cudaMemsetAsync(a.top, 0, 2 * sizeof(uint32_t) * a.n * a.kv_heads, stream) != cudaSuccess) return -3;
+      packed_sizes_kernel<LANES><<<(unsigned)sizes, DELTA_THREADS, 0, stream>>>(a);
+      if (cudaGetLastError() != cudaSuccess) return -3;
+    }
   }
   if (dq) {
     a.units = (int)uq;
