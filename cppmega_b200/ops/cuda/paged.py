@@ -105,11 +105,6 @@ def _plan_write(k, v, k_cache, v_cache, slots, k_scale, v_scale):
                 copy=not (rows_on(k, 16) and rows_on(v, 16) and slots.is_contiguous()), spans=[F_.bytes_spanned(t) for t in (k, v, k_cache, v_cache, k_scale, v_scale)])
 
 
-def _meet(a, a_bytes, b, b_bytes) -> bool:
-    """Whether two ranges of memory have bytes in common."""
-    return a < b + b_bytes and b < a + a_bytes
-
-
 @_on_device
 def cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout) -> bool:
     """False where the kernel does not apply."""
@@ -120,12 +115,13 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout) -> bool
     if (kcp | (vcp or 0)) & (7 if k_scale is not None else 15):
         return False
     k_bytes, v_bytes, kc_bytes, vc_bytes, ks_bytes, vs_bytes = plan.spans
-    if vcp and _meet(kcp, kc_bytes, vcp, vc_bytes):
-        F_.check_apart(layout, k_cache, v_cache)
-    if vsp and _meet(ksp, ks_bytes, vsp, vs_bytes):
-        F_.check_apart(layout, k_scale, v_scale)
-    inside = _meet(kp, k_bytes, kcp, kc_bytes) or vp and (
-        _meet(kp, k_bytes, vcp, vc_bytes) or _meet(vp, v_bytes, kcp, kc_bytes) or _meet(vp, v_bytes, vcp, vc_bytes))
+    inside = -k_bytes < kp - kcp < kc_bytes               # ranges of memory that have bytes in common
+    if vp:
+        inside = inside or -k_bytes < kp - vcp < vc_bytes or -v_bytes < vp - kcp < kc_bytes or -v_bytes < vp - vcp < vc_bytes
+        if -kc_bytes < kcp - vcp < vc_bytes:
+            F_.check_apart(layout, k_cache, v_cache)
+        if vsp and -ks_bytes < ksp - vsp < vs_bytes:
+            F_.check_apart(layout, k_scale, v_scale)
     if plan.copy or inside or (kp | (vp or 0)) & 15:      # a few rows; or rows of the cache itself, read before any is overwritten
         k, v = (None if t is None else t.detach().clone(memory_format=torch.contiguous_format) for t in (k, v))
         slots = slots.contiguous()
