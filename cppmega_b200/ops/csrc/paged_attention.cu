@@ -31,7 +31,7 @@
 // its values zero: half a step is up to 4 % of such a weight).
 //
 // Measured, both kernels: bf16, one sequence of 131071 tokens, 64 heads over 8, 128 wide 93 us (82 at the copy rate; 64 sequences of 8192 tokens, 32
-// heads over 8: 6.7 TB/s).  E4M3, 64 sequences of 100 to 16000 tokens, 32 heads over 8: 100 us (63 at the copy rate; 5.0 TB/s at 16384 each): half
+// heads over 8: 6.7 TB/s).  E4M3, 64 sequences of 100 to 16000 tokens, 32 heads over 8: 104 us (63 at the copy rate; 4.9 TB/s at 16384 each): half
 // the bytes of a key, the same chain of steps, and the conversions.  Short calls are set-up (the lengths, the table, the first rows: 5 us) and the
 // second kernel: 1000 tokens 9.1 us in a graph.
 #include <cuda_fp16.h>
