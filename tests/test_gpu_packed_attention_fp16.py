@@ -154,3 +154,29 @@ def test_keys_far_below_one_without_values():
     want = p @ v[:, 0].double()
     bound = (p * (U + e) + 2.0 ** -32 * (p > 0)) @ v[:, 0].double() + want * (U + e + U) + 2.0 ** -25
     _check(o, want, bound * (1 + U), "o")
+
+
+def test_captured_for_other_lengths_and_sizes():
+    """Forward and backward in a graph: the ends and the upstream gradients change in place, and with them the scales of each sequence."""
+    cu = _i32([0, 100, 200, 256])
+    q, k, v = (_randn(256, n, 64, seed=s).requires_grad_() for s, n in ((0, 4), (1, 2), (2, 2)))
+    go = _randn(256, 4, 64, seed=3)
+
+    def once():
+        o = F_.packed_attention(q, k, v, cu, 0.125)
+        return [o.detach(), *torch.autograd.grad(o, [q, k, v], go)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = once()
+    for ends, std in (([0, 100, 200, 256], 1.0), ([0, 1, 1, 250], 1e3), ([0, 256, 256, 256], 1e-3), ([0, 0, 0, 0], 1.0), ([0, 130, 131, 200], 1e-2)):
+        cu.copy_(_i32(ends))
+        go.copy_(_randn(256, 4, 64, std=std, seed=ends[1]))
+        g.replay()
+        got = [t.clone() for t in outs]
+        assert all(torch.equal(a, b) for a, b in zip(got, once()))
