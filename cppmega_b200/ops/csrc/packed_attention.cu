@@ -730,8 +730,9 @@ __global__ void __launch_bounds__(TILE) packed_join_kernel(const Args a) {
 }
 
 // ---- backward: delta -----------------------------------------------------------------------------------------------------
-// delta[i] = do[i] . o[i] before its rounding, in fp16 also |do| of the row.  DV / 8 lanes a row, four rows of a lane on their way at once: three reads of a row's width at the memory's rate.  Inside the dq kernel, whose blocks have an SM to themselves, nothing would
-// run meanwhile (9000 cycles a block, 120 us at 16384 x 32 rows of 128; here 71).
+// delta[i] = do[i] . o[i] before its rounding, in fp16 also |do| of the row.  DV / 8 lanes a row, four rows of a lane on their way at once: three reads
+// of a row's width at the memory's rate.  Inside the dq kernel, whose blocks have an SM to themselves, nothing would run meanwhile (9000 cycles a
+// block, 120 us at 16384 x 32 rows of 128; here 71).
 constexpr int DELTA_THREADS = 256, DELTA_AHEAD = 4;
 
 // the last sequence that begins at or before row `tok`, of n > 0

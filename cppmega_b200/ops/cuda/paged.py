@@ -38,12 +38,13 @@ def declare(L: ctypes.CDLL) -> None:
 class Plan:
     """What a layout's calls have in common: the library's array of sizes and strides, and what else the wrapper needs."""
 
-    __slots__ = ("numbers", "at", "copy", "shape", "work", "like", "spans")
+    __slots__ = ("numbers", "at", "copy", "shape", "work", "like", "spans", "apart")
 
     def __init__(self, numbers, copy=False, shape=None, work=0, like=False, spans=None):
         self.numbers = (ctypes.c_longlong * len(numbers))(*numbers)
         self.at = ctypes.addressof(self.numbers)
         self.copy, self.shape, self.work, self.like, self.spans = copy, shape, work, like, spans
+        self.apart = set()         # distances at which tensors of this layout have been found not to share memory
 
 
 _plans: dict = {}
@@ -102,7 +103,8 @@ def _plan_write(k, v, k_cache, v_cache, slots, k_scale, v_scale):
         return False
     return Plan([*strides(k), *strides(v, 2), *strides(k_cache), *strides(v_cache, 3), T, heads, dim, 0 if v is None else v.shape[2],
                  k_cache.shape[0], k_cache.shape[1], TYPES[k.dtype], int(q), int(slots.dtype == torch.int64)],
-                copy=not (rows_on(k, 16) and rows_on(v, 16) and slots.is_contiguous()), spans=[F_.bytes_spanned(t) for t in (k, v, k_cache, v_cache, k_scale, v_scale)])
+                copy=not (rows_on(k, 16) and rows_on(v, 16) and slots.is_contiguous()),
+                spans=[F_.bytes_spanned(t) for t in (k, v, k_cache, v_cache, k_scale, v_scale)])
 
 
 @_on_device
@@ -118,10 +120,12 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout) -> bool
     inside = -k_bytes < kp - kcp < kc_bytes               # ranges of memory that have bytes in common
     if vp:
         inside = inside or -k_bytes < kp - vcp < vc_bytes or -v_bytes < vp - kcp < kc_bytes or -v_bytes < vp - vcp < vc_bytes
-        if -kc_bytes < kcp - vcp < vc_bytes:
-            F_.check_apart(layout, k_cache, v_cache)
-        if vsp and -ks_bytes < ksp - vsp < vs_bytes:
-            F_.check_apart(layout, k_scale, v_scale)
+        if -kc_bytes < kcp - vcp < vc_bytes and kcp - vcp not in plan.apart:      # keys and values in one buffer
+            F_.check_apart(k_cache, v_cache)
+            plan.apart.add(kcp - vcp)
+        if vsp and -ks_bytes < ksp - vsp < vs_bytes and (ksp - vsp,) not in plan.apart:
+            F_.check_apart(k_scale, v_scale)
+            plan.apart.add((ksp - vsp,))
     if plan.copy or inside or (kp | (vp or 0)) & 15:      # a few rows; or rows of the cache itself, read before any is overwritten
         k, v = (None if t is None else t.detach().clone(memory_format=torch.contiguous_format) for t in (k, v))
         slots = slots.contiguous()

@@ -606,15 +606,10 @@ def _check_write(k, v, k_cache, v_cache, slots, k_scale, v_scale) -> None:
     _same_device("cache_write", k, v, k_cache, slots)
 
 
-def check_apart(layout, a, b) -> None:
+def check_apart(a, b) -> None:
     """The keys' memory is not the values'.  That goes by addresses too, so every call looks; the kernels' wrapper asks only where the ranges meet."""
-    if b is None or not (torch._C._has_storage(a) and torch._C._has_storage(b)):
-        return
-    place = ("apart", b.data_ptr() - a.data_ptr(), b.shape, layout)
-    if place not in _CHECKED:
-        if _share_memory(a, b):
-            raise ValueError(f"cache_write: keys {tuple(a.shape)} and values {tuple(b.shape)} share memory")
-        _checked(place)
+    if b is not None and torch._C._has_storage(a) and torch._C._has_storage(b) and _share_memory(a, b):
+        raise ValueError(f"cache_write: keys {tuple(a.shape)} and values {tuple(b.shape)} share memory")
 
 
 def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> None:
@@ -638,8 +633,8 @@ def cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> No
         if fn(k, v, k_cache, v_cache, slots, k_scale, v_scale, layout):
             return
         _miss("cache_write(shape/dtype)", k)
-    check_apart(layout, k_cache, v_cache)
-    check_apart(layout, k_scale, v_scale)
+    check_apart(k_cache, v_cache)
+    check_apart(k_scale, v_scale)
     with torch.no_grad():
         ref.cache_write(k, v, k_cache, v_cache, slots, k_scale, v_scale)
 

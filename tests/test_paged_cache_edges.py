@@ -269,3 +269,28 @@ def test_packed_gradients_that_nobody_asks_for_have_no_memory(kernels, wanted):
     (dq, dk, dv), = seen
     assert (dq is not None) == (0 in wanted) and (dk is not None) == (dv is not None) == bool({1, 2} & set(wanted))
     assert [g.shape for g in grads] == [leaves[i].shape for i in wanted]
+
+
+def test_interleaved_caches_are_looked_at_once_for_a_distance(kernels, monkeypatch):
+    """Keys and values in one buffer: their memory is compared once for each way that two tensors of these shapes lie, and again where they lie another
+    way, with the kernels as with the definition."""
+    compared = []
+    share = F_._share_memory
+    monkeypatch.setattr(F_, "_share_memory", lambda a, b: compared.append(1) or share(a, b))
+    kernels.cm_cache_write = lambda *args: 0
+    both, k = torch.zeros(4, 8, 3, 2, 16, dtype=torch.bfloat16), _randn(3, 2, 16)
+    slots = torch.tensor([0, 9, 31])
+    for _ in range(3):
+        F_.cache_write(k, k, both[:, :, 0], both[:, :, 1], slots)
+    assert len(compared) == 1
+    for _ in range(3):
+        F_.cache_write(k, k, both[:, :, 0], both[:, :, 2], slots)
+    assert len(compared) == 2
+    for _ in range(2):
+        with pytest.raises(ValueError, match="share memory"):
+            F_.cache_write(k, k, both[:, :, 0], both[:, :, 0], slots)
+    e4m3 = both.view(torch.uint8).view(torch.float8_e4m3fn)[..., :16]
+    one = torch.zeros(4, 8, 2, dtype=torch.uint8)
+    for _ in range(2):
+        with pytest.raises(ValueError, match="share memory"):
+            F_.cache_write(k, k, e4m3[:, :, 0], e4m3[:, :, 1], slots, one, one)
